@@ -23,8 +23,11 @@ from .dense_loss import (DenseLightningIndexerGradKLLoss, DenseLightningIndexerS
                          dense_lightning_indexer_grad_kl_loss, dense_lightning_indexer_softmax_lse,
                          dense_loss_backward, npu_dense_lightning_indexer_grad_kl_loss,
                          npu_dense_lightning_indexer_softmax_lse)
+from .rotary import (IndexAppendPlan, LatentAppendPlan, RotaryEmbedding, index_cache_append, latent_cache_append,
+                     rotary_embedding, rotary_embedding_grad)
 
-__all__ = ["lightning_indexer", "LightningIndexer", "sparse_flash_attention", "SparseFlashAttention",
+__all__ = ["rotary_embedding", "rotary_embedding_grad", "RotaryEmbedding", "latent_cache_append", "LatentAppendPlan",
+           "index_cache_append", "IndexAppendPlan", "lightning_indexer", "LightningIndexer", "sparse_flash_attention", "SparseFlashAttention",
            "sparse_flash_attention_grad", "SparseFlashAttentionGrad", "sparse_lightning_indexer_grad_kl_loss",
            "SparseLightningIndexerGradKLLoss", "dense_lightning_indexer_softmax_lse",
            "npu_dense_lightning_indexer_softmax_lse", "dense_loss_backward",

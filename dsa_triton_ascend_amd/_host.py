@@ -1,4 +1,4 @@
-"""Host-side helpers shared by the two operators: length normalisation,
+"""Host-side helpers shared by the operators: length normalisation,
 dtype codes, stream handles and the small int32 index arrays the C ABI takes."""
 from __future__ import annotations
 
@@ -119,6 +119,24 @@ def upload(lib, device: torch.device, *arrays: list[int], zero: torch.Tensor | N
 def stream_ptr(device: torch.device) -> int:
     # the raw handle, without the Stream object that torch.cuda.current_stream builds (2.5 us a call)
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
+
+
+class on_device:
+    """Makes a tensors' device current for the launches inside (a stream's kernels need its device to
+    be the current one); nothing to do where it already is."""
+
+    def __init__(self, device: torch.device):
+        self.guard = None
+        if device.index not in (None, torch.cuda.current_device()):
+            self.guard = torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

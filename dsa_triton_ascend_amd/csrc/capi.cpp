@@ -509,4 +509,119 @@ int dsa_dense_li_grad_kl_loss(const void* query, const void* key, const void* qu
                     "dsa_dense_li_grad_kl_loss launch");
 }
 
+namespace {
+// Positions, sections and rotary dimensions, shared by the rotation and the appends
+int check_rotation(const char* fn, int axes, const int32_t* sections, const float* inv_freq, int rotary_start,
+                   int rotary_dim, int width) {
+  if (!inv_freq) return fail(DSA_ERR_INVALID, "%s: null pointer argument", fn);
+  if (rotary_dim < 2 || rotary_dim % 2 != 0 || rotary_dim > 1024 || rotary_start < 0 || rotary_start + rotary_dim > width)
+    return fail(DSA_ERR_INVALID, "%s: rotary dimensions [%d, %d + %d) of a width of %d (an even count, at most 1024)", fn,
+                rotary_start, rotary_start, rotary_dim, width);
+  if (axes < 1 || axes > 4) return fail(DSA_ERR_INVALID, "%s: 1 to 4 position axes, got %d", fn, axes);
+  if (axes > 1 && !sections) return fail(DSA_ERR_INVALID, "%s: several axes need sections", fn);
+  if (sections) {
+    int64_t sum = 0;
+    for (int a = 0; a < axes; ++a) {
+      if (sections[a] < 0) return fail(DSA_ERR_INVALID, "%s: negative section", fn);
+      sum += sections[a];
+    }
+    if (sum != rotary_dim / 2)
+      return fail(DSA_ERR_INVALID, "%s: sections add up to %lld, not to the %d pairs", fn, (long long)sum, rotary_dim / 2);
+  }
+  return DSA_OK;
+}
+
+int check_append(const char* fn, const void* x, int io_dtype, const void* norm_weight, int w_dtype,
+                 const int32_t* row_start, const int32_t* act_q, const int32_t* act_k, const int32_t* block_table,
+                 int batch, int total_rows, int rows_per_batch, int max_blocks, int page_block_size, int64_t num_blocks,
+                 const void* cache) {
+  if (!x || !row_start || !act_q || !act_k || !block_table || !cache)
+    return fail(DSA_ERR_INVALID, "%s: null pointer argument", fn);
+  if (!is16(io_dtype)) return fail(DSA_ERR_INVALID, "%s: io_dtype must be fp16 or bf16", fn);
+  if (norm_weight && !is16(w_dtype) && w_dtype != DSA_DTYPE_F32)
+    return fail(DSA_ERR_INVALID, "%s: norm weights must be fp16, bf16 or fp32", fn);
+  if (batch <= 0 || total_rows < 0 || rows_per_batch < 1 || max_blocks <= 0 || page_block_size <= 0 || num_blocks <= 0)
+    return fail(DSA_ERR_INVALID, "%s: non-positive shape", fn);
+  if (((uintptr_t)cache & 15) != 0) return fail(DSA_ERR_INVALID, "%s: caches must be 16-byte aligned", fn);
+  return DSA_OK;
+}
+}  // namespace
+
+int dsa_rotary(const void* x, int64_t batch_stride, int64_t row_stride, int64_t head_stride, int dtype,
+               const void* positions, int positions_64, int axes, const int32_t* sections, const float* inv_freq,
+               int rows, int rows_per_batch, int heads, int width, int rotary_start, int rotary_dim, int interleaved,
+               int inverse, void* out, void* stream) {
+  if (!x || !positions || !out) return fail(DSA_ERR_INVALID, "dsa_rotary: null pointer argument");
+  if (!is16(dtype) && dtype != DSA_DTYPE_F32) return fail(DSA_ERR_INVALID, "dsa_rotary: dtype must be fp16, bf16 or fp32");
+  if (rows < 0 || rows_per_batch < 1 || heads <= 0 || width <= 0)
+    return fail(DSA_ERR_INVALID, "dsa_rotary: non-positive shape");
+  const int st = check_rotation("dsa_rotary", axes, sections, inv_freq, rotary_start, rotary_dim, width);
+  if (st != DSA_OK) return st;
+  if (width > 4096 || (int64_t)heads * width > (1 << 20))
+    return fail(DSA_ERR_UNSUPPORTED, "dsa_rotary: width %d > 4096, or heads * width > 2^20", width);
+  if (rows == 0) {
+    g_err[0] = 0;
+    return DSA_OK;
+  }
+  RotaryArgs a{x, batch_stride, row_stride, head_stride, dtype, positions, positions_64, axes, sections, inv_freq, rows,
+               rows_per_batch, heads, width, rotary_start, rotary_dim, interleaved, inverse, out};
+  return hip_status(launch_rotary(a, (hipStream_t)stream), "dsa_rotary launch");
+}
+
+int dsa_latent_append(const void* latent, int64_t batch_stride, int64_t row_stride, const void* key_rope,
+                      int64_t rope_batch_stride, int64_t rope_row_stride, int io_dtype, int d, const void* norm_weight,
+                      int w_dtype, float eps, const void* positions, int positions_64, int axes, const int32_t* sections,
+                      const float* inv_freq, int interleaved, const int32_t* row_start, const int32_t* act_q,
+                      const int32_t* act_k, const int32_t* block_table, int batch, int total_rows, int rows_per_batch,
+                      int max_blocks, int page_block_size, int64_t num_blocks, void* key_cache, void* key_rope_cache,
+                      void* stream) {
+  int st = check_append("dsa_latent_append", latent, io_dtype, norm_weight, w_dtype, row_start, act_q, act_k, block_table,
+                        batch, total_rows, rows_per_batch, max_blocks, page_block_size, num_blocks, key_cache);
+  if (st != DSA_OK) return st;
+  if (!key_rope || !key_rope_cache) return fail(DSA_ERR_INVALID, "dsa_latent_append: null pointer argument");
+  if (((uintptr_t)key_rope_cache & 15) != 0)
+    return fail(DSA_ERR_INVALID, "dsa_latent_append: caches must be 16-byte aligned");
+  if (d != 128 && d != 256 && d != 512) return fail(DSA_ERR_INVALID, "D must be one of (128, 256, 512), got %d", d);
+  st = check_rotation("dsa_latent_append", axes, sections, inv_freq, 0, 64, 64);
+  if (st != DSA_OK) return st;
+  if (total_rows == 0) {
+    g_err[0] = 0;
+    return DSA_OK;
+  }
+  AppendArgs a{latent, batch_stride, row_stride, 0, io_dtype, 1, d, key_rope, rope_batch_stride, rope_row_stride,
+               norm_weight ? 1 : 0, norm_weight, nullptr, w_dtype, eps, positions, positions_64, axes, sections, inv_freq,
+               0, 64, interleaved, row_start, act_q, act_k, block_table, batch, total_rows, rows_per_batch, max_blocks,
+               page_block_size, num_blocks, key_cache, key_rope_cache};
+  return hip_status(launch_cache_append(a, (hipStream_t)stream), "dsa_latent_append launch");
+}
+
+int dsa_index_append(const void* index_key, int64_t batch_stride, int64_t row_stride, int64_t head_stride, int io_dtype,
+                     int n2, int w, const void* norm_weight, const void* norm_bias, int w_dtype, float eps,
+                     const void* positions, int positions_64, int axes, const int32_t* sections, const float* inv_freq,
+                     int rotary_start, int rotary_dim, int interleaved, const int32_t* row_start, const int32_t* act_q,
+                     const int32_t* act_k, const int32_t* block_table, int batch, int total_rows, int rows_per_batch,
+                     int max_blocks, int page_block_size, int64_t num_blocks, void* index_cache, void* stream) {
+  int st = check_append("dsa_index_append", index_key, io_dtype, norm_weight, w_dtype, row_start, act_q, act_k, block_table,
+                        batch, total_rows, rows_per_batch, max_blocks, page_block_size, num_blocks, index_cache);
+  if (st != DSA_OK) return st;
+  if (n2 <= 0 || n2 > 65535) return fail(DSA_ERR_INVALID, "dsa_index_append: 1 to 65535 key heads, got %d", n2);
+  if (!li_score_supported_d(w))
+    return fail(DSA_ERR_UNSUPPORTED, "dsa_index_append: D=%d not in {64, 96, 128, 256, 512}", w);
+  if (norm_bias && !norm_weight) return fail(DSA_ERR_INVALID, "dsa_index_append: norm_bias without norm_weight");
+  st = check_rotation("dsa_index_append", axes, sections, inv_freq, rotary_start, rotary_dim, w);
+  if (st != DSA_OK) return st;
+  if (rotary_start % 8 != 0 || rotary_dim % 16 != 0)
+    return fail(DSA_ERR_UNSUPPORTED, "dsa_index_append: rotary_start %d is no multiple of 8, or rotary_dim %d of 16",
+                rotary_start, rotary_dim);
+  if (total_rows == 0) {
+    g_err[0] = 0;
+    return DSA_OK;
+  }
+  AppendArgs a{index_key, batch_stride, row_stride, head_stride, io_dtype, n2, w, nullptr, 0, 0, norm_weight ? 2 : 0,
+               norm_weight, norm_bias, w_dtype, eps, positions, positions_64, axes, sections, inv_freq, rotary_start,
+               rotary_dim, interleaved, row_start, act_q, act_k, block_table, batch, total_rows, rows_per_batch,
+               max_blocks, page_block_size, num_blocks, index_cache, nullptr};
+  return hip_status(launch_cache_append(a, (hipStream_t)stream), "dsa_index_append launch");
+}
+
 }  // extern "C"

@@ -488,3 +488,24 @@ hipError_t launch_dense_li_grad(const void* q, const void* k, const void* qr, co
                                 const int32_t* act_q, const int32_t* act_k, int batch, int s1, int s2, int n1,
                                 int n2, int d, int dr, int nidx1, int didx, float scale, void* dqi, void* dki,
                                 void* dw, float* loss, void* ws, hipStream_t s);
+// Rotary positions: x [batch, rows_per_batch, heads, width] by strides (elements) -> out, contiguous
+struct RotaryArgs {
+  const void* x; int64_t batch_stride, row_stride, head_stride; int io;
+  const void* positions; int wide; int axes; const int32_t* sections;   // sections: host, NULL with one axis
+  const float* freq; int rows, rows_per_batch, heads, width, start, rdim, interleaved, inverse;
+  void* out;
+};
+hipError_t launch_rotary(const RotaryArgs& a, hipStream_t s);
+// New tokens into a paged cache: latents (rope != NULL: normed, beside their rotated rotary keys) or
+// indexer keys (rope NULL: normed and rotated)
+struct AppendArgs {
+  const void* x; int64_t batch_stride, row_stride, head_stride; int io; int heads, width;
+  const void* rope; int64_t rope_batch_stride, rope_row_stride;
+  int norm_kind; const void* norm_w; const void* norm_b; int wdt; float eps;   // 0 none, 1 rms, 2 layer
+  const void* positions; int wide; int axes; const int32_t* sections;
+  const float* freq; int start, rdim, interleaved;
+  const int32_t* row_start; const int32_t* act_q; const int32_t* act_k; const int32_t* table;
+  int batch, total_rows, rows_per_batch, max_blocks, page; int64_t blocks;
+  void* cache; void* rope_cache;
+};
+hipError_t launch_cache_append(const AppendArgs& a, hipStream_t s);

@@ -1,0 +1,290 @@
+"""Rotary positions and the appends to the paged caches, on MI355X.
+
+The reference's operators take queries and keys already rotated and caches already filled; these
+are the steps before them: :func:`rotary_embedding` (and :func:`rotary_embedding_grad`) for
+``query_rope`` / ``key_rope`` and the indexer's queries, :func:`latent_cache_append` and
+:func:`index_cache_append` for the PA_BSND caches that ``sparse_flash_attention``,
+``shared_prefix_attention`` and ``lightning_indexer`` read. Layouts, lengths and block tables are
+those operators'.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _host as H
+from . import _lib
+
+VALID_D = (128, 256, 512)
+D_ROPE = 64
+INDEX_WIDTHS = (64, 96, 128, 256, 512)
+
+
+def _frequencies(inv_freq, pairs=None) -> torch.Tensor:
+    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dim() != 1 or inv_freq.dtype != torch.float32:
+        raise ValueError("inv_freq must be a float32 tensor [rotary_dim / 2]")
+    if inv_freq.numel() == 0 or (pairs is not None and inv_freq.numel() != pairs):
+        raise ValueError(f"inv_freq holds {inv_freq.numel()} pairs" + ("" if pairs is None else f", {pairs} wanted"))
+    return inv_freq.contiguous()
+
+
+def _sections(sections, pairs: int):
+    """(number of position axes, host int32 array or None)"""
+    if sections is None:
+        return 1, None
+    s = [int(v) for v in sections]
+    if not 1 <= len(s) <= 4 or min(s) < 0 or sum(s) != pairs:
+        raise ValueError(f"sections must be 1 to 4 counts of pairs that add up to {pairs}, got {s}")
+    return len(s), (ctypes.c_int32 * len(s))(*s)
+
+
+def _positions(positions, lead, axes: int, sectioned: bool) -> torch.Tensor:
+    """int32 / int64 positions of shape `lead` ([axes] + lead with sections), contiguous"""
+    want = ((axes,) if sectioned else ()) + tuple(lead)
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError("positions must be an int32 or int64 tensor")
+    if tuple(positions.shape) != want:
+        raise ValueError(f"positions must have shape {list(want)}, got {list(positions.shape)}")
+    return positions.contiguous()
+
+
+def _rows_view(x: torch.Tensor, layout: str, what: str):
+    """x with a contiguous last dimension, and its (batch, row, head) strides and rows per batch"""
+    if layout not in ("BSND", "TND"):
+        raise ValueError(f"unsupported layout {layout}")
+    if x.dim() != (4 if layout == "BSND" else 3):
+        raise ValueError(f"{what} must be {'[B, S, N, D]' if layout == 'BSND' else '[T, N, D]'}, got {list(x.shape)}")
+    if x.shape[-1] > 1 and x.stride(-1) != 1:
+        x = x.contiguous()
+    if layout == "BSND":
+        return x, x.stride(0), x.stride(1), x.stride(2), max(1, x.shape[1])
+    return x, 0, x.stride(0), x.stride(1), max(1, x.shape[0])
+
+
+def _rotate(x, positions, inv_freq, sections, rotary_start, interleaved, layout, inverse, what):
+    x, sb, ss, sh, per = _rows_view(x, layout, what)
+    freq = _frequencies(inv_freq)
+    dtype = H.dtype_code(x.dtype, what, allow_f32=True)
+    axes, sec = _sections(sections, freq.numel())
+    pos = _positions(positions, x.shape[:-2], axes, sec is not None)
+    n, width = x.shape[-2:]
+    if rotary_start < 0 or rotary_start + 2 * freq.numel() > width:
+        raise ValueError(f"rotary dimensions [{rotary_start}, {rotary_start} + {2 * freq.numel()}) of a width of {width}")
+    dev = H.require_device(x, pos, freq)
+    lib = _lib.load()
+    with H.on_device(dev):
+        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        if x.numel() == 0:
+            return out
+        _lib.check(lib.dsa_rotary(x.data_ptr(), sb, ss, sh, dtype, pos.data_ptr(), int(pos.dtype == torch.int64), axes, sec,
+                                  freq.data_ptr(), x.numel() // (n * width), per, n, width, int(rotary_start),
+                                  2 * freq.numel(), int(bool(interleaved)), inverse, out.data_ptr(), H.stream_ptr(dev)),
+                   "dsa_rotary")
+    return out
+
+
+def rotary_embedding(x, positions, inv_freq, sections=None, rotary_start=0, interleaved=True, layout="BSND"):
+    """Rotates the dimensions [rotary_start, rotary_start + 2 * len(inv_freq)) of every head of x by
+    its token's position; the others are copied.
+
+    x [B,S,N,D] (BSND) or [T,N,D] (TND), fp16 / bf16 / fp32, any strides; positions int32 / int64
+    [B,S] / [T]; inv_freq fp32, one inverse frequency a pair. Pair i is elements (2i, 2i+1) with
+    `interleaved`, else (i, i + rotary_dim/2). With `sections` (1 to 4 counts of pairs) positions are
+    [axes, B, S] / [axes, T], and each run of pairs turns by the position on its own axis: the time,
+    height and width of an image's or video's tokens. Angles are computed in 64 bits. Returns a new
+    contiguous tensor."""
+    return _rotate(x, positions, inv_freq, sections, rotary_start, interleaved, layout, 0, "x")
+
+
+def rotary_embedding_grad(d_out, positions, inv_freq, sections=None, rotary_start=0, interleaved=True, layout="BSND"):
+    """Gradient of :func:`rotary_embedding` with respect to x: d_out rotated back. (For the gradients
+    ``d_query_rope`` / ``d_key_rope`` of ``sparse_flash_attention_grad``, arguments as in the forward.)"""
+    return _rotate(d_out, positions, inv_freq, sections, rotary_start, interleaved, layout, 1, "d_out")
+
+
+class RotaryEmbedding(torch.nn.Module):
+    """Module form: keeps the inverse frequencies and the layout."""
+
+    def __init__(self, inv_freq, sections=None, rotary_start=0, interleaved=True, layout="BSND"):
+        super().__init__()
+        self.register_buffer("inv_freq", _frequencies(inv_freq), persistent=False)
+        self.sections = sections
+        self.rotary_start = rotary_start
+        self.interleaved = interleaved
+        self.layout = layout
+
+    def forward(self, x, positions):
+        return rotary_embedding(x, positions, self.inv_freq, self.sections, self.rotary_start, self.interleaved, self.layout)
+
+
+class _AppendPlan:
+    """What both appends share: the new tokens' rows, lengths and block table, and the norm's and the
+    rotation's arguments. All in place when the constructor returns, so ``run()`` may be called on
+    another stream; calls of one plan, and calls whose caches are the same, are ordered by the caller.
+    ``act_k`` (and ``block_table``) are read on the device in each run: a loop that keeps the plan may
+    write them anew between runs."""
+
+    def _setup(self, x, caches, block_table, inv_freq, pairs, actual_seq_lengths_kv, actual_seq_lengths_query, positions,
+               sections, layout, norm, more, what, _wait):
+        for c, name in caches:
+            if not isinstance(c, torch.Tensor) or not c.is_contiguous() or c.dim() != 4:
+                raise ValueError(f"{name} must be a contiguous tensor [num_blocks, block_size, N, D]")
+            if c.dtype != x.dtype:
+                raise ValueError(f"{name} dtype {c.dtype} differs from {what} dtype {x.dtype}")
+            if c.shape[:2] != caches[0][0].shape[:2]:
+                raise ValueError("the caches must have the same blocks")
+        self.freq = _frequencies(inv_freq, pairs)
+        self.axes, self.sec = _sections(sections, self.freq.numel())
+        if positions is None and self.axes > 1:
+            raise ValueError("several position axes need positions")
+        self.pos = None if positions is None else _positions(positions, x.shape[:-2], self.axes, self.sec is not None)
+        self.io = H.dtype_code(x.dtype, what)
+        self.wdt = self.io
+        for w in norm:
+            if w is not None:
+                self.wdt = H.dtype_code(w.dtype, "norm weights", allow_f32=True)
+                if w.dtype != norm[0].dtype or w.shape != (x.shape[-1],):
+                    raise ValueError(f"norm weights must share a dtype and have shape [{x.shape[-1]}]")
+        if layout == "TND":
+            act_q = H.per_batch_from_cumsum(H.host_lengths(actual_seq_lengths_query)) \
+                if actual_seq_lengths_query is not None else [x.shape[0]]
+            row_start = H.prefix(act_q)
+            if row_start[-1] > x.shape[0] or min(act_q, default=0) < 0:
+                raise ValueError("actual_seq_lengths_query must be cumulative and within the packed tokens")
+        else:
+            B, S = x.shape[:2]
+            act_q = H.batch_lengths(actual_seq_lengths_query, B, S, "actual_seq_lengths_query")
+            if min(act_q, default=0) < 0 or max(act_q, default=0) > S:
+                raise ValueError(f"actual_seq_lengths_query must lie between 0 and S = {S}")
+            row_start = [b * S for b in range(B + 1)]
+        act_k = H.host_lengths(actual_seq_lengths_kv)
+        if len(act_k) != len(act_q):
+            raise ValueError(f"batch mismatch: {len(act_q)} query batches, {len(act_k)} kv lengths")
+        if block_table.dim() != 2 or block_table.shape[0] != len(act_q):
+            raise ValueError("block_table must be [batch, max_blocks]")
+        self.num_blocks, self.page = caches[0][0].shape[:2]
+        self.batch, self.max_blocks = block_table.shape
+        self.total_rows = x.shape[0] * (x.shape[1] if layout == "BSND" else 1)
+        for q, k in zip(act_q, act_k):
+            if k < 0 or k > self.max_blocks * self.page:
+                raise ValueError(f"kv length {k} outside the block table's {self.max_blocks * self.page} tokens")
+        self.dev = H.require_device(self.x, block_table, self.freq, self.pos, *norm, *more, *[c for c, _ in caches])
+        self.lib = _lib.load()
+        with H.on_device(self.dev):
+            self.block_table = block_table.to(torch.int32).contiguous()
+            if self.batch and self.total_rows:
+                self.row_start, self.act_q, self.act_k = H.upload(self.lib, self.dev, row_start, act_q, act_k, wait=_wait)
+        self.empty = not (self.batch and self.total_rows and self.max_blocks and self.num_blocks and self.page)
+
+    def _places(self):
+        return (self.row_start.data_ptr(), self.act_q.data_ptr(), self.act_k.data_ptr(), self.block_table.data_ptr(),
+                self.batch, self.total_rows, self.per, self.max_blocks, self.page, self.num_blocks)
+
+    def _rotation(self):
+        return (H.ptr(self.pos), int(self.pos is not None and self.pos.dtype == torch.int64), self.axes, self.sec,
+                self.freq.data_ptr())
+
+
+class LatentAppendPlan(_AppendPlan):
+    """Validated arguments of one latent_cache_append call; ``run()`` launches on the current stream."""
+
+    def __init__(self, latent, key_rope, key_cache, key_rope_cache, block_table, inv_freq, actual_seq_lengths_kv,
+                 actual_seq_lengths_query=None, positions=None, norm_weight=None, norm_eps=1e-6, sections=None,
+                 interleaved=True, layout="BSND", *, _wait=True):
+        self.x, self.sb, self.ss, self.sh, self.per = _rows_view(latent, layout, "latent")
+        self.rope, self.rb, self.rs, _, _ = _rows_view(key_rope, layout, "key_rope")
+        d = latent.shape[-1]
+        if d not in VALID_D:
+            raise ValueError(f"D must be one of {VALID_D}, got {d}")
+        if key_rope.dtype != latent.dtype:
+            raise ValueError(f"key_rope dtype {key_rope.dtype} differs from latent dtype {latent.dtype}")
+        if key_rope.shape[-1] != D_ROPE:
+            raise ValueError(f"rope dim must be {D_ROPE}, got {key_rope.shape[-1]}")
+        if latent.shape[-2] != 1 or key_rope.shape[:-1] != latent.shape[:-1]:
+            raise ValueError("Only N2=1 (MQA) is supported, key_rope as many tokens as latent")
+        if tuple(key_cache.shape[2:]) != (1, d) or tuple(key_rope_cache.shape[2:]) != (1, D_ROPE):
+            raise ValueError(f"caches must be [num_blocks, block_size, 1, {d}] and [.., 1, {D_ROPE}]")
+        self._setup(latent, [(key_cache, "key_cache"), (key_rope_cache, "key_rope_cache")], block_table, inv_freq,
+                    D_ROPE // 2, actual_seq_lengths_kv, actual_seq_lengths_query, positions, sections, layout,
+                    (norm_weight,), (key_rope,), "latent", _wait)
+        self.d, self.inter, self.eps = d, int(bool(interleaved)), float(norm_eps)
+        self.norm_weight = None if norm_weight is None else norm_weight.contiguous()
+        self.key_cache, self.key_rope_cache = key_cache, key_rope_cache
+
+    def run(self):
+        if not self.empty:
+            with H.on_device(self.dev):
+                _lib.check(self.lib.dsa_latent_append(
+                    self.x.data_ptr(), self.sb, self.ss, self.rope.data_ptr(), self.rb, self.rs, self.io, self.d,
+                    H.ptr(self.norm_weight), self.wdt, self.eps, *self._rotation(), self.inter, *self._places(),
+                    self.key_cache.data_ptr(), self.key_rope_cache.data_ptr(), H.stream_ptr(self.dev)), "dsa_latent_append")
+        return self.key_cache, self.key_rope_cache
+
+
+class IndexAppendPlan(_AppendPlan):
+    """Validated arguments of one index_cache_append call; ``run()`` launches on the current stream."""
+
+    def __init__(self, index_key, index_cache, block_table, inv_freq, actual_seq_lengths_key,
+                 actual_seq_lengths_query=None, positions=None, norm_weight=None, norm_bias=None, norm_eps=1e-6,
+                 sections=None, rotary_start=0, interleaved=False, layout="BSND", *, _wait=True):
+        if norm_bias is not None and norm_weight is None:
+            raise ValueError("norm_bias needs norm_weight")
+        self.x, self.sb, self.ss, self.sh, self.per = _rows_view(index_key, layout, "index_key")
+        self.n2, self.w = index_key.shape[-2:]
+        if self.w not in INDEX_WIDTHS:
+            raise ValueError(f"D must be one of {INDEX_WIDTHS}, got {self.w}")
+        if tuple(index_cache.shape[2:]) != (self.n2, self.w):
+            raise ValueError(f"index_cache must be [num_blocks, block_size, {self.n2}, {self.w}]")
+        self.start, self.rdim = int(rotary_start), 2 * _frequencies(inv_freq).numel()
+        if self.start < 0 or self.start % 8 or self.rdim % 16 or self.start + self.rdim > self.w:
+            raise ValueError(f"rotary dimensions [{self.start}, {self.start} + {self.rdim}) of {self.w}: the start a "
+                             "multiple of 8, the count of 16")
+        self._setup(index_key, [(index_cache, "index_cache")], block_table, inv_freq, None, actual_seq_lengths_key,
+                    actual_seq_lengths_query, positions, sections, layout, (norm_weight, norm_bias), (), "index_key", _wait)
+        self.inter, self.eps = int(bool(interleaved)), float(norm_eps)
+        self.norm_weight, self.norm_bias = (None if t is None else t.contiguous() for t in (norm_weight, norm_bias))
+        self.index_cache = index_cache
+
+    def run(self):
+        if not self.empty:
+            with H.on_device(self.dev):
+                _lib.check(self.lib.dsa_index_append(
+                    self.x.data_ptr(), self.sb, self.ss, self.sh, self.io, self.n2, self.w, H.ptr(self.norm_weight),
+                    H.ptr(self.norm_bias), self.wdt, self.eps, *self._rotation(), self.start, self.rdim, self.inter,
+                    *self._places(), self.index_cache.data_ptr(), H.stream_ptr(self.dev)), "dsa_index_append")
+        return self.index_cache
+
+
+def latent_cache_append(latent, key_rope, key_cache, key_rope_cache, block_table, inv_freq, actual_seq_lengths_kv,
+                        actual_seq_lengths_query=None, positions=None, norm_weight=None, norm_eps=1e-6, sections=None,
+                        interleaved=True, layout="BSND"):
+    """Writes new tokens' latents (normed) and rotary keys (rotated) into the paged caches that
+    ``sparse_flash_attention`` and ``shared_prefix_attention`` read, in place.
+
+    latent [B,S,1,D] (BSND) or [T,1,D] (TND), key_rope [..,1,64]; key_cache [num_blocks, block_size, 1, D]
+    and key_rope_cache [.., 64], contiguous; block_table [B, max_blocks]; actual_seq_lengths_kv: each
+    sequence's length with its new tokens (per batch, as for the paged reads); actual_seq_lengths_query:
+    how many tokens are new (per batch, BSND; cumulative, TND). Token s of batch b goes to position
+    kv - query + s of its sequence, and turns by that position or by `positions` (as in
+    :func:`rotary_embedding`). norm_weight [D]: root-mean-square norm of the latent (None: stored as it
+    is). Tokens before position 0, or whose block is -1 or outside the cache, are not stored; no other
+    row of the caches changes. Two new tokens must not share a place. Returns the two caches."""
+    return LatentAppendPlan(latent, key_rope, key_cache, key_rope_cache, block_table, inv_freq, actual_seq_lengths_kv,
+                            actual_seq_lengths_query, positions, norm_weight, norm_eps, sections, interleaved, layout,
+                            _wait=False).run()
+
+
+def index_cache_append(index_key, index_cache, block_table, inv_freq, actual_seq_lengths_key,
+                       actual_seq_lengths_query=None, positions=None, norm_weight=None, norm_bias=None, norm_eps=1e-6,
+                       sections=None, rotary_start=0, interleaved=False, layout="BSND"):
+    """Writes new tokens' indexer keys into the paged cache that ``lightning_indexer`` (PA_BSND) reads,
+    in place: layer norm (norm_weight, norm_bias [D]; none if norm_weight is None), then the rotation of
+    the dimensions [rotary_start, rotary_start + 2 * len(inv_freq)), then the store.
+
+    index_key [B,S,N2,D] or [T,N2,D], index_cache [num_blocks, block_size, N2, D], D in
+    (64, 96, 128, 256, 512); places, positions and rules as :func:`latent_cache_append`. Returns the
+    cache."""
+    return IndexAppendPlan(index_key, index_cache, block_table, inv_freq, actual_seq_lengths_key,
+                           actual_seq_lengths_query, positions, norm_weight, norm_bias, norm_eps, sections, rotary_start,
+                           interleaved, layout, _wait=False).run()

@@ -368,6 +368,61 @@ int dsa_dense_li_grad_kl_loss(const void* query, const void* key, const void* qu
                               void* d_query_index, void* d_key_index, void* d_weights, float* loss,
                               void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Rotary positions (no counterpart in the reference, whose operators take rotated queries and
+ * keys). For row r, head h and pair i < rotary_dim / 2 of x[r, h, rotary_start ..]:
+ *   theta = positions[axis(i), r] * inv_freq[i]   (64-bit angles; negated if inverse is not 0)
+ *   (a, b) -> (a cos theta - b sin theta, a sin theta + b cos theta)
+ * with pair i at elements (2 i, 2 i + 1) if interleaved, else (i, i + rotary_dim / 2); the other
+ * elements of a head are copied. inverse = 1 is the gradient of the rotation (and its inverse).
+ *   x: [rows / rows_per_batch, rows_per_batch, heads, width] with the given strides in elements
+ *     (the last dimension contiguous), fp16 / bf16 / fp32, any alignment; out: the same type,
+ *     contiguous, not overlapping x. One rounding, from 32 bits.
+ *   positions: [axes, rows] int32, or int64 if positions_64; 1 <= axes <= 4. sections (host memory,
+ *     [axes], NULL with one axis): axis a has the next sections[a] pairs; they add up to rotary_dim / 2.
+ *   inv_freq [rotary_dim / 2] fp32. rotary_dim even, at most 1024; width <= 4096; heads * width <= 2^20.
+ */
+int dsa_rotary(const void* x, int64_t batch_stride, int64_t row_stride, int64_t head_stride, int dtype,
+               const void* positions, int positions_64, int axes, const int32_t* sections, const float* inv_freq,
+               int rows, int rows_per_batch, int heads, int width, int rotary_start, int rotary_dim, int interleaved,
+               int inverse, void* out, void* stream);
+
+/*
+ * Appends new tokens' latents and rotary keys to the paged caches that dsa_sfa_fwd and
+ * dsa_prefix_attn read (no counterpart in the reference). Packed row r is token s1 = r -
+ * row_start[b] of batch b, at position p = act_k[b] - act_q[b] + s1 of its sequence (act_k counts the
+ * new tokens), so cache row block_table[b, p / page] * page + p % page receives
+ *   key_cache      <- latent * norm_weight / sqrt(mean(latent^2) + eps)   (latent as it is if norm_weight is NULL)
+ *   key_rope_cache <- key_rope rotated as by dsa_rotary, at p or (positions not NULL) at positions[axes, total_rows]
+ * Statistics in 32 bits, one rounding. Rows with s1 >= act_q[b], behind the last batch, at p < 0, or
+ * whose block is -1 or outside the cache are not stored; nothing else of the caches is written. The
+ * rows' blocks must differ: two tokens of one place leave either's values, possibly mixed.
+ *   latent [.., d], key_rope [.., 64] (one head) by batch and row strides in elements as dsa_rotary
+ *   (rows_per_batch >= 1; total_rows for packed ones); d in {128, 256, 512}; caches [num_blocks, page, 1, d | 64],
+ *   16-byte aligned; norm_weight [d] in w_dtype (fp16 / bf16 / fp32); inv_freq [32] fp32.
+ */
+int dsa_latent_append(const void* latent, int64_t batch_stride, int64_t row_stride, const void* key_rope,
+                      int64_t rope_batch_stride, int64_t rope_row_stride, int io_dtype, int d, const void* norm_weight,
+                      int w_dtype, float eps, const void* positions, int positions_64, int axes, const int32_t* sections,
+                      const float* inv_freq, int interleaved, const int32_t* row_start, const int32_t* act_q,
+                      const int32_t* act_k, const int32_t* block_table, int batch, int total_rows, int rows_per_batch,
+                      int max_blocks, int page_block_size, int64_t num_blocks, void* key_cache, void* key_rope_cache,
+                      void* stream);
+
+/*
+ * Appends new tokens' indexer keys to the paged cache that dsa_li_score_paged reads: places, positions
+ * and rules of dsa_latent_append. Each of a token's n2 heads (width w in {64, 96, 128, 256, 512}) is
+ * normed ((x - mean) / sqrt(var + eps) * norm_weight + norm_bias; norm_bias may be NULL; no norm if
+ * norm_weight is NULL), then its elements [rotary_start, rotary_start + rotary_dim) are rotated
+ * (rotary_start a multiple of 8, rotary_dim of 16, inv_freq [rotary_dim / 2]).
+ */
+int dsa_index_append(const void* index_key, int64_t batch_stride, int64_t row_stride, int64_t head_stride, int io_dtype,
+                     int n2, int w, const void* norm_weight, const void* norm_bias, int w_dtype, float eps,
+                     const void* positions, int positions_64, int axes, const int32_t* sections, const float* inv_freq,
+                     int rotary_start, int rotary_dim, int interleaved, const int32_t* row_start, const int32_t* act_q,
+                     const int32_t* act_k, const int32_t* block_table, int batch, int total_rows, int rows_per_batch,
+                     int max_blocks, int page_block_size, int64_t num_blocks, void* index_cache, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
