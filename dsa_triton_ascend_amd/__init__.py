@@ -25,8 +25,9 @@ from .dense_loss import (DenseLightningIndexerGradKLLoss, DenseLightningIndexerS
                          npu_dense_lightning_indexer_softmax_lse)
 from .rotary import (IndexAppendPlan, LatentAppendPlan, RotaryEmbedding, index_cache_append, latent_cache_append,
                      rotary_embedding, rotary_embedding_grad)
+from .shared_prefix import SharedPrefixAttention, SharedPrefixPlan, shared_prefix_attention
 
-__all__ = ["rotary_embedding", "rotary_embedding_grad", "RotaryEmbedding", "latent_cache_append", "LatentAppendPlan",
+__all__ = ["shared_prefix_attention", "SharedPrefixAttention", "SharedPrefixPlan", "rotary_embedding", "rotary_embedding_grad", "RotaryEmbedding", "latent_cache_append", "LatentAppendPlan",
            "index_cache_append", "IndexAppendPlan", "lightning_indexer", "LightningIndexer", "sparse_flash_attention", "SparseFlashAttention",
            "sparse_flash_attention_grad", "SparseFlashAttentionGrad", "sparse_lightning_indexer_grad_kl_loss",
            "SparseLightningIndexerGradKLLoss", "dense_lightning_indexer_softmax_lse",

@@ -139,5 +139,11 @@ class on_device:
             self.guard.__exit__(*exc)
 
 
+def aligned16(t: torch.Tensor) -> torch.Tensor:
+    """t, contiguous and at a 16-byte border (a copy where it is not)"""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()

@@ -423,6 +423,42 @@ int dsa_index_append(const void* index_key, int64_t batch_stride, int64_t row_st
                      const int32_t* act_k, const int32_t* block_table, int batch, int total_rows, int rows_per_batch,
                      int max_blocks, int page_block_size, int64_t num_blocks, void* index_cache, void* stream);
 
+/*
+ * Workspace bytes of dsa_prefix_attn for these bounds (0 where every row has one range of tokens); needs
+ * no initialisation. kv_splits <= 0: the library's choice; pass the same value to both.
+ */
+size_t dsa_prefix_attn_workspace_bytes(int batch, int total_rows, int n1, int d, int prefix, int max_rows_per_batch,
+                                       int max_kv, int kv_splits);
+
+/*
+ * Dense attention over paged latents for a batch whose sequences share their first `prefix` tokens,
+ * MLA-absorb (value = key, one key head; no counterpart in the reference, whose attention is sparse).
+ * Packed row r is query s1 = r - row_start[b] of batch b and sees the tokens
+ *   t < act_k[b] - act_q[b] + s1 + 1 (sparse_mode 3) or t < act_k[b] (sparse_mode 0), 0 <= t < S2,
+ * S2 = max_blocks * page_block_size; act_k counts the prefix. Token t lies in block
+ * block_table[(t < prefix ? 0 : b) * max_blocks + t / page_block_size] (-1, or one outside the cache: a
+ * zero row, as dsa_sfa_fwd reads it): row 0 names the prefix of every sequence, and the other rows'
+ * entries for it are not read. prefix = 0 is dense attention without sharing.
+ *   score = (q . k + q_rope . k_rope) * scale, out = softmax(score) k, sm_max = max score,
+ *   sm_sum = sum exp(score - sm_max)   (both or neither may be NULL)
+ * Rows with s1 >= act_q[b], that see no token, or behind the last batch get out = 0, sm = 0. A row that
+ * sees a latent with values that are not finite gets NaN where the formula does (in those columns at
+ * least) and may get NaN in all; a row that does not see it is not affected.
+ *   query [total_rows, N1, D], query_rope [total_rows, N1, 64], key [num_blocks, page, 1, D], key_rope
+ *   [.., 64], fp16 / bf16, 16-byte aligned; N1 a power of two up to 128; D in {128, 256, 512};
+ *   num_blocks * page and total_rows * N1 < 2^31.
+ *   max_rows_per_batch: a bound on row_start[b+1] - row_start[b]; max_kv: the longest act_k that the caller
+ *   expects. max_kv only chooses how the work is cut: any act_k gives the same result to rounding.
+ *   kv_splits (<= 64): 0, or how many ranges of tokens the prefix (all tokens, where nothing is shared
+ *   among tiles) is cut into. Calls that share a workspace must be ordered.
+ */
+int dsa_prefix_attn(const void* query, const void* query_rope, const void* key, const void* key_rope, int io_dtype,
+                    const int32_t* block_table, int max_blocks, int page_block_size, int64_t num_blocks,
+                    const int32_t* row_start, const int32_t* act_q, const int32_t* act_k, int batch, int total_rows,
+                    int n1, int d, int dr, int prefix, int max_rows_per_batch, int max_kv, int sparse_mode, float scale,
+                    void* out, float* sm_max, float* sm_sum, void* workspace, size_t workspace_bytes, int kv_splits,
+                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif
