@@ -75,17 +75,27 @@ template <int IO> constexpr float lazy_tau() { return IO == IO_F16 ? 8.f : 40.f;
 template <int D> struct Tile {
   static constexpr int KSN = D / 16;           // 32x32x16 steps of the latent part
   static constexpr int KS = (D + DR) / 16;     // and with the rotary part
-  static constexpr int ROW = D * 2 + 128;      // LDS bytes of a token's row
+  static constexpr int ROW = D * 2 + 128;      // LDS bytes of a token's row: 128 modulo 256
   static constexpr int NOPE = BN * ROW;
   static constexpr int ROPE = BN * DR * 2;
   static constexpr int GPW = 10;               // direct-to-LDS loads per wave and tile: 8 rows, rope, ids
 };
-// Start of token t's row: shifted so that the operand reads (8 tokens, one column) and the
-// transposed reads (4 tokens, 32 bytes) land on distinct banks
-template <int D> __device__ __forceinline__ int nope_off(int t) {
-  return t * Tile<D>::ROW + 32 * (t & 3) + 16 * ((t >> 2) & 1);
+// Start of token t's row. In the LDS's 64 banks (256 bytes) it lies at 128 (t % 2) + 64 (t / 2 % 2) + 16
+// (t / 4 % 4): the operand reads (16 tokens, 16 bytes of one column) and the transposed reads (4
+// tokens, 64 bytes) both touch every bank once.
+template <int D> __host__ __device__ constexpr int nope_off(int t) {
+  return t * Tile<D>::ROW + 64 * ((t >> 1) & 1) + 16 * ((t >> 2) & 3);
 }
 __device__ __forceinline__ int rope_off(int t, int c) { return (t >> 3) * 1024 + (c * 8 + (t & 7)) * 16; }
+
+// o *= f on an accumulator element in an AGPR, which the VALU cannot use directly
+__device__ __forceinline__ float agpr_scale(float o, float f) {
+  float t;
+  asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %1, %2\n\tv_accvgpr_write_b32 %0, %1"
+               : "+a"(o), "=&v"(t)
+               : "v"(f));
+  return o;
+}
 
 // v_max3 without the quieting of each operand that fmaxf needs (a NaN score reaches the output
 // through its exponential either way)
@@ -131,49 +141,37 @@ template <int IO, int D, int MT>
 __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D>& L) {
   using C = Tile<D>;
   constexpr int KSPL = NWV / MT;             // waves of a row block
-  constexpr int KSH = C::KS / KSPL;          // their steps of S^T
-  static_assert(C::KS % KSPL == 0, "contraction split");
+  constexpr int KSH = C::KS / KSPL;          // their steps of S^T: wave kh takes steps j * KSPL + kh
+  constexpr int KNH = C::KSN / KSPL;         // of which in the latent part
+  static_assert(C::KS % KSPL == 0 && C::KSN % KSPL == 0 && KSH >= 3, "contraction split");
   constexpr int ON = D / 32 / KSPL;          // their 32-column tiles of O
   constexpr bool QLDS = MT == 4;             // the rotary part of Q stays in LDS
-  constexpr int QF = QLDS ? C::KSN : KSH;    // Q fragments in registers
+  constexpr int QF = QLDS ? KNH : KSH;       // Q fragments in registers
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rb = wave % MT, kh = wave / MT;
-  const int kg = lane >> 5;
-  const int h = it.h0 + rb * 32 + (lane & 31);
+  const int kg = lane >> 5, rr = lane & 31;
+  const int h = it.h0 + rb * 32 + rr;
   const bool valid = h < it.h_end;
-  const int hc = valid ? h : it.h_end - 1;
   const int m_rows = a.rows * a.n1;
-
-  // ---- Q^T fragments (B operand: this lane's head row, 8 values at 16 ks + 8 kg)
-  uint4 qf[QF];
-  {
-    const uint16_t* qn = a.q + (int64_t)hc * D;
-    const uint16_t* qr = a.qr + (int64_t)hc * DR;
-    if constexpr (QLDS) {
-#pragma unroll
-      for (int j = 0; j < QF; ++j) qf[j] = ldg16(qn + j * 16 + kg * 8);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<uint4*>(L.qr + (rb * 32 + (lane & 31)) * (DR + 8) + j * 16 + kg * 8) = ldg16(qr + j * 16 + kg * 8);
-    } else {
-#pragma unroll
-      for (int j = 0; j < QF; ++j) {
-        const int ks = kh * KSH + j;
-        qf[j] = ldg16((ks < C::KSN ? qn + ks * 16 : qr + (ks - C::KSN) * 16) + kg * 8);
-      }
-    }
-  }
   // the softmax works on raw scores times a positive factor: a negative scale negates the query, a
   // zero one becomes 1e-30 (scores round to 0, masked ones stay -inf)
   const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
   const float cpos = a.scale > 0.f ? a.scale : a.scale < 0.f ? -a.scale : 1e-30f;
   const float cl2 = cpos * LOG2E;
+
+  // ---- Q^T fragments (B operand: this lane's head row, 8 values at 16 ks + 8 kg)
+  uint4 qf[QF];
+  {
+    const int hc = valid ? h : it.h_end - 1;
+    const uint16_t* qn = a.q + (int64_t)hc * D + kh * 16 + kg * 8;
+    const uint16_t* qr = a.qr + (int64_t)hc * DR + kh * 16 + kg * 8;
+    auto flipped = [&](uint4 v) { return make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip); };
 #pragma unroll
-  for (int j = 0; j < QF; ++j) {
-    qf[j].x ^= flip;
-    qf[j].y ^= flip;
-    qf[j].z ^= flip;
-    qf[j].w ^= flip;
+    for (int j = 0; j < QF; ++j) qf[j] = flipped(ldg16(j < KNH ? qn + j * KSPL * 16 : qr + (j - KNH) * KSPL * 16));
+    if constexpr (QLDS)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<uint4*>(L.qr + (rb * 32 + rr) * (DR + 8) + j * 16 + kg * 8) = flipped(ldg16(qr + j * 16));
   }
 
   // ---- this head row's tokens: a row that sees none of the item's is dead: it runs along unmasked
@@ -184,9 +182,10 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
     lim = row_limit(a, row, it.b >= 0 ? it.b : batch_of(a, row));
   }
   const bool dead = lim <= it.t_lo;
-  int hi = dead ? 0 : min(lim, it.t_hi), lo = dead ? INT_MAX : hi;
+  lim = dead ? INT_MAX : min(lim, it.t_hi);   // within the item
+  int hi, min_lim;
   {
-    int mx = hi, mn = lo;
+    int mx = dead ? 0 : lim, mn = lim;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       mx = max(mx, __shfl_xor(mx, o));
@@ -197,17 +196,11 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
       L.red[1][wave] = mn;
     }
     __syncthreads();   // (and the rotary part of Q)
-    lim = lo;          // own limit within the item, INT_MAX for dead rows
-    hi = 0;
-    lo = INT_MAX;
-#pragma unroll
-    for (int w = 0; w < NWV; ++w) {
-      hi = max(hi, L.red[0][w]);
-      lo = min(lo, L.red[1][w]);
-    }
+    mx = max(max(L.red[0][0], L.red[0][1]), max(L.red[0][2], L.red[0][3]));
+    mn = min(min(L.red[1][0], L.red[1][1]), min(L.red[1][2], L.red[1][3]));
+    hi = __builtin_amdgcn_readfirstlane(mx);        // end of the item's tokens
+    min_lim = __builtin_amdgcn_readfirstlane(mn);   // from here on some row is masked
   }
-  hi = __builtin_amdgcn_readfirstlane(hi);          // end of the item's tokens
-  const int min_lim = __builtin_amdgcn_readfirstlane(lo);
   const bool direct = a.slots == 1;
   const bool writer = kh == 0 && lane < 32 && valid;   // one lane per head row
   if (hi <= it.t_lo) {   // no row sees any token
@@ -226,32 +219,40 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
 
   // ---- ids and gathers. Wave w copies tokens 8 w .. 8 w + 7 of each tile; their block ids travel the
   // same ordered path four tiles ahead, so nothing waits for them. Tokens past the end repeat the last
-  // one, tiles past the end the last tile: every wave issues the same loads per tile.
-  auto token = [&](int u, int j) { return min(it.t_lo + min(u, ntiles - 1) * BN + wave * 8 + j, hi - 1); };
+  // one, tiles past the end the last tile: every wave issues the same GPW loads per tile.
+  auto token = [&](int u) { return min(it.t_lo + min(u, ntiles - 1) * BN + wave * 8 + (lane & 7), hi - 1); };
   auto page_of = [&](int t) { return (int)(((uint64_t)(uint32_t)t * a.page_mul) >> (31 + a.page_shift)); };
-  auto ids_dma = [&](int u) {
-    const int t = token(u, lane & 7);
+  auto ids_dma = [&](int u) __attribute__((always_inline)) {
+    const int t = token(u);
     const int32_t* src = a.table + (t < a.prefix || it.b < 0 ? 0 : (int64_t)it.b * a.max_blocks) + page_of(t);
     if (lane < 8) lds_dma4_untracked(src, &L.ids[u & 3][wave * 8]);
   };
-  auto gather = [&](int u) {
-    const int t = token(u, lane & 7);
+  // cache row of token 8 w + lane % 8 of tile u, -1: its block is missing
+  auto tile_rows = [&](int u) __attribute__((always_inline)) {
+    const int t = token(u);
     const int32_t id = L.ids[u & 3][wave * 8 + (lane & 7)];
-    const int row = (uint32_t)id < a.blocks ? id * a.page + (t - page_of(t) * a.page) : -1;
-    uint8_t* nope = L.nope[u % NBUF];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int r = __builtin_amdgcn_readlane(row, j);
+    return (uint32_t)id < a.blocks ? id * a.page + (t - page_of(t) * a.page) : -1;
+  };
+  // one of the GPW - 1 gathers of a tile: the latent of token 8 w + j, or (j = 8) the wave's rotary
+  // parts. The empty asm keeps the address arithmetic here, among the MFMAs it is issued with.
+  auto gather_part = [&](int j, int row, uint8_t* nope, uint8_t* rope) __attribute__((always_inline)) {
+    if (j < 8) {
+      int r = __builtin_amdgcn_readlane(row, j);
+      asm volatile("" : "+s"(r));
       const uint16_t* src = r >= 0 ? a.k + (int64_t)r * D : reinterpret_cast<const uint16_t*>(g_zero_row);
       if (lane < D / 8) lds_dma16_sbase_untracked(src, lane * 16, nope + nope_off<D>(wave * 8 + j));
+    } else {
+      int r = row;
+      asm volatile("" : "+v"(r));
+      const uint16_t* src = r >= 0 ? a.kr + (int64_t)r * DR : reinterpret_cast<const uint16_t*>(g_zero_row);
+      lds_dma16_untracked(src + (lane >> 3) * 8, rope + wave * 1024);
     }
-    const uint16_t* src = row >= 0 ? a.kr + (int64_t)row * DR : reinterpret_cast<const uint16_t*>(g_zero_row);
-    lds_dma16_untracked(src + (lane >> 3) * 8, L.rope[u % NBUF] + wave * 1024);
   };
   // A tile that some of the head rows see only in part: a masked token has P = 0, but 0 times a value
   // that is not finite would still reach the rows that do not see it. Such values become 0 in LDS, and
   // the token's score NaN for the rows that do see it. (Each wave its own rows, landed by now.)
-  auto sanitize = [&](int u) {
+  auto is_mixed = [&](int u) { return min_lim < hi && it.t_lo + u * BN + BN > min_lim; };
+  auto sanitize = [&](int u) __attribute__((always_inline)) {
     uint32_t bad = 0;
 #pragma unroll 1
     for (int j = 0; j < 8; ++j) {
@@ -274,120 +275,236 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   for (int u = 0; u < 4; ++u) ids_dma(u);
   wait_vmcnt<0>();
   asm volatile("" ::: "memory");
-  gather(0);
-  gather(1);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int row = tile_rows(u);
+#pragma unroll
+    for (int j = 0; j < 9; ++j) gather_part(j, row, L.nope[u], L.rope[u]);
+  }
 
+  {   // an AGPR operand makes the compiler keep the MFMA accumulators there, the VGPRs free for operands
+    float agpr_hint = 0.f;
+    asm volatile("" : "+a"(agpr_hint));
+  }
   f32x16 o[ON];
 #pragma unroll
   for (int n = 0; n < ON; ++n)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
-  float m_used = -INFINITY, m_true = -INFINITY, l_part = 0.f;
 
-  // S^T rows are permuted so that a lane's 16 scores are tokens 16 (i / 8) + 8 kg + i % 8: the order of
-  // the B operand of the PV product
-  const int rr = lane & 31;
+  // ---- S^T of tile u. Its rows are permuted so that a lane's 16 scores are tokens 16 (i / 8) + 8 kg +
+  // i % 8: the order of the B operand of the PV product. Operands are read KPF steps ahead; `spread(j)`
+  // issues what rides on step j, `pre()` what covers the first operands' latency.
   const int tk = 16 * (rr >> 4) + 8 * ((rr >> 2) & 1) + 4 * ((rr >> 3) & 1) + (rr & 3);
-  const int g16 = lane >> 4, c16 = lane & 15;
-  const int vlane = nope_off<D>((g16 >> 1) * 8 + (c16 >> 2)) + ((g16 & 1) * 16 + 4 * (c16 & 3)) * 2 + kh * (D / KSPL) * 2;
-
-  for (int t = 0; t < ntiles; ++t) {
-    if (t == 0) wait_vmcnt<C::GPW - 1>();   // tile 0 here, tile 1 may be under way
-    else wait_vmcnt<C::GPW>();
-    const int t0 = it.t_lo + t * BN;
-    uint8_t* nope = L.nope[t % NBUF];
-    uint8_t* rope = L.rope[t % NBUF];
-    const bool mixed = min_lim < hi && t0 + BN > min_lim;
-    if (mixed) sanitize(t);
-    lds_barrier();   // tile t resident, every wave done with tile t - 1
-    gather(t + 2);
-    ids_dma(t + 4);
-
-    // ---- S^T
-    f32x16 sv;
+  constexpr int KPF = KSH < 5 ? KSH : 5;
+  auto s_tile = [&](int u, auto&& spread, auto&& pre) __attribute__((always_inline)) -> f32x16 {
+    const uint8_t* arow = L.nope[u % NBUF] + nope_off<D>(tk) + kg * 16 + kh * 32;
+    const uint8_t* rrow = L.rope[u % NBUF] + rope_off(tk, kh * 2 + kg);
+    auto a_frag = [&](int j) -> uint4 {
+      return j < KNH ? *reinterpret_cast<const uint4*>(arow + j * KSPL * 32)
+                     : *reinterpret_cast<const uint4*>(rrow + (j - KNH) * KSPL * 256);
+    };
+    constexpr int NR = QLDS ? KSH - KNH : 1;
+    uint4 qr[NR];
+    auto qr_frag = [&](int j) -> uint4 {
+      return *reinterpret_cast<const uint4*>(L.qr + (rb * 32 + rr) * (DR + 8) + j * 16 + kg * 8);
+    };
+    uint4 af[KPF];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sv[i] = 0.f;
+    for (int j = 0; j < KPF; ++j) af[j] = a_frag(j);
+    pre();
+    f32x16 acc;
 #pragma unroll
     for (int j = 0; j < KSH; ++j) {
-      const int ks = kh * KSH + j;
-      const uint4 kf = *reinterpret_cast<const uint4*>(ks < C::KSN ? nope + nope_off<D>(tk) + kg * 16 + ks * 32
-                                                                   : rope + rope_off(tk, (ks - C::KSN) * 2 + kg));
-      uint4 qv;
-      if (QLDS && j >= C::KSN) {
-        qv = *reinterpret_cast<const uint4*>(L.qr + (rb * 32 + rr) * (DR + 8) + (j - C::KSN) * 16 + kg * 8);
-        qv.x ^= flip, qv.y ^= flip, qv.z ^= flip, qv.w ^= flip;
-      } else {
-        qv = qf[j < QF ? j : 0];
+      uint4 bq;
+      if constexpr (QLDS) bq = j < KNH ? qf[j < QF ? j : 0] : qr[j >= KNH ? j - KNH : 0];
+      else bq = qf[j];
+      if (j == 0) acc = mfma32_vacc_first<IO>(af[0], bq);
+      else if (j < KSH - 1) mfma32_vacc<IO>(acc, af[j % KPF], bq);
+      else acc = mfma32_vacc_last_to<IO>(acc, af[j % KPF], bq);
+      if (j + KPF < KSH) af[j % KPF] = a_frag(j + KPF);
+      if constexpr (QLDS)
+        if (j + KPF < KSH && j + KPF >= KNH) qr[j + KPF - KNH] = qr_frag(j + KPF - KNH);
+      spread(j);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return acc;
+  };
+  // several waves of a row block add their parts in one order: the same bits in each
+  auto put_part = [&](const f32x16& sv) __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<float4*>(&L.x[wave][(g * 64 + lane) * 4]) =
+          make_float4(sv[4 * g], sv[4 * g + 1], sv[4 * g + 2], sv[4 * g + 3]);
+  };
+  auto sum_parts = [&]() __attribute__((always_inline)) -> f32x16 {
+    f32x16 sv;
+#pragma unroll
+    for (int w = 0; w < KSPL; ++w)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 p = *reinterpret_cast<const float4*>(&L.x[rb + MT * w][(g * 64 + lane) * 4]);
+        sv[4 * g] = w == 0 ? p.x : sv[4 * g] + p.x;
+        sv[4 * g + 1] = w == 0 ? p.y : sv[4 * g + 1] + p.y;
+        sv[4 * g + 2] = w == 0 ? p.z : sv[4 * g + 2] + p.z;
+        sv[4 * g + 3] = w == 0 ? p.w : sv[4 * g + 3] + p.w;
       }
-      sv = Mfma<IO>::m32(kf, qv, sv);
-    }
-    if constexpr (KSPL > 1) {   // the waves of a block add their parts in one order: the same bits in each
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<float4*>(&L.x[wave][(g * 64 + lane) * 4]) =
-            make_float4(sv[4 * g], sv[4 * g + 1], sv[4 * g + 2], sv[4 * g + 3]);
-      lds_barrier();
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sv[i] = 0.f;
-#pragma unroll
-      for (int w = 0; w < KSPL; ++w)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float4 p = *reinterpret_cast<const float4*>(&L.x[rb + MT * w][(g * 64 + lane) * 4]);
-          sv[4 * g] += p.x;
-          sv[4 * g + 1] += p.y;
-          sv[4 * g + 2] += p.z;
-          sv[4 * g + 3] += p.w;
-        }
-    }
-    if (mixed) {
-      const uint32_t bad = L.bad[t & 1][0] | L.bad[t & 1][1] | L.bad[t & 1][2] | L.bad[t & 1][3];
+    return sv;
+  };
+  auto mask = [&](int u, f32x16& sv) __attribute__((always_inline)) {
+    const int t0 = it.t_lo + u * BN;
+    if (t0 + BN <= min_lim) return;
+    if (is_mixed(u)) {
+      const uint32_t bad = L.bad[u & 1][0] | L.bad[u & 1][1] | L.bad[u & 1][2] | L.bad[u & 1][3];
       if (bad)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if ((bad >> (16 * (i >> 3) + 8 * kg + (i & 7))) & 1u) sv[i] = __builtin_nanf("");
     }
-    if (t0 + BN > min_lim) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sv[i] = t0 + 16 * (i >> 3) + 8 * kg + (i & 7) < lim ? sv[i] : -INFINITY;
+    for (int i = 0; i < 16; ++i) sv[i] = t0 + 16 * (i >> 3) + 8 * kg + (i & 7) < lim ? sv[i] : -INFINITY;
+  };
+
+  // ---- online softmax in NST stages of a few VALU operations each, placed among the previous tile's
+  // PV MFMAs: 0-3 the maximum, 4 the reference maximum, 5-12 two exponentials each, 13 the sum and the
+  // B operands of the two 16-token steps. Raw scores; max(c s) = c max(s) as c > 0. The reference m_used
+  // moves only past the lazy threshold, so the output's factor alpha is nearly always 1.
+  float m_used = -INFINITY, m_true = -INFINITY, l_part = 0.f, alpha = 1.f;
+  float sm_mx = 0.f, sm_mb = 0.f, sm_sum = 0.f;
+  uint32_t sm_d[4][2];
+  uint4 pb[2], pn[2];   // P of the tile whose PV runs, and of the next one
+  constexpr int NST = 14;
+  auto smx = [&](int st, const f32x16& sv) __attribute__((always_inline)) {
+    if (st < 4) {
+      const int b = 4 * st;
+      sm_mx = st == 0 ? max3(sv[0], sv[1], sv[2]) : max3(sm_mx, sv[b], sv[b + 1]);
+      sm_mx = st == 0 ? max3(sm_mx, sv[3], sv[3]) : max3(sm_mx, sv[b + 2], sv[b + 3]);
+    } else if (st == 4) {
+      const float mx = max_half_swap(sm_mx) * cpos;
+      m_true = max3(m_true, mx, mx);
+      const float m_new = mx > m_used + lazy_tau<IO>() ? mx : m_used;
+      alpha = m_used == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_used - m_new) * LOG2E);
+      m_used = m_new;
+      sm_mb = m_used * LOG2E;
+      sm_sum = 0.f;
+    } else if (st < NST - 1) {
+      const int i = 2 * (st - 5);
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], cl2, -sm_mb));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i + 1], cl2, -sm_mb));
+      sm_sum += p0;
+      sm_sum += p1;
+      sm_d[i >> 2][(i >> 1) & 1] = pack2<IO>(p0, p1);
+    } else {
+      l_part = l_part * alpha + sm_sum;
+      pn[0] = make_uint4(sm_d[0][0], sm_d[0][1], sm_d[1][0], sm_d[1][1]);
+      pn[1] = make_uint4(sm_d[2][0], sm_d[2][1], sm_d[3][0], sm_d[3][1]);
     }
-    // ---- online softmax
-    float mx = max3(sv[0], sv[1], sv[2]);
-#pragma unroll
-    for (int i = 3; i < 15; i += 2) mx = max3(mx, sv[i], sv[i + 1]);
-    mx = max_half_swap(fmaxf(mx, sv[15])) * cpos;
-    m_true = fmaxf(m_true, mx);
-    const float m_new = mx > m_used + lazy_tau<IO>() || m_used == -INFINITY ? mx : m_used;
-    const float alpha = m_used == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_used - m_new) * LOG2E);
-    m_used = m_new;
-    const float mb = m_used * LOG2E;
-    float p[16], sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], cl2, -mb));
-      sum += p[i];
-    }
-    l_part = l_part * alpha + sum;
+  };
+  auto rescale = [&]() __attribute__((always_inline)) {
     if (__builtin_amdgcn_ballot_w64(alpha != 1.f)) {
 #pragma unroll
       for (int n = 0; n < ON; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[n][i] *= alpha;
+        for (int i = 0; i < 16; ++i) o[n][i] = agpr_scale(o[n][i], alpha);
     }
-    // ---- O^T += V^T P^T
+  };
+
+  // ---- O^T += V^T P^T: MFMA m is column tile m % ON of 16-token step m / ON. The transposed operands
+  // run VR MFMAs ahead in one ring across tiles: past a tile's last MFMA the reads go on with the next
+  // tile's first operands, resident since the barrier before.
+  const int g16 = lane >> 4, c16 = lane & 15;
+  // (tok0 has bit 2 clear: four tokens on is 4 ROW + 16 bytes on)
+  const int vlane = nope_off<D>((g16 >> 1) * 8 + (c16 >> 2)) + ((g16 & 1) * 16 + 4 * (c16 & 3)) * 2 + kh * (D / KSPL) * 2;
+  constexpr int NPV = 2 * ON;
+  constexpr int VR = NPV < 8 ? NPV : 8;
+  constexpr int NPRE = NPV >= 16 ? 6 : NPV / 4;                       // before the next tile's S^T
+  constexpr int NMID = KSPL > 1 ? NPRE + (NPV - NPRE) / 2 : NPRE;     // before its partial sums are read
+  uint4 vb[VR];
+  auto v_base = [&](int u) __attribute__((always_inline)) -> uint32_t {
+    uint32_t b = lds_addr(L.nope[u % NBUF]) + vlane;
+    asm volatile("" : "+v"(b));   // constant offsets then go into the reads
+    return b;
+  };
+  auto v_frag = [&](uint32_t b, int m) __attribute__((always_inline)) -> uint4 {
+    const uint32_t p = b + (m / ON) * 16 * C::ROW + (m % ON) * 64;
+    const uint2 lo = ds_read_tr_at(p), hi2 = ds_read_tr_at(p + 4 * C::ROW + 16);
+    return make_uint4(lo.x, lo.y, hi2.x, hi2.y);
+  };
+  auto pv_run = [&](int m0, int m1, uint32_t vbase, uint32_t vnext, bool next, auto&& between)
+      __attribute__((always_inline)) {
 #pragma unroll
-    for (int kq = 0; kq < 2; ++kq) {
-      const uint4 pb = make_uint4(pack2<IO>(p[8 * kq], p[8 * kq + 1]), pack2<IO>(p[8 * kq + 2], p[8 * kq + 3]),
-                                  pack2<IO>(p[8 * kq + 4], p[8 * kq + 5]), pack2<IO>(p[8 * kq + 6], p[8 * kq + 7]));
-#pragma unroll
-      for (int n = 0; n < ON; ++n) {
-        const uint8_t* v = nope + vlane + kq * 16 * C::ROW + n * 64;
-        const uint2 lo2 = ds_read_tr(v), hi2 = ds_read_tr(v + 4 * C::ROW + 16);
-        o[n] = Mfma<IO>::m32(make_uint4(lo2.x, lo2.y, hi2.x, hi2.y), pb, o[n]);
-      }
+    for (int m = m0; m < m1; ++m) {
+      o[m % ON] = Mfma<IO>::m32(vb[m % VR], pb[m / ON], o[m % ON]);
+      if (m + VR < NPV) vb[m % VR] = v_frag(vbase, m + VR);
+      else if (next) vb[m % VR] = v_frag(vnext, m + VR - NPV);
+      between(m);
+      __builtin_amdgcn_sched_barrier(0);
     }
+  };
+
+  wait_vmcnt<C::GPW - 1>();   // tile 0 here, tile 1 may be under way
+  if (is_mixed(0)) sanitize(0);
+  lds_barrier();
+  {
+    f32x16 s0 = s_tile(0, [](int) {}, [] {});
+    if constexpr (KSPL > 1) {
+      put_part(s0);
+      lds_barrier();
+      s0 = sum_parts();
+    }
+    mask(0, s0);
+#pragma unroll
+    for (int st = 0; st < NST; ++st) smx(st, s0);
+    const uint32_t vb0 = v_base(0);
+#pragma unroll
+    for (int m = 0; m < VR; ++m) vb[m] = v_frag(vb0, m);
   }
-  wait_vmcnt<0>();   // the ring's last gathers land before the LDS is released
+  // Iteration t: PV of tile t around S^T of tile t + 1, on whose steps the gathers of tile t + 2 ride; the
+  // softmax of tile t + 1 runs among the last PV MFMAs.
+  for (int tv = 0; tv + 1 < ntiles; ++tv) {
+    const int t = __builtin_amdgcn_readfirstlane(tv);   // (the compiler may keep the counter in a VGPR)
+    pb[0] = pn[0];
+    pb[1] = pn[1];
+    rescale();
+    if (t == 0) wait_vmcnt<0>();   // this wave's part of tile t + 1 (its ids copy may be under way)
+    else wait_vmcnt<1>();
+    if (is_mixed(t + 1)) sanitize(t + 1);
+    lds_barrier();   // tile t + 1 resident; every wave done with tile t - 1, whose buffer is free
+    const int row = tile_rows(t + 2);
+    const int gb = __builtin_amdgcn_readfirstlane((t + 2) % NBUF);   // the free buffer
+    uint8_t* const gnope = L.nope[gb];
+    uint8_t* const grope = L.rope[gb];
+    const uint32_t vbase = v_base(t), vnext = v_base(t + 1);
+    f32x16 s1 = s_tile(
+        t + 1,
+        [&](int ks) __attribute__((always_inline)) {
+#pragma unroll
+          for (int j = 0; j < C::GPW; ++j)
+            if (j * KSH / C::GPW == ks) {
+              if (j < C::GPW - 1) gather_part(j, row, gnope, grope);
+              else ids_dma(t + 4);   // the slot of tile t's ids, read two iterations ago
+            }
+        },
+        [&]() __attribute__((always_inline)) { pv_run(0, NPRE, vbase, vnext, true, [](int) {}); });
+    if constexpr (KSPL > 1) {
+      put_part(s1);
+      pv_run(NPRE, NMID, vbase, vnext, true, [](int) {});
+      lds_barrier();
+      s1 = sum_parts();
+    }
+    mask(t + 1, s1);
+    pv_run(NMID, NPV, vbase, vnext, true, [&](int m) __attribute__((always_inline)) {
+#pragma unroll
+      for (int st = 0; st < NST; ++st)
+        if (st * (NPV - NMID) / NST == m - NMID) smx(st, s1);
+    });
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  pb[0] = pn[0];
+  pb[1] = pn[1];
+  rescale();
+  pv_run(0, NPV, v_base(ntiles - 1), 0u, false, [](int) {});
+  wait_vmcnt<0>();   // the ring's last (unused) gathers land before the LDS is released
 
   // ---- epilogue: lane l holds head row h, columns n * 32 + 8 g + 4 kg + j of o[n][4 g + j]
   const float l_tot = add_half_swap(l_part);
@@ -400,29 +517,38 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
       a.sm_sum[h] = dead ? 0.f : l_tot * exp2f((m_used - m_true) * LOG2E);
     }
   }
-  if (!valid) return;
-  const int c0 = kh * (D / KSPL) + 4 * kg;
   if (!direct) {
-    if (dead) return;
-    float* dst = a.part_o + ((int64_t)it.slot * m_rows + h) * D + c0;
+    if (!valid || dead) return;
+    float* dst = a.part_o + ((int64_t)it.slot * m_rows + h) * D + kh * (D / KSPL) + 4 * kg;
 #pragma unroll
     for (int n = 0; n < ON; ++n)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         *reinterpret_cast<float4*>(dst + n * 32 + 8 * g) =
             make_float4(o[n][4 * g], o[n][4 * g + 1], o[n][4 * g + 2], o[n][4 * g + 3]);
-  } else {
-    const float inv = dead ? 0.f : 1.f / l_tot;
-    uint16_t* dst = a.out + (int64_t)h * D + c0;
+    return;
+  }
+  // two exchanges between lane halves leave lanes 0-31 with columns [0, 8) and [16, 24) of a 32-column
+  // tile, the others with [8, 16) and [24, 32): 16-byte stores
+  const float inv = 1.f / l_tot;
+  uint16_t* dst = a.out + (int64_t)(valid ? h : 0) * D + kh * (D / KSPL) + 8 * kg;
 #pragma unroll
-    for (int n = 0; n < ON; ++n)
+  for (int n = 0; n < ON; ++n) {
+    uint32_t d[4][2];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float v[4];
+    for (int g = 0; g < 4; ++g) {
+      d[g][0] = dead ? 0u : pack2<IO>(o[n][4 * g] * inv, o[n][4 * g + 1] * inv);
+      d[g][1] = dead ? 0u : pack2<IO>(o[n][4 * g + 2] * inv, o[n][4 * g + 3] * inv);
+    }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = dead ? 0.f : o[n][4 * g + j] * inv;
-        *reinterpret_cast<uint2*>(dst + n * 32 + 8 * g) = make_uint2(pack2<IO>(v[0], v[1]), pack2<IO>(v[2], v[3]));
-      }
+    for (int j = 0; j < 2; ++j) {
+      swap_halves(d[0][j], d[1][j]);
+      swap_halves(d[2][j], d[3][j]);
+    }
+    if (valid) {
+      stg16(dst + n * 32, make_uint4(d[0][0], d[0][1], d[1][0], d[1][1]));
+      stg16(dst + n * 32 + 16, make_uint4(d[2][0], d[2][1], d[3][0], d[3][1]));
+    }
   }
 }
 
