@@ -53,9 +53,9 @@ SIGNATURES = {
     "dsa_sfa_bwd_workspace_bytes": (_SZ, [_I, _P, _P, _I, _I, _I, _I, _I, _I, _I64]),
     "dsa_sfa_bwd": (_I, [_P, _P, _P, _P, _I, _P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I,
                          _I, _I64, _I, _F, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
-    "dsa_prefix_attn_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I, _I]),
-    "dsa_prefix_attn": (_I, [_P, _P, _P, _P, _I, _P, _I, _I, _I64, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P,
-                             _P, _P, _P, _SZ, _I, _P]),
+    "dsa_prefix_attn_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I, _I64, _I]),
+    "dsa_prefix_attn": (_I, [_P, _P, _P, _P, _I, _P, _I, _I, _I64, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I64, _I, _F,
+                             _P, _P, _P, _P, _SZ, _I, _P]),
     "dsa_rotary": (_I, [_P, _I64, _I64, _I64, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P]),
     "dsa_latent_append": (_I, [_P, _I64, _I64, _P, _I64, _I64, _I, _I, _P, _I, _F, _P, _I, _I, _P, _P, _I, _P, _P, _P,
                                _P, _I, _I, _I, _I, _I, _I64, _P, _P, _P]),

@@ -625,16 +625,17 @@ int dsa_index_append(const void* index_key, int64_t batch_stride, int64_t row_st
 }
 
 size_t dsa_prefix_attn_workspace_bytes(int batch, int total_rows, int n1, int d, int prefix, int max_rows_per_batch,
-                                       int max_kv, int kv_splits) {
-  if (batch <= 0 || total_rows <= 0 || n1 <= 0 || d <= 0 || prefix < 0 || max_rows_per_batch < 0 || max_kv < 0) return 0;
-  return prefix_attn_workspace_bytes(batch, total_rows, n1, d, prefix, max_rows_per_batch, max_kv, kv_splits);
+                                       int max_kv, int64_t total_kv, int kv_splits) {
+  if (batch <= 0 || total_rows <= 0 || n1 <= 0 || d <= 0 || prefix < 0 || max_rows_per_batch < 0 || max_kv < 0 || total_kv < 0)
+    return 0;
+  return prefix_attn_workspace_bytes(batch, total_rows, n1, d, prefix, max_rows_per_batch, max_kv, total_kv, kv_splits);
 }
 
 int dsa_prefix_attn(const void* query, const void* query_rope, const void* key, const void* key_rope, int io_dtype,
                     const int32_t* block_table, int max_blocks, int page_block_size, int64_t num_blocks,
                     const int32_t* row_start, const int32_t* act_q, const int32_t* act_k, int batch, int total_rows,
-                    int n1, int d, int dr, int prefix, int max_rows_per_batch, int max_kv, int sparse_mode, float scale,
-                    void* out, float* sm_max, float* sm_sum, void* workspace, size_t workspace_bytes, int kv_splits,
+                    int n1, int d, int dr, int prefix, int max_rows_per_batch, int max_kv, int64_t total_kv, int sparse_mode,
+                    float scale, void* out, float* sm_max, float* sm_sum, void* workspace, size_t workspace_bytes, int kv_splits,
                     void* stream) {
   if (!query || !query_rope || !key || !key_rope || !block_table || !row_start || !act_q || !act_k || !out)
     return fail(DSA_ERR_INVALID, "dsa_prefix_attn: null pointer argument");
@@ -646,7 +647,7 @@ int dsa_prefix_attn(const void* query, const void* query_rope, const void* key, 
   if (n1 < 1 || n1 > 128 || (n1 & (n1 - 1)) != 0)
     return fail(DSA_ERR_INVALID, "N1 must be one of (1, 2, 4, 8, 16, 32, 64, 128), got %d", n1);
   if (batch <= 0 || total_rows < 0 || max_blocks <= 0 || page_block_size <= 0 || num_blocks <= 0 || prefix < 0 ||
-      max_rows_per_batch < 0 || max_kv < 0)
+      max_rows_per_batch < 0 || max_kv < 0 || total_kv < 0)
     return fail(DSA_ERR_INVALID, "dsa_prefix_attn: non-positive shape");
   const int64_t s2 = (int64_t)max_blocks * page_block_size;
   if (prefix > s2 || max_kv > s2)
@@ -662,12 +663,12 @@ int dsa_prefix_attn(const void* query, const void* query_rope, const void* key, 
     g_err[0] = 0;
     return DSA_OK;
   }
-  const size_t need = prefix_attn_workspace_bytes(batch, total_rows, n1, d, prefix, max_rows_per_batch, max_kv, kv_splits);
+  const size_t need = prefix_attn_workspace_bytes(batch, total_rows, n1, d, prefix, max_rows_per_batch, max_kv, total_kv, kv_splits);
   if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0))
     return fail(DSA_ERR_INVALID, "dsa_prefix_attn: a 16-byte aligned workspace of %zu bytes required, %zu given", need,
                 workspace ? workspace_bytes : (size_t)0);
   PrefixArgs a{query, query_rope, key, key_rope, io_dtype, block_table, max_blocks, page_block_size, num_blocks, row_start,
-               act_q, act_k, batch, total_rows, n1, d, prefix, max_rows_per_batch, max_kv, sparse_mode, scale, out, sm_max,
+               act_q, act_k, batch, total_rows, n1, d, prefix, max_rows_per_batch, max_kv, total_kv, sparse_mode, scale, out, sm_max,
                sm_sum, workspace, kv_splits};
   return hip_status(launch_prefix_attn(a, (hipStream_t)stream), "dsa_prefix_attn launch");
 }

@@ -15,11 +15,13 @@
 // Both kinds of item, each over a range of tokens, run in one launch; a second one joins the ranges'
 // (max, sum, output) per head row, unless every row had a single range.
 //
-// An item is one work-group of four waves and 32, 64 or 128 head rows (MT 32-row blocks). Tiles of 32
-// tokens go direct to a ring of three LDS buffers, two tiles ahead. S^T = K Q^T has the tokens as M and
+// An item is one work-group of four waves and 32, 64 or 128 head rows. With 64 or 128 (MT = 2, 4 blocks
+// of 32 rows) tiles of 32 tokens go direct to a ring of three LDS buffers, two tiles ahead. S^T = K Q^T has the tokens as M and
 // 32 head rows as N, the contraction split over the 4 / MT waves of a block (summed through LDS); the
 // online softmax runs in each lane's 16 scores of its head row plus one exchange between lane halves,
 // and its result is already the B operand of O^T += V^T P^T, whose columns the block's waves share.
+// With 32 head rows the bytes are the bound: each wave takes every fourth tile by itself, with a tile's
+// buffer and a softmax of its own and no barrier, and the four outputs are joined through LDS at the end.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -52,10 +54,17 @@ struct PfxK {
   uint16_t* out;
   float* sm_max;
   float* sm_sum;
-  float* part_o;    // [slots][rows * n1][D]
+  // Partial outputs of 32 head rows x D values each, a block: as the MFMAs leave them, so that every store
+  // and load is 1 KB in a row (row-major ones, 32 rows x 32 bytes an instruction, took 9.6 us a
+  // work-group of 256 KB). Prefix range s holds block s * p_blocks + h / 32; own range s block s * o_blocks +
+  // (row_start[b] * n1) / 32 + b + (h - row_start[b] * n1) / 32.
+  float4* p_part;
+  float4* o_part;
   float4* part_s;   // [rows * n1][slots]: reference maximum, true maximum, sum
-  int p_mt, p_tiles, p_splits, p_chunk, p_items;   // prefix items
+  int p_blocks, o_blocks, n1_shift;
+  int p_mt, p_tiles, p_splits, p_chunk;            // prefix items
   int o_mt, o_tiles, o_splits, o_chunk, o_base;    // own items (o_base: first token, 0 joined)
+  int per_xcd, o_by_range;                         // work-groups per XCD; own items of a range on one XCD
   int slots;
 };
 
@@ -66,6 +75,16 @@ __device__ const uint4 g_zero_row[(512 + 8) * 2 / 16] = {};
 __device__ __forceinline__ void lds_dma4_untracked(const void* gptr, void* lds_base) {
   const uint32_t m0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds_base;
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(gptr), "s"(m0) : "memory", "m0");
+}
+
+// 16-byte direct-to-LDS load as lds_dma16_sbase_untracked, to LDS address lds + OFF: the sum goes into M0
+// in one instruction (a wave here has its SIMD to itself, so each one it saves shortens the tile)
+template <int OFF>
+__device__ __forceinline__ void lds_dma16_at(uint64_t sbase, uint32_t voff, uint32_t lds) {
+  asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(voff), "s"(sbase), "s"(lds), "n"(OFF)
+               : "memory", "m0", "scc");
 }
 
 // e^TAU is the largest P relative to the reference maximum: finite in the io type (bf16 has fp32's
@@ -106,36 +125,71 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 template <int D> struct PfxLds {
-  uint8_t nope[NBUF][Tile<D>::NOPE];
-  uint8_t rope[NBUF][Tile<D>::ROPE];
   union {
-    uint16_t qr[128 * (DR + 8)];      // MT = 4: the query's rotary part
-    float x[NWV][16 * 64];            // MT < 4: partial scores
+    struct {                              // 64 or 128 head rows: a ring of tiles for the work-group
+      uint8_t nope[NBUF][Tile<D>::NOPE];
+      uint8_t rope[NBUF][Tile<D>::ROPE];
+      union {
+        uint16_t qr[128 * (DR + 8)];      // MT = 4: the query's rotary part
+        float x[NWV][16 * 64];            // MT = 2: partial scores
+      };
+    };
+    struct {                              // 32 head rows: a tile for each wave
+      uint8_t own_nope[NWV][BN * D * 2];
+      uint8_t own_rope[NWV][BN * DR * 2];
+    };
+    float4 join[NWV][16][64];             // the waves' outputs, 128 columns at a time
   };
   int32_t ids[4][BN];
   int red[2][NWV];
-  uint32_t bad[2][NWV];               // tokens of the tile (bit) with values that are not finite
+  uint32_t bad[2][NWV];                   // tokens of the tile (bit) with values that are not finite
+  float4 stat[NWV][32];                   // 32 head rows: the waves' maxima and sums
 };
 
 // limit(h): how many tokens of its sequence head row h's query sees
-__device__ __forceinline__ int row_limit(const PfxK& a, int row, int b) {
-  const int s1 = row - a.row_start[b], aq = a.act_q[b], ak = a.act_k[b];
-  if (s1 >= aq || row >= a.row_start[b + 1]) return 0;
-  const int64_t thr = a.mode == 0 ? (int64_t)ak : (int64_t)ak - aq + s1 + 1;
+struct Seq {
+  int r0, r1, aq, ak;
+};
+__device__ __forceinline__ Seq seq_of(const PfxK& a, int b) { return {a.row_start[b], a.row_start[b + 1], a.act_q[b], a.act_k[b]}; }
+__device__ __forceinline__ int row_limit(const PfxK& a, int row, const Seq& q) {
+  const int s1 = row - q.r0;
+  if (s1 < 0 || s1 >= q.aq || row >= q.r1) return 0;
+  const int64_t thr = a.mode == 0 ? (int64_t)q.ak : (int64_t)q.ak - q.aq + s1 + 1;
   return (int)(thr < 0 ? 0 : thr > a.s2 ? a.s2 : thr);
 }
-__device__ __forceinline__ int batch_of(const PfxK& a, int r) {
-  const int g = min(r / a.guess_rows, a.batch - 1);
-  if (a.row_start[g] <= r && r < a.row_start[g + 1]) return g;
-  return batch_of_row(a.row_start, a.batch, r);
+// Sequence of a packed row: that of evenly split ones (all its values in one round of loads), a search
+// where the guess is wrong
+__device__ __forceinline__ int batch_guess(const PfxK& a, int row) { return min(row / a.guess_rows, a.batch - 1); }
+__device__ __forceinline__ void batch_fix(const PfxK& a, int row, int& b, Seq& q) {
+  if (q.r0 <= row && row < q.r1) return;
+  b = batch_of_row(a.row_start, a.batch, row);
+  q = seq_of(a, b);
 }
 
 struct Item {
   int h0, h_end;   // head rows [h0, min(h0 + 32 MT, h_end))
   int b;           // own items: the sequence; -1: prefix
+  Seq seq;         // own items
   int t_lo, t_hi;  // tokens, before the rows' limits
   int slot;
+  float4* part;    // the item's first block
 };
+
+// Copies head rows [h, h + 32) (rows past the last repeat it) to LDS, whole rows an instruction; chunk c of
+// row r goes to c ^ (r % 16), so that a fragment read (16 rows, one chunk) touches every bank once.
+template <int D>
+__device__ __forceinline__ void stage_q(const uint16_t* q, int64_t h, int rows, uint8_t* dst, int lane) {
+  constexpr int LPR = D / 8, RPI = 64 / LPR;   // lanes a row, rows an instruction
+#pragma unroll
+  for (int j = 0; j < 32 / RPI; ++j) {
+    const int r = j * RPI + lane / LPR;
+    lds_dma16_untracked(q + (h + min(r, rows - 1)) * D + ((lane % LPR) ^ (r & 15)) * 8, dst + j * 1024);
+  }
+}
+template <int D>
+__device__ __forceinline__ uint4 staged_q(const uint8_t* src, int ks, int rr, int kg) {
+  return *reinterpret_cast<const uint4*>(src + rr * (D * 2) + (((2 * ks + kg) ^ (rr & 15)) << 4));
+}
 
 template <int IO, int D, int MT>
 __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D>& L) {
@@ -152,35 +206,35 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   const int kg = lane >> 5, rr = lane & 31;
   const int h = it.h0 + rb * 32 + rr;
   const bool valid = h < it.h_end;
-  const int m_rows = a.rows * a.n1;
   // the softmax works on raw scores times a positive factor: a negative scale negates the query, a
   // zero one becomes 1e-30 (scores round to 0, masked ones stay -inf)
   const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
   const float cpos = a.scale > 0.f ? a.scale : a.scale < 0.f ? -a.scale : 1e-30f;
   const float cl2 = cpos * LOG2E;
 
-  // ---- Q^T fragments (B operand: this lane's head row, 8 values at 16 ks + 8 kg)
+  // ---- this head row's sequence, requested first; then Q^T fragments (B operand: this lane's head row, 8
+  // values at 16 ks + 8 kg), through LDS
+  const int row = (valid ? h : it.h_end - 1) >> a.n1_shift;
+  int b = it.b >= 0 ? it.b : batch_guess(a, row);
+  Seq seq = it.b >= 0 ? it.seq : seq_of(a, b);
+  asm volatile("" ::: "memory");
   uint4 qf[QF];
+  uint8_t* const qs = L.own_nope[wave];
+  const int hb = it.h0 + rb * 32;
+  if (hb < it.h_end) stage_q<D>(a.q, hb, min(32, it.h_end - hb), qs, lane);
+  auto flipped = [&](uint4 v) { return make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip); };
+  constexpr int NQR = QLDS ? 4 : KSH - KNH;
+  uint4 qrv[NQR];
   {
-    const int hc = valid ? h : it.h_end - 1;
-    const uint16_t* qn = a.q + (int64_t)hc * D + kh * 16 + kg * 8;
-    const uint16_t* qr = a.qr + (int64_t)hc * DR + kh * 16 + kg * 8;
-    auto flipped = [&](uint4 v) { return make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip); };
+    const uint16_t* qr = a.qr + (int64_t)(valid ? h : it.h_end - 1) * DR + (QLDS ? 0 : kh * 16) + kg * 8;
 #pragma unroll
-    for (int j = 0; j < QF; ++j) qf[j] = flipped(ldg16(j < KNH ? qn + j * KSPL * 16 : qr + (j - KNH) * KSPL * 16));
-    if constexpr (QLDS)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<uint4*>(L.qr + (rb * 32 + rr) * (DR + 8) + j * 16 + kg * 8) = flipped(ldg16(qr + j * 16));
+    for (int j = 0; j < NQR; ++j) qrv[j] = ldg16(qr + j * (QLDS ? 1 : KSPL) * 16);
   }
 
   // ---- this head row's tokens: a row that sees none of the item's is dead: it runs along unmasked
   // and leaves a sum of 0
-  int lim = 0;
-  if (valid) {
-    const int row = h / a.n1;
-    lim = row_limit(a, row, it.b >= 0 ? it.b : batch_of(a, row));
-  }
+  if (it.b < 0) batch_fix(a, row, b, seq);
+  int lim = valid ? row_limit(a, row, seq) : 0;
   const bool dead = lim <= it.t_lo;
   lim = dead ? INT_MAX : min(lim, it.t_hi);   // within the item
   int hi, min_lim;
@@ -195,7 +249,15 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
       L.red[0][wave] = mx;
       L.red[1][wave] = mn;
     }
-    __syncthreads();   // (and the rotary part of Q)
+    wait_vmcnt<0>();   // Q
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < QF; ++j) qf[j] = j < KNH ? flipped(staged_q<D>(qs, j * KSPL + kh, rr, kg)) : flipped(qrv[j - KNH < NQR ? j - KNH : 0]);
+    __syncthreads();   // every wave has its Q: the staging area becomes the ring
+    if constexpr (QLDS)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<uint4*>(L.qr + (rb * 32 + rr) * (DR + 8) + j * 16 + kg * 8) = flipped(qrv[j]);
     mx = max(max(L.red[0][0], L.red[0][1]), max(L.red[0][2], L.red[0][3]));
     mn = min(min(L.red[1][0], L.red[1][1]), min(L.red[1][2], L.red[1][3]));
     hi = __builtin_amdgcn_readfirstlane(mx);        // end of the item's tokens
@@ -227,27 +289,35 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
     const int32_t* src = a.table + (t < a.prefix || it.b < 0 ? 0 : (int64_t)it.b * a.max_blocks) + page_of(t);
     if (lane < 8) lds_dma4_untracked(src, &L.ids[u & 3][wave * 8]);
   };
-  // cache row of token 8 w + lane % 8 of tile u, -1: its block is missing
-  auto tile_rows = [&](int u) __attribute__((always_inline)) {
+  // where the latent and the rotary part of token 8 w + lane % 8 of tile u lie (a missing block: zeros)
+  struct Source {
+    uint32_t lo, hi;
+    const uint16_t* rope;
+  };
+  auto tile_rows = [&](int u) __attribute__((always_inline)) -> Source {
     const int t = token(u);
     const int32_t id = L.ids[u & 3][wave * 8 + (lane & 7)];
-    return (uint32_t)id < a.blocks ? id * a.page + (t - page_of(t) * a.page) : -1;
+    const bool ok = (uint32_t)id < a.blocks;
+    const int row = id * a.page + (t - page_of(t) * a.page);
+    const uint16_t* zero = reinterpret_cast<const uint16_t*>(g_zero_row);
+    const uint64_t p = (uint64_t)(ok ? a.k + (int64_t)row * D : zero);
+    return {(uint32_t)p, (uint32_t)(p >> 32), (ok ? a.kr + (int64_t)row * DR : zero) + (lane >> 3) * 8};
   };
   // one of the GPW - 1 gathers of a tile: the latent of token 8 w + j, or (j = 8) the wave's rotary
-  // parts. The empty asm keeps the address arithmetic here, among the MFMAs it is issued with.
-  auto gather_part = [&](int j, int row, uint8_t* nope, uint8_t* rope) __attribute__((always_inline)) {
-    if (j < 8) {
-      int r = __builtin_amdgcn_readlane(row, j);
-      asm volatile("" : "+s"(r));
-      const uint16_t* src = r >= 0 ? a.k + (int64_t)r * D : reinterpret_cast<const uint16_t*>(g_zero_row);
-      if (lane < D / 8) lds_dma16_sbase_untracked(src, lane * 16, nope + nope_off<D>(wave * 8 + j));
+  // parts, to the LDS addresses nope and rope (of the tile's buffer, this wave's rows)
+  auto gather_part = [&](auto jc, const Source& src, uint32_t nope, uint32_t rope) __attribute__((always_inline)) {
+    constexpr int j = decltype(jc)::value;
+    if constexpr (j < 8) {
+      const uint64_t p = (uint32_t)__builtin_amdgcn_readlane(src.lo, j) |
+                         (uint64_t)(uint32_t)__builtin_amdgcn_readlane(src.hi, j) << 32;
+      if (lane < D / 8) lds_dma16_at<nope_off<D>(j)>(p, lane * 16, nope);
     } else {
-      int r = row;
-      asm volatile("" : "+v"(r));
-      const uint16_t* src = r >= 0 ? a.kr + (int64_t)r * DR : reinterpret_cast<const uint16_t*>(g_zero_row);
-      lds_dma16_untracked(src + (lane >> 3) * 8, rope + wave * 1024);
+      lds_dma16_untracked(src.rope, (void*)(__attribute__((address_space(3))) void*)(uintptr_t)rope);
     }
   };
+  // LDS addresses of this wave's rows in buffer b (8 w has token bits 0 and 1 clear)
+  auto nope_at = [&](int b) { return (uint32_t)__builtin_amdgcn_readfirstlane(lds_addr(L.nope[b]) + nope_off<D>(wave * 8)); };
+  auto rope_at = [&](int b) { return (uint32_t)__builtin_amdgcn_readfirstlane(lds_addr(L.rope[b]) + wave * 1024); };
   // A tile that some of the head rows see only in part: a masked token has P = 0, but 0 times a value
   // that is not finite would still reach the rows that do not see it. Such values become 0 in LDS, and
   // the token's score NaN for the rows that do see it. (Each wave its own rows, landed by now.)
@@ -277,9 +347,9 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   asm volatile("" ::: "memory");
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const int row = tile_rows(u);
-#pragma unroll
-    for (int j = 0; j < 9; ++j) gather_part(j, row, L.nope[u], L.rope[u]);
+    const Source src = tile_rows(u);
+    const uint32_t gnope = nope_at(u), grope = rope_at(u);
+    static_for<0, C::GPW - 1>([&](auto j) { gather_part(j, src, gnope, grope); });
   }
 
   {   // an AGPR operand makes the compiler keep the MFMA accumulators there, the VGPRs free for operands
@@ -470,20 +540,18 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
     else wait_vmcnt<1>();
     if (is_mixed(t + 1)) sanitize(t + 1);
     lds_barrier();   // tile t + 1 resident; every wave done with tile t - 1, whose buffer is free
-    const int row = tile_rows(t + 2);
-    const int gb = __builtin_amdgcn_readfirstlane((t + 2) % NBUF);   // the free buffer
-    uint8_t* const gnope = L.nope[gb];
-    uint8_t* const grope = L.rope[gb];
+    const Source src = tile_rows(t + 2);
+    const uint32_t gnope = nope_at((t + 2) % NBUF), grope = rope_at((t + 2) % NBUF);   // the free buffer
     const uint32_t vbase = v_base(t), vnext = v_base(t + 1);
     f32x16 s1 = s_tile(
         t + 1,
         [&](int ks) __attribute__((always_inline)) {
-#pragma unroll
-          for (int j = 0; j < C::GPW; ++j)
+          static_for<0, C::GPW>([&](auto j) __attribute__((always_inline)) {
             if (j * KSH / C::GPW == ks) {
-              if (j < C::GPW - 1) gather_part(j, row, gnope, grope);
+              if constexpr (j < C::GPW - 1) gather_part(j, src, gnope, grope);
               else ids_dma(t + 4);   // the slot of tile t's ids, read two iterations ago
             }
+          });
         },
         [&]() __attribute__((always_inline)) { pv_run(0, NPRE, vbase, vnext, true, [](int) {}); });
     if constexpr (KSPL > 1) {
@@ -519,13 +587,12 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   }
   if (!direct) {
     if (!valid || dead) return;
-    float* dst = a.part_o + ((int64_t)it.slot * m_rows + h) * D + kh * (D / KSPL) + 4 * kg;
+    float4* dst = it.part + ((int64_t)rb * (D / 8) + kh * (ON * 4)) * 64 + lane;
 #pragma unroll
     for (int n = 0; n < ON; ++n)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<float4*>(dst + n * 32 + 8 * g) =
-            make_float4(o[n][4 * g], o[n][4 * g + 1], o[n][4 * g + 2], o[n][4 * g + 3]);
+        dst[(n * 4 + g) * 64] = make_float4(o[n][4 * g], o[n][4 * g + 1], o[n][4 * g + 2], o[n][4 * g + 3]);
     return;
   }
   // two exchanges between lane halves leave lanes 0-31 with columns [0, 8) and [16, 24) of a 32-column
@@ -552,31 +619,320 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   }
 }
 
+// 32 head rows: the waves split the tokens. A wave's tile is loaded, then used, so its own loads and
+// products do not overlap; the four waves' do, with up to four tiles (147 KB at D = 512) under way on a
+// CU, which a ring shared by the waves (one tile ahead of two barriers a tile) did not reach.
+template <int IO, int D>
+__device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds<D>& L) {
+  constexpr int KSN = D / 16, KS = (D + DR) / 16, ON = D / 32, ROW = D * 2;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kg = lane >> 5, rr = lane & 31;
+  const int h = it.h0 + rr;
+  const bool valid = h < it.h_end;
+  const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;   // scale: see run_item
+  const float cpos = a.scale > 0.f ? a.scale : a.scale < 0.f ? -a.scale : 1e-30f;
+  const float cl2 = cpos * LOG2E;
+
+  const int row = (valid ? h : it.h_end - 1) >> a.n1_shift;
+  int b = it.b >= 0 ? it.b : batch_guess(a, row);
+  Seq seq = it.b >= 0 ? it.seq : seq_of(a, b);
+  asm volatile("" ::: "memory");
+  uint8_t* const nope = L.own_nope[wave];
+  uint8_t* const rope = L.own_rope[wave];
+  stage_q<D>(a.q, it.h0, min(32, it.h_end - it.h0), nope, lane);   // each wave for itself
+  uint4 qf[KS];
+  {
+    const uint16_t* qr = a.qr + (int64_t)(valid ? h : it.h_end - 1) * DR + kg * 8;
+#pragma unroll
+    for (int j = KSN; j < KS; ++j) qf[j] = ldg16(qr + (j - KSN) * 16);
+  }
+  if (it.b < 0) batch_fix(a, row, b, seq);
+  int lim = valid ? row_limit(a, row, seq) : 0;
+  const bool dead = lim <= it.t_lo;
+  lim = dead ? INT_MAX : min(lim, it.t_hi);
+  int hi, min_lim;
+  {
+    int mx = dead ? 0 : lim, mn = lim;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      mx = max(mx, __shfl_xor(mx, o));
+      mn = min(mn, __shfl_xor(mn, o));
+    }
+    hi = __builtin_amdgcn_readfirstlane(mx);
+    min_lim = __builtin_amdgcn_readfirstlane(mn);
+  }
+  const bool direct = a.slots == 1;
+  const bool writer = wave == 0 && lane < 32 && valid;
+  if (hi <= it.t_lo) {   // no row sees any token (every wave finds the same)
+    if (direct) {
+      for (int i = threadIdx.x; i < 32 * (D / 8); i += NWV * 64) {
+        const int hr = it.h0 + i / (D / 8);
+        if (hr < it.h_end) stg16(a.out + (int64_t)hr * D + (i % (D / 8)) * 8, make_uint4(0, 0, 0, 0));
+      }
+      if (writer && a.sm_max) a.sm_max[h] = a.sm_sum[h] = 0.f;
+    } else if (writer) {
+      a.part_s[(int64_t)h * a.slots + it.slot] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    return;
+  }
+  const int ntiles = (hi - it.t_lo + BN - 1) / BN;
+
+  auto page_of = [&](int t) { return (int)(((uint64_t)(uint32_t)t * a.page_mul) >> (31 + a.page_shift)); };
+  auto token = [&](int u) { return min(it.t_lo + u * BN + rr, hi - 1); };   // tokens past the end: the last one
+  auto block_id = [&](int u) {
+    const int t = token(min(u, ntiles - 1));
+    return a.table[(t < a.prefix || it.b < 0 ? 0 : (int64_t)it.b * a.max_blocks) + page_of(t)];
+  };
+  const uint32_t nope_lds = __builtin_amdgcn_readfirstlane(lds_addr(nope));
+
+  {
+    float agpr_hint = 0.f;
+    asm volatile("" : "+a"(agpr_hint));
+  }
+  f32x16 o[ON];
+#pragma unroll
+  for (int n = 0; n < ON; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
+  float m_used = -INFINITY, m_true = -INFINITY, l_part = 0.f;
+
+  // Rows are unpadded: 16-byte chunk c of token t lies at c ^ kv_swz(t), so both readers' addresses are
+  // a few fixed ones per lane plus constants. Operand read: chunk 2 ks + kg of token tk; transposed read:
+  // tokens t4 (and + 4), chunk 4 n + vc.
+  const int tk = 16 * (rr >> 4) + 8 * ((rr >> 2) & 1) + 4 * ((rr >> 3) & 1) + (rr & 3);
+  const int g16 = lane >> 4, c16 = lane & 15;
+  const int t4 = (g16 >> 1) * 8 + (c16 >> 2), vc = (g16 & 1) * 2 + ((c16 & 3) >> 1);
+  const uint32_t k_at = nope_lds + tk * ROW + ((kg ^ kv_swz(tk & 15)) << 4);
+  const uint32_t v_lo = nope_lds + t4 * ROW + ((vc ^ kv_swz(t4)) << 4) + (c16 & 1) * 8;
+  const uint32_t v_hi = nope_lds + (t4 + 4) * ROW + ((vc ^ kv_swz(t4 + 4)) << 4) + (c16 & 1) * 8;
+  auto k_frag = [&](int j) -> uint4 {
+    return j < KSN ? lds_read16_at((k_at ^ ((j & 7) << 5)) + (j >> 3) * 256)
+                   : *reinterpret_cast<const uint4*>(rope + rope_off(tk, (j - KSN) * 2 + kg));
+  };
+  auto v_frag = [&](int m) -> uint4 {
+    const int n = m % ON, off = (m / ON) * 16 * ROW + (n >> 2) * 256;
+    const uint2 lo = ds_read_tr_at((v_lo ^ ((n & 3) << 6)) + off), hi2 = ds_read_tr_at((v_hi ^ ((n & 3) << 6)) + off);
+    return make_uint4(lo.x, lo.y, hi2.x, hi2.y);
+  };
+
+  int32_t id = wave < ntiles ? block_id(wave) : 0;
+  wait_vmcnt<0>();   // Q
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < KS; ++j) {
+    if (j < KSN) qf[j] = staged_q<D>(nope, j, rr, kg);
+    qf[j] = make_uint4(qf[j].x ^ flip, qf[j].y ^ flip, qf[j].z ^ flip, qf[j].w ^ flip);
+  }
+  for (int uv = wave; uv < ntiles; uv += NWV) {
+    const int u = __builtin_amdgcn_readfirstlane(uv);
+    const int t0 = it.t_lo + u * BN;
+    // ---- the tile: lane l holds where token l % 32 lies
+    {
+      const int t = token(u);
+      const bool ok = (uint32_t)id < a.blocks;
+      const int row = id * a.page + (t - page_of(t) * a.page);
+      const uint16_t* zero = reinterpret_cast<const uint16_t*>(g_zero_row);
+      const uint64_t p = (uint64_t)(ok ? a.k + (int64_t)row * D : zero);
+      const uint64_t pr = (uint64_t)(ok ? a.kr + (int64_t)row * DR : zero);
+      const uint32_t plo = (uint32_t)p, phi = (uint32_t)(p >> 32), rlo = (uint32_t)pr, rhi = (uint32_t)(pr >> 32);
+      // the last tile's reads are done (its products waited for them) before this one overwrites it
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      static_for<0, BN>([&](auto jc) __attribute__((always_inline)) {
+        constexpr int j = decltype(jc)::value;
+        const uint64_t src = (uint32_t)__builtin_amdgcn_readlane(plo, j) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(phi, j) << 32;
+        if (lane < D / 8) lds_dma16_at<j * ROW>(src, (lane * 16) ^ (kv_swz(j & 15) << 4), nope_lds);
+      });
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {   // tokens 8 g + lane % 8, chunk lane / 8
+        const uint32_t lo = __shfl(rlo, 8 * g + (lane & 7)), hi2 = __shfl(rhi, 8 * g + (lane & 7));
+        lds_dma16_untracked((const uint16_t*)(lo | (uint64_t)hi2 << 32) + (lane >> 3) * 8, rope + g * 1024);
+      }
+    }
+    id = block_id(u + NWV);
+    wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    uint32_t bad = 0;
+    if (min_lim < hi && t0 + BN > min_lim) {   // see run_item: values that are not finite, masked for some rows
+#pragma unroll 1
+      for (int j = 0; j < BN; ++j) {
+        uint4* p = reinterpret_cast<uint4*>(nope + j * ROW + (lane % (D / 8)) * 16);
+        uint4 v = *p;
+        bool any = false;
+        constexpr uint32_t EXP = IO == IO_BF16 ? 0x7F80u : 0x7C00u;
+        auto clean = [&](uint32_t w) {
+          if ((w & EXP) == EXP) w &= 0xFFFF0000u, any = true;
+          if (((w >> 16) & EXP) == EXP) w &= 0xFFFFu, any = true;
+          return w;
+        };
+        v = make_uint4(clean(v.x), clean(v.y), clean(v.z), clean(v.w));
+        if (any && lane < D / 8) *p = v;
+        if (__builtin_amdgcn_ballot_w64(any)) bad |= 1u << j;
+      }
+    }
+    // ---- S^T
+    constexpr int KPF = 5;
+    uint4 af[KPF];
+#pragma unroll
+    for (int j = 0; j < KPF; ++j) af[j] = k_frag(j);
+    f32x16 sv;
+#pragma unroll
+    for (int j = 0; j < KS; ++j) {
+      if (j == 0) sv = mfma32_vacc_first<IO>(af[0], qf[0]);
+      else if (j < KS - 1) mfma32_vacc<IO>(sv, af[j % KPF], qf[j]);
+      else sv = mfma32_vacc_last_to<IO>(sv, af[j % KPF], qf[j]);
+      if (j + KPF < KS) af[j % KPF] = k_frag(j + KPF);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    constexpr int VR = 4;
+    uint4 vb[VR];
+#pragma unroll
+    for (int m = 0; m < VR; ++m) vb[m] = v_frag(m);
+    if (bad)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if ((bad >> (16 * (i >> 3) + 8 * kg + (i & 7))) & 1u) sv[i] = __builtin_nanf("");
+    if (t0 + BN > min_lim)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sv[i] = t0 + 16 * (i >> 3) + 8 * kg + (i & 7) < lim ? sv[i] : -INFINITY;
+    // ---- softmax; a row may see nothing of a wave's first tiles
+    float mx = max3(sv[0], sv[1], sv[2]);
+#pragma unroll
+    for (int i = 3; i < 15; i += 2) mx = max3(mx, sv[i], sv[i + 1]);
+    mx = max_half_swap(max3(mx, sv[15], sv[15])) * cpos;
+    m_true = max3(m_true, mx, mx);
+    const float m_new = mx > m_used + lazy_tau<IO>() ? mx : m_used;
+    const float alpha = m_used == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_used - m_new) * LOG2E);
+    m_used = m_new;
+    const float mb = m_used == -INFINITY ? 0.f : m_used * LOG2E;
+    uint32_t d[8];
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[2 * i], cl2, -mb));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[2 * i + 1], cl2, -mb));
+      sum += p0;
+      sum += p1;
+      d[i] = pack2<IO>(p0, p1);
+    }
+    l_part = l_part * alpha + sum;
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.f)) {
+#pragma unroll
+      for (int n = 0; n < ON; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[n][i] = agpr_scale(o[n][i], alpha);
+    }
+    const uint4 pb[2] = {make_uint4(d[0], d[1], d[2], d[3]), make_uint4(d[4], d[5], d[6], d[7])};
+#pragma unroll
+    for (int m = 0; m < 2 * ON; ++m) {
+      o[m % ON] = Mfma<IO>::m32(vb[m % VR], pb[m / ON], o[m % ON]);
+      if (m + VR < 2 * ON) vb[m % VR] = v_frag(m + VR);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  // ---- the waves' outputs joined: each scaled to the common maximum, 128 columns at a time, wave w
+  // adding the four parts of column tile 4 c + w
+  const float l_wave = add_half_swap(l_part);
+  if (lane < 32) L.stat[wave][rr] = make_float4(m_used, m_true, l_wave, 0.f);
+  __syncthreads();   // (also: every wave is done with its tile's buffer)
+  float M = -INFINITY, top = -INFINITY, l_tot = 0.f;
+#pragma unroll
+  for (int w = 0; w < NWV; ++w) {
+    const float4 st = L.stat[w][rr];
+    M = fmaxf(M, st.x);
+    top = fmaxf(top, st.y);
+  }
+#pragma unroll
+  for (int w = 0; w < NWV; ++w) {
+    const float4 st = L.stat[w][rr];
+    l_tot += st.x == -INFINITY ? st.z : st.z * __builtin_amdgcn_exp2f((st.x - M) * LOG2E);
+  }
+  const float f = m_used == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_used - M) * LOG2E);   // (O and l are 0 with -inf)
+  if (a.scale == 0.f) top *= 0.f;
+  if (writer) {
+    if (!direct) {
+      a.part_s[(int64_t)h * a.slots + it.slot] = make_float4(M, top, dead ? 0.f : l_tot, 0.f);
+    } else if (a.sm_max) {
+      a.sm_max[h] = dead ? 0.f : top;
+      a.sm_sum[h] = dead ? 0.f : l_tot * exp2f((M - top) * LOG2E);
+    }
+  }
+  const float inv = dead ? 0.f : 1.f / l_tot;
+#pragma unroll
+  for (int c = 0; c < ON / 4; ++c) {
+    if (c > 0) __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x16& v = o[4 * c + n];
+        L.join[wave][n * 4 + g][lane] = make_float4(v[4 * g] * f, v[4 * g + 1] * f, v[4 * g + 2] * f, v[4 * g + 3] * f);
+      }
+    __syncthreads();
+    float4 v[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      v[g] = L.join[0][wave * 4 + g][lane];
+#pragma unroll
+      for (int w = 1; w < NWV; ++w) {
+        const float4 p = L.join[w][wave * 4 + g][lane];
+        v[g].x += p.x;
+        v[g].y += p.y;
+        v[g].z += p.z;
+        v[g].w += p.w;
+      }
+    }
+    if (!valid) continue;
+    const int n = 4 * c + wave;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      if (direct)
+        *reinterpret_cast<uint2*>(a.out + (int64_t)h * D + n * 32 + 8 * g + 4 * kg) =
+            dead ? make_uint2(0, 0) : make_uint2(pack2<IO>(v[g].x * inv, v[g].y * inv), pack2<IO>(v[g].z * inv, v[g].w * inv));
+      else if (!dead)
+        it.part[(n * 4 + g) * 64 + lane] = v[g];
+    }
+  }
+}
+
 template <int IO, int D>
 __global__ __launch_bounds__(NWV * 64) void prefix_attn_kernel(PfxK a) {
   __shared__ __attribute__((aligned(16))) PfxLds<D> L;
   Item it;
-  int i = blockIdx.x;
   int mt;
-  if (i < a.p_items) {
-    const int sp = i / a.p_tiles, tile = i - sp * a.p_tiles;
+  // Work-groups go round the eight XCDs, each with an L2 of its own: XCD x takes the prefix ranges x, x + 8, ..
+  // for all tiles (so their latents come from HBM once), then own items up to an even count: dense
+  // indexes row by row where XCDs are free, or (joined, at least eight ranges) a run of ranges per XCD.
+  const int x = blockIdx.x & 7, j = blockIdx.x >> 3;
+  const int rem = a.p_splits & 7, lo = a.p_splits / 8 * a.p_tiles, hi = lo + (rem ? a.p_tiles : 0);
+  if (j < (x < rem ? hi : lo)) {
+    const int sp = x + 8 * (j / a.p_tiles), tile = j % a.p_tiles;
     mt = a.p_mt;
     it.h0 = tile * 32 * mt;
     it.h_end = a.rows * a.n1;
     it.b = -1;
+    it.seq = {0, 0, 0, 0};
     it.t_lo = sp * a.p_chunk;
     it.t_hi = sp == a.p_splits - 1 ? a.prefix : min(a.prefix, it.t_lo + a.p_chunk);
     it.slot = sp;
+    it.part = a.p_part + ((int64_t)sp * a.p_blocks + tile * mt) * (D / 8) * 64;
   } else {
-    i -= a.p_items;
-    const int per = a.o_tiles * a.o_splits;
-    const int b = i / per;
-    i -= b * per;
-    const int sp = i / a.o_tiles, tile = a.o_tiles - 1 - (i - sp * a.o_tiles);
+    int i = a.o_by_range ? x * a.per_xcd + j : j < hi ? (j - lo) * (8 - rem) + (x - rem) : (hi - lo) * (8 - rem) + (j - hi) * 8 + x;
+    const int per = a.batch * a.o_tiles;   // items of a range
+    const int sp = i / per;
+    if (sp >= a.o_splits) return;
+    i -= sp * per;
+    const int b = i / a.o_tiles, tile = a.o_tiles - 1 - (i - b * a.o_tiles);   // (causal: the longest first)
     mt = a.o_mt;
-    const int r0 = a.row_start[b], r1 = a.row_start[b + 1];
-    it.h0 = r0 * a.n1 + tile * 32 * mt;
-    it.h_end = r1 * a.n1;
+    it.seq = seq_of(a, b);
+    const int first = it.seq.r0 * a.n1;
+    it.h0 = first + tile * 32 * mt;
+    it.h_end = it.seq.r1 * a.n1;
+    it.b = b;
+    it.t_lo = a.o_base + sp * a.o_chunk;
+    it.t_hi = sp == a.o_splits - 1 ? INT_MAX : it.t_lo + a.o_chunk;
+    it.slot = a.p_splits + sp;
+    it.part = a.o_part + ((int64_t)sp * a.o_blocks + first / 32 + b + tile * mt) * (D / 8) * 64;
     if (a.slots == 1 && b == a.batch - 1) {   // rows behind the last sequence: zeros
       const int64_t end = (int64_t)a.rows * a.n1 * (D / 8);
       for (int64_t j = (int64_t)it.h_end * (D / 8) + tile * (NWV * 64) + threadIdx.x; j < end; j += a.o_tiles * (NWV * 64)) {
@@ -590,61 +946,115 @@ __global__ __launch_bounds__(NWV * 64) void prefix_attn_kernel(PfxK a) {
     it.t_hi = sp == a.o_splits - 1 ? INT_MAX : it.t_lo + a.o_chunk;
     it.slot = a.p_splits + sp;
   }
-  if (mt == 1) run_item<IO, D, 1>(a, it, L);
+  if (mt == 1) run_tokens<IO, D>(a, it, L);
   else if (mt == 2) run_item<IO, D, 2>(a, it, L);
   else run_item<IO, D, 4>(a, it, L);
 }
 
-// Joins the ranges of a head row: M = max m_s, out = sum O_s 2^(m_s - M) / sum l_s 2^(m_s - M), and the
-// rows of no sequence get zeros. 64 lanes hold the row's statistics (a slot each, in turns), D / 4
-// threads its columns.
-template <int IO, int D>
-__global__ __launch_bounds__(256) void prefix_merge_kernel(PfxK a) {
-  constexpr int TPR = D / 4;           // threads a row: 128, 64, 32
-  const int m_rows = a.rows * a.n1;
-  const int h = blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
-  const int c = (threadIdx.x % TPR) * 4;
-  if (h >= m_rows) return;
-  const int row = h / a.n1;
-  const bool live = row_limit(a, row, batch_of(a, row)) > 0;
-  const float4* ps = a.part_s + (int64_t)h * a.slots;
-  float M = -INFINITY, mt = -INFINITY, l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (live) {
-    for (int s = 0; s < a.slots; ++s) {
-      const float4 st = ps[s];
-      if (st.z != 0.f) {   // (NaN sums take part)
-        M = fmaxf(M, st.x);
-        mt = fmaxf(mt, st.y);
-      }
-    }
-    for (int s = 0; s < a.slots; ++s) {
-      const float4 st = ps[s];
-      if (st.z == 0.f) continue;
-      const float w = exp2f((st.x - M) * LOG2E);
-      const float4 v = *reinterpret_cast<const float4*>(a.part_o + ((int64_t)s * m_rows + h) * D + c);
-      l += st.z * w;
-      acc.x += v.x * w;
-      acc.y += v.y * w;
-      acc.z += v.z * w;
-      acc.w += v.w * w;
-    }
-    const float inv = 1.f / l;
-    acc.x *= inv;
-    acc.y *= inv;
-    acc.z *= inv;
-    acc.w *= inv;
-  }
-  *reinterpret_cast<uint2*>(a.out + (int64_t)h * D + c) = make_uint2(pack2<IO>(acc.x, acc.y), pack2<IO>(acc.z, acc.w));
-  if (c == 0 && a.sm_max) {
-    a.sm_max[h] = live ? mt : 0.f;
-    a.sm_sum[h] = live ? l * exp2f((M - mt) * LOG2E) : 0.f;
-  }
-}
-
 constexpr int MAX_SLOTS = 256;
 
-// How a call is cut. Counts are host-known bounds; the kernel's ranges are right for any lengths.
+// Joins the ranges of 32 head rows: M = max m_s, out = sum O_s 2^(m_s - M) / sum l_s 2^(m_s - M); rows that
+// see nothing get zeros. Bound by the partials' bytes where there are many rows, by latency where there
+// are few, so the loads of UN ranges are under way at once and, with few rows and many ranges, SG waves
+// take every SG-th one. A wave's lanes are the 32 rows and two column groups of one of the D / 8 groups of
+// 8 columns: 1 KB of a block. A range that a row saw nothing of has weight 0 and is not read.
+template <int IO, int D, int SG>
+__global__ __launch_bounds__(SG > 1 ? SG * 64 : 256) void prefix_merge_kernel(PfxK a) {
+  constexpr int TPB = SG > 1 ? SG * 64 : 256;
+  constexpr int LPR = TPB / 32;   // threads a row for the statistics
+  constexpr int UN = 8;
+  __shared__ float s_w[MAX_SLOTS][32];
+  __shared__ float s_inv[32];
+  __shared__ int64_t s_own[32];   // where the row's own blocks begin
+  __shared__ float4 s_acc[SG > 1 ? SG : 1][64];
+  const int m_rows = a.rows * a.n1;
+  const int h0 = blockIdx.x * 32;
+  {
+    const int r = threadIdx.x / LPR, j = threadIdx.x % LPR;
+    const int h = min(h0 + r, m_rows - 1);
+    const int row = h >> a.n1_shift;
+    int b = batch_guess(a, row);
+    Seq seq = seq_of(a, b);
+    const float4* ps = a.part_s + (int64_t)h * a.slots;
+    float M = -INFINITY, top = -INFINITY, sum = 0.f;
+    batch_fix(a, row, b, seq);
+    const bool live = row_limit(a, row, seq) > 0;
+    for (int s = j; s < a.slots; s += LPR) {
+      const float4 st = live ? ps[s] : make_float4(0.f, 0.f, 0.f, 0.f);
+      if (st.z != 0.f) {   // (NaN sums take part)
+        M = fmaxf(M, st.x);
+        top = fmaxf(top, st.y);
+      }
+    }
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) {
+      M = fmaxf(M, __shfl_xor(M, o));
+      top = fmaxf(top, __shfl_xor(top, o));
+    }
+    for (int s = j; s < a.slots; s += LPR) {
+      const float4 st = live ? ps[s] : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float w = st.z != 0.f ? exp2f((st.x - M) * LOG2E) : 0.f;
+      s_w[s][r] = w;
+      if (w != 0.f) sum += w * st.z;
+    }
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    if (j == 0) {
+      s_inv[r] = live ? 1.f / sum : 0.f;
+      const int own = h - seq.r0 * a.n1;   // (a row of no sequence reads nothing)
+      s_own[r] = ((int64_t)(seq.r0 * a.n1 / 32 + b + own / 32) * (D / 8)) * 64 + own % 32;
+      if (blockIdx.y == 0 && a.sm_max && h0 + r < m_rows) {
+        a.sm_max[h] = live ? top : 0.f;
+        a.sm_sum[h] = live ? sum * exp2f((M - top) * LOG2E) : 0.f;
+      }
+    }
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int rr = lane & 31, kg = lane >> 5;
+  const int grp = SG > 1 ? blockIdx.y : blockIdx.y * 4 + wave;   // group of 8 columns
+  const int sg = SG > 1 ? wave : 0;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float4* pp = a.p_part + ((int64_t)blockIdx.x * (D / 8) + grp) * 64 + lane;
+  const float4* op = a.o_part + s_own[rr] + grp * 64 + kg * 32;
+  const int64_t p_step = (int64_t)a.p_blocks * (D / 8) * 64, o_step = (int64_t)a.o_blocks * (D / 8) * 64;
+  for (int s0 = sg; s0 < a.slots; s0 += SG * UN) {
+    float w[UN];
+    uint4 v[UN];
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      const int s = s0 + i * SG;
+      w[i] = s < a.slots ? s_w[s][rr] : 0.f;
+      v[i] = ldg16_or0(w[i] != 0.f, s < a.p_splits ? pp + s * p_step : op + (s - a.p_splits) * o_step);
+    }
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      acc.x += w[i] * __uint_as_float(v[i].x);
+      acc.y += w[i] * __uint_as_float(v[i].y);
+      acc.z += w[i] * __uint_as_float(v[i].z);
+      acc.w += w[i] * __uint_as_float(v[i].w);
+    }
+  }
+  if constexpr (SG > 1) {
+    s_acc[sg][lane] = acc;
+    __syncthreads();
+    if (sg != 0) return;
+#pragma unroll
+    for (int g = 1; g < SG; ++g) {
+      const float4 v = s_acc[g][lane];
+      acc.x += v.x;
+      acc.y += v.y;
+      acc.z += v.z;
+      acc.w += v.w;
+    }
+  }
+  if (h0 + rr >= m_rows) return;
+  const float inv = s_inv[rr];
+  *reinterpret_cast<uint2*>(a.out + (int64_t)(h0 + rr) * D + grp * 8 + kg * 4) =
+      make_uint2(pack2<IO>(acc.x * inv, acc.y * inv), pack2<IO>(acc.z * inv, acc.w * inv));
+}
+
+// How a call is cut. Lengths are what the caller expects; the kernels' ranges are right for any.
 struct Cut {
   int p_mt, p_tiles, p_splits, p_chunk;
   int o_mt, o_tiles, o_splits, o_chunk, o_base;
@@ -654,64 +1064,92 @@ struct Cut {
 int mt_for(int64_t head_rows) { return head_rows > 64 ? 4 : head_rows > 32 ? 2 : 1; }
 int up(int x, int to) { return (x + to - 1) / to * to; }
 
-Cut make_cut(int batch, int rows, int n1, int prefix, int max_rows, int max_kv, int kv_splits) {
-  Cut c{};
+// Microseconds of a call by a simple model of what was measured at D = 512 (256 CUs, one item each at a
+// time): an item costs 6 (its rows' sequences, Q, first tile, ends) and 1.55 / 1.3 per 32 tokens for 128 / 64
+// head rows or 3.7 per 128 tokens for 32; partial outputs are written at 7 TB/s, and the join is a launch of
+// 6 that reads them at 6 TB/s. It is there to weigh rounds of items against partials: at 64 x 16 heads
+// after 8192 tokens 16 prefix ranges take 50 us, 8 take 70 and 32 take 70 as well.
+struct Model {
+  double scale;   // of a tile's products against D = 512
+  double item(int mt, int tokens) const {
+    return 6.0 + scale * (mt == 4 ? 1.55 * ((tokens + 31) / 32) : mt == 2 ? 1.3 * ((tokens + 31) / 32) : 3.7 * ((tokens + 127) / 128));
+  }
+};
+
+double cut_cost(const Model& md, const Cut& c, int d, double own_tiles, int own_max, double own_mean) {
+  const double np = (double)c.p_splits * c.p_tiles;
+  const double tp = c.p_splits ? md.item(c.p_mt, c.p_chunk) : 0.0;
+  const double no = own_tiles * std::min((double)c.o_splits, own_mean / c.o_chunk + (c.o_splits > 1 ? 0.5 : 1.0));
+  const double to = own_max > 0 ? md.item(c.o_mt, std::min(c.o_chunk, own_max)) : 3.0;
+  // items past the CUs wait for whole ones, also where others end at once (17 prefix ranges instead of 16
+  // in the example, 272 work-groups: 52 -> 64 us): half an item at least
+  const double n = np + no, grid = np + own_tiles * c.o_splits, longest = std::max(tp, to);
+  const double mean = (np * tp + no * to) / std::max(n, 1.0);
+  double us = longest + (grid > 256.0 ? mean * std::max(std::max(n, 256.0) / 256.0 - 1.0, 0.45) : 0.0);
+  if (c.slots > 1) {
+    const double mb = (np * c.p_mt + no * c.o_mt) * 32.0 * d * 4.0 * 1e-6;
+    us += mb / 7.0 + 6.0 + mb / 6.0;
+  }
+  return us;
+}
+
+// total_kv: the sum of the lengths
+Cut make_cut(int batch, int rows, int n1, int d, int prefix, int max_rows, int max_kv, int64_t total_kv, int kv_splits) {
   const int64_t m = (int64_t)rows * n1;
-  const int own = max_kv > prefix ? max_kv - prefix : 0;
+  const double mean = (double)total_kv / batch;
+  const Model md{(2 * d + 64) / 1088.0};
+  Cut c{}, best{};
+  double least = 1e300;
   c.o_mt = mt_for((int64_t)max_rows * n1);
   c.o_tiles = (int)(((int64_t)max_rows * n1 + 32 * c.o_mt - 1) / (32 * c.o_mt));
-  const int64_t o_all = std::min<int64_t>((int64_t)batch * c.o_tiles, m / (32 * c.o_mt) + batch);
+  c.o_tiles = std::max(c.o_tiles, 1);
+  const double own_tiles = (double)std::min<int64_t>((int64_t)batch * c.o_tiles, m / (32 * c.o_mt) + batch);
+  auto consider = [&](int own_max, double own_mean, int o_splits) {
+    c.o_splits = std::min(std::max(o_splits, 1), std::max(1, MAX_SLOTS - c.p_splits));
+    c.o_chunk = up(std::max((own_max + c.o_splits - 1) / c.o_splits, 1), c.o_mt == 1 ? 4 * BN : BN);
+    c.o_splits = std::max(1, (own_max + c.o_chunk - 1) / c.o_chunk);
+    c.slots = c.p_splits + c.o_splits;
+    const double us = cut_cost(md, c, d, own_tiles, own_max, own_mean);
+    if (us < least) least = us, best = c;
+  };
+  auto more = [](int s) { return s < 24 ? 1 : s < 48 ? 4 : 8; };
+  // joined: each tile over the prefix and its own tokens
   c.p_mt = mt_for(m);
-  c.p_tiles = (int)((m + 32 * c.p_mt - 1) / (32 * c.p_mt));
-  const bool joined = prefix == 0 || o_all * c.o_mt * 8 <= (int64_t)c.p_tiles * c.p_mt * 9;
-  constexpr int CUS = 256;
-  if (joined) {
-    c.p_tiles = 0;
-    c.o_base = 0;
-    const int64_t tiles = std::max<int64_t>(o_all, 1);
-    const int all = std::max(max_kv, 1);
-    int best = 1;
-    double least = 1e30;
-    for (int s = 1; s <= 64 && (s == 1 || (s - 1) * BN < all); ++s) {
-      const int chunk = up((all + s - 1) / s, BN);
-      // rounds of items, each its tiles and a fixed part of about four; the join reads and writes
-      const double cost = (double)((tiles * s + CUS - 1) / CUS) * (chunk / BN + 4) + (s > 1 ? 3.0 + tiles * s * 0.01 : 0.0);
-      if (cost < least) least = cost, best = s;
-    }
-    if (kv_splits > 0) best = kv_splits;
-    c.o_splits = best;
-    c.o_chunk = up((all + best - 1) / best, BN);
-    c.slots = best;
-    return c;
-  }
+  c.o_base = 0;
+  for (int s = kv_splits > 0 ? kv_splits : 1; s <= (kv_splits > 0 ? kv_splits : 192); s += more(s)) consider(max_kv, mean, s);
+  if (prefix == 0) return best;
+  // split: the prefix for all head rows at once, in ranges
+  const int own = std::max(max_kv - prefix, 0);
+  const double own_mean = std::max(mean - prefix, 0.0);
   c.o_base = prefix;
-  // split: ranges of one length for both kinds, as many items as keep the CUs busy
-  int best = BN;
-  double least = 1e30;
-  for (int chunk = BN; chunk <= std::max(prefix, own) + BN; chunk += up(chunk / 8, BN)) {
-    const int64_t np = (prefix + chunk - 1) / chunk, no = (own + chunk - 1) / chunk;
-    if (np + no > MAX_SLOTS) continue;
-    const int64_t items = np * c.p_tiles + no * o_all;
-    const double cost = (double)((items + CUS - 1) / CUS) * (std::min(chunk, std::max(prefix, own)) / (double)BN + 4) +
-                        3.0 + (double)(np + no) * m / 128 * 0.01;
-    if (cost < least) least = cost, best = chunk;
+  c.p_tiles = (int)((m + 32 * c.p_mt - 1) / (32 * c.p_mt));
+  const int gran = c.p_mt == 1 ? 4 * BN : BN;
+  for (int s = kv_splits > 0 ? kv_splits : 1; s <= (kv_splits > 0 ? kv_splits : 192); s += more(s)) {
+    c.p_chunk = up((prefix + s - 1) / s, gran);
+    c.p_splits = (prefix + c.p_chunk - 1) / c.p_chunk;
+    // own ranges as long as a prefix range takes, or one
+    const double fit = md.item(c.p_mt, c.p_chunk) - 6.0;
+    const double per = md.scale * (c.o_mt == 4 ? 1.55 / 32 : c.o_mt == 2 ? 1.3 / 32 : 3.7 / 128);
+    consider(own, own_mean, (int)std::ceil(own * per / std::max(fit, per * BN)));
+    if (c.o_splits > 1) consider(own, own_mean, 1);
+    if (s > 1 && c.p_chunk == gran) break;
   }
-  if (kv_splits > 0) best = up((prefix + kv_splits - 1) / kv_splits, BN);
-  c.p_chunk = c.o_chunk = best;
-  c.p_splits = (prefix + best - 1) / best;
-  c.o_splits = std::max(1, std::min((own + best - 1) / best, MAX_SLOTS - c.p_splits));
-  c.slots = c.p_splits + c.o_splits;
-  return c;
+  return best;
 }
 
 template <int IO>
 hipError_t launch_io(const PfxK& k, int d, hipStream_t s) {
-  const int64_t items = (int64_t)k.p_items + (int64_t)k.batch * k.o_tiles * k.o_splits;
+  const int64_t items = 8 * (int64_t)k.per_xcd;
   const int64_t m = (int64_t)k.rows * k.n1;
+  const unsigned blocks = (unsigned)((m + 31) / 32);
+  // few rows: eight waves share a row group's ranges (a work-group a group of 8 columns)
+  const bool wide = k.slots > 8 && blocks <= 16;
 #define DSA_PFX(DD)                                                                                               \
   hipLaunchKernelGGL((prefix_attn_kernel<IO, DD>), dim3((unsigned)items), dim3(NWV * 64), 0, s, k);                \
-  if (k.slots > 1)                                                                                                 \
-    hipLaunchKernelGGL((prefix_merge_kernel<IO, DD>), dim3((unsigned)((m * (DD / 4) + 255) / 256)), dim3(256), 0, s, k)
+  if (k.slots > 1 && wide)                                                                                         \
+    hipLaunchKernelGGL((prefix_merge_kernel<IO, DD, 8>), dim3(blocks, DD / 8), dim3(512), 0, s, k);                \
+  else if (k.slots > 1)                                                                                            \
+    hipLaunchKernelGGL((prefix_merge_kernel<IO, DD, 1>), dim3(blocks, DD / 32), dim3(256), 0, s, k)
   if (d == 512) {
     DSA_PFX(512);
   } else if (d == 256) {
@@ -724,20 +1162,27 @@ hipError_t launch_io(const PfxK& k, int d, hipStream_t s) {
 }
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// Blocks of 32 head rows: the prefix's, of whole tiles, and the sequences' own, each from a block of its own
+int prefix_blocks(const Cut& c) { return c.p_tiles * c.p_mt; }
+int own_blocks(int batch, int64_t m) { return (int)(m / 32) + batch + 1; }
+size_t block_bytes(int d) { return (size_t)32 * d * sizeof(float); }
 }  // namespace
 }  // namespace dsa
 
 using namespace dsa;
 
-size_t prefix_attn_workspace_bytes(int batch, int rows, int n1, int d, int prefix, int max_rows, int max_kv, int kv_splits) {
-  const Cut c = make_cut(batch, rows, n1, prefix, max_rows, max_kv, kv_splits);
+size_t prefix_attn_workspace_bytes(int batch, int rows, int n1, int d, int prefix, int max_rows, int max_kv, int64_t total_kv,
+                                   int kv_splits) {
+  const Cut c = make_cut(batch, rows, n1, d, prefix, max_rows, max_kv, total_kv, kv_splits);
   if (c.slots == 1) return 0;
   const size_t m = (size_t)rows * n1;
-  return align256(m * c.slots * sizeof(float4)) + m * c.slots * d * sizeof(float);
+  return align256(m * c.slots * sizeof(float4)) +
+         ((size_t)c.p_splits * prefix_blocks(c) + (size_t)c.o_splits * own_blocks(batch, m)) * block_bytes(d);
 }
 
 hipError_t launch_prefix_attn(const PrefixArgs& a, hipStream_t s) {
-  const Cut c = make_cut(a.batch, a.total_rows, a.n1, a.prefix, a.max_rows, a.max_kv, a.kv_splits);
+  const Cut c = make_cut(a.batch, a.total_rows, a.n1, a.d, a.prefix, a.max_rows, a.max_kv, a.total_kv, a.kv_splits);
   PfxK k{};
   k.q = (const uint16_t*)a.q;
   k.qr = (const uint16_t*)a.qr;
@@ -765,17 +1210,24 @@ hipError_t launch_prefix_attn(const PrefixArgs& a, hipStream_t s) {
   k.sm_max = a.sm_max;
   k.sm_sum = a.sm_sum;
   k.part_s = (float4*)a.ws;
-  k.part_o = c.slots > 1 ? (float*)((char*)a.ws + align256((size_t)a.total_rows * a.n1 * c.slots * sizeof(float4))) : nullptr;
+  k.p_blocks = prefix_blocks(c);
+  k.o_blocks = own_blocks(a.batch, (int64_t)a.total_rows * a.n1);
+  k.p_part = c.slots > 1 ? (float4*)((char*)a.ws + align256((size_t)a.total_rows * a.n1 * c.slots * sizeof(float4))) : nullptr;
+  k.o_part = c.slots > 1 ? k.p_part + (size_t)c.p_splits * k.p_blocks * (block_bytes(a.d) / sizeof(float4)) : nullptr;
+  while ((1 << k.n1_shift) < a.n1) ++k.n1_shift;
   k.p_mt = c.p_mt;
   k.p_tiles = c.p_tiles;
   k.p_splits = c.p_splits;
   k.p_chunk = c.p_chunk;
-  k.p_items = c.p_tiles * c.p_splits;
   k.o_mt = c.o_mt;
   k.o_tiles = c.o_tiles;
   k.o_splits = c.o_splits;
   k.o_chunk = c.o_chunk;
   k.o_base = c.o_base;
   k.slots = c.slots;
+  const int most = (c.p_splits + 7) / 8 * c.p_tiles;   // prefix items of an XCD
+  const int64_t all = (int64_t)c.p_splits * c.p_tiles + (int64_t)a.batch * c.o_tiles * c.o_splits;
+  k.per_xcd = (int)std::max<int64_t>(most, (all + 7) / 8);
+  k.o_by_range = c.p_splits == 0 && c.o_splits >= 8;
   return a.io == DSA_DTYPE_BF16 ? launch_io<IO_BF16>(k, a.d, s) : launch_io<IO_F16>(k, a.d, s);
 }

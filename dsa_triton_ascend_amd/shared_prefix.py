@@ -74,7 +74,7 @@ class SharedPrefixPlan:
         self.prefix = int(prefix_length)
         if not 0 <= self.prefix <= s2:
             raise ValueError(f"prefix_length {prefix_length} must lie between 0 and the block table's {s2} tokens")
-        self.max_kv, self.kv_splits = max(act_k, default=0), int(kv_splits)
+        self.max_kv, self.total_kv, self.kv_splits = max(act_k, default=0), sum(act_k), int(kv_splits)
         if not 0 <= self.kv_splits <= 64:
             raise ValueError("kv_splits must lie between 0 and 64")
         self.dev = H.require_device(query, key, query_rope, key_rope, block_table)
@@ -93,7 +93,7 @@ class SharedPrefixPlan:
                 return
             self.block_table = block_table.to(torch.int32).contiguous()
             self.ws_bytes = self.lib.dsa_prefix_attn_workspace_bytes(self.batch, total_rows, N1, D, self.prefix, per,
-                                                                     self.max_kv, self.kv_splits)
+                                                                     self.max_kv, self.total_kv, self.kv_splits)
             self.ws = torch.empty(self.ws_bytes, dtype=torch.uint8, device=self.dev) if self.ws_bytes else None
             self.row_start, self.act_q, self.act_k = H.upload(self.lib, self.dev, row_start, act_q, act_k, wait=_wait)
 
@@ -104,7 +104,7 @@ class SharedPrefixPlan:
                     self.q.data_ptr(), self.qr.data_ptr(), self.kk.data_ptr(), self.kr.data_ptr(), self.io,
                     self.block_table.data_ptr(), self.max_blocks, self.page, self.num_blocks, self.row_start.data_ptr(),
                     self.act_q.data_ptr(), self.act_k.data_ptr(), self.batch, self.total_rows, self.n1, self.d, D_ROPE,
-                    self.prefix, self.max_rows, self.max_kv, self.sparse_mode, self.scale, self.out.data_ptr(),
+                    self.prefix, self.max_rows, self.max_kv, self.total_kv, self.sparse_mode, self.scale, self.out.data_ptr(),
                     self.sm[0].data_ptr() if self.return_lse else None, self.sm[1].data_ptr() if self.return_lse else None,
                     H.ptr(self.ws), self.ws_bytes, self.kv_splits, H.stream_ptr(self.dev)), "dsa_prefix_attn")
         return self.out, self.sm[0], self.sm[1]

@@ -428,7 +428,7 @@ int dsa_index_append(const void* index_key, int64_t batch_stride, int64_t row_st
  * no initialisation. kv_splits <= 0: the library's choice; pass the same value to both.
  */
 size_t dsa_prefix_attn_workspace_bytes(int batch, int total_rows, int n1, int d, int prefix, int max_rows_per_batch,
-                                       int max_kv, int kv_splits);
+                                       int max_kv, int64_t total_kv, int kv_splits);
 
 /*
  * Dense attention over paged latents for a batch whose sequences share their first `prefix` tokens,
@@ -447,17 +447,18 @@ size_t dsa_prefix_attn_workspace_bytes(int batch, int total_rows, int n1, int d,
  *   query [total_rows, N1, D], query_rope [total_rows, N1, 64], key [num_blocks, page, 1, D], key_rope
  *   [.., 64], fp16 / bf16, 16-byte aligned; N1 a power of two up to 128; D in {128, 256, 512};
  *   num_blocks * page and total_rows * N1 < 2^31.
- *   max_rows_per_batch: a bound on row_start[b+1] - row_start[b]; max_kv: the longest act_k that the caller
- *   expects. max_kv only chooses how the work is cut: any act_k gives the same result to rounding.
+ *   max_rows_per_batch: a bound on row_start[b+1] - row_start[b]; max_kv, total_kv: the longest act_k and
+ *   the sum of them that the caller expects. They only choose how the work is cut: any act_k gives the same
+ *   result to rounding.
  *   kv_splits (<= 64): 0, or how many ranges of tokens the prefix (all tokens, where nothing is shared
  *   among tiles) is cut into. Calls that share a workspace must be ordered.
  */
 int dsa_prefix_attn(const void* query, const void* query_rope, const void* key, const void* key_rope, int io_dtype,
                     const int32_t* block_table, int max_blocks, int page_block_size, int64_t num_blocks,
                     const int32_t* row_start, const int32_t* act_q, const int32_t* act_k, int batch, int total_rows,
-                    int n1, int d, int dr, int prefix, int max_rows_per_batch, int max_kv, int sparse_mode, float scale,
-                    void* out, float* sm_max, float* sm_sum, void* workspace, size_t workspace_bytes, int kv_splits,
-                    void* stream);
+                    int n1, int d, int dr, int prefix, int max_rows_per_batch, int max_kv, int64_t total_kv, int sparse_mode,
+                    float scale, void* out, float* sm_max, float* sm_sum, void* workspace, size_t workspace_bytes,
+                    int kv_splits, void* stream);
 
 #ifdef __cplusplus
 }

@@ -45,17 +45,17 @@ def test_packed_lengths_refused():
 def test_c_entry_refuses():
     lib = _lib.load()
     p = ctypes.c_void_p(16)   # never dereferenced: validation fails first
-    base = [p, p, p, p, 1, p, 4, 16, 8, p, p, p, 2, 4, 16, 512, 64, 32, 2, 64, 3, 0.04, p, None, None, p, 1 << 40, 2, None]
-    for at, v, what in ([(i, None, "null") for i in (0, 1, 2, 3, 5, 9, 10, 11, 22)] +
-                        [(4, 2, "io_dtype"), (20, 1, "sparse_mode"), (15, 192, "D must"), (16, 32, "rope dim"), (14, 12, "N1 must"),
+    base = [p, p, p, p, 1, p, 64, 16, 8, p, p, p, 2, 4, 16, 512, 64, 32, 2, 1000, 1600, 3, 0.04, p, None, None, p, 1 << 40, 2, None]
+    for at, v, what in ([(i, None, "null") for i in (0, 1, 2, 3, 5, 9, 10, 11, 23)] +
+                        [(4, 2, "io_dtype"), (21, 1, "sparse_mode"), (20, -1, "shape"), (15, 192, "D must"), (16, 32, "rope dim"), (14, 12, "N1 must"),
                          (12, 0, "shape"), (13, -1, "shape"), (6, 0, "shape"), (7, 0, "shape"), (8, 0, "shape"), (17, -1, "shape"),
-                         (18, -1, "shape"), (19, -1, "shape"), (17, 65, "past"), (19, 65, "past"), (0, ctypes.c_void_p(24), "aligned"),
-                         (22, ctypes.c_void_p(24), "aligned"), (23, p, "both"), (26, 0, "workspace"), (25, None, "workspace")]):
+                         (18, -1, "shape"), (19, -1, "shape"), (17, 1025, "past"), (19, 1025, "past"), (0, ctypes.c_void_p(24), "aligned"),
+                         (23, ctypes.c_void_p(24), "aligned"), (24, p, "both"), (27, 0, "workspace"), (26, None, "workspace")]):
         a = list(base)
         a[at] = v
         assert lib.dsa_prefix_attn(*a) == _lib.DSA_ERR_INVALID, what
         assert what in lib.dsa_last_error().decode(), lib.dsa_last_error()
-    for at, v, what in ((27, 65, "kv_splits"), (8, 1 << 31, "2^31"), (13, 1 << 27, "2^31")):
+    for at, v, what in ((28, 65, "kv_splits"), (8, 1 << 31, "2^31"), (13, 1 << 27, "2^31")):
         a = list(base)
         a[at] = v
         assert lib.dsa_prefix_attn(*a) == _lib.DSA_ERR_UNSUPPORTED and what in lib.dsa_last_error().decode()
@@ -69,10 +69,11 @@ def test_c_entry_refuses():
     (5, 1965, 64, 512, 2048, 655, 2703), (1, 1, 1, 128, 1 << 20, 1, 1 << 21), (96, 384, 128, 128, 100, 4, 5000),
     (300, 300, 1, 256, 5000, 1, 5000), (2, 4000, 128, 512, 0, 2000, 4000)])
 def test_workspace_is_bounded(batch, rows, n1, d, prefix, most, kv):
-    """Partials: at most 256 ranges, and no more than a few items per CU ask for (1 GiB at these sizes)."""
+    """Partials: at most 256 ranges of blocks of 32 head rows (whole tiles of the prefix, a block more for
+    each sequence), and no more than a few items per CU ask for (1 GiB at these sizes)."""
     lib = _lib.load()
     for splits in (0, 1, 64):
-        w = lib.dsa_prefix_attn_workspace_bytes(batch, rows, n1, d, prefix, most, kv, splits)
-        assert w % 16 == 0 and w <= rows * n1 * 256 * (4 * d + 16) + 256
+        w = lib.dsa_prefix_attn_workspace_bytes(batch, rows, n1, d, prefix, most, kv, batch * kv, splits)
+        assert w % 16 == 0 and w <= 256 * ((rows * n1 + 32 * (batch + 5)) * 4 * d + rows * n1 * 16) + 256
         if splits == 0:
             assert w <= 1 << 30
