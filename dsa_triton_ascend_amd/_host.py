@@ -121,22 +121,12 @@ def stream_ptr(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 
-class on_device:
-    """Makes a tensors' device current for the launches inside (a stream's kernels need its device to
-    be the current one); nothing to do where it already is."""
-
-    def __init__(self, device: torch.device):
-        self.guard = None
-        if device.index not in (None, torch.cuda.current_device()):
-            self.guard = torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def on_device(device: torch.device, call):
+    """call() with the tensors' device current: a stream's kernels need its device to be that one"""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return call()
+    with torch.cuda.device(device):
+        return call()
 
 
 def aligned16(t: torch.Tensor) -> torch.Tensor:

@@ -10,6 +10,8 @@
 // written once with 16-byte accesses. What is worth computing once is the angle: it needs 64 bits
 // (position 10^5 times a frequency of 1 leaves 2^-7 of a radian in 32-bit arithmetic), so a
 // work-group turns its tokens' angles into a table of (cos, sin) in LDS, shared by all heads.
+#include <algorithm>
+
 #include "dsa_common.hpp"
 
 namespace dsa {
@@ -235,9 +237,12 @@ hipError_t launch_rotary_io(const RotaryK& k, bool inter, hipStream_t s) {
 // ------------------------------------------------------------------ appends
 // A work-group takes NTOK tokens: one thread each finds its token's place in the cache, all of them
 // fill the table of angles, and the tokens' vectors are normed, rotated and stored, LPV lanes of 8
-// elements to a vector. The vectors are loaded before the places are known, so a decode step's few
-// tokens wait for one chain of memory accesses (lengths, block table), not two.
-constexpr int NTOK = 8;
+// elements to a vector. A decode step's few tokens wait for a chain of memory accesses: so the vectors,
+// the norm's weights, the frequencies and the lengths (of the sequence that evenly split ones give) are
+// all requested first, and only the block table is left behind them.
+// Tokens a work-group: 4 up to this many (64 tokens take 5.1 us, 6.0 with 8), else 8 (6926 tokens of two heads of 128: 7.4
+// us, 8.5 with 4; 18,216 latents 15.1, 15.5 with 16)
+constexpr int APPEND_FEW = 2048;
 
 struct Norm {
   int kind;   // 0 none, 1 root mean square, 2 mean and variance
@@ -270,17 +275,18 @@ struct AppendK {
   int64_t blocks;
 };
 
-// Batch of packed row r: the guess of evenly split batches, checked, else a search
-__device__ __forceinline__ int batch_of(const int32_t* row_start, int batch, int r, int guess_rows) {
-  const int g = guess_rows > 0 ? min(r / guess_rows, batch - 1) : 0;
-  if (row_start[g] <= r && r < row_start[g + 1]) return g;
-  return batch_of_row(row_start, batch, r);
-}
-
-__device__ __forceinline__ float norm_param(const void* p, int dt, int i) {
-  if (dt == DSA_DTYPE_F32) return reinterpret_cast<const float*>(p)[i];
-  const uint16_t u = reinterpret_cast<const uint16_t*>(p)[i];
-  return dt == DSA_DTYPE_BF16 ? bf16_to_f32(u) : f16_to_f32(u);
+// Eight of the norm's parameters from element e on
+__device__ __forceinline__ void norm_params(const void* p, int dt, int e, float (&w)[8]) {
+  if (dt == DSA_DTYPE_F32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = reinterpret_cast<const float*>(p)[e + i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint16_t u = reinterpret_cast<const uint16_t*>(p)[e + i];
+      w[i] = dt == DSA_DTYPE_BF16 ? bf16_to_f32(u) : f16_to_f32(u);
+    }
+  }
 }
 
 template <int IO>
@@ -301,7 +307,8 @@ __device__ __forceinline__ float group_sum(float v) {
 // Norm and rotation of one vector: lane `li` of its LPV lanes holds elements 8 li .. 8 li + 7 (zeros
 // past the width). Statistics, weights and rotation in 32 bits; the caller rounds once.
 template <int LPV>
-__device__ __forceinline__ void norm_vec(const Norm& n, int width, int li, float (&x)[8]) {
+__device__ __forceinline__ void norm_vec(const Norm& n, const float (&w)[8], const float (&b)[8], int width, int li,
+                                         float (&x)[8]) {
   if (n.kind == 0) return;
   const bool in = 8 * li < width;
   float mean = 0.f;
@@ -319,12 +326,8 @@ __device__ __forceinline__ void norm_vec(const Norm& n, int width, int li, float
   }
   q = group_sum<LPV>(in ? q : 0.f) / width;
   const float inv = 1.f / sqrtf(q + n.eps);
-  if (!in) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    x[i] = x[i] * inv * norm_param(n.w, n.wdt, 8 * li + i);
-    if (n.b) x[i] += norm_param(n.b, n.wdt, 8 * li + i);
-  }
+  for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * w[i] + b[i];
 }
 
 template <int LPV>
@@ -354,7 +357,7 @@ __device__ __forceinline__ void rotate_vec(const float2* t, int start, int rdim,
   for (int i = 0; i < 8; ++i) x[i] = low ? x[i] * t[i].x - y[i] * t[i].y : y[i] * t[i].y + x[i] * t[i].x;
 }
 
-template <int IO, int LPV, bool LATENT>
+template <int IO, int LPV, bool LATENT, int NTOK>
 __global__ __launch_bounds__(TPB) void append_kernel(AppendK a) {
   extern __shared__ float2 tab[];   // [NTOK][rdim / 2]
   __shared__ int64_t s_row[NTOK];   // the token's cache row, -1: it has none
@@ -373,41 +376,51 @@ __global__ __launch_bounds__(TPB) void append_kernel(AppendK a) {
   };
   float x[8], xb[8];
   load_a(vi, x);
-  // part b (64 wide): 8 lanes a token, the last wave
-  const int bt = (threadIdx.x & 63) >> 3, bl = threadIdx.x & 7;
-  const bool bwave = LATENT && threadIdx.x >= TPB - 64;
+  // part b (64 wide): 8 lanes a token, the last waves
+  const int bt = ((int)threadIdx.x - (TPB - 8 * NTOK)) >> 3, bl = threadIdx.x & 7;
+  const bool bwave = LATENT && (int)threadIdx.x >= TPB - 8 * NTOK;
 #pragma unroll
   for (int i = 0; i < 8; ++i) xb[i] = 0.f;
   if (bwave && r0 + bt < a.total_rows)
     load8<IO>(reinterpret_cast<const uint16_t*>(a.b.x) + row_offset(a.b.view, r0 + bt) + 8 * bl, a.b.aligned, xb);
 
+  float nw[8], nb[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) nw[i] = nb[i] = 0.f;
+  if (a.norm.kind != 0 && 8 * li < a.a.width) {
+    norm_params(a.norm.w, a.norm.wdt, 8 * li, nw);
+    if (a.norm.b) norm_params(a.norm.b, a.norm.wdt, 8 * li, nb);
+  }
+  const int half = a.rdim / 2;
+  // pair threadIdx.x % half of the table's token threadIdx.x / half (32 pairs: one a thread)
+  const float freq0 = a.freq[(int)threadIdx.x % half];
   if (threadIdx.x < NTOK) {
-    const int r = r0 + threadIdx.x;
+    const int r = min(r0 + (int)threadIdx.x, a.total_rows - 1);
+    int b = a.rows_per_batch > 0 ? min(r / a.rows_per_batch, a.batch - 1) : 0;
+    int rs = a.row_start[b], re = a.row_start[b + 1], aq = a.act_q[b], ak = a.act_k[b];
+    if (r < rs || r >= re) {
+      b = batch_of_row(a.row_start, a.batch, r);
+      rs = a.row_start[b], re = a.row_start[b + 1], aq = a.act_q[b], ak = a.act_k[b];
+    }
     int64_t row = -1;
-    int pos = 0;
-    if (r < a.total_rows) {
-      const int b = batch_of(a.row_start, a.batch, r, a.rows_per_batch);
-      const int s1 = r - a.row_start[b], aq = a.act_q[b], ak = a.act_k[b];
-      pos = ak - aq + s1;
-      // rows past the batch's queries (or past the last batch), and tokens before position 0, have no place
-      if (s1 >= 0 && s1 < aq && r < a.row_start[b + 1] && pos >= 0) {
-        const int pg = pos / a.page;
-        if (pg < a.max_blocks) {
-          const int blk = a.table[(int64_t)b * a.max_blocks + pg];
-          if (blk >= 0 && blk < a.blocks) row = (int64_t)blk * a.page + (pos - pg * a.page);
-        }
+    const int s1 = r - rs, pos = ak - aq + s1;
+    // rows past the batch's queries (or past the last batch), and tokens before position 0, have no place
+    if (r0 + (int)threadIdx.x < a.total_rows && s1 >= 0 && s1 < aq && r < re && pos >= 0) {
+      const int pg = pos / a.page;
+      if (pg < a.max_blocks) {
+        const int blk = a.table[(int64_t)b * a.max_blocks + pg];
+        if (blk >= 0 && blk < a.blocks) row = (int64_t)blk * a.page + (pos - pg * a.page);
       }
     }
     s_row[threadIdx.x] = row;
     s_pos[threadIdx.x] = pos;
   }
   __syncthreads();
-  const int half = a.rdim / 2;
   for (int i = threadIdx.x; i < NTOK * half; i += TPB) {
     const int tok = i / half, pair = i - tok * half;
     if (s_row[tok] >= 0) {
       const int64_t p = a.pos.p ? position_of(a.pos, r0 + tok, pair) : (int64_t)s_pos[tok];
-      tab[i] = cos_sin(p, a.freq[pair]);
+      tab[i] = cos_sin(p, i == (int)threadIdx.x ? freq0 : a.freq[pair]);
     } else {
       tab[i] = make_float2(1.f, 0.f);
     }
@@ -419,7 +432,7 @@ __global__ __launch_bounds__(TPB) void append_kernel(AppendK a) {
     float nx[8];
     if (more) load_a(v + VPP, nx);
     const int tok = min(v / a.a.heads, NTOK - 1), h = v - tok * a.a.heads;
-    norm_vec<LPV>(a.norm, a.a.width, li, x);
+    norm_vec<LPV>(a.norm, nw, nb, a.a.width, li, x);
     if (!LATENT) rotate_vec<LPV>(tab + tok * half, a.start, a.rdim, a.inter, li, x);
     if (v < nvec && 8 * li < a.a.width && s_row[tok] >= 0)
       store_vec<IO, 8>(reinterpret_cast<uint16_t*>(a.a.cache) + (s_row[tok] * a.a.heads + h) * a.a.width + 8 * li, x);
@@ -433,15 +446,19 @@ __global__ __launch_bounds__(TPB) void append_kernel(AppendK a) {
   }
 }
 
-template <int IO, bool LATENT>
-hipError_t launch_append_io(const AppendK& k, hipStream_t s) {
+template <int IO, bool LATENT, int NTOK>
+hipError_t launch_append_n(const AppendK& k, hipStream_t s) {
   const dim3 grid((k.total_rows + NTOK - 1) / NTOK);
   const size_t lds = (size_t)NTOK * (k.rdim / 2) * sizeof(float2);
-  if (k.a.width <= 64) hipLaunchKernelGGL((append_kernel<IO, 8, LATENT>), grid, dim3(TPB), lds, s, k);
-  else if (k.a.width <= 128) hipLaunchKernelGGL((append_kernel<IO, 16, LATENT>), grid, dim3(TPB), lds, s, k);
-  else if (k.a.width <= 256) hipLaunchKernelGGL((append_kernel<IO, 32, LATENT>), grid, dim3(TPB), lds, s, k);
-  else hipLaunchKernelGGL((append_kernel<IO, 64, LATENT>), grid, dim3(TPB), lds, s, k);
+  if (!LATENT && k.a.width <= 64) hipLaunchKernelGGL((append_kernel<IO, 8, LATENT, NTOK>), grid, dim3(TPB), lds, s, k);
+  else if (k.a.width <= 128) hipLaunchKernelGGL((append_kernel<IO, 16, LATENT, NTOK>), grid, dim3(TPB), lds, s, k);
+  else if (k.a.width <= 256) hipLaunchKernelGGL((append_kernel<IO, 32, LATENT, NTOK>), grid, dim3(TPB), lds, s, k);
+  else hipLaunchKernelGGL((append_kernel<IO, 64, LATENT, NTOK>), grid, dim3(TPB), lds, s, k);
   return hipGetLastError();
+}
+template <int IO, bool LATENT>
+hipError_t launch_append_io(const AppendK& k, hipStream_t s) {
+  return k.total_rows > APPEND_FEW ? launch_append_n<IO, LATENT, 8>(k, s) : launch_append_n<IO, LATENT, 4>(k, s);
 }
 
 int is_aligned(const void* p, const View& v) {
@@ -493,7 +510,7 @@ hipError_t launch_cache_append(const AppendArgs& a, hipStream_t s) {
   k.total_rows = a.total_rows;
   k.max_blocks = a.max_blocks;
   k.page = a.page;
-  k.rows_per_batch = a.total_rows % a.batch == 0 ? a.total_rows / a.batch : 0;
+  k.rows_per_batch = std::max(1, a.total_rows / a.batch);
   k.blocks = a.blocks;
   if (a.io == DSA_DTYPE_BF16)
     return latent ? launch_append_io<DSA_DTYPE_BF16, true>(k, s) : launch_append_io<DSA_DTYPE_BF16, false>(k, s);

@@ -9,18 +9,47 @@ same cumulative ``actual_seq_lengths`` and the positions are batch-local.
 ``PrefillPlan`` validates and allocates both calls once; the attention plan
 reads the indexer's index buffer in place, so ``run()`` is three kernel
 launches on the current stream (score, top-k, attention) plus the SFA
-token-list pass, with no host synchronisation between them.
+token-list pass, with no host synchronisation between them. Given inverse frequencies it
+takes the attention's rotary parts unrotated and rotates them first (two launches more).
 """
 from __future__ import annotations
 
+import torch
+
+from . import _host as H
+from . import _lib
 from .lightning_indexer import IndexerPlan
+from .rotary import D_ROPE, _frequencies, _Rotation
 from .sparse_flash_attention import AttentionPlan
 
 
 class PrefillPlan:
     def __init__(self, index_query, index_key, index_weights, query, key, query_rope, key_rope,
                  cu_seqlens, sparse_count=2048, scale_value=1.0, sparse_mode=3,
-                 return_softmax_lse=False, return_value=False, *, _wait=True):
+                 return_softmax_lse=False, return_value=False, inv_freq=None, positions=None, sections=None,
+                 interleaved=True, *, _wait=True):
+        """inv_freq (None: query_rope and key_rope are rotated already), positions (default: each token's
+        place in its sequence), sections and interleaved as in rotary_embedding."""
+        self.rotations = ()
+        if inv_freq is not None:
+            freq = _frequencies(inv_freq, D_ROPE // 2)
+            if positions is None:
+                if sections is not None:
+                    raise ValueError("several position axes need positions")
+                lengths = H.per_batch_from_cumsum(H.host_lengths(cu_seqlens))
+                rows = query_rope.shape[0]
+                within = [p for n in lengths for p in range(n)][:rows]
+                within += [0] * (rows - len(within))
+                dev = H.require_device(query_rope, key_rope, freq)
+                if torch.cuda.is_current_stream_capturing():   # a copy from the host could not be captured
+                    positions = H.upload(_lib.load(), dev, within)[0][:rows]
+                else:
+                    positions = torch.tensor(within, dtype=torch.int32).to(dev)
+            self.rotations = tuple(_Rotation(x, positions, freq, sections, 0, interleaved, "TND", 0, what)
+                                   for x, what in ((query_rope, "query_rope"), (key_rope, "key_rope")))
+            query_rope, key_rope = (r.out for r in self.rotations)
+        elif positions is not None or sections is not None:
+            raise ValueError("positions and sections need inv_freq")
         self.indexer = IndexerPlan(index_query, index_key, index_weights, cu_seqlens, cu_seqlens,
                                    layout_query="TND", layout_key="TND", sparse_count=sparse_count,
                                    sparse_mode=sparse_mode, return_value=return_value, _wait=False)
@@ -43,14 +72,17 @@ class PrefillPlan:
 
     def run(self):
         """Returns (indices, attention_out, softmax_max, softmax_sum)."""
+        for r in self.rotations:
+            r.run()
         self.indexer.run()
         out = self.attention.run()
         return (self.indexer.idx,) + tuple(out)
 
 
 def dsa_prefill(index_query, index_key, index_weights, query, key, query_rope, key_rope, cu_seqlens,
-                sparse_count=2048, scale_value=1.0, sparse_mode=3, return_softmax_lse=False):
+                sparse_count=2048, scale_value=1.0, sparse_mode=3, return_softmax_lse=False, inv_freq=None,
+                positions=None, sections=None, interleaved=True):
     """One-shot form of ``PrefillPlan(...).run()``."""
     return PrefillPlan(index_query, index_key, index_weights, query, key, query_rope, key_rope,
-                       cu_seqlens, sparse_count, scale_value, sparse_mode, return_softmax_lse,
-                       _wait=False).run()
+                       cu_seqlens, sparse_count, scale_value, sparse_mode, return_softmax_lse, inv_freq=inv_freq,
+                       positions=positions, sections=sections, interleaved=interleaved, _wait=False).run()

@@ -50,38 +50,49 @@ def _positions(positions, lead, axes: int, sectioned: bool) -> torch.Tensor:
 
 
 def _rows_view(x: torch.Tensor, layout: str, what: str):
-    """x with a contiguous last dimension, and its (batch, row, head) strides and rows per batch"""
-    if layout not in ("BSND", "TND"):
-        raise ValueError(f"unsupported layout {layout}")
-    if x.dim() != (4 if layout == "BSND" else 3):
-        raise ValueError(f"{what} must be {'[B, S, N, D]' if layout == 'BSND' else '[T, N, D]'}, got {list(x.shape)}")
-    if x.shape[-1] > 1 and x.stride(-1) != 1:
-        x = x.contiguous()
+    """x with a contiguous last dimension, its (batch, row, head) strides and its rows per batch"""
     if layout == "BSND":
-        return x, x.stride(0), x.stride(1), x.stride(2), max(1, x.shape[1])
-    return x, 0, x.stride(0), x.stride(1), max(1, x.shape[0])
+        if x.dim() != 4:
+            raise ValueError(f"{what} must be [B, S, N, D], got {list(x.shape)}")
+    elif layout != "TND":
+        raise ValueError(f"unsupported layout {layout}")
+    elif x.dim() != 3:
+        raise ValueError(f"{what} must be [T, N, D], got {list(x.shape)}")
+    stride = x.stride()
+    if stride[-1] != 1 and x.shape[-1] > 1:
+        x = x.contiguous()
+        stride = x.stride()
+    if layout == "BSND":
+        return x, stride[0], stride[1], stride[2], max(1, x.shape[1])
+    return x, 0, stride[0], stride[1], max(1, x.shape[0])
 
 
-def _rotate(x, positions, inv_freq, sections, rotary_start, interleaved, layout, inverse, what):
-    x, sb, ss, sh, per = _rows_view(x, layout, what)
-    freq = _frequencies(inv_freq)
-    dtype = H.dtype_code(x.dtype, what, allow_f32=True)
-    axes, sec = _sections(sections, freq.numel())
-    pos = _positions(positions, x.shape[:-2], axes, sec is not None)
-    n, width = x.shape[-2:]
-    if rotary_start < 0 or rotary_start + 2 * freq.numel() > width:
-        raise ValueError(f"rotary dimensions [{rotary_start}, {rotary_start} + {2 * freq.numel()}) of a width of {width}")
-    dev = H.require_device(x, pos, freq)
-    lib = _lib.load()
-    with H.on_device(dev):
-        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        if x.numel() == 0:
-            return out
-        _lib.check(lib.dsa_rotary(x.data_ptr(), sb, ss, sh, dtype, pos.data_ptr(), int(pos.dtype == torch.int64), axes, sec,
-                                  freq.data_ptr(), x.numel() // (n * width), per, n, width, int(rotary_start),
-                                  2 * freq.numel(), int(bool(interleaved)), inverse, out.data_ptr(), H.stream_ptr(dev)),
-                   "dsa_rotary")
-    return out
+class _Rotation:
+    """Validated arguments of one rotation and its output; ``run()`` launches on the current stream."""
+
+    def __init__(self, x, positions, inv_freq, sections, rotary_start, interleaved, layout, inverse, what):
+        x, sb, ss, sh, per = _rows_view(x, layout, what)
+        freq = _frequencies(inv_freq)
+        dtype = H.dtype_code(x.dtype, what, allow_f32=True)
+        pairs = freq.numel()
+        axes, sec = _sections(sections, pairs)
+        shape = x.shape
+        pos = _positions(positions, shape[:-2], axes, sec is not None)
+        n, width = shape[-2:]
+        if rotary_start < 0 or rotary_start + 2 * pairs > width:
+            raise ValueError(f"rotary dimensions [{rotary_start}, {rotary_start} + {2 * pairs}) of a width of {width}")
+        self.dev = H.require_device(x, pos, freq)
+        self.lib = _lib.load()
+        self.out = out = torch.empty(shape, dtype=x.dtype, device=self.dev)
+        self.keep = (x, pos, freq, sec)
+        self.args = (x.data_ptr(), sb, ss, sh, dtype, pos.data_ptr(), pos.dtype == torch.int64, axes, sec, freq.data_ptr(),
+                     out.numel() // (n * width), per, n, width, rotary_start, 2 * pairs, bool(interleaved), inverse,
+                     out.data_ptr()) if out.numel() else None
+
+    def run(self):
+        if self.args is not None:
+            H.on_device(self.dev, lambda: _lib.check(self.lib.dsa_rotary(*self.args, H.stream_ptr(self.dev)), "dsa_rotary"))
+        return self.out
 
 
 def rotary_embedding(x, positions, inv_freq, sections=None, rotary_start=0, interleaved=True, layout="BSND"):
@@ -94,13 +105,13 @@ def rotary_embedding(x, positions, inv_freq, sections=None, rotary_start=0, inte
     [axes, B, S] / [axes, T], and each run of pairs turns by the position on its own axis: the time,
     height and width of an image's or video's tokens. Angles are computed in 64 bits. Returns a new
     contiguous tensor."""
-    return _rotate(x, positions, inv_freq, sections, rotary_start, interleaved, layout, 0, "x")
+    return _Rotation(x, positions, inv_freq, sections, rotary_start, interleaved, layout, 0, "x").run()
 
 
 def rotary_embedding_grad(d_out, positions, inv_freq, sections=None, rotary_start=0, interleaved=True, layout="BSND"):
     """Gradient of :func:`rotary_embedding` with respect to x: d_out rotated back. (For the gradients
     ``d_query_rope`` / ``d_key_rope`` of ``sparse_flash_attention_grad``, arguments as in the forward.)"""
-    return _rotate(d_out, positions, inv_freq, sections, rotary_start, interleaved, layout, 1, "d_out")
+    return _Rotation(d_out, positions, inv_freq, sections, rotary_start, interleaved, layout, 1, "d_out").run()
 
 
 class RotaryEmbedding(torch.nn.Module):
@@ -171,19 +182,23 @@ class _AppendPlan:
                 raise ValueError(f"kv length {k} outside the block table's {self.max_blocks * self.page} tokens")
         self.dev = H.require_device(self.x, block_table, self.freq, self.pos, *norm, *more, *[c for c, _ in caches])
         self.lib = _lib.load()
-        with H.on_device(self.dev):
+        self.args = None   # of the launch, but for the stream; None: nothing to do
+        if not (self.batch and self.total_rows and self.max_blocks and self.num_blocks and self.page):
+            return None, None
+
+        def place():
             self.block_table = block_table.to(torch.int32).contiguous()
-            if self.batch and self.total_rows:
-                self.row_start, self.act_q, self.act_k = H.upload(self.lib, self.dev, row_start, act_q, act_k, wait=_wait)
-        self.empty = not (self.batch and self.total_rows and self.max_blocks and self.num_blocks and self.page)
+            return H.upload(self.lib, self.dev, row_start, act_q, act_k, wait=_wait)
 
-    def _places(self):
-        return (self.row_start.data_ptr(), self.act_q.data_ptr(), self.act_k.data_ptr(), self.block_table.data_ptr(),
-                self.batch, self.total_rows, self.per, self.max_blocks, self.page, self.num_blocks)
+        self.row_start, self.act_q, self.act_k = H.on_device(self.dev, place)
+        rotation = (H.ptr(self.pos), self.pos is not None and self.pos.dtype == torch.int64, self.axes, self.sec,
+                    self.freq.data_ptr())
+        return rotation, (self.row_start.data_ptr(), self.act_q.data_ptr(), self.act_k.data_ptr(), self.block_table.data_ptr(),
+                          self.batch, self.total_rows, self.per, self.max_blocks, self.page, self.num_blocks)
 
-    def _rotation(self):
-        return (H.ptr(self.pos), int(self.pos is not None and self.pos.dtype == torch.int64), self.axes, self.sec,
-                self.freq.data_ptr())
+    def _launch(self, entry, what):
+        if self.args is not None:
+            H.on_device(self.dev, lambda: _lib.check(entry(*self.args, H.stream_ptr(self.dev)), what))
 
 
 class LatentAppendPlan(_AppendPlan):
@@ -205,20 +220,18 @@ class LatentAppendPlan(_AppendPlan):
             raise ValueError("Only N2=1 (MQA) is supported, key_rope as many tokens as latent")
         if tuple(key_cache.shape[2:]) != (1, d) or tuple(key_rope_cache.shape[2:]) != (1, D_ROPE):
             raise ValueError(f"caches must be [num_blocks, block_size, 1, {d}] and [.., 1, {D_ROPE}]")
-        self._setup(latent, [(key_cache, "key_cache"), (key_rope_cache, "key_rope_cache")], block_table, inv_freq,
+        rotation, places = self._setup(latent, [(key_cache, "key_cache"), (key_rope_cache, "key_rope_cache")], block_table, inv_freq,
                     D_ROPE // 2, actual_seq_lengths_kv, actual_seq_lengths_query, positions, sections, layout,
                     (norm_weight,), (key_rope,), "latent", _wait)
-        self.d, self.inter, self.eps = d, int(bool(interleaved)), float(norm_eps)
         self.norm_weight = None if norm_weight is None else norm_weight.contiguous()
         self.key_cache, self.key_rope_cache = key_cache, key_rope_cache
+        if places is not None:
+            self.args = (self.x.data_ptr(), self.sb, self.ss, self.rope.data_ptr(), self.rb, self.rs, self.io, d,
+                         H.ptr(self.norm_weight), self.wdt, float(norm_eps), *rotation, bool(interleaved), *places,
+                         key_cache.data_ptr(), key_rope_cache.data_ptr())
 
     def run(self):
-        if not self.empty:
-            with H.on_device(self.dev):
-                _lib.check(self.lib.dsa_latent_append(
-                    self.x.data_ptr(), self.sb, self.ss, self.rope.data_ptr(), self.rb, self.rs, self.io, self.d,
-                    H.ptr(self.norm_weight), self.wdt, self.eps, *self._rotation(), self.inter, *self._places(),
-                    self.key_cache.data_ptr(), self.key_rope_cache.data_ptr(), H.stream_ptr(self.dev)), "dsa_latent_append")
+        self._launch(self.lib.dsa_latent_append, "dsa_latent_append")
         return self.key_cache, self.key_rope_cache
 
 
@@ -240,19 +253,17 @@ class IndexAppendPlan(_AppendPlan):
         if self.start < 0 or self.start % 8 or self.rdim % 16 or self.start + self.rdim > self.w:
             raise ValueError(f"rotary dimensions [{self.start}, {self.start} + {self.rdim}) of {self.w}: the start a "
                              "multiple of 8, the count of 16")
-        self._setup(index_key, [(index_cache, "index_cache")], block_table, inv_freq, None, actual_seq_lengths_key,
+        rotation, places = self._setup(index_key, [(index_cache, "index_cache")], block_table, inv_freq, None, actual_seq_lengths_key,
                     actual_seq_lengths_query, positions, sections, layout, (norm_weight, norm_bias), (), "index_key", _wait)
-        self.inter, self.eps = int(bool(interleaved)), float(norm_eps)
         self.norm_weight, self.norm_bias = (None if t is None else t.contiguous() for t in (norm_weight, norm_bias))
         self.index_cache = index_cache
+        if places is not None:
+            self.args = (self.x.data_ptr(), self.sb, self.ss, self.sh, self.io, self.n2, self.w, H.ptr(self.norm_weight),
+                         H.ptr(self.norm_bias), self.wdt, float(norm_eps), *rotation, self.start, self.rdim,
+                         bool(interleaved), *places, index_cache.data_ptr())
 
     def run(self):
-        if not self.empty:
-            with H.on_device(self.dev):
-                _lib.check(self.lib.dsa_index_append(
-                    self.x.data_ptr(), self.sb, self.ss, self.sh, self.io, self.n2, self.w, H.ptr(self.norm_weight),
-                    H.ptr(self.norm_bias), self.wdt, self.eps, *self._rotation(), self.start, self.rdim, self.inter,
-                    *self._places(), self.index_cache.data_ptr(), H.stream_ptr(self.dev)), "dsa_index_append")
+        self._launch(self.lib.dsa_index_append, "dsa_index_append")
         return self.index_cache
 
 

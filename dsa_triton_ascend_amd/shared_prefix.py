@@ -82,13 +82,14 @@ class SharedPrefixPlan:
         self.scale, self.sparse_mode, self.return_lse = float(scale_value), sparse_mode, return_softmax_lse
         self.q, self.qr, self.kk, self.kr = (H.aligned16(t) for t in (query, query_rope, key, key_rope))
         self.empty = not (self.batch and total_rows and self.num_blocks and s2)
+        self.args = None   # of the launch, but for the stream; None: nothing to do
         sm_shape = (1, total_rows, N1) if layout_query == "TND" else (self.batch, 1, per, N1)
-        with H.on_device(self.dev):
+
+        def place():
             # a cache without a block, or a table without a column, holds no token: zeros, as for rows that see none
-            new = torch.zeros if self.empty else torch.empty
-            self.out = new(query.shape, dtype=query.dtype, device=self.dev)
+            self.out = (torch.zeros if self.empty else torch.empty)(query.shape, dtype=query.dtype, device=self.dev)
             stats = torch.empty if return_softmax_lse and not self.empty else torch.zeros
-            self.sm = stats((2,) + sm_shape, dtype=torch.float32, device=self.dev)
+            self.sm_max, self.sm_sum = self.sm = stats((2,) + sm_shape, dtype=torch.float32, device=self.dev).unbind(0)
             if self.empty:
                 return
             self.block_table = block_table.to(torch.int32).contiguous()
@@ -96,18 +97,21 @@ class SharedPrefixPlan:
                                                                      self.max_kv, self.total_kv, self.kv_splits)
             self.ws = torch.empty(self.ws_bytes, dtype=torch.uint8, device=self.dev) if self.ws_bytes else None
             self.row_start, self.act_q, self.act_k = H.upload(self.lib, self.dev, row_start, act_q, act_k, wait=_wait)
+            lse = self.return_lse
+            self.args = (self.q.data_ptr(), self.qr.data_ptr(), self.kk.data_ptr(), self.kr.data_ptr(), io,
+                         self.block_table.data_ptr(), self.max_blocks, self.page, self.num_blocks, self.row_start.data_ptr(),
+                         self.act_q.data_ptr(), self.act_k.data_ptr(), self.batch, total_rows, N1, D, D_ROPE, self.prefix, per,
+                         self.max_kv, self.total_kv, sparse_mode, self.scale, self.out.data_ptr(),
+                         self.sm_max.data_ptr() if lse else None, self.sm_sum.data_ptr() if lse else None, H.ptr(self.ws),
+                         self.ws_bytes, self.kv_splits)
+
+        H.on_device(self.dev, place)
 
     def run(self):
-        if not self.empty:
-            with H.on_device(self.dev):
-                _lib.check(self.lib.dsa_prefix_attn(
-                    self.q.data_ptr(), self.qr.data_ptr(), self.kk.data_ptr(), self.kr.data_ptr(), self.io,
-                    self.block_table.data_ptr(), self.max_blocks, self.page, self.num_blocks, self.row_start.data_ptr(),
-                    self.act_q.data_ptr(), self.act_k.data_ptr(), self.batch, self.total_rows, self.n1, self.d, D_ROPE,
-                    self.prefix, self.max_rows, self.max_kv, self.total_kv, self.sparse_mode, self.scale, self.out.data_ptr(),
-                    self.sm[0].data_ptr() if self.return_lse else None, self.sm[1].data_ptr() if self.return_lse else None,
-                    H.ptr(self.ws), self.ws_bytes, self.kv_splits, H.stream_ptr(self.dev)), "dsa_prefix_attn")
-        return self.out, self.sm[0], self.sm[1]
+        if self.args is not None:
+            H.on_device(self.dev, lambda: _lib.check(self.lib.dsa_prefix_attn(*self.args, H.stream_ptr(self.dev)),
+                                                     "dsa_prefix_attn"))
+        return self.out, self.sm_max, self.sm_sum
 
 
 def shared_prefix_attention(query, key, value, block_table, prefix_length, scale_value=1.0, actual_seq_lengths_query=None,

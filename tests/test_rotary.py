@@ -120,3 +120,11 @@ def test_c_entries_refuse():
     none = list(idx)
     none[24] = 0
     assert lib.dsa_index_append(*none) == 0
+
+
+def test_prefill_refuses_positions_without_frequencies():
+    z = torch.zeros(4, 1, 64, dtype=BF)
+    for kw, message in ((dict(positions=torch.zeros(4, dtype=torch.long)), "need inv_freq"), (dict(sections=(16, 16)), "need inv_freq"),
+                        (dict(inv_freq=F, sections=(16, 16)), "need positions"), (dict(inv_freq=torch.ones(16)), "32 wanted")):
+        with pytest.raises(ValueError, match=message):
+            dsa.dsa_prefill(z, z, z, z, z, z, z, [4], **kw)

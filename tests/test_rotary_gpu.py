@@ -322,6 +322,40 @@ def test_append_plan_replays_with_new_lengths():
         assert torch.equal(c[:, :, 0].cpu(), want), step
 
 
+@pytest.mark.parametrize("sections", [None, (8, 12, 12)])
+def test_prefill_rotates(sections):
+    """dsa_prefill with inverse frequencies: the bits of rotating first and calling it as before, from a
+    plan run twice with new contents too."""
+    g = torch.Generator().manual_seed(13)
+    lens, dt = [70, 33, 120], torch.bfloat16
+    T, cu = sum(lens), torch.tensor(lens).cumsum(0).tolist()
+    r = lambda *s: torch.randn(*s, generator=g).to(dt).cuda()
+    iq, ik, iw = r(T, 32, 128), r(T, 1, 128), torch.randn(T, 32, generator=g).cuda()
+    q, k, qr, kr = r(T, 16, 512), r(T, 1, 512), r(T, 16, 64), r(T, 1, 64)
+    f = freqs(32)
+    pos = torch.cat([torch.arange(n) for n in lens]).cuda()
+    if sections:
+        pos = torch.randint(0, 500, (3, T), generator=g).cuda()
+    kw = dict(sparse_count=32, scale_value=0.04, return_softmax_lse=True)
+    plan = dsa.PrefillPlan(iq, ik, iw, q, k, qr, kr, cu, inv_freq=f, positions=pos if sections else None, sections=sections, **kw)
+    for step in range(2):
+        rot = [dsa.rotary_embedding(x, pos, f, sections=sections, layout="TND") for x in (qr, kr)]
+        want = dsa.dsa_prefill(iq, ik, iw, q, k, *rot, cu, **kw)
+        got = plan.run()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), step
+        assert torch.equal(got[1], dsa.dsa_prefill(iq, ik, iw, q, k, qr, kr, cu, inv_freq=f, positions=pos, sections=sections, **kw)[1])
+        qr.copy_(r(T, 16, 64))
+    if not sections:   # captured whole, positions and all
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = dsa.dsa_prefill(iq, ik, iw, q, k, qr, kr, cu, inv_freq=f, **kw)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, plan.run()))
+            torch.cuda.synchronize()
+
+
 def test_prefill_then_sparse_attention():
     """The operators as a layer uses them: queries rotated, keys of two prompts appended to the paged
     caches, indexer and sparse attention over them; the same as both on contiguous keys rotated and
