@@ -15,13 +15,12 @@
 // Both kinds of item, each over a range of tokens, run in one launch; a second one joins the ranges'
 // (max, sum, output) per head row, unless every row had a single range.
 //
-// An item is one work-group of four waves and 32, 64 or 128 head rows. With 64 or 128 (MT = 2, 4 blocks
-// of 32 rows) tiles of 32 tokens go direct to a ring of three LDS buffers, two tiles ahead. S^T = K Q^T has the tokens as M and
-// 32 head rows as N, the contraction split over the 4 / MT waves of a block (summed through LDS); the
-// online softmax runs in each lane's 16 scores of its head row plus one exchange between lane halves,
-// and its result is already the B operand of O^T += V^T P^T, whose columns the block's waves share.
-// With 32 head rows the bytes are the bound: each wave takes every fourth tile by itself, with a tile's
-// buffer and a softmax of its own and no barrier, and the four outputs are joined through LDS at the end.
+// An item is one work-group of four waves and 32, 64 or 128 head rows. Tiles of 32 tokens go direct to LDS.
+// S^T = K Q^T has the tokens as M and 32 head rows as N; the online softmax runs in each lane's 16 scores
+// of its head row plus one exchange between lane halves, and its result is already the B operand of
+// O^T += V^T P^T, over all columns. With 128 head rows the matrix units are the bound: a wave for each
+// block of 32, the tiles in a ring of three buffers shared by them. With fewer the bytes are, or the
+// latency: the waves split the tokens and join their outputs through LDS at the end.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -126,15 +125,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 template <int D> struct PfxLds {
   union {
-    struct {                              // 64 or 128 head rows: a ring of tiles for the work-group
+    struct {                              // 128 head rows: a ring of tiles for the work-group
       uint8_t nope[NBUF][Tile<D>::NOPE];
       uint8_t rope[NBUF][Tile<D>::ROPE];
-      union {
-        uint16_t qr[128 * (DR + 8)];      // MT = 4: the query's rotary part
-        float x[NWV][16 * 64];            // MT = 2: partial scores
-      };
+      uint16_t qr[128 * (DR + 8)];        // the query's rotary part
     };
-    struct {                              // 32 head rows: a tile for each wave
+    struct {                              // 32 or 64: the waves' or the groups' tiles; any: Q on its way to registers
       uint8_t own_nope[NWV][BN * D * 2];
       uint8_t own_rope[NWV][BN * DR * 2];
     };
@@ -143,7 +139,7 @@ template <int D> struct PfxLds {
   int32_t ids[4][BN];
   int red[2][NWV];
   uint32_t bad[2][NWV];                   // tokens of the tile (bit) with values that are not finite
-  float4 stat[NWV][32];                   // 32 head rows: the waves' maxima and sums
+  float4 stat[NWV][32];                   // 32 or 64 head rows: the waves' maxima and sums
 };
 
 // limit(h): how many tokens of its sequence head row h's query sees
@@ -191,20 +187,15 @@ __device__ __forceinline__ uint4 staged_q(const uint8_t* src, int ks, int rr, in
   return *reinterpret_cast<const uint4*>(src + rr * (D * 2) + (((2 * ks + kg) ^ (rr & 15)) << 4));
 }
 
-template <int IO, int D, int MT>
+// 128 head rows: wave w has rows 32 w .. 32 w + 31, the tiles are shared.
+template <int IO, int D>
 __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D>& L) {
   using C = Tile<D>;
-  constexpr int KSPL = NWV / MT;             // waves of a row block
-  constexpr int KSH = C::KS / KSPL;          // their steps of S^T: wave kh takes steps j * KSPL + kh
-  constexpr int KNH = C::KSN / KSPL;         // of which in the latent part
-  static_assert(C::KS % KSPL == 0 && C::KSN % KSPL == 0 && KSH >= 3, "contraction split");
-  constexpr int ON = D / 32 / KSPL;          // their 32-column tiles of O
-  constexpr bool QLDS = MT == 4;             // the rotary part of Q stays in LDS
-  constexpr int QF = QLDS ? KNH : KSH;       // Q fragments in registers
+  constexpr int KS = C::KS, KSN = C::KSN;    // steps of S^T, of which in the latent part
+  constexpr int ON = D / 32;                 // 32-column tiles of O
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int rb = wave % MT, kh = wave / MT;
   const int kg = lane >> 5, rr = lane & 31;
-  const int h = it.h0 + rb * 32 + rr;
+  const int h = it.h0 + wave * 32 + rr;
   const bool valid = h < it.h_end;
   // the softmax works on raw scores times a positive factor: a negative scale negates the query, a
   // zero one becomes 1e-30 (scores round to 0, masked ones stay -inf)
@@ -218,17 +209,16 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   int b = it.b >= 0 ? it.b : batch_guess(a, row);
   Seq seq = it.b >= 0 ? it.seq : seq_of(a, b);
   asm volatile("" ::: "memory");
-  uint4 qf[QF];
+  uint4 qf[KSN];   // the latent part; the rotary part stays in LDS
   uint8_t* const qs = L.own_nope[wave];
-  const int hb = it.h0 + rb * 32;
+  const int hb = it.h0 + wave * 32;
   if (hb < it.h_end) stage_q<D>(a.q, hb, min(32, it.h_end - hb), qs, lane);
   auto flipped = [&](uint4 v) { return make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip); };
-  constexpr int NQR = QLDS ? 4 : KSH - KNH;
-  uint4 qrv[NQR];
+  uint4 qrv[4];
   {
-    const uint16_t* qr = a.qr + (int64_t)(valid ? h : it.h_end - 1) * DR + (QLDS ? 0 : kh * 16) + kg * 8;
+    const uint16_t* qr = a.qr + (int64_t)(valid ? h : it.h_end - 1) * DR + kg * 8;
 #pragma unroll
-    for (int j = 0; j < NQR; ++j) qrv[j] = ldg16(qr + j * (QLDS ? 1 : KSPL) * 16);
+    for (int j = 0; j < 4; ++j) qrv[j] = ldg16(qr + j * 16);
   }
 
   // ---- this head row's tokens: a row that sees none of the item's is dead: it runs along unmasked
@@ -252,22 +242,21 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
     wait_vmcnt<0>();   // Q
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int j = 0; j < QF; ++j) qf[j] = j < KNH ? flipped(staged_q<D>(qs, j * KSPL + kh, rr, kg)) : flipped(qrv[j - KNH < NQR ? j - KNH : 0]);
+    for (int j = 0; j < KSN; ++j) qf[j] = flipped(staged_q<D>(qs, j, rr, kg));
     __syncthreads();   // every wave has its Q: the staging area becomes the ring
-    if constexpr (QLDS)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<uint4*>(L.qr + (rb * 32 + rr) * (DR + 8) + j * 16 + kg * 8) = flipped(qrv[j]);
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<uint4*>(L.qr + (wave * 32 + rr) * (DR + 8) + j * 16 + kg * 8) = flipped(qrv[j]);
     mx = max(max(L.red[0][0], L.red[0][1]), max(L.red[0][2], L.red[0][3]));
     mn = min(min(L.red[1][0], L.red[1][1]), min(L.red[1][2], L.red[1][3]));
     hi = __builtin_amdgcn_readfirstlane(mx);        // end of the item's tokens
     min_lim = __builtin_amdgcn_readfirstlane(mn);   // from here on some row is masked
   }
   const bool direct = a.slots == 1;
-  const bool writer = kh == 0 && lane < 32 && valid;   // one lane per head row
+  const bool writer = lane < 32 && valid;   // one lane per head row
   if (hi <= it.t_lo) {   // no row sees any token
     if (direct) {
-      for (int i = threadIdx.x; i < 32 * MT * (D / 8); i += NWV * 64) {
+      for (int i = threadIdx.x; i < 128 * (D / 8); i += NWV * 64) {
         const int hr = it.h0 + i / (D / 8);
         if (hr < it.h_end) stg16(a.out + (int64_t)hr * D + (i % (D / 8)) * 8, make_uint4(0, 0, 0, 0));
       }
@@ -366,18 +355,16 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   // i % 8: the order of the B operand of the PV product. Operands are read KPF steps ahead; `spread(j)`
   // issues what rides on step j, `pre()` what covers the first operands' latency.
   const int tk = 16 * (rr >> 4) + 8 * ((rr >> 2) & 1) + 4 * ((rr >> 3) & 1) + (rr & 3);
-  constexpr int KPF = KSH < 5 ? KSH : 5;
+  constexpr int KPF = 5;
   auto s_tile = [&](int u, auto&& spread, auto&& pre) __attribute__((always_inline)) -> f32x16 {
-    const uint8_t* arow = L.nope[u % NBUF] + nope_off<D>(tk) + kg * 16 + kh * 32;
-    const uint8_t* rrow = L.rope[u % NBUF] + rope_off(tk, kh * 2 + kg);
+    const uint8_t* arow = L.nope[u % NBUF] + nope_off<D>(tk) + kg * 16;
+    const uint8_t* rrow = L.rope[u % NBUF] + rope_off(tk, kg);
     auto a_frag = [&](int j) -> uint4 {
-      return j < KNH ? *reinterpret_cast<const uint4*>(arow + j * KSPL * 32)
-                     : *reinterpret_cast<const uint4*>(rrow + (j - KNH) * KSPL * 256);
+      return j < KSN ? *reinterpret_cast<const uint4*>(arow + j * 32) : *reinterpret_cast<const uint4*>(rrow + (j - KSN) * 256);
     };
-    constexpr int NR = QLDS ? KSH - KNH : 1;
-    uint4 qr[NR];
+    uint4 qr[KS - KSN];
     auto qr_frag = [&](int j) -> uint4 {
-      return *reinterpret_cast<const uint4*>(L.qr + (rb * 32 + rr) * (DR + 8) + j * 16 + kg * 8);
+      return *reinterpret_cast<const uint4*>(L.qr + (wave * 32 + rr) * (DR + 8) + j * 16 + kg * 8);
     };
     uint4 af[KPF];
 #pragma unroll
@@ -385,41 +372,17 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
     pre();
     f32x16 acc;
 #pragma unroll
-    for (int j = 0; j < KSH; ++j) {
-      uint4 bq;
-      if constexpr (QLDS) bq = j < KNH ? qf[j < QF ? j : 0] : qr[j >= KNH ? j - KNH : 0];
-      else bq = qf[j];
+    for (int j = 0; j < KS; ++j) {
+      const uint4 bq = j < KSN ? qf[j < KSN ? j : 0] : qr[j >= KSN ? j - KSN : 0];
       if (j == 0) acc = mfma32_vacc_first<IO>(af[0], bq);
-      else if (j < KSH - 1) mfma32_vacc<IO>(acc, af[j % KPF], bq);
+      else if (j < KS - 1) mfma32_vacc<IO>(acc, af[j % KPF], bq);
       else acc = mfma32_vacc_last_to<IO>(acc, af[j % KPF], bq);
-      if (j + KPF < KSH) af[j % KPF] = a_frag(j + KPF);
-      if constexpr (QLDS)
-        if (j + KPF < KSH && j + KPF >= KNH) qr[j + KPF - KNH] = qr_frag(j + KPF - KNH);
+      if (j + KPF < KS) af[j % KPF] = a_frag(j + KPF);
+      if (j + KPF < KS && j + KPF >= KSN) qr[j + KPF - KSN] = qr_frag(j + KPF - KSN);
       spread(j);
       __builtin_amdgcn_sched_barrier(0);
     }
     return acc;
-  };
-  // several waves of a row block add their parts in one order: the same bits in each
-  auto put_part = [&](const f32x16& sv) __attribute__((always_inline)) {
-#pragma unroll
-    for (int g = 0; g < 4; ++g)
-      *reinterpret_cast<float4*>(&L.x[wave][(g * 64 + lane) * 4]) =
-          make_float4(sv[4 * g], sv[4 * g + 1], sv[4 * g + 2], sv[4 * g + 3]);
-  };
-  auto sum_parts = [&]() __attribute__((always_inline)) -> f32x16 {
-    f32x16 sv;
-#pragma unroll
-    for (int w = 0; w < KSPL; ++w)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const float4 p = *reinterpret_cast<const float4*>(&L.x[rb + MT * w][(g * 64 + lane) * 4]);
-        sv[4 * g] = w == 0 ? p.x : sv[4 * g] + p.x;
-        sv[4 * g + 1] = w == 0 ? p.y : sv[4 * g + 1] + p.y;
-        sv[4 * g + 2] = w == 0 ? p.z : sv[4 * g + 2] + p.z;
-        sv[4 * g + 3] = w == 0 ? p.w : sv[4 * g + 3] + p.w;
-      }
-    return sv;
   };
   auto mask = [&](int u, f32x16& sv) __attribute__((always_inline)) {
     const int t0 = it.t_lo + u * BN;
@@ -484,11 +447,10 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   // tile's first operands, resident since the barrier before.
   const int g16 = lane >> 4, c16 = lane & 15;
   // (tok0 has bit 2 clear: four tokens on is 4 ROW + 16 bytes on)
-  const int vlane = nope_off<D>((g16 >> 1) * 8 + (c16 >> 2)) + ((g16 & 1) * 16 + 4 * (c16 & 3)) * 2 + kh * (D / KSPL) * 2;
+  const int vlane = nope_off<D>((g16 >> 1) * 8 + (c16 >> 2)) + ((g16 & 1) * 16 + 4 * (c16 & 3)) * 2;
   constexpr int NPV = 2 * ON;
   constexpr int VR = NPV < 8 ? NPV : 8;
-  constexpr int NPRE = NPV >= 16 ? 6 : NPV / 4;                       // before the next tile's S^T
-  constexpr int NMID = KSPL > 1 ? NPRE + (NPV - NPRE) / 2 : NPRE;     // before its partial sums are read
+  constexpr int NPRE = NPV >= 16 ? 6 : NPV / 4;   // before the next tile's S^T
   uint4 vb[VR];
   auto v_base = [&](int u) __attribute__((always_inline)) -> uint32_t {
     uint32_t b = lds_addr(L.nope[u % NBUF]) + vlane;
@@ -517,11 +479,6 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   lds_barrier();
   {
     f32x16 s0 = s_tile(0, [](int) {}, [] {});
-    if constexpr (KSPL > 1) {
-      put_part(s0);
-      lds_barrier();
-      s0 = sum_parts();
-    }
     mask(0, s0);
 #pragma unroll
     for (int st = 0; st < NST; ++st) smx(st, s0);
@@ -547,24 +504,18 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
         t + 1,
         [&](int ks) __attribute__((always_inline)) {
           static_for<0, C::GPW>([&](auto j) __attribute__((always_inline)) {
-            if (j * KSH / C::GPW == ks) {
+            if (j * KS / C::GPW == ks) {
               if constexpr (j < C::GPW - 1) gather_part(j, src, gnope, grope);
               else ids_dma(t + 4);   // the slot of tile t's ids, read two iterations ago
             }
           });
         },
         [&]() __attribute__((always_inline)) { pv_run(0, NPRE, vbase, vnext, true, [](int) {}); });
-    if constexpr (KSPL > 1) {
-      put_part(s1);
-      pv_run(NPRE, NMID, vbase, vnext, true, [](int) {});
-      lds_barrier();
-      s1 = sum_parts();
-    }
     mask(t + 1, s1);
-    pv_run(NMID, NPV, vbase, vnext, true, [&](int m) __attribute__((always_inline)) {
+    pv_run(NPRE, NPV, vbase, vnext, true, [&](int m) __attribute__((always_inline)) {
 #pragma unroll
       for (int st = 0; st < NST; ++st)
-        if (st * (NPV - NMID) / NST == m - NMID) smx(st, s1);
+        if (st * (NPV - NPRE) / NST == m - NPRE) smx(st, s1);
     });
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -587,7 +538,7 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   }
   if (!direct) {
     if (!valid || dead) return;
-    float4* dst = it.part + ((int64_t)rb * (D / 8) + kh * (ON * 4)) * 64 + lane;
+    float4* dst = it.part + (int64_t)wave * (D / 8) * 64 + lane;
 #pragma unroll
     for (int n = 0; n < ON; ++n)
 #pragma unroll
@@ -598,7 +549,7 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   // two exchanges between lane halves leave lanes 0-31 with columns [0, 8) and [16, 24) of a 32-column
   // tile, the others with [8, 16) and [24, 32): 16-byte stores
   const float inv = 1.f / l_tot;
-  uint16_t* dst = a.out + (int64_t)(valid ? h : 0) * D + kh * (D / KSPL) + 8 * kg;
+  uint16_t* dst = a.out + (int64_t)(valid ? h : 0) * D + 8 * kg;
 #pragma unroll
   for (int n = 0; n < ON; ++n) {
     uint32_t d[4][2];
@@ -619,15 +570,21 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   }
 }
 
-// 32 head rows: the waves split the tokens. A wave's tile is loaded, then used, so its own loads and
-// products do not overlap; the four waves' do, with up to four tiles (147 KB at D = 512) under way on a
-// CU, which a ring shared by the waves (one tile ahead of two barriers a tile) did not reach.
-template <int IO, int D>
+// 32 or 64 head rows (MT = 1, 2 blocks): the waves split the tokens, NG = 4 / MT groups taking every NG-th
+// tile, each wave with all of the contraction and of the columns of its row block.
+//  * MT = 1: a wave's tile is loaded, then used, without a barrier; the four waves' loads and products
+//    overlap, with up to four tiles (147 KB at D = 512) under way on a CU.
+//  * MT = 2: the two waves of a group share its tile, each copying half of the next one into a second buffer
+//    while they use this one: a barrier a tile. (Four waves on one tile, the contraction split and summed
+//    through LDS, took 3285 cycles per 32 tokens, as long as 128 head rows do.)
+template <int IO, int D, int MT>
 __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds<D>& L) {
   constexpr int KSN = D / 16, KS = (D + DR) / 16, ON = D / 32, ROW = D * 2;
+  constexpr int NG = NWV / MT, OWN = BN / MT;   // token groups; tokens of a tile that a wave copies
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rb = wave % MT, grp = wave / MT;
   const int kg = lane >> 5, rr = lane & 31;
-  const int h = it.h0 + rr;
+  const int hb = it.h0 + rb * 32, h = hb + rr;
   const bool valid = h < it.h_end;
   const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;   // scale: see run_item
   const float cpos = a.scale > 0.f ? a.scale : a.scale < 0.f ? -a.scale : 1e-30f;
@@ -637,9 +594,7 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
   int b = it.b >= 0 ? it.b : batch_guess(a, row);
   Seq seq = it.b >= 0 ? it.seq : seq_of(a, b);
   asm volatile("" ::: "memory");
-  uint8_t* const nope = L.own_nope[wave];
-  uint8_t* const rope = L.own_rope[wave];
-  stage_q<D>(a.q, it.h0, min(32, it.h_end - it.h0), nope, lane);   // each wave for itself
+  if (hb < it.h_end) stage_q<D>(a.q, hb, min(32, it.h_end - hb), L.own_nope[wave], lane);   // each wave for itself
   uint4 qf[KS];
   {
     const uint16_t* qr = a.qr + (int64_t)(valid ? h : it.h_end - 1) * DR + kg * 8;
@@ -658,14 +613,30 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
       mx = max(mx, __shfl_xor(mx, o));
       mn = min(mn, __shfl_xor(mn, o));
     }
+    wait_vmcnt<0>();   // Q
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < KS; ++j) {
+      if (j < KSN) qf[j] = staged_q<D>(L.own_nope[wave], j, rr, kg);
+      qf[j] = make_uint4(qf[j].x ^ flip, qf[j].y ^ flip, qf[j].z ^ flip, qf[j].w ^ flip);
+    }
+    if constexpr (MT > 1) {
+      if (lane == 0) {
+        L.red[0][wave] = mx;
+        L.red[1][wave] = mn;
+      }
+      __syncthreads();   // (and every wave has its Q: the staging area becomes the tiles' buffers)
+      mx = max(L.red[0][0], L.red[0][1]);
+      mn = min(L.red[1][0], L.red[1][1]);
+    }
     hi = __builtin_amdgcn_readfirstlane(mx);
     min_lim = __builtin_amdgcn_readfirstlane(mn);
   }
   const bool direct = a.slots == 1;
-  const bool writer = wave == 0 && lane < 32 && valid;
+  const bool writer = grp == 0 && lane < 32 && valid;
   if (hi <= it.t_lo) {   // no row sees any token (every wave finds the same)
     if (direct) {
-      for (int i = threadIdx.x; i < 32 * (D / 8); i += NWV * 64) {
+      for (int i = threadIdx.x; i < 32 * MT * (D / 8); i += NWV * 64) {
         const int hr = it.h0 + i / (D / 8);
         if (hr < it.h_end) stg16(a.out + (int64_t)hr * D + (i % (D / 8)) * 8, make_uint4(0, 0, 0, 0));
       }
@@ -678,12 +649,15 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
   const int ntiles = (hi - it.t_lo + BN - 1) / BN;
 
   auto page_of = [&](int t) { return (int)(((uint64_t)(uint32_t)t * a.page_mul) >> (31 + a.page_shift)); };
-  auto token = [&](int u) { return min(it.t_lo + u * BN + rr, hi - 1); };   // tokens past the end: the last one
+  // the token that this lane looks up; tokens past the end: the last one, tiles past the end: the last tile
+  auto token = [&](int u) { return min(it.t_lo + min(u, ntiles - 1) * BN + rb * OWN + (lane & (OWN - 1)), hi - 1); };
   auto block_id = [&](int u) {
-    const int t = token(min(u, ntiles - 1));
+    const int t = token(u);
     return a.table[(t < a.prefix || it.b < 0 ? 0 : (int64_t)it.b * a.max_blocks) + page_of(t)];
   };
-  const uint32_t nope_lds = __builtin_amdgcn_readfirstlane(lds_addr(nope));
+  // the group's buffers: one (MT = 1), or two in turn
+  const uint32_t nope_lds = __builtin_amdgcn_readfirstlane(lds_addr(L.own_nope[grp * MT]));
+  const uint32_t rope_lds = __builtin_amdgcn_readfirstlane(lds_addr(L.own_rope[grp * MT]));
 
   {
     float agpr_hint = 0.f;
@@ -705,88 +679,117 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
   const uint32_t k_at = nope_lds + tk * ROW + ((kg ^ kv_swz(tk & 15)) << 4);
   const uint32_t v_lo = nope_lds + t4 * ROW + ((vc ^ kv_swz(t4)) << 4) + (c16 & 1) * 8;
   const uint32_t v_hi = nope_lds + (t4 + 4) * ROW + ((vc ^ kv_swz(t4 + 4)) << 4) + (c16 & 1) * 8;
-  auto k_frag = [&](int j) -> uint4 {
-    return j < KSN ? lds_read16_at((k_at ^ ((j & 7) << 5)) + (j >> 3) * 256)
-                   : *reinterpret_cast<const uint4*>(rope + rope_off(tk, (j - KSN) * 2 + kg));
+  const uint32_t r_at = rope_lds + rope_off(tk, kg);
+  struct Base {
+    uint32_t k, r, lo, hi;
   };
-  auto v_frag = [&](int m) -> uint4 {
+  // the lane's addresses in a buffer, opaque to the compiler: it would keep each of their combinations with
+  // the constants in a register of its own
+  auto base_of = [&](uint32_t buf) __attribute__((always_inline)) -> Base {
+    Base b{k_at + buf * (BN * ROW), r_at + buf * (BN * DR * 2), v_lo + buf * (BN * ROW), v_hi + buf * (BN * ROW)};
+    asm volatile("" : "+v"(b.k), "+v"(b.r), "+v"(b.lo), "+v"(b.hi));
+    return b;
+  };
+  auto k_frag = [&](int j, const Base& b) __attribute__((always_inline)) -> uint4 {
+    return lds_read16_at(j < KSN ? (b.k ^ ((j & 7) << 5)) + (j >> 3) * 256 : b.r + (j - KSN) * 256);
+  };
+  auto v_frag = [&](int m, const Base& b) __attribute__((always_inline)) -> uint4 {
     const int n = m % ON, off = (m / ON) * 16 * ROW + (n >> 2) * 256;
-    const uint2 lo = ds_read_tr_at((v_lo ^ ((n & 3) << 6)) + off), hi2 = ds_read_tr_at((v_hi ^ ((n & 3) << 6)) + off);
+    const uint2 lo = ds_read_tr_at((b.lo ^ ((n & 3) << 6)) + off), hi2 = ds_read_tr_at((b.hi ^ ((n & 3) << 6)) + off);
     return make_uint4(lo.x, lo.y, hi2.x, hi2.y);
   };
-
-  int32_t id = wave < ntiles ? block_id(wave) : 0;
-  wait_vmcnt<0>();   // Q
-  asm volatile("" ::: "memory");
+  // this wave's part of tile u to buffer buf: lane l holds where token OWN rb + l % OWN lies
+  auto load_tile = [&](int u, int32_t id, uint32_t buf) __attribute__((always_inline)) {
+    const int t = token(u);
+    const bool ok = (uint32_t)id < a.blocks;
+    const int row = id * a.page + (t - page_of(t) * a.page);
+    const uint16_t* zero = reinterpret_cast<const uint16_t*>(g_zero_row);
+    const uint64_t p = (uint64_t)(ok ? a.k + (int64_t)row * D : zero);
+    const uint64_t pr = (uint64_t)(ok ? a.kr + (int64_t)row * DR : zero);
+    const uint32_t plo = (uint32_t)p, phi = (uint32_t)(p >> 32), rlo = (uint32_t)pr, rhi = (uint32_t)(pr >> 32);
+    const uint32_t dst = __builtin_amdgcn_readfirstlane(nope_lds + buf * (BN * ROW) + rb * OWN * ROW);
+    const uint32_t rdst = __builtin_amdgcn_readfirstlane(rope_lds + buf * (BN * DR * 2) + rb * (OWN / 8) * 1024);
+    static_for<0, OWN>([&](auto jc) __attribute__((always_inline)) {   // (OWN rb is a multiple of 16: the same permutation)
+      constexpr int j = decltype(jc)::value;
+      const uint64_t src = (uint32_t)__builtin_amdgcn_readlane(plo, j) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(phi, j) << 32;
+      if (lane < D / 8) lds_dma16_at<j * ROW>(src, (lane * 16) ^ (kv_swz(j & 15) << 4), dst);
+    });
 #pragma unroll
-  for (int j = 0; j < KS; ++j) {
-    if (j < KSN) qf[j] = staged_q<D>(nope, j, rr, kg);
-    qf[j] = make_uint4(qf[j].x ^ flip, qf[j].y ^ flip, qf[j].z ^ flip, qf[j].w ^ flip);
+    for (int g = 0; g < OWN / 8; ++g) {   // tokens 8 g + lane % 8, chunk lane / 8
+      const uint32_t lo = __shfl(rlo, 8 * g + (lane & 7)), hi2 = __shfl(rhi, 8 * g + (lane & 7));
+      lds_dma16_untracked((const uint16_t*)(lo | (uint64_t)hi2 << 32) + (lane >> 3) * 8,
+                          (void*)(__attribute__((address_space(3))) void*)(uintptr_t)(rdst + g * 1024));
+    }
+  };
+  // values that are not finite, masked for some rows (see run_item): this wave's tokens of the tile
+  auto sanitize = [&](uint32_t buf) __attribute__((always_inline)) -> uint32_t {
+    uint32_t bad = 0;
+#pragma unroll 1
+    for (int j = rb * OWN; j < rb * OWN + OWN; ++j) {
+      uint4* p = reinterpret_cast<uint4*>(L.own_nope[grp * MT + buf] + j * ROW + (lane % (D / 8)) * 16);
+      uint4 v = *p;
+      bool any = false;
+      constexpr uint32_t EXP = IO == IO_BF16 ? 0x7F80u : 0x7C00u;
+      auto clean = [&](uint32_t w) {
+        if ((w & EXP) == EXP) w &= 0xFFFF0000u, any = true;
+        if (((w >> 16) & EXP) == EXP) w &= 0xFFFFu, any = true;
+        return w;
+      };
+      v = make_uint4(clean(v.x), clean(v.y), clean(v.z), clean(v.w));
+      if (any && lane < D / 8) *p = v;
+      if (__builtin_amdgcn_ballot_w64(any)) bad |= 1u << j;
+    }
+    return bad;
+  };
+
+  // MT = 1: the wave's own tiles only; MT = 2: every wave the same number of turns, for their barriers
+  int32_t id = block_id(grp);
+  if constexpr (MT > 1) {
+    load_tile(grp, id, 0);
+    id = block_id(grp + NG);
   }
-  for (int uv = wave; uv < ntiles; uv += NWV) {
-    const int u = __builtin_amdgcn_readfirstlane(uv);
+  for (int uv = MT > 1 ? 0 : grp; uv < ntiles; uv += NG) {
+    const int u0 = __builtin_amdgcn_readfirstlane(uv);
+    const int u = MT > 1 ? u0 + grp : u0;
+    const uint32_t buf = MT > 1 ? (u0 / NG) & 1 : 0;
     const int t0 = it.t_lo + u * BN;
-    // ---- the tile: lane l holds where token l % 32 lies
-    {
-      const int t = token(u);
-      const bool ok = (uint32_t)id < a.blocks;
-      const int row = id * a.page + (t - page_of(t) * a.page);
-      const uint16_t* zero = reinterpret_cast<const uint16_t*>(g_zero_row);
-      const uint64_t p = (uint64_t)(ok ? a.k + (int64_t)row * D : zero);
-      const uint64_t pr = (uint64_t)(ok ? a.kr + (int64_t)row * DR : zero);
-      const uint32_t plo = (uint32_t)p, phi = (uint32_t)(p >> 32), rlo = (uint32_t)pr, rhi = (uint32_t)(pr >> 32);
+    if constexpr (MT == 1) {
       // the last tile's reads are done (its products waited for them) before this one overwrites it
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      static_for<0, BN>([&](auto jc) __attribute__((always_inline)) {
-        constexpr int j = decltype(jc)::value;
-        const uint64_t src = (uint32_t)__builtin_amdgcn_readlane(plo, j) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(phi, j) << 32;
-        if (lane < D / 8) lds_dma16_at<j * ROW>(src, (lane * 16) ^ (kv_swz(j & 15) << 4), nope_lds);
-      });
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {   // tokens 8 g + lane % 8, chunk lane / 8
-        const uint32_t lo = __shfl(rlo, 8 * g + (lane & 7)), hi2 = __shfl(rhi, 8 * g + (lane & 7));
-        lds_dma16_untracked((const uint16_t*)(lo | (uint64_t)hi2 << 32) + (lane >> 3) * 8, rope + g * 1024);
-      }
+      load_tile(u, id, 0);
+      id = block_id(u + NG);
     }
-    id = block_id(u + NWV);
     wait_vmcnt<0>();
     asm volatile("" ::: "memory");
-    uint32_t bad = 0;
-    if (min_lim < hi && t0 + BN > min_lim) {   // see run_item: values that are not finite, masked for some rows
-#pragma unroll 1
-      for (int j = 0; j < BN; ++j) {
-        uint4* p = reinterpret_cast<uint4*>(nope + j * ROW + (lane % (D / 8)) * 16);
-        uint4 v = *p;
-        bool any = false;
-        constexpr uint32_t EXP = IO == IO_BF16 ? 0x7F80u : 0x7C00u;
-        auto clean = [&](uint32_t w) {
-          if ((w & EXP) == EXP) w &= 0xFFFF0000u, any = true;
-          if (((w >> 16) & EXP) == EXP) w &= 0xFFFFu, any = true;
-          return w;
-        };
-        v = make_uint4(clean(v.x), clean(v.y), clean(v.z), clean(v.w));
-        if (any && lane < D / 8) *p = v;
-        if (__builtin_amdgcn_ballot_w64(any)) bad |= 1u << j;
-      }
+    // (a turn past the end is the last tile again, masked for every row)
+    const bool mixed = (min_lim < hi && t0 + BN > min_lim) || t0 >= hi;
+    uint32_t bad = mixed ? sanitize(buf) : 0;
+    if constexpr (MT > 1) {
+      if (mixed && lane == 0) L.bad[buf][wave] = bad;
+      lds_barrier();   // the tile is here; both waves are done with the other buffer
+      load_tile(u + NG, id, buf ^ 1);
+      id = block_id(u + 2 * NG);
+      if (mixed) bad = L.bad[buf][grp * MT] | L.bad[buf][grp * MT + 1];
     }
     // ---- S^T
     constexpr int KPF = 5;
+    const Base at = base_of(buf);
     uint4 af[KPF];
 #pragma unroll
-    for (int j = 0; j < KPF; ++j) af[j] = k_frag(j);
+    for (int j = 0; j < KPF; ++j) af[j] = k_frag(j, at);
     f32x16 sv;
 #pragma unroll
     for (int j = 0; j < KS; ++j) {
       if (j == 0) sv = mfma32_vacc_first<IO>(af[0], qf[0]);
       else if (j < KS - 1) mfma32_vacc<IO>(sv, af[j % KPF], qf[j]);
       else sv = mfma32_vacc_last_to<IO>(sv, af[j % KPF], qf[j]);
-      if (j + KPF < KS) af[j % KPF] = k_frag(j + KPF);
+      if (j + KPF < KS) af[j % KPF] = k_frag(j + KPF, at);
       __builtin_amdgcn_sched_barrier(0);
     }
     constexpr int VR = 4;
     uint4 vb[VR];
 #pragma unroll
-    for (int m = 0; m < VR; ++m) vb[m] = v_frag(m);
+    for (int m = 0; m < VR; ++m) vb[m] = v_frag(m, at);
     if (bad)
 #pragma unroll
       for (int i = 0; i < 16; ++i)
@@ -825,26 +828,28 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
 #pragma unroll
     for (int m = 0; m < 2 * ON; ++m) {
       o[m % ON] = Mfma<IO>::m32(vb[m % VR], pb[m / ON], o[m % ON]);
-      if (m + VR < 2 * ON) vb[m % VR] = v_frag(m + VR);
+      if (m + VR < 2 * ON) vb[m % VR] = v_frag(m + VR, at);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
 
-  // ---- the waves' outputs joined: each scaled to the common maximum, 128 columns at a time, wave w
-  // adding the four parts of column tile 4 c + w
+  if constexpr (MT > 1) wait_vmcnt<0>();   // the last (unused) loads land before their buffer is used again
+
+  // ---- the groups' outputs joined: each scaled to the common maximum, 128 columns at a time, a wave adding
+  // its row block's parts of MT column tiles
   const float l_wave = add_half_swap(l_part);
   if (lane < 32) L.stat[wave][rr] = make_float4(m_used, m_true, l_wave, 0.f);
-  __syncthreads();   // (also: every wave is done with its tile's buffer)
+  __syncthreads();   // (also: every wave is done with its tiles)
   float M = -INFINITY, top = -INFINITY, l_tot = 0.f;
 #pragma unroll
-  for (int w = 0; w < NWV; ++w) {
-    const float4 st = L.stat[w][rr];
+  for (int g = 0; g < NG; ++g) {
+    const float4 st = L.stat[rb + MT * g][rr];
     M = fmaxf(M, st.x);
     top = fmaxf(top, st.y);
   }
 #pragma unroll
-  for (int w = 0; w < NWV; ++w) {
-    const float4 st = L.stat[w][rr];
+  for (int g = 0; g < NG; ++g) {
+    const float4 st = L.stat[rb + MT * g][rr];
     l_tot += st.x == -INFINITY ? st.z : st.z * __builtin_amdgcn_exp2f((st.x - M) * LOG2E);
   }
   const float f = m_used == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_used - M) * LOG2E);   // (O and l are 0 with -inf)
@@ -869,28 +874,27 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
         L.join[wave][n * 4 + g][lane] = make_float4(v[4 * g] * f, v[4 * g + 1] * f, v[4 * g + 2] * f, v[4 * g + 3] * f);
       }
     __syncthreads();
-    float4 v[4];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      v[g] = L.join[0][wave * 4 + g][lane];
+    for (int k = 0; k < MT; ++k) {
+      const int nt = grp * MT + k, n = 4 * c + nt;
 #pragma unroll
-      for (int w = 1; w < NWV; ++w) {
-        const float4 p = L.join[w][wave * 4 + g][lane];
-        v[g].x += p.x;
-        v[g].y += p.y;
-        v[g].z += p.z;
-        v[g].w += p.w;
+      for (int q = 0; q < 4; ++q) {
+        float4 v = L.join[rb][nt * 4 + q][lane];
+#pragma unroll
+        for (int g = 1; g < NG; ++g) {
+          const float4 p = L.join[rb + MT * g][nt * 4 + q][lane];
+          v.x += p.x;
+          v.y += p.y;
+          v.z += p.z;
+          v.w += p.w;
+        }
+        if (!valid) continue;
+        if (direct)
+          *reinterpret_cast<uint2*>(a.out + (int64_t)h * D + n * 32 + 8 * q + 4 * kg) =
+              dead ? make_uint2(0, 0) : make_uint2(pack2<IO>(v.x * inv, v.y * inv), pack2<IO>(v.z * inv, v.w * inv));
+        else if (!dead)
+          it.part[((int64_t)rb * (D / 8) + n * 4 + q) * 64 + lane] = v;
       }
-    }
-    if (!valid) continue;
-    const int n = 4 * c + wave;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      if (direct)
-        *reinterpret_cast<uint2*>(a.out + (int64_t)h * D + n * 32 + 8 * g + 4 * kg) =
-            dead ? make_uint2(0, 0) : make_uint2(pack2<IO>(v[g].x * inv, v[g].y * inv), pack2<IO>(v[g].z * inv, v[g].w * inv));
-      else if (!dead)
-        it.part[(n * 4 + g) * 64 + lane] = v[g];
     }
   }
 }
@@ -946,9 +950,9 @@ __global__ __launch_bounds__(NWV * 64) void prefix_attn_kernel(PfxK a) {
     it.t_hi = sp == a.o_splits - 1 ? INT_MAX : it.t_lo + a.o_chunk;
     it.slot = a.p_splits + sp;
   }
-  if (mt == 1) run_tokens<IO, D>(a, it, L);
-  else if (mt == 2) run_item<IO, D, 2>(a, it, L);
-  else run_item<IO, D, 4>(a, it, L);
+  if (mt == 1) run_tokens<IO, D, 1>(a, it, L);
+  else if (mt == 2) run_tokens<IO, D, 2>(a, it, L);
+  else run_item<IO, D>(a, it, L);
 }
 
 constexpr int MAX_SLOTS = 256;

@@ -21,8 +21,8 @@ def test_chains_never_touched_in_flight(tmp_path):
     lines = asm.read_text().splitlines()
     chains, bad = chain_violations(lines)
     found = {n: c for n, c in chains_by_kernel(lines).items() if "prefix_attn_kernel" in n}
-    # per type and D: 128 and 64 head rows, each with the first tile's chain and the loop's, and 32 with one
-    assert len(found) == 6 and min(found.values()) >= 5 and sum(found.values()) == chains
+    # per type and D: 128 head rows with the first tile's chain and the loop's, 64 and 32 with one each
+    assert len(found) == 6 and min(found.values()) >= 4 and sum(found.values()) == chains
     assert not bad, f"accumulator touched while its chain is in flight: {bad[:5]}"
     # every direct-to-LDS load takes its LDS address from a scalar register
     assert not [l for l in lines if re.search(r"s_mov_b32 m0, v", l)]
