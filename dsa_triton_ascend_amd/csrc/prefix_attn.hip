@@ -698,27 +698,33 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
     const uint2 lo = ds_read_tr_at((b.lo ^ ((n & 3) << 6)) + off), hi2 = ds_read_tr_at((b.hi ^ ((n & 3) << 6)) + off);
     return make_uint4(lo.x, lo.y, hi2.x, hi2.y);
   };
-  // this wave's part of tile u to buffer buf: lane l holds where token OWN rb + l % OWN lies
-  auto load_tile = [&](int u, int32_t id, uint32_t buf) __attribute__((always_inline)) {
+  // This wave's part of tile u to buffer buf, in OWN + OWN / 8 loads: lane l holds where token OWN rb + l % OWN
+  // lies (a missing block: zeros).
+  struct Source {
+    uint32_t lo, hi, rlo, rhi, dst, rdst;
+  };
+  auto source_of = [&](int u, int32_t id, uint32_t buf) __attribute__((always_inline)) -> Source {
     const int t = token(u);
     const bool ok = (uint32_t)id < a.blocks;
     const int row = id * a.page + (t - page_of(t) * a.page);
     const uint16_t* zero = reinterpret_cast<const uint16_t*>(g_zero_row);
     const uint64_t p = (uint64_t)(ok ? a.k + (int64_t)row * D : zero);
     const uint64_t pr = (uint64_t)(ok ? a.kr + (int64_t)row * DR : zero);
-    const uint32_t plo = (uint32_t)p, phi = (uint32_t)(p >> 32), rlo = (uint32_t)pr, rhi = (uint32_t)(pr >> 32);
-    const uint32_t dst = __builtin_amdgcn_readfirstlane(nope_lds + buf * (BN * ROW) + rb * OWN * ROW);
-    const uint32_t rdst = __builtin_amdgcn_readfirstlane(rope_lds + buf * (BN * DR * 2) + rb * (OWN / 8) * 1024);
-    static_for<0, OWN>([&](auto jc) __attribute__((always_inline)) {   // (OWN rb is a multiple of 16: the same permutation)
-      constexpr int j = decltype(jc)::value;
-      const uint64_t src = (uint32_t)__builtin_amdgcn_readlane(plo, j) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(phi, j) << 32;
-      if (lane < D / 8) lds_dma16_at<j * ROW>(src, (lane * 16) ^ (kv_swz(j & 15) << 4), dst);
-    });
-#pragma unroll
-    for (int g = 0; g < OWN / 8; ++g) {   // tokens 8 g + lane % 8, chunk lane / 8
-      const uint32_t lo = __shfl(rlo, 8 * g + (lane & 7)), hi2 = __shfl(rhi, 8 * g + (lane & 7));
+    return {(uint32_t)p, (uint32_t)(p >> 32), (uint32_t)pr, (uint32_t)(pr >> 32),
+            (uint32_t)__builtin_amdgcn_readfirstlane(nope_lds + buf * (BN * ROW) + rb * OWN * ROW),
+            (uint32_t)__builtin_amdgcn_readfirstlane(rope_lds + buf * (BN * DR * 2) + rb * (OWN / 8) * 1024)};
+  };
+  constexpr int NLD = OWN + OWN / 8;
+  auto load_part = [&](auto jc, const Source& s) __attribute__((always_inline)) {
+    constexpr int j = decltype(jc)::value;
+    if constexpr (j < OWN) {   // (OWN rb is a multiple of 16: the same permutation for every wave)
+      const uint64_t src = (uint32_t)__builtin_amdgcn_readlane(s.lo, j) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(s.hi, j) << 32;
+      if (lane < D / 8) lds_dma16_at<j * ROW>(src, (lane * 16) ^ (kv_swz(j & 15) << 4), s.dst);
+    } else {   // tokens 8 g + lane % 8, chunk lane / 8
+      constexpr int g = j - OWN;
+      const uint32_t lo = __shfl(s.rlo, 8 * g + (lane & 7)), hi2 = __shfl(s.rhi, 8 * g + (lane & 7));
       lds_dma16_untracked((const uint16_t*)(lo | (uint64_t)hi2 << 32) + (lane >> 3) * 8,
-                          (void*)(__attribute__((address_space(3))) void*)(uintptr_t)(rdst + g * 1024));
+                          (void*)(__attribute__((address_space(3))) void*)(uintptr_t)(s.rdst + g * 1024));
     }
   };
   // values that are not finite, masked for some rows (see run_item): this wave's tokens of the tile
@@ -745,7 +751,8 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
   // MT = 1: the wave's own tiles only; MT = 2: every wave the same number of turns, for their barriers
   int32_t id = block_id(grp);
   if constexpr (MT > 1) {
-    load_tile(grp, id, 0);
+    const Source src = source_of(grp, id, 0);
+    static_for<0, NLD>([&](auto j) __attribute__((always_inline)) { load_part(j, src); });
     id = block_id(grp + NG);
   }
   for (int uv = MT > 1 ? 0 : grp; uv < ntiles; uv += NG) {
@@ -753,10 +760,12 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
     const int u = MT > 1 ? u0 + grp : u0;
     const uint32_t buf = MT > 1 ? (u0 / NG) & 1 : 0;
     const int t0 = it.t_lo + u * BN;
+    Source src;
     if constexpr (MT == 1) {
       // the last tile's reads are done (its products waited for them) before this one overwrites it
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      load_tile(u, id, 0);
+      src = source_of(u, id, 0);
+      static_for<0, NLD>([&](auto j) __attribute__((always_inline)) { load_part(j, src); });
       id = block_id(u + NG);
     }
     wait_vmcnt<0>();
@@ -767,8 +776,7 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
     if constexpr (MT > 1) {
       if (mixed && lane == 0) L.bad[buf][wave] = bad;
       lds_barrier();   // the tile is here; both waves are done with the other buffer
-      load_tile(u + NG, id, buf ^ 1);
-      id = block_id(u + 2 * NG);
+      src = source_of(u + NG, id, buf ^ 1);
       if (mixed) bad = L.bad[buf][grp * MT] | L.bad[buf][grp * MT + 1];
     }
     // ---- S^T
@@ -784,8 +792,13 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
       else if (j < KS - 1) mfma32_vacc<IO>(sv, af[j % KPF], qf[j]);
       else sv = mfma32_vacc_last_to<IO>(sv, af[j % KPF], qf[j]);
       if (j + KPF < KS) af[j % KPF] = k_frag(j + KPF, at);
+      if constexpr (MT > 1)   // the next tile's loads ride on the chain
+        static_for<0, NLD>([&](auto i) __attribute__((always_inline)) {
+          if (i * KS / NLD == j) load_part(i, src);
+        });
       __builtin_amdgcn_sched_barrier(0);
     }
+    if constexpr (MT > 1) id = block_id(u + 2 * NG);
     constexpr int VR = 4;
     uint4 vb[VR];
 #pragma unroll
