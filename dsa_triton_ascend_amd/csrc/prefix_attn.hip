@@ -203,6 +203,18 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   const float cpos = a.scale > 0.f ? a.scale : a.scale < 0.f ? -a.scale : 1e-30f;
   const float cl2 = cpos * LOG2E;
 
+  // ---- block ids of the first tiles, requested before the item's end is known. Wave w copies tokens 8 w ..
+  // 8 w + 7 of each tile; their block ids travel the same ordered path four tiles ahead, so nothing waits for
+  // them. Tokens past the end (and tiles: every wave issues the same GPW loads per tile) read zeros.
+  auto token = [&](int u) { return it.t_lo + u * BN + wave * 8 + (lane & 7); };
+  auto page_of = [&](int t) { return (int)(((uint64_t)(uint32_t)t * a.page_mul) >> (31 + a.page_shift)); };
+  auto ids_dma = [&](int u) __attribute__((always_inline)) {
+    const int t = min(token(u), a.s2 - 1);
+    const int32_t* src = a.table + (t < a.prefix || it.b < 0 ? 0 : (int64_t)it.b * a.max_blocks) + page_of(t);
+    if (lane < 8) lds_dma4_untracked(src, &L.ids[u & 3][wave * 8]);
+  };
+#pragma unroll
+  for (int u = 0; u < 4; ++u) ids_dma(u);
   // ---- this head row's sequence, requested first; then Q^T fragments (B operand: this lane's head row, 8
   // values at 16 ks + 8 kg), through LDS
   const int row = (valid ? h : it.h_end - 1) >> a.n1_shift;
@@ -239,7 +251,7 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
       L.red[0][wave] = mx;
       L.red[1][wave] = mn;
     }
-    wait_vmcnt<0>();   // Q
+    wait_vmcnt<0>();   // Q and the first ids
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int j = 0; j < KSN; ++j) qf[j] = flipped(staged_q<D>(qs, j, rr, kg));
@@ -268,16 +280,6 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   }
   const int ntiles = (hi - it.t_lo + BN - 1) / BN;
 
-  // ---- ids and gathers. Wave w copies tokens 8 w .. 8 w + 7 of each tile; their block ids travel the
-  // same ordered path four tiles ahead, so nothing waits for them. Tokens past the end repeat the last
-  // one, tiles past the end the last tile: every wave issues the same GPW loads per tile.
-  auto token = [&](int u) { return min(it.t_lo + min(u, ntiles - 1) * BN + wave * 8 + (lane & 7), hi - 1); };
-  auto page_of = [&](int t) { return (int)(((uint64_t)(uint32_t)t * a.page_mul) >> (31 + a.page_shift)); };
-  auto ids_dma = [&](int u) __attribute__((always_inline)) {
-    const int t = token(u);
-    const int32_t* src = a.table + (t < a.prefix || it.b < 0 ? 0 : (int64_t)it.b * a.max_blocks) + page_of(t);
-    if (lane < 8) lds_dma4_untracked(src, &L.ids[u & 3][wave * 8]);
-  };
   // where the latent and the rotary part of token 8 w + lane % 8 of tile u lie (a missing block: zeros)
   struct Source {
     uint32_t lo, hi;
@@ -286,7 +288,7 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   auto tile_rows = [&](int u) __attribute__((always_inline)) -> Source {
     const int t = token(u);
     const int32_t id = L.ids[u & 3][wave * 8 + (lane & 7)];
-    const bool ok = (uint32_t)id < a.blocks;
+    const bool ok = (uint32_t)id < a.blocks && t < hi;
     const int row = id * a.page + (t - page_of(t) * a.page);
     const uint16_t* zero = reinterpret_cast<const uint16_t*>(g_zero_row);
     const uint64_t p = (uint64_t)(ok ? a.k + (int64_t)row * D : zero);
@@ -330,10 +332,6 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
     }
     if (lane == 0) L.bad[u & 1][wave] = bad;
   };
-#pragma unroll
-  for (int u = 0; u < 4; ++u) ids_dma(u);
-  wait_vmcnt<0>();
-  asm volatile("" ::: "memory");
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const Source src = tile_rows(u);
@@ -590,6 +588,15 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
   const float cpos = a.scale > 0.f ? a.scale : a.scale < 0.f ? -a.scale : 1e-30f;
   const float cl2 = cpos * LOG2E;
 
+  // the token that this lane looks up, its block requested before the item's end is known (tokens past it,
+  // and tiles, read zeros)
+  auto page_of = [&](int t) { return (int)(((uint64_t)(uint32_t)t * a.page_mul) >> (31 + a.page_shift)); };
+  auto token = [&](int u) { return it.t_lo + u * BN + rb * OWN + (lane & (OWN - 1)); };
+  auto block_id = [&](int u) {
+    const int t = min(token(u), a.s2 - 1);
+    return a.table[(t < a.prefix || it.b < 0 ? 0 : (int64_t)it.b * a.max_blocks) + page_of(t)];
+  };
+  int32_t id = block_id(grp);
   const int row = (valid ? h : it.h_end - 1) >> a.n1_shift;
   int b = it.b >= 0 ? it.b : batch_guess(a, row);
   Seq seq = it.b >= 0 ? it.seq : seq_of(a, b);
@@ -648,13 +655,6 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
   }
   const int ntiles = (hi - it.t_lo + BN - 1) / BN;
 
-  auto page_of = [&](int t) { return (int)(((uint64_t)(uint32_t)t * a.page_mul) >> (31 + a.page_shift)); };
-  // the token that this lane looks up; tokens past the end: the last one, tiles past the end: the last tile
-  auto token = [&](int u) { return min(it.t_lo + min(u, ntiles - 1) * BN + rb * OWN + (lane & (OWN - 1)), hi - 1); };
-  auto block_id = [&](int u) {
-    const int t = token(u);
-    return a.table[(t < a.prefix || it.b < 0 ? 0 : (int64_t)it.b * a.max_blocks) + page_of(t)];
-  };
   // the group's buffers: one (MT = 1), or two in turn
   const uint32_t nope_lds = __builtin_amdgcn_readfirstlane(lds_addr(L.own_nope[grp * MT]));
   const uint32_t rope_lds = __builtin_amdgcn_readfirstlane(lds_addr(L.own_rope[grp * MT]));
@@ -705,7 +705,7 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
   };
   auto source_of = [&](int u, int32_t id, uint32_t buf) __attribute__((always_inline)) -> Source {
     const int t = token(u);
-    const bool ok = (uint32_t)id < a.blocks;
+    const bool ok = (uint32_t)id < a.blocks && t < hi;
     const int row = id * a.page + (t - page_of(t) * a.page);
     const uint16_t* zero = reinterpret_cast<const uint16_t*>(g_zero_row);
     const uint64_t p = (uint64_t)(ok ? a.k + (int64_t)row * D : zero);
@@ -749,7 +749,6 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
   };
 
   // MT = 1: the wave's own tiles only; MT = 2: every wave the same number of turns, for their barriers
-  int32_t id = block_id(grp);
   if constexpr (MT > 1) {
     const Source src = source_of(grp, id, 0);
     static_for<0, NLD>([&](auto j) __attribute__((always_inline)) { load_part(j, src); });
@@ -770,8 +769,7 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
     }
     wait_vmcnt<0>();
     asm volatile("" ::: "memory");
-    // (a turn past the end is the last tile again, masked for every row)
-    const bool mixed = (min_lim < hi && t0 + BN > min_lim) || t0 >= hi;
+    const bool mixed = min_lim < hi && t0 + BN > min_lim;
     uint32_t bad = mixed ? sanitize(buf) : 0;
     if constexpr (MT > 1) {
       if (mixed && lane == 0) L.bad[buf][wave] = bad;
@@ -1082,18 +1080,19 @@ int mt_for(int64_t head_rows) { return head_rows > 64 ? 4 : head_rows > 32 ? 2 :
 int up(int x, int to) { return (x + to - 1) / to * to; }
 
 // Microseconds of a call by a simple model of what was measured at D = 512 (256 CUs, one item each at a
-// time): an item costs 6 (its rows' sequences, Q, first tile, ends) and 1.55 / 1.3 per 32 tokens for 128 / 64
-// head rows or 3.7 per 128 tokens for 32; partial outputs are written at 7 TB/s, and the join is a launch of
+// time): an item costs 6 (its rows' sequences, Q, first tile, ends) and 1.55 / 0.95 per 32 tokens for 128 / 64
+// head rows or 3.7 per 128 tokens for 32; the latents come at 4.9 TB/s; partial outputs are written at 7 TB/s, and the join is a launch of
 // 6 that reads them at 6 TB/s. It is there to weigh rounds of items against partials: at 64 x 16 heads
 // after 8192 tokens 16 prefix ranges take 50 us, 8 take 70 and 32 take 70 as well.
 struct Model {
   double scale;   // of a tile's products against D = 512
   double item(int mt, int tokens) const {
-    return 6.0 + scale * (mt == 4 ? 1.55 * ((tokens + 31) / 32) : mt == 2 ? 1.3 * ((tokens + 31) / 32) : 3.7 * ((tokens + 127) / 128));
+    return 6.0 + scale * (mt == 4 ? 1.55 * ((tokens + 31) / 32) : mt == 2 ? 0.95 * ((tokens + 31) / 32) : 3.7 * ((tokens + 127) / 128));
   }
 };
 
-double cut_cost(const Model& md, const Cut& c, int d, double own_tiles, int own_max, double own_mean) {
+double cut_cost(const Model& md, const Cut& c, int d, double own_tiles, int own_max, double own_mean,
+                double latents_mb) {
   const double np = (double)c.p_splits * c.p_tiles;
   const double tp = c.p_splits ? md.item(c.p_mt, c.p_chunk) : 0.0;
   const double no = own_tiles * std::min((double)c.o_splits, own_mean / c.o_chunk + (c.o_splits > 1 ? 0.5 : 1.0));
@@ -1103,6 +1102,9 @@ double cut_cost(const Model& md, const Cut& c, int d, double own_tiles, int own_
   const double n = np + no, grid = np + own_tiles * c.o_splits, longest = std::max(tp, to);
   const double mean = (np * tp + no * to) / std::max(n, 1.0);
   double us = longest + (grid > 256.0 ? mean * std::max(std::max(n, 256.0) / 256.0 - 1.0, 0.45) : 0.0);
+  // the later of both, and more where they are near
+  const double hbm = 6.0 + latents_mb / 4.9;
+  us = std::max(us, hbm) + 0.25 * std::min(us, hbm);
   if (c.slots > 1) {
     const double mb = (np * c.p_mt + no * c.o_mt) * 32.0 * d * 4.0 * 1e-6;
     us += mb / 7.0 + 6.0 + mb / 6.0;
@@ -1115,6 +1117,7 @@ Cut make_cut(int batch, int rows, int n1, int d, int prefix, int max_rows, int m
   const int64_t m = (int64_t)rows * n1;
   const double mean = (double)total_kv / batch;
   const Model md{(2 * d + 64) / 1088.0};
+  const double latents_mb = (prefix + std::max(mean - prefix, 0.0) * batch) * (d + 64) * 2e-6;
   Cut c{}, best{};
   double least = 1e300;
   c.o_mt = mt_for((int64_t)max_rows * n1);
@@ -1126,7 +1129,7 @@ Cut make_cut(int batch, int rows, int n1, int d, int prefix, int max_rows, int m
     c.o_chunk = up(std::max((own_max + c.o_splits - 1) / c.o_splits, 1), c.o_mt == 1 ? 4 * BN : BN);
     c.o_splits = std::max(1, (own_max + c.o_chunk - 1) / c.o_chunk);
     c.slots = c.p_splits + c.o_splits;
-    const double us = cut_cost(md, c, d, own_tiles, own_max, own_mean);
+    const double us = cut_cost(md, c, d, own_tiles, own_max, own_mean, latents_mb);
     if (us < least) least = us, best = c;
   };
   auto more = [](int s) { return s < 24 ? 1 : s < 48 ? 4 : 8; };
@@ -1146,7 +1149,7 @@ Cut make_cut(int batch, int rows, int n1, int d, int prefix, int max_rows, int m
     c.p_splits = (prefix + c.p_chunk - 1) / c.p_chunk;
     // own ranges as long as a prefix range takes, or one
     const double fit = md.item(c.p_mt, c.p_chunk) - 6.0;
-    const double per = md.scale * (c.o_mt == 4 ? 1.55 / 32 : c.o_mt == 2 ? 1.3 / 32 : 3.7 / 128);
+    const double per = md.scale * (c.o_mt == 4 ? 1.55 / 32 : c.o_mt == 2 ? 0.95 / 32 : 3.7 / 128);
     consider(own, own_mean, (int)std::ceil(own * per / std::max(fit, per * BN)));
     if (c.o_splits > 1) consider(own, own_mean, 1);
     if (s > 1 && c.p_chunk == gran) break;
