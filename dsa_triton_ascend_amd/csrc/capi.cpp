@@ -532,8 +532,8 @@ int check_rotation(const char* fn, int axes, const int32_t* sections, const floa
 }
 
 int check_append(const char* fn, const void* x, int io_dtype, const void* norm_weight, int w_dtype,
-                 const int32_t* row_start, const int32_t* act_q, const int32_t* act_k, const int32_t* block_table,
-                 int batch, int total_rows, int rows_per_batch, int max_blocks, int page_block_size, int64_t num_blocks,
+                 const int32_t* row_start, const int32_t* act_q, const int32_t* act_k, int lengths_host,
+                 const int32_t* block_table, int batch, int total_rows, int rows_per_batch, int max_blocks, int page_block_size, int64_t num_blocks,
                  const void* cache) {
   if (!x || !row_start || !act_q || !act_k || !block_table || !cache)
     return fail(DSA_ERR_INVALID, "%s: null pointer argument", fn);
@@ -543,6 +543,8 @@ int check_append(const char* fn, const void* x, int io_dtype, const void* norm_w
   if (batch <= 0 || total_rows < 0 || rows_per_batch < 1 || max_blocks <= 0 || page_block_size <= 0 || num_blocks <= 0)
     return fail(DSA_ERR_INVALID, "%s: non-positive shape", fn);
   if (((uintptr_t)cache & 15) != 0) return fail(DSA_ERR_INVALID, "%s: caches must be 16-byte aligned", fn);
+  if (lengths_host && batch > (APPEND_ARG_LENGTHS - 1) / 3)
+    return fail(DSA_ERR_UNSUPPORTED, "%s: host lengths of at most %d sequences, got %d", fn, (APPEND_ARG_LENGTHS - 1) / 3, batch);
   return DSA_OK;
 }
 }  // namespace
@@ -572,11 +574,11 @@ int dsa_latent_append(const void* latent, int64_t batch_stride, int64_t row_stri
                       int64_t rope_batch_stride, int64_t rope_row_stride, int io_dtype, int d, const void* norm_weight,
                       int w_dtype, float eps, const void* positions, int positions_64, int axes, const int32_t* sections,
                       const float* inv_freq, int interleaved, const int32_t* row_start, const int32_t* act_q,
-                      const int32_t* act_k, const int32_t* block_table, int batch, int total_rows, int rows_per_batch,
-                      int max_blocks, int page_block_size, int64_t num_blocks, void* key_cache, void* key_rope_cache,
+                      const int32_t* act_k, int lengths_host, const int32_t* block_table, int batch, int total_rows,
+                      int rows_per_batch, int max_blocks, int page_block_size, int64_t num_blocks, void* key_cache, void* key_rope_cache,
                       void* stream) {
-  int st = check_append("dsa_latent_append", latent, io_dtype, norm_weight, w_dtype, row_start, act_q, act_k, block_table,
-                        batch, total_rows, rows_per_batch, max_blocks, page_block_size, num_blocks, key_cache);
+  int st = check_append("dsa_latent_append", latent, io_dtype, norm_weight, w_dtype, row_start, act_q, act_k,
+                        lengths_host, block_table, batch, total_rows, rows_per_batch, max_blocks, page_block_size, num_blocks, key_cache);
   if (st != DSA_OK) return st;
   if (!key_rope || !key_rope_cache) return fail(DSA_ERR_INVALID, "dsa_latent_append: null pointer argument");
   if (((uintptr_t)key_rope_cache & 15) != 0)
@@ -590,8 +592,8 @@ int dsa_latent_append(const void* latent, int64_t batch_stride, int64_t row_stri
   }
   AppendArgs a{latent, batch_stride, row_stride, 0, io_dtype, 1, d, key_rope, rope_batch_stride, rope_row_stride,
                norm_weight ? 1 : 0, norm_weight, nullptr, w_dtype, eps, positions, positions_64, axes, sections, inv_freq,
-               0, 64, interleaved, row_start, act_q, act_k, block_table, batch, total_rows, rows_per_batch, max_blocks,
-               page_block_size, num_blocks, key_cache, key_rope_cache};
+               0, 64, interleaved, row_start, act_q, act_k, lengths_host, block_table, batch, total_rows,
+               rows_per_batch, max_blocks, page_block_size, num_blocks, key_cache, key_rope_cache};
   return hip_status(launch_cache_append(a, (hipStream_t)stream), "dsa_latent_append launch");
 }
 
@@ -599,10 +601,10 @@ int dsa_index_append(const void* index_key, int64_t batch_stride, int64_t row_st
                      int n2, int w, const void* norm_weight, const void* norm_bias, int w_dtype, float eps,
                      const void* positions, int positions_64, int axes, const int32_t* sections, const float* inv_freq,
                      int rotary_start, int rotary_dim, int interleaved, const int32_t* row_start, const int32_t* act_q,
-                     const int32_t* act_k, const int32_t* block_table, int batch, int total_rows, int rows_per_batch,
-                     int max_blocks, int page_block_size, int64_t num_blocks, void* index_cache, void* stream) {
-  int st = check_append("dsa_index_append", index_key, io_dtype, norm_weight, w_dtype, row_start, act_q, act_k, block_table,
-                        batch, total_rows, rows_per_batch, max_blocks, page_block_size, num_blocks, index_cache);
+                     const int32_t* act_k, int lengths_host, const int32_t* block_table, int batch, int total_rows,
+                     int rows_per_batch, int max_blocks, int page_block_size, int64_t num_blocks, void* index_cache, void* stream) {
+  int st = check_append("dsa_index_append", index_key, io_dtype, norm_weight, w_dtype, row_start, act_q, act_k,
+                        lengths_host, block_table, batch, total_rows, rows_per_batch, max_blocks, page_block_size, num_blocks, index_cache);
   if (st != DSA_OK) return st;
   if (n2 <= 0 || n2 > 65535) return fail(DSA_ERR_INVALID, "dsa_index_append: 1 to 65535 key heads, got %d", n2);
   if (!li_score_supported_d(w))
@@ -619,7 +621,7 @@ int dsa_index_append(const void* index_key, int64_t batch_stride, int64_t row_st
   }
   AppendArgs a{index_key, batch_stride, row_stride, head_stride, io_dtype, n2, w, nullptr, 0, 0, norm_weight ? 2 : 0,
                norm_weight, norm_bias, w_dtype, eps, positions, positions_64, axes, sections, inv_freq, rotary_start,
-               rotary_dim, interleaved, row_start, act_q, act_k, block_table, batch, total_rows, rows_per_batch,
+               rotary_dim, interleaved, row_start, act_q, act_k, lengths_host, block_table, batch, total_rows, rows_per_batch,
                max_blocks, page_block_size, num_blocks, index_cache, nullptr};
   return hip_status(launch_cache_append(a, (hipStream_t)stream), "dsa_index_append launch");
 }

@@ -498,13 +498,14 @@ struct RotaryArgs {
 hipError_t launch_rotary(const RotaryArgs& a, hipStream_t s);
 // New tokens into a paged cache: latents (rope != NULL: normed, beside their rotated rotary keys) or
 // indexer keys (rope NULL: normed and rotated)
+constexpr int APPEND_ARG_LENGTHS = 56;   // lengths_host: 3 batch + 1 values as kernel arguments
 struct AppendArgs {
   const void* x; int64_t batch_stride, row_stride, head_stride; int io; int heads, width;
   const void* rope; int64_t rope_batch_stride, rope_row_stride;
   int norm_kind; const void* norm_w; const void* norm_b; int wdt; float eps;   // 0 none, 1 rms, 2 layer
   const void* positions; int wide; int axes; const int32_t* sections;
   const float* freq; int start, rdim, interleaved;
-  const int32_t* row_start; const int32_t* act_q; const int32_t* act_k; const int32_t* table;
+  const int32_t* row_start; const int32_t* act_q; const int32_t* act_k; int lengths_host; const int32_t* table;
   int batch, total_rows, rows_per_batch, max_blocks, page; int64_t blocks;
   void* cache; void* rope_cache;
 };

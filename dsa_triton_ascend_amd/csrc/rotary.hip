@@ -11,6 +11,7 @@
 // (position 10^5 times a frequency of 1 leaves 2^-7 of a radian in 32-bit arithmetic), so a
 // work-group turns its tokens' angles into a table of (cos, sin) in LDS, shared by all heads.
 #include <algorithm>
+#include <cstring>
 
 #include "dsa_common.hpp"
 
@@ -244,6 +245,24 @@ hipError_t launch_rotary_io(const RotaryK& k, bool inter, hipStream_t s) {
 // us, 8.5 with 4; 18,216 latents 15.1, 15.5 with 16)
 constexpr int APPEND_FEW = 2048;
 
+// The lengths of a call, [row_start | act_q | act_k], from device memory or as a kernel argument (a one-shot
+// call of few sequences: no upload before it)
+struct DeviceLens {
+  const int32_t* row_start;
+  const int32_t* act_q;
+  const int32_t* act_k;
+  __device__ __forceinline__ int rs(int b) const { return row_start[b]; }
+  __device__ __forceinline__ int aq(int b) const { return act_q[b]; }
+  __device__ __forceinline__ int ak(int b) const { return act_k[b]; }
+};
+struct ArgLens {
+  int32_t v[APPEND_ARG_LENGTHS];
+  int batch;
+  __device__ __forceinline__ int rs(int b) const { return v[b]; }
+  __device__ __forceinline__ int aq(int b) const { return v[batch + 1 + b]; }
+  __device__ __forceinline__ int ak(int b) const { return v[2 * batch + 1 + b]; }
+};
+
 struct Norm {
   int kind;   // 0 none, 1 root mean square, 2 mean and variance
   const void* w;
@@ -267,9 +286,6 @@ struct AppendK {
   int inter;
   const float* freq;
   Positions pos;     // pos.p NULL: a token's place in its sequence
-  const int32_t* row_start;
-  const int32_t* act_q;
-  const int32_t* act_k;
   const int32_t* table;
   int batch, total_rows, max_blocks, page, rows_per_batch;
   int64_t blocks;
@@ -357,8 +373,8 @@ __device__ __forceinline__ void rotate_vec(const float2* t, int start, int rdim,
   for (int i = 0; i < 8; ++i) x[i] = low ? x[i] * t[i].x - y[i] * t[i].y : y[i] * t[i].y + x[i] * t[i].x;
 }
 
-template <int IO, int LPV, bool LATENT, int NTOK>
-__global__ __launch_bounds__(TPB) void append_kernel(AppendK a) {
+template <int IO, int LPV, bool LATENT, int NTOK, typename Lens>
+__global__ __launch_bounds__(TPB) void append_kernel(AppendK a, Lens lens) {
   extern __shared__ float2 tab[];   // [NTOK][rdim / 2]
   __shared__ int64_t s_row[NTOK];   // the token's cache row, -1: it has none
   __shared__ int s_pos[NTOK];
@@ -397,10 +413,15 @@ __global__ __launch_bounds__(TPB) void append_kernel(AppendK a) {
   if (threadIdx.x < NTOK) {
     const int r = min(r0 + (int)threadIdx.x, a.total_rows - 1);
     int b = a.rows_per_batch > 0 ? min(r / a.rows_per_batch, a.batch - 1) : 0;
-    int rs = a.row_start[b], re = a.row_start[b + 1], aq = a.act_q[b], ak = a.act_k[b];
-    if (r < rs || r >= re) {
-      b = batch_of_row(a.row_start, a.batch, r);
-      rs = a.row_start[b], re = a.row_start[b + 1], aq = a.act_q[b], ak = a.act_k[b];
+    int rs = lens.rs(b), re = lens.rs(b + 1), aq = lens.aq(b), ak = lens.ak(b);
+    if (r < rs || r >= re) {   // the last sequence that begins at or before r
+      int lo = 0, hi = a.batch - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (lens.rs(mid) <= r) lo = mid; else hi = mid - 1;
+      }
+      b = lo;
+      rs = lens.rs(b), re = lens.rs(b + 1), aq = lens.aq(b), ak = lens.ak(b);
     }
     int64_t row = -1;
     const int s1 = r - rs, pos = ak - aq + s1;
@@ -446,19 +467,28 @@ __global__ __launch_bounds__(TPB) void append_kernel(AppendK a) {
   }
 }
 
-template <int IO, bool LATENT, int NTOK>
-hipError_t launch_append_n(const AppendK& k, hipStream_t s) {
+template <int IO, bool LATENT, int NTOK, typename Lens>
+hipError_t launch_append_n(const AppendK& k, const Lens& l, hipStream_t s) {
   const dim3 grid((k.total_rows + NTOK - 1) / NTOK);
   const size_t lds = (size_t)NTOK * (k.rdim / 2) * sizeof(float2);
-  if (!LATENT && k.a.width <= 64) hipLaunchKernelGGL((append_kernel<IO, 8, LATENT, NTOK>), grid, dim3(TPB), lds, s, k);
-  else if (k.a.width <= 128) hipLaunchKernelGGL((append_kernel<IO, 16, LATENT, NTOK>), grid, dim3(TPB), lds, s, k);
-  else if (k.a.width <= 256) hipLaunchKernelGGL((append_kernel<IO, 32, LATENT, NTOK>), grid, dim3(TPB), lds, s, k);
-  else hipLaunchKernelGGL((append_kernel<IO, 64, LATENT, NTOK>), grid, dim3(TPB), lds, s, k);
+  if (!LATENT && k.a.width <= 64) hipLaunchKernelGGL((append_kernel<IO, 8, LATENT, NTOK, Lens>), grid, dim3(TPB), lds, s, k, l);
+  else if (k.a.width <= 128) hipLaunchKernelGGL((append_kernel<IO, 16, LATENT, NTOK, Lens>), grid, dim3(TPB), lds, s, k, l);
+  else if (k.a.width <= 256) hipLaunchKernelGGL((append_kernel<IO, 32, LATENT, NTOK, Lens>), grid, dim3(TPB), lds, s, k, l);
+  else hipLaunchKernelGGL((append_kernel<IO, 64, LATENT, NTOK, Lens>), grid, dim3(TPB), lds, s, k, l);
   return hipGetLastError();
 }
 template <int IO, bool LATENT>
-hipError_t launch_append_io(const AppendK& k, hipStream_t s) {
-  return k.total_rows > APPEND_FEW ? launch_append_n<IO, LATENT, 8>(k, s) : launch_append_n<IO, LATENT, 4>(k, s);
+hipError_t launch_append_io(const AppendK& k, const AppendArgs& a, hipStream_t s) {
+  if (a.lengths_host) {
+    ArgLens l{};
+    std::memcpy(l.v, a.row_start, sizeof(int32_t) * (a.batch + 1));
+    std::memcpy(l.v + a.batch + 1, a.act_q, sizeof(int32_t) * a.batch);
+    std::memcpy(l.v + 2 * a.batch + 1, a.act_k, sizeof(int32_t) * a.batch);
+    l.batch = a.batch;
+    return k.total_rows > APPEND_FEW ? launch_append_n<IO, LATENT, 8>(k, l, s) : launch_append_n<IO, LATENT, 4>(k, l, s);
+  }
+  const DeviceLens l{a.row_start, a.act_q, a.act_k};
+  return k.total_rows > APPEND_FEW ? launch_append_n<IO, LATENT, 8>(k, l, s) : launch_append_n<IO, LATENT, 4>(k, l, s);
 }
 
 int is_aligned(const void* p, const View& v) {
@@ -502,9 +532,6 @@ hipError_t launch_cache_append(const AppendArgs& a, hipStream_t s) {
   k.inter = a.interleaved;
   k.freq = a.freq;
   k.pos = make_positions(a.positions, a.wide, a.total_rows, a.axes, a.sections, a.rdim / 2);
-  k.row_start = a.row_start;
-  k.act_q = a.act_q;
-  k.act_k = a.act_k;
   k.table = a.table;
   k.batch = a.batch;
   k.total_rows = a.total_rows;
@@ -513,6 +540,6 @@ hipError_t launch_cache_append(const AppendArgs& a, hipStream_t s) {
   k.rows_per_batch = std::max(1, a.total_rows / a.batch);
   k.blocks = a.blocks;
   if (a.io == DSA_DTYPE_BF16)
-    return latent ? launch_append_io<DSA_DTYPE_BF16, true>(k, s) : launch_append_io<DSA_DTYPE_BF16, false>(k, s);
-  return latent ? launch_append_io<DSA_DTYPE_F16, true>(k, s) : launch_append_io<DSA_DTYPE_F16, false>(k, s);
+    return latent ? launch_append_io<DSA_DTYPE_BF16, true>(k, a, s) : launch_append_io<DSA_DTYPE_BF16, false>(k, a, s);
+  return latent ? launch_append_io<DSA_DTYPE_F16, true>(k, a, s) : launch_append_io<DSA_DTYPE_F16, false>(k, a, s);
 }

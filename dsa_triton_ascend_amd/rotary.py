@@ -10,6 +10,7 @@ those operators'.
 from __future__ import annotations
 
 import ctypes
+from array import array
 
 import torch
 
@@ -19,6 +20,7 @@ from . import _lib
 VALID_D = (128, 256, 512)
 D_ROPE = 64
 INDEX_WIDTHS = (64, 96, 128, 256, 512)
+ARG_SEQUENCES = 18   # sequences whose lengths a call takes from the host
 
 
 def _frequencies(inv_freq, pairs=None) -> torch.Tensor:
@@ -137,7 +139,7 @@ class _AppendPlan:
     write them anew between runs."""
 
     def _setup(self, x, caches, block_table, inv_freq, pairs, actual_seq_lengths_kv, actual_seq_lengths_query, positions,
-               sections, layout, norm, more, what, _wait):
+               sections, layout, norm, more, what, _once):
         for c, name in caches:
             if not isinstance(c, torch.Tensor) or not c.is_contiguous() or c.dim() != 4:
                 raise ValueError(f"{name} must be a contiguous tensor [num_blocks, block_size, N, D]")
@@ -186,15 +188,23 @@ class _AppendPlan:
         if not (self.batch and self.total_rows and self.max_blocks and self.num_blocks and self.page):
             return None, None
 
-        def place():
+        batch = self.batch
+        if _once and batch <= ARG_SEQUENCES:   # the lengths go with the call: no upload before it
             self.block_table = block_table.to(torch.int32).contiguous()
-            return H.upload(self.lib, self.dev, row_start, act_q, act_k, wait=_wait)
+            self.lengths = array("i", row_start + act_q + act_k)
+            at = self.lengths.buffer_info()[0]
+            lengths = (at, at + 4 * (batch + 1), at + 4 * (2 * batch + 1), True)
+        else:
+            def place():
+                self.block_table = block_table.to(torch.int32).contiguous()
+                return H.upload(self.lib, self.dev, row_start, act_q, act_k, wait=not _once)
 
-        self.row_start, self.act_q, self.act_k = H.on_device(self.dev, place)
+            self.row_start, self.act_q, self.act_k = H.on_device(self.dev, place)
+            lengths = (self.row_start.data_ptr(), self.act_q.data_ptr(), self.act_k.data_ptr(), False)
         rotation = (H.ptr(self.pos), self.pos is not None and self.pos.dtype == torch.int64, self.axes, self.sec,
                     self.freq.data_ptr())
-        return rotation, (self.row_start.data_ptr(), self.act_q.data_ptr(), self.act_k.data_ptr(), self.block_table.data_ptr(),
-                          self.batch, self.total_rows, self.per, self.max_blocks, self.page, self.num_blocks)
+        return rotation, (*lengths, self.block_table.data_ptr(), batch, self.total_rows, self.per, self.max_blocks, self.page,
+                          self.num_blocks)
 
     def _launch(self, entry, what):
         if self.args is not None:
@@ -206,7 +216,7 @@ class LatentAppendPlan(_AppendPlan):
 
     def __init__(self, latent, key_rope, key_cache, key_rope_cache, block_table, inv_freq, actual_seq_lengths_kv,
                  actual_seq_lengths_query=None, positions=None, norm_weight=None, norm_eps=1e-6, sections=None,
-                 interleaved=True, layout="BSND", *, _wait=True):
+                 interleaved=True, layout="BSND", *, _once=False):
         self.x, self.sb, self.ss, self.sh, self.per = _rows_view(latent, layout, "latent")
         self.rope, self.rb, self.rs, _, _ = _rows_view(key_rope, layout, "key_rope")
         d = latent.shape[-1]
@@ -222,7 +232,7 @@ class LatentAppendPlan(_AppendPlan):
             raise ValueError(f"caches must be [num_blocks, block_size, 1, {d}] and [.., 1, {D_ROPE}]")
         rotation, places = self._setup(latent, [(key_cache, "key_cache"), (key_rope_cache, "key_rope_cache")], block_table, inv_freq,
                     D_ROPE // 2, actual_seq_lengths_kv, actual_seq_lengths_query, positions, sections, layout,
-                    (norm_weight,), (key_rope,), "latent", _wait)
+                    (norm_weight,), (key_rope,), "latent", _once)
         self.norm_weight = None if norm_weight is None else norm_weight.contiguous()
         self.key_cache, self.key_rope_cache = key_cache, key_rope_cache
         if places is not None:
@@ -240,7 +250,7 @@ class IndexAppendPlan(_AppendPlan):
 
     def __init__(self, index_key, index_cache, block_table, inv_freq, actual_seq_lengths_key,
                  actual_seq_lengths_query=None, positions=None, norm_weight=None, norm_bias=None, norm_eps=1e-6,
-                 sections=None, rotary_start=0, interleaved=False, layout="BSND", *, _wait=True):
+                 sections=None, rotary_start=0, interleaved=False, layout="BSND", *, _once=False):
         if norm_bias is not None and norm_weight is None:
             raise ValueError("norm_bias needs norm_weight")
         self.x, self.sb, self.ss, self.sh, self.per = _rows_view(index_key, layout, "index_key")
@@ -254,7 +264,7 @@ class IndexAppendPlan(_AppendPlan):
             raise ValueError(f"rotary dimensions [{self.start}, {self.start} + {self.rdim}) of {self.w}: the start a "
                              "multiple of 8, the count of 16")
         rotation, places = self._setup(index_key, [(index_cache, "index_cache")], block_table, inv_freq, None, actual_seq_lengths_key,
-                    actual_seq_lengths_query, positions, sections, layout, (norm_weight, norm_bias), (), "index_key", _wait)
+                    actual_seq_lengths_query, positions, sections, layout, (norm_weight, norm_bias), (), "index_key", _once)
         self.norm_weight, self.norm_bias = (None if t is None else t.contiguous() for t in (norm_weight, norm_bias))
         self.index_cache = index_cache
         if places is not None:
@@ -283,7 +293,7 @@ def latent_cache_append(latent, key_rope, key_cache, key_rope_cache, block_table
     row of the caches changes. Two new tokens must not share a place. Returns the two caches."""
     return LatentAppendPlan(latent, key_rope, key_cache, key_rope_cache, block_table, inv_freq, actual_seq_lengths_kv,
                             actual_seq_lengths_query, positions, norm_weight, norm_eps, sections, interleaved, layout,
-                            _wait=False).run()
+                            _once=True).run()
 
 
 def index_cache_append(index_key, index_cache, block_table, inv_freq, actual_seq_lengths_key,
@@ -298,4 +308,4 @@ def index_cache_append(index_key, index_cache, block_table, inv_freq, actual_seq
     cache."""
     return IndexAppendPlan(index_key, index_cache, block_table, inv_freq, actual_seq_lengths_key,
                            actual_seq_lengths_query, positions, norm_weight, norm_bias, norm_eps, sections, rotary_start,
-                           interleaved, layout, _wait=False).run()
+                           interleaved, layout, _once=True).run()

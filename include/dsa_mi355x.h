@@ -400,13 +400,15 @@ int dsa_rotary(const void* x, int64_t batch_stride, int64_t row_stride, int64_t 
  *   latent [.., d], key_rope [.., 64] (one head) by batch and row strides in elements as dsa_rotary
  *   (rows_per_batch >= 1; total_rows for packed ones); d in {128, 256, 512}; caches [num_blocks, page, 1, d | 64],
  *   16-byte aligned; norm_weight [d] in w_dtype (fp16 / bf16 / fp32); inv_freq [32] fp32.
+ *   lengths_host: 0, or row_start, act_q and act_k are host memory, read within the call (at most 18
+ *   sequences: they travel as kernel arguments, and become part of a graph that captures the call).
  */
 int dsa_latent_append(const void* latent, int64_t batch_stride, int64_t row_stride, const void* key_rope,
                       int64_t rope_batch_stride, int64_t rope_row_stride, int io_dtype, int d, const void* norm_weight,
                       int w_dtype, float eps, const void* positions, int positions_64, int axes, const int32_t* sections,
                       const float* inv_freq, int interleaved, const int32_t* row_start, const int32_t* act_q,
-                      const int32_t* act_k, const int32_t* block_table, int batch, int total_rows, int rows_per_batch,
-                      int max_blocks, int page_block_size, int64_t num_blocks, void* key_cache, void* key_rope_cache,
+                      const int32_t* act_k, int lengths_host, const int32_t* block_table, int batch, int total_rows,
+                      int rows_per_batch, int max_blocks, int page_block_size, int64_t num_blocks, void* key_cache, void* key_rope_cache,
                       void* stream);
 
 /*
@@ -420,8 +422,8 @@ int dsa_index_append(const void* index_key, int64_t batch_stride, int64_t row_st
                      int n2, int w, const void* norm_weight, const void* norm_bias, int w_dtype, float eps,
                      const void* positions, int positions_64, int axes, const int32_t* sections, const float* inv_freq,
                      int rotary_start, int rotary_dim, int interleaved, const int32_t* row_start, const int32_t* act_q,
-                     const int32_t* act_k, const int32_t* block_table, int batch, int total_rows, int rows_per_batch,
-                     int max_blocks, int page_block_size, int64_t num_blocks, void* index_cache, void* stream);
+                     const int32_t* act_k, int lengths_host, const int32_t* block_table, int batch, int total_rows,
+                     int rows_per_batch, int max_blocks, int page_block_size, int64_t num_blocks, void* index_cache, void* stream);
 
 /*
  * Workspace bytes of dsa_prefix_attn for these bounds (0 where every row has one range of tokens); needs

@@ -99,18 +99,21 @@ def test_c_entries_refuse():
     refused(lib.dsa_rotary, base, 13, 5000, "width", _lib.DSA_ERR_UNSUPPORTED)
     refused(lib.dsa_rotary, base, 12, 20000, "2^20", _lib.DSA_ERR_UNSUPPORTED)
 
-    lat = [p, 0, 512, p, 0, 64, 1, 512, None, 1, 1e-6, None, 0, 1, None, p, 1, p, p, p, p, 2, 4, 4, 3, 16, 8, p, p, None]
-    for at, v, what in ((0, None, "null"), (3, None, "null"), (15, None, "null"), (17, None, "null"), (20, None, "null"),
-                        (27, None, "null"), (28, None, "null"), (6, 2, "io_dtype"), (7, 320, "D must"), (13, 2, "sections"),
-                        (21, 0, "shape"), (23, 0, "shape"), (24, 0, "shape"), (25, 0, "shape"), (26, 0, "shape"),
-                        (27, ctypes.c_void_p(24), "aligned"), (28, ctypes.c_void_p(24), "aligned")):
+    lat = [p, 0, 512, p, 0, 64, 1, 512, None, 1, 1e-6, None, 0, 1, None, p, 1, p, p, p, 0, p, 2, 4, 4, 3, 16, 8, p, p, None]
+    for at, v, what in ((0, None, "null"), (3, None, "null"), (15, None, "null"), (17, None, "null"), (21, None, "null"),
+                        (28, None, "null"), (29, None, "null"), (6, 2, "io_dtype"), (7, 320, "D must"), (13, 2, "sections"),
+                        (22, 0, "shape"), (24, 0, "shape"), (25, 0, "shape"), (26, 0, "shape"), (27, 0, "shape"),
+                        (28, ctypes.c_void_p(24), "aligned"), (29, ctypes.c_void_p(24), "aligned")):
         refused(lib.dsa_latent_append, lat, at, v, what)
+    bad = list(lat)
+    bad[20], bad[22] = 1, 19
+    assert lib.dsa_latent_append(*bad) == _lib.DSA_ERR_UNSUPPORTED and b"18 sequences" in lib.dsa_last_error()
     bad = list(lat)
     bad[8], bad[9] = p, 7
     assert lib.dsa_latent_append(*bad) == _lib.DSA_ERR_INVALID and b"norm weights" in lib.dsa_last_error()
 
-    idx = [p, 0, 128, 128, 1, 1, 128, p, p, 2, 1e-6, None, 0, 1, None, p, 0, 64, 0, p, p, p, p, 2, 4, 4, 3, 16, 8, p, None]
-    for at, v, what in ((0, None, "null"), (15, None, "null"), (29, None, "null"), (4, 2, "io_dtype"), (5, 0, "heads"),
+    idx = [p, 0, 128, 128, 1, 1, 128, p, p, 2, 1e-6, None, 0, 1, None, p, 0, 64, 0, p, p, p, 0, p, 2, 4, 4, 3, 16, 8, p, None]
+    for at, v, what in ((0, None, "null"), (15, None, "null"), (30, None, "null"), (4, 2, "io_dtype"), (5, 0, "heads"),
                         (7, None, "norm_bias"), (9, 9, "norm weights"), (17, 256, "rotary")):
         refused(lib.dsa_index_append, idx, at, v, what)
     refused(lib.dsa_index_append, idx, 6, 72, "D=72", _lib.DSA_ERR_UNSUPPORTED)
@@ -118,7 +121,7 @@ def test_c_entries_refuse():
     refused(lib.dsa_index_append, idx, 17, 24, "of 16", _lib.DSA_ERR_UNSUPPORTED)
     # nothing to do: no launch
     none = list(idx)
-    none[24] = 0
+    none[25] = 0
     assert lib.dsa_index_append(*none) == 0
 
 

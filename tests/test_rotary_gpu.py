@@ -283,6 +283,34 @@ def test_append_strides_and_constant_rows():
         assert int((c.abs().sum(-1) > 0).sum()) == sum(nq) - 1   # the zero vector stays zero
 
 
+@pytest.mark.parametrize("batch", [17, 18, 19, 40])
+def test_append_lengths_as_arguments_and_uploaded(batch):
+    """One-shot calls up to 18 sequences take their lengths along, longer ones and plans upload them: the same
+    caches from both, uneven packed sequences with empty ones and rows behind the last among them."""
+    g = torch.Generator().manual_seed(14)
+    tokens = torch.randint(0, 5, (batch,), generator=g).tolist()
+    kv = [t + int(torch.randint(0, 40, (1,), generator=g)) for t in tokens]
+    table, blocks = block_table(kv, 8, g)
+    T, cu = sum(tokens) + 2, torch.tensor(tokens).cumsum(0).tolist()
+    x, r = torch.randn(T, 1, 256, generator=g).half().cuda(), torch.randn(T, 1, 64, generator=g).half().cuda()
+    key = torch.randn(T, 2, 64, generator=g).half().cuda()
+    f, got = freqs(32), []
+    for plan in (False, True):
+        c, rc, ic = (torch.zeros(blocks, 8, n, w, dtype=torch.half, device="cuda") for n, w in ((1, 256), (1, 64), (2, 64)))
+        if plan:
+            dsa.LatentAppendPlan(x, r, c, rc, table.cuda(), f, kv, cu, layout="TND").run()
+            dsa.IndexAppendPlan(key, ic, table.cuda(), f, kv, cu, layout="TND").run()
+        else:
+            dsa.latent_cache_append(x, r, c, rc, table.cuda(), f, kv, cu, layout="TND")
+            dsa.index_cache_append(key, ic, table.cuda(), f, kv, cu, layout="TND")
+        got.append((c, rc, ic))
+    rows, pos, slots = places(table, tokens, kv, 8, blocks)
+    want = torch.zeros(blocks * 8, 256, dtype=torch.half)
+    want[slots] = x.cpu()[rows, 0]
+    assert torch.equal(got[0][0].cpu().view(-1, 256), want)
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 def test_append_far_cache_rows():
     """Cache rows past 2^31 bytes (and elements): block 70000 of 64 tokens of 512."""
     cache = torch.zeros(70001, 64, 1, 512, dtype=torch.bfloat16, device="cuda")
