@@ -285,9 +285,9 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
     uint32_t lo, hi;
     const uint16_t* rope;
   };
-  auto tile_rows = [&](int u) __attribute__((always_inline)) -> Source {
+  auto tile_id = [&](int u) { return L.ids[u & 3][wave * 8 + (lane & 7)]; };
+  auto tile_rows = [&](int u, int32_t id) __attribute__((always_inline)) -> Source {
     const int t = token(u);
-    const int32_t id = L.ids[u & 3][wave * 8 + (lane & 7)];
     const bool ok = (uint32_t)id < a.blocks && t < hi;
     const int row = id * a.page + (t - page_of(t) * a.page);
     const uint16_t* zero = reinterpret_cast<const uint16_t*>(g_zero_row);
@@ -334,7 +334,7 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   };
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const Source src = tile_rows(u);
+    const Source src = tile_rows(u, tile_id(u));
     const uint32_t gnope = nope_at(u), grope = rope_at(u);
     static_for<0, C::GPW - 1>([&](auto j) { gather_part(j, src, gnope, grope); });
   }
@@ -493,16 +493,18 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
     rescale();
     if (t == 0) wait_vmcnt<0>();   // this wave's part of tile t + 1 (its ids copy may be under way)
     else wait_vmcnt<1>();
+    const int32_t id = tile_id(t + 2);
     if (is_mixed(t + 1)) sanitize(t + 1);
     lds_barrier();   // tile t + 1 resident; every wave done with tile t - 1, whose buffer is free
-    const Source src = tile_rows(t + 2);
+    Source src;   // (computed behind the chain's first MFMA)
     const uint32_t gnope = nope_at((t + 2) % NBUF), grope = rope_at((t + 2) % NBUF);   // the free buffer
     const uint32_t vbase = v_base(t), vnext = v_base(t + 1);
     f32x16 s1 = s_tile(
         t + 1,
         [&](int ks) __attribute__((always_inline)) {
+          if (ks == 0) src = tile_rows(t + 2, id);
           static_for<0, C::GPW>([&](auto j) __attribute__((always_inline)) {
-            if (j * KS / C::GPW == ks) {
+            if (1 + j * (KS - 1) / C::GPW == ks) {
               if constexpr (j < C::GPW - 1) gather_part(j, src, gnope, grope);
               else ids_dma(t + 4);   // the slot of tile t's ids, read two iterations ago
             }
