@@ -134,7 +134,7 @@ template <int D> struct PfxLds {
       uint8_t own_nope[NWV][BN * D * 2];
       uint8_t own_rope[NWV][BN * DR * 2];
     };
-    float4 join[NWV][16][64];             // the waves' outputs, 128 columns at a time
+    float4 join[D > 128 ? 2 : 1][NWV][16][64];   // the waves' outputs, 128 columns at a time
   };
   int32_t ids[4][BN];
   int red[2][NWV];
@@ -241,12 +241,9 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   lim = dead ? INT_MAX : min(lim, it.t_hi);   // within the item
   int hi, min_lim;
   {
-    int mx = dead ? 0 : lim, mn = lim;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      mx = max(mx, __shfl_xor(mx, o));
-      mn = min(mn, __shfl_xor(mn, o));
-    }
+    // (VALU scans; the last lane has the wave's. Limits are not negative.)
+    int mx = __builtin_amdgcn_readlane((int)wave_incl_max(dead ? 0u : (uint32_t)lim), 63);
+    int mn = __builtin_amdgcn_readlane(wave_incl_min_i32(lim), 63);
     if (lane == 0) {
       L.red[0][wave] = mx;
       L.red[1][wave] = mn;
@@ -616,12 +613,9 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
   lim = dead ? INT_MAX : min(lim, it.t_hi);
   int hi, min_lim;
   {
-    int mx = dead ? 0 : lim, mn = lim;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      mx = max(mx, __shfl_xor(mx, o));
-      mn = min(mn, __shfl_xor(mn, o));
-    }
+    // (VALU scans; the last lane has the wave's. Limits are not negative.)
+    int mx = __builtin_amdgcn_readlane((int)wave_incl_max(dead ? 0u : (uint32_t)lim), 63);
+    int mn = __builtin_amdgcn_readlane(wave_incl_min_i32(lim), 63);
     wait_vmcnt<0>();   // Q
     asm volatile("" ::: "memory");
 #pragma unroll
@@ -877,31 +871,32 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
   }
   const float inv = dead ? 0.f : 1.f / l_tot;
 #pragma unroll
-  for (int c = 0; c < ON / 4; ++c) {
-    if (c > 0) __syncthreads();
+  for (int c = 0; c < ON / 4; ++c) {   // two buffers in turn: one barrier each
+    float4(*const join)[16][64] = L.join[c & 1];
+    if (valid)   // (a mask: fewer lanes, fewer LDS cycles)
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
+      for (int n = 0; n < 4; ++n)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x16& v = o[4 * c + n];
-        L.join[wave][n * 4 + g][lane] = make_float4(v[4 * g] * f, v[4 * g + 1] * f, v[4 * g + 2] * f, v[4 * g + 3] * f);
-      }
-    __syncthreads();
+        for (int g = 0; g < 4; ++g) {
+          const f32x16& v = o[4 * c + n];
+          join[wave][n * 4 + g][lane] = make_float4(v[4 * g] * f, v[4 * g + 1] * f, v[4 * g + 2] * f, v[4 * g + 3] * f);
+        }
+    lds_barrier();
+    if (!valid) continue;
 #pragma unroll
     for (int k = 0; k < MT; ++k) {
       const int nt = grp * MT + k, n = 4 * c + nt;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        float4 v = L.join[rb][nt * 4 + q][lane];
+        float4 v = join[rb][nt * 4 + q][lane];
 #pragma unroll
         for (int g = 1; g < NG; ++g) {
-          const float4 p = L.join[rb + MT * g][nt * 4 + q][lane];
+          const float4 p = join[rb + MT * g][nt * 4 + q][lane];
           v.x += p.x;
           v.y += p.y;
           v.z += p.z;
           v.w += p.w;
         }
-        if (!valid) continue;
         if (direct)
           *reinterpret_cast<uint2*>(a.out + (int64_t)h * D + n * 32 + 8 * q + 4 * kg) =
               dead ? make_uint2(0, 0) : make_uint2(pack2<IO>(v.x * inv, v.y * inv), pack2<IO>(v.z * inv, v.w * inv));
@@ -972,30 +967,46 @@ constexpr int MAX_SLOTS = 256;
 
 // Joins the ranges of 32 head rows: M = max m_s, out = sum O_s 2^(m_s - M) / sum l_s 2^(m_s - M); rows that
 // see nothing get zeros. Bound by the partials' bytes where there are many rows, by latency where there
-// are few, so the loads of UN ranges are under way at once and, with few rows and many ranges, SG waves
-// take every SG-th one. A wave's lanes are the 32 rows and two column groups of one of the D / 8 groups of
-// 8 columns: 1 KB of a block. A range that a row saw nothing of has weight 0 and is not read.
+// are few, so the first PF ranges' partials are requested before the weights are known (a range that a row
+// saw nothing of has weight 0: its partial, whatever it holds, is left out), later ones UN at a time; with
+// few rows and many ranges, SG waves take every SG-th one. A wave's lanes are the 32 rows and two column
+// groups of one of the D / 8 groups of 8 columns: 1 KB of a block.
 template <int IO, int D, int SG>
 __global__ __launch_bounds__(SG > 1 ? SG * 64 : 256) void prefix_merge_kernel(PfxK a) {
   constexpr int TPB = SG > 1 ? SG * 64 : 256;
   constexpr int LPR = TPB / 32;   // threads a row for the statistics
-  constexpr int UN = 8;
+  constexpr int PF = 12, UN = 8;
   __shared__ float s_w[MAX_SLOTS][32];
   __shared__ float s_inv[32];
-  __shared__ int64_t s_own[32];   // where the row's own blocks begin
   __shared__ float4 s_acc[SG > 1 ? SG : 1][64];
   const int m_rows = a.rows * a.n1;
   const int h0 = blockIdx.x * 32;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int rr = lane & 31, kg = lane >> 5;
+  const int grp = SG > 1 ? blockIdx.y : blockIdx.y * 4 + wave;   // group of 8 columns
+  const int sg = SG > 1 ? wave : 0;
+  // the sequences of this thread's row of the statistics and of this lane's row of the output
+  const int sr = threadIdx.x / LPR, j = threadIdx.x % LPR;
+  const int sh = min(h0 + sr, m_rows - 1), oh = min(h0 + rr, m_rows - 1);
+  int sb = batch_guess(a, sh >> a.n1_shift), ob = batch_guess(a, oh >> a.n1_shift);
+  Seq sq = seq_of(a, sb), oq = seq_of(a, ob);
+  batch_fix(a, sh >> a.n1_shift, sb, sq);
+  batch_fix(a, oh >> a.n1_shift, ob, oq);
+  const bool live = row_limit(a, sh >> a.n1_shift, sq) > 0, o_live = row_limit(a, oh >> a.n1_shift, oq) > 0;
+  const int own = oh - oq.r0 * a.n1;
+  const float4* pp = a.p_part + ((int64_t)blockIdx.x * (D / 8) + grp) * 64 + lane;
+  const float4* op = a.o_part + ((int64_t)(oq.r0 * a.n1 / 32 + ob + own / 32) * (D / 8) + grp) * 64 + kg * 32 + own % 32;
+  const int64_t p_step = (int64_t)a.p_blocks * (D / 8) * 64, o_step = (int64_t)a.o_blocks * (D / 8) * 64;
+  auto part = [&](int s) { return s < a.p_splits ? pp + s * p_step : op + (s - a.p_splits) * o_step; };
+  uint4 first[PF];
+#pragma unroll
+  for (int i = 0; i < PF; ++i) {
+    const int s = sg + i * SG;
+    first[i] = ldg16_or0(o_live && s < a.slots, part(s));
+  }
   {
-    const int r = threadIdx.x / LPR, j = threadIdx.x % LPR;
-    const int h = min(h0 + r, m_rows - 1);
-    const int row = h >> a.n1_shift;
-    int b = batch_guess(a, row);
-    Seq seq = seq_of(a, b);
-    const float4* ps = a.part_s + (int64_t)h * a.slots;
+    const float4* ps = a.part_s + (int64_t)sh * a.slots;
     float M = -INFINITY, top = -INFINITY, sum = 0.f;
-    batch_fix(a, row, b, seq);
-    const bool live = row_limit(a, row, seq) > 0;
     for (int s = j; s < a.slots; s += LPR) {
       const float4 st = live ? ps[s] : make_float4(0.f, 0.f, 0.f, 0.f);
       if (st.z != 0.f) {   // (NaN sums take part)
@@ -1011,46 +1022,45 @@ __global__ __launch_bounds__(SG > 1 ? SG * 64 : 256) void prefix_merge_kernel(Pf
     for (int s = j; s < a.slots; s += LPR) {
       const float4 st = live ? ps[s] : make_float4(0.f, 0.f, 0.f, 0.f);
       const float w = st.z != 0.f ? exp2f((st.x - M) * LOG2E) : 0.f;
-      s_w[s][r] = w;
+      s_w[s][sr] = w;
       if (w != 0.f) sum += w * st.z;
     }
 #pragma unroll
     for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
     if (j == 0) {
-      s_inv[r] = live ? 1.f / sum : 0.f;
-      const int own = h - seq.r0 * a.n1;   // (a row of no sequence reads nothing)
-      s_own[r] = ((int64_t)(seq.r0 * a.n1 / 32 + b + own / 32) * (D / 8)) * 64 + own % 32;
-      if (blockIdx.y == 0 && a.sm_max && h0 + r < m_rows) {
-        a.sm_max[h] = live ? top : 0.f;
-        a.sm_sum[h] = live ? sum * exp2f((M - top) * LOG2E) : 0.f;
+      s_inv[sr] = live ? 1.f / sum : 0.f;
+      if (blockIdx.y == 0 && a.sm_max && h0 + sr < m_rows) {
+        a.sm_max[sh] = live ? top : 0.f;
+        a.sm_sum[sh] = live ? sum * exp2f((M - top) * LOG2E) : 0.f;
       }
     }
   }
   __syncthreads();
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int rr = lane & 31, kg = lane >> 5;
-  const int grp = SG > 1 ? blockIdx.y : blockIdx.y * 4 + wave;   // group of 8 columns
-  const int sg = SG > 1 ? wave : 0;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  const float4* pp = a.p_part + ((int64_t)blockIdx.x * (D / 8) + grp) * 64 + lane;
-  const float4* op = a.o_part + s_own[rr] + grp * 64 + kg * 32;
-  const int64_t p_step = (int64_t)a.p_blocks * (D / 8) * 64, o_step = (int64_t)a.o_blocks * (D / 8) * 64;
-  for (int s0 = sg; s0 < a.slots; s0 += SG * UN) {
+  auto add = [&](float w, const uint4& v) {
+    if (w != 0.f) {
+      acc.x += w * __uint_as_float(v.x);
+      acc.y += w * __uint_as_float(v.y);
+      acc.z += w * __uint_as_float(v.z);
+      acc.w += w * __uint_as_float(v.w);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < PF; ++i) {
+    const int s = sg + i * SG;
+    if (s < a.slots) add(s_w[s][rr], first[i]);
+  }
+  for (int s0 = sg + PF * SG; s0 < a.slots; s0 += SG * UN) {
     float w[UN];
     uint4 v[UN];
 #pragma unroll
     for (int i = 0; i < UN; ++i) {
       const int s = s0 + i * SG;
       w[i] = s < a.slots ? s_w[s][rr] : 0.f;
-      v[i] = ldg16_or0(w[i] != 0.f, s < a.p_splits ? pp + s * p_step : op + (s - a.p_splits) * o_step);
+      v[i] = ldg16_or0(w[i] != 0.f, part(s));
     }
 #pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      acc.x += w[i] * __uint_as_float(v[i].x);
-      acc.y += w[i] * __uint_as_float(v[i].y);
-      acc.z += w[i] * __uint_as_float(v[i].z);
-      acc.w += w[i] * __uint_as_float(v[i].w);
-    }
+    for (int i = 0; i < UN; ++i) add(w[i], v[i]);
   }
   if constexpr (SG > 1) {
     s_acc[sg][lane] = acc;
