@@ -134,7 +134,7 @@ template <int D> struct PfxLds {
       uint8_t own_nope[NWV][BN * D * 2];
       uint8_t own_rope[NWV][BN * DR * 2];
     };
-    float4 join[D > 128 ? 2 : 1][NWV][16][64];   // the waves' outputs, 128 columns at a time
+    float4 join[NWV][D > 128 ? 32 : 16][64];   // the waves' outputs, up to 256 columns at a time
   };
   int32_t ids[4][BN];
   int red[2][NWV];
@@ -176,12 +176,13 @@ struct Item {
 template <int D>
 __device__ __forceinline__ void stage_q(const uint16_t* q, int64_t h, int rows, uint8_t* dst, int lane) {
   constexpr int LPR = D / 8, RPI = 64 / LPR;   // lanes a row, rows an instruction
-#pragma unroll
+#pragma unroll 4
   for (int j = 0; j < 32 / RPI; ++j) {
     const int r = j * RPI + lane / LPR;
     lds_dma16_untracked(q + (h + min(r, rows - 1)) * D + ((lane % LPR) ^ (r & 15)) * 8, dst + j * 1024);
   }
 }
+__device__ __forceinline__ uint4 flipped(uint4 v, uint32_t f) { return make_uint4(v.x ^ f, v.y ^ f, v.z ^ f, v.w ^ f); }
 template <int D>
 __device__ __forceinline__ uint4 staged_q(const uint8_t* src, int ks, int rr, int kg) {
   return *reinterpret_cast<const uint4*>(src + rr * (D * 2) + (((2 * ks + kg) ^ (rr & 15)) << 4));
@@ -225,7 +226,6 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   uint8_t* const qs = L.own_nope[wave];
   const int hb = it.h0 + wave * 32;
   if (hb < it.h_end) stage_q<D>(a.q, hb, min(32, it.h_end - hb), qs, lane);
-  auto flipped = [&](uint4 v) { return make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip); };
   uint4 qrv[4];
   {
     const uint16_t* qr = a.qr + (int64_t)(valid ? h : it.h_end - 1) * DR + kg * 8;
@@ -251,11 +251,11 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
     wait_vmcnt<0>();   // Q and the first ids
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int j = 0; j < KSN; ++j) qf[j] = flipped(staged_q<D>(qs, j, rr, kg));
+    for (int j = 0; j < KSN; ++j) qf[j] = flipped(staged_q<D>(qs, j, rr, kg), flip);
     __syncthreads();   // every wave has its Q: the staging area becomes the ring
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<uint4*>(L.qr + (wave * 32 + rr) * (DR + 8) + j * 16 + kg * 8) = flipped(qrv[j]);
+      *reinterpret_cast<uint4*>(L.qr + (wave * 32 + rr) * (DR + 8) + j * 16 + kg * 8) = flipped(qrv[j], flip);
     mx = max(max(L.red[0][0], L.red[0][1]), max(L.red[0][2], L.red[0][3]));
     mn = min(min(L.red[1][0], L.red[1][1]), min(L.red[1][2], L.red[1][3]));
     hi = __builtin_amdgcn_readfirstlane(mx);        // end of the item's tokens
@@ -583,7 +583,6 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
   const int kg = lane >> 5, rr = lane & 31;
   const int hb = it.h0 + rb * 32, h = hb + rr;
   const bool valid = h < it.h_end;
-  const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;   // scale: see run_item
   const float cpos = a.scale > 0.f ? a.scale : a.scale < 0.f ? -a.scale : 1e-30f;
   const float cl2 = cpos * LOG2E;
 
@@ -619,10 +618,10 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
     wait_vmcnt<0>();   // Q
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int j = 0; j < KS; ++j) {
-      if (j < KSN) qf[j] = staged_q<D>(L.own_nope[wave], j, rr, kg);
-      qf[j] = make_uint4(qf[j].x ^ flip, qf[j].y ^ flip, qf[j].z ^ flip, qf[j].w ^ flip);
-    }
+    for (int j = 0; j < KSN; ++j) qf[j] = staged_q<D>(L.own_nope[wave], j, rr, kg);
+    if (__builtin_expect(a.scale < 0.f, 0))
+#pragma unroll
+      for (int j = 0; j < KS; ++j) qf[j] = flipped(qf[j], 0x80008000u);
     if constexpr (MT > 1) {
       if (lane == 0) {
         L.red[0][wave] = mx;
@@ -842,12 +841,13 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
 
   if constexpr (MT > 1) wait_vmcnt<0>();   // the last (unused) loads land before their buffer is used again
 
-  // ---- the groups' outputs joined: each scaled to the common maximum, 128 columns at a time, a wave adding
-  // its row block's parts of MT column tiles
+  // ---- the groups' outputs joined, up to 256 columns at a time: sum over the groups of O_g 2^(m_g - M). Code
+  // that runs once is fetched at about a byte a cycle, so the outputs go to LDS as they are and a rolled loop
+  // scales and adds them (unrolled, with the scaling before it, this took 4.1 of a 128-token item's 10.9 us).
   const float l_wave = add_half_swap(l_part);
   if (lane < 32) L.stat[wave][rr] = make_float4(m_used, m_true, l_wave, 0.f);
   __syncthreads();   // (also: every wave is done with its tiles)
-  float M = -INFINITY, top = -INFINITY, l_tot = 0.f;
+  float M = -INFINITY, top = -INFINITY, l_tot = 0.f, f[NG];
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
     const float4 st = L.stat[rb + MT * g][rr];
@@ -857,9 +857,9 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
     const float4 st = L.stat[rb + MT * g][rr];
-    l_tot += st.x == -INFINITY ? st.z : st.z * __builtin_amdgcn_exp2f((st.x - M) * LOG2E);
+    f[g] = st.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((st.x - M) * LOG2E);   // (O and l are 0 with -inf)
+    l_tot += st.z * f[g];
   }
-  const float f = m_used == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_used - M) * LOG2E);   // (O and l are 0 with -inf)
   if (a.scale == 0.f) top *= 0.f;
   if (writer) {
     if (!direct) {
@@ -870,40 +870,39 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
     }
   }
   const float inv = dead ? 0.f : 1.f / l_tot;
+  constexpr int NC = ON < 8 ? ON : 8;   // column tiles at a time
+  float4* const part = it.part + (int64_t)rb * (D / 8) * 64 + lane;
+  uint16_t* const out = a.out + (int64_t)(valid ? h : 0) * D + 4 * kg;
 #pragma unroll
-  for (int c = 0; c < ON / 4; ++c) {   // two buffers in turn: one barrier each
-    float4(*const join)[16][64] = L.join[c & 1];
+  for (int c = 0; c < ON; c += NC) {
+    if (c > 0) lds_barrier();
     if (valid)   // (a mask: fewer lanes, fewer LDS cycles)
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int n = 0; n < NC; ++n)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const f32x16& v = o[4 * c + n];
-          join[wave][n * 4 + g][lane] = make_float4(v[4 * g] * f, v[4 * g + 1] * f, v[4 * g + 2] * f, v[4 * g + 3] * f);
+          const f32x16& v = o[c + n];
+          L.join[wave][n * 4 + g][lane] = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
         }
     lds_barrier();
-    if (!valid) continue;
+    if (valid && !(dead && !direct))
+#pragma unroll 2
+      for (int e = grp; e < NC * 4; e += NG) {   // groups of 8 columns
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < MT; ++k) {
-      const int nt = grp * MT + k, n = 4 * c + nt;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float4 v = join[rb][nt * 4 + q][lane];
-#pragma unroll
-        for (int g = 1; g < NG; ++g) {
-          const float4 p = join[rb + MT * g][nt * 4 + q][lane];
-          v.x += p.x;
-          v.y += p.y;
-          v.z += p.z;
-          v.w += p.w;
+        for (int g = 0; g < NG; ++g) {
+          const float4 p = L.join[rb + MT * g][e][lane];
+          v.x += p.x * f[g];
+          v.y += p.y * f[g];
+          v.z += p.z * f[g];
+          v.w += p.w * f[g];
         }
         if (direct)
-          *reinterpret_cast<uint2*>(a.out + (int64_t)h * D + n * 32 + 8 * q + 4 * kg) =
+          *reinterpret_cast<uint2*>(out + (c * 4 + e) * 8) =
               dead ? make_uint2(0, 0) : make_uint2(pack2<IO>(v.x * inv, v.y * inv), pack2<IO>(v.z * inv, v.w * inv));
-        else if (!dead)
-          it.part[((int64_t)rb * (D / 8) + n * 4 + q) * 64 + lane] = v;
+        else
+          part[(c * 4 + e) * 64] = v;
       }
-    }
   }
 }
 
