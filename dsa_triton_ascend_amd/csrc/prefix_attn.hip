@@ -64,6 +64,7 @@ struct PfxK {
   int p_mt, p_tiles, p_splits, p_chunk;            // prefix items
   int o_mt, o_tiles, o_splits, o_chunk, o_base;    // own items (o_base: first token, 0 joined)
   int per_xcd, o_by_range;                         // work-groups per XCD; own items of a range on one XCD
+  int o_items, o_compact;                          // own items of a range; numbered through (uneven sequences)
   int slots;
 };
 
@@ -929,29 +930,46 @@ __global__ __launch_bounds__(NWV * 64) void prefix_attn_kernel(PfxK a) {
     it.part = a.p_part + ((int64_t)sp * a.p_blocks + tile * mt) * (D / 8) * 64;
   } else {
     int i = a.o_by_range ? x * a.per_xcd + j : j < hi ? (j - lo) * (8 - rem) + (x - rem) : (hi - lo) * (8 - rem) + (j - hi) * 8 + x;
-    const int per = a.batch * a.o_tiles;   // items of a range
-    const int sp = i / per;
+    const int sp = i / a.o_items;
     if (sp >= a.o_splits) return;
-    i -= sp * per;
-    const int b = i / a.o_tiles, tile = a.o_tiles - 1 - (i - b * a.o_tiles);   // (causal: the longest first)
+    i -= sp * a.o_items;
     mt = a.o_mt;
+    // o_tiles items a sequence, or (sequences much shorter than the longest) numbered through: those of
+    // sequence b begin at row_start[b] * n1 / (32 mt) + b, which leaves each enough
+    int b, n;   // the sequence, how many of its items are before this one
+    if (a.o_compact) {
+      auto first_item = [&](int q) { return a.row_start[q] * a.n1 / (32 * mt) + q; };
+      int below = 0, above = a.batch - 1;
+      while (below < above) {
+        const int mid = (below + above + 1) >> 1;
+        if (first_item(mid) <= i) below = mid; else above = mid - 1;
+      }
+      b = below;
+      n = i - first_item(b);
+    } else {
+      b = i / a.o_tiles;
+      n = i - b * a.o_tiles;
+    }
     it.seq = seq_of(a, b);
     const int first = it.seq.r0 * a.n1;
-    it.h0 = first + tile * 32 * mt;
     it.h_end = it.seq.r1 * a.n1;
+    const int tiles = (it.h_end - first + 32 * mt - 1) / (32 * mt);
+    const int tile = tiles - 1 - n;   // (causal: the longest first)
+    it.h0 = first + tile * 32 * mt;
     it.b = b;
     it.t_lo = a.o_base + sp * a.o_chunk;
     it.t_hi = sp == a.o_splits - 1 ? INT_MAX : it.t_lo + a.o_chunk;
     it.slot = a.p_splits + sp;
     it.part = a.o_part + ((int64_t)sp * a.o_blocks + first / 32 + b + tile * mt) * (D / 8) * 64;
-    if (a.slots == 1 && b == a.batch - 1) {   // rows behind the last sequence: zeros
+    if (a.slots == 1 && b == a.batch - 1) {   // rows behind the last sequence: zeros, by its items
+      const int share = a.o_compact ? a.o_items - (i - n) : a.o_tiles;
       const int64_t end = (int64_t)a.rows * a.n1 * (D / 8);
-      for (int64_t j = (int64_t)it.h_end * (D / 8) + tile * (NWV * 64) + threadIdx.x; j < end; j += a.o_tiles * (NWV * 64)) {
-        stg16(a.out + j * 8, make_uint4(0, 0, 0, 0));
-        if (a.sm_max && j % (D / 8) == 0) a.sm_max[j / (D / 8)] = a.sm_sum[j / (D / 8)] = 0.f;
+      for (int64_t q = (int64_t)it.h_end * (D / 8) + n * (NWV * 64) + threadIdx.x; q < end; q += (int64_t)share * (NWV * 64)) {
+        stg16(a.out + q * 8, make_uint4(0, 0, 0, 0));
+        if (a.sm_max && q % (D / 8) == 0) a.sm_max[q / (D / 8)] = a.sm_sum[q / (D / 8)] = 0.f;
       }
     }
-    if (it.h0 >= it.h_end) return;
+    if (tile < 0) return;
     it.b = b;
     it.t_lo = a.o_base + sp * a.o_chunk;
     it.t_hi = sp == a.o_splits - 1 ? INT_MAX : it.t_lo + a.o_chunk;
@@ -1257,7 +1275,11 @@ hipError_t launch_prefix_attn(const PrefixArgs& a, hipStream_t s) {
   k.o_base = c.o_base;
   k.slots = c.slots;
   const int most = (c.p_splits + 7) / 8 * c.p_tiles;   // prefix items of an XCD
-  const int64_t all = (int64_t)c.p_splits * c.p_tiles + (int64_t)a.batch * c.o_tiles * c.o_splits;
+  const int64_t even = (int64_t)a.batch * c.o_tiles, through = (int64_t)a.total_rows * a.n1 / (32 * c.o_mt) + a.batch;
+  k.o_compact = even > through + through / 2;
+  k.o_items = (int)(k.o_compact ? through : even);
+  const int64_t all = (int64_t)c.p_splits * c.p_tiles + (int64_t)k.o_items * c.o_splits;
+  if (all > INT_MAX - 16) return hipErrorInvalidConfiguration;
   k.per_xcd = (int)std::max<int64_t>(most, (all + 7) / 8);
   k.o_by_range = c.p_splits == 0 && c.o_splits >= 8;
   return a.io == DSA_DTYPE_BF16 ? launch_io<IO_BF16>(k, a.d, s) : launch_io<IO_F16>(k, a.d, s);

@@ -83,6 +83,8 @@ class _Rotation:
         n, width = shape[-2:]
         if rotary_start < 0 or rotary_start + 2 * pairs > width:
             raise ValueError(f"rotary dimensions [{rotary_start}, {rotary_start} + {2 * pairs}) of a width of {width}")
+        if x.numel() // max(1, n * width) >= 2 ** 31:
+            raise ValueError("2^31 tokens or more")
         self.dev = H.require_device(x, pos, freq)
         self.lib = _lib.load()
         self.out = out = torch.empty(shape, dtype=x.dtype, device=self.dev)
@@ -179,7 +181,9 @@ class _AppendPlan:
         self.num_blocks, self.page = caches[0][0].shape[:2]
         self.batch, self.max_blocks = block_table.shape
         self.total_rows = x.shape[0] * (x.shape[1] if layout == "BSND" else 1)
-        for q, k in zip(act_q, act_k):
+        if self.total_rows >= 2 ** 31:
+            raise ValueError("2^31 tokens or more")
+        for k in act_k:
             if k < 0 or k > self.max_blocks * self.page:
                 raise ValueError(f"kv length {k} outside the block table's {self.max_blocks * self.page} tokens")
         self.dev = H.require_device(self.x, block_table, self.freq, self.pos, *norm, *more, *[c for c, _ in caches])

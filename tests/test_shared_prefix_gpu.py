@@ -105,6 +105,8 @@ CASES = [  # n1, d, tokens, kv, prefix, page, mode, packed
     (2, 512, [130], [131], 64, 33, 3, True),
     (128, 512, [2, 2], [2500, 1300], 1027, 64, 0, False),
     (16, 128, [1] * 40, list(range(2100, 2140)), 2048, 128, 3, False),
+    (16, 128, [900] + [1, 0, 2] * 20, [1100] + [205, 201, 260] * 20, 200, 64, 3, True),   # one long prompt, many short
+    (128, 256, [0, 3, 150, 0, 0, 1, 0], [40, 50, 170, 33, 0, 41, 60], 33, 16, 3, True),  # rows packed between empty sequences
 ]
 
 
@@ -116,6 +118,18 @@ def test_against_formula(dtype, case):
     scale = 1 / math.sqrt(d + 64)
     want = exact(t, tokens, kv, prefix, scale, mode, packed)
     check(call(t, tokens, kv, prefix, scale, mode, packed), want)
+
+
+@pytest.mark.parametrize("tokens,tail", [([1200, 3, 5], 700), ([3, 5, 1200], 700), ([900], 1), ([0, 0, 40], 300), ([2, 0], 90)])
+def test_rows_behind_the_last_sequence_are_zeros(tokens, tail):
+    """Many rows behind the last sequence, of one range (no join): evenly split and numbered-through items."""
+    kv = [max(t, 1) for t in tokens]
+    t = make(BF, 64, 128, tokens, kv, 0, 16, True, 300, tail=tail)
+    for splits in (1, 3):
+        with torch.no_grad():
+            junk = torch.full((sum(tokens) + tail + 8, 64, 128), float("nan"), dtype=BF, device="cuda")   # what the output's memory held
+        del junk
+        check(call(t, tokens, kv, 0, 0.07, 3, True, kv_splits=splits), exact(t, tokens, kv, 0, 0.07, 3, True))
 
 
 @pytest.mark.parametrize("splits", [1, 2, 5, 64])
