@@ -27,6 +27,7 @@ struct View {
   int rows_per_batch;
 };
 __device__ __forceinline__ int64_t row_offset(const View& v, int r) {
+  if (v.batch == v.row * v.rows_per_batch) return r * v.row;   // evenly spaced rows: no division
   const int b = r / v.rows_per_batch;
   return b * v.batch + (r - b * v.rows_per_batch) * v.row;
 }
@@ -199,6 +200,11 @@ __global__ __launch_bounds__(TPB) void rotary_kernel(RotaryK a) {
   }
 }
 
+// (rows of a single batch are evenly spaced, whatever its stride)
+View make_view(int64_t batch, int64_t row, int64_t head, int rows_per_batch, int rows) {
+  return {rows <= rows_per_batch ? row * rows_per_batch : batch, row, head, rows_per_batch};
+}
+
 Positions make_positions(const void* p, int wide, int rows, int axes, const int32_t* sections, int pairs) {
   Positions ps{p, wide, rows, {axes, {pairs, pairs, pairs, pairs}}};
   int end = 0;
@@ -267,7 +273,7 @@ struct Norm {
   int kind;   // 0 none, 1 root mean square, 2 mean and variance
   const void* w;
   const void* b;
-  int wdt;
+  int wdt, w_aligned, b_aligned;
   float eps;
 };
 
@@ -291,18 +297,34 @@ struct AppendK {
   int64_t blocks;
 };
 
-// Eight of the norm's parameters from element e on
-__device__ __forceinline__ void norm_params(const void* p, int dt, int e, float (&w)[8]) {
+// Eight of the norm's parameters from element e on, by 16-byte loads where they may be
+__device__ __forceinline__ void norm_params(const void* p, int dt, int aligned, int e, float (&w)[8]) {
   if (dt == DSA_DTYPE_F32) {
+    const float* f = reinterpret_cast<const float*>(p) + e;
+    if (aligned) {
+      const uint4 u = ldg16(f), v = ldg16(f + 4);
+      const uint32_t b[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = reinterpret_cast<const float*>(p)[e + i];
+      for (int i = 0; i < 8; ++i) w[i] = __uint_as_float(b[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = f[i];
+    }
+    return;
+  }
+  const uint16_t* h = reinterpret_cast<const uint16_t*>(p) + e;
+  uint16_t b[8];
+  if (aligned) {
+    const uint4 u = ldg16(h);
+    const uint32_t d[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = (uint16_t)(d[i / 2] >> (16 * (i & 1)));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint16_t u = reinterpret_cast<const uint16_t*>(p)[e + i];
-      w[i] = dt == DSA_DTYPE_BF16 ? bf16_to_f32(u) : f16_to_f32(u);
-    }
+    for (int i = 0; i < 8; ++i) b[i] = h[i];
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = dt == DSA_DTYPE_BF16 ? bf16_to_f32(b[i]) : f16_to_f32(b[i]);
 }
 
 template <int IO>
@@ -381,9 +403,10 @@ __global__ __launch_bounds__(TPB) void append_kernel(AppendK a, Lens lens) {
   constexpr int VPP = TPB / LPV;    // vectors a pass of the work-group
   const int r0 = blockIdx.x * NTOK;
   const int li = threadIdx.x % LPV, vi = threadIdx.x / LPV;
-  const int nvec = NTOK * a.a.heads;
+  const int heads = LATENT ? 1 : a.a.heads, half = LATENT ? 32 : a.rdim / 2;
+  const int nvec = NTOK * heads;
   auto load_a = [&](int v, float (&x)[8]) __attribute__((always_inline)) {
-    const int tok = v / a.a.heads, h = v - tok * a.a.heads;
+    const int tok = heads == 1 ? v : v / heads, h = v - tok * heads;
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = 0.f;
     if (v < nvec && r0 + tok < a.total_rows && 8 * li < a.a.width)
@@ -404,10 +427,9 @@ __global__ __launch_bounds__(TPB) void append_kernel(AppendK a, Lens lens) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) nw[i] = nb[i] = 0.f;
   if (a.norm.kind != 0 && 8 * li < a.a.width) {
-    norm_params(a.norm.w, a.norm.wdt, 8 * li, nw);
-    if (a.norm.b) norm_params(a.norm.b, a.norm.wdt, 8 * li, nb);
+    norm_params(a.norm.w, a.norm.wdt, a.norm.w_aligned, 8 * li, nw);
+    if (a.norm.b) norm_params(a.norm.b, a.norm.wdt, a.norm.b_aligned, 8 * li, nb);
   }
-  const int half = a.rdim / 2;
   // pair threadIdx.x % half of the table's token threadIdx.x / half (32 pairs: one a thread)
   const float freq0 = a.freq[(int)threadIdx.x % half];
   if (threadIdx.x < NTOK) {
@@ -452,11 +474,11 @@ __global__ __launch_bounds__(TPB) void append_kernel(AppendK a, Lens lens) {
     const bool more = v0 + VPP < nvec;
     float nx[8];
     if (more) load_a(v + VPP, nx);
-    const int tok = min(v / a.a.heads, NTOK - 1), h = v - tok * a.a.heads;
+    const int tok = min(heads == 1 ? v : v / heads, NTOK - 1), h = v - tok * heads;
     norm_vec<LPV>(a.norm, nw, nb, a.a.width, li, x);
     if (!LATENT) rotate_vec<LPV>(tab + tok * half, a.start, a.rdim, a.inter, li, x);
     if (v < nvec && 8 * li < a.a.width && s_row[tok] >= 0)
-      store_vec<IO, 8>(reinterpret_cast<uint16_t*>(a.a.cache) + (s_row[tok] * a.a.heads + h) * a.a.width + 8 * li, x);
+      store_vec<IO, 8>(reinterpret_cast<uint16_t*>(a.a.cache) + (s_row[tok] * heads + h) * a.a.width + 8 * li, x);
     if (more)
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = nx[i];
@@ -503,7 +525,7 @@ hipError_t launch_rotary(const RotaryArgs& a, hipStream_t s) {
   RotaryK k{};
   k.x = a.x;
   k.out = a.out;
-  k.view = {a.batch_stride, a.row_stride, a.head_stride, a.rows_per_batch};
+  k.view = make_view(a.batch_stride, a.row_stride, a.head_stride, a.rows_per_batch, a.rows);
   k.pos = make_positions(a.positions, a.wide, a.rows, a.axes, a.sections, a.rdim / 2);
   k.freq = a.freq;
   k.rows = a.rows;
@@ -519,14 +541,14 @@ hipError_t launch_rotary(const RotaryArgs& a, hipStream_t s) {
 
 hipError_t launch_cache_append(const AppendArgs& a, hipStream_t s) {
   AppendK k{};
-  const View va{a.batch_stride, a.row_stride, a.head_stride, a.rows_per_batch};
+  const View va = make_view(a.batch_stride, a.row_stride, a.head_stride, a.rows_per_batch, a.total_rows);
   k.a = {a.x, va, is_aligned(a.x, va), a.heads, a.width, a.cache};
   const bool latent = a.rope != nullptr;
   if (latent) {
-    const View vb{a.rope_batch_stride, a.rope_row_stride, 0, a.rows_per_batch};
+    const View vb = make_view(a.rope_batch_stride, a.rope_row_stride, 0, a.rows_per_batch, a.total_rows);
     k.b = {a.rope, vb, is_aligned(a.rope, vb), 1, 64, a.rope_cache};
   }
-  k.norm = {a.norm_kind, a.norm_w, a.norm_b, a.wdt, a.eps};
+  k.norm = {a.norm_kind, a.norm_w, a.norm_b, a.wdt, ((uintptr_t)a.norm_w & 15) == 0, ((uintptr_t)a.norm_b & 15) == 0, a.eps};
   k.start = a.start;
   k.rdim = a.rdim;
   k.inter = a.interleaved;

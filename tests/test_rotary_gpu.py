@@ -87,7 +87,7 @@ def test_rotary_far_positions(inter):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("how", ["slice", "odd", "heads", "batch", "last", "expand"])
+@pytest.mark.parametrize("how", ["slice", "odd", "heads", "batch", "last", "expand", "broadcast", "one batch"])
 def test_rotary_strides(dtype, how):
     g = torch.Generator().manual_seed(6)
     B, S, N, W = 3, 4, 6, 64
@@ -95,7 +95,9 @@ def test_rotary_strides(dtype, how):
     x = {"slice": lambda: r(B, S, N, 192)[..., 128:], "odd": lambda: r(B, S, N, W + 3)[..., 1:W + 1],
          "heads": lambda: r(B, S, W * N).view(B, S, N, W).transpose(1, 2).contiguous().transpose(1, 2),
          "batch": lambda: r(S, B, N, W).transpose(0, 1), "last": lambda: r(B, S, W, N).transpose(2, 3),
-         "expand": lambda: r(B, S, 1, W).expand(B, S, N, W)}[how]()
+         "expand": lambda: r(B, S, 1, W).expand(B, S, N, W), "broadcast": lambda: r(1, S, 1, W).expand(B, S, N, W),
+         "one batch": lambda: r(7, S, N, W)[3::4]}[how]()
+    B = x.shape[0]
     pos = torch.randint(0, 9000, (B, S), generator=g).cuda()
     f = freqs(32)
     for inter in (True, False):
@@ -309,6 +311,18 @@ def test_append_lengths_as_arguments_and_uploaded(batch):
     want[slots] = x.cpu()[rows, 0]
     assert torch.equal(got[0][0].cpu().view(-1, 256), want)
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_append_broadcast_tokens():
+    """The same new tokens for every sequence (a batch stride of 0), and a batch of one cut from more."""
+    x, r = torch.randn(1, 3, 1, 128).half().cuda(), torch.randn(1, 3, 1, 64).half().cuda()
+    table = torch.arange(8).int().view(4, 2).cuda()
+    for tokens, rows in ((x.expand(4, 3, 1, 128), 4), (torch.cat([x * 0, x, x * 0])[1::2], 1)):
+        c, rc = (torch.zeros(8, 4, 1, w, dtype=torch.half, device="cuda") for w in (128, 64))
+        dsa.latent_cache_append(tokens, r.expand(rows, 3, 1, 64), c, rc, table[:rows], freqs(32), [5] * rows)
+        for b in range(rows):
+            got = c[table[b].long()].reshape(8, 128)
+            assert torch.equal(got[2:5], x[0, :, 0]) and not got[:2].any() and not got[5:].any()
 
 
 def test_append_far_cache_rows():
