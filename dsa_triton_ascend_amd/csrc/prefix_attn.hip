@@ -842,9 +842,10 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
 
   if constexpr (MT > 1) wait_vmcnt<0>();   // the last (unused) loads land before their buffer is used again
 
-  // ---- the groups' outputs joined, up to 256 columns at a time: sum over the groups of O_g 2^(m_g - M). Code
-  // that runs once is fetched at about a byte a cycle, so the outputs go to LDS as they are and a rolled loop
-  // scales and adds them (unrolled, with the scaling before it, this took 4.1 of a 128-token item's 10.9 us).
+  // ---- the groups' outputs joined, up to 256 columns at a time: sum over the groups of O_g 2^(m_g - M). The
+  // outputs go to LDS as they are and a rolled loop scales and adds them: little code for what runs once (with
+  // this, less of it in the prologue, and two groups a barrier, 16.2 us a call instead of 17.1 for 4 rows of 16
+  // heads after 304 tokens).
   const float l_wave = add_half_swap(l_part);
   if (lane < 32) L.stat[wave][rr] = make_float4(m_used, m_true, l_wave, 0.f);
   __syncthreads();   // (also: every wave is done with its tiles)
@@ -970,10 +971,6 @@ __global__ __launch_bounds__(NWV * 64) void prefix_attn_kernel(PfxK a) {
       }
     }
     if (tile < 0) return;
-    it.b = b;
-    it.t_lo = a.o_base + sp * a.o_chunk;
-    it.t_hi = sp == a.o_splits - 1 ? INT_MAX : it.t_lo + a.o_chunk;
-    it.slot = a.p_splits + sp;
   }
   if (mt == 1) run_tokens<IO, D, 1>(a, it, L);
   else if (mt == 2) run_tokens<IO, D, 2>(a, it, L);
@@ -1110,8 +1107,8 @@ int up(int x, int to) { return (x + to - 1) / to * to; }
 
 // Microseconds of a call by a simple model of what was measured at D = 512 (256 CUs, one item each at a
 // time): an item costs 6 (its rows' sequences, Q, first tile, ends) and 1.55 / 0.95 per 32 tokens for 128 / 64
-// head rows or 3.7 per 128 tokens for 32; the latents come at 4.9 TB/s; partial outputs are written at 7 TB/s, and the join is a launch of
-// 6 that reads them at 6 TB/s. It is there to weigh rounds of items against partials: at 64 x 16 heads
+// head rows or 3.7 per 128 tokens for 32; the latents come at 4.9 TB/s; partial outputs are written at 7 TB/s,
+// and the join is a launch of 6 that reads them at 6 TB/s. It is there to weigh rounds of items against partials: at 64 x 16 heads
 // after 8192 tokens 16 prefix ranges take 50 us, 8 take 70 and 32 take 70 as well.
 struct Model {
   double scale;   // of a tile's products against D = 512

@@ -247,8 +247,8 @@ hipError_t launch_rotary_io(const RotaryK& k, bool inter, hipStream_t s) {
 // elements to a vector. A decode step's few tokens wait for a chain of memory accesses: so the vectors,
 // the norm's weights, the frequencies and the lengths (of the sequence that evenly split ones give) are
 // all requested first, and only the block table is left behind them.
-// Tokens a work-group: 4 up to this many (64 tokens take 5.1 us, 6.0 with 8), else 8 (6926 tokens of two heads of 128: 7.4
-// us, 8.5 with 4; 18,216 latents 15.1, 15.5 with 16)
+// Tokens a work-group: 4 up to this many (64 latents take 4.7 us, with 8 tokens 0.9 more), else 8 (6926 tokens of two
+// heads of 128: 7.2 us, with 4 tokens 1.1 more; 18,216 latents 12.3, 3.4 TB/s, with 16 tokens 0.4 more)
 constexpr int APPEND_FEW = 2048;
 
 // The lengths of a call, [row_start | act_q | act_k], from device memory or as a kernel argument (a one-shot

@@ -108,7 +108,7 @@ def rotary_embedding(x, positions, inv_freq, sections=None, rotary_start=0, inte
     `interleaved`, else (i, i + rotary_dim/2). With `sections` (1 to 4 counts of pairs) positions are
     [axes, B, S] / [axes, T], and each run of pairs turns by the position on its own axis: the time,
     height and width of an image's or video's tokens. Angles are computed in 64 bits. Returns a new
-    contiguous tensor."""
+    contiguous tensor, which autograd does not follow: :func:`rotary_embedding_grad` is the gradient."""
     return _Rotation(x, positions, inv_freq, sections, rotary_start, interleaved, layout, 0, "x").run()
 
 
@@ -137,8 +137,8 @@ class _AppendPlan:
     """What both appends share: the new tokens' rows, lengths and block table, and the norm's and the
     rotation's arguments. All in place when the constructor returns, so ``run()`` may be called on
     another stream; calls of one plan, and calls whose caches are the same, are ordered by the caller.
-    ``act_k`` (and ``block_table``) are read on the device in each run: a loop that keeps the plan may
-    write them anew between runs."""
+    ``act_k``, ``block_table`` and the operands are read on the device in each run: a loop that keeps the
+    plan may write them anew between runs (in the plan's copy, where one had to be made contiguous)."""
 
     def _setup(self, x, caches, block_table, inv_freq, pairs, actual_seq_lengths_kv, actual_seq_lengths_query, positions,
                sections, layout, norm, more, what, _once):
@@ -187,6 +187,7 @@ class _AppendPlan:
             if k < 0 or k > self.max_blocks * self.page:
                 raise ValueError(f"kv length {k} outside the block table's {self.max_blocks * self.page} tokens")
         self.dev = H.require_device(self.x, block_table, self.freq, self.pos, *norm, *more, *[c for c, _ in caches])
+        self.norm = tuple(None if w is None else w.contiguous() for w in norm)   # before the upload that is waited for
         self.lib = _lib.load()
         self.args = None   # of the launch, but for the stream; None: nothing to do
         if not (self.batch and self.total_rows and self.max_blocks and self.num_blocks and self.page):
@@ -237,7 +238,7 @@ class LatentAppendPlan(_AppendPlan):
         rotation, places = self._setup(latent, [(key_cache, "key_cache"), (key_rope_cache, "key_rope_cache")], block_table, inv_freq,
                     D_ROPE // 2, actual_seq_lengths_kv, actual_seq_lengths_query, positions, sections, layout,
                     (norm_weight,), (key_rope,), "latent", _once)
-        self.norm_weight = None if norm_weight is None else norm_weight.contiguous()
+        self.norm_weight, = self.norm
         self.key_cache, self.key_rope_cache = key_cache, key_rope_cache
         if places is not None:
             self.args = (self.x.data_ptr(), self.sb, self.ss, self.rope.data_ptr(), self.rb, self.rs, self.io, d,
@@ -269,7 +270,7 @@ class IndexAppendPlan(_AppendPlan):
                              "multiple of 8, the count of 16")
         rotation, places = self._setup(index_key, [(index_cache, "index_cache")], block_table, inv_freq, None, actual_seq_lengths_key,
                     actual_seq_lengths_query, positions, sections, layout, (norm_weight, norm_bias), (), "index_key", _once)
-        self.norm_weight, self.norm_bias = (None if t is None else t.contiguous() for t in (norm_weight, norm_bias))
+        self.norm_weight, self.norm_bias = self.norm
         self.index_cache = index_cache
         if places is not None:
             self.args = (self.x.data_ptr(), self.sb, self.ss, self.sh, self.io, self.n2, self.w, H.ptr(self.norm_weight),

@@ -18,8 +18,10 @@ from .sparse_flash_attention import D_ROPE, VALID_D, VALID_N1
 class SharedPrefixPlan:
     """Validated arguments of one shared_prefix_attention call (outputs, workspace, int32 index arrays),
     all in place when the constructor returns; ``run()`` launches on the current stream, which may be
-    another one. ``act_k`` (and the block table, where it was int32 and contiguous) are read on the
-    device in each run: a loop that keeps the plan may write them anew between runs."""
+    another one. Query, caches, ``act_k`` and the block table are read on the device in each run: a loop that
+    keeps the plan may write them anew between runs. Of an operand that was not contiguous, at a 16-byte border
+    and (the block table) int32, the plan reads its own copy (``q``, ``qr``, ``kk``, ``kr``, ``block_table``):
+    a cache that grows between runs has to be contiguous."""
 
     def __init__(self, query, key, value, block_table, prefix_length, scale_value=1.0, actual_seq_lengths_query=None,
                  actual_seq_lengths_kv=None, query_rope=None, key_rope=None, layout_query="BSND", layout_kv="PA_BSND",

@@ -364,6 +364,46 @@ def test_append_plan_replays_with_new_lengths():
         assert torch.equal(c[:, :, 0].cpu(), want), step
 
 
+def test_append_plan_is_in_place_when_built(monkeypatch):
+    """A plan's own copies (here of norm weights with a stride) are made before the wait in its constructor:
+    a run on another stream right after it reads them, however busy the building stream is then."""
+    from dsa_triton_ascend_amd import _host
+
+    upload = _host.upload
+
+    def upload_then_busy(*args, **kw):
+        lengths = upload(*args, **kw)
+        torch.cuda._sleep(100_000_000)
+        return lengths
+
+    g = torch.Generator().manual_seed(21)
+    table = torch.arange(2, dtype=torch.int32, device="cuda").view(1, 2)
+    x = torch.randn(1, 3, 1, 512, generator=g).bfloat16().cuda()
+    k = torch.randn(1, 3, 1, 128, generator=g).bfloat16().cuda()
+    r = torch.zeros(1, 3, 1, 64, dtype=torch.bfloat16, device="cuda")
+    w = (1 + torch.rand(512, 2, generator=g)).cuda()
+    freq = freqs(32)
+    caches = lambda width: torch.zeros(2, 16, 1, width, dtype=torch.bfloat16, device="cuda")
+    want = dsa.latent_cache_append(x, r, caches(512), caches(64), table, freq, [3], norm_weight=w[:, 0].contiguous())[0].cpu()
+    want_k = dsa.index_cache_append(k, caches(128), table, freq, [3], norm_weight=w[:128, 0].contiguous(),
+                                    norm_bias=w[:128, 1].contiguous()).cpu()
+    c, rc, ck = caches(512), caches(64), caches(128)
+    torch.cuda.synchronize()
+    monkeypatch.setattr(_host, "upload", upload_then_busy)
+    build, other = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(build):
+        plan = dsa.LatentAppendPlan(x, r, c, rc, table, freq, [3], norm_weight=w[:, 0])
+        with torch.cuda.stream(other):
+            plan.run()
+        other.synchronize()
+        keys = dsa.IndexAppendPlan(k, ck, table, freq, [3], norm_weight=w[:128, 0], norm_bias=w[:128, 1])
+        with torch.cuda.stream(other):
+            keys.run()
+        other.synchronize()
+    torch.cuda.synchronize()
+    assert torch.equal(c.cpu(), want) and torch.equal(ck.cpu(), want_k)
+
+
 @pytest.mark.parametrize("sections", [None, (8, 12, 12)])
 def test_prefill_rotates(sections):
     """dsa_prefill with inverse frequencies: the bits of rotating first and calling it as before, from a
