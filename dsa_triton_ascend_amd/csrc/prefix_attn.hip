@@ -226,7 +226,10 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   uint4 qf[KSN];   // the latent part; the rotary part stays in LDS
   uint8_t* const qs = L.own_nope[wave];
   const int hb = it.h0 + wave * 32;
-  if (hb < it.h_end) stage_q<D>(a.q, hb, min(32, it.h_end - hb), qs, lane);
+  // (a wave behind the last head row takes that one: the scores of whatever the LDS holds would grow, and
+  // rescale the outputs, every few tiles, 2.7 us a tile instead of 1.5)
+  const int hq = min(hb, it.h_end - 1);
+  stage_q<D>(a.q, hq, min(32, it.h_end - hq), qs, lane);
   uint4 qrv[4];
   {
     const uint16_t* qr = a.qr + (int64_t)(valid ? h : it.h_end - 1) * DR + kg * 8;
@@ -600,7 +603,8 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
   int b = it.b >= 0 ? it.b : batch_guess(a, row);
   Seq seq = it.b >= 0 ? it.seq : seq_of(a, b);
   asm volatile("" ::: "memory");
-  if (hb < it.h_end) stage_q<D>(a.q, hb, min(32, it.h_end - hb), L.own_nope[wave], lane);   // each wave for itself
+  const int hq = min(hb, it.h_end - 1);   // (as in run_item)
+  stage_q<D>(a.q, hq, min(32, it.h_end - hq), L.own_nope[wave], lane);   // each wave for itself
   uint4 qf[KS];
   {
     const uint16_t* qr = a.qr + (int64_t)(valid ? h : it.h_end - 1) * DR + kg * 8;
@@ -913,13 +917,16 @@ __global__ __launch_bounds__(NWV * 64) void prefix_attn_kernel(PfxK a) {
   __shared__ __attribute__((aligned(16))) PfxLds<D> L;
   Item it;
   int mt;
-  // Work-groups go round the eight XCDs, each with an L2 of its own: XCD x takes the prefix ranges x, x + 8, ..
-  // for all tiles (so their latents come from HBM once), then own items up to an even count: dense
-  // indexes row by row where XCDs are free, or (joined, at least eight ranges) a run of ranges per XCD.
+  // Work-groups go round the eight XCDs, each with an L2 of its own and 32 CUs: XCD x takes an eighth of the
+  // prefix items, numbered range by range (so a range's latents come from HBM once or twice, and no XCD has
+  // an item more than another, which cost a round of them where whole ranges went to one: 84 us instead of 58
+  // for 34 ranges of 7 tiles), then own items up to an even count: dense indexes row by row, or (joined, at
+  // least eight ranges) a run of ranges per XCD.
   const int x = blockIdx.x & 7, j = blockIdx.x >> 3;
-  const int rem = a.p_splits & 7, lo = a.p_splits / 8 * a.p_tiles, hi = lo + (rem ? a.p_tiles : 0);
+  const int np = a.p_splits * a.p_tiles, rem = np & 7, lo = np >> 3, hi = lo + (rem ? 1 : 0);
   if (j < (x < rem ? hi : lo)) {
-    const int sp = x + 8 * (j / a.p_tiles), tile = j % a.p_tiles;
+    const int i = x * lo + min(x, rem) + j;
+    const int sp = i / a.p_tiles, tile = i - sp * a.p_tiles;
     mt = a.p_mt;
     it.h0 = tile * 32 * mt;
     it.h_end = a.rows * a.n1;
@@ -1271,13 +1278,12 @@ hipError_t launch_prefix_attn(const PrefixArgs& a, hipStream_t s) {
   k.o_chunk = c.o_chunk;
   k.o_base = c.o_base;
   k.slots = c.slots;
-  const int most = (c.p_splits + 7) / 8 * c.p_tiles;   // prefix items of an XCD
   const int64_t even = (int64_t)a.batch * c.o_tiles, through = (int64_t)a.total_rows * a.n1 / (32 * c.o_mt) + a.batch;
   k.o_compact = even > through + through / 2;
   k.o_items = (int)(k.o_compact ? through : even);
   const int64_t all = (int64_t)c.p_splits * c.p_tiles + (int64_t)k.o_items * c.o_splits;
   if (all > INT_MAX - 16) return hipErrorInvalidConfiguration;
-  k.per_xcd = (int)std::max<int64_t>(most, (all + 7) / 8);
+  k.per_xcd = (int)((all + 7) / 8);
   k.o_by_range = c.p_splits == 0 && c.o_splits >= 8;
   return a.io == DSA_DTYPE_BF16 ? launch_io<IO_BF16>(k, a.d, s) : launch_io<IO_F16>(k, a.d, s);
 }
