@@ -11,7 +11,13 @@ Drop-in operators with the reference's Python signatures:
 and :class:`PrefillPlan` / :func:`dsa_prefill`, the two chained on one packed
 (TND) batch with the indexer's top-k feeding the attention in place.
 
-Both run hand-written gfx950 HIP kernels through the C ABI of
+Beside them, what a model needs around these paths:
+
+* :func:`rotary_embedding` / :func:`rotary_embedding_grad` — rotary positions
+* :func:`latent_cache_append`, :func:`index_cache_append` — new tokens into the paged caches
+* :func:`shared_prefix_attention` — dense attention over a paged cache, a common prefix computed once
+
+All run hand-written gfx950 HIP kernels through the C ABI of
 ``libdsa_mi355x.so`` (include/dsa_mi355x.h); PyTorch tensors are only buffers.
 """
 from .lightning_indexer import LightningIndexer, lightning_indexer
@@ -27,11 +33,13 @@ from .rotary import (IndexAppendPlan, LatentAppendPlan, RotaryEmbedding, index_c
                      rotary_embedding, rotary_embedding_grad)
 from .shared_prefix import SharedPrefixAttention, SharedPrefixPlan, shared_prefix_attention
 
-__all__ = ["shared_prefix_attention", "SharedPrefixAttention", "SharedPrefixPlan", "rotary_embedding", "rotary_embedding_grad", "RotaryEmbedding", "latent_cache_append", "LatentAppendPlan",
-           "index_cache_append", "IndexAppendPlan", "lightning_indexer", "LightningIndexer", "sparse_flash_attention", "SparseFlashAttention",
+__all__ = ["lightning_indexer", "LightningIndexer", "sparse_flash_attention", "SparseFlashAttention",
            "sparse_flash_attention_grad", "SparseFlashAttentionGrad", "sparse_lightning_indexer_grad_kl_loss",
            "SparseLightningIndexerGradKLLoss", "dense_lightning_indexer_softmax_lse",
            "npu_dense_lightning_indexer_softmax_lse", "dense_loss_backward",
            "dense_lightning_indexer_grad_kl_loss", "npu_dense_lightning_indexer_grad_kl_loss",
            "DenseLightningIndexerSoftmaxLse", "DenseLossBackward", "DenseLightningIndexerGradKLLoss",
-           "PrefillPlan", "dsa_prefill"]
+           "PrefillPlan", "dsa_prefill",
+           "rotary_embedding", "rotary_embedding_grad", "RotaryEmbedding", "latent_cache_append", "LatentAppendPlan",
+           "index_cache_append", "IndexAppendPlan", "shared_prefix_attention", "SharedPrefixAttention",
+           "SharedPrefixPlan"]

@@ -1116,7 +1116,7 @@ int up(int x, int to) { return (x + to - 1) / to * to; }
 // time): an item costs 6 (its rows' sequences, Q, first tile, ends) and 1.55 / 0.95 per 32 tokens for 128 / 64
 // head rows or 3.7 per 128 tokens for 32; the latents come at 4.9 TB/s; partial outputs are written at 7 TB/s,
 // and the join is a launch of 6 that reads them at 6 TB/s. It is there to weigh rounds of items against partials: at 64 x 16 heads
-// after 8192 tokens 16 prefix ranges take 50 us, 8 take 70 and 32 take 70 as well.
+// after 8192 tokens 16 prefix ranges take 47 us, 8 take 65 and 32 take 65 as well.
 struct Model {
   double scale;   // of a tile's products against D = 512
   double item(int mt, int tokens) const {
@@ -1130,8 +1130,8 @@ double cut_cost(const Model& md, const Cut& c, int d, double own_tiles, int own_
   const double tp = c.p_splits ? md.item(c.p_mt, c.p_chunk) : 0.0;
   const double no = own_tiles * std::min((double)c.o_splits, own_mean / c.o_chunk + (c.o_splits > 1 ? 0.5 : 1.0));
   const double to = own_max > 0 ? md.item(c.o_mt, std::min(c.o_chunk, own_max)) : 3.0;
-  // items past the CUs wait for whole ones, also where others end at once (17 prefix ranges instead of 16
-  // in the example, 272 work-groups: 52 -> 64 us): half an item at least
+  // items past the CUs wait for whole ones, also where others end at once (18 prefix ranges instead of 16
+  // in the example, 272 work-groups: 47 -> 61 us): half an item at least
   const double n = np + no, grid = np + own_tiles * c.o_splits, longest = std::max(tp, to);
   const double mean = (np * tp + no * to) / std::max(n, 1.0);
   double us = longest + (grid > 256.0 ? mean * std::max(std::max(n, 256.0) / 256.0 - 1.0, 0.45) : 0.0);
