@@ -1112,15 +1112,20 @@ struct Cut {
 int mt_for(int64_t head_rows) { return head_rows > 64 ? 4 : head_rows > 32 ? 2 : 1; }
 int up(int x, int to) { return (x + to - 1) / to * to; }
 
-// Microseconds of a call by a simple model of what was measured at D = 512 (256 CUs, one item each at a
-// time): an item costs 6 (its rows' sequences, Q, first tile, ends) and 1.55 / 0.95 per 32 tokens for 128 / 64
-// head rows or 3.7 per 128 tokens for 32; the latents come at 4.9 TB/s; partial outputs are written at 7 TB/s,
-// and the join is a launch of 6 that reads them at 6 TB/s. It is there to weigh rounds of items against partials: at 64 x 16 heads
-// after 8192 tokens 16 prefix ranges take 47 us, 8 take 65 and 32 take 65 as well.
+// Microseconds of a call by a simple model of what was measured (256 CUs, one item each at a time): an item
+// costs 6 (its rows' sequences, Q, first tile, ends) and, at D = 512 / 128, per 32 tokens 1.55 / 0.93 for 128
+// head rows, 0.95 / 0.71 for 64, or per 128 tokens 3.7 / 3.0 for 32 (narrow latents: the tile's chain of loads,
+// softmax and waits, not its products); the latents come at 4.9 TB/s; partial outputs are written at 7 TB/s,
+// and the join is a launch of 6 that reads them at 6 TB/s. It is there to weigh rounds of items against
+// partials: at 64 x 16 heads after 8192 tokens 16 prefix ranges take 47 us, 8 take 65 and 32 take 65 as well.
 struct Model {
-  double scale;   // of a tile's products against D = 512
+  int d;
+  double tokens32(int mt) const {   // 32 tokens of an item
+    return mt == 4 ? 0.72 + 1.62e-3 * d : mt == 2 ? 0.63 + 6.25e-4 * d : 0.6875 + 4.6e-4 * d;
+  }
   double item(int mt, int tokens) const {
-    return 6.0 + scale * (mt == 4 ? 1.55 * ((tokens + 31) / 32) : mt == 2 ? 0.95 * ((tokens + 31) / 32) : 3.7 * ((tokens + 127) / 128));
+    const int gran = mt == 1 ? 4 * BN : BN;
+    return 6.0 + tokens32(mt) * ((tokens + gran - 1) / gran * (gran / BN));
   }
 };
 
@@ -1149,7 +1154,7 @@ double cut_cost(const Model& md, const Cut& c, int d, double own_tiles, int own_
 Cut make_cut(int batch, int rows, int n1, int d, int prefix, int max_rows, int max_kv, int64_t total_kv, int kv_splits) {
   const int64_t m = (int64_t)rows * n1;
   const double mean = (double)total_kv / batch;
-  const Model md{(2 * d + 64) / 1088.0};
+  const Model md{d};
   const double latents_mb = (prefix + std::max(mean - prefix, 0.0) * batch) * (d + 64) * 2e-6;
   Cut c{}, best{};
   double least = 1e300;
@@ -1182,7 +1187,7 @@ Cut make_cut(int batch, int rows, int n1, int d, int prefix, int max_rows, int m
     c.p_splits = (prefix + c.p_chunk - 1) / c.p_chunk;
     // own ranges as long as a prefix range takes, or one
     const double fit = md.item(c.p_mt, c.p_chunk) - 6.0;
-    const double per = md.scale * (c.o_mt == 4 ? 1.55 / 32 : c.o_mt == 2 ? 0.95 / 32 : 3.7 / 128);
+    const double per = md.tokens32(c.o_mt) / BN;
     consider(own, own_mean, (int)std::ceil(own * per / std::max(fit, per * BN)));
     if (c.o_splits > 1) consider(own, own_mean, 1);
     if (s > 1 && c.p_chunk == gran) break;
