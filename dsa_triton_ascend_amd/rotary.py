@@ -142,33 +142,39 @@ class _AppendPlan:
 
     def _setup(self, x, caches, block_table, inv_freq, pairs, actual_seq_lengths_kv, actual_seq_lengths_query, positions,
                sections, layout, norm, more, what, _once):
+        shape, dtype = x.shape, x.dtype   # (each .shape builds an object: a call's time is its host path)
+        blocks = None
         for c, name in caches:
             if not isinstance(c, torch.Tensor) or not c.is_contiguous() or c.dim() != 4:
                 raise ValueError(f"{name} must be a contiguous tensor [num_blocks, block_size, N, D]")
-            if c.dtype != x.dtype:
-                raise ValueError(f"{name} dtype {c.dtype} differs from {what} dtype {x.dtype}")
-            if c.shape[:2] != caches[0][0].shape[:2]:
+            if c.dtype != dtype:
+                raise ValueError(f"{name} dtype {c.dtype} differs from {what} dtype {dtype}")
+            num_blocks, page, _, _ = c.shape
+            if blocks is not None and blocks != (num_blocks, page):
                 raise ValueError("the caches must have the same blocks")
+            blocks = num_blocks, page
         self.freq = _frequencies(inv_freq, pairs)
         self.axes, self.sec = _sections(sections, self.freq.numel())
         if positions is None and self.axes > 1:
             raise ValueError("several position axes need positions")
-        self.pos = None if positions is None else _positions(positions, x.shape[:-2], self.axes, self.sec is not None)
-        self.io = H.dtype_code(x.dtype, what)
+        self.pos = None if positions is None else _positions(positions, shape[:-2], self.axes, self.sec is not None)
+        self.io = H.dtype_code(dtype, what)
         self.wdt = self.io
         for w in norm:
             if w is not None:
                 self.wdt = H.dtype_code(w.dtype, "norm weights", allow_f32=True)
-                if w.dtype != norm[0].dtype or w.shape != (x.shape[-1],):
-                    raise ValueError(f"norm weights must share a dtype and have shape [{x.shape[-1]}]")
+                if w.dtype != norm[0].dtype or w.shape != (shape[-1],):
+                    raise ValueError(f"norm weights must share a dtype and have shape [{shape[-1]}]")
         if layout == "TND":
+            self.total_rows = shape[0]
             act_q = H.per_batch_from_cumsum(H.host_lengths(actual_seq_lengths_query)) \
-                if actual_seq_lengths_query is not None else [x.shape[0]]
+                if actual_seq_lengths_query is not None else [shape[0]]
             row_start = H.prefix(act_q)
-            if row_start[-1] > x.shape[0] or min(act_q, default=0) < 0:
+            if row_start[-1] > shape[0] or min(act_q, default=0) < 0:
                 raise ValueError("actual_seq_lengths_query must be cumulative and within the packed tokens")
         else:
-            B, S = x.shape[:2]
+            B, S = shape[0], shape[1]
+            self.total_rows = B * S
             act_q = H.batch_lengths(actual_seq_lengths_query, B, S, "actual_seq_lengths_query")
             if min(act_q, default=0) < 0 or max(act_q, default=0) > S:
                 raise ValueError(f"actual_seq_lengths_query must lie between 0 and S = {S}")
@@ -176,24 +182,23 @@ class _AppendPlan:
         act_k = H.host_lengths(actual_seq_lengths_kv)
         if len(act_k) != len(act_q):
             raise ValueError(f"batch mismatch: {len(act_q)} query batches, {len(act_k)} kv lengths")
-        if block_table.dim() != 2 or block_table.shape[0] != len(act_q):
+        table = block_table.shape
+        if len(table) != 2 or table[0] != len(act_q):
             raise ValueError("block_table must be [batch, max_blocks]")
-        self.num_blocks, self.page = caches[0][0].shape[:2]
-        self.batch, self.max_blocks = block_table.shape
-        self.total_rows = x.shape[0] * (x.shape[1] if layout == "BSND" else 1)
+        self.num_blocks, self.page = num_blocks, page = blocks
+        self.batch, self.max_blocks = batch, max_blocks = table
         if self.total_rows >= 2 ** 31:
             raise ValueError("2^31 tokens or more")
         for k in act_k:
-            if k < 0 or k > self.max_blocks * self.page:
-                raise ValueError(f"kv length {k} outside the block table's {self.max_blocks * self.page} tokens")
+            if k < 0 or k > max_blocks * page:
+                raise ValueError(f"kv length {k} outside the block table's {max_blocks * page} tokens")
         self.dev = H.require_device(self.x, block_table, self.freq, self.pos, *norm, *more, *[c for c, _ in caches])
         self.norm = tuple(None if w is None else w.contiguous() for w in norm)   # before the upload that is waited for
         self.lib = _lib.load()
         self.args = None   # of the launch, but for the stream; None: nothing to do
-        if not (self.batch and self.total_rows and self.max_blocks and self.num_blocks and self.page):
+        if not (batch and self.total_rows and max_blocks and num_blocks and page):
             return None, None
 
-        batch = self.batch
         if _once and batch <= ARG_SEQUENCES:   # the lengths go with the call: no upload before it
             self.block_table = block_table.to(torch.int32).contiguous()
             self.lengths = array("i", row_start + act_q + act_k)
@@ -208,8 +213,8 @@ class _AppendPlan:
             lengths = (self.row_start.data_ptr(), self.act_q.data_ptr(), self.act_k.data_ptr(), False)
         rotation = (H.ptr(self.pos), self.pos is not None and self.pos.dtype == torch.int64, self.axes, self.sec,
                     self.freq.data_ptr())
-        return rotation, (*lengths, self.block_table.data_ptr(), batch, self.total_rows, self.per, self.max_blocks, self.page,
-                          self.num_blocks)
+        return rotation, (*lengths, self.block_table.data_ptr(), batch, self.total_rows, self.per, max_blocks, page,
+                          num_blocks)
 
     def _launch(self, entry, what):
         if self.args is not None:
@@ -224,16 +229,17 @@ class LatentAppendPlan(_AppendPlan):
                  interleaved=True, layout="BSND", *, _once=False):
         self.x, self.sb, self.ss, self.sh, self.per = _rows_view(latent, layout, "latent")
         self.rope, self.rb, self.rs, _, _ = _rows_view(key_rope, layout, "key_rope")
-        d = latent.shape[-1]
+        shape, rope_shape, cache_shape, rope_cache_shape = latent.shape, key_rope.shape, key_cache.shape, key_rope_cache.shape
+        d = shape[-1]
         if d not in VALID_D:
             raise ValueError(f"D must be one of {VALID_D}, got {d}")
         if key_rope.dtype != latent.dtype:
             raise ValueError(f"key_rope dtype {key_rope.dtype} differs from latent dtype {latent.dtype}")
-        if key_rope.shape[-1] != D_ROPE:
-            raise ValueError(f"rope dim must be {D_ROPE}, got {key_rope.shape[-1]}")
-        if latent.shape[-2] != 1 or key_rope.shape[:-1] != latent.shape[:-1]:
+        if rope_shape[-1] != D_ROPE:
+            raise ValueError(f"rope dim must be {D_ROPE}, got {rope_shape[-1]}")
+        if shape[-2] != 1 or rope_shape[:-1] != shape[:-1]:
             raise ValueError("Only N2=1 (MQA) is supported, key_rope as many tokens as latent")
-        if tuple(key_cache.shape[2:]) != (1, d) or tuple(key_rope_cache.shape[2:]) != (1, D_ROPE):
+        if cache_shape[2:] != (1, d) or rope_cache_shape[2:] != (1, D_ROPE):
             raise ValueError(f"caches must be [num_blocks, block_size, 1, {d}] and [.., 1, {D_ROPE}]")
         rotation, places = self._setup(latent, [(key_cache, "key_cache"), (key_rope_cache, "key_rope_cache")], block_table, inv_freq,
                     D_ROPE // 2, actual_seq_lengths_kv, actual_seq_lengths_query, positions, sections, layout,
