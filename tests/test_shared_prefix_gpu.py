@@ -141,6 +141,14 @@ def test_forced_splits(splits, case):
     check(call(t, tokens, kv, prefix, 0.05, mode, packed, kv_splits=splits), want)
 
 
+@pytest.mark.parametrize("splits", [3, 5, 7, 11])
+def test_prefix_items_over_the_xcds(splits):
+    """Numbers of prefix items that eight does not divide, the last tile with rows of one wave only (816 head rows)."""
+    kv = [701 + b % 60 for b in range(51)]
+    t = make(BF, 16, 128, [1] * 51, kv, 700, 64, False, 400)
+    check(call(t, [1] * 51, kv, 700, 0.05, 3, False, kv_splits=splits), exact(t, [1] * 51, kv, 700, 0.05, 3, False))
+
+
 @pytest.mark.parametrize("n1", [1, 2, 4, 8, 16, 32, 64, 128])
 @pytest.mark.parametrize("d", [128, 256, 512])
 def test_head_counts(n1, d):
