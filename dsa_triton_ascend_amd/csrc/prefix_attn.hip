@@ -1042,7 +1042,8 @@ __global__ __launch_bounds__(SG > 1 ? SG * 64 : 256) void prefix_merge_kernel(Pf
     }
     for (int s = j; s < a.slots; s += LPR) {
       const float4 st = live ? ps[s] : make_float4(0.f, 0.f, 0.f, 0.f);
-      const float w = st.z != 0.f ? exp2f((st.x - M) * LOG2E) : 0.f;
+      // (a range whose scores are all NaN has no maximum, -inf: its weight is its sum, or the NaN would be left out)
+      const float w = st.z != st.z ? st.z : st.z != 0.f ? exp2f((st.x - M) * LOG2E) : 0.f;
       s_w[s][sr] = w;
       if (w != 0.f) sum += w * st.z;
     }
