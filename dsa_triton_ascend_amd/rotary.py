@@ -119,7 +119,7 @@ def rotary_embedding_grad(d_out, positions, inv_freq, sections=None, rotary_star
 
 
 class RotaryEmbedding(torch.nn.Module):
-    """Module form: keeps the inverse frequencies and the layout."""
+    """Module form: keeps the inverse frequencies (float32 through casts of the module) and the layout."""
 
     def __init__(self, inv_freq, sections=None, rotary_start=0, interleaved=True, layout="BSND"):
         super().__init__()
@@ -128,6 +128,13 @@ class RotaryEmbedding(torch.nn.Module):
         self.rotary_start = rotary_start
         self.interleaved = interleaved
         self.layout = layout
+
+    def _apply(self, fn, recurse=True):
+        freq = self.inv_freq   # follows the module's device, not its type: 16 bits would turn far positions wrongly
+        super()._apply(fn, recurse)
+        if self.inv_freq.dtype != freq.dtype:
+            self.inv_freq = freq.to(self.inv_freq.device)
+        return self
 
     def forward(self, x, positions):
         return rotary_embedding(x, positions, self.inv_freq, self.sections, self.rotary_start, self.interleaved, self.layout)

@@ -131,3 +131,18 @@ def test_prefill_refuses_positions_without_frequencies():
                         (dict(inv_freq=F, sections=(16, 16)), "need positions"), (dict(inv_freq=torch.ones(16)), "32 wanted")):
         with pytest.raises(ValueError, match=message):
             dsa.dsa_prefill(z, z, z, z, z, z, z, [4], **kw)
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.double(), lambda m: m.bfloat16().float(),
+                                  lambda m: m.to(torch.float16).to("cpu", torch.float32), lambda m: m.type(torch.bfloat16)])
+def test_module_keeps_its_frequencies_through_casts(cast):
+    """A model's cast to its type must not round the frequencies: 8 bits of them would turn far positions by
+    whole turns, and any other type than float32 is refused."""
+    f = 1.0 / 10000 ** (torch.arange(32) / 32)
+    model = torch.nn.Sequential(torch.nn.Linear(4, 4), dsa.RotaryEmbedding(f))
+    cast(model)
+    assert model[1].inv_freq.dtype == torch.float32 and torch.equal(model[1].inv_freq, f)
+    assert [n for n, _ in model.named_buffers()] == ["1.inv_freq"] and not any("inv_freq" in k for k in model.state_dict())
+    with pytest.raises(ValueError, match="GPU"):   # all that is left to refuse: X is on the CPU
+        model[1](X, POS)
+    assert model.to("meta")[1].inv_freq.device.type == "meta"
