@@ -202,7 +202,7 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
   // the softmax works on raw scores times a positive factor: a negative scale negates the query, a
   // zero one becomes 1e-30 (scores round to 0, masked ones stay -inf)
   const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-  const float cpos = a.scale > 0.f ? a.scale : a.scale < 0.f ? -a.scale : 1e-30f;
+  const float cpos = a.scale == 0.f ? 1e-30f : fabsf(a.scale);
   const float cl2 = cpos * LOG2E;
 
   // ---- block ids of the first tiles, requested before the item's end is known. Wave w copies tokens 8 w ..
@@ -587,7 +587,7 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
   const int kg = lane >> 5, rr = lane & 31;
   const int hb = it.h0 + rb * 32, h = hb + rr;
   const bool valid = h < it.h_end;
-  const float cpos = a.scale > 0.f ? a.scale : a.scale < 0.f ? -a.scale : 1e-30f;
+  const float cpos = a.scale == 0.f ? 1e-30f : fabsf(a.scale);
   const float cl2 = cpos * LOG2E;
 
   // the token that this lane looks up, its block requested before the item's end is known (tokens past it,

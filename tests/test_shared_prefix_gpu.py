@@ -339,3 +339,17 @@ def test_append_then_attend():
         check(call(t, nq, lens, 0, 0.04, 3, True), exact(t, nq, lens, 0, 0.04, 3, True))   # the rows' own tables agree
         a, b_ = (call(t, nq, lens, p, 0.04, 3, True)[0].double() for p in (P, 0))
         assert float((a - b_).abs().max()) < 2 ** -6 * float(a.abs().max())
+
+
+@pytest.mark.parametrize("n1", [8, 32, 128])
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf")])
+def test_scales_that_are_not_finite(scale, n1):
+    """The formula's scores are NaN or of infinite size then, and so no row that sees a token has a finite value; rows
+    that see none stay zeros."""
+    tokens, kv = [2, 2], [300, 1]
+    t = make(BF, n1, 128, tokens, kv, 200, 32, False, 17)
+    for splits in (1, 3):
+        out, _, total = call(t, tokens, kv, 200, scale, 3, False, kv_splits=splits)
+        seen = torch.tensor([[True, True], [False, True]])
+        assert torch.isnan(out[seen.cuda()]).all() and not out[1, 0].any()
+        assert not torch.isfinite(total.reshape(2, 2, n1)[0]).any() and not total.reshape(2, 2, n1)[1, 0].any()
