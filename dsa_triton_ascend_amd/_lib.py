@@ -57,6 +57,7 @@ SIGNATURES = {
     "dsa_prefix_attn": (_I, [_P, _P, _P, _P, _I, _P, _I, _I, _I64, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I64, _I, _F,
                              _P, _P, _P, _P, _SZ, _I, _P]),
     "dsa_rotary": (_I, [_P, _I64, _I64, _I64, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P]),
+    "dsa_row_positions": (_I, [_P, _I, _I, _P, _P]),
     "dsa_latent_append": (_I, [_P, _I64, _I64, _P, _I64, _I64, _I, _I, _P, _I, _F, _P, _I, _I, _P, _P, _I, _P, _P, _P, _I,
                                _P, _I, _I, _I, _I, _I, _I64, _P, _P, _P]),
     "dsa_index_append": (_I, [_P, _I64, _I64, _I64, _I, _I, _I, _P, _P, _I, _F, _P, _I, _I, _P, _P, _I, _I, _I, _P, _P,

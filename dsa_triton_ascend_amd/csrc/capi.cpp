@@ -570,6 +570,16 @@ int dsa_rotary(const void* x, int64_t batch_stride, int64_t row_stride, int64_t 
   return hip_status(launch_rotary(a, (hipStream_t)stream), "dsa_rotary launch");
 }
 
+int dsa_row_positions(const int32_t* row_start, int batch, int rows, int32_t* positions, void* stream) {
+  if (!row_start || !positions) return fail(DSA_ERR_INVALID, "dsa_row_positions: null pointer argument");
+  if (batch <= 0 || rows < 0) return fail(DSA_ERR_INVALID, "dsa_row_positions: non-positive shape");
+  if (rows == 0) {
+    g_err[0] = 0;
+    return DSA_OK;
+  }
+  return hip_status(launch_row_positions(row_start, batch, rows, positions, (hipStream_t)stream), "dsa_row_positions launch");
+}
+
 int dsa_latent_append(const void* latent, int64_t batch_stride, int64_t row_stride, const void* key_rope,
                       int64_t rope_batch_stride, int64_t rope_row_stride, int io_dtype, int d, const void* norm_weight,
                       int w_dtype, float eps, const void* positions, int positions_64, int axes, const int32_t* sections,

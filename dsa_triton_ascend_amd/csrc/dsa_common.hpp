@@ -496,6 +496,7 @@ struct RotaryArgs {
   void* out;
 };
 hipError_t launch_rotary(const RotaryArgs& a, hipStream_t s);
+hipError_t launch_row_positions(const int32_t* row_start, int batch, int rows, int32_t* positions, hipStream_t s);
 // New tokens into a paged cache: latents (rope != NULL: normed, beside their rotated rotary keys) or
 // indexer keys (rope NULL: normed and rotated)
 constexpr int APPEND_ARG_LENGTHS = 56;   // lengths_host: 3 batch + 1 values as kernel arguments

@@ -14,12 +14,9 @@ takes the attention's rotary parts unrotated and rotates them first (two launche
 """
 from __future__ import annotations
 
-import torch
-
 from . import _host as H
-from . import _lib
 from .lightning_indexer import IndexerPlan
-from .rotary import D_ROPE, _frequencies, _Rotation
+from .rotary import D_ROPE, _frequencies, _Rotation, _row_positions
 from .sparse_flash_attention import AttentionPlan
 
 
@@ -36,15 +33,8 @@ class PrefillPlan:
             if positions is None:
                 if sections is not None:
                     raise ValueError("several position axes need positions")
-                lengths = H.per_batch_from_cumsum(H.host_lengths(cu_seqlens))
-                rows = query_rope.shape[0]
-                within = [p for n in lengths for p in range(n)][:rows]
-                within += [0] * (rows - len(within))
-                dev = H.require_device(query_rope, key_rope, freq)
-                if torch.cuda.is_current_stream_capturing():   # a copy from the host could not be captured
-                    positions = H.upload(_lib.load(), dev, within)[0][:rows]
-                else:
-                    positions = torch.tensor(within, dtype=torch.int32).to(dev)
+                positions = _row_positions(H.per_batch_from_cumsum(H.host_lengths(cu_seqlens)), query_rope.shape[0],
+                                           H.require_device(query_rope, key_rope, freq))
             self.rotations = tuple(_Rotation(x, positions, freq, sections, 0, interleaved, "TND", 0, what)
                                    for x, what in ((query_rope, "query_rope"), (key_rope, "key_rope")))
             query_rope, key_rope = (r.out for r in self.rotations)

@@ -69,6 +69,21 @@ def _rows_view(x: torch.Tensor, layout: str, what: str):
     return x, 0, stride[0], stride[1], max(1, x.shape[0])
 
 
+def _row_positions(lengths, rows: int, dev) -> torch.Tensor:
+    """int32 [rows]: each packed row's place in its sequence, 0 behind the last, written on the current stream"""
+    def place():
+        if not lengths:
+            return torch.zeros(rows, dtype=torch.int32, device=dev)
+        lib = _lib.load()
+        row_start, = H.upload(lib, dev, H.prefix(lengths), wait=False)
+        out = torch.empty(rows, dtype=torch.int32, device=dev)
+        _lib.check(lib.dsa_row_positions(row_start.data_ptr(), len(lengths), rows, out.data_ptr(), H.stream_ptr(dev)),
+                   "dsa_row_positions")
+        return out
+
+    return H.on_device(dev, place)
+
+
 class _Rotation:
     """Validated arguments of one rotation and its output; ``run()`` launches on the current stream."""
 

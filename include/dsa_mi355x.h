@@ -388,6 +388,12 @@ int dsa_rotary(const void* x, int64_t batch_stride, int64_t row_stride, int64_t 
                int inverse, void* out, void* stream);
 
 /*
+ * positions[r] = r - row_start[b] for the rows r of packed sequence b (row_start [batch + 1] on the device,
+ * ascending from 0), 0 for rows behind the last: dsa_rotary's positions of a prefill. positions [rows].
+ */
+int dsa_row_positions(const int32_t* row_start, int batch, int rows, int32_t* positions, void* stream);
+
+/*
  * Appends new tokens' latents and rotary keys to the paged caches that dsa_sfa_fwd and
  * dsa_prefix_attn read (no counterpart in the reference). Packed row r is token s1 = r -
  * row_start[b] of batch b, at position p = act_k[b] - act_q[b] + s1 of its sequence (act_k counts the

@@ -146,3 +146,12 @@ def test_module_keeps_its_frequencies_through_casts(cast):
     with pytest.raises(ValueError, match="GPU"):   # all that is left to refuse: X is on the CPU
         model[1](X, POS)
     assert model.to("meta")[1].inv_freq.device.type == "meta"
+
+
+def test_row_positions_refuses():
+    lib = _lib.load()
+    p = ctypes.c_void_p(16)   # never dereferenced
+    for args, what in (((None, 1, 4, p, None), "null"), ((p, 1, 4, None, None), "null"), ((p, 0, 4, p, None), "shape"),
+                       ((p, 1, -1, p, None), "shape")):
+        assert lib.dsa_row_positions(*args) == _lib.DSA_ERR_INVALID and what in lib.dsa_last_error().decode()
+    assert lib.dsa_row_positions(p, 1, 0, p, None) == 0   # no rows: no launch

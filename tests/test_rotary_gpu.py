@@ -472,3 +472,34 @@ def test_prefill_then_sparse_attention():
     out2, _, _ = dsa.sparse_flash_attention(q.to(dev), k.to(dev), k.to(dev), idx, 576 ** -0.5, query_rope=qrot,
                                             key_rope=kr.to(dev), sparse_mode=3)
     assert float((out.float() - out2.float()).abs().max()) <= 2 ** -6 * float(out2.float().abs().max())
+
+
+@pytest.mark.parametrize("lengths,tail", [([5], 0), ([0, 3, 0, 0, 300, 1], 9), ([257] * 70 + [0], 0), ([0], 3), ([], 4)])
+def test_row_positions(lengths, tail):
+    from dsa_triton_ascend_amd.rotary import _row_positions
+    rows = sum(lengths) + tail
+    want = [p for n in lengths for p in range(n)] + [0] * tail
+    assert _row_positions(lengths, rows, torch.device("cuda")).tolist() == want
+
+
+def test_prefill_makes_its_positions_without_waiting():
+    """A one-shot dsa_prefill that rotates only queues work: the host does not wait for what runs before it."""
+    g = torch.Generator().manual_seed(15)
+    lens, dt = [300, 0, 212], torch.bfloat16
+    T, cu = sum(lens), torch.tensor(lens).cumsum(0).tolist()
+    r = lambda *s: torch.randn(*s, generator=g).to(dt).cuda()
+    args = (r(T, 32, 128), r(T, 1, 128), torch.randn(T, 32, generator=g).cuda(), r(T, 16, 512), r(T, 1, 512), r(T, 16, 64),
+            r(T, 1, 64), cu)
+    kw = dict(sparse_count=64, scale_value=0.04)
+    f = freqs(32)
+    pos = torch.cat([torch.arange(n) for n in lens]).cuda()
+    want = dsa.dsa_prefill(*args, inv_freq=f, positions=pos, **kw)
+    dsa.dsa_prefill(*args, inv_freq=f, **kw)   # the allocator has its memory
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)
+    before = torch.cuda.Event()
+    before.record()
+    got = dsa.dsa_prefill(*args, inv_freq=f, **kw)
+    assert not before.query()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
