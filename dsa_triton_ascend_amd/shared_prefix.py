@@ -50,7 +50,8 @@ class SharedPrefixPlan:
         if key.shape[-1] != D or query_rope.shape[:-1] != query.shape[:-1] or key_rope.shape[:-1] != key.shape[:-1]:
             raise ValueError("query, query_rope, key and key_rope shapes do not match")
         if layout_query == "TND":
-            act_q = H.per_batch_from_cumsum(H.host_lengths(actual_seq_lengths_query))
+            act_q = [query.shape[0]] if actual_seq_lengths_query is None \
+                else H.per_batch_from_cumsum(H.host_lengths(actual_seq_lengths_query))
             total_rows, per = query.shape[0], max(act_q, default=0)
             row_start = H.prefix(act_q)
             if row_start[-1] > total_rows or min(act_q, default=0) < 0:
@@ -122,7 +123,7 @@ def shared_prefix_attention(query, key, value, block_table, prefix_length, scale
     """Dense attention over a paged latent cache; the first `prefix_length` tokens of all sequences are
     the same and are computed for the whole batch at once.
 
-    query [B,S,N1,D] (BSND) or [T,N1,D] (TND, cumulative actual_seq_lengths_query) and query_rope [..,64],
+    query [B,S,N1,D] (BSND) or [T,N1,D] (TND, cumulative actual_seq_lengths_query; None: one sequence) and query_rope [..,64],
     fp16 / bf16; key [num_blocks, block_size, 1, D] and key_rope [.., 64] (`value` is ignored: value = key,
     as in sparse_flash_attention); block_table [B, max_blocks]; actual_seq_lengths_kv: each sequence's
     length, prefix included (default: the whole table). Tokens below prefix_length are read through

@@ -77,3 +77,10 @@ def test_workspace_is_bounded(batch, rows, n1, d, prefix, most, kv):
         assert w % 16 == 0 and w <= 256 * ((rows * n1 + 32 * (batch + 5)) * 4 * d + rows * n1 * 16) + 256
         if splits == 0:
             assert w <= 1 << 30
+
+
+def test_packed_without_lengths_is_one_sequence():
+    a = args(query=Z(6, 16, 512), query_rope=Z(6, 16, 64), layout_query="TND")
+    for change, message in ((dict(), "block_table"), (dict(block_table=Z(1, 4, dtype=torch.int32), actual_seq_lengths_kv=[40]), "GPU")):
+        with pytest.raises(ValueError, match=message):
+            dsa.shared_prefix_attention(**{**a, **change})

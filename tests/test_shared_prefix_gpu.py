@@ -353,3 +353,10 @@ def test_scales_that_are_not_finite(scale, n1):
         seen = torch.tensor([[True, True], [False, True]])
         assert torch.isnan(out[seen.cuda()]).all() and not out[1, 0].any()
         assert not torch.isfinite(total.reshape(2, 2, n1)[0]).any() and not total.reshape(2, 2, n1)[1, 0].any()
+
+
+def test_packed_without_lengths_is_one_sequence():
+    t = make(BF, 16, 128, [37], [300], 0, 32, True, 18)
+    kw = dict(actual_seq_lengths_kv=[300], query_rope=t["qr"], key_rope=t["kr"], layout_query="TND", return_softmax_lse=True)
+    got = dsa.shared_prefix_attention(t["q"], t["k"], t["k"], t["table"], 0, 0.05, **kw)
+    check(got, exact(t, [37], [300], 0, 0.05, 3, True))
