@@ -542,6 +542,7 @@ int check_append(const char* fn, const void* x, int io_dtype, const void* norm_w
     return fail(DSA_ERR_INVALID, "%s: norm weights must be fp16, bf16 or fp32", fn);
   if (batch <= 0 || total_rows < 0 || rows_per_batch < 1 || max_blocks <= 0 || page_block_size <= 0 || num_blocks <= 0)
     return fail(DSA_ERR_INVALID, "%s: non-positive shape", fn);
+  if (total_rows > INT_MAX - 4096) return fail(DSA_ERR_UNSUPPORTED, "%s: %d rows, 2^31 - 4096 or more", fn, total_rows);
   if (((uintptr_t)cache & 15) != 0) return fail(DSA_ERR_INVALID, "%s: caches must be 16-byte aligned", fn);
   if (lengths_host && batch > (APPEND_ARG_LENGTHS - 1) / 3)
     return fail(DSA_ERR_UNSUPPORTED, "%s: host lengths of at most %d sequences, got %d", fn, (APPEND_ARG_LENGTHS - 1) / 3, batch);
@@ -561,6 +562,7 @@ int dsa_rotary(const void* x, int64_t batch_stride, int64_t row_stride, int64_t 
   if (st != DSA_OK) return st;
   if (width > 4096 || (int64_t)heads * width > (1 << 20))
     return fail(DSA_ERR_UNSUPPORTED, "dsa_rotary: width %d > 4096, or heads * width > 2^20", width);
+  if (rows > INT_MAX - 4096) return fail(DSA_ERR_UNSUPPORTED, "dsa_rotary: %d rows, 2^31 - 4096 or more", rows);
   if (rows == 0) {
     g_err[0] = 0;
     return DSA_OK;

@@ -21,6 +21,14 @@ namespace {
 constexpr int TPB = 256;
 constexpr double INV_2PI = 0.15915494309189533577;
 
+// A launch holds fewer than 2^32 threads in x: work-groups past GRID_X of them go on in z. (Rows end 4096 short of
+// 2^31, so that the last group's row numbers do not overflow: the entries refuse more.)
+constexpr int GRID_X = 1 << 23;
+__device__ __forceinline__ int group_id() { return (int)blockIdx.z * GRID_X + (int)blockIdx.x; }
+dim3 grid_of(int64_t groups, unsigned y) {
+  return dim3((unsigned)std::min<int64_t>(groups, GRID_X), y, (unsigned)((groups + GRID_X - 1) / GRID_X));
+}
+
 // Rows of a [batch, rows_per_batch, heads, width] view: elements between them
 struct View {
   int64_t batch, row, head;
@@ -121,7 +129,8 @@ __global__ __launch_bounds__(TPB) void rotary_kernel(RotaryK a) {
   extern __shared__ float2 tab[];                   // [group][rdim / 2]
   const int half = a.rdim / 2;
   const int upr = a.heads * a.uph;
-  const int r0 = blockIdx.x * a.group;
+  if ((int64_t)group_id() * a.group >= a.rows) return;   // (of the last z, the whole group)
+  const int r0 = group_id() * a.group;
   const int nrot = V == 1 ? half : INTER ? a.rdim / V : half / V;   // rotating units of a head
   const T* x = reinterpret_cast<const T*>(a.x);
   T* out = reinterpret_cast<T*>(a.out);
@@ -223,7 +232,7 @@ hipError_t launch_rotary_v(RotaryK k, hipStream_t s) {
   // enough work-groups of four units a thread to fill the chip twice over
   const bool many = upr >= 4 * TPB && (int64_t)k.rows * upr >= (int64_t)4 * TPB * 4096;
   const int per = TPB * (many ? 4 : 1);
-  const dim3 grid((k.rows + k.group - 1) / k.group, upr >= TPB ? (upr + per - 1) / per : 1);
+  const dim3 grid = grid_of(((int64_t)k.rows + k.group - 1) / k.group, upr >= TPB ? (upr + per - 1) / per : 1);
   if (many) hipLaunchKernelGGL((rotary_kernel<IO, V, INTER, 4>), grid, dim3(TPB), lds, s, k);
   else hipLaunchKernelGGL((rotary_kernel<IO, V, INTER, 1>), grid, dim3(TPB), lds, s, k);
   return hipGetLastError();
@@ -411,7 +420,8 @@ __global__ __launch_bounds__(TPB) void append_kernel(AppendK a, Lens lens) {
   __shared__ int64_t s_row[NTOK];   // the token's cache row, -1: it has none
   __shared__ int s_pos[NTOK];
   constexpr int VPP = TPB / LPV;    // vectors a pass of the work-group
-  const int r0 = blockIdx.x * NTOK;
+  if ((int64_t)group_id() * NTOK >= a.total_rows) return;
+  const int r0 = group_id() * NTOK;
   const int li = threadIdx.x % LPV, vi = threadIdx.x / LPV;
   const int heads = LATENT ? 1 : a.a.heads, half = LATENT ? 32 : a.rdim / 2;
   const int nvec = NTOK * heads;
@@ -501,7 +511,7 @@ __global__ __launch_bounds__(TPB) void append_kernel(AppendK a, Lens lens) {
 
 template <int IO, bool LATENT, int NTOK, typename Lens>
 hipError_t launch_append_n(const AppendK& k, const Lens& l, hipStream_t s) {
-  const dim3 grid((k.total_rows + NTOK - 1) / NTOK);
+  const dim3 grid = grid_of(((int64_t)k.total_rows + NTOK - 1) / NTOK, 1);
   const size_t lds = (size_t)NTOK * (k.rdim / 2) * sizeof(float2);
   if (!LATENT && k.a.width <= 64) hipLaunchKernelGGL((append_kernel<IO, 8, LATENT, NTOK, Lens>), grid, dim3(TPB), lds, s, k, l);
   else if (k.a.width <= 128) hipLaunchKernelGGL((append_kernel<IO, 16, LATENT, NTOK, Lens>), grid, dim3(TPB), lds, s, k, l);

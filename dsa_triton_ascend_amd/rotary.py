@@ -21,6 +21,7 @@ VALID_D = (128, 256, 512)
 D_ROPE = 64
 INDEX_WIDTHS = (64, 96, 128, 256, 512)
 ARG_SEQUENCES = 18   # sequences whose lengths a call takes from the host
+MAX_ROWS = 2 ** 31 - 1 - 4096   # tokens a call takes
 
 
 def _frequencies(inv_freq, pairs=None) -> torch.Tensor:
@@ -94,12 +95,12 @@ class _Rotation:
         pairs = freq.numel()
         axes, sec = _sections(sections, pairs)
         shape = x.shape
-        pos = _positions(positions, shape[:-2], axes, sec is not None)
         n, width = shape[-2:]
+        if x.numel() // max(1, n * width) > MAX_ROWS:
+            raise ValueError(f"more than {MAX_ROWS} tokens")
+        pos = _positions(positions, shape[:-2], axes, sec is not None)
         if rotary_start < 0 or rotary_start + 2 * pairs > width:
             raise ValueError(f"rotary dimensions [{rotary_start}, {rotary_start} + {2 * pairs}) of a width of {width}")
-        if x.numel() // max(1, n * width) >= 2 ** 31:
-            raise ValueError("2^31 tokens or more")
         self.dev = H.require_device(x, pos, freq)
         self.lib = _lib.load()
         self.out = out = torch.empty_like(x, memory_format=torch.contiguous_format)   # (half of torch.empty's time)
@@ -209,8 +210,8 @@ class _AppendPlan:
             raise ValueError("block_table must be [batch, max_blocks]")
         self.num_blocks, self.page = num_blocks, page = blocks
         self.batch, self.max_blocks = batch, max_blocks = table
-        if self.total_rows >= 2 ** 31:
-            raise ValueError("2^31 tokens or more")
+        if self.total_rows > MAX_ROWS:
+            raise ValueError(f"more than {MAX_ROWS} tokens")
         for k in act_k:
             if k < 0 or k > max_blocks * page:
                 raise ValueError(f"kv length {k} outside the block table's {max_blocks * page} tokens")
@@ -319,8 +320,8 @@ def latent_cache_append(latent, key_rope, key_cache, key_rope_cache, block_table
     latent [B,S,1,D] (BSND) or [T,1,D] (TND), key_rope [..,1,64]; key_cache [num_blocks, block_size, 1, D]
     and key_rope_cache [.., 64], contiguous; block_table [B, max_blocks]; actual_seq_lengths_kv: each
     sequence's length with its new tokens (per batch, as for the paged reads); actual_seq_lengths_query:
-    how many tokens are new (per batch, BSND; cumulative, TND). Token s of batch b goes to position
-    kv - query + s of its sequence, and turns by that position or by `positions` (as in
+    how many tokens are new (per batch, BSND; cumulative, TND; None: all of S, or one packed sequence).
+    Token s of batch b goes to position kv - query + s of its sequence, and turns by that position or by `positions` (as in
     :func:`rotary_embedding`). norm_weight [D]: root-mean-square norm of the latent (None: stored as it
     is). Tokens before position 0, or whose block is -1 or outside the cache, are not stored; no other
     row of the caches changes. Two new tokens must not share a place. Returns the two caches."""

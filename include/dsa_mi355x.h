@@ -380,7 +380,8 @@ int dsa_dense_li_grad_kl_loss(const void* query, const void* key, const void* qu
  *     contiguous, not overlapping x. One rounding, from 32 bits.
  *   positions: [axes, rows] int32, or int64 if positions_64; 1 <= axes <= 4. sections (host memory,
  *     [axes], NULL with one axis): axis a has the next sections[a] pairs; they add up to rotary_dim / 2.
- *   inv_freq [rotary_dim / 2] fp32. rotary_dim even, at most 1024; width <= 4096; heads * width <= 2^20.
+ *   inv_freq [rotary_dim / 2] fp32. rotary_dim even, at most 1024; width <= 4096; heads * width <= 2^20;
+ *   rows < 2^31 - 4096.
  */
 int dsa_rotary(const void* x, int64_t batch_stride, int64_t row_stride, int64_t head_stride, int dtype,
                const void* positions, int positions_64, int axes, const int32_t* sections, const float* inv_freq,
@@ -406,6 +407,7 @@ int dsa_row_positions(const int32_t* row_start, int batch, int rows, int32_t* po
  *   latent [.., d], key_rope [.., 64] (one head) by batch and row strides in elements as dsa_rotary
  *   (rows_per_batch >= 1; total_rows for packed ones); d in {128, 256, 512}; caches [num_blocks, page, 1, d | 64],
  *   16-byte aligned; norm_weight [d] in w_dtype (fp16 / bf16 / fp32); inv_freq [32] fp32.
+ *   total_rows < 2^31 - 4096.
  *   lengths_host: 0, or row_start, act_q and act_k are host memory, read within the call (at most 18
  *   sequences: they travel as kernel arguments, and become part of a graph that captures the call).
  */

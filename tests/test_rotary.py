@@ -155,3 +155,17 @@ def test_row_positions_refuses():
                        ((p, 1, -1, p, None), "shape")):
         assert lib.dsa_row_positions(*args) == _lib.DSA_ERR_INVALID and what in lib.dsa_last_error().decode()
     assert lib.dsa_row_positions(p, 1, 0, p, None) == 0   # no rows: no launch
+
+
+def test_more_rows_than_a_call_takes():
+    """Refused before any launch: the last groups' row numbers would overflow."""
+    wide = torch.empty(1, 1, 1, 2, dtype=BF).expand(1, 2 ** 31 - 4096, 1, 2)
+    pos = torch.empty(1, 1, dtype=torch.int32).expand(1, 2 ** 31 - 4096)
+    with pytest.raises(ValueError, match="more than 2147479551 tokens"):
+        dsa.rotary_embedding(wide, pos, torch.ones(1))
+    lib, p = _lib.load(), ctypes.c_void_p(16)
+    for rows in (2 ** 31 - 4096, 2 ** 31 - 1):
+        assert lib.dsa_rotary(p, 0, 64, 64, 1, p, 0, 1, None, p, rows, rows, 2, 64, 0, 64, 1, 0, p, None) == _lib.DSA_ERR_UNSUPPORTED
+        assert b"rows" in lib.dsa_last_error()
+        lat = [p, 0, 512, p, 0, 64, 1, 512, None, 1, 1e-6, None, 0, 1, None, p, 1, p, p, p, 0, p, 2, rows, 4, 3, 16, 8, p, p, None]
+        assert lib.dsa_latent_append(*lat) == _lib.DSA_ERR_UNSUPPORTED and b"rows" in lib.dsa_last_error()

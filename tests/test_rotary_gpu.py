@@ -503,3 +503,28 @@ def test_prefill_makes_its_positions_without_waiting():
     assert not before.query()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_rotary_of_more_rows_than_one_grid_dimension():
+    """2^24 work-groups and more (rows of one each): 2^32 threads would not fit a launch's x."""
+    rows = 2 ** 24 + 13
+    x = torch.randn(1, 130, 2, generator=torch.Generator().manual_seed(22)).bfloat16().cuda().expand(rows, 130, 2)
+    pos = (torch.arange(rows, dtype=torch.int32) % 7).cuda()
+    y = dsa.rotary_embedding(x, pos, freqs(1), layout="TND")
+    near(y[:7], turned(x[:7], pos[:7], freqs(1), None, 0, True), 6e-6)
+    assert rows % 7 == 0 and bool((y.view(-1, 7, 130, 2) == y[:7]).all())
+
+
+def test_append_of_more_tokens_than_one_grid_dimension():
+    """2^24 work-groups of eight tokens and more; all but the first and the last tokens have no block."""
+    T, page = 2 ** 27 + 9, 2 ** 20
+    key = torch.randn(1, 1, 64, generator=torch.Generator().manual_seed(23)).half().cuda().expand(T, 1, 64)
+    cache = torch.zeros(2, page, 1, 64, dtype=torch.half, device="cuda")
+    table = torch.full((1, 129), -1, dtype=torch.int32)
+    table[0, 0], table[0, 128] = 1, 0
+    f = freqs(32)
+    dsa.index_cache_append(key, cache, table.cuda(), f, [T], [T], layout="TND")
+    for block, pos in ((1, torch.arange(page)), (0, torch.arange(2 ** 27, T))):
+        # (the 64-bit angle of a position below 2^27 is good to 2^27 2^-52 = 3e-8: inside the bound)
+        near(cache[block, :len(pos)], turned(key[:len(pos)], pos, f, None, 0, False), 6e-6)
+        assert not cache[block, len(pos):].any()
