@@ -668,6 +668,8 @@ int dsa_prefix_attn(const void* query, const void* query_rope, const void* key, 
     return fail(DSA_ERR_INVALID, "dsa_prefix_attn: prefix or max_kv past the %lld tokens of a block-table row", (long long)s2);
   if (s2 > INT_MAX - 4096 || num_blocks > INT_MAX / page_block_size || (int64_t)total_rows * n1 > INT_MAX - 4096)
     return fail(DSA_ERR_UNSUPPORTED, "dsa_prefix_attn: 2^31 tokens, cache rows or head rows");
+  // (the join has a work-group of 256 threads for 32 head rows, and a launch fewer than 2^32 threads)
+  if ((int64_t)total_rows * n1 > (1 << 29) - 32) return fail(DSA_ERR_UNSUPPORTED, "dsa_prefix_attn: 2^29 head rows");
   if ((((uintptr_t)query | (uintptr_t)query_rope | (uintptr_t)key | (uintptr_t)key_rope | (uintptr_t)out) & 15) != 0)
     return fail(DSA_ERR_INVALID, "dsa_prefix_attn: tensors must be 16-byte aligned");
   if ((sm_max == nullptr) != (sm_sum == nullptr))

@@ -1286,9 +1286,9 @@ hipError_t launch_prefix_attn(const PrefixArgs& a, hipStream_t s) {
   k.slots = c.slots;
   const int64_t even = (int64_t)a.batch * c.o_tiles, through = (int64_t)a.total_rows * a.n1 / (32 * c.o_mt) + a.batch;
   k.o_compact = even > through + through / 2;
-  k.o_items = (int)(k.o_compact ? through : even);
-  const int64_t all = (int64_t)c.p_splits * c.p_tiles + (int64_t)k.o_items * c.o_splits;
-  if (all > INT_MAX - 16) return hipErrorInvalidConfiguration;
+  const int64_t own = k.o_compact ? through : even, all = (int64_t)c.p_splits * c.p_tiles + own * c.o_splits;
+  if (all >= (1 << 24) - 8) return hipErrorInvalidConfiguration;   // 2^32 threads, before anything is launched
+  k.o_items = (int)own;
   k.per_xcd = (int)((all + 7) / 8);
   k.o_by_range = c.p_splits == 0 && c.o_splits >= 8;
   return a.io == DSA_DTYPE_BF16 ? launch_io<IO_BF16>(k, a.d, s) : launch_io<IO_F16>(k, a.d, s);

@@ -456,7 +456,7 @@ size_t dsa_prefix_attn_workspace_bytes(int batch, int total_rows, int n1, int d,
  * least) and may get NaN in all; a row that does not see it is not affected.
  *   query [total_rows, N1, D], query_rope [total_rows, N1, 64], key [num_blocks, page, 1, D], key_rope
  *   [.., 64], fp16 / bf16, 16-byte aligned; N1 a power of two up to 128; D in {128, 256, 512};
- *   num_blocks * page and total_rows * N1 < 2^31.
+ *   num_blocks * page < 2^31, total_rows * N1 <= 2^29 - 32.
  *   max_rows_per_batch: a bound on row_start[b+1] - row_start[b]; max_kv, total_kv: the longest act_k and
  *   the sum of them that the caller expects. They only choose how the work is cut: any act_k gives the same
  *   result to rounding.

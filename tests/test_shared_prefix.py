@@ -84,3 +84,10 @@ def test_packed_without_lengths_is_one_sequence():
     for change, message in ((dict(), "block_table"), (dict(block_table=Z(1, 4, dtype=torch.int32), actual_seq_lengths_kv=[40]), "GPU")):
         with pytest.raises(ValueError, match=message):
             dsa.shared_prefix_attention(**{**a, **change})
+
+
+def test_c_entry_refuses_more_head_rows_than_a_launch_holds():
+    lib, p = _lib.load(), ctypes.c_void_p(16)
+    for rows in ((1 << 25) - 1, 1 << 25, 1 << 26):
+        a = [p, p, p, p, 1, p, 64, 16, 8, p, p, p, 2, rows, 16, 512, 64, 32, 2, 1000, 1600, 3, 0.04, p, None, None, p, 1 << 60, 2, None]
+        assert lib.dsa_prefix_attn(*a) == _lib.DSA_ERR_UNSUPPORTED and b"2^29" in lib.dsa_last_error()
