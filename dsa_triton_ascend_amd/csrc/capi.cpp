@@ -679,14 +679,15 @@ int dsa_prefix_attn(const void* query, const void* query_rope, const void* key, 
     g_err[0] = 0;
     return DSA_OK;
   }
-  const size_t need = prefix_attn_workspace_bytes(batch, total_rows, n1, d, prefix, max_rows_per_batch, max_kv, total_kv, kv_splits);
-  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0))
-    return fail(DSA_ERR_INVALID, "dsa_prefix_attn: a 16-byte aligned workspace of %zu bytes required, %zu given", need,
-                workspace ? workspace_bytes : (size_t)0);
   PrefixArgs a{query, query_rope, key, key_rope, io_dtype, block_table, max_blocks, page_block_size, num_blocks, row_start,
                act_q, act_k, batch, total_rows, n1, d, prefix, max_rows_per_batch, max_kv, total_kv, sparse_mode, scale, out, sm_max,
-               sm_sum, workspace, kv_splits};
-  return hip_status(launch_prefix_attn(a, (hipStream_t)stream), "dsa_prefix_attn launch");
+               sm_sum, workspace, workspace_bytes, kv_splits};
+  size_t lacking = 0;
+  const hipError_t e = launch_prefix_attn(a, &lacking, (hipStream_t)stream);
+  if (lacking > 0)
+    return fail(DSA_ERR_INVALID, "dsa_prefix_attn: a 16-byte aligned workspace of %zu bytes required, %zu given", lacking,
+                workspace ? workspace_bytes : (size_t)0);
+  return hip_status(e, "dsa_prefix_attn launch");
 }
 
 }  // extern "C"

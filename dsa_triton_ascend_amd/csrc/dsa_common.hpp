@@ -517,8 +517,9 @@ struct PrefixArgs {
   const int32_t* table; int max_blocks, page; int64_t blocks;
   const int32_t* row_start; const int32_t* act_q; const int32_t* act_k;
   int batch, total_rows, n1, d, prefix, max_rows, max_kv; int64_t total_kv; int sparse_mode; float scale;
-  void* out; float* sm_max; float* sm_sum; void* ws; int kv_splits;
+  void* out; float* sm_max; float* sm_sum; void* ws; size_t ws_bytes; int kv_splits;
 };
 size_t prefix_attn_workspace_bytes(int batch, int rows, int n1, int d, int prefix, int max_rows, int max_kv, int64_t total_kv,
                                    int kv_splits);
-hipError_t launch_prefix_attn(const PrefixArgs& a, hipStream_t s);
+// *lacking: 0, or (nothing is launched) the bytes of a workspace that the call needs and has not
+hipError_t launch_prefix_attn(const PrefixArgs& a, size_t* lacking, hipStream_t s);

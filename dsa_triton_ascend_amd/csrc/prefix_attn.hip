@@ -1226,6 +1226,11 @@ size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 int prefix_blocks(const Cut& c) { return c.p_tiles * c.p_mt; }
 int own_blocks(int batch, int64_t m) { return (int)(m / 32) + batch + 1; }
 size_t block_bytes(int d) { return (size_t)32 * d * sizeof(float); }
+size_t workspace_bytes(const Cut& c, int batch, size_t m, int d) {
+  if (c.slots == 1) return 0;
+  return align256(m * c.slots * sizeof(float4)) +
+         ((size_t)c.p_splits * prefix_blocks(c) + (size_t)c.o_splits * own_blocks(batch, m)) * block_bytes(d);
+}
 }  // namespace
 }  // namespace dsa
 
@@ -1233,15 +1238,15 @@ using namespace dsa;
 
 size_t prefix_attn_workspace_bytes(int batch, int rows, int n1, int d, int prefix, int max_rows, int max_kv, int64_t total_kv,
                                    int kv_splits) {
-  const Cut c = make_cut(batch, rows, n1, d, prefix, max_rows, max_kv, total_kv, kv_splits);
-  if (c.slots == 1) return 0;
-  const size_t m = (size_t)rows * n1;
-  return align256(m * c.slots * sizeof(float4)) +
-         ((size_t)c.p_splits * prefix_blocks(c) + (size_t)c.o_splits * own_blocks(batch, m)) * block_bytes(d);
+  return workspace_bytes(make_cut(batch, rows, n1, d, prefix, max_rows, max_kv, total_kv, kv_splits), batch, (size_t)rows * n1, d);
 }
 
-hipError_t launch_prefix_attn(const PrefixArgs& a, hipStream_t s) {
+// (the search for the cut takes 1 to 4 us, so that a call makes one: it checks the workspace too)
+hipError_t launch_prefix_attn(const PrefixArgs& a, size_t* lacking, hipStream_t s) {
   const Cut c = make_cut(a.batch, a.total_rows, a.n1, a.d, a.prefix, a.max_rows, a.max_kv, a.total_kv, a.kv_splits);
+  const size_t need = workspace_bytes(c, a.batch, (size_t)a.total_rows * a.n1, a.d);
+  *lacking = need > 0 && (!a.ws || a.ws_bytes < need || ((uintptr_t)a.ws & 15) != 0) ? need : 0;
+  if (*lacking) return hipSuccess;
   PfxK k{};
   k.q = (const uint16_t*)a.q;
   k.qr = (const uint16_t*)a.qr;
