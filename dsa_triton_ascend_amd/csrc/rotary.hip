@@ -491,17 +491,13 @@ __global__ __launch_bounds__(TPB) void append_kernel(AppendK a, Lens lens) {
   __syncthreads();
   for (int v0 = 0; v0 < nvec; v0 += VPP) {
     const int v = v0 + vi;
-    const bool more = v0 + VPP < nvec;
-    float nx[8];
-    if (more) load_a(v + VPP, nx);
     const int tok = min(heads == 1 ? v : v / heads, NTOK - 1), h = v - tok * heads;
     norm_vec<LPV>(a.norm, nw, nb, a.a.width, li, x);
     if (!LATENT) rotate_vec<LPV>(tab + tok * half, a.start, a.rdim, a.inter, li, x);
     if (v < nvec && 8 * li < a.a.width && s_row[tok] >= 0)
       store_vec<IO, 8>(reinterpret_cast<uint16_t*>(a.a.cache) + (s_row[tok] * heads + h) * a.a.width + 8 * li, x);
-    if (more)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = nx[i];
+    // (requesting it before this pass's norm and store took longer: 16 x 32 heads of 128 17.9 us instead of 17.1)
+    if (v0 + VPP < nvec) load_a(v + VPP, x);
   }
   if (bwave) {
     rotate_vec<8>(tab + bt * half, 0, a.rdim, a.inter, bl, xb);
