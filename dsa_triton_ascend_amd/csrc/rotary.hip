@@ -120,8 +120,7 @@ struct RotaryK {
 // the two groups of V elements whose pairs are half the rotary width apart. V = 1: any alignment
 // and any even rotary width (INTER: the two elements of a pair).
 // A work-group takes `group` whole rows where a row has fewer units than threads, else
-// UPT * TPB units of one row; UPT = 4 keeps 64 bytes in flight per thread where there is much to
-// move (8192 rows of 128 heads: 52.7 us, 5.1 TB/s), UPT = 1 spreads small calls over more CUs.
+// UPT * TPB units of one row (8192 rows of 128 heads of 64, bf16: 50.7 us a call, 5.3 TB/s).
 template <int IO, int V, bool INTER, int UPT>
 __global__ __launch_bounds__(TPB) void rotary_kernel(RotaryK a) {
   using T = typename Elem<IO>::T;
@@ -229,12 +228,20 @@ hipError_t launch_rotary_v(RotaryK k, hipStream_t s) {
   const int upr = k.heads * k.uph;
   k.group = upr >= TPB ? 1 : TPB / upr;
   const size_t lds = (size_t)k.group * half * sizeof(float2);
-  // enough work-groups of four units a thread to fill the chip twice over
-  const bool many = upr >= 4 * TPB && (int64_t)k.rows * upr >= (int64_t)4 * TPB * 4096;
-  const int per = TPB * (many ? 4 : 1);
-  const dim3 grid = grid_of(((int64_t)k.rows + k.group - 1) / k.group, upr >= TPB ? (upr + per - 1) / per : 1);
-  if (many) hipLaunchKernelGGL((rotary_kernel<IO, V, INTER, 4>), grid, dim3(TPB), lds, s, k);
-  else hipLaunchKernelGGL((rotary_kernel<IO, V, INTER, 1>), grid, dim3(TPB), lds, s, k);
+  const int64_t groups = ((int64_t)k.rows + k.group - 1) / k.group;
+  // Four units a thread, 64 bytes in flight each, for 2^24 units or more of 16-bit neighbours (bf16, inputs from HBM,
+  // one unit's time first): rows of 128 heads of 64, 16,384: 103 -> 101 us, 32,768: 197 -> 190; of 128, 8192: 103.4 ->
+  // 102.4, 32,768: 395 -> 375. Below that they lose (4096 rows of 64: 28.5 -> 29.7), and so they do with pairs half a
+  // width apart (16,384: 101 -> 104) and in fp32 (16,384: 194 -> 201).
+  if constexpr (INTER && V == 8) {
+    if (upr >= 4 * TPB && (int64_t)k.rows * upr >= 1 << 24) {
+      const dim3 grid = grid_of(groups, (upr + 4 * TPB - 1) / (4 * TPB));
+      hipLaunchKernelGGL((rotary_kernel<IO, V, INTER, 4>), grid, dim3(TPB), lds, s, k);
+      return hipGetLastError();
+    }
+  }
+  const dim3 grid = grid_of(groups, upr >= TPB ? (upr + TPB - 1) / TPB : 1);
+  hipLaunchKernelGGL((rotary_kernel<IO, V, INTER, 1>), grid, dim3(TPB), lds, s, k);
   return hipGetLastError();
 }
 
@@ -266,8 +273,10 @@ __global__ __launch_bounds__(TPB) void row_positions_kernel(const int32_t* row_s
 // elements to a vector. A decode step's few tokens wait for a chain of memory accesses: so the vectors,
 // the norm's weights, the frequencies and the lengths (of the sequence that evenly split ones give) are
 // all requested first, and only the block table is left behind them.
-// Tokens a work-group: 4 up to this many (64 latents take 4.7 us, with 8 tokens 0.9 more), else 8 (6926 tokens of two
-// heads of 128: 7.2 us, with 4 tokens 1.1 more; 18,216 latents 12.3, 3.4 TB/s, with 16 tokens 0.4 more)
+// Tokens a work-group: 4 up to this many, else 8. Launches of a replayed graph, four sequences, us with 4 / 8 tokens,
+// latents of 512, of 128, and keys of two heads of 128: 256 tokens 4.3 / 4.9, 4.0 / 4.1, 5.4 / 5.6; 2048: 4.6 / 5.2,
+// 4.3 / 4.2, 5.8 / 5.7; 4096: 5.1 / 5.7, 4.5 / 4.4, 6.6 / 6.1; 6926: 6.5 / 6.7, 5.3 / 4.8, 8.2 / 7.1; 18,216: 13.5 /
+// 12.4, 10.2 / 7.6, 17.0 / 11.8. (One border for all: latents of 512 have theirs near 8000, the others near 1500.)
 constexpr int APPEND_FEW = 2048;
 
 // The lengths of a call, [row_start | act_q | act_k], from device memory or as a kernel argument (a one-shot

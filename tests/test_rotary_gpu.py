@@ -528,3 +528,20 @@ def test_append_of_more_tokens_than_one_grid_dimension():
         # (the 64-bit angle of a position below 2^27 is good to 2^27 2^-52 = 3e-8: inside the bound)
         near(cache[block, :len(pos)], turned(key[:len(pos)], pos, f, None, 0, False), 6e-6)
         assert not cache[block, len(pos):].any()
+
+
+@pytest.mark.parametrize("heads,width,start", [(128, 64, 0), (131, 72, 8)])
+def test_rotary_of_many_units(heads, width, start):
+    """2^24 units of 16 bytes and more (four a thread), whole rows of work-groups and ragged ones, both directions."""
+    rows = 2 ** 24 // (heads * (width // 8)) + 3
+    x = torch.randn(rows, heads, width, device="cuda", generator=torch.Generator("cuda").manual_seed(24)).bfloat16()
+    pos, f = torch.arange(rows).cuda() * 7, freqs(32)
+    pick = torch.cat([torch.arange(40), torch.randint(0, rows, (200,), generator=torch.Generator().manual_seed(25)),
+                      torch.arange(rows - 40, rows)])
+    for fn, back in ((dsa.rotary_embedding, False), (dsa.rotary_embedding_grad, True)):
+        y = fn(x, pos, f, rotary_start=start, layout="TND")
+        near(y[pick.cuda()], turned(x[pick.cuda()], pos[pick.cuda()], f, None, start, True, back), 6e-6)
+        assert torch.equal(y[..., :start], x[..., :start]) and torch.equal(y[..., start + 64:], x[..., start + 64:])
+        few = torch.cat([fn(p, q, f, rotary_start=start, layout="TND") for p, q in zip(x.split(2000), pos.split(2000))])
+        # the small calls' roundings may differ: at most a step of the value, and 32-bit errors of both
+        assert bool(((y.float() - few.float()).abs() <= 2.0 ** -7 * few.float().abs() + 1.2e-5).all())
