@@ -1201,8 +1201,13 @@ hipError_t launch_io(const PfxK& k, int d, hipStream_t s) {
   const int64_t items = 8 * (int64_t)k.per_xcd;
   const int64_t m = (int64_t)k.rows * k.n1;
   const unsigned blocks = (unsigned)((m + 31) / 32);
-  // few rows: eight waves share a row group's ranges (a work-group a group of 8 columns)
-  const bool wide = k.slots > 8 && blocks <= 16;
+  // Few rows: eight waves share a row group's ranges (a work-group a group of 8 columns), up to three such work-groups a
+  // CU. Calls of 16 heads, us with one / eight waves a range group: D = 512, 4 sequences, 17 ranges 20.8 / 19.2, 129: 49.7
+  // / 32; 16 sequences, 10: 18.4 / 18.3, 104: 56.3 / 48.6; 24 (768 work-groups), 12: 22.9 / 23.2, 70: 58.0 / 55.7; 32: 12:
+  // 24.0 / 26.1, 33: 38.5 / 41.9. D = 128, 32, 23: 17.5 / 15.3; 64 (512), 12: 15.7 / 15.6, 25: 28.8 / 27.4; 128, 17: 39.6
+  // / 41.7. Up to eight ranges it makes no difference with few rows (4 sequences, 7: 18.0 / 17.8) and costs with more
+  // (24, 5: 17.9 / 19.4).
+  const bool wide = k.slots > 8 && blocks * (d / 8) <= 768;
 #define DSA_PFX(DD)                                                                                               \
   hipLaunchKernelGGL((prefix_attn_kernel<IO, DD>), dim3((unsigned)items), dim3(NWV * 64), 0, s, k);                \
   if (k.slots > 1 && wide)                                                                                         \
@@ -1290,6 +1295,9 @@ hipError_t launch_prefix_attn(const PrefixArgs& a, size_t* lacking, hipStream_t 
   k.o_base = c.o_base;
   k.slots = c.slots;
   const int64_t even = (int64_t)a.batch * c.o_tiles, through = (int64_t)a.total_rows * a.n1 / (32 * c.o_mt) + a.batch;
+  // Numbering through costs a search, and items that are not there cost a work-group each. One prompt and up to 64 of an
+  // eighth of it (16 heads, D = 512), us without / with it: 1.45 times the items 22.8 / 23.0, 1.7: 37.7 / 36.7, 2.9: 28.9 /
+  // 27.5, 4.8: 74 / 39, 5.9: 215 / 58.
   k.o_compact = even > through + through / 2;
   const int64_t own = k.o_compact ? through : even, all = (int64_t)c.p_splits * c.p_tiles + own * c.o_splits;
   if (all >= (1 << 24) - 8) return hipErrorInvalidConfiguration;   // 2^32 threads, before anything is launched
