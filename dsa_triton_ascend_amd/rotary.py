@@ -122,9 +122,10 @@ def rotary_embedding(x, positions, inv_freq, sections=None, rotary_start=0, inte
     x [B,S,N,D] (BSND) or [T,N,D] (TND), fp16 / bf16 / fp32, any strides; positions int32 / int64
     [B,S] / [T]; inv_freq fp32, one inverse frequency a pair. Pair i is elements (2i, 2i+1) with
     `interleaved`, else (i, i + rotary_dim/2). With `sections` (1 to 4 counts of pairs) positions are
-    [axes, B, S] / [axes, T], and each run of pairs turns by the position on its own axis: the time,
-    height and width of an image's or video's tokens. Angles are computed in 64 bits. Returns a new
-    contiguous tensor, which autograd does not follow: :func:`rotary_embedding_grad` is the gradient."""
+    [axes, B, S] / [axes, T], and each run of consecutive pairs turns by the position on its own axis: the
+    time, height and width of an image's or video's tokens (not axes dealt out pair by pair). Angles are
+    computed in 64 bits. Returns a new contiguous tensor, which autograd does not follow:
+    :func:`rotary_embedding_grad` is the gradient."""
     return _Rotation(x, positions, inv_freq, sections, rotary_start, interleaved, layout, 0, "x").run()
 
 

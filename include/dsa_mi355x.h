@@ -379,7 +379,8 @@ int dsa_dense_li_grad_kl_loss(const void* query, const void* key, const void* qu
  *     (the last dimension contiguous), fp16 / bf16 / fp32, any alignment; out: the same type,
  *     contiguous, not overlapping x. One rounding, from 32 bits.
  *   positions: [axes, rows] int32, or int64 if positions_64; 1 <= axes <= 4. sections (host memory,
- *     [axes], NULL with one axis): axis a has the next sections[a] pairs; they add up to rotary_dim / 2.
+ *     [axes], NULL with one axis): axis a has the next sections[a] pairs (axes that alternate pair by pair cannot
+ *     be expressed); they add up to rotary_dim / 2.
  *   inv_freq [rotary_dim / 2] fp32. rotary_dim even, at most 1024; width <= 4096; heads * width <= 2^20;
  *   rows < 2^31 - 4096.
  */
@@ -453,13 +454,15 @@ size_t dsa_prefix_attn_workspace_bytes(int batch, int total_rows, int n1, int d,
  *   sm_sum = sum exp(score - sm_max)   (both or neither may be NULL)
  * Rows with s1 >= act_q[b], that see no token, or behind the last batch get out = 0, sm = 0. A row that
  * sees a latent with values that are not finite gets NaN where the formula does (in those columns at
- * least) and may get NaN in all; a row that does not see it is not affected.
+ * least) and may get NaN in all; a row that does not see it is not affected. Where a score is NaN, sm_sum is NaN;
+ * sm_max need not be.
  *   query [total_rows, N1, D], query_rope [total_rows, N1, 64], key [num_blocks, page, 1, D], key_rope
  *   [.., 64], fp16 / bf16, 16-byte aligned; N1 a power of two up to 128; D in {128, 256, 512};
  *   num_blocks * page < 2^31, total_rows * N1 <= 2^29 - 32.
  *   max_rows_per_batch: a bound on row_start[b+1] - row_start[b]; max_kv, total_kv: the longest act_k and
  *   the sum of them that the caller expects. They only choose how the work is cut: any act_k gives the same
- *   result to rounding.
+ *   result to rounding. Where act_k grows between replays, give the lengths that it will have: the last range of a
+ *   sequence takes all tokens past max_kv, one after another.
  *   kv_splits (<= 64): 0, or how many ranges of tokens the prefix (all tokens, where nothing is shared
  *   among tiles) is cut into. Calls that share a workspace must be ordered.
  */
