@@ -89,9 +89,13 @@ __device__ __forceinline__ void lds_dma16_at(uint64_t sbase, uint32_t voff, uint
                : "memory", "m0", "scc");
 }
 
-// e^TAU is the largest P relative to the reference maximum: finite in the io type (bf16 has fp32's
-// exponents; fp16 ends at e^11.09), so the output is rescaled only when a tile exceeds it
-template <int IO> constexpr float lazy_tau() { return IO == IO_F16 ? 8.f : 40.f; }
+// P = e^(score - reference). The reference moves, and the output is rescaled, only when a tile's P would exceed
+// e^LIMIT, which is finite in the io type (bf16 has fp32's exponents; fp16 ends at e^11.09); it moves to GAP below
+// that tile's maximum. fp16 rounds P below 2^-14 = e^-9.7 to steps of 2^-24: with the gap a weight is off by at most
+// 2^-25 e^-6 of the row's largest, 3e-5 of it for 400,000 tokens together (without one, 60,000 tokens 17.5 below a
+// single one were lost altogether, and with them values of 1.5e-3).
+template <int IO> constexpr float lazy_limit() { return IO == IO_F16 ? 10.5f : 40.f; }
+template <int IO> constexpr float lazy_gap() { return IO == IO_F16 ? 6.f : 0.f; }
 
 template <int D> struct Tile {
   static constexpr int KSN = D / 16;           // 32x32x16 steps of the latent part
@@ -416,7 +420,7 @@ __device__ __forceinline__ void run_item(const PfxK& a, const Item& it, PfxLds<D
     } else if (st == 4) {
       const float mx = max_half_swap(sm_mx) * cpos;
       m_true = max3(m_true, mx, mx);
-      const float m_new = mx > m_used + lazy_tau<IO>() ? mx : m_used;
+      const float m_new = mx > m_used + lazy_limit<IO>() ? mx - lazy_gap<IO>() : m_used;
       alpha = m_used == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_used - m_new) * LOG2E);
       m_used = m_new;
       sm_mb = m_used * LOG2E;
@@ -816,7 +820,7 @@ __device__ __forceinline__ void run_tokens(const PfxK& a, const Item& it, PfxLds
     for (int i = 3; i < 15; i += 2) mx = max3(mx, sv[i], sv[i + 1]);
     mx = max_half_swap(max3(mx, sv[15], sv[15])) * cpos;
     m_true = max3(m_true, mx, mx);
-    const float m_new = mx > m_used + lazy_tau<IO>() ? mx : m_used;
+    const float m_new = mx > m_used + lazy_limit<IO>() ? mx - lazy_gap<IO>() : m_used;
     const float alpha = m_used == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_used - m_new) * LOG2E);
     m_used = m_new;
     const float mb = m_used == -INFINITY ? 0.f : m_used * LOG2E;

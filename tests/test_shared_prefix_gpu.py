@@ -360,3 +360,26 @@ def test_packed_without_lengths_is_one_sequence():
     kw = dict(actual_seq_lengths_kv=[300], query_rope=t["qr"], key_rope=t["kr"], layout_query="TND", return_softmax_lse=True)
     got = dsa.shared_prefix_attention(t["q"], t["k"], t["k"], t["table"], 0, 0.05, **kw)
     check(got, exact(t, [37], [300], 0, 0.05, 3, True))
+
+
+@pytest.mark.parametrize("gap", [10.0, 15.0, 17.5, 20.0])
+@pytest.mark.parametrize("n1", [16, 64, 128])
+def test_small_weights_of_many_tokens(n1, gap):
+    """One token whose score is `gap` above those of 60,000 others: together their weights (4.5e-5 to 2.1e-9 each) are
+    seen in the columns where the one is zero. A weight below fp16's normal numbers is off by half of its smallest
+    step, 2^-25, where the row's largest is e^6 or more: 60,001 of them by 4.4e-6 at most, beside the usual bound."""
+    kv, page = 60001, 512
+    t = make(HF, n1, 128, [1], [kv], 0, page, False, 19)
+    k = t["k"]
+    k.zero_()
+    t["kr"].zero_()
+    t["q"].zero_()
+    t["q"][..., 0] = 1.0
+    k[..., 1:] = 1.0
+    at = 777
+    k[t["table"][0, at // page].long(), at % page, 0, 0] = gap
+    k[t["table"][0, at // page].long(), at % page, 0, 1:] = 0.0
+    for splits in (1, 0):
+        want = list(exact(t, [1], [kv], 0, 1.0, 3, False))
+        want[3] = want[3] + kv * 2.0 ** -25 * math.exp(-6)
+        check(call(t, [1], [kv], 0, 1.0, 3, False, kv_splits=splits), want)
