@@ -545,3 +545,26 @@ def test_rotary_of_many_units(heads, width, start):
         few = torch.cat([fn(p, q, f, rotary_start=start, layout="TND") for p, q in zip(x.split(2000), pos.split(2000))])
         # the small calls' roundings may differ: at most a step of the value, and 32-bit errors of both
         assert bool(((y.float() - few.float()).abs() <= 2.0 ** -7 * few.float().abs() + 1.2e-5).all())
+
+
+def test_prefill_plan_that_rotates_runs_on_another_stream():
+    """A kept PrefillPlan's positions are in place when its constructor returns, however busy the stream it was built on."""
+    g = torch.Generator().manual_seed(26)
+    lens, dt = [90, 0, 40], torch.bfloat16
+    T, cu = sum(lens) + 6, torch.tensor(lens).cumsum(0).tolist()   # six rows behind the last sequence
+    r = lambda *s: torch.randn(*s, generator=g).to(dt).cuda()
+    args = (r(T, 32, 128), r(T, 1, 128), torch.randn(T, 32, generator=g).cuda(), r(T, 16, 512), r(T, 1, 512), r(T, 16, 64),
+            r(T, 1, 64), cu)
+    kw = dict(sparse_count=32, scale_value=0.04, inv_freq=freqs(32))
+    pos = torch.cat([torch.arange(n) for n in lens] + [torch.zeros(6, dtype=torch.long)]).cuda()
+    want = [o.clone() for o in dsa.PrefillPlan(*args, positions=pos, **kw).run()]
+    torch.cuda.synchronize()
+    build, use = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(build):
+        torch.cuda._sleep(40_000_000)
+        plan = dsa.PrefillPlan(*args, **kw)
+    with torch.cuda.stream(use):
+        got = plan.run()
+    torch.cuda.synchronize()
+    n = sum(lens)
+    assert torch.equal(got[0][:n], want[0][:n]) and torch.equal(got[1][:n], want[1][:n])
