@@ -18,11 +18,12 @@
 // An item is one work-group of four waves and 32, 64 or 128 head rows. Tiles of 32 tokens go direct to LDS.
 // S^T = K Q^T has the tokens as M and 32 head rows as N; the online softmax runs in each lane's 16 scores
 // of its head row plus one exchange between lane halves, and its result is already the B operand of
-// O^T += V^T P^T, over all columns. P is rounded to the io type for that product, as the sparse attention's is (the
-// 16-bit products are twice as fast as any with more bits of P): errors against 64 bits are 3 to 25% above those of
-// 32-bit P, half a step of the type relative at most. The sums of P, the scores and O are in 32 bits. With 128 head rows the matrix units are the bound: a wave for each
-// block of 32, the tiles in a ring of three buffers shared by them. With fewer the bytes are, or the
-// latency: the waves split the tokens and join their outputs through LDS at the end.
+// O^T += V^T P^T, over all columns. P is rounded to the io type for that product, as the sparse attention's is (more
+// bits of it would take a second product): the output's errors against 64 bits are 3 to 30% above those of 32-bit P.
+// The sums of P, the scores and O are in 32 bits.
+// With 128 head rows the matrix units are the bound: a wave for each block of 32, the tiles in a ring of three
+// buffers shared by them. With fewer the bytes are, or the latency: the waves split the tokens and join their
+// outputs through LDS at the end.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -1121,8 +1122,9 @@ int up(int x, int to) { return (x + to - 1) / to * to; }
 
 // Microseconds of a call by a simple model of what was measured (256 CUs, one item each at a time): an item
 // costs 6 (its rows' sequences, Q, first tile, ends) and, at D = 512 / 128, per 32 tokens 1.55 / 0.93 for 128
-// head rows (D = 512: 1.4 where few items run, 1.9 with all CUs busy, whose clock is 2.0 GHz then), 0.95 / 0.71 for 64, or per 128 tokens 3.7 / 3.0 for 32 (narrow latents: the tile's chain of loads,
-// softmax and waits, not its products); the latents come at 4.9 TB/s; partial outputs are written at 7 TB/s,
+// head rows (D = 512: 1.4 where few items run, 1.9 with all CUs busy, whose clock is 2.0 GHz then), 0.95 / 0.71
+// for 64, or per 128 tokens 3.7 / 3.0 for 32 (narrow latents: the tile's chain of loads, softmax and waits, not its
+// products); the latents come at 4.9 TB/s; partial outputs are written at 7 TB/s,
 // and the join is a launch of 6 that reads them at 6 TB/s. It is there to weigh rounds of items against
 // partials: at 64 x 16 heads after 8192 tokens 16 prefix ranges take 47 us, 8 take 65 and 32 take 65 as well.
 struct Model {
