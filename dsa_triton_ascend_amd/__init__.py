@@ -16,6 +16,7 @@ Beside them, what a model needs around these paths:
 * :func:`rotary_embedding` / :func:`rotary_embedding_grad` — rotary positions
 * :func:`latent_cache_append`, :func:`index_cache_append` — new tokens into the paged caches
 * :func:`shared_prefix_attention` — dense attention over a paged cache, a common prefix computed once
+* :func:`layer_norm` / :func:`layer_norm_grad` — the norm of an indexer's keys or of hidden rows
 
 All run hand-written gfx950 HIP kernels through the C ABI of
 ``libdsa_mi355x.so`` (include/dsa_mi355x.h); PyTorch tensors are only buffers.
@@ -32,6 +33,7 @@ from .dense_loss import (DenseLightningIndexerGradKLLoss, DenseLightningIndexerS
 from .rotary import (IndexAppendPlan, LatentAppendPlan, RotaryEmbedding, index_cache_append, latent_cache_append,
                      rotary_embedding, rotary_embedding_grad)
 from .shared_prefix import SharedPrefixAttention, SharedPrefixPlan, shared_prefix_attention
+from .layer_norm import LayerNorm, layer_norm, layer_norm_grad
 
 __all__ = ["lightning_indexer", "LightningIndexer", "sparse_flash_attention", "SparseFlashAttention",
            "sparse_flash_attention_grad", "SparseFlashAttentionGrad", "sparse_lightning_indexer_grad_kl_loss",
@@ -42,4 +44,4 @@ __all__ = ["lightning_indexer", "LightningIndexer", "sparse_flash_attention", "S
            "PrefillPlan", "dsa_prefill",
            "rotary_embedding", "rotary_embedding_grad", "RotaryEmbedding", "latent_cache_append", "LatentAppendPlan",
            "index_cache_append", "IndexAppendPlan", "shared_prefix_attention", "SharedPrefixAttention",
-           "SharedPrefixPlan"]
+           "SharedPrefixPlan", "layer_norm", "layer_norm_grad", "LayerNorm"]

@@ -690,4 +690,66 @@ int dsa_prefix_attn(const void* query, const void* query_rope, const void* key, 
   return hip_status(e, "dsa_prefix_attn launch");
 }
 
+namespace {
+int check_norm(const char* fn, const void* x, int64_t row_stride, int dtype, int64_t rows, int width, const void* w, int w_dtype) {
+  if (!x) return fail(DSA_ERR_INVALID, "%s: null pointer argument", fn);
+  if (!is16(dtype) && dtype != DSA_DTYPE_F32) return fail(DSA_ERR_INVALID, "%s: dtype must be fp16, bf16 or fp32", fn);
+  if (w && !is16(w_dtype) && w_dtype != DSA_DTYPE_F32)
+    return fail(DSA_ERR_INVALID, "%s: norm weights must be fp16, bf16 or fp32", fn);
+  if (rows < 0 || width <= 0) return fail(DSA_ERR_INVALID, "%s: non-positive shape", fn);
+  if (width > DSA_NORM_MAX_WIDTH) return fail(DSA_ERR_UNSUPPORTED, "%s: width %d > %d", fn, width, DSA_NORM_MAX_WIDTH);
+  if (rows > INT64_MAX / 8 / width || row_stride < 0 || (rows > 1 && row_stride > INT64_MAX / 8 / rows))
+    return fail(DSA_ERR_UNSUPPORTED, "%s: rows or strides past 64 bits of bytes", fn);
+  return DSA_OK;
+}
+}  // namespace
+
+int dsa_layer_norm(const void* x, int64_t row_stride, int dtype, int64_t rows, int width, const void* norm_weight,
+                   const void* norm_bias, int w_dtype, float eps, void* y, float* mean, float* rstd, void* stream) {
+  const int st = check_norm("dsa_layer_norm", x, row_stride, dtype, rows, width, norm_weight, w_dtype);
+  if (st != DSA_OK) return st;
+  if (!y) return fail(DSA_ERR_INVALID, "dsa_layer_norm: null pointer argument");
+  if (norm_bias && !norm_weight) return fail(DSA_ERR_INVALID, "dsa_layer_norm: norm_bias without norm_weight");
+  if ((mean == nullptr) != (rstd == nullptr))
+    return fail(DSA_ERR_INVALID, "dsa_layer_norm: mean and rstd must both be given or both NULL");
+  if (rows == 0) {
+    g_err[0] = 0;
+    return DSA_OK;
+  }
+  NormArgs a{};
+  a.x = x, a.x_stride = row_stride, a.io = dtype, a.rows = rows, a.width = width, a.w = norm_weight, a.b = norm_bias;
+  a.wdt = w_dtype, a.eps = eps, a.y = y, a.mean = mean, a.rstd = rstd;
+  return hip_status(launch_layer_norm(a, (hipStream_t)stream), "dsa_layer_norm launch");
+}
+
+size_t dsa_layer_norm_grad_workspace_bytes(int64_t rows, int width) {
+  if (rows <= 0 || width <= 0 || width > DSA_NORM_MAX_WIDTH) return 0;
+  return layer_norm_grad_workspace_bytes(rows, width);
+}
+
+int dsa_layer_norm_grad(const void* d_out, int64_t d_row_stride, const void* x, int64_t row_stride, int dtype, int64_t rows,
+                        int width, const float* mean, const float* rstd, const void* norm_weight, int w_dtype, void* d_x,
+                        void* d_weight, void* d_bias, void* workspace, size_t workspace_bytes, void* stream) {
+  int st = check_norm("dsa_layer_norm_grad", x, row_stride, dtype, rows, width, norm_weight, w_dtype);
+  if (st != DSA_OK) return st;
+  st = check_norm("dsa_layer_norm_grad", d_out, d_row_stride, dtype, rows, width, norm_weight, w_dtype);
+  if (st != DSA_OK) return st;
+  if (!mean || !rstd || !d_x) return fail(DSA_ERR_INVALID, "dsa_layer_norm_grad: null pointer argument");
+  if ((d_weight || d_bias) && !norm_weight)
+    return fail(DSA_ERR_INVALID, "dsa_layer_norm_grad: d_weight or d_bias without norm_weight");
+  const size_t need = d_weight || d_bias ? dsa_layer_norm_grad_workspace_bytes(rows, width) : 0;
+  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0))
+    return fail(DSA_ERR_INVALID, "dsa_layer_norm_grad: a 16-byte aligned workspace of %zu bytes required, %zu given", need,
+                workspace ? workspace_bytes : (size_t)0);
+  if (rows == 0 && !d_weight && !d_bias) {
+    g_err[0] = 0;
+    return DSA_OK;
+  }
+  NormArgs a{};
+  a.x = x, a.x_stride = row_stride, a.io = dtype, a.rows = rows, a.width = width, a.w = norm_weight, a.wdt = w_dtype;
+  a.y = d_x, a.mean = const_cast<float*>(mean), a.rstd = const_cast<float*>(rstd), a.d = d_out, a.d_stride = d_row_stride;
+  a.dw = d_weight, a.db = d_bias, a.part = (float*)workspace;
+  return hip_status(launch_layer_norm_grad(a, (hipStream_t)stream), "dsa_layer_norm_grad launch");
+}
+
 }  // extern "C"

@@ -523,3 +523,14 @@ size_t prefix_attn_workspace_bytes(int batch, int rows, int n1, int d, int prefi
                                    int kv_splits);
 // *lacking: 0, or (nothing is launched) the bytes of a workspace that the call needs and has not
 hipError_t launch_prefix_attn(const PrefixArgs& a, size_t* lacking, hipStream_t s);
+// Layer norm over the last dimension; rows by strides (elements), y, dx contiguous
+struct NormArgs {
+  const void* x; int64_t x_stride; int io; int64_t rows; int width;
+  const void* w; const void* b; int wdt; float eps;
+  void* y;                      // gradient: dx
+  float* mean; float* rstd;     // forward: NULL or outputs
+  const void* d; int64_t d_stride; void* dw; void* db; float* part;   // gradient
+};
+hipError_t launch_layer_norm(const NormArgs& a, hipStream_t s);
+size_t layer_norm_grad_workspace_bytes(int64_t rows, int width);
+hipError_t launch_layer_norm_grad(const NormArgs& a, hipStream_t s);

@@ -13,7 +13,7 @@
 #include <algorithm>
 #include <cstring>
 
-#include "dsa_common.hpp"
+#include "elements.hpp"
 
 namespace dsa {
 namespace {
@@ -67,40 +67,6 @@ __device__ __forceinline__ float2 cos_sin(int64_t pos, float freq) {
   float s, c;
   sincospif(2.f * (float)turns, &s, &c);
   return make_float2(c, s);
-}
-
-// ------------------------------------------------------------------ element types
-template <int IO> struct Elem { using T = uint16_t; static constexpr int V = 8; };
-template <> struct Elem<DSA_DTYPE_F32> { using T = float; static constexpr int V = 4; };
-
-template <int IO, int V>
-__device__ __forceinline__ void load_vec(const typename Elem<IO>::T* p, float (&x)[V]) {
-  if constexpr (V == 1) {
-    if constexpr (IO == DSA_DTYPE_F32) x[0] = p[0];
-    else x[0] = to_f32<IO>(p[0]);
-  } else if constexpr (IO == DSA_DTYPE_F32) {
-    const uint4 u = ldg16(p);
-    x[0] = __uint_as_float(u.x), x[1] = __uint_as_float(u.y), x[2] = __uint_as_float(u.z), x[3] = __uint_as_float(u.w);
-  } else {
-    const uint4 u = ldg16(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = to_f32<IO>((uint16_t)(w[i] & 0xFFFFu));
-      x[2 * i + 1] = to_f32<IO>((uint16_t)(w[i] >> 16));
-    }
-  }
-}
-template <int IO, int V>
-__device__ __forceinline__ void store_vec(typename Elem<IO>::T* p, const float (&x)[V]) {
-  if constexpr (V == 1) {
-    if constexpr (IO == DSA_DTYPE_F32) p[0] = x[0];
-    else p[0] = from_f32<IO>(x[0]);
-  } else if constexpr (IO == DSA_DTYPE_F32) {
-    stg16(p, make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])));
-  } else {
-    stg16(p, make_uint4(pack2<IO>(x[0], x[1]), pack2<IO>(x[2], x[3]), pack2<IO>(x[4], x[5]), pack2<IO>(x[6], x[7])));
-  }
 }
 
 // ------------------------------------------------------------------ rotary

@@ -473,6 +473,32 @@ int dsa_prefix_attn(const void* query, const void* query_rope, const void* key, 
                     float scale, void* out, float* sm_max, float* sm_sum, void* workspace, size_t workspace_bytes,
                     int kv_splits, void* stream);
 
+#define DSA_NORM_MAX_WIDTH 16384
+
+/*
+ * Layer norm of each row of x (no counterpart in the reference):
+ *   mean = sum x / width, rstd = 1 / sqrt(sum (x - mean)^2 / width + eps), y = (x - mean) rstd norm_weight + norm_bias
+ *   x [rows, width], row_stride elements between rows (any alignment; 16-byte borders are read faster), fp16 /
+ *   bf16 / fp32; y [rows, width] contiguous, not overlapping x; norm_weight, norm_bias [width] in w_dtype (fp16 / bf16 /
+ *   fp32), both or the bias NULL; mean, rstd [rows] fp32, both or neither NULL. Statistics in 32 bits, one
+ *   rounding. width <= DSA_NORM_MAX_WIDTH.
+ */
+int dsa_layer_norm(const void* x, int64_t row_stride, int dtype, int64_t rows, int width, const void* norm_weight,
+                   const void* norm_bias, int w_dtype, float eps, void* y, float* mean, float* rstd, void* stream);
+
+/*
+ * Its gradients: with h = (x - mean) rstd, g = d_out norm_weight,
+ *   d_x = (g - sum g / width - h sum(g h) / width) rstd, d_weight = sum over rows of d_out h, d_bias = sum of d_out
+ *   mean, rstd as the forward left them; d_out rows by d_row_stride; d_x contiguous, in dtype; d_weight, d_bias
+ *   [width] in w_dtype, each NULL if not wanted (both without norm_weight); with no rows they are zeros. The sums
+ *   over rows have a fixed order. workspace: dsa_layer_norm_grad_workspace_bytes, 16-byte aligned, needs no
+ *   initialisation (not read without d_weight and d_bias). Calls that share a workspace must be ordered.
+ */
+size_t dsa_layer_norm_grad_workspace_bytes(int64_t rows, int width);
+int dsa_layer_norm_grad(const void* d_out, int64_t d_row_stride, const void* x, int64_t row_stride, int dtype, int64_t rows,
+                        int width, const float* mean, const float* rstd, const void* norm_weight, int w_dtype, void* d_x,
+                        void* d_weight, void* d_bias, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
