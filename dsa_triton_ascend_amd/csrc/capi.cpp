@@ -752,4 +752,79 @@ int dsa_layer_norm_grad(const void* d_out, int64_t d_row_stride, const void* x, 
   return hip_status(launch_layer_norm_grad(a, (hipStream_t)stream), "dsa_layer_norm_grad launch");
 }
 
+namespace {
+int check_dense(const char* fn, const DenseArgs& a) {
+  const bool rope = a.dr > 0;
+  if (!a.q.p || !a.k.p || !a.v.p || (rope && (!a.qr.p || !a.kr.p)) || !a.row_start || !a.key_start || !a.act_q || !a.act_k)
+    return fail(DSA_ERR_INVALID, "%s: null pointer argument", fn);
+  if (!is16(a.io)) return fail(DSA_ERR_INVALID, "%s: io_dtype must be fp16 or bf16", fn);
+  if (a.sparse_mode != 0 && a.sparse_mode != 3)
+    return fail(DSA_ERR_INVALID, "Only sparse_mode 0 (full) / 3 (rightDownCausal) supported");
+  if (a.d != 64 && a.d != 128) return fail(DSA_ERR_INVALID, "D must be one of (64, 128), got %d", a.d);
+  if (a.dr != 0 && (a.dr != 64 || a.d != 128))
+    return fail(DSA_ERR_INVALID, "rope dim must be 0, or 64 beside D = 128, got %d", a.dr);
+  if (a.batch <= 0 || a.total_rows < 0 || a.total_keys < 0 || a.n1 <= 0 || a.n2 <= 0 || a.rows_behind < 0 || a.max_rows < 0 || a.max_kv < 0)
+    return fail(DSA_ERR_INVALID, "%s: non-positive shape", fn);
+  if (a.n1 % a.n2 != 0) return fail(DSA_ERR_INVALID, "%s: N1=%d not divisible by N2=%d", fn, a.n1, a.n2);
+  if (a.rows_behind > a.total_rows || a.max_rows > a.total_rows || a.max_kv > a.total_keys)
+    return fail(DSA_ERR_INVALID, "%s: rows_behind, max_rows or max_kv past the tensors' rows", fn);
+  if (a.stat_padded && a.total_rows % a.batch != 0)
+    return fail(DSA_ERR_INVALID, "%s: padded statistics of rows that do not split evenly", fn);
+  if ((int64_t)a.total_rows * a.n1 >= (1 << 30) || (int64_t)a.total_keys * a.n2 >= (1 << 30) || a.batch > 65535)
+    return fail(DSA_ERR_UNSUPPORTED, "%s: 2^30 head rows, or more than 65535 sequences", fn);
+  for (const DenseTensor* t : {&a.q, &a.qr, &a.k, &a.kr, &a.v}) {
+    if (!rope && (t == &a.qr || t == &a.kr)) continue;
+    if (((uintptr_t)t->p & 15) != 0 || t->row % 8 != 0 || t->head % 8 != 0)
+      return fail(DSA_ERR_INVALID, "%s: rows and heads must begin on 16-byte borders", fn);
+    if (t->row < 0 || t->head < 0 || t->row >= (1 << 24) || t->head >= (1ll << 40))
+      return fail(DSA_ERR_UNSUPPORTED, "%s: row strides of 2^24 elements", fn);
+  }
+  return DSA_OK;
+}
+}  // namespace
+
+size_t dsa_dense_attn_workspace_bytes(int batch, int total_rows, int rows_behind, int n1, int n2, int d, int max_rows, int max_kv,
+                                      int kv_splits) {
+  if (batch <= 0 || total_rows <= 0 || rows_behind < 0 || n1 <= 0 || n2 <= 0 || n1 % n2 != 0 || d <= 0 || max_rows < 0 || max_kv < 0)
+    return 0;
+  DenseArgs a{};
+  a.batch = batch, a.total_rows = total_rows, a.rows_behind = rows_behind, a.n1 = n1, a.n2 = n2, a.d = d;
+  a.max_rows = max_rows, a.max_kv = max_kv, a.kv_splits = kv_splits;
+  return dense_attn_workspace_bytes(a);
+}
+
+int dsa_dense_attn(const void* query, int64_t q_row, int64_t q_head, const void* query_rope, int64_t qr_row, int64_t qr_head,
+                   const void* key, int64_t k_row, int64_t k_head, const void* key_rope, int64_t kr_row, int64_t kr_head,
+                   const void* value, int64_t v_row, int64_t v_head, int io_dtype, const int32_t* row_start,
+                   const int32_t* key_start, const int32_t* act_q, const int32_t* act_k, int batch, int total_rows,
+                   int total_keys, int rows_behind, int n1, int n2, int d, int dr, int max_rows, int max_kv, int sparse_mode,
+                   float scale, void* out, int stat_padded, float* sm_max, float* sm_sum, void* workspace,
+                   size_t workspace_bytes, int kv_splits, void* stream) {
+  DenseArgs a{};
+  a.q = {query, q_row, q_head}, a.qr = {query_rope, qr_row, qr_head}, a.k = {key, k_row, k_head};
+  a.kr = {key_rope, kr_row, kr_head}, a.v = {value, v_row, v_head}, a.io = io_dtype;
+  a.row_start = row_start, a.key_start = key_start, a.act_q = act_q, a.act_k = act_k, a.batch = batch;
+  a.total_rows = total_rows, a.total_keys = total_keys, a.rows_behind = rows_behind, a.n1 = n1, a.n2 = n2, a.d = d, a.dr = dr;
+  a.max_rows = max_rows, a.max_kv = max_kv, a.sparse_mode = sparse_mode, a.scale = scale, a.out = out;
+  a.stat_padded = stat_padded, a.sm_max = sm_max, a.sm_sum = sm_sum, a.ws = workspace, a.ws_bytes = workspace_bytes;
+  a.kv_splits = kv_splits;
+  const int st = check_dense("dsa_dense_attn", a);
+  if (st != DSA_OK) return st;
+  if (!out) return fail(DSA_ERR_INVALID, "dsa_dense_attn: null pointer argument");
+  if (((uintptr_t)out & 15) != 0) return fail(DSA_ERR_INVALID, "dsa_dense_attn: out must be 16-byte aligned");
+  if ((sm_max == nullptr) != (sm_sum == nullptr))
+    return fail(DSA_ERR_INVALID, "dsa_dense_attn: sm_max and sm_sum must both be given or both NULL");
+  if (kv_splits > 64) return fail(DSA_ERR_UNSUPPORTED, "dsa_dense_attn: kv_splits=%d > 64", kv_splits);
+  if (total_rows == 0) {
+    g_err[0] = 0;
+    return DSA_OK;
+  }
+  size_t lacking = 0;
+  const hipError_t e = launch_dense_attn(a, &lacking, (hipStream_t)stream);
+  if (lacking > 0)
+    return fail(DSA_ERR_INVALID, "dsa_dense_attn: a 16-byte aligned workspace of %zu bytes required, %zu given", lacking,
+                workspace ? workspace_bytes : (size_t)0);
+  return hip_status(e, "dsa_dense_attn launch");
+}
+
 }  // extern "C"

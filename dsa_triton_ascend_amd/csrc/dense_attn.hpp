@@ -1,0 +1,169 @@
+// What the dense attention's forward and backward kernels share: sequences and their masks, tiles of keys,
+// values, queries or output gradients in LDS, and the reading of MFMA operands from them.
+#pragma once
+
+#include <climits>
+#include <cmath>
+
+#include "dsa_common.hpp"
+
+namespace dsa {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// A tensor [rows, heads, width] by strides in elements
+struct Rows {
+  const uint16_t* p;
+  int64_t row, head;
+};
+
+// Lengths of a call. Sequence b's query rows begin at row_start[b], its keys at key_start[b]; sequence `batch` is
+// what lies behind the last one, nothing of which is seen.
+struct Lens {
+  const int32_t* row_start;
+  const int32_t* key_start;
+  const int32_t* act_q;
+  const int32_t* act_k;
+  int batch, rows, keys, mode;   // rows, keys: of the tensors
+};
+struct Seq {
+  int r0, rows;   // first query row, rows that belong to it (act_q of them are queries)
+  int k0, keys;
+  int aq, ak;
+};
+__device__ __forceinline__ Seq seq_of(const Lens& l, int b) {
+  Seq q;
+  q.r0 = l.row_start[b];
+  q.k0 = l.key_start[b];
+  const bool tail = b >= l.batch;
+  q.rows = (tail ? l.rows : l.row_start[b + 1]) - q.r0;
+  q.keys = (tail ? l.keys : l.key_start[b + 1]) - q.k0;
+  q.aq = tail ? 0 : min(l.act_q[b], q.rows);
+  q.ak = tail ? 0 : min(l.act_k[b], q.keys);
+  return q;
+}
+// how many of its tokens query s of a sequence sees
+__device__ __forceinline__ int limit_of(const Lens& l, const Seq& q, int s) {
+  if (s >= q.aq) return 0;
+  return l.mode == 0 ? q.ak : max(0, q.ak - q.aq + s + 1);
+}
+// the first query that sees token t (aq if none does)
+__device__ __forceinline__ int first_query(const Lens& l, const Seq& q, int t) {
+  if (t >= q.ak) return q.aq;
+  return l.mode == 0 ? 0 : min(q.aq, max(0, t - (q.ak - q.aq)));
+}
+
+// ---------------------------------------------------------------- tiles in LDS
+// Rows of RB = 256 or 128 bytes, unpadded, so that direct-to-LDS loads fill them (a wave's 64 lanes 1 KB in a row). A
+// row's 16-byte chunks are permuted: c lies at c ^ swizzle(row). Operand reads (16 rows, one chunk) and
+// transposed reads (4 rows, 64 bytes) both touch every bank once. Rows of 128 bytes share a line of the banks by twos.
+__host__ __device__ constexpr int line_swz(int l) { return ((l & 1) << 2) | (l & 2) | ((l >> 2) & 1); }
+template <int RB>
+__device__ __forceinline__ constexpr uint32_t tile_off(int t, int c) {
+  if constexpr (RB == 256) return (uint32_t)(t * 256 + ((c ^ kv_swz(t & 15)) << 4));
+  else return (uint32_t)(t * 128 + ((c ^ line_swz((t >> 1) & 7)) << 4));
+}
+
+// One wave's share of the loads of a tile of BN rows by NW waves: CNT loads; load j covers the rows STEP j + first ..
+template <int RB, int BN, int NW> struct Share {
+  static constexpr int RPL = 1024 / RB;          // rows a load
+  static constexpr int STEP = RPL * NW;
+  static constexpr int CNT = BN / STEP;
+  static_assert(BN % STEP == 0 && STEP % 16 == 0, "every load of a wave has the same permutation");
+  int row;        // this lane's row of load 0
+  uint32_t col;   // byte of its chunk in the row
+  __device__ __forceinline__ Share(int wave, int lane) {
+    row = wave * RPL + lane / (RB / 16);
+    const int c = lane & (RB / 16 - 1);
+    col = (uint32_t)((RB == 256 ? c ^ kv_swz(row & 15) : c ^ line_swz((row >> 1) & 7)) << 4);
+  }
+};
+
+// Token order of the S tiles: with row m of the operand at token tk(m), a lane's 16 accumulators of a 32-row tile
+// are tokens 16 (i / 8) + 8 (lane / 32) + i % 8, the order in which the next product takes them as an operand.
+__device__ __forceinline__ int s_row(int m) { return 16 * (m >> 4) + 8 * ((m >> 2) & 1) + 4 * ((m >> 3) & 1) + (m & 3); }
+__device__ __forceinline__ int s_token(int i, int kg) { return 16 * (i >> 3) + 8 * kg + (i & 7); }
+
+// Operand fragment: row t, values 16 ks + 8 kg .. of a tile
+template <int RB>
+__device__ __forceinline__ uint4 op_frag(uint32_t tile, int t, int ks, int kg) {
+  return lds_read16_at(tile + tile_off<RB>(t, 2 * ks + kg));
+}
+// Transposed operand fragment: column 32 n + lane % 32 of the rows t0 + 8 (lane / 32) .. + 7 (t0 a multiple of 16)
+template <int RB>
+__device__ __forceinline__ uint4 tr_frag(uint32_t tile, int t0, int n, int lane) {
+  const int g16 = lane >> 4, c16 = lane & 15;
+  const int t4 = t0 + (g16 >> 1) * 8 + (c16 >> 2), c = 4 * n + (g16 & 1) * 2 + ((c16 & 3) >> 1), o = (c16 & 1) * 8;
+  const uint2 lo = ds_read_tr_at(tile + tile_off<RB>(t4, c) + o), hi = ds_read_tr_at(tile + tile_off<RB>(t4 + 4, c) + o);
+  return make_uint4(lo.x, lo.y, hi.x, hi.y);
+}
+
+// Values that are not finite become zeros in this wave's share of a tile (its loads have landed); returns the rows
+// (bit) that held one.
+template <int IO, int RB, int BN, int NW>
+__device__ __forceinline__ uint64_t clean_share(uint32_t tile, int wave, int lane) {
+  static_assert(BN <= 64, "a bit a row");
+  using Sh = Share<RB, BN, NW>;
+  constexpr uint32_t EXP = IO == IO_BF16 ? 0x7F80u : 0x7C00u;
+  uint64_t bad = 0;
+#pragma unroll 1
+  for (int j = 0; j < Sh::CNT; ++j) {
+    const uint32_t at = tile + (uint32_t)((j * NW + wave) * 1024 + lane * 16);
+    const uint4 v = lds_read16_at(at);
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if ((w[i] & EXP) == EXP) w[i] &= 0xFFFF0000u, any = true;
+      if (((w[i] >> 16) & EXP) == EXP) w[i] &= 0xFFFFu, any = true;
+    }
+    if (any) *(__attribute__((address_space(3))) u32x4v*)(uintptr_t)at = __builtin_bit_cast(u32x4v, make_uint4(w[0], w[1], w[2], w[3]));
+    const uint64_t lanes = __builtin_amdgcn_ballot_w64(any);
+    if (lanes) {
+#pragma unroll
+      for (int r = 0; r < Sh::RPL; ++r)
+        if ((lanes >> (r * (RB / 16))) & ((1ull << (RB / 16)) - 1)) bad |= 1ull << (j * Sh::STEP + wave * Sh::RPL + r);
+    }
+  }
+  return bad;
+}
+
+__device__ __forceinline__ uint4 flipped(uint4 v, uint32_t f) { return make_uint4(v.x ^ f, v.y ^ f, v.z ^ f, v.w ^ f); }
+
+// v_max3 without the quieting of each operand that fmaxf needs (a NaN score reaches the output
+// through its exponential either way)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// The four groups of four accumulators of a 32-column tile, packed, exchanged between lane halves: lanes 0-31
+// then hold columns [0, 8) and [16, 24), the others [8, 16) and [24, 32), each 16 bytes.
+template <int IO>
+__device__ __forceinline__ void pack_tile(const f32x16& v, float f, uint4 (&out)[2]) {
+  uint32_t d[4][2];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    d[g][0] = pack2<IO>(v[4 * g] * f, v[4 * g + 1] * f);
+    d[g][1] = pack2<IO>(v[4 * g + 2] * f, v[4 * g + 3] * f);
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    swap_halves(d[0][j], d[1][j]);
+    swap_halves(d[2][j], d[3][j]);
+  }
+  out[0] = make_uint4(d[0][0], d[0][1], d[1][0], d[1][1]);
+  out[1] = make_uint4(d[2][0], d[2][1], d[3][0], d[3][1]);
+}
+
+// Work-groups of a launch: tiles of rows of every sequence and key head. Even numbering, levels of one tile of
+// each (the last, which see most, first); or numbered through, where sequences are much shorter than the longest:
+// those of sequence b begin at start(b) * per / tile + b, which leaves each enough.
+struct Tiles {
+  int seqs, heads;       // sequences (with what lies behind the last), key heads
+  int even;              // tiles of the longest, 0: numbered through
+  int through;           // tiles of all sequences, numbered through
+};
+
+}  // namespace dsa

@@ -534,3 +534,19 @@ struct NormArgs {
 hipError_t launch_layer_norm(const NormArgs& a, hipStream_t s);
 size_t layer_norm_grad_workspace_bytes(int64_t rows, int width);
 hipError_t launch_layer_norm_grad(const NormArgs& a, hipStream_t s);
+// Dense attention over keys and values of their own: tensors [rows, heads, width] by strides (elements)
+struct DenseTensor {
+  const void* p; int64_t row, head;
+};
+struct DenseArgs {
+  DenseTensor q, qr, k, kr, v; int io;
+  const int32_t* row_start; const int32_t* key_start;   // [batch + 1]
+  const int32_t* act_q; const int32_t* act_k;
+  int batch, total_rows, total_keys, n1, n2, d, dr, rows_behind, max_rows, max_kv, sparse_mode; float scale;
+  int stat_padded;              // statistics [batch, n2, rows a sequence, n1 / n2], else [n2, total_rows, n1 / n2]
+  void* out; float* sm_max; float* sm_sum;
+  void* ws; size_t ws_bytes; int kv_splits;
+};
+size_t dense_attn_workspace_bytes(const DenseArgs& a);
+// *lacking: 0, or (nothing is launched) the bytes of a workspace that the call needs and has not
+hipError_t launch_dense_attn(const DenseArgs& a, size_t* lacking, hipStream_t s);

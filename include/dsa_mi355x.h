@@ -473,6 +473,42 @@ int dsa_prefix_attn(const void* query, const void* query_rope, const void* key, 
                     float scale, void* out, float* sm_max, float* sm_sum, void* workspace, size_t workspace_bytes,
                     int kv_splits, void* stream);
 
+/*
+ * Workspace bytes of dsa_dense_attn for these bounds (0 where every row has one range of tokens); needs no
+ * initialisation. kv_splits <= 0: the library's choice; pass the same value to both.
+ */
+size_t dsa_dense_attn_workspace_bytes(int batch, int total_rows, int rows_behind, int n1, int n2, int d, int max_rows, int max_kv,
+                                      int kv_splits);
+
+/*
+ * Dense attention of whole prompts, of chunks of them or of single tokens over keys and values of their own
+ * (no counterpart in the reference, whose attention is sparse). Query head h reads key head h / (N1 / N2). Packed row
+ * r is query s = r - row_start[b] of batch b and sees the tokens t < act_k[b] - act_q[b] + s + 1 (sparse_mode 3: its
+ * last query is its last token) or t < act_k[b] (sparse_mode 0) of its sequence, key rows key_start[b] + t.
+ *   score = (q . k + q_rope . k_rope) * scale, out = softmax(score) v, sm_max = max score,
+ *   sm_sum = sum exp(score - sm_max)   (both or neither may be NULL)
+ * Rows with s >= act_q[b], that see no token, or behind the last batch get out = 0, sm = 0. A row that sees a value that
+ * is not finite gets NaN in that column at least, and may get NaN in all; a row that does not see it is not affected. Where
+ * a score is NaN, sm_sum is NaN; sm_max need not be.
+ *   query [total_rows, N1, D], query_rope [.., 64], key [total_keys, N2, D], key_rope [.., 64], value [total_keys, N2, D]:
+ *   rows and heads by strides in elements (0 for heads that share one), multiples of 8, on 16-byte borders, row
+ *   strides below 2^24; fp16 / bf16; D in {64, 128}, dr 0 or (D = 128) 64. total_rows * N1 and total_keys * N2 < 2^30.
+ *   out [total_rows, N1, D] contiguous; sm_max, sm_sum fp32 [batch, N2, total_rows / batch, N1 / N2] (stat_padded:
+ *   row_start[b] = b * total_rows / batch) or [N2, total_rows, N1 / N2].
+ *   row_start, key_start [batch + 1] ascending from 0, act_q, act_k [batch], on the device. rows_behind: total_rows -
+ *   row_start[batch]; max_rows: the most of row_start[b + 1] - row_start[b] and rows_behind; max_kv: the longest act_k that
+ *   the caller expects (it only chooses how the work is cut).
+ *   kv_splits (<= 64): 0, or how many ranges of tokens a row's are cut into. Calls that share a workspace must be
+ *   ordered.
+ */
+int dsa_dense_attn(const void* query, int64_t q_row, int64_t q_head, const void* query_rope, int64_t qr_row, int64_t qr_head,
+                   const void* key, int64_t k_row, int64_t k_head, const void* key_rope, int64_t kr_row, int64_t kr_head,
+                   const void* value, int64_t v_row, int64_t v_head, int io_dtype, const int32_t* row_start,
+                   const int32_t* key_start, const int32_t* act_q, const int32_t* act_k, int batch, int total_rows,
+                   int total_keys, int rows_behind, int n1, int n2, int d, int dr, int max_rows, int max_kv, int sparse_mode,
+                   float scale, void* out, int stat_padded, float* sm_max, float* sm_sum, void* workspace,
+                   size_t workspace_bytes, int kv_splits, void* stream);
+
 #define DSA_NORM_MAX_WIDTH 16384
 
 /*
