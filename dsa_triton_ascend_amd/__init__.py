@@ -16,7 +16,7 @@ Beside them, what a model needs around these paths:
 * :func:`rotary_embedding` / :func:`rotary_embedding_grad` — rotary positions
 * :func:`latent_cache_append`, :func:`index_cache_append` — new tokens into the paged caches
 * :func:`shared_prefix_attention` — dense attention over a paged cache, a common prefix computed once
-* :func:`dense_attention` — dense attention of whole prompts with grouped key heads
+* :func:`dense_attention` / :func:`dense_attention_grad` — dense attention of whole prompts with grouped key heads
 * :func:`layer_norm` / :func:`layer_norm_grad` — the norm of an indexer's keys or of hidden rows
 
 All run hand-written gfx950 HIP kernels through the C ABI of
@@ -34,7 +34,8 @@ from .dense_loss import (DenseLightningIndexerGradKLLoss, DenseLightningIndexerS
 from .rotary import (IndexAppendPlan, LatentAppendPlan, RotaryEmbedding, index_cache_append, latent_cache_append,
                      rotary_embedding, rotary_embedding_grad)
 from .shared_prefix import SharedPrefixAttention, SharedPrefixPlan, shared_prefix_attention
-from .dense_attention import DenseAttention, DenseAttentionPlan, dense_attention
+from .dense_attention import (DenseAttention, DenseAttentionGradPlan, DenseAttentionPlan, dense_attention,
+                              dense_attention_grad)
 from .layer_norm import LayerNorm, layer_norm, layer_norm_grad
 
 __all__ = ["lightning_indexer", "LightningIndexer", "sparse_flash_attention", "SparseFlashAttention",
@@ -46,5 +47,6 @@ __all__ = ["lightning_indexer", "LightningIndexer", "sparse_flash_attention", "S
            "PrefillPlan", "dsa_prefill",
            "rotary_embedding", "rotary_embedding_grad", "RotaryEmbedding", "latent_cache_append", "LatentAppendPlan",
            "index_cache_append", "IndexAppendPlan", "shared_prefix_attention", "SharedPrefixAttention",
-           "SharedPrefixPlan", "dense_attention", "DenseAttention", "DenseAttentionPlan",
+           "SharedPrefixPlan", "dense_attention", "dense_attention_grad", "DenseAttention", "DenseAttentionPlan",
+           "DenseAttentionGradPlan",
            "layer_norm", "layer_norm_grad", "LayerNorm"]

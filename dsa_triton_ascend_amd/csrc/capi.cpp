@@ -827,4 +827,63 @@ int dsa_dense_attn(const void* query, int64_t q_row, int64_t q_head, const void*
   return hip_status(e, "dsa_dense_attn launch");
 }
 
+size_t dsa_dense_attn_grad_workspace_bytes(int batch, int total_rows, int total_keys, int rows_behind, int keys_behind, int n1,
+                                           int n2, int d, int dr, int max_rows, int max_keys, int max_kv, int splits) {
+  if (batch <= 0 || total_rows < 0 || total_keys < 0 || rows_behind < 0 || keys_behind < 0 || n1 <= 0 || n2 <= 0 || n1 % n2 != 0 ||
+      d <= 0 || dr < 0 || max_rows < 0 || max_keys < 0 || max_kv < 0)
+    return 0;
+  DenseGradArgs g{};
+  DenseArgs& a = g.f;
+  a.batch = batch, a.total_rows = total_rows, a.total_keys = total_keys, a.rows_behind = rows_behind, a.n1 = n1, a.n2 = n2;
+  a.d = d, a.dr = dr, a.max_rows = max_rows, a.max_kv = max_kv, a.kv_splits = splits, g.keys_behind = keys_behind, g.max_keys = max_keys;
+  return dense_grad_workspace_bytes(g);
+}
+
+int dsa_dense_attn_grad(const void* query, int64_t q_row, int64_t q_head, const void* query_rope, int64_t qr_row, int64_t qr_head,
+                        const void* key, int64_t k_row, int64_t k_head, const void* key_rope, int64_t kr_row, int64_t kr_head,
+                        const void* value, int64_t v_row, int64_t v_head, const void* d_out, int64_t d_row, int64_t d_head,
+                        const void* out, int64_t o_row, int64_t o_head, int io_dtype, const int32_t* row_start,
+                        const int32_t* key_start, const int32_t* act_q, const int32_t* act_k, int batch, int total_rows,
+                        int total_keys, int rows_behind, int keys_behind, int n1, int n2, int d, int dr, int max_rows,
+                        int max_keys, int max_kv, int sparse_mode, float scale, int stat_padded, const float* sm_max,
+                        const float* sm_sum, void* d_query, void* d_query_rope, void* d_key, void* d_key_rope, void* d_value,
+                        void* workspace, size_t workspace_bytes, int splits, void* stream) {
+  static const char* fn = "dsa_dense_attn_grad";
+  DenseGradArgs g{};
+  DenseArgs& a = g.f;
+  a.q = {query, q_row, q_head}, a.qr = {query_rope, qr_row, qr_head}, a.k = {key, k_row, k_head};
+  a.kr = {key_rope, kr_row, kr_head}, a.v = {value, v_row, v_head}, a.io = io_dtype;
+  a.row_start = row_start, a.key_start = key_start, a.act_q = act_q, a.act_k = act_k, a.batch = batch;
+  a.total_rows = total_rows, a.total_keys = total_keys, a.rows_behind = rows_behind, a.n1 = n1, a.n2 = n2, a.d = d, a.dr = dr;
+  a.max_rows = max_rows, a.max_kv = max_kv, a.sparse_mode = sparse_mode, a.scale = scale, a.stat_padded = stat_padded;
+  a.sm_max = const_cast<float*>(sm_max), a.sm_sum = const_cast<float*>(sm_sum), a.ws = workspace, a.ws_bytes = workspace_bytes;
+  a.kv_splits = splits, g.d_out = {d_out, d_row, d_head}, g.out = {out, o_row, o_head}, g.keys_behind = keys_behind;
+  g.max_keys = max_keys, g.dq = d_query, g.dqr = d_query_rope, g.dk = d_key, g.dkr = d_key_rope, g.dv = d_value;
+  const int st = check_dense(fn, a);
+  if (st != DSA_OK) return st;
+  if (!d_out || !out || !sm_max || !sm_sum || !d_query || !d_key || !d_value || (dr > 0 && (!d_query_rope || !d_key_rope)))
+    return fail(DSA_ERR_INVALID, "%s: null pointer argument", fn);
+  for (const DenseTensor* t : {&g.d_out, &g.out}) {
+    if (((uintptr_t)t->p & 15) != 0 || t->row % 8 != 0 || t->head % 8 != 0)
+      return fail(DSA_ERR_INVALID, "%s: rows and heads must begin on 16-byte borders", fn);
+    if (t->row < 0 || t->head < 0 || t->row >= (1 << 24) || t->head >= (1ll << 40))
+      return fail(DSA_ERR_UNSUPPORTED, "%s: row strides of 2^24 elements", fn);
+  }
+  if ((((uintptr_t)d_query | (uintptr_t)d_query_rope | (uintptr_t)d_key | (uintptr_t)d_key_rope | (uintptr_t)d_value) & 15) != 0)
+    return fail(DSA_ERR_INVALID, "%s: outputs must be 16-byte aligned", fn);
+  if (keys_behind < 0 || keys_behind > total_keys || max_keys < 0 || max_keys > total_keys)
+    return fail(DSA_ERR_INVALID, "%s: keys_behind or max_keys past the tensors' rows", fn);
+  if (splits > 64) return fail(DSA_ERR_UNSUPPORTED, "%s: splits=%d > 64", fn, splits);
+  if (total_rows == 0 && total_keys == 0) {
+    g_err[0] = 0;
+    return DSA_OK;
+  }
+  size_t lacking = 0;
+  const hipError_t e = launch_dense_grad(g, &lacking, (hipStream_t)stream);
+  if (lacking > 0)
+    return fail(DSA_ERR_INVALID, "%s: a 16-byte aligned workspace of %zu bytes required, %zu given", fn, lacking,
+                workspace ? workspace_bytes : (size_t)0);
+  return hip_status(e, "dsa_dense_attn_grad launch");
+}
+
 }  // extern "C"

@@ -1,0 +1,711 @@
+// Gradients of the dense attention of whole prompts, for gfx950.
+//
+// With P = e^(score - max) / sum, dP = dO . v, delta = dO . O (both per head row), dS = P (dP - delta):
+//   dV = P^T dO,   dK = scale dS^T Q,   dQ = scale dS K,
+// dK and dV summed over the queries and heads that read them. P is made again from the scores and the statistics:
+// keeping it would cost more bytes than its product costs time.
+//
+// Three launches, without atomics, so results do not depend on timing:
+//  * rows: delta and the logarithm of the sum for every head row (fp16: also the norms that bound dS);
+//  * keys: a work-group has 128 tokens of one key head, 32 a wave, K and V in registers, and runs over the head rows
+//    that see them (the group's heads are rows side by side): S = Q K^T and dP = dO V^T with the head rows as M, whose
+//    results are already the B operands of dV^T += dO^T P and dK^T += Q^T dS;
+//  * queries: 128 head rows, 32 a wave, Q and dO in registers, running over the tokens: S^T = K Q^T, dP^T = V dO^T,
+//    dQ^T += K^T dS^T.
+// S and dP are computed in both, 7 products instead of 5; what that saves is the addition of dQ from many work-groups,
+// in 32 bits and an order of its own. P and dS are rounded to the io type for their products.
+#include <algorithm>
+
+#include "dense_attn.hpp"
+
+namespace dsa {
+namespace {
+
+constexpr int NWV = 4;
+constexpr int BN = 64;     // rows of a tile in LDS
+constexpr int NBUF = 2;
+constexpr int TOK = NWV * 32;     // tokens, or head rows, of a work-group
+constexpr int PREP = 512;         // work-groups of the first launch
+
+// fp16 keeps 11 bits down to 2^-14 and none below 2^-25. P <= 1 is multiplied by 2^15 for its product. dS is bounded by
+// 2 max|dO| max|v| (row norms), and multiplied by the power of two that takes this bound to 2^15.
+template <int IO> constexpr float p_shift() { return IO == IO_F16 ? 15.f : 0.f; }
+
+struct GradK {
+  Rows q, qr, k, kr, v, d, o;
+  Lens len;
+  int heads, key_heads, per;
+  uint32_t per_mul;        // r / per for r < 2^31: see rows_of
+  int per_shift;
+  int q_seqs, k_seqs;      // sequences, with what lies behind the last
+  int q_even, k_even;      // tiles of the longest, 0: numbered through
+  float scale;
+  int64_t stat_head;
+  int stat_padded, s1;     // s1: rows of a sequence of padded statistics
+  const float* sm_max;
+  const float* sm_sum;
+  float* lse;              // [key heads][rows * per]: log2 of the sum of e^score, +inf for rows that see nothing
+  float* delta;
+  float* norms;            // fp16: [2][PREP] largest |dO|^2 and |v|^2
+  uint16_t* dq;
+  uint16_t* dqr;
+  uint16_t* dk;
+  uint16_t* dkr;
+  uint16_t* dv;
+  int k_splits, k_chunk, k_blocks;   // ranges of head rows; blocks of 32 tokens, all key heads
+  int q_splits, q_chunk, q_blocks;   // ranges of tokens; blocks of 32 head rows
+  float4* k_part;
+  float4* q_part;
+};
+
+__device__ __forceinline__ int row_div(const GradK& a, int r) { return (int)(((uint64_t)(uint32_t)r * a.per_mul) >> (31 + a.per_shift)); }
+
+// ---------------------------------------------------------------- rows
+template <int IO, int D>
+__global__ __launch_bounds__(256) void dense_prep_kernel(GradK a) {
+  constexpr int LPR = D / 8;   // lanes a row
+  const int lane = threadIdx.x & 63;
+  const int slot = threadIdx.x / LPR, c = (threadIdx.x % LPR) * 8;
+  auto values = [&](const uint16_t* p, float (&x)[8]) {
+    const uint4 u = ldg16(p + c);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[2 * i] = to_f32<IO>((uint16_t)w[i]), x[2 * i + 1] = to_f32<IO>((uint16_t)(w[i] >> 16));
+  };
+  auto row_sum = [&](float x) {
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) x += __shfl_xor(x, o);
+    return x;
+  };
+  constexpr int SLOTS = 256 / LPR;
+  float most_d = 0.f, most_v = 0.f;
+  const int64_t total = (int64_t)a.len.rows * a.heads;
+  for (int64_t i = (int64_t)blockIdx.x * SLOTS + slot; i < total; i += (int64_t)gridDim.x * SLOTS) {
+    const int64_t row = i / a.heads;
+    const int h = (int)(i - row * a.heads);
+    const int n = row_div(a, h), g = h - n * a.per;
+    float d[8], o[8], s = 0.f, q = 0.f;
+    values(a.d.p + row * a.d.row + h * a.d.head, d);
+    values(a.o.p + row * a.o.row + h * a.o.head, o);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(d[e], o[e], s), q = fmaf(d[e], d[e], q);
+    const int64_t at = n * (int64_t)a.len.rows * a.per + row * a.per + g;
+    int64_t st = at;
+    if (a.stat_padded) {
+      const int64_t b = row / a.s1;
+      st = ((b * a.key_heads + n) * a.s1 + (row - b * a.s1)) * a.per + g;
+    }
+    const float m = a.sm_max[st], l = a.sm_sum[st];
+    s = row_sum(s);
+    if constexpr (IO == IO_F16) {
+      q = row_sum(q);
+      // (rows that see nothing, padding among them, do not count; those that are not finite give NaN whatever the factor)
+      if (l != 0.f && q < INFINITY) most_d = fmaxf(most_d, q);
+    }
+    if (c == 0) {
+      a.lse[at] = l == 0.f ? INFINITY : m * LOG2E + log2f(l) - p_shift<IO>();
+      a.delta[at] = s;
+    }
+  }
+  if constexpr (IO == IO_F16) {
+    const int64_t keys = (int64_t)a.len.keys * a.key_heads;
+    for (int64_t i = (int64_t)blockIdx.x * SLOTS + slot; i < keys; i += (int64_t)gridDim.x * SLOTS) {
+      const int64_t row = i / a.key_heads;
+      const int b = batch_of_row(a.len.key_start, a.len.batch, (int)row);
+      if (row - a.len.key_start[b] >= a.len.act_k[b]) continue;   // padding
+      float v[8], q = 0.f;
+      values(a.v.p + row * a.v.row + (i - row * a.key_heads) * a.v.head, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q = fmaf(v[e], v[e], q);
+      q = row_sum(q);
+      if (q < INFINITY) most_v = fmaxf(most_v, q);
+    }
+    __shared__ float red[2][4];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      most_d = fmaxf(most_d, __shfl_xor(most_d, o));
+      most_v = fmaxf(most_v, __shfl_xor(most_v, o));
+    }
+    if (lane == 0) red[0][threadIdx.x >> 6] = most_d, red[1][threadIdx.x >> 6] = most_v;
+    __syncthreads();
+    if (threadIdx.x < 2) {
+      const float* r = red[threadIdx.x];
+      a.norms[threadIdx.x * PREP + blockIdx.x] = fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]));
+    }
+  }
+}
+
+// The factor of dS (a power of two) and the one that undoes it, by the whole work-group
+template <int IO>
+__device__ __forceinline__ float2 ds_factor(const GradK& a, float (*red)[NWV]) {
+  if constexpr (IO != IO_F16) return make_float2(1.f, 1.f);
+  float m[2];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    m[w] = 0.f;
+#pragma unroll
+    for (int i = 0; i < PREP; i += NWV * 64) m[w] = fmaxf(m[w], a.norms[w * PREP + i + threadIdx.x]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m[w] = fmaxf(m[w], __shfl_xor(m[w], o));
+    if ((threadIdx.x & 63) == 0) red[w][threadIdx.x >> 6] = m[w];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 2; ++w) m[w] = fmaxf(fmaxf(red[w][0], red[w][1]), fmaxf(red[w][2], red[w][3]));
+  // 2 |dO| |v| 2^e <= 2^15: 2^e = 2^floor(14 - log2(|dO| |v|)); no more than fp32's exponents hold
+  const float e = floorf(14.f - 0.5f * (log2f(fmaxf(m[0], 1e-30f)) + log2f(fmaxf(m[1], 1e-30f))));
+  const float f = exp2f(fminf(fmaxf(e, -100.f), 100.f));
+  return make_float2(f, 1.f / f);
+}
+
+// ---------------------------------------------------------------- which tile
+// i: the work-group; count(q) rows (or tokens) of a sequence, per of them a position of starts[]. Returns the sequence,
+// the tile's number from the sequence's first and the key head; tile < 0: none.
+struct Place {
+  int b, n, tile, sp;
+};
+template <typename F>
+__device__ __forceinline__ Place place_of(int i, int seqs, int heads, int splits, int even, const int32_t* starts, int per, F&& tiles_of) {
+  Place p;
+  if (even) {
+    const int pairs = seqs * heads, level = i / pairs;
+    i -= level * pairs;
+    p.b = i / heads;
+    p.n = i - p.b * heads;
+    p.sp = level % splits;
+    p.tile = level / splits;
+    if (p.tile >= tiles_of(p.b)) p.tile = -1;
+    return p;
+  }
+  p.sp = i % splits;
+  i /= splits;
+  p.n = i % heads;
+  i /= heads;
+  int lo = 0, hi = seqs - 1;
+  auto first = [&](int s) { return (int)((int64_t)starts[s] * per / TOK) + s; };
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first(mid) <= i) lo = mid; else hi = mid - 1;
+  }
+  p.b = lo;
+  p.tile = i - first(lo);
+  if (p.tile >= tiles_of(lo)) p.tile = -1;
+  return p;
+}
+
+// ---------------------------------------------------------------- keys
+template <int D, int DR> struct KeyLds {
+  uint8_t q[NBUF][BN * D * 2];
+  uint8_t d[NBUF][BN * D * 2];
+  uint8_t qr[NBUF][DR ? BN * DR * 2 : 16];
+  float lse[NBUF][BN];
+  float delta[NBUF][BN];
+  uint64_t bad[NBUF][NWV];
+  float red[2][NWV];
+};
+
+__device__ __forceinline__ void lds_dma4(const void* gptr, void* lds_base) {
+  const uint32_t m0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds_base;
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(gptr), "s"(m0) : "memory", "m0");
+}
+
+template <int IO, int D, int DR>
+__global__ __launch_bounds__(NWV * 64) void dense_keys_kernel(GradK a) {
+  constexpr int KSN = D / 16, KS = (D + DR) / 16, ON = D / 32, RN = DR / 32, RB = D * 2;
+  __shared__ __attribute__((aligned(16))) KeyLds<D, DR> L;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kg = lane >> 5, rr = lane & 31;
+  const Place at = place_of(blockIdx.x, a.k_seqs, a.key_heads, a.k_splits, a.k_even, a.len.key_start, 1, [&](int b) {
+    const Seq q = seq_of(a.len, b);
+    return (q.keys + TOK - 1) / TOK;
+  });
+  if (at.tile < 0) return;
+  const int b = at.b, n = at.n;
+  const Seq seq = seq_of(a.len, b);
+  const float2 factor = ds_factor<IO>(a, L.red);
+
+  const int t0 = at.tile * TOK, t_end = min(seq.keys, t0 + TOK), t_seen = min(t_end, seq.ak);
+  const int t = t0 + wave * 32 + rr;
+  // head rows [r_lo, r_hi) see some of these tokens, from r_full on all of them; this range's share
+  const int r_end = seq.aq * a.per;
+  const int r_lo = max(first_query(a.len, seq, t0) * a.per, at.sp * a.k_chunk);
+  const int r_hi = at.sp == a.k_splits - 1 ? r_end : min(r_end, (at.sp + 1) * a.k_chunk);
+  const int r_full = t_seen > t0 ? first_query(a.len, seq, t_seen - 1) * a.per : 0;
+  const int w_first = t0 + wave * 32 < t_seen ? first_query(a.len, seq, t0 + wave * 32) * a.per : INT_MAX;
+  const int my_first = t < t_seen ? first_query(a.len, seq, t) * a.per : INT_MAX;
+  const int ntiles = t_seen > t0 && r_hi > r_lo ? (r_hi - r_lo + BN - 1) / BN : 0;
+
+  f32x16 dk[ON + RN], dv[ON];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+#pragma unroll
+    for (int c = 0; c < ON + RN; ++c) dk[c][i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < ON; ++c) dv[c][i] = 0.f;
+  }
+
+  if (ntiles > 0) {
+    const float sl2 = a.scale * LOG2E;
+    const Share<RB, BN, NWV> sh(wave, lane);
+    const Share<DR ? DR * 2 : 128, BN, NWV> shr(wave, lane);
+    // (rows past the last repeat it; they are masked)
+    auto load_rows = [&](auto share, const Rows& x, int r0, uint8_t* dst) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < share.CNT; ++j) {
+        const int r = min(r0 + j * share.STEP + share.row, r_hi - 1), s = row_div(a, r), g = r - s * a.per;
+        const char* p = reinterpret_cast<const char*>(x.p + (int64_t)(seq.r0 + s) * x.row + (int64_t)(n * a.per + g) * x.head);
+        lds_dma16_untracked(p + share.col, dst + (j * NWV + wave) * 1024);
+      }
+    };
+    const int64_t stat0 = n * (int64_t)a.len.rows * a.per + (int64_t)seq.r0 * a.per;
+    auto load_tile = [&](int u) __attribute__((always_inline)) {
+      const int r0 = r_lo + u * BN, buf = u % NBUF;
+      load_rows(sh, a.q, r0, L.q[buf]);
+      load_rows(sh, a.d, r0, L.d[buf]);
+      if constexpr (DR > 0) load_rows(shr, a.qr, r0, L.qr[buf]);
+      if (wave == 0) lds_dma4(a.lse + stat0 + min(r0 + lane, r_hi - 1), L.lse[buf]);
+      if (wave == 1) lds_dma4(a.delta + stat0 + min(r0 + lane, r_hi - 1), L.delta[buf]);
+    };
+    load_tile(0);
+    uint4 kf[KS], vf[KSN];
+    {
+      const int64_t tt = seq.k0 + min(t, t_seen - 1);
+      const uint16_t* kp = a.k.p + tt * a.k.row + n * a.k.head + kg * 8;
+      const uint16_t* vp = a.v.p + tt * a.v.row + n * a.v.head + kg * 8;
+#pragma unroll
+      for (int j = 0; j < KSN; ++j) kf[j] = ldg16(kp + j * 16), vf[j] = ldg16(vp + j * 16);
+      if constexpr (DR > 0) {
+        const uint16_t* rp = a.kr.p + tt * a.kr.row + n * a.kr.head + kg * 8;
+#pragma unroll
+        for (int j = KSN; j < KS; ++j) kf[j] = ldg16(rp + (j - KSN) * 16);
+      }
+    }
+    const int qk = s_row(rr);
+    for (int u = 0; u < ntiles; ++u) {
+      const int r0 = r_lo + u * BN, buf = u % NBUF;
+      // (a masked pair has P = dS = 0, but 0 times a value that is not finite would reach tokens that the row does not see)
+      const bool mixed = r0 < r_full || r0 + BN > r_hi;
+      wait_vmcnt<0>();
+      asm volatile("" ::: "memory");
+      if (mixed) {
+        uint64_t bad = clean_share<IO, RB, BN, NWV>(lds_addr(L.q[buf]), wave, lane) |
+                       clean_share<IO, RB, BN, NWV>(lds_addr(L.d[buf]), wave, lane);
+        if constexpr (DR > 0) bad |= clean_share<IO, 128, BN, NWV>(lds_addr(L.qr[buf]), wave, lane);
+        if (lane == 0) L.bad[buf][wave] = bad;
+      }
+      lds_barrier();
+      if (u + 1 < ntiles) load_tile(u + 1);
+      if (r0 + BN <= w_first) continue;
+      uint64_t bad = 0;
+      if (mixed) bad = L.bad[buf][0] | L.bad[buf][1] | L.bad[buf][2] | L.bad[buf][3];
+      const uint32_t qt = lds_addr(L.q[buf]), dt = lds_addr(L.d[buf]), qrt = lds_addr(L.qr[buf]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        f32x16 s, dp;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < KS; ++j)
+          s = Mfma<IO>::m32(j < KSN ? op_frag<RB>(qt, h * 32 + qk, j, kg) : op_frag<128>(qrt, h * 32 + qk, j - KSN, kg), kf[j], s);
+#pragma unroll
+        for (int j = 0; j < KSN; ++j) dp = Mfma<IO>::m32(op_frag<RB>(dt, h * 32 + qk, j, kg), vf[j], dp);
+        uint32_t pd[8], sd[8];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {   // rows 16 x + 8 kg + 0 .. 7
+          const float* lp = &L.lse[buf][h * 32 + 16 * x + 8 * kg];
+          const float* ep = &L.delta[buf][h * 32 + 16 * x + 8 * kg];
+          float p[8], ds[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int i = 8 * x + e;
+            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sl2, -lp[e]));
+            ds[e] = p[e] * (dp[i] - ep[e]);
+          }
+          if (bad)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if ((bad >> (h * 32 + 16 * x + 8 * kg + e)) & 1u) p[e] = ds[e] = __builtin_nanf("");
+          if (mixed)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int r = r0 + h * 32 + 16 * x + 8 * kg + e;
+              if (r < my_first || r >= r_hi) p[e] = ds[e] = 0.f;
+            }
+          if constexpr (IO == IO_F16) {
+            const float f = factor.x * 0x1p-15f;   // (P has the factor 2^15)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ds[e] *= f;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            pd[4 * x + e] = pack2<IO>(p[2 * e], p[2 * e + 1]);
+            sd[4 * x + e] = pack2<IO>(ds[2 * e], ds[2 * e + 1]);
+          }
+        }
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          const uint4 pb = make_uint4(pd[4 * st], pd[4 * st + 1], pd[4 * st + 2], pd[4 * st + 3]);
+          const uint4 sb = make_uint4(sd[4 * st], sd[4 * st + 1], sd[4 * st + 2], sd[4 * st + 3]);
+#pragma unroll
+          for (int c = 0; c < ON; ++c) {
+            dv[c] = Mfma<IO>::m32(tr_frag<RB>(dt, h * 32 + st * 16, c, lane), pb, dv[c]);
+            dk[c] = Mfma<IO>::m32(tr_frag<RB>(qt, h * 32 + st * 16, c, lane), sb, dk[c]);
+          }
+#pragma unroll
+          for (int c = 0; c < RN; ++c) dk[ON + c] = Mfma<IO>::m32(tr_frag<128>(qrt, h * 32 + st * 16, c, lane), sb, dk[ON + c]);
+        }
+      }
+    }
+  }
+
+  // lane l: token t, columns c * 32 + 8 g + 4 kg + j
+  const float fk = a.scale * factor.y, fv = IO == IO_F16 ? 0x1p-15f : 1.f;
+  if (a.k_splits > 1) {
+    const int blk = n * (a.k_blocks / a.key_heads) + seq.k0 / 32 + b + at.tile * NWV + wave;
+    if (t0 + wave * 32 >= seq.keys) return;
+    float4* dst = a.k_part + ((int64_t)at.sp * a.k_blocks + blk) * ((2 * D + DR) / 8) * 64 + lane;
+#pragma unroll
+    for (int c = 0; c < ON + RN + ON; ++c) {
+      const f32x16& v = c < ON + RN ? dk[c < ON + RN ? c : 0] : dv[c >= ON + RN ? c - ON - RN : 0];
+      const float f = c < ON + RN ? fk : fv;
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        dst[(c * 4 + g) * 64] = make_float4(v[4 * g] * f, v[4 * g + 1] * f, v[4 * g + 2] * f, v[4 * g + 3] * f);
+    }
+    return;
+  }
+  const bool live = t < t_seen, valid = t < t_end;
+  const int64_t tt = (int64_t)(seq.k0 + t) * a.key_heads + n;
+  auto store = [&](const f32x16& v, float f, uint16_t* dst) __attribute__((always_inline)) {
+    uint4 w[2];
+    pack_tile<IO>(v, f, w);
+    if (valid) {
+      stg16(dst + 8 * kg, live ? w[0] : make_uint4(0, 0, 0, 0));
+      stg16(dst + 8 * kg + 16, live ? w[1] : make_uint4(0, 0, 0, 0));
+    }
+  };
+#pragma unroll
+  for (int c = 0; c < ON; ++c) store(dk[c], fk, a.dk + tt * D + c * 32);
+#pragma unroll
+  for (int c = 0; c < RN; ++c) store(dk[ON + c], fk, a.dkr + tt * DR + c * 32);
+#pragma unroll
+  for (int c = 0; c < ON; ++c) store(dv[c], fv, a.dv + tt * D + c * 32);
+}
+
+// ---------------------------------------------------------------- queries
+template <int D, int DR> struct QueryLds {
+  uint8_t k[NBUF][BN * D * 2];
+  uint8_t v[NBUF][BN * D * 2];
+  uint8_t kr[NBUF][DR ? BN * DR * 2 : 16];
+  uint64_t bad[NBUF][NWV];
+  float red[2][NWV];
+};
+
+template <int IO, int D, int DR>
+__global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
+  constexpr int KSN = D / 16, KS = (D + DR) / 16, ON = D / 32, RN = DR / 32, RB = D * 2;
+  __shared__ __attribute__((aligned(16))) QueryLds<D, DR> L;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kg = lane >> 5, rr = lane & 31;
+  Place at = place_of(blockIdx.x, a.q_seqs, a.key_heads, a.q_splits, a.q_even, a.len.row_start, a.per, [&](int b) {
+    const Seq q = seq_of(a.len, b);
+    return (q.rows * a.per + TOK - 1) / TOK;
+  });
+  if (at.tile < 0) return;
+  const int b = at.b, n = at.n;
+  const Seq seq = seq_of(a.len, b);
+  at.tile = (seq.rows * a.per + TOK - 1) / TOK - 1 - at.tile;   // the last, which see most, first
+  const float2 factor = ds_factor<IO>(a, L.red);
+
+  const int r_base = at.tile * TOK, r_end = min(seq.rows * a.per, r_base + TOK);
+  const int t_lo = at.sp * a.q_chunk, t_hi = at.sp == a.q_splits - 1 ? INT_MAX : t_lo + a.q_chunk;
+  auto seen = [&](int x, int y) {
+    return x >= y || x / a.per >= seq.aq ? 0 : min(limit_of(a.len, seq, min((y - 1) / a.per, seq.aq - 1)), t_hi);
+  };
+  const int hi = seen(r_base, r_end);
+  const int min_lim = max(t_lo + 1, limit_of(a.len, seq, r_base / a.per));
+  const int ntiles = hi > t_lo ? (hi - t_lo + BN - 1) / BN : 0;
+  const int w_base = r_base + wave * 32, w_hi = seen(w_base, min(r_end, w_base + 32));
+  const int row = w_base + rr;
+  const bool valid = row < r_end;
+  const int r = valid ? row : r_end - 1, s = r / a.per, g = r - s * a.per;
+  const int lim = valid ? min(limit_of(a.len, seq, s), t_hi) : 0;
+  const bool dead = lim <= t_lo;
+
+  f32x16 dq[ON + RN];
+#pragma unroll
+  for (int c = 0; c < ON + RN; ++c)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dq[c][i] = 0.f;
+
+  if (ntiles > 0) {
+    const float sl2 = a.scale * LOG2E;
+    const Share<RB, BN, NWV> sh(wave, lane);
+    const Share<DR ? DR * 2 : 128, BN, NWV> shr(wave, lane);
+    const uint16_t* const kb = a.k.p + (int64_t)seq.k0 * a.k.row + n * a.k.head;
+    const uint16_t* const vb = a.v.p + (int64_t)seq.k0 * a.v.row + n * a.v.head;
+    const uint16_t* const krb = DR ? a.kr.p + (int64_t)seq.k0 * a.kr.row + n * a.kr.head : nullptr;
+    const uint32_t k_row = (uint32_t)a.k.row * 2, v_row = (uint32_t)a.v.row * 2, kr_row = (uint32_t)a.kr.row * 2;
+    auto load_rows = [&](auto share, const uint16_t* base, uint32_t row_bytes, int t0, uint8_t* dst) __attribute__((always_inline)) {
+      const char* p = reinterpret_cast<const char*>(base) + (int64_t)t0 * row_bytes;
+#pragma unroll
+      for (int j = 0; j < share.CNT; ++j) {
+        const int t = min(j * share.STEP + share.row, seq.ak - 1 - t0);
+        lds_dma16_sbase_untracked(p, (uint32_t)t * row_bytes + share.col, dst + (j * NWV + wave) * 1024);
+      }
+    };
+    auto load_tile = [&](int u) __attribute__((always_inline)) {
+      const int t0 = t_lo + u * BN, buf = u % NBUF;
+      load_rows(sh, kb, k_row, t0, L.k[buf]);
+      load_rows(sh, vb, v_row, t0, L.v[buf]);
+      if constexpr (DR > 0) load_rows(shr, krb, kr_row, t0, L.kr[buf]);
+    };
+    load_tile(0);
+    uint4 qf[KS], df[KSN];
+    const int64_t stat = n * (int64_t)a.len.rows * a.per + (int64_t)seq.r0 * a.per + r;
+    const float lse = a.lse[stat], delta = a.delta[stat];
+    {
+      const int64_t q_row = seq.r0 + s, head = n * a.per + g;
+      const uint16_t* qp = a.q.p + q_row * a.q.row + head * a.q.head + kg * 8;
+      const uint16_t* dp = a.d.p + q_row * a.d.row + head * a.d.head + kg * 8;
+#pragma unroll
+      for (int j = 0; j < KSN; ++j) qf[j] = ldg16(qp + j * 16), df[j] = ldg16(dp + j * 16);
+      if constexpr (DR > 0) {
+        const uint16_t* rp = a.qr.p + q_row * a.qr.row + head * a.qr.head + kg * 8;
+#pragma unroll
+        for (int j = KSN; j < KS; ++j) qf[j] = ldg16(rp + (j - KSN) * 16);
+      }
+    }
+    const float fs = IO == IO_F16 ? factor.x * 0x1p-15f : 1.f;
+    const int tk = s_row(rr);
+    for (int u = 0; u < ntiles; ++u) {
+      const int t0 = t_lo + u * BN, buf = u % NBUF;
+      const bool mixed = t0 + BN > min_lim;
+      wait_vmcnt<0>();
+      asm volatile("" ::: "memory");
+      if (mixed) {
+        uint64_t bad = clean_share<IO, RB, BN, NWV>(lds_addr(L.k[buf]), wave, lane);
+        if constexpr (DR > 0) bad |= clean_share<IO, 128, BN, NWV>(lds_addr(L.kr[buf]), wave, lane);
+        if (lane == 0) L.bad[buf][wave] = bad;
+      }
+      lds_barrier();
+      if (u + 1 < ntiles) load_tile(u + 1);
+      if (t0 >= w_hi) continue;
+      uint64_t bad = 0;
+      if (mixed) bad = L.bad[buf][0] | L.bad[buf][1] | L.bad[buf][2] | L.bad[buf][3];
+      const uint32_t kt = lds_addr(L.k[buf]), vt = lds_addr(L.v[buf]), krt = lds_addr(L.kr[buf]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        f32x16 sv, dp;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sv[i] = dp[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < KS; ++j)
+          sv = Mfma<IO>::m32(j < KSN ? op_frag<RB>(kt, h * 32 + tk, j, kg) : op_frag<128>(krt, h * 32 + tk, j - KSN, kg), qf[j], sv);
+#pragma unroll
+        for (int j = 0; j < KSN; ++j) dp = Mfma<IO>::m32(op_frag<RB>(vt, h * 32 + tk, j, kg), df[j], dp);
+        float ds[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], sl2, -lse));
+          ds[i] = p * (dp[i] - delta);
+          if constexpr (IO == IO_F16) ds[i] *= fs;
+        }
+        if (bad)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if ((bad >> (h * 32 + s_token(i, kg))) & 1u) ds[i] = __builtin_nanf("");
+        if (mixed)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (t0 + h * 32 + s_token(i, kg) >= lim) ds[i] = 0.f;
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = pack2<IO>(ds[2 * i], ds[2 * i + 1]);
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          const uint4 sb = make_uint4(w[4 * st], w[4 * st + 1], w[4 * st + 2], w[4 * st + 3]);
+#pragma unroll
+          for (int c = 0; c < ON; ++c) dq[c] = Mfma<IO>::m32(tr_frag<RB>(kt, h * 32 + st * 16, c, lane), sb, dq[c]);
+#pragma unroll
+          for (int c = 0; c < RN; ++c) dq[ON + c] = Mfma<IO>::m32(tr_frag<128>(krt, h * 32 + st * 16, c, lane), sb, dq[ON + c]);
+        }
+      }
+    }
+  }
+
+  const float f = a.scale * factor.y;
+  if (a.q_splits > 1) {
+    if (w_base >= r_end) return;
+    const int blk = n * (a.q_blocks / a.key_heads) + (int)((int64_t)seq.r0 * a.per / 32) + b + w_base / 32;
+    float4* dst = a.q_part + ((int64_t)at.sp * a.q_blocks + blk) * ((D + DR) / 8) * 64 + lane;
+#pragma unroll
+    for (int c = 0; c < ON + RN; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        dst[(c * 4 + e) * 64] = dead ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                     : make_float4(dq[c][4 * e] * f, dq[c][4 * e + 1] * f, dq[c][4 * e + 2] * f, dq[c][4 * e + 3] * f);
+    return;
+  }
+  const int64_t head_row = (int64_t)(seq.r0 + s) * a.heads + n * a.per + g;
+  auto store = [&](const f32x16& v, uint16_t* dst) __attribute__((always_inline)) {
+    uint4 w[2];
+    pack_tile<IO>(v, f, w);
+    if (valid) {
+      stg16(dst + 8 * kg, dead ? make_uint4(0, 0, 0, 0) : w[0]);
+      stg16(dst + 8 * kg + 16, dead ? make_uint4(0, 0, 0, 0) : w[1]);
+    }
+  };
+#pragma unroll
+  for (int c = 0; c < ON; ++c) store(dq[c], a.dq + head_row * D + c * 32);
+#pragma unroll
+  for (int c = 0; c < RN; ++c) store(dq[ON + c], a.dqr + head_row * DR + c * 32);
+}
+
+// ---------------------------------------------------------------- joins
+// Adds the ranges' blocks of 32 rows (tokens or head rows), in order. The columns are those of one, two or three
+// outputs side by side: D + DR (+ D).
+template <int IO, int D, int DR, bool KEYS>
+__global__ __launch_bounds__(256) void dense_join_kernel(GradK a) {
+  constexpr int W8 = ((KEYS ? 2 * D : D) + DR) / 8;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rr = lane & 31, kg = lane >> 5;
+  const int blocks = KEYS ? a.k_blocks : a.q_blocks, splits = KEYS ? a.k_splits : a.q_splits, per = KEYS ? 1 : a.per;
+  const int seqs = KEYS ? a.k_seqs : a.q_seqs;
+  const int32_t* starts = KEYS ? a.len.key_start : a.len.row_start;
+  const int per_head = blocks / a.key_heads, n = (int)blockIdx.x / per_head, i = (int)blockIdx.x - n * per_head;
+  auto first = [&](int s) { return (int)((int64_t)starts[s] * per / 32) + s; };
+  int lo = 0, up = seqs - 1;
+  while (lo < up) {
+    const int mid = (lo + up + 1) >> 1;
+    if (first(mid) <= i) lo = mid; else up = mid - 1;
+  }
+  const Seq seq = seq_of(a.len, lo);
+  const int count = KEYS ? seq.keys : seq.rows * a.per, row = (i - first(lo)) * 32 + rr;
+  if (row - rr >= count) return;
+  const bool seen = KEYS ? row < seq.ak : true;
+  int64_t out_row;
+  if constexpr (KEYS) out_row = (int64_t)(seq.k0 + row) * a.key_heads + n;
+  else {
+    const int s = row / a.per;
+    out_row = (int64_t)(seq.r0 + s) * a.heads + n * a.per + (row - s * a.per);
+  }
+  for (int grp = wave; grp < W8; grp += 4) {
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4* p = (KEYS ? a.k_part : a.q_part) + ((int64_t)blockIdx.x * W8 + grp) * 64 + lane;
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) {
+      const uint4 v = ldg16(p + (int64_t)k * blocks * W8 * 64);
+      acc.x += __uint_as_float(v.x);
+      acc.y += __uint_as_float(v.y);
+      acc.z += __uint_as_float(v.z);
+      acc.w += __uint_as_float(v.w);
+    }
+    if (row >= count) continue;
+    const int c = grp * 8;
+    uint16_t* dst;
+    if (c < D) dst = (KEYS ? a.dk : a.dq) + out_row * D + c;
+    else if (c < D + DR) dst = (KEYS ? a.dkr : a.dqr) + out_row * DR + (c - D);
+    else dst = a.dv + out_row * D + (c - D - DR);
+    *reinterpret_cast<uint2*>(dst + kg * 4) = seen ? make_uint2(pack2<IO>(acc.x, acc.y), pack2<IO>(acc.z, acc.w)) : make_uint2(0, 0);
+  }
+}
+
+// ---------------------------------------------------------------- how a call is cut
+int64_t div_up(int64_t x, int64_t y) { return (x + y - 1) / y; }
+struct Part {   // one of the two main launches
+  int even, splits, chunk, blocks, seqs;
+  int64_t groups;
+};
+Part make_part(int64_t total, int64_t longest, int batch, bool behind, int heads, int64_t other, int forced) {
+  Part p{};
+  const int64_t seqs = batch + (behind ? 1 : 0);
+  const int64_t tiles = std::max<int64_t>(1, div_up(longest, TOK));
+  const int64_t even = tiles * seqs, through = total / TOK + seqs;
+  const bool compact = even > through + through / 2;
+  const int64_t real = (total / TOK + batch) * heads;
+  int64_t splits = forced;
+  if (splits <= 0) splits = real >= 256 ? 1 : std::max<int64_t>(1, std::min<int64_t>(512 / real, other / 512));
+  splits = std::min<int64_t>(splits, 64);
+  p.chunk = (int)(div_up(std::max<int64_t>(div_up(other, splits), 1), BN) * BN);
+  p.splits = (int)std::max<int64_t>(1, div_up(other, p.chunk));
+  p.even = compact ? 0 : (int)tiles;
+  p.seqs = (int)seqs;
+  p.groups = (compact ? through : even) * heads * p.splits;
+  p.blocks = (int)((total / 32 + seqs + 1) * heads);
+  return p;
+}
+struct Cut {
+  Part keys, queries;
+  size_t stats, norms, k_part, q_part, bytes;
+};
+size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+Cut make_cut(const DenseGradArgs& g) {
+  const DenseArgs& a = g.f;
+  const int64_t per = a.n1 / a.n2, w = 8;
+  Cut c{};
+  c.keys = make_part(a.total_keys, g.max_keys, a.batch, g.keys_behind > 0, a.n2, a.max_rows * per, a.kv_splits);
+  c.queries = make_part((int64_t)a.total_rows * per, a.max_rows * per, a.batch, a.rows_behind > 0, a.n2, a.max_kv, a.kv_splits);
+  c.stats = align256((size_t)a.total_rows * a.n1 * sizeof(float));
+  c.norms = 2 * PREP * sizeof(float);
+  if (c.keys.splits > 1) c.k_part = (size_t)c.keys.splits * c.keys.blocks * (size_t)((2 * a.d + a.dr) / w) * 64 * sizeof(float4);
+  if (c.queries.splits > 1) c.q_part = (size_t)c.queries.splits * c.queries.blocks * (size_t)((a.d + a.dr) / w) * 64 * sizeof(float4);
+  c.bytes = 2 * c.stats + c.norms + c.k_part + c.q_part;
+  return c;
+}
+
+template <int IO, int D, int DR>
+hipError_t launch_d(const GradK& k, const Cut& c, hipStream_t s) {
+  hipLaunchKernelGGL((dense_prep_kernel<IO, D>), dim3(PREP), dim3(256), 0, s, k);
+  hipLaunchKernelGGL((dense_keys_kernel<IO, D, DR>), dim3((unsigned)c.keys.groups), dim3(NWV * 64), 0, s, k);
+  if (c.keys.splits > 1)
+    hipLaunchKernelGGL((dense_join_kernel<IO, D, DR, true>), dim3((unsigned)c.keys.blocks), dim3(256), 0, s, k);
+  hipLaunchKernelGGL((dense_queries_kernel<IO, D, DR>), dim3((unsigned)c.queries.groups), dim3(NWV * 64), 0, s, k);
+  if (c.queries.splits > 1)
+    hipLaunchKernelGGL((dense_join_kernel<IO, D, DR, false>), dim3((unsigned)c.queries.blocks), dim3(256), 0, s, k);
+  return hipGetLastError();
+}
+template <int IO>
+hipError_t launch_io(const GradK& k, const Cut& c, int d, int dr, hipStream_t s) {
+  if (d == 64) return launch_d<IO, 64, 0>(k, c, s);
+  return dr ? launch_d<IO, 128, 64>(k, c, s) : launch_d<IO, 128, 0>(k, c, s);
+}
+
+}  // namespace
+}  // namespace dsa
+
+using namespace dsa;
+
+size_t dense_grad_workspace_bytes(const DenseGradArgs& a) { return make_cut(a).bytes; }
+
+hipError_t launch_dense_grad(const DenseGradArgs& g, size_t* lacking, hipStream_t s) {
+  const DenseArgs& a = g.f;
+  const Cut c = make_cut(g);
+  *lacking = !a.ws || a.ws_bytes < c.bytes || ((uintptr_t)a.ws & 15) != 0 ? c.bytes : 0;
+  if (*lacking) return hipSuccess;
+  if (c.keys.groups >= (1 << 24) || c.queries.groups >= (1 << 24)) return hipErrorInvalidConfiguration;   // 2^32 threads
+  GradK k{};
+  auto rows = [](const DenseTensor& t) { return Rows{(const uint16_t*)t.p, t.row, t.head}; };
+  k.q = rows(a.q), k.qr = rows(a.qr), k.k = rows(a.k), k.kr = rows(a.kr), k.v = rows(a.v), k.d = rows(g.d_out), k.o = rows(g.out);
+  k.len = {a.row_start, a.key_start, a.act_q, a.act_k, a.batch, a.total_rows, a.total_keys, a.sparse_mode};
+  k.heads = a.n1;
+  k.key_heads = a.n2;
+  k.per = a.n1 / a.n2;
+  while ((1 << k.per_shift) < k.per) ++k.per_shift;
+  k.per_mul = (uint32_t)(((1ull << (31 + k.per_shift)) + k.per - 1) / k.per);
+  k.q_seqs = c.queries.seqs, k.k_seqs = c.keys.seqs, k.q_even = c.queries.even, k.k_even = c.keys.even;
+  k.scale = a.scale;
+  k.stat_padded = a.stat_padded;
+  k.s1 = std::max(1, a.total_rows / a.batch);
+  k.sm_max = a.sm_max;
+  k.sm_sum = a.sm_sum;
+  char* ws = (char*)a.ws;
+  k.lse = (float*)ws;
+  k.delta = (float*)(ws + c.stats);
+  k.norms = (float*)(ws + 2 * c.stats);
+  k.k_part = (float4*)(ws + 2 * c.stats + c.norms);
+  k.q_part = (float4*)(ws + 2 * c.stats + c.norms + c.k_part);
+  k.dq = (uint16_t*)g.dq, k.dqr = (uint16_t*)g.dqr, k.dk = (uint16_t*)g.dk, k.dkr = (uint16_t*)g.dkr, k.dv = (uint16_t*)g.dv;
+  k.k_splits = c.keys.splits, k.k_chunk = c.keys.chunk, k.k_blocks = c.keys.blocks;
+  k.q_splits = c.queries.splits, k.q_chunk = c.queries.chunk, k.q_blocks = c.queries.blocks;
+  return a.io == DSA_DTYPE_BF16 ? launch_io<IO_BF16>(k, c, a.d, a.dr, s) : launch_io<IO_F16>(k, c, a.d, a.dr, s);
+}

@@ -550,3 +550,10 @@ struct DenseArgs {
 size_t dense_attn_workspace_bytes(const DenseArgs& a);
 // *lacking: 0, or (nothing is launched) the bytes of a workspace that the call needs and has not
 hipError_t launch_dense_attn(const DenseArgs& a, size_t* lacking, hipStream_t s);
+struct DenseGradArgs {
+  DenseArgs f;                  // the forward's arguments and statistics (f.out is not used; kv_splits: of both launches)
+  DenseTensor d_out, out; int keys_behind, max_keys;
+  void* dq; void* dqr; void* dk; void* dkr; void* dv;
+};
+size_t dense_grad_workspace_bytes(const DenseGradArgs& a);
+hipError_t launch_dense_grad(const DenseGradArgs& a, size_t* lacking, hipStream_t s);

@@ -106,9 +106,11 @@ class _Arguments:
         rows = [b - a for a, b in zip(self.row_start, self.row_start[1:])]
         self.rows_behind = self.total_rows - self.row_start[-1]
         self.max_rows, self.max_kv = max(rows + [self.rows_behind]), max(self.act_k, default=0)
+        keys = [b - a for a, b in zip(self.key_start, self.key_start[1:])]
+        self.keys_behind = self.total_keys - self.key_start[-1]
+        self.max_keys = max(keys + [self.keys_behind])
         self.scale, self.sparse_mode = float(scale_value), sparse_mode
         self.operands = (query, query_rope, key, key_rope, value)
-        self.dev = H.require_device(*self.operands)
 
     def place(self, lib, wait):
         """Operands and lengths on the device, with the device current"""
@@ -117,10 +119,10 @@ class _Arguments:
         self.d_row_start, self.d_key_start, self.d_act_q, self.d_act_k = H.upload(
             lib, self.dev, self.row_start, self.key_start, self.act_q, self.act_k, wait=wait)
 
-    def tensors(self):
+    def tensors(self, *more):
         """Pointers and strides as the C entries take them"""
         out = []
-        for t in (self.q, self.qr, self.k, self.kr, self.v):
+        for t in (self.q, self.qr, self.k, self.kr, self.v) + more:
             out += [None, 0, 0] if t is None else [t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0,
                                                    t.stride(1) if t.shape[1] > 1 else 0]
         return out
@@ -144,7 +146,8 @@ class DenseAttentionPlan:
                                         actual_seq_lengths_kv, scale_value, layout, sparse_mode)
         if not 0 <= int(kv_splits) <= 64:
             raise ValueError("kv_splits must lie between 0 and 64")
-        self.dev, self.return_lse = a.dev, return_softmax_lse
+        self.dev = a.dev = H.require_device(*a.operands)
+        self.return_lse = return_softmax_lse
         self.lib = _lib.load()
         self.args = None   # of the launch, but for the stream; None: nothing to do
 
@@ -191,6 +194,70 @@ def dense_attention(query, key, value, scale_value=1.0, actual_seq_lengths_query
     follow it: :func:`dense_attention_grad` is the gradient. `kv_splits` > 0 forces the number of token ranges (tuning)."""
     return DenseAttentionPlan(query, key, value, scale_value, actual_seq_lengths_query, actual_seq_lengths_kv, query_rope,
                               key_rope, layout, sparse_mode, return_softmax_lse, kv_splits, _wait=False).run()
+
+
+class DenseAttentionGradPlan:
+    """Validated arguments of one dense_attention_grad call (outputs, workspace, int32 index arrays), all in place when
+    the constructor returns; ``run()`` launches on the current stream, which may be another one. Operands are read in
+    each run, as by :class:`DenseAttentionPlan`."""
+
+    def __init__(self, query, key, value, d_out, out, softmax_max, softmax_sum, scale_value=1.0, query_rope=None, key_rope=None,
+                 actual_seq_lengths_query=None, actual_seq_lengths_kv=None, layout="BSND", sparse_mode=3, splits=0, *, _wait=True):
+        for t, what in ((d_out, "d_out"), (out, "out")):
+            if not isinstance(t, torch.Tensor) or t.shape != query.shape or t.dtype != query.dtype:
+                raise ValueError(f"{what} must have the query's shape and dtype")
+        a = self.arguments = _Arguments(query, key, value, query_rope, key_rope, actual_seq_lengths_query,
+                                        actual_seq_lengths_kv, scale_value, layout, sparse_mode)
+        for t in (softmax_max, softmax_sum):
+            if t.dtype != torch.float32 or tuple(t.shape) != a.stat_shape:
+                raise ValueError(f"softmax_max and softmax_sum must be float32 of shape {list(a.stat_shape)}")
+        if not 0 <= int(splits) <= 64:
+            raise ValueError("splits must lie between 0 and 64")
+        self.dev = a.dev = H.require_device(*a.operands, d_out, out, softmax_max, softmax_sum)
+        self.lib = _lib.load()
+        self.args = None   # of the launch, but for the stream; None: nothing to do
+
+        def place():
+            empty = not (a.batch and a.total_rows and a.total_keys)
+            new = torch.zeros if empty else torch.empty
+            self.grads = tuple(None if t is None else new(t.shape, dtype=t.dtype, device=self.dev)
+                               for t in (query, key, value, query_rope, key_rope))
+            if empty:
+                return
+            size = self.lib.dsa_dense_attn_grad_workspace_bytes(a.batch, a.total_rows, a.total_keys, a.rows_behind,
+                                                                a.keys_behind, a.n1, a.n2, a.d, a.dr, a.max_rows, a.max_keys,
+                                                                a.max_kv, int(splits))
+            self.ws = torch.empty(size, dtype=torch.uint8, device=self.dev)
+            self.d, self.o = (_packed(t, a.n1) for t in (d_out, out))
+            self.sm_max, self.sm_sum = softmax_max.contiguous(), softmax_sum.contiguous()
+            a.place(self.lib, _wait)
+            dq, dk, dv, dqr, dkr = self.grads
+            self.args = (*a.tensors(self.d, self.o), a.io, *a.lengths(), a.total_rows, a.total_keys, a.rows_behind,
+                         a.keys_behind, a.n1, a.n2, a.d, a.dr, a.max_rows, a.max_keys, a.max_kv, a.sparse_mode, a.scale, a.padded,
+                         self.sm_max.data_ptr(), self.sm_sum.data_ptr(), dq.data_ptr(), H.ptr(dqr), dk.data_ptr(), H.ptr(dkr),
+                         dv.data_ptr(), self.ws.data_ptr(), size, int(splits))
+
+        H.on_device(self.dev, place)
+
+    def run(self):
+        if self.args is not None:
+            H.on_device(self.dev, lambda: _lib.check(self.lib.dsa_dense_attn_grad(*self.args, H.stream_ptr(self.dev)),
+                                                     "dsa_dense_attn_grad"))
+        return self.grads
+
+
+def dense_attention_grad(query, key, value, d_out, out, softmax_max, softmax_sum, scale_value=1.0, query_rope=None,
+                         key_rope=None, actual_seq_lengths_query=None, actual_seq_lengths_kv=None, layout="BSND",
+                         sparse_mode=3, splits=0):
+    """Gradients of :func:`dense_attention`: ``(d_query, d_key, d_value, d_query_rope, d_key_rope)``, contiguous, in the
+    operands' shapes and dtype (None without rotary parts). d_out: the gradient of attention_out; out, softmax_max and
+    softmax_sum as the forward returned them with return_softmax_lse; the other arguments as in the forward. The gradients
+    of a key head are summed over its query heads in 32 bits; where key heads share one expanded rotary key, each has
+    its own d_key_rope, and their sum is the shared one's. Rows and keys that take no part get zeros. Results do not
+    depend on timing. `splits` > 0 forces the number of ranges that sums over rows and keys are cut into (tuning)."""
+    return DenseAttentionGradPlan(query, key, value, d_out, out, softmax_max, softmax_sum, scale_value, query_rope, key_rope,
+                                  actual_seq_lengths_query, actual_seq_lengths_kv, layout, sparse_mode, splits,
+                                  _wait=False).run()
 
 
 class DenseAttention(torch.nn.Module):

@@ -509,6 +509,33 @@ int dsa_dense_attn(const void* query, int64_t q_row, int64_t q_head, const void*
                    float scale, void* out, int stat_padded, float* sm_max, float* sm_sum, void* workspace,
                    size_t workspace_bytes, int kv_splits, void* stream);
 
+/*
+ * Gradients of dsa_dense_attn: with P = exp(score - sm_max) / sm_sum, dP = d_out . v, dS = P (dP - d_out . out),
+ *   d_query = scale dS (key | key_rope), d_key = scale dS^T (query | query_rope), d_value = P^T d_out,
+ * those of a key head summed over its query heads. query .. value, lengths, bounds and statistics as in the forward, whose
+ * out, sm_max and sm_sum are given (out and d_out [total_rows, N1, D] by strides as the operands); outputs
+ * contiguous: d_query [total_rows, N1, D], d_query_rope [.., 64], d_key and d_value [total_keys, N2, D], d_key_rope
+ * [total_keys, N2, 64] (heads that share a rotary key get one gradient each). Rows and keys that take no part get zeros.
+ * Values that are not finite reach the gradients of what sees them only.
+ *   keys_behind: total_keys - key_start[batch]; max_keys: the most of key_start[b + 1] - key_start[b] and keys_behind.
+ *   splits (<= 64): 0, or the ranges that each key's rows and each row's keys are cut into. Sums have a fixed order.
+ *   fp16: dS gets a factor, a power of two from the largest norms of d_out's and value's rows, so that neither its small
+ *   values nor its large ones leave the type's range.
+ *   workspace: dsa_dense_attn_grad_workspace_bytes, 16-byte aligned, needs no initialisation. Calls that share one must be
+ *   ordered.
+ */
+size_t dsa_dense_attn_grad_workspace_bytes(int batch, int total_rows, int total_keys, int rows_behind, int keys_behind, int n1,
+                                           int n2, int d, int dr, int max_rows, int max_keys, int max_kv, int splits);
+int dsa_dense_attn_grad(const void* query, int64_t q_row, int64_t q_head, const void* query_rope, int64_t qr_row, int64_t qr_head,
+                        const void* key, int64_t k_row, int64_t k_head, const void* key_rope, int64_t kr_row, int64_t kr_head,
+                        const void* value, int64_t v_row, int64_t v_head, const void* d_out, int64_t d_row, int64_t d_head,
+                        const void* out, int64_t o_row, int64_t o_head, int io_dtype, const int32_t* row_start,
+                        const int32_t* key_start, const int32_t* act_q, const int32_t* act_k, int batch, int total_rows,
+                        int total_keys, int rows_behind, int keys_behind, int n1, int n2, int d, int dr, int max_rows,
+                        int max_keys, int max_kv, int sparse_mode, float scale, int stat_padded, const float* sm_max,
+                        const float* sm_sum, void* d_query, void* d_query_rope, void* d_key, void* d_key_rope, void* d_value,
+                        void* workspace, size_t workspace_bytes, int splits, void* stream);
+
 #define DSA_NORM_MAX_WIDTH 16384
 
 /*

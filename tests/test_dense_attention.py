@@ -1,4 +1,4 @@
-"""Refusals of dense_attention and its C entry, without a GPU."""
+"""Refusals of dense_attention, dense_attention_grad and their C entries, without a GPU."""
 import ctypes
 
 import pytest
@@ -46,9 +46,9 @@ def test_packed_lengths_refused():
 
 
 def test_splits_refused():
-    dev = "GPU"   # (the operands' device is checked first)
-    with pytest.raises(ValueError, match=dev):
-        dsa.dense_attention(**args(), kv_splits=65)
+    for n in (65, -1):
+        with pytest.raises(ValueError, match="kv_splits"):
+            dsa.dense_attention(**args(), kv_splits=n)
 
 
 P = ctypes.c_void_p(16)   # never dereferenced: validation fails first
@@ -86,3 +86,42 @@ def test_workspace_sizes():
     assert 0 < w < 1 << 26
     assert lib.dsa_dense_attn_workspace_bytes(4, 4, 0, 32, 4, 128, 1, 8190, 1) == 0
     assert lib.dsa_dense_attn_workspace_bytes(4, 4, 0, 32, 3, 128, 1, 8190, 0) == 0
+
+
+def grad_args(**change):
+    a = args(d_out=Z(2, 3, 8, 128), out=Z(2, 3, 8, 128), softmax_max=Z(2, 4, 3, 2, dtype=torch.float32),
+             softmax_sum=Z(2, 4, 3, 2, dtype=torch.float32))
+    a.update(change)
+    return a
+
+
+GRAD_REFUSED = REFUSED[1:3] + REFUSED[4:] + [
+    (dict(d_out=Z(2, 3, 8, 64)), "d_out must"), (dict(out=Z(2, 3, 8, 128, dtype=torch.half)), "out must"), (dict(d_out=None), "d_out must"),
+    (dict(softmax_max=Z(2, 4, 3, 2)), "softmax_max"), (dict(softmax_sum=Z(2, 1, 3, 8, dtype=torch.float32)), "softmax_max and"),
+    (dict(splits=65), "splits"), (dict(splits=-1), "splits")]
+
+
+@pytest.mark.parametrize("change,message", GRAD_REFUSED)
+def test_gradient_refuses(change, message):
+    a = grad_args(**change)
+    if "query" in change:   # the gradient's operands have the query's shape
+        a.update(d_out=a["query"], out=a["query"])
+    with pytest.raises(ValueError, match=message):
+        dsa.dense_attention_grad(**a)
+
+
+GRAD_BASE = T * 7 + [1, P, P, P, P, 2, 6, 10, 0, 0, 8, 4, 128, 64, 3, 5, 5, 3, 0.1, 1, P, P, P, P, P, P, P, P, 1 << 40, 0, None]
+
+
+def test_c_gradient_entry_refuses():
+    lib = _lib.load()
+    odd = ctypes.c_void_p(24)
+    for changes, st, what in ([([(i, None)], -1, "null") for i in (0, 3, 6, 9, 12, 15, 18, 22, 23, 24, 25, 41, 42, 43, 44, 45, 46, 47)] + [
+            ([(21, 2)], -1, "io_dtype"), ([(38, 1)], -1, "sparse_mode"), ([(33, 96)], -1, "D must"), ([(34, 32)], -1, "rope dim"),
+            ([(26, 0)], -1, "shape"), ([(32, 3)], -1, "divisible"), ([(30, 11)], -1, "past"), ([(36, 11)], -1, "past"),
+            ([(30, -1)], -1, "past"), ([(15, odd)], -1, "16-byte"), ([(19, 4)], -1, "16-byte"), ([(16, 1 << 24)], -2, "strides"),
+            ([(43, odd)], -1, "aligned"), ([(50, 65)], -2, "splits"), ([(48, None)], -1, "workspace"), ([(49, 16)], -1, "workspace")]):
+        assert call(lib.dsa_dense_attn_grad, GRAD_BASE, changes) == st, what
+        assert what in lib.dsa_last_error().decode(), (what, lib.dsa_last_error())
+    none = [(27, 0), (28, 0), (35, 0), (36, 0), (37, 0), (26, 1)]
+    assert call(lib.dsa_dense_attn_grad, GRAD_BASE, none) == 0   # nothing: no launch
