@@ -18,7 +18,7 @@ namespace {
 
 constexpr int NWV = 4;
 constexpr int BN = 64;     // tokens a tile
-constexpr int NBUF = 2;
+constexpr int NBUF = 3;
 
 // P = e^(score - reference). The reference moves, and the output is rescaled, only when a tile's P would exceed
 // e^LIMIT, which is finite in the io type (bf16 has fp32's exponents; fp16 ends at e^11.09); it moves to GAP below
@@ -132,14 +132,14 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
     qp[m] = a.q.p + (seq.r0 + s) * a.q.row + (n * a.per + g) * a.q.head;
     if constexpr (DR > 0) qrp[m] = a.qr.p + (seq.r0 + s) * a.qr.row + (n * a.per + g) * a.qr.head;
   }
-  const int w_base = r_base + wave * RT * 32, w_hi = seen(w_base, min(r_end, w_base + RT * 32));
 
   f32x16 o[RT][ON];
-  float m_used[RT], m_true[RT], l_part[RT];
+  float m_used[RT], m_true[RT], l_part[RT], alpha[RT];
 #pragma unroll
   for (int m = 0; m < RT; ++m) {
     m_used[m] = m_true[m] = -INFINITY;
     l_part[m] = 0.f;
+    alpha[m] = 1.f;
 #pragma unroll
     for (int c = 0; c < ON; ++c)
 #pragma unroll
@@ -153,116 +153,292 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
     const float cpos = a.scale == 0.f ? 1e-30f : fabsf(a.scale);
     const float cl2 = cpos * LOG2E;
 
+    // ---- tiles: each wave loads a share, in GPW loads
     const Share<RB, BN, NWV> sh(wave, lane);
-    const Share<DR ? DR * 2 : 128, BN, NWV> shr(wave, lane);
-    const uint16_t* const kb = a.k.p + (int64_t)seq.k0 * a.k.row + n * a.k.head;
-    const uint16_t* const vb = a.v.p + (int64_t)seq.k0 * a.v.row + n * a.v.head;
-    const uint16_t* const krb = DR ? a.kr.p + (int64_t)seq.k0 * a.kr.row + n * a.kr.head : nullptr;
+    using ShR = Share<DR ? DR * 2 : 128, BN, NWV>;
+    const ShR shr(wave, lane);
+    constexpr int CK = sh.CNT, CR = DR ? ShR::CNT : 0, GPW = 2 * CK + CR;
     const uint32_t k_row = (uint32_t)a.k.row * 2, v_row = (uint32_t)a.v.row * 2, kr_row = (uint32_t)a.kr.row * 2;
-    // (rows past the last token repeat it; they are masked)
-    auto load_rows = [&](auto share, const uint16_t* base, uint32_t row_bytes, int t0, uint8_t* dst) __attribute__((always_inline)) {
-      const char* p = reinterpret_cast<const char*>(base) + (int64_t)t0 * row_bytes;
-#pragma unroll
-      for (int j = 0; j < share.CNT; ++j) {
-        const int t = min(j * share.STEP + share.row, seq.ak - 1 - t0);
-        lds_dma16_sbase_untracked(p, (uint32_t)t * row_bytes + share.col, dst + (j * NWV + wave) * 1024);
+    const char* const kb = reinterpret_cast<const char*>(a.k.p + (int64_t)seq.k0 * a.k.row + n * a.k.head);
+    const char* const vb = reinterpret_cast<const char*>(a.v.p + (int64_t)seq.k0 * a.v.row + n * a.v.head);
+    const char* const krb = DR ? reinterpret_cast<const char*>(a.kr.p + (int64_t)seq.k0 * a.kr.row + n * a.kr.head) : nullptr;
+    const uint32_t k_off = sh.row * k_row + sh.col, v_off = sh.row * v_row + sh.col, kr_off = shr.row * kr_row + shr.col;
+    // load j of tile u (rows past the last token repeat it; they are masked)
+    auto load_part = [&](auto jc, int u, int buf, bool whole) __attribute__((always_inline)) {
+      constexpr int j = decltype(jc)::value;
+      constexpr int what = j < CK ? 0 : j < 2 * CK ? 1 : 2, i = what == 0 ? j : what == 1 ? j - CK : j - 2 * CK;
+      constexpr int step = i * (what == 2 ? ShR::STEP : sh.STEP);
+      const int t0 = t_lo + u * BN;
+      const uint32_t row = what == 0 ? k_row : what == 1 ? v_row : kr_row;
+      const char* p = (what == 0 ? kb : what == 1 ? vb : krb) + (int64_t)t0 * row;
+      uint8_t* dst = (what == 0 ? L.k[buf] : what == 1 ? L.v[buf] : L.kr[buf]) + (i * NWV + wave) * 1024;
+      if (whole) {
+        lds_dma16_sbase_untracked(p + step * (int64_t)row, what == 0 ? k_off : what == 1 ? v_off : kr_off, dst);
+      } else {
+        const int t = min(step + (what == 2 ? shr.row : sh.row), seq.ak - 1 - t0);
+        lds_dma16_sbase_untracked(p, (uint32_t)t * row + (what == 2 ? shr.col : sh.col), dst);
       }
     };
-    auto load_tile = [&](int u) __attribute__((always_inline)) {
-      const int t0 = t_lo + u * BN, buf = u % NBUF;
-      load_rows(sh, kb, k_row, t0, L.k[buf]);
-      load_rows(sh, vb, v_row, t0, L.v[buf]);
-      if constexpr (DR > 0) load_rows(shr, krb, kr_row, t0, L.kr[buf]);
+    auto load_tile = [&](int u, int buf) __attribute__((always_inline)) {
+      static_for<0, GPW>([&](auto j) __attribute__((always_inline)) { load_part(j, u, buf, false); });
     };
-    load_tile(0);
+    // A tile that some rows see only in part: a masked token has P = 0, but 0 times a value that is not finite would
+    // still reach the rows that do not see it. Such values become 0 in LDS, and the token's score NaN for the
+    // rows that do see it.
+    auto is_mixed = [&](int u) { return t_lo + u * BN + BN > min_lim; };
+    auto sanitize = [&](int u, int buf) __attribute__((always_inline)) {
+      if (!is_mixed(u)) return;
+      const uint64_t bad = clean_share<IO, RB, BN, NWV>(lds_addr(L.v[buf]), wave, lane);
+      if (lane == 0) L.bad[buf][wave] = bad;
+    };
+    load_tile(0, 0);
     uint4 qf[RT][KS];
 #pragma unroll
     for (int m = 0; m < RT; ++m)
 #pragma unroll
       for (int j = 0; j < KS; ++j)
         qf[m][j] = flipped(j < KSN ? ldg16(qp[m] + j * 16 + kg * 8) : ldg16(qrp[m] + (j - KSN) * 16 + kg * 8), flip);
+#pragma unroll
+    for (int m = 0; m < RT; ++m)
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        i32x4v v = __builtin_bit_cast(i32x4v, qf[m][j]);
+        asm volatile("" : "+a"(v));
+        qf[m][j] = __builtin_bit_cast(uint4, v);
+      }
 
-    const int tk = s_row(rr);
-    for (int u = 0; u < ntiles; ++u) {
-      const int t0 = t_lo + u * BN, buf = u % NBUF;
-      // A tile that some rows see only in part: a masked token has P = 0, but 0 times a value that is not finite would
-      // still reach the rows that do not see it. Such values become 0 in LDS, and the token's score NaN for the
-      // rows that do see it.
-      const bool mixed = t0 + BN > min_lim;
+    // ---- operand addresses of this lane in a buffer; those of the other fragments differ by an exclusive or of
+    // constants in the chunk bits, kept in registers and moved to another buffer once a tile
+    const int tk = s_row(rr), g16 = lane >> 4, c16 = lane & 15;
+    const int t4 = (g16 >> 1) * 8 + (c16 >> 2), vc = (g16 & 1) * 2 + ((c16 & 3) >> 1);
+    const uint32_t k_lane = tile_off<RB>(tk, kg), r_lane = tile_off<128>(tk, kg);
+    const uint32_t v_lo = tile_off<RB>(t4, vc) + (c16 & 1) * 8, v_hi = tile_off<RB>(t4 + 4, vc) + (c16 & 1) * 8;
+    uint32_t ka[KSN], ra[DR ? KS - KSN : 1], va[ON], vh[ON];
+    auto point_k = [&](int buf) __attribute__((always_inline)) {
+      const uint32_t kt = lds_addr(L.k[buf]), rt = lds_addr(L.kr[buf]);
+#pragma unroll
+      for (int j = 0; j < KSN; ++j) {
+        ka[j] = kt + (k_lane ^ (j << 5));
+        asm volatile("" : "+v"(ka[j]));
+      }
+      if constexpr (DR > 0)
+#pragma unroll
+        for (int j = 0; j < KS - KSN; ++j) {
+          ra[j] = rt + (r_lane ^ (j << 5));
+          asm volatile("" : "+v"(ra[j]));
+        }
+    };
+    auto point_v = [&](int buf) __attribute__((always_inline)) {
+      const uint32_t vt = lds_addr(L.v[buf]);
+#pragma unroll
+      for (int c = 0; c < ON; ++c) {
+        va[c] = vt + (v_lo ^ (c << 6));
+        vh[c] = vt + (v_hi ^ (c << 6));
+        asm volatile("" : "+v"(va[c]), "+v"(vh[c]));
+      }
+    };
+    auto k_frag = [&](int j, int h) __attribute__((always_inline)) -> uint4 {
+      return lds_read16_at(j < KSN ? ka[j < KSN ? j : 0] + h * 32 * RB : ra[j >= KSN ? j - KSN : 0] + h * 32 * 128);
+    };
+    // column tile i % ON of the 16 tokens i / ON of half h
+    auto v_frag = [&](int i, int h) __attribute__((always_inline)) -> uint4 {
+      const int off = (h * 32 + (i / ON) * 16) * RB;
+      const uint2 lo = ds_read_tr_at(va[i % ON] + off), hi2 = ds_read_tr_at(vh[i % ON] + off);
+      return make_uint4(lo.x, lo.y, hi2.x, hi2.y);
+    };
+
+    // ---- online softmax of 32 tokens in NST stages of a few VALU operations, placed among the MFMAs of the products
+    // before and after it. Raw scores; max(c s) = c max(s) as c > 0. The reference m_used moves only past the
+    // lazy threshold, so the output's factor alpha is nearly always 1.
+    constexpr int NST = 13;
+    float sm_mx[RT], sm_mb[RT], sm_sum[RT], sm_p[RT];
+    auto stage = [&](int st, int m, f32x16& sv, uint4 (&pn)[2]) __attribute__((always_inline)) {
+      if (st < 2) {
+        float mx = st == 0 ? max3(sv[0], sv[1], sv[2]) : max3(sm_mx[m], sv[9], sv[10]);
+        mx = st == 0 ? max3(mx, sv[3], sv[4]) : max3(mx, sv[11], sv[12]);
+        mx = st == 0 ? max3(mx, sv[5], sv[6]) : max3(mx, sv[13], sv[14]);
+        sm_mx[m] = st == 0 ? max3(mx, sv[7], sv[8]) : max3(mx, sv[15], sv[15]);
+      } else if (st == 2) {
+        sm_mx[m] = max_half_swap(sm_mx[m]) * cpos;
+        m_true[m] = max3(m_true[m], sm_mx[m], sm_mx[m]);
+      } else if (st == 3) {
+        const float m_new = sm_mx[m] > m_used[m] + lazy_limit<IO>() ? sm_mx[m] - lazy_gap<IO>() : m_used[m];
+        alpha[m] = m_used[m] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_used[m] - m_new) * LOG2E);
+        m_used[m] = m_new;
+        sm_mb[m] = m_new == -INFINITY ? 0.f : m_new * LOG2E;
+        sm_sum[m] = 0.f;
+      } else if (st < 12) {
+        const int i = st - 4;
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[2 * i], cl2, -sm_mb[m]));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[2 * i + 1], cl2, -sm_mb[m]));
+        sm_sum[m] += p0;
+        sm_sum[m] += p1;
+        uint32_t w = pack2<IO>(p0, p1);
+        asm volatile("" : "+v"(w));   // here, not where the next step needs it
+        uint4& q = pn[i >> 2];
+        if ((i & 3) == 0) q.x = w;
+        else if ((i & 3) == 1) q.y = w;
+        else if ((i & 3) == 2) q.z = w;
+        else q.w = w;
+      } else {
+        l_part[m] = l_part[m] * alpha[m] + sm_sum[m];
+      }
+    };
+    auto mask = [&](int u, int buf, int h, f32x16 (&sv)[RT]) __attribute__((always_inline)) {
+      if (!is_mixed(u)) return;
+      const int t0 = t_lo + u * BN + h * 32;
+      const uint64_t all = L.bad[buf][0] | L.bad[buf][1] | L.bad[buf][2] | L.bad[buf][3];
+      const uint32_t bad = (uint32_t)(all >> (h * 32));
+#pragma unroll
+      for (int m = 0; m < RT; ++m) {
+        if (__builtin_amdgcn_readfirstlane(bad))
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if ((bad >> s_token(i, kg)) & 1u) sv[m][i] = __builtin_nanf("");
+        const int l = dead[m] ? INT_MAX : lim[m] - t0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sv[m][i] = s_token(i, kg) < l ? sv[m][i] : -INFINITY;
+      }
+    };
+    auto rescale = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int m = 0; m < RT; ++m)
+        if (__builtin_amdgcn_ballot_w64(alpha[m] != 1.f)) {
+#pragma unroll
+          for (int c = 0; c < ON; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[m][c][i] = agpr_scale(o[m][c][i], alpha[m]);
+        }
+#pragma unroll
+      for (int m = 0; m < RT; ++m)
+#pragma unroll
+        for (int c = 0; c < ON; ++c) asm volatile("" : "+a"(o[m][c]));   // whole accumulators, in AGPRs, across the branch
+    };
+
+    // ---- One step handles the 32 tokens i = (tile u, half h): O += V P of the tokens before them, then S of the tokens
+    // after them, each MFMA followed by a stage of this one's softmax. Fragments are read a few MFMAs ahead, past the
+    // end of one product for the next.
+    constexpr int NPV = 2 * ON, NM = (NPV + KS) * RT;
+    constexpr int VR = NPV < 4 ? NPV : 4, KR = KS < 4 ? KS : 4;
+    uint4 vfr[VR], kfr[KR];
+    auto step = [&](auto pvc, auto sc, auto hc, f32x16 (&cur)[RT], f32x16 (&next)[RT], uint4 (&pb)[RT][2], uint4 (&pn)[RT][2],
+                    auto&& between, auto&& ride) __attribute__((always_inline)) {
+      constexpr bool PV = decltype(pvc)::value, S = decltype(sc)::value;
+      constexpr int H = decltype(hc)::value;   // half of the product's tokens: V's and the next S's are the same
+      constexpr int M0 = PV ? NPV * RT : 0, NMM = M0 + (S ? KS * RT : 0);
+      constexpr int LEAD = NMM > 8 ? 2 : 0;   // (the scores' last products are on their way)
+      auto softmax_at = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int st = 0; st < NST; ++st)
+#pragma unroll
+          for (int m = 0; m < RT; ++m)
+            if (LEAD + (st * RT + m) * (NMM - LEAD) / (NST * RT) == slot) stage(st, m, cur[m], pn[m]);
+      };
+      if constexpr (NMM == 0) {
+#pragma unroll
+        for (int st = 0; st < NST; ++st)
+#pragma unroll
+          for (int m = 0; m < RT; ++m) stage(st, m, cur[m], pn[m]);
+      }
+      if constexpr (PV)
+        static_for<0, M0>([&](auto jc) __attribute__((always_inline)) {
+          constexpr int j = decltype(jc)::value, i = j / RT, m = j % RT;
+          o[m][i % ON] = Mfma<IO>::m32(vfr[i % VR], pb[m][i / ON], o[m][i % ON]);
+          if constexpr (m == RT - 1 && i + VR < NPV) vfr[i % VR] = v_frag(i + VR, H);
+          if constexpr (S && m == 0 && i < KR) kfr[i] = k_frag(i, H);
+          softmax_at(j);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      between();
+      if constexpr (S)
+        static_for<0, KS * RT>([&](auto jc) __attribute__((always_inline)) {
+          constexpr int j = decltype(jc)::value, i = j / RT, m = j % RT;
+          if constexpr (i < KS - 1) mfma32_va<IO, i == 0>(next[m], kfr[i % KR], qf[m][i]);
+          else if constexpr (m == RT - 1 && RT == 2) mfma32_va_last2<IO>(next[0], next[1], kfr[i % KR], qf[0][i], qf[1][i]);
+          else if constexpr (RT == 1) mfma32_va_last<IO>(next[0], kfr[i % KR], qf[0][i]);
+          if constexpr (m == RT - 1 && i + KR < KS) kfr[i % KR] = k_frag(i + KR, H);
+          if constexpr (m == 0 && i >= KS - VR) vfr[i - (KS - VR)] = v_frag(i - (KS - VR), 1 - H);
+          ride(jc);
+          softmax_at(M0 + j);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    auto first_k = [&](int h) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < KR; ++i) kfr[i] = k_frag(i, h);
+    };
+    std::true_type yes;
+    std::false_type no;
+    std::integral_constant<int, 0> h0;
+    std::integral_constant<int, 1> h1;
+    auto nothing = [](auto...) __attribute__((always_inline)) {};
+
+    wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    sanitize(0, 0);
+    lds_barrier();
+    if (ntiles > 1) load_tile(1, 1);
+    f32x16 s0[RT], s1[RT];
+    uint4 p0[RT][2], p1[RT][2];
+    point_k(0);
+    first_k(0);
+    static_for<0, KS>([&](auto ic) __attribute__((always_inline)) {
+      constexpr int i = decltype(ic)::value;
+      if constexpr (i < KS - 1)
+#pragma unroll
+        for (int m = 0; m < RT; ++m) mfma32_va<IO, i == 0>(s0[m], kfr[i % KR], qf[m][i]);
+      else if constexpr (RT == 2) mfma32_va_last2<IO>(s0[0], s0[1], kfr[i % KR], qf[0][i], qf[1][i]);
+      else mfma32_va_last<IO>(s0[0], kfr[i % KR], qf[0][i]);
+      if constexpr (i + KR < KS) kfr[i % KR] = k_frag(i + KR, 0);
+    });
+    first_k(1);
+    int buf = 0;   // of tile u
+    // Step (u, 0): tile u + 1 has landed by the middle of it, when nobody needs tile u - 1 any more
+    auto middle = [&](int u) __attribute__((always_inline)) {
+      const int nb = buf == NBUF - 1 ? 0 : buf + 1;
       wait_vmcnt<0>();
       asm volatile("" ::: "memory");
-      if (mixed) {
-        const uint64_t bad = clean_share<IO, RB, BN, NWV>(lds_addr(L.v[buf]), wave, lane);
-        if (lane == 0) L.bad[buf][wave] = bad;
-      }
-      lds_barrier();   // tile u is here, tile u - 1 done with
-      if (u + 1 < ntiles) load_tile(u + 1);
-      if (t0 >= w_hi) continue;
-      uint64_t bad = 0;
-      if (mixed) bad = L.bad[buf][0] | L.bad[buf][1] | L.bad[buf][2] | L.bad[buf][3];
-      const uint32_t kt = lds_addr(L.k[buf]), vt = lds_addr(L.v[buf]), krt = lds_addr(L.kr[buf]);
+      if (u + 1 < ntiles) sanitize(u + 1, nb);
+      lds_barrier();
+    };
+    auto half0 = [&](auto pvc, int u) __attribute__((always_inline)) {
+      mask(u, buf, 0, s0);
+      const int lb = buf == 0 ? NBUF - 1 : buf - 1;   // tile u - 1's, for tile u + 2
+      const bool more = u + 2 < ntiles, whole = t_lo + (u + 3) * BN <= seq.ak;
+      step(pvc, yes, h1, s0, s1, p1, p0, [&]() __attribute__((always_inline)) {
+             middle(u);
+             point_v(buf);
+           },
+           [&](auto jc) __attribute__((always_inline)) {
+             constexpr int j = decltype(jc)::value;
+             static_for<0, GPW>([&](auto g) __attribute__((always_inline)) {
+               if constexpr (g * (KS * RT) / GPW == j)
+                 if (more) load_part(g, u + 2, lb, whole);
+             });
+           });
+      rescale();
+    };
+    half0(no, 0);
+    for (int uv = 0; uv + 1 < ntiles; ++uv) {
+      const int u = __builtin_amdgcn_readfirstlane(uv);
+      const int nb = buf == NBUF - 1 ? 0 : buf + 1;
+      point_k(nb);
+      mask(u, buf, 1, s1);
+      step(yes, yes, h0, s1, s0, p0, p1, nothing, nothing);
+      rescale();
+      buf = nb;
+      half0(yes, u + 1);
+    }
+    mask(ntiles - 1, buf, 1, s1);
+    step(yes, no, h0, s1, s0, p0, p1, nothing, nothing);
+    rescale();
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        f32x16 sv[RT];
+    for (int i = 0; i < VR; ++i) vfr[i] = v_frag(i, 1);
 #pragma unroll
-        for (int m = 0; m < RT; ++m)
+    for (int i = 0; i < NPV; ++i) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sv[m][i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < KS; ++j) {
-          const uint4 af = j < KSN ? op_frag<RB>(kt, h * 32 + tk, j, kg) : op_frag<128>(krt, h * 32 + tk, j - KSN, kg);
-#pragma unroll
-          for (int m = 0; m < RT; ++m) sv[m] = Mfma<IO>::m32(af, qf[m][j], sv[m]);
-        }
-        uint4 pb[RT][2];
-#pragma unroll
-        for (int m = 0; m < RT; ++m) {
-          if (bad)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if ((bad >> (h * 32 + s_token(i, kg))) & 1u) sv[m][i] = __builtin_nanf("");
-          if (t0 + h * 32 + 32 > min_lim)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              sv[m][i] = t0 + h * 32 + s_token(i, kg) < lim[m] || dead[m] ? sv[m][i] : -INFINITY;
-          float mx = max3(sv[m][0], sv[m][1], sv[m][2]);
-#pragma unroll
-          for (int i = 3; i < 15; i += 2) mx = max3(mx, sv[m][i], sv[m][i + 1]);
-          mx = max_half_swap(max3(mx, sv[m][15], sv[m][15])) * cpos;
-          m_true[m] = max3(m_true[m], mx, mx);
-          const float m_new = mx > m_used[m] + lazy_limit<IO>() ? mx - lazy_gap<IO>() : m_used[m];
-          const float alpha = m_used[m] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_used[m] - m_new) * LOG2E);
-          m_used[m] = m_new;
-          const float mb = m_new == -INFINITY ? 0.f : m_new * LOG2E;
-          uint32_t d[8];
-          float sum = 0.f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[m][2 * i], cl2, -mb));
-            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[m][2 * i + 1], cl2, -mb));
-            sum += p0;
-            sum += p1;
-            d[i] = pack2<IO>(p0, p1);
-          }
-          l_part[m] = l_part[m] * alpha + sum;
-          pb[m][0] = make_uint4(d[0], d[1], d[2], d[3]);
-          pb[m][1] = make_uint4(d[4], d[5], d[6], d[7]);
-          if (__builtin_amdgcn_ballot_w64(alpha != 1.f)) {
-#pragma unroll
-            for (int c = 0; c < ON; ++c)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[m][c][i] *= alpha;
-          }
-        }
-#pragma unroll
-        for (int st = 0; st < 2; ++st)
-#pragma unroll
-          for (int c = 0; c < ON; ++c) {
-            const uint4 vf = tr_frag<RB>(vt, h * 32 + st * 16, c, lane);
-#pragma unroll
-            for (int m = 0; m < RT; ++m) o[m][c] = Mfma<IO>::m32(vf, pb[m][st], o[m][c]);
-          }
-      }
+      for (int m = 0; m < RT; ++m) o[m][i % ON] = Mfma<IO>::m32(vfr[i % VR], p1[m][i / ON], o[m][i % ON]);
+      if (i + VR < NPV) vfr[i % VR] = v_frag(i + VR, 1);
     }
   }
 

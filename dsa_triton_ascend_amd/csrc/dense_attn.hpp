@@ -128,6 +128,45 @@ __device__ __forceinline__ uint64_t clean_share(uint32_t tile, int wave, int lan
   return bad;
 }
 
+// 32x32x16 chains whose accumulators stay in VGPRs (their results go to the VALU) and whose second operand, loaded
+// once, lies in AGPRs. The compiler does not see these as MFMAs: the last ones of a chain end with the wait states that a
+// VALU read of their results needs (8 passes: 12; 16 are waited), in the same statement, as the compiler may copy an
+// accumulator between two of them.
+template <int IO, bool FIRST>
+__device__ __forceinline__ void mfma32_va(f32x16& c, uint4 a, uint4 b) {
+  const i32x4v av = __builtin_bit_cast(i32x4v, a), bv = __builtin_bit_cast(i32x4v, b);
+  if constexpr (IO == IO_BF16 && FIRST) asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(av), "a"(bv));
+  else if constexpr (IO == IO_BF16) asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(av), "a"(bv));
+  else if constexpr (FIRST) asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(c) : "v"(av), "a"(bv));
+  else asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(c) : "v"(av), "a"(bv));
+}
+template <int IO>
+__device__ __forceinline__ void mfma32_va_last(f32x16& c, uint4 a, uint4 b) {
+  const i32x4v av = __builtin_bit_cast(i32x4v, a), bv = __builtin_bit_cast(i32x4v, b);
+  if constexpr (IO == IO_BF16) asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0\n\ts_nop 15" : "+v"(c) : "v"(av), "a"(bv));
+  else asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0\n\ts_nop 15" : "+v"(c) : "v"(av), "a"(bv));
+}
+// the last step of two chains with the same first operand
+template <int IO>
+__device__ __forceinline__ void mfma32_va_last2(f32x16& c0, f32x16& c1, uint4 a, uint4 b0, uint4 b1) {
+  const i32x4v av = __builtin_bit_cast(i32x4v, a), v0 = __builtin_bit_cast(i32x4v, b0), v1 = __builtin_bit_cast(i32x4v, b1);
+  if constexpr (IO == IO_BF16)
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %2, %3, %0\n\tv_mfma_f32_32x32x16_bf16 %1, %2, %4, %1\n\ts_nop 15"
+                 : "+v"(c0), "+v"(c1) : "v"(av), "a"(v0), "a"(v1));
+  else
+    asm volatile("v_mfma_f32_32x32x16_f16 %0, %2, %3, %0\n\tv_mfma_f32_32x32x16_f16 %1, %2, %4, %1\n\ts_nop 15"
+                 : "+v"(c0), "+v"(c1) : "v"(av), "a"(v0), "a"(v1));
+}
+
+// o *= f on an accumulator element in an AGPR, which the VALU cannot use directly
+__device__ __forceinline__ float agpr_scale(float o, float f) {
+  float t;
+  asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %1, %2\n\tv_accvgpr_write_b32 %0, %1"
+               : "+a"(o), "=&v"(t)
+               : "v"(f));
+  return o;
+}
+
 __device__ __forceinline__ uint4 flipped(uint4 v, uint32_t f) { return make_uint4(v.x ^ f, v.y ^ f, v.z ^ f, v.w ^ f); }
 
 // v_max3 without the quieting of each operand that fmaxf needs (a NaN score reaches the output
