@@ -566,10 +566,10 @@ Cut make_cut(const DenseArgs& a) {
   Cut c{};
   // 256 rows a work-group where that leaves two rounds of the CUs, else 128
   auto tiles = [&](int rows) { return div_up((int64_t)a.max_rows * per, rows); };
-  c.rt = (int64_t)a.total_rows * per / 256 * a.n2 >= 512 ? 2 : 1;
+  c.rt = (int64_t)a.total_rows * per * a.n2 / 256 >= 160 ? 2 : 1;
   const int rows = 128 * c.rt;
   const int64_t even = std::max<int64_t>(1, tiles(rows)) * seqs, through = (int64_t)a.total_rows * per / rows + seqs;
-  const bool compact = even > through + through / 2;
+  const bool compact = even > 4 * through;
   const int64_t items = (compact ? through : even) * a.n2;
   const int64_t real = ((int64_t)a.total_rows * per / rows + a.batch) * a.n2;   // about so many have rows
   int splits = a.kv_splits;

@@ -621,7 +621,7 @@ Part make_part(int64_t total, int64_t longest, int batch, bool behind, int heads
   const int64_t seqs = batch + (behind ? 1 : 0);
   const int64_t tiles = std::max<int64_t>(1, div_up(longest, TOK));
   const int64_t even = tiles * seqs, through = total / TOK + seqs;
-  const bool compact = even > through + through / 2;
+  const bool compact = even > 4 * through;
   const int64_t real = (total / TOK + batch) * heads;
   int64_t splits = forced;
   if (splits <= 0) splits = real >= 256 ? 1 : std::max<int64_t>(1, std::min<int64_t>(512 / real, other / 512));
