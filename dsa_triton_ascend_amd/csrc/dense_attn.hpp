@@ -158,6 +158,55 @@ __device__ __forceinline__ void mfma32_va_last2(f32x16& c0, f32x16& c1, uint4 a,
                  : "+v"(c0), "+v"(c1) : "v"(av), "a"(v0), "a"(v1));
 }
 
+// the last steps of two chains
+template <int IO>
+__device__ __forceinline__ void mfma32_va_end2(f32x16& c0, uint4 a0, uint4 b0, f32x16& c1, uint4 a1, uint4 b1) {
+  const i32x4v p0 = __builtin_bit_cast(i32x4v, a0), p1 = __builtin_bit_cast(i32x4v, a1);
+  const i32x4v v0 = __builtin_bit_cast(i32x4v, b0), v1 = __builtin_bit_cast(i32x4v, b1);
+  if constexpr (IO == IO_BF16)
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %2, %4, %0\n\tv_mfma_f32_32x32x16_bf16 %1, %3, %5, %1\n\ts_nop 15"
+                 : "+v"(c0), "+v"(c1) : "v"(p0), "v"(p1), "a"(v0), "a"(v1));
+  else
+    asm volatile("v_mfma_f32_32x32x16_f16 %0, %2, %4, %0\n\tv_mfma_f32_32x32x16_f16 %1, %3, %5, %1\n\ts_nop 15"
+                 : "+v"(c0), "+v"(c1) : "v"(p0), "v"(p1), "a"(v0), "a"(v1));
+}
+// v in AGPRs from here on
+__device__ __forceinline__ uint4 in_agprs(uint4 u) {
+  i32x4v v = __builtin_bit_cast(i32x4v, u);
+  asm volatile("" : "+a"(v));
+  return __builtin_bit_cast(uint4, v);
+}
+
+// Addresses of a lane's operand fragments in a tile: those of one row (tk) or of one group of rows (transposed) differ by
+// an exclusive or of constants in the chunk bits. Kept in registers and moved to another buffer once a tile, so that
+// halves of a tile and other arrays of the same layout are constant offsets.
+template <int RB> struct OpAddr {
+  uint32_t a[RB / 32];
+  __device__ __forceinline__ void point(uint32_t tile, uint32_t lane) {
+#pragma unroll
+    for (int j = 0; j < RB / 32; ++j) {
+      a[j] = tile + (lane ^ (j << 5));
+      asm volatile("" : "+v"(a[j]));
+    }
+  }
+};
+template <int RB> struct TrAddr {
+  uint32_t lo[RB / 64], hi[RB / 64];
+  __device__ __forceinline__ void point(uint32_t tile, uint32_t lane_lo, uint32_t lane_hi) {
+#pragma unroll
+    for (int c = 0; c < RB / 64; ++c) {
+      lo[c] = tile + (lane_lo ^ (c << 6));
+      hi[c] = tile + (lane_hi ^ (c << 6));
+      asm volatile("" : "+v"(lo[c]), "+v"(hi[c]));
+    }
+  }
+  // column tile c of the 16 rows at byte offset off
+  __device__ __forceinline__ uint4 frag(int c, int off) const {
+    const uint2 l = ds_read_tr_at(lo[c] + off), h = ds_read_tr_at(hi[c] + off);
+    return make_uint4(l.x, l.y, h.x, h.y);
+  }
+};
+
 // o *= f on an accumulator element in an AGPR, which the VALU cannot use directly
 __device__ __forceinline__ float agpr_scale(float o, float f) {
   float t;

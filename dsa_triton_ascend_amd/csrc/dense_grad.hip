@@ -23,7 +23,7 @@ namespace {
 
 constexpr int NWV = 4;
 constexpr int BN = 64;     // rows of a tile in LDS
-constexpr int NBUF = 2;
+constexpr int NBUF = 3;
 constexpr int TOK = NWV * 32;     // tokens, or head rows, of a work-group
 constexpr int PREP = 512;         // work-groups of the first launch
 
@@ -37,6 +37,7 @@ struct GradK {
   int heads, key_heads, per;
   uint32_t per_mul;        // r / per for r < 2^31: see rows_of
   int per_shift;
+  int linear;              // the heads of a group divide 16: see the loads of the keys' kernel
   int q_seqs, k_seqs;      // sequences, with what lies behind the last
   int q_even, k_even;      // tiles of the longest, 0: numbered through
   float scale;
@@ -195,8 +196,10 @@ __device__ __forceinline__ Place place_of(int i, int seqs, int heads, int splits
 
 // ---------------------------------------------------------------- keys
 template <int D, int DR> struct KeyLds {
-  uint8_t q[NBUF][BN * D * 2];
-  uint8_t d[NBUF][BN * D * 2];
+  struct {
+    uint8_t q[BN * D * 2];   // (d lies at a constant offset from q)
+    uint8_t d[BN * D * 2];
+  } t[NBUF];
   uint8_t qr[NBUF][DR ? BN * DR * 2 : 16];
   float lse[NBUF][BN];
   float delta[NBUF][BN];
@@ -231,7 +234,6 @@ __global__ __launch_bounds__(NWV * 64) void dense_keys_kernel(GradK a) {
   const int r_lo = max(first_query(a.len, seq, t0) * a.per, at.sp * a.k_chunk);
   const int r_hi = at.sp == a.k_splits - 1 ? r_end : min(r_end, (at.sp + 1) * a.k_chunk);
   const int r_full = t_seen > t0 ? first_query(a.len, seq, t_seen - 1) * a.per : 0;
-  const int w_first = t0 + wave * 32 < t_seen ? first_query(a.len, seq, t0 + wave * 32) * a.per : INT_MAX;
   const int my_first = t < t_seen ? first_query(a.len, seq, t) * a.per : INT_MAX;
   const int ntiles = t_seen > t0 && r_hi > r_lo ? (r_hi - r_lo + BN - 1) / BN : 0;
 
@@ -246,27 +248,60 @@ __global__ __launch_bounds__(NWV * 64) void dense_keys_kernel(GradK a) {
 
   if (ntiles > 0) {
     const float sl2 = a.scale * LOG2E;
-    const Share<RB, BN, NWV> sh(wave, lane);
-    const Share<DR ? DR * 2 : 128, BN, NWV> shr(wave, lane);
-    // (rows past the last repeat it; they are masked)
-    auto load_rows = [&](auto share, const Rows& x, int r0, uint8_t* dst) __attribute__((always_inline)) {
-#pragma unroll
-      for (int j = 0; j < share.CNT; ++j) {
-        const int r = min(r0 + j * share.STEP + share.row, r_hi - 1), s = row_div(a, r), g = r - s * a.per;
-        const char* p = reinterpret_cast<const char*>(x.p + (int64_t)(seq.r0 + s) * x.row + (int64_t)(n * a.per + g) * x.head);
-        lds_dma16_untracked(p + share.col, dst + (j * NWV + wave) * 1024);
+    // ---- tiles of head rows: each wave loads a share, in GPW loads. Where the group's heads divide the rows of one
+    // load of all waves, a lane's rows are of one head, and evenly spaced.
+    using Sh = Share<RB, BN, NWV>;
+    using ShR = Share<DR ? DR * 2 : 128, BN, NWV>;
+    const Sh sh(wave, lane);
+    const ShR shr(wave, lane);
+    constexpr int CQ = Sh::CNT, CR = DR ? ShR::CNT : 0, GPW = 2 * CQ + CR;
+    const uint16_t* const qb = a.q.p + (int64_t)seq.r0 * a.q.row + (int64_t)n * a.per * a.q.head;
+    const uint16_t* const db = a.d.p + (int64_t)seq.r0 * a.d.row + (int64_t)n * a.per * a.d.head;
+    const uint16_t* const qrb = DR ? a.qr.p + (int64_t)seq.r0 * a.qr.row + (int64_t)n * a.per * a.qr.head : nullptr;
+    auto place = [&](const Rows& x, int r) {   // of head row r, in bytes
+      const int s = row_div(a, r);
+      return ((int64_t)s * x.row + (int64_t)(r - s * a.per) * x.head) * 2;
+    };
+    const bool linear = a.linear;
+    const uint32_t q_off = linear ? (uint32_t)place(a.q, sh.row) + sh.col : 0, d_off = linear ? (uint32_t)place(a.d, sh.row) + sh.col : 0;
+    const uint32_t qr_off = DR && linear ? (uint32_t)place(a.qr, shr.row) + shr.col : 0;
+    const int per_shift = a.per_shift;   // (linear: per is a power of two)
+    const int64_t stat0 = n * (int64_t)a.len.rows * a.per + (int64_t)seq.r0 * a.per;
+    // load j of tile u (rows past the last repeat it; they are masked)
+    auto load_part = [&](auto jc, int u, int buf, bool fast) __attribute__((always_inline)) {
+      constexpr int j = decltype(jc)::value;
+      constexpr int what = j < CQ ? 0 : j < 2 * CQ ? 1 : 2, i = what == 0 ? j : what == 1 ? j - CQ : j - 2 * CQ;
+      constexpr int step = i * (what == 2 ? ShR::STEP : Sh::STEP);
+      const int r0 = r_lo + u * BN;
+      const Rows& x = what == 0 ? a.q : what == 1 ? a.d : a.qr;
+      const char* p = reinterpret_cast<const char*>(what == 0 ? qb : what == 1 ? db : qrb);
+      uint8_t* dst = (what == 0 ? L.t[buf].q : what == 1 ? L.t[buf].d : L.qr[buf]) + (i * NWV + wave) * 1024;
+      if (fast) {
+        lds_dma16_sbase_untracked(p + (int64_t)((r0 + step) >> per_shift) * x.row * 2, what == 0 ? q_off : what == 1 ? d_off : qr_off, dst);
+      } else {
+        const int r = min(r0 + step + (what == 2 ? shr.row : sh.row), r_hi - 1);
+        lds_dma16_untracked(p + place(x, r) + (what == 2 ? shr.col : sh.col), dst);
       }
     };
-    const int64_t stat0 = n * (int64_t)a.len.rows * a.per + (int64_t)seq.r0 * a.per;
-    auto load_tile = [&](int u) __attribute__((always_inline)) {
-      const int r0 = r_lo + u * BN, buf = u % NBUF;
-      load_rows(sh, a.q, r0, L.q[buf]);
-      load_rows(sh, a.d, r0, L.d[buf]);
-      if constexpr (DR > 0) load_rows(shr, a.qr, r0, L.qr[buf]);
-      if (wave == 0) lds_dma4(a.lse + stat0 + min(r0 + lane, r_hi - 1), L.lse[buf]);
-      if (wave == 1) lds_dma4(a.delta + stat0 + min(r0 + lane, r_hi - 1), L.delta[buf]);
+    auto load_stats = [&](int u, int buf) __attribute__((always_inline)) {
+      const int64_t r = stat0 + min(r_lo + u * BN + lane, r_hi - 1);
+      if (wave == 0) lds_dma4(a.lse + r, L.lse[buf]);
+      if (wave == 1) lds_dma4(a.delta + r, L.delta[buf]);
     };
-    load_tile(0);
+    auto load_tile = [&](int u, int buf) __attribute__((always_inline)) {
+      static_for<0, GPW>([&](auto j) __attribute__((always_inline)) { load_part(j, u, buf, false); });
+      load_stats(u, buf);
+    };
+    // (a masked pair has P = dS = 0, but 0 times a value that is not finite would reach tokens that the row does not see)
+    auto is_mixed = [&](int u) { return r_lo + u * BN < r_full || r_lo + u * BN + BN > r_hi; };
+    auto sanitize = [&](int u, int buf) __attribute__((always_inline)) {
+      if (!is_mixed(u)) return;
+      uint64_t bad = clean_share<IO, RB, BN, NWV>(lds_addr(L.t[buf].q), wave, lane) |
+                     clean_share<IO, RB, BN, NWV>(lds_addr(L.t[buf].d), wave, lane);
+      if constexpr (DR > 0) bad |= clean_share<IO, 128, BN, NWV>(lds_addr(L.qr[buf]), wave, lane);
+      if (lane == 0) L.bad[buf][wave] = bad;
+    };
+    load_tile(0, 0);
     uint4 kf[KS], vf[KSN];
     {
       const int64_t tt = seq.k0 + min(t, t_seen - 1);
@@ -279,83 +314,211 @@ __global__ __launch_bounds__(NWV * 64) void dense_keys_kernel(GradK a) {
 #pragma unroll
         for (int j = KSN; j < KS; ++j) kf[j] = ldg16(rp + (j - KSN) * 16);
       }
+#pragma unroll
+      for (int j = 0; j < KS; ++j) kf[j] = in_agprs(kf[j]);
+#pragma unroll
+      for (int j = 0; j < KSN; ++j) vf[j] = in_agprs(vf[j]);
     }
-    const int qk = s_row(rr);
-    for (int u = 0; u < ntiles; ++u) {
-      const int r0 = r_lo + u * BN, buf = u % NBUF;
-      // (a masked pair has P = dS = 0, but 0 times a value that is not finite would reach tokens that the row does not see)
-      const bool mixed = r0 < r_full || r0 + BN > r_hi;
-      wait_vmcnt<0>();
-      asm volatile("" ::: "memory");
-      if (mixed) {
-        uint64_t bad = clean_share<IO, RB, BN, NWV>(lds_addr(L.q[buf]), wave, lane) |
-                       clean_share<IO, RB, BN, NWV>(lds_addr(L.d[buf]), wave, lane);
-        if constexpr (DR > 0) bad |= clean_share<IO, 128, BN, NWV>(lds_addr(L.qr[buf]), wave, lane);
-        if (lane == 0) L.bad[buf][wave] = bad;
+
+    // ---- operands
+    constexpr int DOFF = BN * D * 2;   // from a place in q to the same in d
+    const int qk = s_row(rr), g16 = lane >> 4, c16 = lane & 15;
+    const int r4 = (g16 >> 1) * 8 + (c16 >> 2), vc = (g16 & 1) * 2 + ((c16 & 3) >> 1), o8 = (c16 & 1) * 8;
+    const uint32_t op_lane = tile_off<RB>(qk, kg), opr_lane = tile_off<128>(qk, kg);
+    const uint32_t tr_lo = tile_off<RB>(r4, vc) + o8, tr_hi = tile_off<RB>(r4 + 4, vc) + o8;
+    const uint32_t trr_lo = tile_off<128>(r4, vc) + o8, trr_hi = tile_off<128>(r4 + 4, vc) + o8;
+    OpAddr<RB> op;
+    OpAddr<128> opr;
+    TrAddr<RB> tr;
+    TrAddr<128> trr;
+    auto point_op = [&](int buf) __attribute__((always_inline)) {
+      op.point(lds_addr(L.t[buf].q), op_lane);
+      if constexpr (DR > 0) opr.point(lds_addr(L.qr[buf]), opr_lane);
+    };
+    auto point_tr = [&](int buf) __attribute__((always_inline)) {
+      tr.point(lds_addr(L.t[buf].q), tr_lo, tr_hi);
+      if constexpr (DR > 0) trr.point(lds_addr(L.qr[buf]), trr_lo, trr_hi);
+    };
+    auto q_frag = [&](int j, int h) __attribute__((always_inline)) -> uint4 {
+      return lds_read16_at(j < KSN ? op.a[j < KSN ? j : 0] + h * 32 * RB : opr.a[j >= KSN ? j - KSN : 0] + h * 32 * 128);
+    };
+    auto d_frag = [&](int j, int h) __attribute__((always_inline)) -> uint4 { return lds_read16_at(op.a[j] + h * 32 * RB + DOFF); };
+    // product i of a half's NP: column tiles of dV, dK and dK's rotary part for 16 rows, then for the next 16
+    constexpr int NC = 2 * ON + RN, NP = 2 * NC;
+    auto t_frag = [&](int i, int h) __attribute__((always_inline)) -> uint4 {
+      const int st = i / NC, c = i % NC;
+      if (c < ON) return tr.frag(c < ON ? c : 0, (h * 32 + st * 16) * RB + DOFF);
+      if (c < 2 * ON) return tr.frag(c >= ON && c < 2 * ON ? c - ON : 0, (h * 32 + st * 16) * RB);
+      return trr.frag(c >= 2 * ON ? c - 2 * ON : 0, (h * 32 + st * 16) * 128);
+    };
+
+    // ---- P and dS of 32 rows in NST stages of two rows each, placed among the products before and after them
+    constexpr int NST = 8;
+    float4 lse4[4], del4[4];   // rows 16 x + 8 kg + 4 y + 0 .. 3 at [2 x + y]
+    auto stats = [&](int buf, int h) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = h * 32 + 16 * (e >> 1) + 8 * kg + 4 * (e & 1);
+        lse4[e] = *reinterpret_cast<const float4*>(&L.lse[buf][at]);
+        del4[e] = *reinterpret_cast<const float4*>(&L.delta[buf][at]);
       }
-      lds_barrier();
-      if (u + 1 < ntiles) load_tile(u + 1);
-      if (r0 + BN <= w_first) continue;
-      uint64_t bad = 0;
-      if (mixed) bad = L.bad[buf][0] | L.bad[buf][1] | L.bad[buf][2] | L.bad[buf][3];
-      const uint32_t qt = lds_addr(L.q[buf]), dt = lds_addr(L.d[buf]), qrt = lds_addr(L.qr[buf]);
+    };
+    const float f16 = factor.x * 0x1p-15f;   // (fp16's P has the factor 2^15)
+    auto stage = [&](int st, f32x16& sv, f32x16& dp, uint32_t (&pw)[8], uint32_t (&sw)[8]) __attribute__((always_inline)) {
+      const int i = 2 * st;
+      const float4 l4 = lse4[i >> 2], d4 = del4[i >> 2];
+      const float l0 = i & 2 ? l4.z : l4.x, l1 = i & 2 ? l4.w : l4.y, e0 = i & 2 ? d4.z : d4.x, e1 = i & 2 ? d4.w : d4.y;
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], sl2, -l0));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i + 1], sl2, -l1));
+      float w0 = p0 * (dp[i] - e0), w1 = p1 * (dp[i + 1] - e1);
+      if constexpr (IO == IO_F16) w0 *= f16, w1 *= f16;
+      pw[st] = pack2<IO>(p0, p1);
+      sw[st] = pack2<IO>(w0, w1);
+      asm volatile("" : "+v"(pw[st]), "+v"(sw[st]));   // here, not where the next step needs them
+    };
+    auto mask = [&](int u, int buf, int h, uint32_t (&pw)[8], uint32_t (&sw)[8]) __attribute__((always_inline)) {
+      if (!is_mixed(u)) return;
+      const uint64_t all = L.bad[buf][0] | L.bad[buf][1] | L.bad[buf][2] | L.bad[buf][3];
+      const uint32_t bad = (uint32_t)(all >> (h * 32));
+      const int r0 = r_lo + u * BN + h * 32, first = my_first - r0, last = r_hi - r0;   // rows [first, last) see the token
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        f32x16 s, dp;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < KS; ++j)
-          s = Mfma<IO>::m32(j < KSN ? op_frag<RB>(qt, h * 32 + qk, j, kg) : op_frag<128>(qrt, h * 32 + qk, j - KSN, kg), kf[j], s);
-#pragma unroll
-        for (int j = 0; j < KSN; ++j) dp = Mfma<IO>::m32(op_frag<RB>(dt, h * 32 + qk, j, kg), vf[j], dp);
-        uint32_t pd[8], sd[8];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {   // rows 16 x + 8 kg + 0 .. 7
-          const float* lp = &L.lse[buf][h * 32 + 16 * x + 8 * kg];
-          const float* ep = &L.delta[buf][h * 32 + 16 * x + 8 * kg];
-          float p[8], ds[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int i = 8 * x + e;
-            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sl2, -lp[e]));
-            ds[e] = p[e] * (dp[i] - ep[e]);
-          }
-          if (bad)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if ((bad >> (h * 32 + 16 * x + 8 * kg + e)) & 1u) p[e] = ds[e] = __builtin_nanf("");
-          if (mixed)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int r = r0 + h * 32 + 16 * x + 8 * kg + e;
-              if (r < my_first || r >= r_hi) p[e] = ds[e] = 0.f;
-            }
-          if constexpr (IO == IO_F16) {
-            const float f = factor.x * 0x1p-15f;   // (P has the factor 2^15)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) ds[e] *= f;
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            pd[4 * x + e] = pack2<IO>(p[2 * e], p[2 * e + 1]);
-            sd[4 * x + e] = pack2<IO>(ds[2 * e], ds[2 * e + 1]);
-          }
-        }
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          const uint4 pb = make_uint4(pd[4 * st], pd[4 * st + 1], pd[4 * st + 2], pd[4 * st + 3]);
-          const uint4 sb = make_uint4(sd[4 * st], sd[4 * st + 1], sd[4 * st + 2], sd[4 * st + 3]);
-#pragma unroll
-          for (int c = 0; c < ON; ++c) {
-            dv[c] = Mfma<IO>::m32(tr_frag<RB>(dt, h * 32 + st * 16, c, lane), pb, dv[c]);
-            dk[c] = Mfma<IO>::m32(tr_frag<RB>(qt, h * 32 + st * 16, c, lane), sb, dk[c]);
-          }
-#pragma unroll
-          for (int c = 0; c < RN; ++c) dk[ON + c] = Mfma<IO>::m32(tr_frag<128>(qrt, h * 32 + st * 16, c, lane), sb, dk[ON + c]);
-        }
+      for (int i = 0; i < 8; ++i) {
+        const int x = s_token(2 * i, kg);
+        const uint32_t nan = ((bad >> x) & 1u ? 0x7FFFu : 0u) | ((bad >> (x + 1)) & 1u ? 0x7FFF0000u : 0u);
+        const uint32_t keep = (x >= first && x < last ? 0xFFFFu : 0u) | (x + 1 >= first && x + 1 < last ? 0xFFFF0000u : 0u);
+        pw[i] = (pw[i] | nan) & keep;
+        sw[i] = (sw[i] | nan) & keep;
       }
+    };
+
+    // ---- One step handles 32 rows: the products of the rows before them, S and dP of the rows after them, each MFMA
+    // followed by a part of this one's P and dS. Fragments are read a few MFMAs ahead.
+    constexpr int LAG = KS - KSN, NS = KS + KSN;   // S and dP end together
+    constexpr int TR = 4, QR = 4, DRING = 4;
+    uint4 tf[TR], qf[QR], df[DRING];
+    auto step = [&](auto pvc, auto sc, auto hc, f32x16& cs, f32x16& cd, f32x16& ns, f32x16& nd, uint32_t (&pb)[8], uint32_t (&sb)[8],
+                    uint32_t (&pn)[8], uint32_t (&sn)[8], auto&& between, auto&& ride) __attribute__((always_inline)) {
+      constexpr bool PV = decltype(pvc)::value, S = decltype(sc)::value;
+      constexpr int H = decltype(hc)::value;
+      constexpr int M0 = PV ? NP : 0, NMM = M0 + (S ? NS : 0), LEAD = NMM > 8 ? 2 : 0;
+      auto values_at = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int st = 0; st < NST; ++st)
+          if (LEAD + st * (NMM - LEAD) / NST == slot) stage(st, cs, cd, pn, sn);
+      };
+      if constexpr (PV)
+        static_for<0, NP>([&](auto ic) __attribute__((always_inline)) {
+          constexpr int i = decltype(ic)::value, st = i / NC, c = i % NC;
+          const uint4 b = c < ON ? make_uint4(pb[4 * st], pb[4 * st + 1], pb[4 * st + 2], pb[4 * st + 3])
+                                 : make_uint4(sb[4 * st], sb[4 * st + 1], sb[4 * st + 2], sb[4 * st + 3]);
+          if constexpr (c < ON) dv[c] = Mfma<IO>::m32(tf[i % TR], b, dv[c]);
+          else dk[c - ON] = Mfma<IO>::m32(tf[i % TR], b, dk[c - ON]);
+          if constexpr (i + TR < NP) tf[i % TR] = t_frag(i + TR, H);
+          if constexpr (S && i < QR) qf[i] = q_frag(i, H);
+          if constexpr (S && i >= QR && i < QR + DRING) df[i - QR] = d_frag(i - QR, H);
+          values_at(i);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      between();
+      if constexpr (S)
+        static_for<0, NS>([&](auto jc) __attribute__((always_inline)) {
+          constexpr int j = decltype(jc)::value;
+          constexpr bool is_s = j < LAG || (j - LAG) % 2 == 0;
+          constexpr int i = j < LAG ? j : is_s ? LAG + (j - LAG) / 2 : (j - LAG) / 2;   // step of its chain
+          if constexpr (j == NS - 1) mfma32_va_end2<IO>(ns, qf[(KS - 1) % QR], kf[KS - 1], nd, df[(KSN - 1) % DRING], vf[KSN - 1]);
+          else if constexpr (is_s && i < KS - 1) {
+            mfma32_va<IO, i == 0>(ns, qf[i % QR], kf[i]);
+            if constexpr (i + QR < KS) qf[i % QR] = q_frag(i + QR, H);
+          } else if constexpr (!is_s) {
+            mfma32_va<IO, i == 0>(nd, df[i % DRING], vf[i]);
+            if constexpr (i + DRING < KSN) df[i % DRING] = d_frag(i + DRING, H);
+          }
+          if constexpr (j >= NS - TR) tf[j - (NS - TR)] = t_frag(j - (NS - TR), 1 - H);
+          ride(jc);
+          values_at(M0 + j);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    std::true_type yes;
+    std::false_type no;
+    std::integral_constant<int, 0> h0;
+    std::integral_constant<int, 1> h1;
+    auto nothing = [](auto...) __attribute__((always_inline)) {};
+
+    wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    sanitize(0, 0);
+    lds_barrier();
+    if (ntiles > 1) load_tile(1, 1);
+    f32x16 s0, s1, d0, d1;
+    uint32_t p0[8], p1[8], w0[8], w1[8];
+    point_op(0);
+#pragma unroll
+    for (int j = 0; j < KS - 1; ++j) {
+      const uint4 f = q_frag(j, 0);
+      if (j == 0) mfma32_va<IO, true>(s0, f, kf[j]);
+      else mfma32_va<IO, false>(s0, f, kf[j]);
     }
+#pragma unroll
+    for (int j = 0; j < KSN - 1; ++j) {
+      const uint4 f = d_frag(j, 0);
+      if (j == 0) mfma32_va<IO, true>(d0, f, vf[j]);
+      else mfma32_va<IO, false>(d0, f, vf[j]);
+    }
+    mfma32_va_end2<IO>(s0, q_frag(KS - 1, 0), kf[KS - 1], d0, d_frag(KSN - 1, 0), vf[KSN - 1]);
+#pragma unroll
+    for (int j = 0; j < QR; ++j) qf[j] = q_frag(j, 1);
+#pragma unroll
+    for (int j = 0; j < DRING; ++j) df[j] = d_frag(j, 1);
+    int buf = 0;   // of tile u
+    // Step (u, 0): tile u + 1 has landed by the middle of it, when nobody needs tile u - 1 any more
+    auto half0 = [&](auto pvc, int u) __attribute__((always_inline)) {
+      const int nb = buf == NBUF - 1 ? 0 : buf + 1, lb = buf == 0 ? NBUF - 1 : buf - 1;   // of tiles u + 1 and u - 1 (u + 2)
+      stats(buf, 0);
+      const bool more = u + 2 < ntiles, fast = linear && r_lo + (u + 3) * BN <= r_hi;
+      step(pvc, yes, h1, s0, d0, s1, d1, p1, w1, p0, w0,
+           [&]() __attribute__((always_inline)) {
+             wait_vmcnt<0>();
+             asm volatile("" ::: "memory");
+             if (u + 1 < ntiles) sanitize(u + 1, nb);
+             lds_barrier();
+             point_tr(buf);
+           },
+           [&](auto jc) __attribute__((always_inline)) {
+             constexpr int j = decltype(jc)::value;
+             static_for<0, GPW>([&](auto g) __attribute__((always_inline)) {
+               if constexpr (g * NS / GPW == j)
+                 if (more) load_part(g, u + 2, lb, fast);
+             });
+             if constexpr (j == NS - 1)
+               if (more) load_stats(u + 2, lb);
+           });
+      mask(u, buf, 0, p0, w0);
+    };
+    half0(no, 0);
+    for (int uv = 0; uv + 1 < ntiles; ++uv) {
+      const int u = __builtin_amdgcn_readfirstlane(uv);
+      const int nb = buf == NBUF - 1 ? 0 : buf + 1;
+      point_op(nb);
+      stats(buf, 1);
+      step(yes, yes, h0, s1, d1, s0, d0, p0, w0, p1, w1, nothing, nothing);
+      mask(u, buf, 1, p1, w1);
+      buf = nb;
+      half0(yes, u + 1);
+    }
+    stats(buf, 1);
+    step(yes, no, h0, s1, d1, s0, d0, p0, w0, p1, w1, nothing, nothing);
+    mask(ntiles - 1, buf, 1, p1, w1);
+#pragma unroll
+    for (int i = 0; i < TR; ++i) tf[i] = t_frag(i, 1);
+    static_for<0, NP>([&](auto ic) __attribute__((always_inline)) {
+      constexpr int i = decltype(ic)::value, st = i / NC, c = i % NC;
+      const uint4 b = c < ON ? make_uint4(p1[4 * st], p1[4 * st + 1], p1[4 * st + 2], p1[4 * st + 3])
+                             : make_uint4(w1[4 * st], w1[4 * st + 1], w1[4 * st + 2], w1[4 * st + 3]);
+      if constexpr (c < ON) dv[c] = Mfma<IO>::m32(tf[i % TR], b, dv[c]);
+      else dk[c - ON] = Mfma<IO>::m32(tf[i % TR], b, dk[c - ON]);
+      if constexpr (i + TR < NP) tf[i % TR] = t_frag(i + TR, 1);
+    });
   }
 
   // lane l: token t, columns c * 32 + 8 g + 4 kg + j
@@ -394,12 +557,21 @@ __global__ __launch_bounds__(NWV * 64) void dense_keys_kernel(GradK a) {
 
 // ---------------------------------------------------------------- queries
 template <int D, int DR> struct QueryLds {
-  uint8_t k[NBUF][BN * D * 2];
-  uint8_t v[NBUF][BN * D * 2];
+  struct {
+    uint8_t k[BN * D * 2];   // (v lies at a constant offset from k)
+    uint8_t v[BN * D * 2];
+  } t[NBUF];
   uint8_t kr[NBUF][DR ? BN * DR * 2 : 16];
   uint64_t bad[NBUF][NWV];
   float red[2][NWV];
 };
+
+// delta = dO . O takes the rounded output, off by half a step of it: next to nothing beside dP where a row's weight
+// lies on many tokens, as much as the rounding of dS where it lies on few. The sum of P dP over the row's tokens is the
+// same number without that error, and comes along here for one operation an element: it goes to the keys' kernel, which
+// runs after this one. This kernel itself needs it beforehand: rows of up to SHORT tokens run over them once more first
+// (random queries and keys, bf16, 200 tokens: dQ's error against 64 bits 1.57 times that of rounding the exact one, 1.43 so).
+constexpr int SHORT = 256;
 
 template <int IO, int D, int DR>
 __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
@@ -425,7 +597,7 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
   const int hi = seen(r_base, r_end);
   const int min_lim = max(t_lo + 1, limit_of(a.len, seq, r_base / a.per));
   const int ntiles = hi > t_lo ? (hi - t_lo + BN - 1) / BN : 0;
-  const int w_base = r_base + wave * 32, w_hi = seen(w_base, min(r_end, w_base + 32));
+  const int w_base = r_base + wave * 32;
   const int row = w_base + rr;
   const bool valid = row < r_end;
   const int r = valid ? row : r_end - 1, s = r / a.per, g = r - s * a.per;
@@ -439,31 +611,51 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
     for (int i = 0; i < 16; ++i) dq[c][i] = 0.f;
 
   if (ntiles > 0) {
-    const float sl2 = a.scale * LOG2E;
-    const Share<RB, BN, NWV> sh(wave, lane);
-    const Share<DR ? DR * 2 : 128, BN, NWV> shr(wave, lane);
-    const uint16_t* const kb = a.k.p + (int64_t)seq.k0 * a.k.row + n * a.k.head;
-    const uint16_t* const vb = a.v.p + (int64_t)seq.k0 * a.v.row + n * a.v.head;
-    const uint16_t* const krb = DR ? a.kr.p + (int64_t)seq.k0 * a.kr.row + n * a.kr.head : nullptr;
+    // (a zero scale becomes 1e-30: scores round to 0, and a masked one, of the sign that makes it so, to P = 0)
+    const float sl2 = (a.scale == 0.f ? 1e-30f : a.scale) * LOG2E;
+    const float masked = sl2 > 0.f ? -INFINITY : INFINITY;
+    using Sh = Share<RB, BN, NWV>;
+    using ShR = Share<DR ? DR * 2 : 128, BN, NWV>;
+    const Sh sh(wave, lane);
+    const ShR shr(wave, lane);
+    constexpr int CK = Sh::CNT, CR = DR ? ShR::CNT : 0, GPW = 2 * CK + CR;
     const uint32_t k_row = (uint32_t)a.k.row * 2, v_row = (uint32_t)a.v.row * 2, kr_row = (uint32_t)a.kr.row * 2;
-    auto load_rows = [&](auto share, const uint16_t* base, uint32_t row_bytes, int t0, uint8_t* dst) __attribute__((always_inline)) {
-      const char* p = reinterpret_cast<const char*>(base) + (int64_t)t0 * row_bytes;
-#pragma unroll
-      for (int j = 0; j < share.CNT; ++j) {
-        const int t = min(j * share.STEP + share.row, seq.ak - 1 - t0);
-        lds_dma16_sbase_untracked(p, (uint32_t)t * row_bytes + share.col, dst + (j * NWV + wave) * 1024);
+    const char* const kb = reinterpret_cast<const char*>(a.k.p + (int64_t)seq.k0 * a.k.row + n * a.k.head);
+    const char* const vb = reinterpret_cast<const char*>(a.v.p + (int64_t)seq.k0 * a.v.row + n * a.v.head);
+    const char* const krb = DR ? reinterpret_cast<const char*>(a.kr.p + (int64_t)seq.k0 * a.kr.row + n * a.kr.head) : nullptr;
+    const uint32_t k_off = sh.row * k_row + sh.col, v_off = sh.row * v_row + sh.col, kr_off = shr.row * kr_row + shr.col;
+    // load j of tile u (rows past the last token repeat it; they are masked)
+    auto load_part = [&](auto jc, int u, int buf, bool whole) __attribute__((always_inline)) {
+      constexpr int j = decltype(jc)::value;
+      constexpr int what = j < CK ? 0 : j < 2 * CK ? 1 : 2, i = what == 0 ? j : what == 1 ? j - CK : j - 2 * CK;
+      constexpr int step = i * (what == 2 ? ShR::STEP : Sh::STEP);
+      const int t0 = t_lo + u * BN;
+      const uint32_t row = what == 0 ? k_row : what == 1 ? v_row : kr_row;
+      const char* p = (what == 0 ? kb : what == 1 ? vb : krb) + (int64_t)t0 * row;
+      uint8_t* dst = (what == 0 ? L.t[buf].k : what == 1 ? L.t[buf].v : L.kr[buf]) + (i * NWV + wave) * 1024;
+      if (whole) {
+        lds_dma16_sbase_untracked(p + step * (int64_t)row, what == 0 ? k_off : what == 1 ? v_off : kr_off, dst);
+      } else {
+        const int t = min(step + (what == 2 ? shr.row : sh.row), seq.ak - 1 - t0);
+        lds_dma16_sbase_untracked(p, (uint32_t)t * row + (what == 2 ? shr.col : sh.col), dst);
       }
     };
-    auto load_tile = [&](int u) __attribute__((always_inline)) {
-      const int t0 = t_lo + u * BN, buf = u % NBUF;
-      load_rows(sh, kb, k_row, t0, L.k[buf]);
-      load_rows(sh, vb, v_row, t0, L.v[buf]);
-      if constexpr (DR > 0) load_rows(shr, krb, kr_row, t0, L.kr[buf]);
+    auto load_tile = [&](int u, int buf) __attribute__((always_inline)) {
+      static_for<0, GPW>([&](auto j) __attribute__((always_inline)) { load_part(j, u, buf, false); });
     };
-    load_tile(0);
+    // (a masked token has dS = 0, but 0 times a value that is not finite would reach rows that do not see it)
+    auto is_mixed = [&](int u) { return t_lo + u * BN + BN > min_lim; };
+    auto sanitize = [&](int u, int buf) __attribute__((always_inline)) {
+      if (!is_mixed(u)) return;
+      uint64_t bad = clean_share<IO, RB, BN, NWV>(lds_addr(L.t[buf].k), wave, lane);
+      if constexpr (DR > 0) bad |= clean_share<IO, 128, BN, NWV>(lds_addr(L.kr[buf]), wave, lane);
+      if (lane == 0) L.bad[buf][wave] = bad;
+    };
+    load_tile(0, 0);
     uint4 qf[KS], df[KSN];
     const int64_t stat = n * (int64_t)a.len.rows * a.per + (int64_t)seq.r0 * a.per + r;
-    const float lse = a.lse[stat], delta = a.delta[stat];
+    const float lse = a.lse[stat];
+    float delta = a.delta[stat];
     {
       const int64_t q_row = seq.r0 + s, head = n * a.per + g;
       const uint16_t* qp = a.q.p + q_row * a.q.row + head * a.q.head + kg * 8;
@@ -475,63 +667,227 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
 #pragma unroll
         for (int j = KSN; j < KS; ++j) qf[j] = ldg16(rp + (j - KSN) * 16);
       }
+#pragma unroll
+      for (int j = 0; j < KS; ++j) qf[j] = in_agprs(qf[j]);
+#pragma unroll
+      for (int j = 0; j < KSN; ++j) df[j] = in_agprs(df[j]);
     }
-    const float fs = IO == IO_F16 ? factor.x * 0x1p-15f : 1.f;
-    const int tk = s_row(rr);
-    for (int u = 0; u < ntiles; ++u) {
-      const int t0 = t_lo + u * BN, buf = u % NBUF;
-      const bool mixed = t0 + BN > min_lim;
-      wait_vmcnt<0>();
-      asm volatile("" ::: "memory");
-      if (mixed) {
-        uint64_t bad = clean_share<IO, RB, BN, NWV>(lds_addr(L.k[buf]), wave, lane);
-        if constexpr (DR > 0) bad |= clean_share<IO, 128, BN, NWV>(lds_addr(L.kr[buf]), wave, lane);
-        if (lane == 0) L.bad[buf][wave] = bad;
+
+    // ---- operands
+    constexpr int VOFF = BN * D * 2;   // from a place in k to the same in v
+    const int tk = s_row(rr), g16 = lane >> 4, c16 = lane & 15;
+    const int r4 = (g16 >> 1) * 8 + (c16 >> 2), vc = (g16 & 1) * 2 + ((c16 & 3) >> 1), o8 = (c16 & 1) * 8;
+    const uint32_t op_lane = tile_off<RB>(tk, kg), opr_lane = tile_off<128>(tk, kg);
+    const uint32_t tr_lo = tile_off<RB>(r4, vc) + o8, tr_hi = tile_off<RB>(r4 + 4, vc) + o8;
+    const uint32_t trr_lo = tile_off<128>(r4, vc) + o8, trr_hi = tile_off<128>(r4 + 4, vc) + o8;
+    OpAddr<RB> op;
+    OpAddr<128> opr;
+    TrAddr<RB> tr;
+    TrAddr<128> trr;
+    auto point_op = [&](int buf) __attribute__((always_inline)) {
+      op.point(lds_addr(L.t[buf].k), op_lane);
+      if constexpr (DR > 0) opr.point(lds_addr(L.kr[buf]), opr_lane);
+    };
+    auto point_tr = [&](int buf) __attribute__((always_inline)) {
+      tr.point(lds_addr(L.t[buf].k), tr_lo, tr_hi);
+      if constexpr (DR > 0) trr.point(lds_addr(L.kr[buf]), trr_lo, trr_hi);
+    };
+    auto k_frag = [&](int j, int h) __attribute__((always_inline)) -> uint4 {
+      return lds_read16_at(j < KSN ? op.a[j < KSN ? j : 0] + h * 32 * RB : opr.a[j >= KSN ? j - KSN : 0] + h * 32 * 128);
+    };
+    auto v_frag = [&](int j, int h) __attribute__((always_inline)) -> uint4 { return lds_read16_at(op.a[j] + h * 32 * RB + VOFF); };
+    // product i of a half's NP: column tiles of dQ and its rotary part for 16 tokens, then for the next 16
+    constexpr int NC = ON + RN, NP = 2 * NC;
+    auto t_frag = [&](int i, int h) __attribute__((always_inline)) -> uint4 {
+      const int st = i / NC, c = i % NC;
+      if (c < ON) return tr.frag(c < ON ? c : 0, (h * 32 + st * 16) * RB);
+      return trr.frag(c >= ON ? c - ON : 0, (h * 32 + st * 16) * 128);
+    };
+    // S^T and dP^T of half h of the tile that op points to, by themselves
+    auto scores = [&](int h, f32x16& sv, f32x16& dp) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < KS - 1; ++j) {
+        const uint4 f = k_frag(j, h);
+        if (j == 0) mfma32_va<IO, true>(sv, f, qf[j]);
+        else mfma32_va<IO, false>(sv, f, qf[j]);
       }
+#pragma unroll
+      for (int j = 0; j < KSN - 1; ++j) {
+        const uint4 f = v_frag(j, h);
+        if (j == 0) mfma32_va<IO, true>(dp, f, df[j]);
+        else mfma32_va<IO, false>(dp, f, df[j]);
+      }
+      mfma32_va_end2<IO>(sv, k_frag(KS - 1, h), qf[KS - 1], dp, v_frag(KSN - 1, h), df[KSN - 1]);
+    };
+    auto mask = [&](int u, int buf, int h, f32x16& sv, f32x16& dp) __attribute__((always_inline)) {
+      if (!is_mixed(u)) return;
+      const int l = lim - (t_lo + u * BN + h * 32);
+      const uint64_t all = L.bad[buf][0] | L.bad[buf][1] | L.bad[buf][2] | L.bad[buf][3];
+      const uint32_t bad = (uint32_t)(all >> (h * 32));
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if ((bad >> s_token(i, kg)) & 1u) sv[i] = __builtin_nanf("");
+        if (s_token(i, kg) >= l) sv[i] = masked, dp[i] = 0.f;
+      }
+    };
+    float sum = 0.f;   // of P dP
+    // (only where this range is all that every row of the work-group sees)
+    if (t_lo == 0 && limit_of(a.len, seq, min((r_end - 1) / a.per, seq.aq - 1)) <= min(SHORT, t_hi)) {
+      for (int u = 0; u < ntiles; ++u) {
+        if (u > 0) {
+          lds_barrier();   // every wave is done with the buffer
+          load_tile(u, 0);
+        }
+        wait_vmcnt<0>();
+        asm volatile("" ::: "memory");
+        sanitize(u, 0);
+        lds_barrier();
+        point_op(0);
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          f32x16 sv, dp;
+          if (h == 0) scores(0, sv, dp);
+          else scores(1, sv, dp);
+          mask(u, 0, h, sv, dp);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum = fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], sl2, -lse)), dp[i], sum);
+        }
+      }
+      delta = add_half_swap(sum) * (IO == IO_F16 ? 0x1p-15f : 1.f);
+      sum = 0.f;
       lds_barrier();
-      if (u + 1 < ntiles) load_tile(u + 1);
-      if (t0 >= w_hi) continue;
-      uint64_t bad = 0;
-      if (mixed) bad = L.bad[buf][0] | L.bad[buf][1] | L.bad[buf][2] | L.bad[buf][3];
-      const uint32_t kt = lds_addr(L.k[buf]), vt = lds_addr(L.v[buf]), krt = lds_addr(L.kr[buf]);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        f32x16 sv, dp;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sv[i] = dp[i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < KS; ++j)
-          sv = Mfma<IO>::m32(j < KSN ? op_frag<RB>(kt, h * 32 + tk, j, kg) : op_frag<128>(krt, h * 32 + tk, j - KSN, kg), qf[j], sv);
-#pragma unroll
-        for (int j = 0; j < KSN; ++j) dp = Mfma<IO>::m32(op_frag<RB>(vt, h * 32 + tk, j, kg), df[j], dp);
-        float ds[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], sl2, -lse));
-          ds[i] = p * (dp[i] - delta);
-          if constexpr (IO == IO_F16) ds[i] *= fs;
-        }
-        if (bad)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if ((bad >> (h * 32 + s_token(i, kg))) & 1u) ds[i] = __builtin_nanf("");
-        if (mixed)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (t0 + h * 32 + s_token(i, kg) >= lim) ds[i] = 0.f;
-        uint32_t w[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = pack2<IO>(ds[2 * i], ds[2 * i + 1]);
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          const uint4 sb = make_uint4(w[4 * st], w[4 * st + 1], w[4 * st + 2], w[4 * st + 3]);
-#pragma unroll
-          for (int c = 0; c < ON; ++c) dq[c] = Mfma<IO>::m32(tr_frag<RB>(kt, h * 32 + st * 16, c, lane), sb, dq[c]);
-#pragma unroll
-          for (int c = 0; c < RN; ++c) dq[ON + c] = Mfma<IO>::m32(tr_frag<128>(krt, h * 32 + st * 16, c, lane), sb, dq[ON + c]);
-        }
-      }
+      load_tile(0, 0);   // (anew also where it is the only one: cleaned values are gone from it)
     }
+
+    // ---- dS of 32 tokens in NST stages of two each, placed among the products before and after them
+    constexpr int NST = 8;
+    const float fs = factor.x * 0x1p-15f;   // (fp16's P has the factor 2^15)
+    auto stage = [&](int st, f32x16& sv, f32x16& dp, uint32_t (&wn)[8]) __attribute__((always_inline)) {
+      const int i = 2 * st;
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], sl2, -lse));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i + 1], sl2, -lse));
+      sum = fmaf(p0, dp[i], sum);
+      sum = fmaf(p1, dp[i + 1], sum);
+      float x0 = p0 * (dp[i] - delta), x1 = p1 * (dp[i + 1] - delta);
+      if constexpr (IO == IO_F16) x0 *= fs, x1 *= fs;
+      wn[st] = pack2<IO>(x0, x1);
+      asm volatile("" : "+v"(wn[st]), "+v"(sum));   // here, not where the next step needs it
+    };
+
+    // ---- One step handles 32 tokens: the products of those before them, S and dP of those after them, each MFMA
+    // followed by a part of this one's dS. Fragments are read a few MFMAs ahead.
+    constexpr int LAG = KS - KSN, NS = KS + KSN;   // S and dP end together
+    constexpr int TR = 4, KR = 4, VR = 4;
+    uint4 tf[TR], kf[KR], vf[VR];
+    auto step = [&](auto pvc, auto sc, auto hc, f32x16& cs, f32x16& cd, f32x16& ns, f32x16& nd, uint32_t (&wb)[8], uint32_t (&wn)[8],
+                    auto&& between, auto&& ride) __attribute__((always_inline)) {
+      constexpr bool PV = decltype(pvc)::value, S = decltype(sc)::value;
+      constexpr int H = decltype(hc)::value;
+      constexpr int M0 = PV ? NP : 0, NMM = M0 + (S ? NS : 0), LEAD = NMM > 8 ? 2 : 0;
+      auto values_at = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int st = 0; st < NST; ++st)
+          if (LEAD + st * (NMM - LEAD) / NST == slot) stage(st, cs, cd, wn);
+      };
+      if constexpr (PV)
+        static_for<0, NP>([&](auto ic) __attribute__((always_inline)) {
+          constexpr int i = decltype(ic)::value, st = i / NC, c = i % NC;
+          dq[c] = Mfma<IO>::m32(tf[i % TR], make_uint4(wb[4 * st], wb[4 * st + 1], wb[4 * st + 2], wb[4 * st + 3]), dq[c]);
+          if constexpr (i + TR < NP) tf[i % TR] = t_frag(i + TR, H);
+          if constexpr (S)
+            static_for<0, KR + VR>([&](auto gc) __attribute__((always_inline)) {
+              constexpr int g = decltype(gc)::value;
+              if constexpr (g * NP / (KR + VR) == i) {
+                if constexpr (g < KR) kf[g] = k_frag(g, H);
+                else vf[g - KR] = v_frag(g - KR, H);
+              }
+            });
+          values_at(i);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      between();
+      if constexpr (S)
+        static_for<0, NS>([&](auto jc) __attribute__((always_inline)) {
+          constexpr int j = decltype(jc)::value;
+          constexpr bool is_s = j < LAG || (j - LAG) % 2 == 0;
+          constexpr int i = j < LAG ? j : is_s ? LAG + (j - LAG) / 2 : (j - LAG) / 2;   // step of its chain
+          if constexpr (j == NS - 1) mfma32_va_end2<IO>(ns, kf[(KS - 1) % KR], qf[KS - 1], nd, vf[(KSN - 1) % VR], df[KSN - 1]);
+          else if constexpr (is_s && i < KS - 1) {
+            mfma32_va<IO, i == 0>(ns, kf[i % KR], qf[i]);
+            if constexpr (i + KR < KS) kf[i % KR] = k_frag(i + KR, H);
+          } else if constexpr (!is_s) {
+            mfma32_va<IO, i == 0>(nd, vf[i % VR], df[i]);
+            if constexpr (i + VR < KSN) vf[i % VR] = v_frag(i + VR, H);
+          }
+          if constexpr (j >= NS - TR) tf[j - (NS - TR)] = t_frag(j - (NS - TR), 1 - H);
+          ride(jc);
+          values_at(M0 + j);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    std::true_type yes;
+    std::false_type no;
+    std::integral_constant<int, 0> h0;
+    std::integral_constant<int, 1> h1;
+    auto nothing = [](auto...) __attribute__((always_inline)) {};
+
+    wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    sanitize(0, 0);
+    lds_barrier();
+    if (ntiles > 1) load_tile(1, 1);
+    f32x16 s0, s1, d0, d1;
+    uint32_t w0[8], w1[8];
+    point_op(0);
+    scores(0, s0, d0);
+#pragma unroll
+    for (int j = 0; j < KR; ++j) kf[j] = k_frag(j, 1);
+#pragma unroll
+    for (int j = 0; j < VR; ++j) vf[j] = v_frag(j, 1);
+    int buf = 0;   // of tile u
+    // Step (u, 0): tile u + 1 has landed by the middle of it, when nobody needs tile u - 1 any more
+    auto half0 = [&](auto pvc, int u) __attribute__((always_inline)) {
+      const int nb = buf == NBUF - 1 ? 0 : buf + 1, lb = buf == 0 ? NBUF - 1 : buf - 1;   // of tiles u + 1 and u - 1 (u + 2)
+      mask(u, buf, 0, s0, d0);
+      const bool more = u + 2 < ntiles, whole = t_lo + (u + 3) * BN <= seq.ak;
+      step(pvc, yes, h1, s0, d0, s1, d1, w1, w0,
+           [&]() __attribute__((always_inline)) {
+             wait_vmcnt<0>();
+             asm volatile("" ::: "memory");
+             if (u + 1 < ntiles) sanitize(u + 1, nb);
+             lds_barrier();
+             point_tr(buf);
+           },
+           [&](auto jc) __attribute__((always_inline)) {
+             constexpr int j = decltype(jc)::value;
+             static_for<0, GPW>([&](auto g) __attribute__((always_inline)) {
+               if constexpr (g * NS / GPW == j)
+                 if (more) load_part(g, u + 2, lb, whole);
+             });
+           });
+    };
+    half0(no, 0);
+    for (int uv = 0; uv + 1 < ntiles; ++uv) {
+      const int u = __builtin_amdgcn_readfirstlane(uv);
+      const int nb = buf == NBUF - 1 ? 0 : buf + 1;
+      point_op(nb);
+      mask(u, buf, 1, s1, d1);
+      step(yes, yes, h0, s1, d1, s0, d0, w0, w1, nothing, nothing);
+      buf = nb;
+      half0(yes, u + 1);
+    }
+    mask(ntiles - 1, buf, 1, s1, d1);
+    step(yes, no, h0, s1, d1, s0, d0, w0, w1, nothing, nothing);
+#pragma unroll
+    for (int i = 0; i < TR; ++i) tf[i] = t_frag(i, 1);
+    static_for<0, NP>([&](auto ic) __attribute__((always_inline)) {
+      constexpr int i = decltype(ic)::value, st = i / NC, c = i % NC;
+      dq[c] = Mfma<IO>::m32(tf[i % TR], make_uint4(w1[4 * st], w1[4 * st + 1], w1[4 * st + 2], w1[4 * st + 3]), dq[c]);
+      if constexpr (i + TR < NP) tf[i % TR] = t_frag(i + TR, 1);
+    });
+    sum = add_half_swap(sum) * (IO == IO_F16 ? 0x1p-15f : 1.f);
+    // (all that the row sees lies in this range: others keep dO . O)
+    if (lane < 32 && valid && !dead && t_lo == 0 && (at.sp == a.q_splits - 1 || limit_of(a.len, seq, s) <= t_hi)) a.delta[stat] = sum;
   }
 
   const float f = a.scale * factor.y;
@@ -656,12 +1012,12 @@ Cut make_cut(const DenseGradArgs& g) {
 template <int IO, int D, int DR>
 hipError_t launch_d(const GradK& k, const Cut& c, hipStream_t s) {
   hipLaunchKernelGGL((dense_prep_kernel<IO, D>), dim3(PREP), dim3(256), 0, s, k);
-  hipLaunchKernelGGL((dense_keys_kernel<IO, D, DR>), dim3((unsigned)c.keys.groups), dim3(NWV * 64), 0, s, k);
-  if (c.keys.splits > 1)
-    hipLaunchKernelGGL((dense_join_kernel<IO, D, DR, true>), dim3((unsigned)c.keys.blocks), dim3(256), 0, s, k);
   hipLaunchKernelGGL((dense_queries_kernel<IO, D, DR>), dim3((unsigned)c.queries.groups), dim3(NWV * 64), 0, s, k);
   if (c.queries.splits > 1)
     hipLaunchKernelGGL((dense_join_kernel<IO, D, DR, false>), dim3((unsigned)c.queries.blocks), dim3(256), 0, s, k);
+  hipLaunchKernelGGL((dense_keys_kernel<IO, D, DR>), dim3((unsigned)c.keys.groups), dim3(NWV * 64), 0, s, k);
+  if (c.keys.splits > 1)
+    hipLaunchKernelGGL((dense_join_kernel<IO, D, DR, true>), dim3((unsigned)c.keys.blocks), dim3(256), 0, s, k);
   return hipGetLastError();
 }
 template <int IO>
@@ -692,6 +1048,9 @@ hipError_t launch_dense_grad(const DenseGradArgs& g, size_t* lacking, hipStream_
   k.per = a.n1 / a.n2;
   while ((1 << k.per_shift) < k.per) ++k.per_shift;
   k.per_mul = (uint32_t)(((1ull << (31 + k.per_shift)) + k.per - 1) / k.per);
+  k.linear = 16 % k.per == 0;
+  for (const DenseTensor* t : {&a.q, &a.qr, &g.d_out})   // (a lane's offset has 32 bits)
+    if ((a.dr > 0 || t != &a.qr) && (16 * t->row + k.per * t->head) * 2 >= (1ll << 31)) k.linear = 0;
   k.q_seqs = c.queries.seqs, k.k_seqs = c.keys.seqs, k.q_even = c.queries.even, k.k_even = c.keys.even;
   k.scale = a.scale;
   k.stat_padded = a.stat_padded;
