@@ -16,7 +16,6 @@
 namespace dsa {
 namespace {
 
-constexpr int NWV = 4;
 constexpr int BN = 64;     // tokens a tile
 constexpr int NBUF = 3;
 
@@ -59,10 +58,10 @@ template <int D, int DR> struct FwdLds {
   uint8_t k[NBUF][BN * D * 2];
   uint8_t v[NBUF][BN * D * 2];
   uint8_t kr[NBUF][DR ? BN * DR * 2 : 16];
-  uint64_t bad[NBUF][NWV];
+  uint64_t bad[NBUF][8];
 };
 
-template <int IO, int D, int DR, int RT>
+template <int IO, int D, int DR, int NWV, int RT>
 __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
   constexpr int KSN = D / 16, KS = (D + DR) / 16, ON = D / 32, RB = D * 2;
   constexpr int ROWS = NWV * 32 * RT;
@@ -287,7 +286,9 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
     auto mask = [&](int u, int buf, int h, f32x16 (&sv)[RT]) __attribute__((always_inline)) {
       if (!is_mixed(u)) return;
       const int t0 = t_lo + u * BN + h * 32;
-      const uint64_t all = L.bad[buf][0] | L.bad[buf][1] | L.bad[buf][2] | L.bad[buf][3];
+      uint64_t all = 0;
+#pragma unroll
+      for (int w = 0; w < NWV; ++w) all |= L.bad[buf][w];
       const uint32_t bad = (uint32_t)(all >> (h * 32));
 #pragma unroll
       for (int m = 0; m < RT; ++m) {
@@ -319,7 +320,7 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
     // after them, each MFMA followed by a stage of this one's softmax. Fragments are read a few MFMAs ahead, past the
     // end of one product for the next.
     constexpr int NPV = 2 * ON, NM = (NPV + KS) * RT;
-    constexpr int VR = NPV < 4 ? NPV : 4, KR = KS < 4 ? KS : 4;
+    constexpr int RING = NWV == 8 ? 2 : 4, VR = NPV < RING ? NPV : RING, KR = KS < RING ? KS : RING;
     uint4 vfr[VR], kfr[KR];
     auto step = [&](auto pvc, auto sc, auto hc, f32x16 (&cur)[RT], f32x16 (&next)[RT], uint4 (&pb)[RT][2], uint4 (&pn)[RT][2],
                     auto&& between, auto&& ride) __attribute__((always_inline)) {
@@ -595,8 +596,9 @@ size_t workspace_bytes(const Cut& c, int d) {
 
 template <int IO, int D, int DR>
 hipError_t launch_d(const DenseK& k, const Cut& c, hipStream_t s) {
-  if (c.rt == 2) hipLaunchKernelGGL((dense_attn_kernel<IO, D, DR, 2>), dim3((unsigned)c.groups), dim3(NWV * 64), 0, s, k);
-  else hipLaunchKernelGGL((dense_attn_kernel<IO, D, DR, 1>), dim3((unsigned)c.groups), dim3(NWV * 64), 0, s, k);
+  // 256 rows: eight waves of 32, two a SIMD, or (192 wide scores: their queries leave no room for that) four of 64
+  if (c.rt == 2) hipLaunchKernelGGL((dense_attn_kernel<IO, D, DR, DR ? 4 : 8, DR ? 2 : 1>), dim3((unsigned)c.groups), dim3(DR ? 256 : 512), 0, s, k);
+  else hipLaunchKernelGGL((dense_attn_kernel<IO, D, DR, 4, 1>), dim3((unsigned)c.groups), dim3(256), 0, s, k);
   if (c.splits > 1) hipLaunchKernelGGL((dense_merge_kernel<IO, D>), dim3((unsigned)c.blocks), dim3(256), 0, s, k);
   return hipGetLastError();
 }
