@@ -46,7 +46,7 @@ struct GradK {
   const float* sm_max;
   const float* sm_sum;
   float* lse;              // [key heads][rows * per]: log2 of the sum of e^score, +inf for rows that see nothing
-  float* delta;
+  float* delta;            // -delta
   float* norms;            // fp16: [2][PREP] largest |dO|^2 and |v|^2
   uint16_t* dq;
   uint16_t* dqr;
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(256) void dense_prep_kernel(GradK a) {
     }
     if (c == 0) {
       a.lse[at] = l == 0.f ? INFINITY : m * LOG2E + log2f(l) - p_shift<IO>();
-      a.delta[at] = s;
+      a.delta[at] = -s;
     }
   }
   if constexpr (IO == IO_F16) {
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(256) void dense_prep_kernel(GradK a) {
 }
 
 // The factor of dS (a power of two) and the one that undoes it, by the whole work-group
-template <int IO>
+template <int IO, int NWV>
 __device__ __forceinline__ float2 ds_factor(const GradK& a, float (*red)[NWV]) {
   if constexpr (IO != IO_F16) return make_float2(1.f, 1.f);
   float m[2];
@@ -152,7 +152,11 @@ __device__ __forceinline__ float2 ds_factor(const GradK& a, float (*red)[NWV]) {
   }
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 2; ++w) m[w] = fmaxf(fmaxf(red[w][0], red[w][1]), fmaxf(red[w][2], red[w][3]));
+  for (int w = 0; w < 2; ++w) {
+    m[w] = red[w][0];
+#pragma unroll
+    for (int i = 1; i < NWV; ++i) m[w] = fmaxf(m[w], red[w][i]);
+  }
   // 2 |dO| |v| 2^e <= 2^15: 2^e = 2^floor(14 - log2(|dO| |v|)); no more than fp32's exponents hold
   const float e = floorf(14.f - 0.5f * (log2f(fmaxf(m[0], 1e-30f)) + log2f(fmaxf(m[1], 1e-30f))));
   const float f = exp2f(fminf(fmaxf(e, -100.f), 100.f));
@@ -195,16 +199,26 @@ __device__ __forceinline__ Place place_of(int i, int seqs, int heads, int splits
 }
 
 // ---------------------------------------------------------------- keys
+// Eight waves, two for each 32 of the 128 tokens: with one wave a SIMD, which issues an instruction every 8 cycles,
+// the products waited for the rest (32 rows took 2,400 cycles for 1,024 of MFMAs); one wave cannot have less than 192 registers of
+// dK, dV, K and V at D = 128, so the two split the products. The first makes S and P and adds to dV; the second takes P, in 32
+// bits, from LDS, makes dP and dS and adds to dK, one tile of 32 rows behind. Each adds the tile before while the VALU works on
+// the present one. Tiles lie in a ring of KRING, loaded two ahead; one barrier a tile.
+constexpr int KB = 32;      // rows of a tile
+constexpr int KRING = 5;
+constexpr int KW = 8;       // waves
+
 template <int D, int DR> struct KeyLds {
   struct {
-    uint8_t q[BN * D * 2];   // (d lies at a constant offset from q)
-    uint8_t d[BN * D * 2];
-  } t[NBUF];
-  uint8_t qr[NBUF][DR ? BN * DR * 2 : 16];
-  float lse[NBUF][BN];
-  float delta[NBUF][BN];
-  uint64_t bad[NBUF][NWV];
-  float red[2][NWV];
+    uint8_t q[KB * D * 2];   // (d lies at a constant offset from q)
+    uint8_t d[KB * D * 2];
+  } t[KRING];
+  uint8_t qr[KRING][DR ? KB * DR * 2 : 16];
+  float4 p[2][4][4][64];
+  float lse[KRING][64];     // (KB of them count: a wave loads 64)
+  float delta[KRING][64];
+  uint32_t bad[KRING][KW];
+  float red[2][KW];
 };
 
 __device__ __forceinline__ void lds_dma4(const void* gptr, void* lds_base) {
@@ -213,11 +227,14 @@ __device__ __forceinline__ void lds_dma4(const void* gptr, void* lds_base) {
 }
 
 template <int IO, int D, int DR>
-__global__ __launch_bounds__(NWV * 64) void dense_keys_kernel(GradK a) {
+__global__ __launch_bounds__(KW * 64) void dense_keys_kernel(GradK a) {
   constexpr int KSN = D / 16, KS = (D + DR) / 16, ON = D / 32, RN = DR / 32, RB = D * 2;
+  constexpr bool WIDE = RB == 256;   // a wave loads rows of q and of d, else of one of them
   __shared__ __attribute__((aligned(16))) KeyLds<D, DR> L;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kg = lane >> 5, rr = lane & 31;
+  const int pair = wave & 3;
+  const bool second = wave >= 4;
   const Place at = place_of(blockIdx.x, a.k_seqs, a.key_heads, a.k_splits, a.k_even, a.len.key_start, 1, [&](int b) {
     const Seq q = seq_of(a.len, b);
     return (q.keys + TOK - 1) / TOK;
@@ -225,334 +242,372 @@ __global__ __launch_bounds__(NWV * 64) void dense_keys_kernel(GradK a) {
   if (at.tile < 0) return;
   const int b = at.b, n = at.n;
   const Seq seq = seq_of(a.len, b);
-  const float2 factor = ds_factor<IO>(a, L.red);
+  const float2 factor = ds_factor<IO, KW>(a, L.red);
 
   const int t0 = at.tile * TOK, t_end = min(seq.keys, t0 + TOK), t_seen = min(t_end, seq.ak);
-  const int t = t0 + wave * 32 + rr;
+  const int t = t0 + pair * 32 + rr;
   // head rows [r_lo, r_hi) see some of these tokens, from r_full on all of them; this range's share
   const int r_end = seq.aq * a.per;
-  const int r_lo = max(first_query(a.len, seq, t0) * a.per, at.sp * a.k_chunk);
-  const int r_hi = at.sp == a.k_splits - 1 ? r_end : min(r_end, (at.sp + 1) * a.k_chunk);
-  const int r_full = t_seen > t0 ? first_query(a.len, seq, t_seen - 1) * a.per : 0;
+  const int r_lo = __builtin_amdgcn_readfirstlane(max(first_query(a.len, seq, t0) * a.per, at.sp * a.k_chunk));
+  const int r_hi = __builtin_amdgcn_readfirstlane(at.sp == a.k_splits - 1 ? r_end : min(r_end, (at.sp + 1) * a.k_chunk));
+  const int r_full = __builtin_amdgcn_readfirstlane(t_seen > t0 ? first_query(a.len, seq, t_seen - 1) * a.per : 0);
   const int my_first = t < t_seen ? first_query(a.len, seq, t) * a.per : INT_MAX;
-  const int ntiles = t_seen > t0 && r_hi > r_lo ? (r_hi - r_lo + BN - 1) / BN : 0;
+  const int ntiles = __builtin_amdgcn_readfirstlane(t_seen > t0 && r_hi > r_lo ? (r_hi - r_lo + KB - 1) / KB : 0);
 
-  f32x16 dk[ON + RN], dv[ON];
+  // The sums of this wave's N column tiles (none: zeros) go out: lane l has token t, columns c * 32 + 8 g + 4 kg + j
+  auto finish = [&](auto nc, const f32x16* acc, float f) __attribute__((always_inline)) {
+    constexpr int N = decltype(nc)::value;
+    if (a.k_splits > 1) {
+      const int blk = n * (a.k_blocks / a.key_heads) + seq.k0 / 32 + b + at.tile * 4 + pair;
+      if (t0 + pair * 32 >= seq.keys) return;
+      float4* dst = a.k_part + ((int64_t)at.sp * a.k_blocks + blk) * ((2 * D + DR) / 8) * 64 + (second ? 0 : (D + DR) / 8 * 64) + lane;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+      for (int c = 0; c < N; ++c)
 #pragma unroll
-    for (int c = 0; c < ON + RN; ++c) dk[c][i] = 0.f;
+        for (int g = 0; g < 4; ++g)
+          dst[(c * 4 + g) * 64] = make_float4(acc[c][4 * g] * f, acc[c][4 * g + 1] * f, acc[c][4 * g + 2] * f, acc[c][4 * g + 3] * f);
+      return;
+    }
+    const bool live = t < t_seen, valid = t < t_end;
+    const int64_t tt = (int64_t)(seq.k0 + t) * a.key_heads + n;
 #pragma unroll
-    for (int c = 0; c < ON; ++c) dv[c][i] = 0.f;
-  }
-
-  if (ntiles > 0) {
-    const float sl2 = a.scale * LOG2E;
-    // ---- tiles of head rows: each wave loads a share, in GPW loads. Where the group's heads divide the rows of one
-    // load of all waves, a lane's rows are of one head, and evenly spaced.
-    using Sh = Share<RB, BN, NWV>;
-    using ShR = Share<DR ? DR * 2 : 128, BN, NWV>;
-    const Sh sh(wave, lane);
-    const ShR shr(wave, lane);
-    constexpr int CQ = Sh::CNT, CR = DR ? ShR::CNT : 0, GPW = 2 * CQ + CR;
-    const uint16_t* const qb = a.q.p + (int64_t)seq.r0 * a.q.row + (int64_t)n * a.per * a.q.head;
-    const uint16_t* const db = a.d.p + (int64_t)seq.r0 * a.d.row + (int64_t)n * a.per * a.d.head;
-    const uint16_t* const qrb = DR ? a.qr.p + (int64_t)seq.r0 * a.qr.row + (int64_t)n * a.per * a.qr.head : nullptr;
-    auto place = [&](const Rows& x, int r) {   // of head row r, in bytes
-      const int s = row_div(a, r);
-      return ((int64_t)s * x.row + (int64_t)(r - s * a.per) * x.head) * 2;
-    };
-    const bool linear = a.linear;
-    const uint32_t q_off = linear ? (uint32_t)place(a.q, sh.row) + sh.col : 0, d_off = linear ? (uint32_t)place(a.d, sh.row) + sh.col : 0;
-    const uint32_t qr_off = DR && linear ? (uint32_t)place(a.qr, shr.row) + shr.col : 0;
-    const int per_shift = a.per_shift;   // (linear: per is a power of two)
-    const int64_t stat0 = n * (int64_t)a.len.rows * a.per + (int64_t)seq.r0 * a.per;
-    // load j of tile u (rows past the last repeat it; they are masked)
-    auto load_part = [&](auto jc, int u, int buf, bool fast) __attribute__((always_inline)) {
-      constexpr int j = decltype(jc)::value;
-      constexpr int what = j < CQ ? 0 : j < 2 * CQ ? 1 : 2, i = what == 0 ? j : what == 1 ? j - CQ : j - 2 * CQ;
-      constexpr int step = i * (what == 2 ? ShR::STEP : Sh::STEP);
-      const int r0 = r_lo + u * BN;
-      const Rows& x = what == 0 ? a.q : what == 1 ? a.d : a.qr;
-      const char* p = reinterpret_cast<const char*>(what == 0 ? qb : what == 1 ? db : qrb);
-      uint8_t* dst = (what == 0 ? L.t[buf].q : what == 1 ? L.t[buf].d : L.qr[buf]) + (i * NWV + wave) * 1024;
-      if (fast) {
-        lds_dma16_sbase_untracked(p + (int64_t)((r0 + step) >> per_shift) * x.row * 2, what == 0 ? q_off : what == 1 ? d_off : qr_off, dst);
-      } else {
-        const int r = min(r0 + step + (what == 2 ? shr.row : sh.row), r_hi - 1);
-        lds_dma16_untracked(p + place(x, r) + (what == 2 ? shr.col : sh.col), dst);
+    for (int c = 0; c < N; ++c) {
+      uint4 w[2];
+      pack_tile<IO>(acc[c], f, w);
+      uint16_t* dst = (c >= ON ? a.dkr + tt * DR + (c - ON) * 32 : (second ? a.dk : a.dv) + tt * D + c * 32) + 8 * kg;
+      if (valid) {
+        stg16(dst, live ? w[0] : make_uint4(0, 0, 0, 0));
+        stg16(dst + 16, live ? w[1] : make_uint4(0, 0, 0, 0));
       }
-    };
-    auto load_stats = [&](int u, int buf) __attribute__((always_inline)) {
-      const int64_t r = stat0 + min(r_lo + u * BN + lane, r_hi - 1);
-      if (wave == 0) lds_dma4(a.lse + r, L.lse[buf]);
-      if (wave == 1) lds_dma4(a.delta + r, L.delta[buf]);
-    };
-    auto load_tile = [&](int u, int buf) __attribute__((always_inline)) {
-      static_for<0, GPW>([&](auto j) __attribute__((always_inline)) { load_part(j, u, buf, false); });
-      load_stats(u, buf);
-    };
-    // (a masked pair has P = dS = 0, but 0 times a value that is not finite would reach tokens that the row does not see)
-    auto is_mixed = [&](int u) { return r_lo + u * BN < r_full || r_lo + u * BN + BN > r_hi; };
-    auto sanitize = [&](int u, int buf) __attribute__((always_inline)) {
-      if (!is_mixed(u)) return;
-      uint64_t bad = clean_share<IO, RB, BN, NWV>(lds_addr(L.t[buf].q), wave, lane) |
-                     clean_share<IO, RB, BN, NWV>(lds_addr(L.t[buf].d), wave, lane);
-      if constexpr (DR > 0) bad |= clean_share<IO, 128, BN, NWV>(lds_addr(L.qr[buf]), wave, lane);
-      if (lane == 0) L.bad[buf][wave] = bad;
-    };
-    load_tile(0, 0);
-    uint4 kf[KS], vf[KSN];
-    {
-      const int64_t tt = seq.k0 + min(t, t_seen - 1);
-      const uint16_t* kp = a.k.p + tt * a.k.row + n * a.k.head + kg * 8;
-      const uint16_t* vp = a.v.p + tt * a.v.row + n * a.v.head + kg * 8;
-#pragma unroll
-      for (int j = 0; j < KSN; ++j) kf[j] = ldg16(kp + j * 16), vf[j] = ldg16(vp + j * 16);
-      if constexpr (DR > 0) {
-        const uint16_t* rp = a.kr.p + tt * a.kr.row + n * a.kr.head + kg * 8;
-#pragma unroll
-        for (int j = KSN; j < KS; ++j) kf[j] = ldg16(rp + (j - KSN) * 16);
-      }
-#pragma unroll
-      for (int j = 0; j < KS; ++j) kf[j] = in_agprs(kf[j]);
-#pragma unroll
-      for (int j = 0; j < KSN; ++j) vf[j] = in_agprs(vf[j]);
-    }
-
-    // ---- operands
-    constexpr int DOFF = BN * D * 2;   // from a place in q to the same in d
-    const int qk = s_row(rr), g16 = lane >> 4, c16 = lane & 15;
-    const int r4 = (g16 >> 1) * 8 + (c16 >> 2), vc = (g16 & 1) * 2 + ((c16 & 3) >> 1), o8 = (c16 & 1) * 8;
-    const uint32_t op_lane = tile_off<RB>(qk, kg), opr_lane = tile_off<128>(qk, kg);
-    const uint32_t tr_lo = tile_off<RB>(r4, vc) + o8, tr_hi = tile_off<RB>(r4 + 4, vc) + o8;
-    const uint32_t trr_lo = tile_off<128>(r4, vc) + o8, trr_hi = tile_off<128>(r4 + 4, vc) + o8;
-    OpAddr<RB> op;
-    OpAddr<128> opr;
-    TrAddr<RB> tr;
-    TrAddr<128> trr;
-    auto point_op = [&](int buf) __attribute__((always_inline)) {
-      op.point(lds_addr(L.t[buf].q), op_lane);
-      if constexpr (DR > 0) opr.point(lds_addr(L.qr[buf]), opr_lane);
-    };
-    auto point_tr = [&](int buf) __attribute__((always_inline)) {
-      tr.point(lds_addr(L.t[buf].q), tr_lo, tr_hi);
-      if constexpr (DR > 0) trr.point(lds_addr(L.qr[buf]), trr_lo, trr_hi);
-    };
-    auto q_frag = [&](int j, int h) __attribute__((always_inline)) -> uint4 {
-      return lds_read16_at(j < KSN ? op.a[j < KSN ? j : 0] + h * 32 * RB : opr.a[j >= KSN ? j - KSN : 0] + h * 32 * 128);
-    };
-    auto d_frag = [&](int j, int h) __attribute__((always_inline)) -> uint4 { return lds_read16_at(op.a[j] + h * 32 * RB + DOFF); };
-    // product i of a half's NP: column tiles of dV, dK and dK's rotary part for 16 rows, then for the next 16
-    constexpr int NC = 2 * ON + RN, NP = 2 * NC;
-    auto t_frag = [&](int i, int h) __attribute__((always_inline)) -> uint4 {
-      const int st = i / NC, c = i % NC;
-      if (c < ON) return tr.frag(c < ON ? c : 0, (h * 32 + st * 16) * RB + DOFF);
-      if (c < 2 * ON) return tr.frag(c >= ON && c < 2 * ON ? c - ON : 0, (h * 32 + st * 16) * RB);
-      return trr.frag(c >= 2 * ON ? c - 2 * ON : 0, (h * 32 + st * 16) * 128);
-    };
-
-    // ---- P and dS of 32 rows in NST stages of two rows each, placed among the products before and after them
-    constexpr int NST = 8;
-    float4 lse4[4], del4[4];   // rows 16 x + 8 kg + 4 y + 0 .. 3 at [2 x + y]
-    auto stats = [&](int buf, int h) __attribute__((always_inline)) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int at = h * 32 + 16 * (e >> 1) + 8 * kg + 4 * (e & 1);
-        lse4[e] = *reinterpret_cast<const float4*>(&L.lse[buf][at]);
-        del4[e] = *reinterpret_cast<const float4*>(&L.delta[buf][at]);
-      }
-    };
-    const float f16 = factor.x * 0x1p-15f;   // (fp16's P has the factor 2^15)
-    auto stage = [&](int st, f32x16& sv, f32x16& dp, uint32_t (&pw)[8], uint32_t (&sw)[8]) __attribute__((always_inline)) {
-      const int i = 2 * st;
-      const float4 l4 = lse4[i >> 2], d4 = del4[i >> 2];
-      const float l0 = i & 2 ? l4.z : l4.x, l1 = i & 2 ? l4.w : l4.y, e0 = i & 2 ? d4.z : d4.x, e1 = i & 2 ? d4.w : d4.y;
-      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], sl2, -l0));
-      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i + 1], sl2, -l1));
-      float w0 = p0 * (dp[i] - e0), w1 = p1 * (dp[i + 1] - e1);
-      if constexpr (IO == IO_F16) w0 *= f16, w1 *= f16;
-      pw[st] = pack2<IO>(p0, p1);
-      sw[st] = pack2<IO>(w0, w1);
-      asm volatile("" : "+v"(pw[st]), "+v"(sw[st]));   // here, not where the next step needs them
-    };
-    auto mask = [&](int u, int buf, int h, uint32_t (&pw)[8], uint32_t (&sw)[8]) __attribute__((always_inline)) {
-      if (!is_mixed(u)) return;
-      const uint64_t all = L.bad[buf][0] | L.bad[buf][1] | L.bad[buf][2] | L.bad[buf][3];
-      const uint32_t bad = (uint32_t)(all >> (h * 32));
-      const int r0 = r_lo + u * BN + h * 32, first = my_first - r0, last = r_hi - r0;   // rows [first, last) see the token
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int x = s_token(2 * i, kg);
-        const uint32_t nan = ((bad >> x) & 1u ? 0x7FFFu : 0u) | ((bad >> (x + 1)) & 1u ? 0x7FFF0000u : 0u);
-        const uint32_t keep = (x >= first && x < last ? 0xFFFFu : 0u) | (x + 1 >= first && x + 1 < last ? 0xFFFF0000u : 0u);
-        pw[i] = (pw[i] | nan) & keep;
-        sw[i] = (sw[i] | nan) & keep;
-      }
-    };
-
-    // ---- One step handles 32 rows: the products of the rows before them, S and dP of the rows after them, each MFMA
-    // followed by a part of this one's P and dS. Fragments are read a few MFMAs ahead.
-    constexpr int LAG = KS - KSN, NS = KS + KSN;   // S and dP end together
-    constexpr int TR = 4, QR = 4, DRING = 4;
-    uint4 tf[TR], qf[QR], df[DRING];
-    auto step = [&](auto pvc, auto sc, auto hc, f32x16& cs, f32x16& cd, f32x16& ns, f32x16& nd, uint32_t (&pb)[8], uint32_t (&sb)[8],
-                    uint32_t (&pn)[8], uint32_t (&sn)[8], auto&& between, auto&& ride) __attribute__((always_inline)) {
-      constexpr bool PV = decltype(pvc)::value, S = decltype(sc)::value;
-      constexpr int H = decltype(hc)::value;
-      constexpr int M0 = PV ? NP : 0, NMM = M0 + (S ? NS : 0), LEAD = NMM > 8 ? 2 : 0;
-      auto values_at = [&](int slot) __attribute__((always_inline)) {
-#pragma unroll
-        for (int st = 0; st < NST; ++st)
-          if (LEAD + st * (NMM - LEAD) / NST == slot) stage(st, cs, cd, pn, sn);
-      };
-      if constexpr (PV)
-        static_for<0, NP>([&](auto ic) __attribute__((always_inline)) {
-          constexpr int i = decltype(ic)::value, st = i / NC, c = i % NC;
-          const uint4 b = c < ON ? make_uint4(pb[4 * st], pb[4 * st + 1], pb[4 * st + 2], pb[4 * st + 3])
-                                 : make_uint4(sb[4 * st], sb[4 * st + 1], sb[4 * st + 2], sb[4 * st + 3]);
-          if constexpr (c < ON) dv[c] = Mfma<IO>::m32(tf[i % TR], b, dv[c]);
-          else dk[c - ON] = Mfma<IO>::m32(tf[i % TR], b, dk[c - ON]);
-          if constexpr (i + TR < NP) tf[i % TR] = t_frag(i + TR, H);
-          if constexpr (S && i < QR) qf[i] = q_frag(i, H);
-          if constexpr (S && i >= QR && i < QR + DRING) df[i - QR] = d_frag(i - QR, H);
-          values_at(i);
-          __builtin_amdgcn_sched_barrier(0);
-        });
-      between();
-      if constexpr (S)
-        static_for<0, NS>([&](auto jc) __attribute__((always_inline)) {
-          constexpr int j = decltype(jc)::value;
-          constexpr bool is_s = j < LAG || (j - LAG) % 2 == 0;
-          constexpr int i = j < LAG ? j : is_s ? LAG + (j - LAG) / 2 : (j - LAG) / 2;   // step of its chain
-          if constexpr (j == NS - 1) mfma32_va_end2<IO>(ns, qf[(KS - 1) % QR], kf[KS - 1], nd, df[(KSN - 1) % DRING], vf[KSN - 1]);
-          else if constexpr (is_s && i < KS - 1) {
-            mfma32_va<IO, i == 0>(ns, qf[i % QR], kf[i]);
-            if constexpr (i + QR < KS) qf[i % QR] = q_frag(i + QR, H);
-          } else if constexpr (!is_s) {
-            mfma32_va<IO, i == 0>(nd, df[i % DRING], vf[i]);
-            if constexpr (i + DRING < KSN) df[i % DRING] = d_frag(i + DRING, H);
-          }
-          if constexpr (j >= NS - TR) tf[j - (NS - TR)] = t_frag(j - (NS - TR), 1 - H);
-          ride(jc);
-          values_at(M0 + j);
-          __builtin_amdgcn_sched_barrier(0);
-        });
-    };
-    std::true_type yes;
-    std::false_type no;
-    std::integral_constant<int, 0> h0;
-    std::integral_constant<int, 1> h1;
-    auto nothing = [](auto...) __attribute__((always_inline)) {};
-
-    wait_vmcnt<0>();
-    asm volatile("" ::: "memory");
-    sanitize(0, 0);
-    lds_barrier();
-    if (ntiles > 1) load_tile(1, 1);
-    f32x16 s0, s1, d0, d1;
-    uint32_t p0[8], p1[8], w0[8], w1[8];
-    point_op(0);
-#pragma unroll
-    for (int j = 0; j < KS - 1; ++j) {
-      const uint4 f = q_frag(j, 0);
-      if (j == 0) mfma32_va<IO, true>(s0, f, kf[j]);
-      else mfma32_va<IO, false>(s0, f, kf[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < KSN - 1; ++j) {
-      const uint4 f = d_frag(j, 0);
-      if (j == 0) mfma32_va<IO, true>(d0, f, vf[j]);
-      else mfma32_va<IO, false>(d0, f, vf[j]);
-    }
-    mfma32_va_end2<IO>(s0, q_frag(KS - 1, 0), kf[KS - 1], d0, d_frag(KSN - 1, 0), vf[KSN - 1]);
-#pragma unroll
-    for (int j = 0; j < QR; ++j) qf[j] = q_frag(j, 1);
-#pragma unroll
-    for (int j = 0; j < DRING; ++j) df[j] = d_frag(j, 1);
-    int buf = 0;   // of tile u
-    // Step (u, 0): tile u + 1 has landed by the middle of it, when nobody needs tile u - 1 any more
-    auto half0 = [&](auto pvc, int u) __attribute__((always_inline)) {
-      const int nb = buf == NBUF - 1 ? 0 : buf + 1, lb = buf == 0 ? NBUF - 1 : buf - 1;   // of tiles u + 1 and u - 1 (u + 2)
-      stats(buf, 0);
-      const bool more = u + 2 < ntiles, fast = linear && r_lo + (u + 3) * BN <= r_hi;
-      step(pvc, yes, h1, s0, d0, s1, d1, p1, w1, p0, w0,
-           [&]() __attribute__((always_inline)) {
-             wait_vmcnt<0>();
-             asm volatile("" ::: "memory");
-             if (u + 1 < ntiles) sanitize(u + 1, nb);
-             lds_barrier();
-             point_tr(buf);
-           },
-           [&](auto jc) __attribute__((always_inline)) {
-             constexpr int j = decltype(jc)::value;
-             static_for<0, GPW>([&](auto g) __attribute__((always_inline)) {
-               if constexpr (g * NS / GPW == j)
-                 if (more) load_part(g, u + 2, lb, fast);
-             });
-             if constexpr (j == NS - 1)
-               if (more) load_stats(u + 2, lb);
-           });
-      mask(u, buf, 0, p0, w0);
-    };
-    half0(no, 0);
-    for (int uv = 0; uv + 1 < ntiles; ++uv) {
-      const int u = __builtin_amdgcn_readfirstlane(uv);
-      const int nb = buf == NBUF - 1 ? 0 : buf + 1;
-      point_op(nb);
-      stats(buf, 1);
-      step(yes, yes, h0, s1, d1, s0, d0, p0, w0, p1, w1, nothing, nothing);
-      mask(u, buf, 1, p1, w1);
-      buf = nb;
-      half0(yes, u + 1);
-    }
-    stats(buf, 1);
-    step(yes, no, h0, s1, d1, s0, d0, p0, w0, p1, w1, nothing, nothing);
-    mask(ntiles - 1, buf, 1, p1, w1);
-#pragma unroll
-    for (int i = 0; i < TR; ++i) tf[i] = t_frag(i, 1);
-    static_for<0, NP>([&](auto ic) __attribute__((always_inline)) {
-      constexpr int i = decltype(ic)::value, st = i / NC, c = i % NC;
-      const uint4 b = c < ON ? make_uint4(p1[4 * st], p1[4 * st + 1], p1[4 * st + 2], p1[4 * st + 3])
-                             : make_uint4(w1[4 * st], w1[4 * st + 1], w1[4 * st + 2], w1[4 * st + 3]);
-      if constexpr (c < ON) dv[c] = Mfma<IO>::m32(tf[i % TR], b, dv[c]);
-      else dk[c - ON] = Mfma<IO>::m32(tf[i % TR], b, dk[c - ON]);
-      if constexpr (i + TR < NP) tf[i % TR] = t_frag(i + TR, 1);
-    });
-  }
-
-  // lane l: token t, columns c * 32 + 8 g + 4 kg + j
-  const float fk = a.scale * factor.y, fv = IO == IO_F16 ? 0x1p-15f : 1.f;
-  if (a.k_splits > 1) {
-    const int blk = n * (a.k_blocks / a.key_heads) + seq.k0 / 32 + b + at.tile * NWV + wave;
-    if (t0 + wave * 32 >= seq.keys) return;
-    float4* dst = a.k_part + ((int64_t)at.sp * a.k_blocks + blk) * ((2 * D + DR) / 8) * 64 + lane;
-#pragma unroll
-    for (int c = 0; c < ON + RN + ON; ++c) {
-      const f32x16& v = c < ON + RN ? dk[c < ON + RN ? c : 0] : dv[c >= ON + RN ? c - ON - RN : 0];
-      const float f = c < ON + RN ? fk : fv;
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        dst[(c * 4 + g) * 64] = make_float4(v[4 * g] * f, v[4 * g + 1] * f, v[4 * g + 2] * f, v[4 * g + 3] * f);
-    }
-    return;
-  }
-  const bool live = t < t_seen, valid = t < t_end;
-  const int64_t tt = (int64_t)(seq.k0 + t) * a.key_heads + n;
-  auto store = [&](const f32x16& v, float f, uint16_t* dst) __attribute__((always_inline)) {
-    uint4 w[2];
-    pack_tile<IO>(v, f, w);
-    if (valid) {
-      stg16(dst + 8 * kg, live ? w[0] : make_uint4(0, 0, 0, 0));
-      stg16(dst + 8 * kg + 16, live ? w[1] : make_uint4(0, 0, 0, 0));
     }
   };
+  constexpr int AN = ON + RN;   // the second wave's dK; the first one's dV has ON
+  std::integral_constant<int, ON> n_dv;
+  std::integral_constant<int, AN> n_dk;
+  if (ntiles == 0) {
+    f32x16 zero[AN];
 #pragma unroll
-  for (int c = 0; c < ON; ++c) store(dk[c], fk, a.dk + tt * D + c * 32);
+    for (int c = 0; c < AN; ++c)
 #pragma unroll
-  for (int c = 0; c < RN; ++c) store(dk[ON + c], fk, a.dkr + tt * DR + c * 32);
+      for (int i = 0; i < 16; ++i) zero[c][i] = 0.f;
+    if (second) finish(n_dk, zero, 0.f);
+    else finish(n_dv, zero, 0.f);
+    return;
+  }
+  const float sl2 = a.scale * LOG2E;
+  // ---- tiles of head rows. Where the group's heads divide 16, a lane's rows are of one head, and evenly spaced.
+  using Sh = Share<RB, KB, WIDE ? KW : 4>;
+  using ShR = Share<128, KB, 4>;
+  const int lw = WIDE ? wave : pair;
+  const Sh sh(lw, lane);
+  const ShR shr(pair, lane);
+  auto place = [&](const Rows& x, int r) {   // of head row r, in bytes
+    const int s = row_div(a, r);
+    return ((int64_t)s * x.row + (int64_t)(r - s * a.per) * x.head) * 2;
+  };
+  auto base_of = [&](const Rows& x) {
+    return reinterpret_cast<const char*>(x.p + (int64_t)seq.r0 * x.row + (int64_t)n * a.per * x.head);
+  };
+  const char* const qb = base_of(a.q);
+  const char* const db = base_of(a.d);
+  const char* const qrb = DR ? base_of(a.qr) : nullptr;
+  const bool linear = a.linear;
+  const uint32_t q_off = linear ? (uint32_t)place(a.q, sh.row) + sh.col : 0, d_off = linear ? (uint32_t)place(a.d, sh.row) + sh.col : 0;
+  const uint32_t qr_off = DR && linear ? (uint32_t)place(a.qr, shr.row) + shr.col : 0;
+  const int64_t stat0 = n * (int64_t)a.len.rows * a.per + (int64_t)seq.r0 * a.per;
+  // this wave's loads of tile u (rows past the last repeat it; they are masked), and how many they are
+  auto load_rows = [&](const Rows& x, const char* p, uint32_t off, int row, uint32_t col, int r0, void* dst) __attribute__((always_inline)) {
+    if (linear && r0 + KB <= r_hi) lds_dma16_sbase_untracked(p + (int64_t)(r0 >> a.per_shift) * x.row * 2, off, dst);
+    else lds_dma16_untracked(p + place(x, min(r0 + row, r_hi - 1)) + col, dst);
+  };
+  auto load_tile = [&](int u, int buf) __attribute__((always_inline)) {
+    const int r0 = r_lo + u * KB;
+    if (WIDE || !second) load_rows(a.q, qb, q_off, sh.row, sh.col, r0, L.t[buf].q + lw * 1024);
+    if (WIDE || second) load_rows(a.d, db, d_off, sh.row, sh.col, r0, L.t[buf].d + lw * 1024);
+    if constexpr (DR > 0)
+      if (!second) load_rows(a.qr, qrb, qr_off, shr.row, shr.col, r0, L.qr[buf] + pair * 1024);
+    if (pair == 0) {
+      const int64_t r = stat0 + min(r0 + lane, r_hi - 1);
+      if (second) lds_dma4(a.delta + r, L.delta[buf]);
+      else lds_dma4(a.lse + r, L.lse[buf]);
+    }
+  };
+  const int loads = (WIDE ? 2 : 1) + (DR > 0 && !second ? 1 : 0) + (pair == 0 ? 1 : 0);
+  // (a masked pair has P = dS = 0, but 0 times a value that is not finite would reach tokens that the row does not see)
+  auto is_mixed = [&](int u) { return r_lo + u * KB < r_full || r_lo + u * KB + KB > r_hi; };
+  auto sanitize = [&](int u, int buf) __attribute__((always_inline)) {
+    if (!is_mixed(u)) return;
+    uint32_t bad = 0;
+    if (WIDE || !second) bad |= (uint32_t)clean_share<IO, RB, KB, WIDE ? KW : 4>(lds_addr(L.t[buf].q), lw, lane);
+    if (WIDE || second) bad |= (uint32_t)clean_share<IO, RB, KB, WIDE ? KW : 4>(lds_addr(L.t[buf].d), lw, lane);
+    if constexpr (DR > 0)
+      if (!second) bad |= (uint32_t)clean_share<IO, 128, KB, 4>(lds_addr(L.qr[buf]), pair, lane);
+    if (lane == 0) L.bad[buf][wave] = bad;
+  };
+  auto next = [](int buf) { return buf == KRING - 1 ? 0 : buf + 1; };
+  auto before = [](int buf) { return buf == 0 ? KRING - 1 : buf - 1; };
+  // The beginning of phase u: tile u is in LDS for everyone, and tile u - 3 done with
+  int buf = 0;   // of tile u
+  auto begin = [&](int u) __attribute__((always_inline)) {
+    if (u < ntiles) {
+      if (u + 1 >= ntiles) wait_vmcnt<0>();
+      else if (loads == 1) wait_vmcnt<1>();
+      else if (loads == 2) wait_vmcnt<2>();
+      else if (loads == 3) wait_vmcnt<3>();
+      else wait_vmcnt<4>();
+      asm volatile("" ::: "memory");
+      sanitize(u, buf);
+    }
+    lds_barrier();
+    if (u + 2 < ntiles) load_tile(u + 2, next(next(buf)));
+  };
+  auto bad_rows = [&](int buf) {
+    uint32_t bad = 0;
 #pragma unroll
-  for (int c = 0; c < ON; ++c) store(dv[c], fv, a.dv + tt * D + c * 32);
+    for (int w = 0; w < KW; ++w) bad |= L.bad[buf][w];
+    return bad;
+  };
+
+  load_tile(0, 0);
+  if (ntiles > 1) load_tile(1, 1);
+  uint4 opf[KS];   // this wave's K (first) or V (second)
+  {
+    const int64_t tt = seq.k0 + min(t, t_seen - 1);
+    const Rows& x = second ? a.v : a.k;
+    const uint16_t* p = x.p + tt * x.row + n * x.head + kg * 8;
+#pragma unroll
+    for (int j = 0; j < KSN; ++j) opf[j] = ldg16(p + j * 16);
+    if constexpr (DR > 0)
+      if (!second) {
+        const uint16_t* rp = a.kr.p + tt * a.kr.row + n * a.kr.head + kg * 8;
+#pragma unroll
+        for (int j = KSN; j < KS; ++j) opf[j] = ldg16(rp + (j - KSN) * 16);
+      }
+  }
+
+  // ---- operands
+  constexpr int DOFF = KB * D * 2;   // from a place in q to the same in d
+  const int qk = s_row(rr), g16 = lane >> 4, c16 = lane & 15;
+  const int r4 = (g16 >> 1) * 8 + (c16 >> 2), vc = (g16 & 1) * 2 + ((c16 & 3) >> 1), o8 = (c16 & 1) * 8;
+  const uint32_t op_lane = tile_off<RB>(qk, kg), opr_lane = tile_off<128>(qk, kg);
+  const uint32_t tr_lo = tile_off<RB>(r4, vc) + o8, tr_hi = tile_off<RB>(r4 + 4, vc) + o8;
+  const uint32_t trr_lo = tile_off<128>(r4, vc) + o8, trr_hi = tile_off<128>(r4 + 4, vc) + o8;
+  OpAddr<RB> op;
+  OpAddr<128> opr;
+  TrAddr<RB> tr;
+  TrAddr<128> trr;
+  constexpr int OR = 4, TR = 4;
+  std::true_type yes;
+  std::false_type no;
+  uint32_t words[8];   // the tile before: P (first) or dS (second)
+
+  if (!second) {
+#pragma unroll
+    for (int j = 0; j < KS; ++j) opf[j] = in_agprs(opf[j]);
+    f32x16 acc[ON];
+#pragma unroll
+    for (int c = 0; c < ON; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[c][i] = 0.f;
+    // phase u: S of tile u, dV of tile u - 1, P of tile u
+    auto phase = [&](auto sc, auto vc, int u) __attribute__((always_inline)) {
+      constexpr bool S = decltype(sc)::value, DV = decltype(vc)::value;
+      f32x16 s;
+      float4 lse4[4];
+      uint4 of[OR], tf[TR];
+      if constexpr (S) {
+        op.point(lds_addr(L.t[buf].q), op_lane);
+        if constexpr (DR > 0) opr.point(lds_addr(L.qr[buf]), opr_lane);
+      }
+      auto q_frag = [&](int j) __attribute__((always_inline)) -> uint4 {
+        return lds_read16_at(j < KSN ? op.a[j < KSN ? j : 0] : opr.a[j >= KSN ? j - KSN : 0]);
+      };
+      auto t_frag = [&](int i) __attribute__((always_inline)) -> uint4 { return tr.frag(i % ON, (i / ON) * 16 * RB + DOFF); };
+      if constexpr (S) {
+#pragma unroll
+        for (int j = 0; j < OR; ++j) of[j] = q_frag(j);
+      }
+      if constexpr (DV) tr.point(lds_addr(L.t[before(buf)].q), tr_lo, tr_hi);
+      if constexpr (S) {
+        static_for<0, KS>([&](auto jc) __attribute__((always_inline)) {
+          constexpr int j = decltype(jc)::value;
+          if constexpr (j < KS - 1) mfma32_va<IO, j == 0>(s, of[j % OR], opf[j]);
+          else mfma32_va_last<IO>(s, of[j % OR], opf[j]);
+          if constexpr (j + OR < KS) of[j % OR] = q_frag(j + OR);
+          if constexpr (j >= KS - 4) lse4[j - (KS - 4)] = *reinterpret_cast<const float4*>(
+              &L.lse[buf][16 * ((j - (KS - 4)) >> 1) + 8 * kg + 4 * ((j - (KS - 4)) & 1)]);
+          if constexpr (DV && j >= KS - TR && j - (KS - TR) < 2 * ON) tf[j - (KS - TR)] = t_frag(j - (KS - TR));
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      } else {
+#pragma unroll
+        for (int i = 0; i < TR; ++i) tf[i] = t_frag(i);
+      }
+      auto exps = [&](int e) __attribute__((always_inline)) {   // two rows
+        const float4 l = lse4[e >> 1];
+        s[2 * e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e], sl2, -(e & 1 ? l.z : l.x)));
+        s[2 * e + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e + 1], sl2, -(e & 1 ? l.w : l.y)));
+      };
+      if constexpr (DV)
+        static_for<0, 2 * ON>([&](auto ic) __attribute__((always_inline)) {
+          constexpr int i = decltype(ic)::value, st = i / ON;
+          acc[i % ON] = Mfma<IO>::m32(tf[i % TR], make_uint4(words[4 * st], words[4 * st + 1], words[4 * st + 2], words[4 * st + 3]), acc[i % ON]);
+          if constexpr (i + TR < 2 * ON) tf[i % TR] = t_frag(i + TR);
+          if constexpr (S)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (e * 2 * ON / 8 == i) exps(e);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      else if constexpr (S)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) exps(e);
+      if constexpr (S) {
+        if (is_mixed(u)) {
+          int k = kg;
+          asm volatile("" : "+v"(k));   // (what follows from it is not kept in registers for these few tiles)
+          const uint32_t bad = bad_rows(buf);
+          const int r0 = r_lo + u * KB, first = my_first - r0, last = r_hi - r0;   // rows [first, last) see the token
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int x = s_token(i, k);
+            if ((bad >> x) & 1u) s[i] = __builtin_nanf("");
+            if (x < first || x >= last) s[i] = 0.f;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) L.p[u & 1][pair][e][lane] = make_float4(s[4 * e], s[4 * e + 1], s[4 * e + 2], s[4 * e + 3]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) words[e] = pack2<IO>(s[2 * e], s[2 * e + 1]);
+      }
+#pragma unroll
+      for (int c = 0; c < ON; ++c) asm volatile("" : "+a"(acc[c]));   // whole accumulators, in AGPRs, from phase to phase
+      buf = next(buf);
+    };
+    begin(0);
+    phase(yes, no, 0);
+    if (ntiles > 1) {
+      int u = 1;
+      do {
+        u = __builtin_amdgcn_readfirstlane(u);
+        begin(u);
+        phase(yes, yes, u);
+      } while (++u < ntiles);
+    }
+    begin(ntiles);
+    phase(no, yes, ntiles);
+    begin(ntiles + 1);
+    finish(n_dv, acc, IO == IO_F16 ? 0x1p-15f : 1.f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < KSN; ++j) opf[j] = in_agprs(opf[j]);
+    const float f16 = factor.x * 0x1p-15f;   // (fp16's P has the factor 2^15)
+    f32x16 acc[AN];
+#pragma unroll
+    for (int c = 0; c < AN; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[c][i] = 0.f;
+    // phase u: dP and dS of tile u - 1, dK of tile u - 2
+    auto phase = [&](auto sc, auto kc, int u) __attribute__((always_inline)) {
+      constexpr bool S = decltype(sc)::value, DK = decltype(kc)::value;
+      constexpr int NC = ON + RN, NP = 2 * NC;
+      const int vb = before(buf), kb = before(vb);
+      f32x16 d;
+      float4 p4[4];
+      uint4 of[OR], tf[TR];
+      auto d_frag = [&](int j) __attribute__((always_inline)) -> uint4 { return lds_read16_at(op.a[j] + DOFF); };
+      auto t_frag = [&](int i) __attribute__((always_inline)) -> uint4 {
+        const int st = i / NC, c = i % NC;
+        if (c < ON) return tr.frag(c < ON ? c : 0, st * 16 * RB);
+        return trr.frag(c >= ON ? c - ON : 0, st * 16 * 128);
+      };
+      if constexpr (S) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {   // dP - delta
+          const float4 v = *reinterpret_cast<const float4*>(&L.delta[vb][16 * (e >> 1) + 8 * kg + 4 * (e & 1)]);
+          d[4 * e] = v.x, d[4 * e + 1] = v.y, d[4 * e + 2] = v.z, d[4 * e + 3] = v.w;
+        }
+        op.point(lds_addr(L.t[vb].q), op_lane);
+#pragma unroll
+        for (int j = 0; j < OR; ++j) of[j] = d_frag(j);
+      }
+      if constexpr (DK) {
+        tr.point(lds_addr(L.t[kb].q), tr_lo, tr_hi);
+        if constexpr (DR > 0) trr.point(lds_addr(L.qr[kb]), trr_lo, trr_hi);
+      }
+      if constexpr (S) {
+        static_for<0, KSN>([&](auto jc) __attribute__((always_inline)) {
+          constexpr int j = decltype(jc)::value;
+          if constexpr (j < KSN - 1) mfma32_va<IO, false>(d, of[j % OR], opf[j]);
+          else mfma32_va_last<IO>(d, of[j % OR], opf[j]);
+          if constexpr (j + OR < KSN) of[j % OR] = d_frag(j + OR);
+          if constexpr (j >= KSN - 4) p4[j - (KSN - 4)] = L.p[(u - 1) & 1][pair][j - (KSN - 4)][lane];
+          if constexpr (DK && j >= KSN - TR) tf[j - (KSN - TR)] = t_frag(j - (KSN - TR));
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      } else {
+#pragma unroll
+        for (int i = 0; i < TR; ++i) tf[i] = t_frag(i);
+      }
+      uint32_t fresh[8];
+      auto values = [&](int e) __attribute__((always_inline)) {   // two rows
+        const float4 p = p4[e >> 1];
+        float x = (e & 1 ? p.z : p.x) * d[2 * e], y = (e & 1 ? p.w : p.y) * d[2 * e + 1];
+        if constexpr (IO == IO_F16) x *= f16, y *= f16;
+        fresh[e] = pack2<IO>(x, y);
+        asm volatile("" : "+v"(fresh[e]));   // here, not where the next phase needs it
+      };
+      if constexpr (DK)
+        static_for<0, NP>([&](auto ic) __attribute__((always_inline)) {
+          constexpr int i = decltype(ic)::value, st = i / NC, c = i % NC;
+          acc[c] = Mfma<IO>::m32(tf[i % TR], make_uint4(words[4 * st], words[4 * st + 1], words[4 * st + 2], words[4 * st + 3]), acc[c]);
+          if constexpr (i + TR < NP) tf[i % TR] = t_frag(i + TR);
+          if constexpr (S)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (e * NP / 8 == i) values(e);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      else if constexpr (S)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) values(e);
+      if constexpr (S) {
+        if (is_mixed(u - 1)) {
+          int k = kg;
+          asm volatile("" : "+v"(k));   // (what follows from it is not kept in registers for these few tiles)
+          const uint32_t bad = bad_rows(vb);
+          const int r0 = r_lo + (u - 1) * KB, first = my_first - r0, last = r_hi - r0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int x = s_token(2 * e, k);
+            const uint32_t nan = ((bad >> x) & 1u ? 0x7FFFu : 0u) | ((bad >> (x + 1)) & 1u ? 0x7FFF0000u : 0u);
+            const uint32_t keep = (x >= first && x < last ? 0xFFFFu : 0u) | (x + 1 >= first && x + 1 < last ? 0xFFFF0000u : 0u);
+            fresh[e] = (fresh[e] | nan) & keep;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) words[e] = fresh[e];
+      }
+#pragma unroll
+      for (int c = 0; c < AN; ++c) asm volatile("" : "+a"(acc[c]));
+      buf = next(buf);
+    };
+    begin(0);
+    buf = next(buf);
+    begin(1);
+    phase(yes, no, 1);
+    if (ntiles > 1) {
+      int u = 2;
+      do {
+        u = __builtin_amdgcn_readfirstlane(u);
+        begin(u);
+        phase(yes, yes, u);
+      } while (++u <= ntiles);
+    }
+    begin(ntiles + 1);
+    phase(no, yes, ntiles + 1);
+    finish(n_dk, acc, a.scale * factor.y);
+  }
 }
 
 // ---------------------------------------------------------------- queries
@@ -587,7 +642,7 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
   const int b = at.b, n = at.n;
   const Seq seq = seq_of(a.len, b);
   at.tile = (seq.rows * a.per + TOK - 1) / TOK - 1 - at.tile;   // the last, which see most, first
-  const float2 factor = ds_factor<IO>(a, L.red);
+  const float2 factor = ds_factor<IO, NWV>(a, L.red);
 
   const int r_base = at.tile * TOK, r_end = min(seq.rows * a.per, r_base + TOK);
   const int t_lo = at.sp * a.q_chunk, t_hi = at.sp == a.q_splits - 1 ? INT_MAX : t_lo + a.q_chunk;
@@ -655,7 +710,7 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
     uint4 qf[KS], df[KSN];
     const int64_t stat = n * (int64_t)a.len.rows * a.per + (int64_t)seq.r0 * a.per + r;
     const float lse = a.lse[stat];
-    float delta = a.delta[stat];
+    float delta = -a.delta[stat];
     {
       const int64_t q_row = seq.r0 + s, head = n * a.per + g;
       const uint16_t* qp = a.q.p + q_row * a.q.row + head * a.q.head + kg * 8;
@@ -887,7 +942,7 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
     });
     sum = add_half_swap(sum) * (IO == IO_F16 ? 0x1p-15f : 1.f);
     // (all that the row sees lies in this range: others keep dO . O)
-    if (lane < 32 && valid && !dead && t_lo == 0 && (at.sp == a.q_splits - 1 || limit_of(a.len, seq, s) <= t_hi)) a.delta[stat] = sum;
+    if (lane < 32 && valid && !dead && t_lo == 0 && (at.sp == a.q_splits - 1 || limit_of(a.len, seq, s) <= t_hi)) a.delta[stat] = -sum;
   }
 
   const float f = a.scale * factor.y;
@@ -1015,7 +1070,7 @@ hipError_t launch_d(const GradK& k, const Cut& c, hipStream_t s) {
   hipLaunchKernelGGL((dense_queries_kernel<IO, D, DR>), dim3((unsigned)c.queries.groups), dim3(NWV * 64), 0, s, k);
   if (c.queries.splits > 1)
     hipLaunchKernelGGL((dense_join_kernel<IO, D, DR, false>), dim3((unsigned)c.queries.blocks), dim3(256), 0, s, k);
-  hipLaunchKernelGGL((dense_keys_kernel<IO, D, DR>), dim3((unsigned)c.keys.groups), dim3(NWV * 64), 0, s, k);
+  hipLaunchKernelGGL((dense_keys_kernel<IO, D, DR>), dim3((unsigned)c.keys.groups), dim3(KW * 64), 0, s, k);
   if (c.keys.splits > 1)
     hipLaunchKernelGGL((dense_join_kernel<IO, D, DR, true>), dim3((unsigned)c.keys.blocks), dim3(256), 0, s, k);
   return hipGetLastError();
@@ -1038,7 +1093,7 @@ hipError_t launch_dense_grad(const DenseGradArgs& g, size_t* lacking, hipStream_
   const Cut c = make_cut(g);
   *lacking = !a.ws || a.ws_bytes < c.bytes || ((uintptr_t)a.ws & 15) != 0 ? c.bytes : 0;
   if (*lacking) return hipSuccess;
-  if (c.keys.groups >= (1 << 24) || c.queries.groups >= (1 << 24)) return hipErrorInvalidConfiguration;   // 2^32 threads
+  if (c.keys.groups >= (1 << 23) || c.queries.groups >= (1 << 24)) return hipErrorInvalidConfiguration;   // 2^32 threads
   GradK k{};
   auto rows = [](const DenseTensor& t) { return Rows{(const uint16_t*)t.p, t.row, t.head}; };
   k.q = rows(a.q), k.qr = rows(a.qr), k.k = rows(a.k), k.kr = rows(a.kr), k.v = rows(a.v), k.d = rows(g.d_out), k.o = rows(g.out);
