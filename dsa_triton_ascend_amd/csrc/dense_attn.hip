@@ -152,34 +152,34 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
     const float cpos = a.scale == 0.f ? 1e-30f : fabsf(a.scale);
     const float cl2 = cpos * LOG2E;
 
-    // ---- tiles: each wave loads a share, in GPW loads
-    const Share<RB, BN, NWV> sh(wave, lane);
-    using ShR = Share<DR ? DR * 2 : 128, BN, NWV>;
-    const ShR shr(wave, lane);
-    constexpr int CK = sh.CNT, CR = DR ? ShR::CNT : 0, GPW = 2 * CK + CR;
-    const uint32_t k_row = (uint32_t)a.k.row * 2, v_row = (uint32_t)a.v.row * 2, kr_row = (uint32_t)a.kr.row * 2;
-    const char* const kb = reinterpret_cast<const char*>(a.k.p + (int64_t)seq.k0 * a.k.row + n * a.k.head);
-    const char* const vb = reinterpret_cast<const char*>(a.v.p + (int64_t)seq.k0 * a.v.row + n * a.v.head);
-    const char* const krb = DR ? reinterpret_cast<const char*>(a.kr.p + (int64_t)seq.k0 * a.kr.row + n * a.kr.head) : nullptr;
-    const uint32_t k_off = sh.row * k_row + sh.col, v_off = sh.row * v_row + sh.col, kr_off = shr.row * kr_row + shr.col;
-    // load j of tile u (rows past the last token repeat it; they are masked)
-    auto load_part = [&](auto jc, int u, int buf, bool whole) __attribute__((always_inline)) {
+    // ---- tiles: each wave loads a share, in GPW loads, one tile after another (past the last one it again, into
+    // buffers that nobody reads: no load then depends on a branch)
+    Stream<RB, BN, NWV> ks(a.k.p + (int64_t)(seq.k0 + t_lo) * a.k.row + n * a.k.head, (uint32_t)a.k.row * 2, L.k[0], wave, lane);
+    Stream<RB, BN, NWV> vs(a.v.p + (int64_t)(seq.k0 + t_lo) * a.v.row + n * a.v.head, (uint32_t)a.v.row * 2, L.v[0], wave, lane);
+    Stream<128, BN, NWV> rs(DR ? a.kr.p + (int64_t)(seq.k0 + t_lo) * a.kr.row + n * a.kr.head : nullptr, (uint32_t)a.kr.row * 2, L.kr[0], wave, lane);
+    constexpr int CK = ks.sh.CNT, CR = DR ? rs.sh.CNT : 0, GPW = 2 * CK + CR;
+    auto load_part = [&](auto jc, int buf) __attribute__((always_inline)) {
       constexpr int j = decltype(jc)::value;
-      constexpr int what = j < CK ? 0 : j < 2 * CK ? 1 : 2, i = what == 0 ? j : what == 1 ? j - CK : j - 2 * CK;
-      constexpr int step = i * (what == 2 ? ShR::STEP : sh.STEP);
-      const int t0 = t_lo + u * BN;
-      const uint32_t row = what == 0 ? k_row : what == 1 ? v_row : kr_row;
-      const char* p = (what == 0 ? kb : what == 1 ? vb : krb) + (int64_t)t0 * row;
-      uint8_t* dst = (what == 0 ? L.k[buf] : what == 1 ? L.v[buf] : L.kr[buf]) + (i * NWV + wave) * 1024;
-      if (whole) {
-        lds_dma16_sbase_untracked(p + step * (int64_t)row, what == 0 ? k_off : what == 1 ? v_off : kr_off, dst);
-      } else {
-        const int t = min(step + (what == 2 ? shr.row : sh.row), seq.ak - 1 - t0);
-        lds_dma16_sbase_untracked(p, (uint32_t)t * row + (what == 2 ? shr.col : sh.col), dst);
-      }
+      if constexpr (j < CK) ks.template load<j>(buf * (BN * RB));
+      else if constexpr (j < 2 * CK) vs.template load<j - CK>(buf * (BN * RB));
+      else rs.template load<j - 2 * CK>(buf * (BN * 128));
     };
-    auto load_tile = [&](int u, int buf) __attribute__((always_inline)) {
-      static_for<0, GPW>([&](auto j) __attribute__((always_inline)) { load_part(j, u, buf, false); });
+    // the streams to tile u, from the tile before it
+    auto aim = [&](int u) __attribute__((always_inline)) {
+      const int last = seq.ak - 1 - (t_lo + u * BN);
+      ks.aim(last);
+      vs.aim(last);
+      if constexpr (DR > 0) rs.aim(last);
+    };
+    auto advance = [&](int u) __attribute__((always_inline)) {
+      if (u >= ntiles) return;
+      ks.base += (int64_t)BN * ks.row_bytes;
+      vs.base += (int64_t)BN * vs.row_bytes;
+      if constexpr (DR > 0) rs.base += (int64_t)BN * rs.row_bytes;
+      if (t_lo + (u + 1) * BN > seq.ak) aim(u);
+    };
+    auto load_tile = [&](int buf) __attribute__((always_inline)) {
+      static_for<0, GPW>([&](auto j) __attribute__((always_inline)) { load_part(j, buf); });
     };
     // A tile that some rows see only in part: a masked token has P = 0, but 0 times a value that is not finite would
     // still reach the rows that do not see it. Such values become 0 in LDS, and the token's score NaN for the
@@ -190,7 +190,8 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
       const uint64_t bad = clean_share<IO, RB, BN, NWV>(lds_addr(L.v[buf]), wave, lane);
       if (lane == 0) L.bad[buf][wave] = bad;
     };
-    load_tile(0, 0);
+    aim(0);
+    load_tile(0);
     uint4 qf[RT][KS];
 #pragma unroll
     for (int m = 0; m < RT; ++m)
@@ -378,7 +379,8 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
     asm volatile("" ::: "memory");
     sanitize(0, 0);
     lds_barrier();
-    if (ntiles > 1) load_tile(1, 1);
+    advance(1);
+    load_tile(1);
     f32x16 s0[RT], s1[RT];
     uint4 p0[RT][2], p1[RT][2];
     point_k(0);
@@ -405,7 +407,7 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
     auto half0 = [&](auto pvc, int u) __attribute__((always_inline)) {
       mask(u, buf, 0, s0);
       const int lb = buf == 0 ? NBUF - 1 : buf - 1;   // tile u - 1's, for tile u + 2
-      const bool more = u + 2 < ntiles, whole = t_lo + (u + 3) * BN <= seq.ak;
+      advance(u + 2);
       step(pvc, yes, h1, s0, s1, p1, p0, [&]() __attribute__((always_inline)) {
              middle(u);
              point_v(buf);
@@ -413,8 +415,7 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
            [&](auto jc) __attribute__((always_inline)) {
              constexpr int j = decltype(jc)::value;
              static_for<0, GPW>([&](auto g) __attribute__((always_inline)) {
-               if constexpr (g * (KS * RT) / GPW == j)
-                 if (more) load_part(g, u + 2, lb, whole);
+               if constexpr (g * (KS * RT) / GPW == j) load_part(g, lb);
              });
            });
       rescale();
@@ -441,6 +442,7 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
       for (int m = 0; m < RT; ++m) o[m][i % ON] = Mfma<IO>::m32(vfr[i % VR], p1[m][i / ON], o[m][i % ON]);
       if (i + VR < NPV) vfr[i % VR] = v_frag(i + VR, 1);
     }
+    wait_vmcnt<0>();   // the last (unused) loads land before the LDS is released
   }
 
   // ---- lane l holds head row rr, columns c * 32 + 8 g + 4 kg + j of o[c][4 g + j]

@@ -79,6 +79,37 @@ template <int RB, int BN, int NW> struct Share {
   }
 };
 
+// 16-byte direct-to-LDS load as lds_dma16_sbase_untracked, to LDS address lds + OFF: the sum goes into M0 in one
+// instruction
+template <int OFF>
+__device__ __forceinline__ void lds_dma16_at(const void* sbase, uint32_t voff, uint32_t lds) {
+  asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(voff), "s"(sbase), "s"(lds), "n"(OFF)
+               : "memory", "m0", "scc");
+}
+
+// The loads of one array's tiles, one tile after another: this wave's share as offsets from a base that moves from
+// tile to tile. Rows past the last repeat it (they are masked); as only the last tile has any, the offsets are
+// made anew for that one and stay.
+template <int RB, int BN, int NW> struct Stream {
+  using Sh = Share<RB, BN, NW>;
+  Sh sh;
+  const char* base;      // of the next tile
+  uint32_t row_bytes;
+  uint32_t lds;          // this wave's first place in buffer 0
+  uint32_t off[Sh::CNT];
+  __device__ __forceinline__ Stream(const uint16_t* p, uint32_t row_bytes_, const void* buf, int wave, int lane)
+      : sh(wave, lane), base(reinterpret_cast<const char*>(p)), row_bytes(row_bytes_), lds(lds_addr(buf) + wave * 1024) {}
+  __device__ __forceinline__ void aim(int last) {   // last: the last row there is, from the tile's first
+#pragma unroll
+    for (int i = 0; i < Sh::CNT; ++i) off[i] = (uint32_t)min(i * Sh::STEP + sh.row, last) * row_bytes + sh.col;
+  }
+  template <int I> __device__ __forceinline__ void load(uint32_t buf_bytes) const {
+    lds_dma16_at<I * NW * 1024>(base, off[I], lds + buf_bytes);
+  }
+};
+
 // Token order of the S tiles: with row m of the operand at token tk(m), a lane's 16 accumulators of a 32-row tile
 // are tokens 16 (i / 8) + 8 (lane / 32) + i % 8, the order in which the next product takes them as an operand.
 __device__ __forceinline__ int s_row(int m) { return 16 * (m >> 4) + 8 * ((m >> 2) & 1) + 4 * ((m >> 3) & 1) + (m & 3); }

@@ -312,20 +312,43 @@ __global__ __launch_bounds__(KW * 64) void dense_keys_kernel(GradK a) {
   const char* const db = base_of(a.d);
   const char* const qrb = DR ? base_of(a.qr) : nullptr;
   const bool linear = a.linear;
-  const uint32_t q_off = linear ? (uint32_t)place(a.q, sh.row) + sh.col : 0, d_off = linear ? (uint32_t)place(a.d, sh.row) + sh.col : 0;
-  const uint32_t qr_off = DR && linear ? (uint32_t)place(a.qr, shr.row) + shr.col : 0;
   const int64_t stat0 = n * (int64_t)a.len.rows * a.per + (int64_t)seq.r0 * a.per;
-  // this wave's loads of tile u (rows past the last repeat it; they are masked), and how many they are
-  auto load_rows = [&](const Rows& x, const char* p, uint32_t off, int row, uint32_t col, int r0, void* dst) __attribute__((always_inline)) {
-    if (linear && r0 + KB <= r_hi) lds_dma16_sbase_untracked(p + (int64_t)(r0 >> a.per_shift) * x.row * 2, off, dst);
-    else lds_dma16_untracked(p + place(x, min(r0 + row, r_hi - 1)) + col, dst);
+  // Tile u has the head rows from first_row(u) on: the last rows first, which all work-groups of a key head see, so that
+  // they read the same ones at the same time (from the first on, each began at rows of its own, and 63% of the loads missed the
+  // L2). Rows past the last repeat it (they are masked); only tile 0 has any.
+  auto first_row = [&](int u) { return r_lo + (ntiles - 1 - u) * KB; };
+  struct Flow {   // of one array, the heads of a group dividing 16
+    const char* base;   // of the next tile
+    int64_t step;
+    uint32_t off;
   };
+  auto flow_of = [&](const Rows& x, const char* p) {
+    const int64_t step = (int64_t)(KB >> a.per_shift) * x.row * 2;
+    return Flow{p + (int64_t)(first_row(0) >> a.per_shift) * x.row * 2, step, 0};
+  };
+  Flow fq = flow_of(a.q, qb), fd = flow_of(a.d, db), fr = DR ? flow_of(a.qr, qrb) : Flow{};
+  auto aim = [&](int u) __attribute__((always_inline)) {
+    const int last = r_hi - 1 - first_row(u);
+    fq.off = (uint32_t)place(a.q, min(sh.row, last)) + sh.col;
+    fd.off = (uint32_t)place(a.d, min(sh.row, last)) + sh.col;
+    if constexpr (DR > 0) fr.off = (uint32_t)place(a.qr, min(shr.row, last)) + shr.col;
+  };
+  auto load_rows = [&](const Rows& x, const char* p, Flow& f, int row, uint32_t col, int r0, uint32_t dst) __attribute__((always_inline)) {
+    if (linear) {
+      lds_dma16_at<0>(f.base, f.off, dst);
+      f.base -= f.step;
+    } else {
+      lds_dma16_untracked(p + place(x, min(r0 + row, r_hi - 1)) + col, (void*)(__attribute__((address_space(3))) void*)(uintptr_t)dst);
+    }
+  };
+  const uint32_t q_lds = lds_addr(L.t[0].q) + lw * 1024, r_lds = lds_addr(L.qr[0]) + pair * 1024;
+  // this wave's loads of tile u, one tile after another
   auto load_tile = [&](int u, int buf) __attribute__((always_inline)) {
-    const int r0 = r_lo + u * KB;
-    if (WIDE || !second) load_rows(a.q, qb, q_off, sh.row, sh.col, r0, L.t[buf].q + lw * 1024);
-    if (WIDE || second) load_rows(a.d, db, d_off, sh.row, sh.col, r0, L.t[buf].d + lw * 1024);
+    const int r0 = first_row(u);
+    if (WIDE || !second) load_rows(a.q, qb, fq, sh.row, sh.col, r0, q_lds + buf * (2 * KB * RB));
+    if (WIDE || second) load_rows(a.d, db, fd, sh.row, sh.col, r0, q_lds + buf * (2 * KB * RB) + KB * RB);
     if constexpr (DR > 0)
-      if (!second) load_rows(a.qr, qrb, qr_off, shr.row, shr.col, r0, L.qr[buf] + pair * 1024);
+      if (!second) load_rows(a.qr, qrb, fr, shr.row, shr.col, r0, r_lds + buf * (KB * 128));
     if (pair == 0) {
       const int64_t r = stat0 + min(r0 + lane, r_hi - 1);
       if (second) lds_dma4(a.delta + r, L.delta[buf]);
@@ -334,7 +357,7 @@ __global__ __launch_bounds__(KW * 64) void dense_keys_kernel(GradK a) {
   };
   const int loads = (WIDE ? 2 : 1) + (DR > 0 && !second ? 1 : 0) + (pair == 0 ? 1 : 0);
   // (a masked pair has P = dS = 0, but 0 times a value that is not finite would reach tokens that the row does not see)
-  auto is_mixed = [&](int u) { return r_lo + u * KB < r_full || r_lo + u * KB + KB > r_hi; };
+  auto is_mixed = [&](int u) { return first_row(u) < r_full || first_row(u) + KB > r_hi; };
   auto sanitize = [&](int u, int buf) __attribute__((always_inline)) {
     if (!is_mixed(u)) return;
     uint32_t bad = 0;
@@ -368,8 +391,12 @@ __global__ __launch_bounds__(KW * 64) void dense_keys_kernel(GradK a) {
     return bad;
   };
 
+  aim(0);
   load_tile(0, 0);
-  if (ntiles > 1) load_tile(1, 1);
+  if (ntiles > 1) {
+    aim(1);
+    load_tile(1, 1);
+  }
   uint4 opf[KS];   // this wave's K (first) or V (second)
   {
     const int64_t tt = seq.k0 + min(t, t_seen - 1);
@@ -467,7 +494,7 @@ __global__ __launch_bounds__(KW * 64) void dense_keys_kernel(GradK a) {
           int k = kg;
           asm volatile("" : "+v"(k));   // (what follows from it is not kept in registers for these few tiles)
           const uint32_t bad = bad_rows(buf);
-          const int r0 = r_lo + u * KB, first = my_first - r0, last = r_hi - r0;   // rows [first, last) see the token
+          const int r0 = first_row(u), first = my_first - r0, last = r_hi - r0;   // rows [first, last) see the token
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int x = s_token(i, k);
@@ -576,7 +603,7 @@ __global__ __launch_bounds__(KW * 64) void dense_keys_kernel(GradK a) {
           int k = kg;
           asm volatile("" : "+v"(k));   // (what follows from it is not kept in registers for these few tiles)
           const uint32_t bad = bad_rows(vb);
-          const int r0 = r_lo + (u - 1) * KB, first = my_first - r0, last = r_hi - r0;
+          const int r0 = first_row(u - 1), first = my_first - r0, last = r_hi - r0;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int x = s_token(2 * e, k);
@@ -669,34 +696,36 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
     // (a zero scale becomes 1e-30: scores round to 0, and a masked one, of the sign that makes it so, to P = 0)
     const float sl2 = (a.scale == 0.f ? 1e-30f : a.scale) * LOG2E;
     const float masked = sl2 > 0.f ? -INFINITY : INFINITY;
-    using Sh = Share<RB, BN, NWV>;
-    using ShR = Share<DR ? DR * 2 : 128, BN, NWV>;
-    const Sh sh(wave, lane);
-    const ShR shr(wave, lane);
-    constexpr int CK = Sh::CNT, CR = DR ? ShR::CNT : 0, GPW = 2 * CK + CR;
-    const uint32_t k_row = (uint32_t)a.k.row * 2, v_row = (uint32_t)a.v.row * 2, kr_row = (uint32_t)a.kr.row * 2;
-    const char* const kb = reinterpret_cast<const char*>(a.k.p + (int64_t)seq.k0 * a.k.row + n * a.k.head);
-    const char* const vb = reinterpret_cast<const char*>(a.v.p + (int64_t)seq.k0 * a.v.row + n * a.v.head);
-    const char* const krb = DR ? reinterpret_cast<const char*>(a.kr.p + (int64_t)seq.k0 * a.kr.row + n * a.kr.head) : nullptr;
-    const uint32_t k_off = sh.row * k_row + sh.col, v_off = sh.row * v_row + sh.col, kr_off = shr.row * kr_row + shr.col;
-    // load j of tile u (rows past the last token repeat it; they are masked)
-    auto load_part = [&](auto jc, int u, int buf, bool whole) __attribute__((always_inline)) {
+    // (as in the forward: past the last tile it again)
+    Stream<RB, BN, NWV> ks(a.k.p + (int64_t)(seq.k0 + t_lo) * a.k.row + n * a.k.head, (uint32_t)a.k.row * 2, L.t[0].k, wave, lane);
+    Stream<RB, BN, NWV> vs(a.v.p + (int64_t)(seq.k0 + t_lo) * a.v.row + n * a.v.head, (uint32_t)a.v.row * 2, L.t[0].v, wave, lane);
+    Stream<128, BN, NWV> rs(DR ? a.kr.p + (int64_t)(seq.k0 + t_lo) * a.kr.row + n * a.kr.head : nullptr, (uint32_t)a.kr.row * 2, L.kr[0], wave, lane);
+    constexpr int CK = ks.sh.CNT, CR = DR ? rs.sh.CNT : 0, GPW = 2 * CK + CR;
+    auto load_part = [&](auto jc, int buf) __attribute__((always_inline)) {
       constexpr int j = decltype(jc)::value;
-      constexpr int what = j < CK ? 0 : j < 2 * CK ? 1 : 2, i = what == 0 ? j : what == 1 ? j - CK : j - 2 * CK;
-      constexpr int step = i * (what == 2 ? ShR::STEP : Sh::STEP);
-      const int t0 = t_lo + u * BN;
-      const uint32_t row = what == 0 ? k_row : what == 1 ? v_row : kr_row;
-      const char* p = (what == 0 ? kb : what == 1 ? vb : krb) + (int64_t)t0 * row;
-      uint8_t* dst = (what == 0 ? L.t[buf].k : what == 1 ? L.t[buf].v : L.kr[buf]) + (i * NWV + wave) * 1024;
-      if (whole) {
-        lds_dma16_sbase_untracked(p + step * (int64_t)row, what == 0 ? k_off : what == 1 ? v_off : kr_off, dst);
-      } else {
-        const int t = min(step + (what == 2 ? shr.row : sh.row), seq.ak - 1 - t0);
-        lds_dma16_sbase_untracked(p, (uint32_t)t * row + (what == 2 ? shr.col : sh.col), dst);
-      }
+      if constexpr (j < CK) ks.template load<j>(buf * (2 * BN * RB));
+      else if constexpr (j < 2 * CK) vs.template load<j - CK>(buf * (2 * BN * RB));
+      else rs.template load<j - 2 * CK>(buf * (BN * 128));
     };
-    auto load_tile = [&](int u, int buf) __attribute__((always_inline)) {
-      static_for<0, GPW>([&](auto j) __attribute__((always_inline)) { load_part(j, u, buf, false); });
+    auto aim = [&](int u) __attribute__((always_inline)) {
+      const int last = seq.ak - 1 - (t_lo + u * BN);
+      ks.aim(last);
+      vs.aim(last);
+      if constexpr (DR > 0) rs.aim(last);
+    };
+    auto move = [&](int64_t tiles) __attribute__((always_inline)) {
+      ks.base += tiles * (int64_t)BN * ks.row_bytes;
+      vs.base += tiles * (int64_t)BN * vs.row_bytes;
+      if constexpr (DR > 0) rs.base += tiles * (int64_t)BN * rs.row_bytes;
+    };
+    // the streams to tile u, from the tile before it
+    auto advance = [&](int u) __attribute__((always_inline)) {
+      if (u >= ntiles) return;
+      move(1);
+      if (t_lo + (u + 1) * BN > seq.ak) aim(u);
+    };
+    auto load_tile = [&](int buf) __attribute__((always_inline)) {
+      static_for<0, GPW>([&](auto j) __attribute__((always_inline)) { load_part(j, buf); });
     };
     // (a masked token has dS = 0, but 0 times a value that is not finite would reach rows that do not see it)
     auto is_mixed = [&](int u) { return t_lo + u * BN + BN > min_lim; };
@@ -706,7 +735,8 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
       if constexpr (DR > 0) bad |= clean_share<IO, 128, BN, NWV>(lds_addr(L.kr[buf]), wave, lane);
       if (lane == 0) L.bad[buf][wave] = bad;
     };
-    load_tile(0, 0);
+    aim(0);
+    load_tile(0);
     uint4 qf[KS], df[KSN];
     const int64_t stat = n * (int64_t)a.len.rows * a.per + (int64_t)seq.r0 * a.per + r;
     const float lse = a.lse[stat];
@@ -791,7 +821,8 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
       for (int u = 0; u < ntiles; ++u) {
         if (u > 0) {
           lds_barrier();   // every wave is done with the buffer
-          load_tile(u, 0);
+          advance(u);
+          load_tile(0);
         }
         wait_vmcnt<0>();
         asm volatile("" ::: "memory");
@@ -811,7 +842,9 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
       delta = add_half_swap(sum) * (IO == IO_F16 ? 0x1p-15f : 1.f);
       sum = 0.f;
       lds_barrier();
-      load_tile(0, 0);   // (anew also where it is the only one: cleaned values are gone from it)
+      move(1 - ntiles);
+      aim(0);
+      load_tile(0);   // (anew also where it is the only one: cleaned values are gone from it)
     }
 
     // ---- dS of 32 tokens in NST stages of two each, placed among the products before and after them
@@ -890,7 +923,8 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
     asm volatile("" ::: "memory");
     sanitize(0, 0);
     lds_barrier();
-    if (ntiles > 1) load_tile(1, 1);
+    advance(1);
+    load_tile(1);
     f32x16 s0, s1, d0, d1;
     uint32_t w0[8], w1[8];
     point_op(0);
@@ -904,7 +938,7 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
     auto half0 = [&](auto pvc, int u) __attribute__((always_inline)) {
       const int nb = buf == NBUF - 1 ? 0 : buf + 1, lb = buf == 0 ? NBUF - 1 : buf - 1;   // of tiles u + 1 and u - 1 (u + 2)
       mask(u, buf, 0, s0, d0);
-      const bool more = u + 2 < ntiles, whole = t_lo + (u + 3) * BN <= seq.ak;
+      advance(u + 2);
       step(pvc, yes, h1, s0, d0, s1, d1, w1, w0,
            [&]() __attribute__((always_inline)) {
              wait_vmcnt<0>();
@@ -916,8 +950,7 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
            [&](auto jc) __attribute__((always_inline)) {
              constexpr int j = decltype(jc)::value;
              static_for<0, GPW>([&](auto g) __attribute__((always_inline)) {
-               if constexpr (g * NS / GPW == j)
-                 if (more) load_part(g, u + 2, lb, whole);
+               if constexpr (g * NS / GPW == j) load_part(g, lb);
              });
            });
     };
@@ -940,6 +973,7 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
       dq[c] = Mfma<IO>::m32(tf[i % TR], make_uint4(w1[4 * st], w1[4 * st + 1], w1[4 * st + 2], w1[4 * st + 3]), dq[c]);
       if constexpr (i + TR < NP) tf[i % TR] = t_frag(i + TR, 1);
     });
+    wait_vmcnt<0>();   // the last (unused) loads land before the LDS is released
     sum = add_half_swap(sum) * (IO == IO_F16 ? 0x1p-15f : 1.f);
     // (all that the row sees lies in this range: others keep dO . O)
     if (lane < 32 && valid && !dead && t_lo == 0 && (at.sp == a.q_splits - 1 || limit_of(a.len, seq, s) <= t_hi)) a.delta[stat] = -sum;
