@@ -205,10 +205,12 @@ __device__ __forceinline__ Place place_of(int i, int seqs, int heads, int splits
 // bits, from LDS, makes dP and dS and adds to dK, one tile of 32 rows behind. Each adds the tile before while the VALU works on
 // the present one. Tiles lie in a ring of KRING, loaded two ahead; one barrier a tile.
 constexpr int KB = 32;      // rows of a tile
-constexpr int KRING = 5;
+// tiles in the ring: two behind the present one, the others under way
+template <int D, int DR> constexpr int key_ring() { return D == 64 ? 5 : DR ? 6 : 7; }
 constexpr int KW = 8;       // waves
 
 template <int D, int DR> struct KeyLds {
+  static constexpr int KRING = key_ring<D, DR>();
   struct {
     uint8_t q[KB * D * 2];   // (d lies at a constant offset from q)
     uint8_t d[KB * D * 2];
@@ -229,6 +231,7 @@ __device__ __forceinline__ void lds_dma4(const void* gptr, void* lds_base) {
 template <int IO, int D, int DR>
 __global__ __launch_bounds__(KW * 64) void dense_keys_kernel(GradK a) {
   constexpr int KSN = D / 16, KS = (D + DR) / 16, ON = D / 32, RN = DR / 32, RB = D * 2;
+  constexpr int KRING = key_ring<D, DR>(), AHEAD = KRING - 3;
   constexpr bool WIDE = RB == 256;   // a wave loads rows of q and of d, else of one of them
   __shared__ __attribute__((aligned(16))) KeyLds<D, DR> L;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -368,21 +371,23 @@ __global__ __launch_bounds__(KW * 64) void dense_keys_kernel(GradK a) {
     if (lane == 0) L.bad[buf][wave] = bad;
   };
   auto next = [](int buf) { return buf == KRING - 1 ? 0 : buf + 1; };
+  auto ahead = [](int buf) { return buf + AHEAD >= KRING ? buf + AHEAD - KRING : buf + AHEAD; };
   auto before = [](int buf) { return buf == 0 ? KRING - 1 : buf - 1; };
   // The beginning of phase u: tile u is in LDS for everyone, and tile u - 3 done with
   int buf = 0;   // of tile u
   auto begin = [&](int u) __attribute__((always_inline)) {
     if (u < ntiles) {
-      if (u + 1 >= ntiles) wait_vmcnt<0>();
-      else if (loads == 1) wait_vmcnt<1>();
-      else if (loads == 2) wait_vmcnt<2>();
-      else if (loads == 3) wait_vmcnt<3>();
-      else wait_vmcnt<4>();
+      // (the last few tiles wait for all that is under way)
+      if (u + AHEAD > ntiles) wait_vmcnt<0>();
+      else if (loads == 1) wait_vmcnt<AHEAD - 1>();
+      else if (loads == 2) wait_vmcnt<2 * (AHEAD - 1)>();
+      else if (loads == 3) wait_vmcnt<3 * (AHEAD - 1)>();
+      else wait_vmcnt<4 * (AHEAD - 1)>();
       asm volatile("" ::: "memory");
       sanitize(u, buf);
     }
     lds_barrier();
-    if (u + 2 < ntiles) load_tile(u + 2, next(next(buf)));
+    if (u + AHEAD < ntiles) load_tile(u + AHEAD, ahead(buf));
   };
   auto bad_rows = [&](int buf) {
     uint32_t bad = 0;
@@ -393,10 +398,10 @@ __global__ __launch_bounds__(KW * 64) void dense_keys_kernel(GradK a) {
 
   aim(0);
   load_tile(0, 0);
-  if (ntiles > 1) {
-    aim(1);
-    load_tile(1, 1);
-  }
+  if (ntiles > 1) aim(1);
+#pragma unroll
+  for (int u = 1; u < AHEAD; ++u)
+    if (u < ntiles) load_tile(u, u);
   uint4 opf[KS];   // this wave's K (first) or V (second)
   {
     const int64_t tt = seq.k0 + min(t, t_seen - 1);
