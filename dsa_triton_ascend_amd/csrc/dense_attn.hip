@@ -173,9 +173,9 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
     };
     auto advance = [&](int u) __attribute__((always_inline)) {
       if (u >= ntiles) return;
-      ks.base += (int64_t)BN * ks.row_bytes;
-      vs.base += (int64_t)BN * vs.row_bytes;
-      if constexpr (DR > 0) rs.base += (int64_t)BN * rs.row_bytes;
+      ks.base = uniform(ks.base + (int64_t)BN * ks.row_bytes);
+      vs.base = uniform(vs.base + (int64_t)BN * vs.row_bytes);
+      if constexpr (DR > 0) rs.base = uniform(rs.base + (int64_t)BN * rs.row_bytes);
       if (t_lo + (u + 1) * BN > seq.ak) aim(u);
     };
     auto load_tile = [&](int buf) __attribute__((always_inline)) {

@@ -89,6 +89,13 @@ __device__ __forceinline__ void lds_dma16_at(const void* sbase, uint32_t voff, u
                : "memory", "m0", "scc");
 }
 
+// p, which is the same in all lanes, in scalar registers
+__device__ __forceinline__ const char* uniform(const char* p) {
+  const uint64_t v = (uint64_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  return (const char*)(lo | (uint64_t)hi << 32);
+}
+
 // The loads of one array's tiles, one tile after another: this wave's share as offsets from a base that moves from
 // tile to tile. Rows past the last repeat it (they are masked); as only the last tile has any, the offsets are
 // made anew for that one and stay.

@@ -199,28 +199,16 @@ __device__ __forceinline__ Place place_of(int i, int seqs, int heads, int splits
 }
 
 // ---------------------------------------------------------------- keys
-// Eight waves, two for each 32 of the 128 tokens: with one wave a SIMD, which issues an instruction every 8 cycles,
-// the products waited for the rest (32 rows took 2,400 cycles for 1,024 of MFMAs); one wave cannot have less than 192 registers of
-// dK, dV, K and V at D = 128, so the two split the products. The first makes S and P and adds to dV; the second takes P, in 32
-// bits, from LDS, makes dP and dS and adds to dK, one tile of 32 rows behind. Each adds the tile before while the VALU works on
-// the present one. Tiles lie in a ring of KRING, loaded two ahead; one barrier a tile.
-constexpr int KB = 32;      // rows of a tile
-// tiles in the ring: two behind the present one, the others under way
-template <int D, int DR> constexpr int key_ring() { return D == 64 ? 5 : DR ? 6 : 7; }
-constexpr int KW = 8;       // waves
-
 template <int D, int DR> struct KeyLds {
-  static constexpr int KRING = key_ring<D, DR>();
   struct {
-    uint8_t q[KB * D * 2];   // (d lies at a constant offset from q)
-    uint8_t d[KB * D * 2];
-  } t[KRING];
-  uint8_t qr[KRING][DR ? KB * DR * 2 : 16];
-  float4 p[2][4][4][64];
-  float lse[KRING][64];     // (KB of them count: a wave loads 64)
-  float delta[KRING][64];
-  uint32_t bad[KRING][KW];
-  float red[2][KW];
+    uint8_t q[BN * D * 2];   // (d lies at a constant offset from q)
+    uint8_t d[BN * D * 2];
+  } t[NBUF];
+  uint8_t qr[NBUF][DR ? BN * DR * 2 : 16];
+  float lse[NBUF][BN];
+  float delta[NBUF][BN];
+  uint64_t bad[NBUF][NWV];
+  float red[2][NWV];
 };
 
 __device__ __forceinline__ void lds_dma4(const void* gptr, void* lds_base) {
@@ -228,16 +216,12 @@ __device__ __forceinline__ void lds_dma4(const void* gptr, void* lds_base) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(gptr), "s"(m0) : "memory", "m0");
 }
 
-template <int IO, int D, int DR>
-__global__ __launch_bounds__(KW * 64) void dense_keys_kernel(GradK a) {
+template <int IO, int D, int DR, bool LINEAR>
+__global__ __launch_bounds__(NWV * 64) void dense_keys_kernel(GradK a) {
   constexpr int KSN = D / 16, KS = (D + DR) / 16, ON = D / 32, RN = DR / 32, RB = D * 2;
-  constexpr int KRING = key_ring<D, DR>(), AHEAD = KRING - 3;
-  constexpr bool WIDE = RB == 256;   // a wave loads rows of q and of d, else of one of them
   __shared__ __attribute__((aligned(16))) KeyLds<D, DR> L;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kg = lane >> 5, rr = lane & 31;
-  const int pair = wave & 3;
-  const bool second = wave >= 4;
   const Place at = place_of(blockIdx.x, a.k_seqs, a.key_heads, a.k_splits, a.k_even, a.len.key_start, 1, [&](int b) {
     const Seq q = seq_of(a.len, b);
     return (q.keys + TOK - 1) / TOK;
@@ -245,401 +229,384 @@ __global__ __launch_bounds__(KW * 64) void dense_keys_kernel(GradK a) {
   if (at.tile < 0) return;
   const int b = at.b, n = at.n;
   const Seq seq = seq_of(a.len, b);
-  const float2 factor = ds_factor<IO, KW>(a, L.red);
+  const float2 factor = ds_factor<IO, NWV>(a, L.red);
 
   const int t0 = at.tile * TOK, t_end = min(seq.keys, t0 + TOK), t_seen = min(t_end, seq.ak);
-  const int t = t0 + pair * 32 + rr;
+  const int t = t0 + wave * 32 + rr;
   // head rows [r_lo, r_hi) see some of these tokens, from r_full on all of them; this range's share
   const int r_end = seq.aq * a.per;
   const int r_lo = __builtin_amdgcn_readfirstlane(max(first_query(a.len, seq, t0) * a.per, at.sp * a.k_chunk));
   const int r_hi = __builtin_amdgcn_readfirstlane(at.sp == a.k_splits - 1 ? r_end : min(r_end, (at.sp + 1) * a.k_chunk));
-  const int r_full = __builtin_amdgcn_readfirstlane(t_seen > t0 ? first_query(a.len, seq, t_seen - 1) * a.per : 0);
+  const int r_full = t_seen > t0 ? first_query(a.len, seq, t_seen - 1) * a.per : 0;
   const int my_first = t < t_seen ? first_query(a.len, seq, t) * a.per : INT_MAX;
-  const int ntiles = __builtin_amdgcn_readfirstlane(t_seen > t0 && r_hi > r_lo ? (r_hi - r_lo + KB - 1) / KB : 0);
+  const int ntiles = t_seen > t0 && r_hi > r_lo ? (r_hi - r_lo + BN - 1) / BN : 0;
 
-  // The sums of this wave's N column tiles (none: zeros) go out: lane l has token t, columns c * 32 + 8 g + 4 kg + j
-  auto finish = [&](auto nc, const f32x16* acc, float f) __attribute__((always_inline)) {
-    constexpr int N = decltype(nc)::value;
-    if (a.k_splits > 1) {
-      const int blk = n * (a.k_blocks / a.key_heads) + seq.k0 / 32 + b + at.tile * 4 + pair;
-      if (t0 + pair * 32 >= seq.keys) return;
-      float4* dst = a.k_part + ((int64_t)at.sp * a.k_blocks + blk) * ((2 * D + DR) / 8) * 64 + (second ? 0 : (D + DR) / 8 * 64) + lane;
+  f32x16 dk[ON + RN], dv[ON];
 #pragma unroll
-      for (int c = 0; c < N; ++c)
+  for (int i = 0; i < 16; ++i) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          dst[(c * 4 + g) * 64] = make_float4(acc[c][4 * g] * f, acc[c][4 * g + 1] * f, acc[c][4 * g + 2] * f, acc[c][4 * g + 3] * f);
-      return;
-    }
-    const bool live = t < t_seen, valid = t < t_end;
-    const int64_t tt = (int64_t)(seq.k0 + t) * a.key_heads + n;
+    for (int c = 0; c < ON + RN; ++c) dk[c][i] = 0.f;
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
-      uint4 w[2];
-      pack_tile<IO>(acc[c], f, w);
-      uint16_t* dst = (c >= ON ? a.dkr + tt * DR + (c - ON) * 32 : (second ? a.dk : a.dv) + tt * D + c * 32) + 8 * kg;
-      if (valid) {
-        stg16(dst, live ? w[0] : make_uint4(0, 0, 0, 0));
-        stg16(dst + 16, live ? w[1] : make_uint4(0, 0, 0, 0));
-      }
-    }
-  };
-  constexpr int AN = ON + RN;   // the second wave's dK; the first one's dV has ON
-  std::integral_constant<int, ON> n_dv;
-  std::integral_constant<int, AN> n_dk;
-  if (ntiles == 0) {
-    f32x16 zero[AN];
-#pragma unroll
-    for (int c = 0; c < AN; ++c)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) zero[c][i] = 0.f;
-    if (second) finish(n_dk, zero, 0.f);
-    else finish(n_dv, zero, 0.f);
-    return;
+    for (int c = 0; c < ON; ++c) dv[c][i] = 0.f;
   }
-  const float sl2 = a.scale * LOG2E;
-  // ---- tiles of head rows. Where the group's heads divide 16, a lane's rows are of one head, and evenly spaced.
-  using Sh = Share<RB, KB, WIDE ? KW : 4>;
-  using ShR = Share<128, KB, 4>;
-  const int lw = WIDE ? wave : pair;
-  const Sh sh(lw, lane);
-  const ShR shr(pair, lane);
-  auto place = [&](const Rows& x, int r) {   // of head row r, in bytes
-    const int s = row_div(a, r);
-    return ((int64_t)s * x.row + (int64_t)(r - s * a.per) * x.head) * 2;
-  };
-  auto base_of = [&](const Rows& x) {
-    return reinterpret_cast<const char*>(x.p + (int64_t)seq.r0 * x.row + (int64_t)n * a.per * x.head);
-  };
-  const char* const qb = base_of(a.q);
-  const char* const db = base_of(a.d);
-  const char* const qrb = DR ? base_of(a.qr) : nullptr;
-  const bool linear = a.linear;
-  const int64_t stat0 = n * (int64_t)a.len.rows * a.per + (int64_t)seq.r0 * a.per;
-  // Tile u has the head rows from first_row(u) on: the last rows first, which all work-groups of a key head see, so that
-  // they read the same ones at the same time (from the first on, each began at rows of its own, and 63% of the loads missed the
-  // L2). Rows past the last repeat it (they are masked); only tile 0 has any.
-  auto first_row = [&](int u) { return r_lo + (ntiles - 1 - u) * KB; };
-  struct Flow {   // of one array, the heads of a group dividing 16
-    const char* base;   // of the next tile
-    int64_t step;
-    uint32_t off;
-  };
-  auto flow_of = [&](const Rows& x, const char* p) {
-    const int64_t step = (int64_t)(KB >> a.per_shift) * x.row * 2;
-    return Flow{p + (int64_t)(first_row(0) >> a.per_shift) * x.row * 2, step, 0};
-  };
-  Flow fq = flow_of(a.q, qb), fd = flow_of(a.d, db), fr = DR ? flow_of(a.qr, qrb) : Flow{};
-  auto aim = [&](int u) __attribute__((always_inline)) {
-    const int last = r_hi - 1 - first_row(u);
-    fq.off = (uint32_t)place(a.q, min(sh.row, last)) + sh.col;
-    fd.off = (uint32_t)place(a.d, min(sh.row, last)) + sh.col;
-    if constexpr (DR > 0) fr.off = (uint32_t)place(a.qr, min(shr.row, last)) + shr.col;
-  };
-  auto load_rows = [&](const Rows& x, const char* p, Flow& f, int row, uint32_t col, int r0, uint32_t dst) __attribute__((always_inline)) {
-    if (linear) {
-      lds_dma16_at<0>(f.base, f.off, dst);
-      f.base -= f.step;
-    } else {
-      lds_dma16_untracked(p + place(x, min(r0 + row, r_hi - 1)) + col, (void*)(__attribute__((address_space(3))) void*)(uintptr_t)dst);
-    }
-  };
-  const uint32_t q_lds = lds_addr(L.t[0].q) + lw * 1024, r_lds = lds_addr(L.qr[0]) + pair * 1024;
-  // this wave's loads of tile u, one tile after another
-  auto load_tile = [&](int u, int buf) __attribute__((always_inline)) {
-    const int r0 = first_row(u);
-    if (WIDE || !second) load_rows(a.q, qb, fq, sh.row, sh.col, r0, q_lds + buf * (2 * KB * RB));
-    if (WIDE || second) load_rows(a.d, db, fd, sh.row, sh.col, r0, q_lds + buf * (2 * KB * RB) + KB * RB);
-    if constexpr (DR > 0)
-      if (!second) load_rows(a.qr, qrb, fr, shr.row, shr.col, r0, r_lds + buf * (KB * 128));
-    if (pair == 0) {
-      const int64_t r = stat0 + min(r0 + lane, r_hi - 1);
-      if (second) lds_dma4(a.delta + r, L.delta[buf]);
-      else lds_dma4(a.lse + r, L.lse[buf]);
-    }
-  };
-  const int loads = (WIDE ? 2 : 1) + (DR > 0 && !second ? 1 : 0) + (pair == 0 ? 1 : 0);
-  // (a masked pair has P = dS = 0, but 0 times a value that is not finite would reach tokens that the row does not see)
-  auto is_mixed = [&](int u) { return first_row(u) < r_full || first_row(u) + KB > r_hi; };
-  auto sanitize = [&](int u, int buf) __attribute__((always_inline)) {
-    if (!is_mixed(u)) return;
-    uint32_t bad = 0;
-    if (WIDE || !second) bad |= (uint32_t)clean_share<IO, RB, KB, WIDE ? KW : 4>(lds_addr(L.t[buf].q), lw, lane);
-    if (WIDE || second) bad |= (uint32_t)clean_share<IO, RB, KB, WIDE ? KW : 4>(lds_addr(L.t[buf].d), lw, lane);
-    if constexpr (DR > 0)
-      if (!second) bad |= (uint32_t)clean_share<IO, 128, KB, 4>(lds_addr(L.qr[buf]), pair, lane);
-    if (lane == 0) L.bad[buf][wave] = bad;
-  };
-  auto next = [](int buf) { return buf == KRING - 1 ? 0 : buf + 1; };
-  auto ahead = [](int buf) { return buf + AHEAD >= KRING ? buf + AHEAD - KRING : buf + AHEAD; };
-  auto before = [](int buf) { return buf == 0 ? KRING - 1 : buf - 1; };
-  // The beginning of phase u: tile u is in LDS for everyone, and tile u - 3 done with
-  int buf = 0;   // of tile u
-  auto begin = [&](int u) __attribute__((always_inline)) {
-    if (u < ntiles) {
-      // (the last few tiles wait for all that is under way)
-      if (u + AHEAD > ntiles) wait_vmcnt<0>();
-      else if (loads == 1) wait_vmcnt<AHEAD - 1>();
-      else if (loads == 2) wait_vmcnt<2 * (AHEAD - 1)>();
-      else if (loads == 3) wait_vmcnt<3 * (AHEAD - 1)>();
-      else wait_vmcnt<4 * (AHEAD - 1)>();
-      asm volatile("" ::: "memory");
-      sanitize(u, buf);
-    }
-    lds_barrier();
-    if (u + AHEAD < ntiles) load_tile(u + AHEAD, ahead(buf));
-  };
-  auto bad_rows = [&](int buf) {
-    uint32_t bad = 0;
-#pragma unroll
-    for (int w = 0; w < KW; ++w) bad |= L.bad[buf][w];
-    return bad;
-  };
 
-  aim(0);
-  load_tile(0, 0);
-  if (ntiles > 1) aim(1);
+  if (ntiles > 0) {
+    const float sl2 = a.scale * LOG2E;
+    // ---- tiles of head rows: each wave loads a share, in GPW loads (past the last tile it again, into buffers that nobody
+    // reads: no load then depends on a branch). Tile u has the rows from first_row(u) on: the last rows first, which
+    // all work-groups of a key head see, so that they read the same ones at the same time (from the first on, each began at
+    // rows of its own, and 63% of the loads missed the L2). Rows past the last repeat it (they are masked); only tile 0
+    // has any. LINEAR: the group's heads divide 16, so that a lane's rows of all tiles are of one head and evenly spaced.
+    auto first_row = [&](int u) { return r_lo + (ntiles - 1 - u) * BN; };
+    using Sh = Share<RB, BN, NWV>;
+    using ShR = Share<DR ? DR * 2 : 128, BN, NWV>;
+    const Sh sh(wave, lane);
+    const ShR shr(wave, lane);
+    constexpr int CQ = Sh::CNT, CR = DR ? ShR::CNT : 0, GPW = 2 * CQ + CR + 1;
+    auto place = [&](const Rows& x, int r) {   // of head row r, in bytes
+      const int s = row_div(a, r);
+      return ((int64_t)s * x.row + (int64_t)(r - s * a.per) * x.head) * 2;
+    };
+    auto base_of = [&](const Rows& x) {
+      return reinterpret_cast<const char*>(x.p + (int64_t)seq.r0 * x.row + (int64_t)n * a.per * x.head);
+    };
+    const char* const qb = base_of(a.q);
+    const char* const db = base_of(a.d);
+    const char* const qrb = DR ? base_of(a.qr) : nullptr;
+    const int64_t stat0 = n * (int64_t)a.len.rows * a.per + (int64_t)seq.r0 * a.per;
+    const float* const stat = ((wave & 1) ? a.delta : a.lse) + stat0;   // (two waves each, the same values)
+    const uint32_t q_lds = lds_addr(L.t[0].q) + wave * 1024, r_lds = lds_addr(L.qr[0]) + wave * 1024;
+    const uint32_t s_lds = lds_addr((wave & 1) ? L.delta[0] : L.lse[0]);
+    // (linear) of the tile that is loaded next: bases, and this lane's offsets from them
+    const int64_t q_step = (int64_t)(BN >> a.per_shift) * a.q.row * 2, d_step = (int64_t)(BN >> a.per_shift) * a.d.row * 2,
+                  r_step = DR ? (int64_t)(BN >> a.per_shift) * a.qr.row * 2 : 0;
+    const char* qn = qb + (int64_t)(first_row(0) >> a.per_shift) * a.q.row * 2;
+    const char* dn = db + (int64_t)(first_row(0) >> a.per_shift) * a.d.row * 2;
+    const char* rn = DR ? qrb + (int64_t)(first_row(0) >> a.per_shift) * a.qr.row * 2 : nullptr;
+    uint32_t q_off[CQ], d_off[CQ], r_off[CR ? CR : 1];
+    int load_row = first_row(0);
+    auto aim = [&]() __attribute__((always_inline)) {
+      if constexpr (LINEAR) {
+        const int last = r_hi - 1 - load_row;
 #pragma unroll
-  for (int u = 1; u < AHEAD; ++u)
-    if (u < ntiles) load_tile(u, u);
-  uint4 opf[KS];   // this wave's K (first) or V (second)
-  {
-    const int64_t tt = seq.k0 + min(t, t_seen - 1);
-    const Rows& x = second ? a.v : a.k;
-    const uint16_t* p = x.p + tt * x.row + n * x.head + kg * 8;
+        for (int i = 0; i < CQ; ++i) {
+          const int r = min(i * Sh::STEP + sh.row, last);
+          q_off[i] = (uint32_t)place(a.q, r) + sh.col;
+          d_off[i] = (uint32_t)place(a.d, r) + sh.col;
+        }
+        if constexpr (DR > 0)
 #pragma unroll
-    for (int j = 0; j < KSN; ++j) opf[j] = ldg16(p + j * 16);
-    if constexpr (DR > 0)
-      if (!second) {
+          for (int i = 0; i < CR; ++i) r_off[i] = (uint32_t)place(a.qr, min(i * ShR::STEP + shr.row, last)) + shr.col;
+      }
+    };
+    auto load_part = [&](auto jc, int buf) __attribute__((always_inline)) {
+      constexpr int j = decltype(jc)::value;
+      constexpr int what = j == GPW - 1 ? 3 : j < CQ ? 0 : j < 2 * CQ ? 1 : 2, i = what == 0 ? j : what == 1 ? j - CQ : what == 2 ? j - 2 * CQ : 0;
+      if constexpr (what == 3) {
+        lds_dma4(stat + min(load_row + lane, r_hi - 1), (void*)(__attribute__((address_space(3))) void*)(uintptr_t)(s_lds + buf * (BN * 4)));
+      } else {
+        const uint32_t dst = what == 2 ? r_lds + buf * (BN * 128) : q_lds + buf * (2 * BN * RB);
+        constexpr int at = (what == 1 ? BN * RB : 0) + i * NWV * 1024;
+        if constexpr (LINEAR) {
+          lds_dma16_at<at>(what == 0 ? qn : what == 1 ? dn : rn, what == 0 ? q_off[what == 0 ? i : 0] : what == 1 ? d_off[what == 1 ? i : 0] : r_off[what == 2 ? i : 0], dst);
+        } else {
+          const int r = min(load_row + i * (what == 2 ? ShR::STEP : Sh::STEP) + (what == 2 ? shr.row : sh.row), r_hi - 1);
+          lds_dma16_untracked((what == 0 ? qb : what == 1 ? db : qrb) + place(what == 0 ? a.q : what == 1 ? a.d : a.qr, r) + (what == 2 ? shr.col : sh.col),
+                              (void*)(__attribute__((address_space(3))) void*)(uintptr_t)(dst + at));
+        }
+      }
+    };
+    auto load_tile = [&](int buf) __attribute__((always_inline)) {
+      static_for<0, GPW>([&](auto j) __attribute__((always_inline)) { load_part(j, buf); });
+    };
+    // from tile u - 1 to tile u
+    auto advance = [&](int u) __attribute__((always_inline)) {
+      if (u >= ntiles) return;
+      load_row -= BN;
+      if constexpr (LINEAR) {
+        qn = uniform(qn - q_step);
+        dn = uniform(dn - d_step);
+        if constexpr (DR > 0) rn = uniform(rn - r_step);
+      }
+      if (u == 1) aim();   // (whole from here on)
+    };
+    // (a masked pair has P = dS = 0, but 0 times a value that is not finite would reach tokens that the row does not see)
+    auto is_mixed = [&](int u) { return first_row(u) < r_full || first_row(u) + BN > r_hi; };
+    auto sanitize = [&](int u, int buf) __attribute__((always_inline)) {
+      if (!is_mixed(u)) return;
+      uint64_t bad = clean_share<IO, RB, BN, NWV>(lds_addr(L.t[buf].q), wave, lane) |
+                     clean_share<IO, RB, BN, NWV>(lds_addr(L.t[buf].d), wave, lane);
+      if constexpr (DR > 0) bad |= clean_share<IO, 128, BN, NWV>(lds_addr(L.qr[buf]), wave, lane);
+      if (lane == 0) L.bad[buf][wave] = bad;
+    };
+    aim();
+    load_tile(0);
+    uint4 kf[KS], vf[KSN];
+    {
+      const int64_t tt = seq.k0 + min(t, t_seen - 1);
+      const uint16_t* kp = a.k.p + tt * a.k.row + n * a.k.head + kg * 8;
+      const uint16_t* vp = a.v.p + tt * a.v.row + n * a.v.head + kg * 8;
+#pragma unroll
+      for (int j = 0; j < KSN; ++j) kf[j] = ldg16(kp + j * 16), vf[j] = ldg16(vp + j * 16);
+      if constexpr (DR > 0) {
         const uint16_t* rp = a.kr.p + tt * a.kr.row + n * a.kr.head + kg * 8;
 #pragma unroll
-        for (int j = KSN; j < KS; ++j) opf[j] = ldg16(rp + (j - KSN) * 16);
-      }
-  }
-
-  // ---- operands
-  constexpr int DOFF = KB * D * 2;   // from a place in q to the same in d
-  const int qk = s_row(rr), g16 = lane >> 4, c16 = lane & 15;
-  const int r4 = (g16 >> 1) * 8 + (c16 >> 2), vc = (g16 & 1) * 2 + ((c16 & 3) >> 1), o8 = (c16 & 1) * 8;
-  const uint32_t op_lane = tile_off<RB>(qk, kg), opr_lane = tile_off<128>(qk, kg);
-  const uint32_t tr_lo = tile_off<RB>(r4, vc) + o8, tr_hi = tile_off<RB>(r4 + 4, vc) + o8;
-  const uint32_t trr_lo = tile_off<128>(r4, vc) + o8, trr_hi = tile_off<128>(r4 + 4, vc) + o8;
-  OpAddr<RB> op;
-  OpAddr<128> opr;
-  TrAddr<RB> tr;
-  TrAddr<128> trr;
-  constexpr int OR = 4, TR = 4;
-  std::true_type yes;
-  std::false_type no;
-  uint32_t words[8];   // the tile before: P (first) or dS (second)
-
-  if (!second) {
-#pragma unroll
-    for (int j = 0; j < KS; ++j) opf[j] = in_agprs(opf[j]);
-    f32x16 acc[ON];
-#pragma unroll
-    for (int c = 0; c < ON; ++c)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[c][i] = 0.f;
-    // phase u: S of tile u, dV of tile u - 1, P of tile u
-    auto phase = [&](auto sc, auto vc, int u) __attribute__((always_inline)) {
-      constexpr bool S = decltype(sc)::value, DV = decltype(vc)::value;
-      f32x16 s;
-      float4 lse4[4];
-      uint4 of[OR], tf[TR];
-      if constexpr (S) {
-        op.point(lds_addr(L.t[buf].q), op_lane);
-        if constexpr (DR > 0) opr.point(lds_addr(L.qr[buf]), opr_lane);
-      }
-      auto q_frag = [&](int j) __attribute__((always_inline)) -> uint4 {
-        return lds_read16_at(j < KSN ? op.a[j < KSN ? j : 0] : opr.a[j >= KSN ? j - KSN : 0]);
-      };
-      auto t_frag = [&](int i) __attribute__((always_inline)) -> uint4 { return tr.frag(i % ON, (i / ON) * 16 * RB + DOFF); };
-      if constexpr (S) {
-#pragma unroll
-        for (int j = 0; j < OR; ++j) of[j] = q_frag(j);
-      }
-      if constexpr (DV) tr.point(lds_addr(L.t[before(buf)].q), tr_lo, tr_hi);
-      if constexpr (S) {
-        static_for<0, KS>([&](auto jc) __attribute__((always_inline)) {
-          constexpr int j = decltype(jc)::value;
-          if constexpr (j < KS - 1) mfma32_va<IO, j == 0>(s, of[j % OR], opf[j]);
-          else mfma32_va_last<IO>(s, of[j % OR], opf[j]);
-          if constexpr (j + OR < KS) of[j % OR] = q_frag(j + OR);
-          if constexpr (j >= KS - 4) lse4[j - (KS - 4)] = *reinterpret_cast<const float4*>(
-              &L.lse[buf][16 * ((j - (KS - 4)) >> 1) + 8 * kg + 4 * ((j - (KS - 4)) & 1)]);
-          if constexpr (DV && j >= KS - TR && j - (KS - TR) < 2 * ON) tf[j - (KS - TR)] = t_frag(j - (KS - TR));
-          __builtin_amdgcn_sched_barrier(0);
-        });
-      } else {
-#pragma unroll
-        for (int i = 0; i < TR; ++i) tf[i] = t_frag(i);
-      }
-      auto exps = [&](int e) __attribute__((always_inline)) {   // two rows
-        const float4 l = lse4[e >> 1];
-        s[2 * e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e], sl2, -(e & 1 ? l.z : l.x)));
-        s[2 * e + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e + 1], sl2, -(e & 1 ? l.w : l.y)));
-      };
-      if constexpr (DV)
-        static_for<0, 2 * ON>([&](auto ic) __attribute__((always_inline)) {
-          constexpr int i = decltype(ic)::value, st = i / ON;
-          acc[i % ON] = Mfma<IO>::m32(tf[i % TR], make_uint4(words[4 * st], words[4 * st + 1], words[4 * st + 2], words[4 * st + 3]), acc[i % ON]);
-          if constexpr (i + TR < 2 * ON) tf[i % TR] = t_frag(i + TR);
-          if constexpr (S)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (e * 2 * ON / 8 == i) exps(e);
-          __builtin_amdgcn_sched_barrier(0);
-        });
-      else if constexpr (S)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) exps(e);
-      if constexpr (S) {
-        if (is_mixed(u)) {
-          int k = kg;
-          asm volatile("" : "+v"(k));   // (what follows from it is not kept in registers for these few tiles)
-          const uint32_t bad = bad_rows(buf);
-          const int r0 = first_row(u), first = my_first - r0, last = r_hi - r0;   // rows [first, last) see the token
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int x = s_token(i, k);
-            if ((bad >> x) & 1u) s[i] = __builtin_nanf("");
-            if (x < first || x >= last) s[i] = 0.f;
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) L.p[u & 1][pair][e][lane] = make_float4(s[4 * e], s[4 * e + 1], s[4 * e + 2], s[4 * e + 3]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) words[e] = pack2<IO>(s[2 * e], s[2 * e + 1]);
+        for (int j = KSN; j < KS; ++j) kf[j] = ldg16(rp + (j - KSN) * 16);
       }
 #pragma unroll
-      for (int c = 0; c < ON; ++c) asm volatile("" : "+a"(acc[c]));   // whole accumulators, in AGPRs, from phase to phase
-      buf = next(buf);
-    };
-    begin(0);
-    phase(yes, no, 0);
-    if (ntiles > 1) {
-      int u = 1;
-      do {
-        u = __builtin_amdgcn_readfirstlane(u);
-        begin(u);
-        phase(yes, yes, u);
-      } while (++u < ntiles);
+      for (int j = 0; j < KS; ++j) kf[j] = in_agprs(kf[j]);
+#pragma unroll
+      for (int j = 0; j < KSN; ++j) vf[j] = in_agprs(vf[j]);
     }
-    begin(ntiles);
-    phase(no, yes, ntiles);
-    begin(ntiles + 1);
-    finish(n_dv, acc, IO == IO_F16 ? 0x1p-15f : 1.f);
-  } else {
-#pragma unroll
-    for (int j = 0; j < KSN; ++j) opf[j] = in_agprs(opf[j]);
+
+    // ---- operands
+    constexpr int DOFF = BN * D * 2;   // from a place in q to the same in d
+    const int qk = s_row(rr), g16 = lane >> 4, c16 = lane & 15;
+    const int r4 = (g16 >> 1) * 8 + (c16 >> 2), vc = (g16 & 1) * 2 + ((c16 & 3) >> 1), o8 = (c16 & 1) * 8;
+    const uint32_t op_lane = tile_off<RB>(qk, kg), opr_lane = tile_off<128>(qk, kg);
+    const uint32_t tr_lo = tile_off<RB>(r4, vc) + o8, tr_hi = tile_off<RB>(r4 + 4, vc) + o8;
+    const uint32_t trr_lo = tile_off<128>(r4, vc) + o8, trr_hi = tile_off<128>(r4 + 4, vc) + o8;
+    OpAddr<RB> op;
+    OpAddr<128> opr;
+    TrAddr<RB> tr;
+    TrAddr<128> trr;
+    auto point_op = [&](int buf) __attribute__((always_inline)) {
+      op.point(lds_addr(L.t[buf].q), op_lane);
+      if constexpr (DR > 0) opr.point(lds_addr(L.qr[buf]), opr_lane);
+    };
+    auto point_tr = [&](int buf) __attribute__((always_inline)) {
+      tr.point(lds_addr(L.t[buf].q), tr_lo, tr_hi);
+      if constexpr (DR > 0) trr.point(lds_addr(L.qr[buf]), trr_lo, trr_hi);
+    };
+    auto q_frag = [&](int j, int h) __attribute__((always_inline)) -> uint4 {
+      return lds_read16_at(j < KSN ? op.a[j < KSN ? j : 0] + h * 32 * RB : opr.a[j >= KSN ? j - KSN : 0] + h * 32 * 128);
+    };
+    auto d_frag = [&](int j, int h) __attribute__((always_inline)) -> uint4 { return lds_read16_at(op.a[j] + h * 32 * RB + DOFF); };
+    // product i of a half's NP: column tiles of dV, dK and dK's rotary part for 16 rows, then for the next 16
+    constexpr int NC = 2 * ON + RN, NP = 2 * NC;
+    auto t_frag = [&](int i, int h) __attribute__((always_inline)) -> uint4 {
+      const int st = i / NC, c = i % NC;
+      if (c < ON) return tr.frag(c < ON ? c : 0, (h * 32 + st * 16) * RB + DOFF);
+      if (c < 2 * ON) return tr.frag(c >= ON && c < 2 * ON ? c - ON : 0, (h * 32 + st * 16) * RB);
+      return trr.frag(c >= 2 * ON ? c - 2 * ON : 0, (h * 32 + st * 16) * 128);
+    };
+
+    // ---- P and dS of 32 rows in NST stages of two rows each, placed among the products before and after them
+    constexpr int NST = 8;
+    struct Four {
+      float4 v[4];   // rows 16 x + 8 kg + 4 y + 0 .. 3 at [2 x + y]
+    };
+    auto four = [&](const float* p, int e) __attribute__((always_inline)) {
+      return *reinterpret_cast<const float4*>(p + 16 * (e >> 1) + 8 * kg + 4 * (e & 1));
+    };
+    // dP starts from -delta
+    auto start = [&](f32x16& d, const float* p, int e) __attribute__((always_inline)) {
+      const float4 v = four(p, e);
+      d[4 * e] = v.x, d[4 * e + 1] = v.y, d[4 * e + 2] = v.z, d[4 * e + 3] = v.w;
+    };
     const float f16 = factor.x * 0x1p-15f;   // (fp16's P has the factor 2^15)
-    f32x16 acc[AN];
+    auto stage = [&](int st, f32x16& sv, f32x16& dp, Four& lse, uint32_t (&pw)[8], uint32_t (&sw)[8]) __attribute__((always_inline)) {
+      const int i = 2 * st;
+      const float4 l4 = lse.v[i >> 2];
+      const float l0 = i & 2 ? l4.z : l4.x, l1 = i & 2 ? l4.w : l4.y;
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], sl2, -l0));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i + 1], sl2, -l1));
+      float w0 = p0 * dp[i], w1 = p1 * dp[i + 1];
+      if constexpr (IO == IO_F16) w0 *= f16, w1 *= f16;
+      pw[st] = pack2<IO>(p0, p1);
+      sw[st] = pack2<IO>(w0, w1);
+      asm volatile("" : "+v"(pw[st]), "+v"(sw[st]));   // here, not where the next step needs them
+    };
+    auto mask = [&](int u, int buf, int h, uint32_t (&pw)[8], uint32_t (&sw)[8]) __attribute__((always_inline)) {
+      if (!is_mixed(u)) return;
+      const uint64_t all = L.bad[buf][0] | L.bad[buf][1] | L.bad[buf][2] | L.bad[buf][3];
+      const uint32_t bad = (uint32_t)(all >> (h * 32));
+      const int r0 = first_row(u) + h * 32, first = my_first - r0, last = r_hi - r0;   // rows [first, last) see the token
+      int k = kg;
+      asm volatile("" : "+v"(k));   // (what follows from it is not kept in registers for these few tiles)
 #pragma unroll
-    for (int c = 0; c < AN; ++c)
+      for (int i = 0; i < 8; ++i) {
+        const int x = s_token(2 * i, k);
+        const uint32_t nan = ((bad >> x) & 1u ? 0x7FFFu : 0u) | ((bad >> (x + 1)) & 1u ? 0x7FFF0000u : 0u);
+        const uint32_t keep = (x >= first && x < last ? 0xFFFFu : 0u) | (x + 1 >= first && x + 1 < last ? 0xFFFF0000u : 0u);
+        pw[i] = (pw[i] | nan) & keep;
+        sw[i] = (sw[i] | nan) & keep;
+      }
+    };
+
+    // ---- One step handles 32 rows: the products of the rows before them, S and dP of the rows after them, each MFMA
+    // followed by a part of this one's P and dS. Fragments are read a few MFMAs ahead.
+    constexpr int LAG = KS - KSN, NS = KS + KSN;   // S and dP end together
+    constexpr int TR = 4, QR = 4, DRING = 4;
+    uint4 tf[TR], qf[QR], df[DRING];
+    // (nbuf: the buffer of the rows whose S and dP are made here)
+    auto step = [&](auto pvc, auto sc, auto hc, int nbuf, f32x16& cs, f32x16& cd, Four& cl, f32x16& ns, f32x16& nd, Four& nl,
+                    uint32_t (&pb)[8], uint32_t (&sb)[8], uint32_t (&pn)[8], uint32_t (&sn)[8], auto&& between, auto&& ride) __attribute__((always_inline)) {
+      constexpr bool PV = decltype(pvc)::value, S = decltype(sc)::value;
+      constexpr int H = decltype(hc)::value;
+      constexpr int M0 = PV ? NP : 0, NMM = M0 + (S ? NS : 0), LEAD = NMM > 8 ? 2 : 0;
+      auto values_at = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[c][i] = 0.f;
-    // phase u: dP and dS of tile u - 1, dK of tile u - 2
-    auto phase = [&](auto sc, auto kc, int u) __attribute__((always_inline)) {
-      constexpr bool S = decltype(sc)::value, DK = decltype(kc)::value;
-      constexpr int NC = ON + RN, NP = 2 * NC;
-      const int vb = before(buf), kb = before(vb);
-      f32x16 d;
-      float4 p4[4];
-      uint4 of[OR], tf[TR];
-      auto d_frag = [&](int j) __attribute__((always_inline)) -> uint4 { return lds_read16_at(op.a[j] + DOFF); };
-      auto t_frag = [&](int i) __attribute__((always_inline)) -> uint4 {
-        const int st = i / NC, c = i % NC;
-        if (c < ON) return tr.frag(c < ON ? c : 0, st * 16 * RB);
-        return trr.frag(c >= ON ? c - ON : 0, st * 16 * 128);
+        for (int st = 0; st < NST; ++st)
+          if (LEAD + st * (NMM - LEAD) / NST == slot) stage(st, cs, cd, cl, pn, sn);
       };
-      if constexpr (S) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {   // dP - delta
-          const float4 v = *reinterpret_cast<const float4*>(&L.delta[vb][16 * (e >> 1) + 8 * kg + 4 * (e & 1)]);
-          d[4 * e] = v.x, d[4 * e + 1] = v.y, d[4 * e + 2] = v.z, d[4 * e + 3] = v.w;
-        }
-        op.point(lds_addr(L.t[vb].q), op_lane);
-#pragma unroll
-        for (int j = 0; j < OR; ++j) of[j] = d_frag(j);
-      }
-      if constexpr (DK) {
-        tr.point(lds_addr(L.t[kb].q), tr_lo, tr_hi);
-        if constexpr (DR > 0) trr.point(lds_addr(L.qr[kb]), trr_lo, trr_hi);
-      }
-      if constexpr (S) {
-        static_for<0, KSN>([&](auto jc) __attribute__((always_inline)) {
-          constexpr int j = decltype(jc)::value;
-          if constexpr (j < KSN - 1) mfma32_va<IO, false>(d, of[j % OR], opf[j]);
-          else mfma32_va_last<IO>(d, of[j % OR], opf[j]);
-          if constexpr (j + OR < KSN) of[j % OR] = d_frag(j + OR);
-          if constexpr (j >= KSN - 4) p4[j - (KSN - 4)] = L.p[(u - 1) & 1][pair][j - (KSN - 4)][lane];
-          if constexpr (DK && j >= KSN - TR) tf[j - (KSN - TR)] = t_frag(j - (KSN - TR));
-          __builtin_amdgcn_sched_barrier(0);
-        });
-      } else {
-#pragma unroll
-        for (int i = 0; i < TR; ++i) tf[i] = t_frag(i);
-      }
-      uint32_t fresh[8];
-      auto values = [&](int e) __attribute__((always_inline)) {   // two rows
-        const float4 p = p4[e >> 1];
-        float x = (e & 1 ? p.z : p.x) * d[2 * e], y = (e & 1 ? p.w : p.y) * d[2 * e + 1];
-        if constexpr (IO == IO_F16) x *= f16, y *= f16;
-        fresh[e] = pack2<IO>(x, y);
-        asm volatile("" : "+v"(fresh[e]));   // here, not where the next phase needs it
-      };
-      if constexpr (DK)
+      if constexpr (PV)
         static_for<0, NP>([&](auto ic) __attribute__((always_inline)) {
           constexpr int i = decltype(ic)::value, st = i / NC, c = i % NC;
-          acc[c] = Mfma<IO>::m32(tf[i % TR], make_uint4(words[4 * st], words[4 * st + 1], words[4 * st + 2], words[4 * st + 3]), acc[c]);
-          if constexpr (i + TR < NP) tf[i % TR] = t_frag(i + TR);
-          if constexpr (S)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (e * NP / 8 == i) values(e);
+          const uint4 b = c < ON ? make_uint4(pb[4 * st], pb[4 * st + 1], pb[4 * st + 2], pb[4 * st + 3])
+                                 : make_uint4(sb[4 * st], sb[4 * st + 1], sb[4 * st + 2], sb[4 * st + 3]);
+          if constexpr (c < ON) dv[c] = Mfma<IO>::m32(tf[i % TR], b, dv[c]);
+          else dk[c - ON] = Mfma<IO>::m32(tf[i % TR], b, dk[c - ON]);
+          if constexpr (i + TR < NP) tf[i % TR] = t_frag(i + TR, H);
+          if constexpr (S)   // meanwhile, what the next ones begin with
+            static_for<0, 4 + QR + DRING>([&](auto gc) __attribute__((always_inline)) {
+              constexpr int g = decltype(gc)::value;
+              if constexpr (g * NP / (4 + QR + DRING) == i) {
+                if constexpr (g < 4) start(nd, &L.delta[nbuf][H * 32], g);
+                else if constexpr (g < 4 + QR) qf[g - 4] = q_frag(g - 4, H);
+                else df[g - 4 - QR] = d_frag(g - 4 - QR, H);
+              }
+            });
+          values_at(i);
           __builtin_amdgcn_sched_barrier(0);
         });
-      else if constexpr (S)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) values(e);
-      if constexpr (S) {
-        if (is_mixed(u - 1)) {
-          int k = kg;
-          asm volatile("" : "+v"(k));   // (what follows from it is not kept in registers for these few tiles)
-          const uint32_t bad = bad_rows(vb);
-          const int r0 = first_row(u - 1), first = my_first - r0, last = r_hi - r0;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int x = s_token(2 * e, k);
-            const uint32_t nan = ((bad >> x) & 1u ? 0x7FFFu : 0u) | ((bad >> (x + 1)) & 1u ? 0x7FFF0000u : 0u);
-            const uint32_t keep = (x >= first && x < last ? 0xFFFFu : 0u) | (x + 1 >= first && x + 1 < last ? 0xFFFF0000u : 0u);
-            fresh[e] = (fresh[e] | nan) & keep;
+      between();
+      if constexpr (S)
+        static_for<0, NS>([&](auto jc) __attribute__((always_inline)) {
+          constexpr int j = decltype(jc)::value;
+          constexpr bool is_s = j < LAG || (j - LAG) % 2 == 0;
+          constexpr int i = j < LAG ? j : is_s ? LAG + (j - LAG) / 2 : (j - LAG) / 2;   // step of its chain
+          if constexpr (j == NS - 1) mfma32_va_end2<IO>(ns, qf[(KS - 1) % QR], kf[KS - 1], nd, df[(KSN - 1) % DRING], vf[KSN - 1]);
+          else if constexpr (is_s && i < KS - 1) {
+            mfma32_va<IO, i == 0>(ns, qf[i % QR], kf[i]);
+            if constexpr (i + QR < KS) qf[i % QR] = q_frag(i + QR, H);
+          } else if constexpr (!is_s) {
+            mfma32_va<IO, false>(nd, df[i % DRING], vf[i]);
+            if constexpr (i + DRING < KSN) df[i % DRING] = d_frag(i + DRING, H);
           }
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) words[e] = fresh[e];
-      }
-#pragma unroll
-      for (int c = 0; c < AN; ++c) asm volatile("" : "+a"(acc[c]));
-      buf = next(buf);
+          if constexpr (j >= NS - TR) tf[j - (NS - TR)] = t_frag(j - (NS - TR), 1 - H);
+          else if constexpr (j >= NS - TR - 4) nl.v[j - (NS - TR - 4)] = four(&L.lse[nbuf][H * 32], j - (NS - TR - 4));
+          ride(jc);
+          values_at(M0 + j);
+          __builtin_amdgcn_sched_barrier(0);
+        });
     };
-    begin(0);
-    buf = next(buf);
-    begin(1);
-    phase(yes, no, 1);
+    std::true_type yes;
+    std::false_type no;
+    std::integral_constant<int, 0> h0;
+    std::integral_constant<int, 1> h1;
+    auto nothing = [](auto...) __attribute__((always_inline)) {};
+
+    wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    sanitize(0, 0);
+    lds_barrier();
+    advance(1);
+    load_tile(1);
+    f32x16 s0, s1, d0, d1;
+    Four l0, l1;
+    uint32_t p0[8], p1[8], w0[8], w1[8];
+    point_op(0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      start(d0, L.delta[0], e);
+      start(d1, &L.delta[0][32], e);
+      l0.v[e] = four(L.lse[0], e);
+    }
+#pragma unroll
+    for (int j = 0; j < KS - 1; ++j) {
+      const uint4 f = q_frag(j, 0);
+      if (j == 0) mfma32_va<IO, true>(s0, f, kf[j]);
+      else mfma32_va<IO, false>(s0, f, kf[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < KSN - 1; ++j) mfma32_va<IO, false>(d0, d_frag(j, 0), vf[j]);
+    mfma32_va_end2<IO>(s0, q_frag(KS - 1, 0), kf[KS - 1], d0, d_frag(KSN - 1, 0), vf[KSN - 1]);
+#pragma unroll
+    for (int j = 0; j < QR; ++j) qf[j] = q_frag(j, 1);
+#pragma unroll
+    for (int j = 0; j < DRING; ++j) df[j] = d_frag(j, 1);
+    int buf = 0;   // of tile u
+    // Step (u, 0): tile u + 1 has landed by the middle of it, when nobody needs tile u - 1 any more
+    auto half0 = [&](auto pvc, int u) __attribute__((always_inline)) {
+      const int nb = buf == NBUF - 1 ? 0 : buf + 1, lb = buf == 0 ? NBUF - 1 : buf - 1;   // of tiles u + 1 and u - 1 (u + 2)
+      advance(u + 2);
+      step(pvc, yes, h1, buf, s0, d0, l0, s1, d1, l1, p1, w1, p0, w0,
+           [&]() __attribute__((always_inline)) {
+             wait_vmcnt<0>();
+             asm volatile("" ::: "memory");
+             if (u + 1 < ntiles) sanitize(u + 1, nb);
+             lds_barrier();
+             point_tr(buf);
+           },
+           [&](auto jc) __attribute__((always_inline)) {
+             constexpr int j = decltype(jc)::value;
+             static_for<0, GPW>([&](auto g) __attribute__((always_inline)) {
+               if constexpr (g * NS / GPW == j) load_part(g, lb);
+             });
+           });
+      mask(u, buf, 0, p0, w0);
+    };
+    half0(no, 0);
     if (ntiles > 1) {
-      int u = 2;
+      int u = 0;
       do {
         u = __builtin_amdgcn_readfirstlane(u);
-        begin(u);
-        phase(yes, yes, u);
-      } while (++u <= ntiles);
+        const int nb = buf == NBUF - 1 ? 0 : buf + 1;
+        point_op(nb);
+        step(yes, yes, h0, nb, s1, d1, l1, s0, d0, l0, p0, w0, p1, w1, nothing, nothing);
+        mask(u, buf, 1, p1, w1);
+        buf = nb;
+        half0(yes, u + 1);
+      } while (++u + 1 < ntiles);
     }
-    begin(ntiles + 1);
-    phase(no, yes, ntiles + 1);
-    finish(n_dk, acc, a.scale * factor.y);
+    step(yes, no, h0, 0, s1, d1, l1, s0, d0, l0, p0, w0, p1, w1, nothing, nothing);
+    mask(ntiles - 1, buf, 1, p1, w1);
+#pragma unroll
+    for (int i = 0; i < TR; ++i) tf[i] = t_frag(i, 1);
+    static_for<0, NP>([&](auto ic) __attribute__((always_inline)) {
+      constexpr int i = decltype(ic)::value, st = i / NC, c = i % NC;
+      const uint4 b = c < ON ? make_uint4(p1[4 * st], p1[4 * st + 1], p1[4 * st + 2], p1[4 * st + 3])
+                             : make_uint4(w1[4 * st], w1[4 * st + 1], w1[4 * st + 2], w1[4 * st + 3]);
+      if constexpr (c < ON) dv[c] = Mfma<IO>::m32(tf[i % TR], b, dv[c]);
+      else dk[c - ON] = Mfma<IO>::m32(tf[i % TR], b, dk[c - ON]);
+      if constexpr (i + TR < NP) tf[i % TR] = t_frag(i + TR, 1);
+    });
+    wait_vmcnt<0>();   // the last (unused) loads land before the LDS is released
   }
+
+  // lane l: token t, columns c * 32 + 8 g + 4 kg + j
+  const float fk = a.scale * factor.y, fv = IO == IO_F16 ? 0x1p-15f : 1.f;
+  if (a.k_splits > 1) {
+    const int blk = n * (a.k_blocks / a.key_heads) + seq.k0 / 32 + b + at.tile * NWV + wave;
+    if (t0 + wave * 32 >= seq.keys) return;
+    float4* dst = a.k_part + ((int64_t)at.sp * a.k_blocks + blk) * ((2 * D + DR) / 8) * 64 + lane;
+#pragma unroll
+    for (int c = 0; c < ON + RN + ON; ++c) {
+      const f32x16& v = c < ON + RN ? dk[c < ON + RN ? c : 0] : dv[c >= ON + RN ? c - ON - RN : 0];
+      const float f = c < ON + RN ? fk : fv;
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        dst[(c * 4 + g) * 64] = make_float4(v[4 * g] * f, v[4 * g + 1] * f, v[4 * g + 2] * f, v[4 * g + 3] * f);
+    }
+    return;
+  }
+  const bool live = t < t_seen, valid = t < t_end;
+  const int64_t tt = (int64_t)(seq.k0 + t) * a.key_heads + n;
+  auto store = [&](const f32x16& v, float f, uint16_t* dst) __attribute__((always_inline)) {
+    uint4 w[2];
+    pack_tile<IO>(v, f, w);
+    if (valid) {
+      stg16(dst + 8 * kg, live ? w[0] : make_uint4(0, 0, 0, 0));
+      stg16(dst + 8 * kg + 16, live ? w[1] : make_uint4(0, 0, 0, 0));
+    }
+  };
+#pragma unroll
+  for (int c = 0; c < ON; ++c) store(dk[c], fk, a.dk + tt * D + c * 32);
+#pragma unroll
+  for (int c = 0; c < RN; ++c) store(dk[ON + c], fk, a.dkr + tt * DR + c * 32);
+#pragma unroll
+  for (int c = 0; c < ON; ++c) store(dv[c], fv, a.dv + tt * D + c * 32);
 }
 
 // ---------------------------------------------------------------- queries
@@ -719,9 +686,9 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
       if constexpr (DR > 0) rs.aim(last);
     };
     auto move = [&](int64_t tiles) __attribute__((always_inline)) {
-      ks.base += tiles * (int64_t)BN * ks.row_bytes;
-      vs.base += tiles * (int64_t)BN * vs.row_bytes;
-      if constexpr (DR > 0) rs.base += tiles * (int64_t)BN * rs.row_bytes;
+      ks.base = uniform(ks.base + tiles * (int64_t)BN * ks.row_bytes);
+      vs.base = uniform(vs.base + tiles * (int64_t)BN * vs.row_bytes);
+      if constexpr (DR > 0) rs.base = uniform(rs.base + tiles * (int64_t)BN * rs.row_bytes);
     };
     // the streams to tile u, from the tile before it
     auto advance = [&](int u) __attribute__((always_inline)) {
@@ -1109,7 +1076,8 @@ hipError_t launch_d(const GradK& k, const Cut& c, hipStream_t s) {
   hipLaunchKernelGGL((dense_queries_kernel<IO, D, DR>), dim3((unsigned)c.queries.groups), dim3(NWV * 64), 0, s, k);
   if (c.queries.splits > 1)
     hipLaunchKernelGGL((dense_join_kernel<IO, D, DR, false>), dim3((unsigned)c.queries.blocks), dim3(256), 0, s, k);
-  hipLaunchKernelGGL((dense_keys_kernel<IO, D, DR>), dim3((unsigned)c.keys.groups), dim3(KW * 64), 0, s, k);
+  if (k.linear) hipLaunchKernelGGL((dense_keys_kernel<IO, D, DR, true>), dim3((unsigned)c.keys.groups), dim3(NWV * 64), 0, s, k);
+  else hipLaunchKernelGGL((dense_keys_kernel<IO, D, DR, false>), dim3((unsigned)c.keys.groups), dim3(NWV * 64), 0, s, k);
   if (c.keys.splits > 1)
     hipLaunchKernelGGL((dense_join_kernel<IO, D, DR, true>), dim3((unsigned)c.keys.blocks), dim3(256), 0, s, k);
   return hipGetLastError();
@@ -1132,7 +1100,7 @@ hipError_t launch_dense_grad(const DenseGradArgs& g, size_t* lacking, hipStream_
   const Cut c = make_cut(g);
   *lacking = !a.ws || a.ws_bytes < c.bytes || ((uintptr_t)a.ws & 15) != 0 ? c.bytes : 0;
   if (*lacking) return hipSuccess;
-  if (c.keys.groups >= (1 << 23) || c.queries.groups >= (1 << 24)) return hipErrorInvalidConfiguration;   // 2^32 threads
+  if (c.keys.groups >= (1 << 24) || c.queries.groups >= (1 << 24)) return hipErrorInvalidConfiguration;   // 2^32 threads
   GradK k{};
   auto rows = [](const DenseTensor& t) { return Rows{(const uint16_t*)t.p, t.row, t.head}; };
   k.q = rows(a.q), k.qr = rows(a.qr), k.k = rows(a.k), k.kr = rows(a.kr), k.v = rows(a.v), k.d = rows(g.d_out), k.o = rows(g.out);
