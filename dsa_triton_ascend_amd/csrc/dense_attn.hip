@@ -487,15 +487,19 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
 }
 
 // Joins the ranges of 32 head rows: M = max m_s, out = sum O_s 2^(m_s - M) / sum l_s 2^(m_s - M); rows that see nothing
-// get zeros. A work-group has a block of 32 head rows; its waves take the D / 8 groups of 8 columns.
+// get zeros. A work-group has 32 columns of a block of 32 head rows. All its threads fetch the ranges' statistics at once,
+// its waves take every fourth range, and their sums are added in the order of the waves.
 constexpr int MAX_SPLITS = 64;
 template <int IO, int D>
 __global__ __launch_bounds__(256) void dense_merge_kernel(DenseK a) {
   __shared__ float s_w[MAX_SPLITS][32];
-  __shared__ float s_inv[32];
+  __shared__ float2 s_top[8][32];   // of the ranges that 32 threads have: largest reference, true maximum
+  __shared__ float s_sum[8][32];
+  __shared__ float4 s_part[3][4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rr = lane & 31, kg = lane >> 5;
   // the sequence of this block
-  const int per_head = a.blocks / a.tiles.heads, n = (int)blockIdx.x / per_head, i = (int)blockIdx.x - n * per_head;
+  const int block = blockIdx.x / (D / 32), col = blockIdx.x % (D / 32);
+  const int per_head = a.blocks / a.tiles.heads, n = block / per_head, i = block - n * per_head;
   auto first = [&](int s) { return (int)((int64_t)a.len.row_start[s] * a.per / 32) + s; };
   int lo = 0, up = a.tiles.seqs - 1;
   while (lo < up) {
@@ -508,52 +512,82 @@ __global__ __launch_bounds__(256) void dense_merge_kernel(DenseK a) {
   const int row = r0 + rr, s = row / a.per, g = row - s * a.per;
   const bool valid = row < (int64_t)seq.rows * a.per;
   const int lim = valid ? limit_of(a.len, seq, s) : 0;
-  if (threadIdx.x < 32) {
-    const float4* ps = a.part_s + (int64_t)blockIdx.x * 32 + rr;
-    const int64_t step = (int64_t)a.blocks * 32;
-    float M = -INFINITY, top = -INFINITY, sum = 0.f;
-    const int most = lim > 0 ? min(a.splits, (lim + a.chunk - 1) / a.chunk) : 0;   // ranges that this row sees
-    for (int k = 0; k < most; ++k) {
-      const float4 st = ps[k * step];
-      if (st.z != 0.f) M = fmaxf(M, st.x), top = fmaxf(top, st.y);
-    }
-    for (int k = 0; k < a.splits; ++k) {
-      float w = 0.f;
-      if (k < most) {
-        const float4 st = ps[k * step];
-        // (a range whose scores are all NaN has no maximum: its weight is its sum, or the NaN would be left out)
-        w = st.z != st.z ? st.z : st.z != 0.f ? exp2f((st.x - M) * LOG2E) : 0.f;
-        if (w != 0.f) sum += w * st.z;
-      }
-      s_w[k][rr] = w;
-    }
-    s_inv[rr] = lim > 0 ? 1.f / sum : 0.f;
-    if (a.sm_max && valid) {
-      const int64_t at = stat_at(a, seq, n, row);
-      a.sm_max[at] = lim > 0 ? top : 0.f;
-      a.sm_sum[at] = lim > 0 ? sum * exp2f((M - top) * LOG2E) : 0.f;
-    }
+  const int most = lim > 0 ? min(a.splits, (lim + a.chunk - 1) / a.chunk) : 0;   // ranges that this row sees
+  const int k8 = threadIdx.x >> 5;
+  float4 st[MAX_SPLITS / 8];
+#pragma unroll
+  for (int j = 0; j < MAX_SPLITS / 8; ++j) {
+    const int k = k8 + 8 * j;
+    st[j] = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+    if (k < most) st[j] = a.part_s[((int64_t)k * a.blocks + block) * 32 + rr];
   }
+  float M = -INFINITY, top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < MAX_SPLITS / 8; ++j)
+    if (st[j].z != 0.f) M = fmaxf(M, st[j].x), top = fmaxf(top, st[j].y);
+  s_top[k8][rr] = make_float2(M, top);
   __syncthreads();
-  const float inv = s_inv[rr];
-  for (int grp = wave; grp < D / 8; grp += 4) {
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float4* p = a.part + ((int64_t)blockIdx.x * (D / 8) + grp) * 64 + lane;
-    const int64_t step = (int64_t)a.blocks * (D / 8) * 64;
-#pragma unroll 4
-    for (int k = 0; k < a.splits; ++k) {
-      const float w = s_w[k][rr];
-      if (w != 0.f) {
-        const uint4 v = ldg16(p + k * step);
-        acc.x += w * __uint_as_float(v.x);
-        acc.y += w * __uint_as_float(v.y);
-        acc.z += w * __uint_as_float(v.z);
-        acc.w += w * __uint_as_float(v.w);
-      }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) M = fmaxf(M, s_top[j][rr].x), top = fmaxf(top, s_top[j][rr].y);
+#pragma unroll
+  for (int j = 0; j < MAX_SPLITS / 8; ++j) {
+    // (a range whose scores are all NaN has no maximum: its weight is its sum, or the NaN would be left out)
+    const float w = st[j].z != st[j].z ? st[j].z : st[j].z != 0.f ? exp2f((st[j].x - M) * LOG2E) : 0.f;
+    if (w != 0.f) sum += w * st[j].z;
+    s_w[k8 + 8 * j][rr] = w;
+  }
+  s_sum[k8][rr] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sum += s_sum[j][rr];
+  if (a.sm_max && col == 0 && threadIdx.x < 32 && valid) {
+    const int64_t at = stat_at(a, seq, n, row);
+    a.sm_max[at] = lim > 0 ? top : 0.f;
+    a.sm_sum[at] = lim > 0 ? sum * exp2f((M - top) * LOG2E) : 0.f;
+  }
+  float4 acc[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float4* p = a.part + ((int64_t)block * (D / 8) + col * 4) * 64 + lane;
+  const int64_t step = (int64_t)a.blocks * (D / 8) * 64;
+  for (int k0 = wave; k0 < a.splits; k0 += 16) {
+    float w[4];
+    uint4 v[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[j] = k0 + 4 * j < a.splits ? s_w[k0 + 4 * j][rr] : 0.f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[j][c] = make_uint4(0, 0, 0, 0);
+      if (w[j] != 0.f)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[j][c] = ldg16(p + (k0 + 4 * j) * step + c * 64);
     }
-    if (valid)
-      *reinterpret_cast<uint2*>(a.out + ((int64_t)(seq.r0 + s) * a.heads + n * a.per + g) * D + grp * 8 + kg * 4) =
-          lim > 0 ? make_uint2(pack2<IO>(acc.x * inv, acc.y * inv), pack2<IO>(acc.z * inv, acc.w * inv)) : make_uint2(0, 0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        acc[c].x += w[j] * __uint_as_float(v[j][c].x);
+        acc[c].y += w[j] * __uint_as_float(v[j][c].y);
+        acc[c].z += w[j] * __uint_as_float(v[j][c].z);
+        acc[c].w += w[j] * __uint_as_float(v[j][c].w);
+      }
+  }
+  if (wave)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) s_part[wave - 1][c][lane] = acc[c];
+  __syncthreads();
+  if (wave || !valid) return;
+  const float inv = lim > 0 ? 1.f / sum : 0.f;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+#pragma unroll
+    for (int w = 0; w < 3; ++w) {
+      const float4 v = s_part[w][c][lane];
+      acc[c].x += v.x, acc[c].y += v.y, acc[c].z += v.z, acc[c].w += v.w;
+    }
+    *reinterpret_cast<uint2*>(a.out + ((int64_t)(seq.r0 + s) * a.heads + n * a.per + g) * D + (col * 4 + c) * 8 + kg * 4) =
+        lim > 0 ? make_uint2(pack2<IO>(acc[c].x * inv, acc[c].y * inv), pack2<IO>(acc[c].z * inv, acc[c].w * inv)) : make_uint2(0, 0);
   }
 }
 
@@ -574,11 +608,11 @@ Cut make_cut(const DenseArgs& a) {
   const int64_t even = std::max<int64_t>(1, tiles(rows)) * seqs, through = (int64_t)a.total_rows * per / rows + seqs;
   const bool compact = even > 4 * through;
   const int64_t items = (compact ? through : even) * a.n2;
-  const int64_t real = ((int64_t)a.total_rows * per / rows + a.batch) * a.n2;   // about so many have rows
+  const int64_t real = std::min(even, (int64_t)a.total_rows * per / rows + a.batch) * a.n2;   // about so many have rows
   int splits = a.kv_splits;
   if (splits <= 0) {
     splits = 1;
-    if (real < 256) splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(real, 1), a.max_kv / 256));
+    if (real < 256) splits = (int)std::max<int64_t>(1, std::min<int64_t>(256 / std::max<int64_t>(real, 1), a.max_kv / 128));
   }
   splits = std::min(splits, MAX_SPLITS);
   c.chunk = (int)div_up(std::max<int64_t>(div_up(a.max_kv, splits), 1), BN) * BN;
@@ -601,7 +635,7 @@ hipError_t launch_d(const DenseK& k, const Cut& c, hipStream_t s) {
   // 256 rows: eight waves of 32, two a SIMD, or (192 wide scores: their queries leave no room for that) four of 64
   if (c.rt == 2) hipLaunchKernelGGL((dense_attn_kernel<IO, D, DR, DR ? 4 : 8, DR ? 2 : 1>), dim3((unsigned)c.groups), dim3(DR ? 256 : 512), 0, s, k);
   else hipLaunchKernelGGL((dense_attn_kernel<IO, D, DR, 4, 1>), dim3((unsigned)c.groups), dim3(256), 0, s, k);
-  if (c.splits > 1) hipLaunchKernelGGL((dense_merge_kernel<IO, D>), dim3((unsigned)c.blocks), dim3(256), 0, s, k);
+  if (c.splits > 1) hipLaunchKernelGGL((dense_merge_kernel<IO, D>), dim3((unsigned)c.blocks * (D / 32)), dim3(256), 0, s, k);
   return hipGetLastError();
 }
 template <int IO>
@@ -622,7 +656,7 @@ hipError_t launch_dense_attn(const DenseArgs& a, size_t* lacking, hipStream_t s)
   const size_t need = workspace_bytes(c, a.d);
   *lacking = need > 0 && (!a.ws || a.ws_bytes < need || ((uintptr_t)a.ws & 15) != 0) ? need : 0;
   if (*lacking) return hipSuccess;
-  if (c.groups >= (1 << 24)) return hipErrorInvalidConfiguration;   // 2^32 threads
+  if (c.groups >= (1 << 24) || (c.splits > 1 && (int64_t)c.blocks * (a.d / 32) >= (1 << 24))) return hipErrorInvalidConfiguration;   // 2^32 threads
   DenseK k{};
   auto rows = [](const DenseTensor& t) { return Rows{(const uint16_t*)t.p, t.row, t.head}; };
   k.q = rows(a.q), k.qr = rows(a.qr), k.k = rows(a.k), k.kr = rows(a.kr), k.v = rows(a.v);

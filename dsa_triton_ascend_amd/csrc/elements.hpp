@@ -9,16 +9,17 @@ namespace dsa {
 template <int IO> struct Elem { using T = uint16_t; static constexpr int V = 8; };
 template <> struct Elem<DSA_DTYPE_F32> { using T = float; static constexpr int V = 4; };
 
+// V elements as they lie in memory
+template <int IO, int V> struct Raw { using T = uint4; };
+template <int IO> struct Raw<IO, 1> { using T = typename Elem<IO>::T; };
 template <int IO, int V>
-__device__ __forceinline__ void load_vec(const typename Elem<IO>::T* p, float (&x)[V]) {
+__device__ __forceinline__ void widen(typename Raw<IO, V>::T u, float (&x)[V]) {
   if constexpr (V == 1) {
-    if constexpr (IO == DSA_DTYPE_F32) x[0] = p[0];
-    else x[0] = to_f32<IO>(p[0]);
+    if constexpr (IO == DSA_DTYPE_F32) x[0] = u;
+    else x[0] = to_f32<IO>(u);
   } else if constexpr (IO == DSA_DTYPE_F32) {
-    const uint4 u = ldg16(p);
     x[0] = __uint_as_float(u.x), x[1] = __uint_as_float(u.y), x[2] = __uint_as_float(u.z), x[3] = __uint_as_float(u.w);
   } else {
-    const uint4 u = ldg16(p);
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -26,6 +27,12 @@ __device__ __forceinline__ void load_vec(const typename Elem<IO>::T* p, float (&
       x[2 * i + 1] = to_f32<IO>((uint16_t)(w[i] >> 16));
     }
   }
+}
+
+template <int IO, int V>
+__device__ __forceinline__ void load_vec(const typename Elem<IO>::T* p, float (&x)[V]) {
+  if constexpr (V == 1) widen<IO, V>(p[0], x);
+  else widen<IO, V>(ldg16(p), x);
 }
 template <int IO, int V>
 __device__ __forceinline__ void store_vec(typename Elem<IO>::T* p, const float (&x)[V]) {

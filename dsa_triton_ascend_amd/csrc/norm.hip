@@ -26,10 +26,10 @@ struct NormK {
   const void* d;        // gradient: of y
   int64_t x_stride, d_stride;
   int64_t rows;
-  int width, tr;        // threads a row
+  int width, tr;        // threads a row: a power of two, or the whole work-group's waves
   const void* w;
   const void* b;
-  int wdt, w_vec;       // w_vec: w and b by 16 (8) byte loads
+  int wdt;
   float eps, inv_n;
   void* y;              // forward: y; gradient: dx (contiguous)
   float* mean;
@@ -38,38 +38,34 @@ struct NormK {
   int* groups;          // host: how many work-groups the gradient's launch has
 };
 
-// V parameters from column c on (c + V <= width)
-template <int V>
-__device__ __forceinline__ void params(const void* p, int dt, int vec, int c, float (&w)[V]) {
-  if (V > 1 && vec) {
-    if (dt == DSA_DTYPE_F32) {
-      const float* f = reinterpret_cast<const float*>(p) + c;
+// The same 16-byte accesses whatever the alignment: rows of an odd width begin anywhere
+template <int IO, int V>
+__device__ __forceinline__ typename Raw<IO, V>::T load_any(const typename Elem<IO>::T* p) {
+  typename Raw<IO, V>::T u;
+  __builtin_memcpy(&u, p, sizeof(u));
+  return u;
+}
+template <int IO, int V>
+__device__ __forceinline__ void store_any(typename Elem<IO>::T* p, const float (&x)[V]) {
+  typename Elem<IO>::T v[V];
 #pragma unroll
-      for (int i = 0; i + 4 <= V; i += 4) {
-        const uint4 u = ldg16(f + i);
-        w[i] = __uint_as_float(u.x), w[i + 1] = __uint_as_float(u.y), w[i + 2] = __uint_as_float(u.z),
-        w[i + 3] = __uint_as_float(u.w);
-      }
-    } else {
-      const uint16_t* h = reinterpret_cast<const uint16_t*>(p) + c;
-      uint2 u[V / 4 + 1];
-#pragma unroll
-      for (int i = 0; i + 4 <= V; i += 4) u[i / 4] = *reinterpret_cast<const uint2*>(h + i);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const uint16_t v = (uint16_t)((i & 2 ? u[i / 4].y : u[i / 4].x) >> (16 * (i & 1)));
-        w[i] = dt == DSA_DTYPE_BF16 ? bf16_to_f32(v) : f16_to_f32(v);
-      }
-    }
-    return;
+  for (int e = 0; e < V; ++e) {
+    if constexpr (IO == DSA_DTYPE_F32) v[e] = x[e];
+    else v[e] = from_f32<IO>(x[e]);
   }
+  __builtin_memcpy(p, v, sizeof(v));
+}
+
+// V parameters from column c on
+template <int V>
+__device__ __forceinline__ void params(const void* p, int dt, int c, float (&w)[V]) {
+  if (dt == DSA_DTYPE_F32) {
+    __builtin_memcpy(w, reinterpret_cast<const float*>(p) + c, sizeof(w));
+  } else {
+    uint16_t v[V];
+    __builtin_memcpy(v, reinterpret_cast<const uint16_t*>(p) + c, sizeof(v));
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if (dt == DSA_DTYPE_F32) w[i] = reinterpret_cast<const float*>(p)[c + i];
-    else {
-      const uint16_t v = reinterpret_cast<const uint16_t*>(p)[c + i];
-      w[i] = dt == DSA_DTYPE_BF16 ? bf16_to_f32(v) : f16_to_f32(v);
-    }
+    for (int e = 0; e < V; ++e) w[e] = dt == DSA_DTYPE_BF16 ? bf16_to_f32(v[e]) : f16_to_f32(v[e]);
   }
 }
 
@@ -101,7 +97,7 @@ __device__ __forceinline__ void row_sums(float (&v)[N], int tr, float (*red)[16]
   if (tr <= 64) return;
   float (*buf)[N] = red[turn & 1];
   ++turn;
-  const int wave = threadIdx.x >> 6, first = wave & ~((tr >> 6) - 1);
+  const int wave = threadIdx.x >> 6, first = tr < (int)blockDim.x ? wave & ~((tr >> 6) - 1) : 0;
   if ((threadIdx.x & 63) == 0)
 #pragma unroll
     for (int i = 0; i < N; ++i) buf[wave][i] = v[i];
@@ -113,81 +109,86 @@ __device__ __forceinline__ void row_sums(float (&v)[N], int tr, float (*red)[16]
     for (int i = 0; i < N; ++i) v[i] += buf[first + k][i];
 }
 
+// A row in units of V columns, UPT of them to a thread. The last unit ends with the row, so it may begin with columns of
+// the one before it: both make the same outputs of those, but only the other one adds them to sums.
+template <int V>
+struct Columns {
+  int t, tr, width;
+  __device__ __forceinline__ int of(int i) const { return (t + i * tr) * V; }
+  __device__ __forceinline__ int at(int i) const { return min(of(i), width - V); }   // where unit i lies
+  __device__ __forceinline__ int skip(int i) const { return max(0, of(i) - at(i)); }   // not added; V or more: no unit
+};
+
 // UPT units of V elements a thread; T threads a work-group at most
 template <int IO, int V, int UPT, int T>
 __global__ __launch_bounds__(T) void layer_norm_kernel(NormK a) {
   using E = typename Elem<IO>::T;
   __shared__ float red[2][16][1];
-  const int slots = (int)blockDim.x / a.tr, slot = (int)threadIdx.x / a.tr, t = (int)threadIdx.x & (a.tr - 1);
+  const int slots = (int)blockDim.x / a.tr, slot = (int)threadIdx.x / a.tr;
+  const Columns<V> col{(int)threadIdx.x - slot * a.tr, a.tr, a.width};
   int turn = 0;
-  auto col = [&](int i) { return (t + i * a.tr) * V; };
-  // the parameters stay in registers from row to row where they are few, else each row reads them (from a
-  // cache) when it needs them; the opaque zero keeps the compiler from holding them all the same
-  constexpr bool HOLD = UPT * V <= 16;
-  const void* const wp = a.w;
-  const void* const bp = a.b;
-  float w[HOLD ? UPT : 1][V], b[HOLD ? UPT : 1][V];
-  if constexpr (HOLD) {
+  float w[UPT][V], b[UPT][V];
 #pragma unroll
-    for (int i = 0; i < UPT; ++i) {
+  for (int i = 0; i < UPT; ++i) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) w[i][e] = 1.f, b[i][e] = 0.f;
-      if (wp && col(i) < a.width) params<V>(wp, a.wdt, a.w_vec, col(i), w[i]);
-      if (bp && col(i) < a.width) params<V>(bp, a.wdt, a.w_vec, col(i), b[i]);
-    }
+    for (int e = 0; e < V; ++e) w[i][e] = 1.f, b[i][e] = 0.f;
+    if (a.w) params<V>(a.w, a.wdt, col.at(i), w[i]);
+    if (a.b) params<V>(a.b, a.wdt, col.at(i), b[i]);
   }
+  typename Raw<IO, V>::T next[UPT];
+  auto fetch = [&](int64_t r) {
+    const E* x = reinterpret_cast<const E*>(a.x) + min(r, a.rows - 1) * a.x_stride;
+#pragma unroll
+    for (int i = 0; i < UPT; ++i) next[i] = load_any<IO, V>(x + col.at(i));
+  };
+  fetch((int64_t)blockIdx.x * slots + slot);
   for (int64_t base = (int64_t)blockIdx.x * slots; base < a.rows; base += (int64_t)gridDim.x * slots) {
     const int64_t r = base + slot;
-    const bool ok = r < a.rows;
-    const E* x = reinterpret_cast<const E*>(a.x) + (ok ? r : a.rows - 1) * a.x_stride;
     float v[UPT][V], s[1] = {0.f};
 #pragma unroll
+    for (int i = 0; i < UPT; ++i) widen<IO, V>(next[i], v[i]);
+    fetch(r + (int64_t)gridDim.x * slots);
+#pragma unroll
     for (int i = 0; i < UPT; ++i) {
-      if (col(i) < a.width) load_vec<IO, V>(x + col(i), v[i]);
-      else
+      const int skip = col.skip(i);
+      if (skip == 0) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[i][e] = 0.f;
+        for (int e = 0; e < V; ++e) s[0] += v[i][e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[0] += e >= skip ? v[i][e] : 0.f;
+      }
     }
-#pragma unroll
-    for (int i = 0; i < UPT; ++i)
-#pragma unroll
-      for (int e = 0; e < V; ++e) s[0] += v[i][e];
     row_sums<1>(s, a.tr, red, turn);
     const float mean = s[0] * a.inv_n;
     s[0] = 0.f;
 #pragma unroll
-    for (int i = 0; i < UPT; ++i)
-      if (col(i) < a.width)
+    for (int i = 0; i < UPT; ++i) {
+      const int skip = col.skip(i);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          v[i][e] -= mean;
-          s[0] = fmaf(v[i][e], v[i][e], s[0]);
-        }
+      for (int e = 0; e < V; ++e) v[i][e] -= mean;
+      if (skip == 0) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[0] = fmaf(v[i][e], v[i][e], s[0]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[0] += e >= skip ? v[i][e] * v[i][e] : 0.f;
+      }
+    }
     row_sums<1>(s, a.tr, red, turn);
     const float rstd = 1.f / sqrtf(s[0] * a.inv_n + a.eps);
-    if (!ok) continue;   // (the slots' trips through the barriers are the same: base is the work-group's)
-    if (t == 0 && a.mean) {
+    if (r >= a.rows) continue;   // (the slots' trips through the barriers are the same: base is the work-group's)
+    if (col.t == 0 && a.mean) {
       a.mean[r] = mean;
       a.rstd[r] = rstd;
     }
     E* y = reinterpret_cast<E*>(a.y) + r * a.width;
-    int again = 0;   // opaque
-    asm volatile("" : "+v"(again));
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
-      if (col(i) >= a.width) continue;
-      if constexpr (HOLD) {
+      if (col.of(i) >= a.width) continue;
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[i][e] = fmaf(v[i][e] * rstd, w[i][e], b[i][e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) w[0][e] = 1.f, b[0][e] = 0.f;
-        if (wp) params<V>(wp, a.wdt, a.w_vec, col(i) + again, w[0]);
-        if (bp) params<V>(bp, a.wdt, a.w_vec, col(i) + again, b[0]);
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[i][e] = fmaf(v[i][e] * rstd, w[0][e], b[0][e]);
-      }
-      store_vec<IO, V>(y + col(i), v[i]);
+      for (int e = 0; e < V; ++e) v[i][e] = fmaf(v[i][e] * rstd, w[i][e], b[i][e]);
+      store_any<IO, V>(y + col.at(i), v[i]);
     }
   }
 }
@@ -196,10 +197,10 @@ template <int IO, int V, int UPT, int T>
 __global__ __launch_bounds__(T) void layer_norm_grad_kernel(NormK a) {
   using E = typename Elem<IO>::T;
   __shared__ float red[2][16][2];
-  extern __shared__ float join[];   // [2][width] of one slot, where a work-group has several
-  const int slots = (int)blockDim.x / a.tr, slot = (int)threadIdx.x / a.tr, t = (int)threadIdx.x & (a.tr - 1);
+  extern __shared__ float join[];   // [slots][2][width], where a work-group has several
+  const int slots = (int)blockDim.x / a.tr, slot = (int)threadIdx.x / a.tr;
+  const Columns<V> col{(int)threadIdx.x - slot * a.tr, a.tr, a.width};
   int turn = 0;
-  auto col = [&](int i) { return (t + i * a.tr) * V; };
   float w[UPT][V], dw[UPT][V], db[UPT][V];
 #pragma unroll
   for (int i = 0; i < UPT; ++i) {
@@ -208,26 +209,41 @@ __global__ __launch_bounds__(T) void layer_norm_grad_kernel(NormK a) {
       w[i][e] = 1.f;
       dw[i][e] = db[i][e] = 0.f;
     }
-    if (a.w && col(i) < a.width) params<V>(a.w, a.wdt, a.w_vec, col(i), w[i]);
+    if (a.w) params<V>(a.w, a.wdt, col.at(i), w[i]);
   }
+  // the next row's elements are on their way while this one's sums are made (16383 rows of 4096 in bf16: 157 -> 83 us),
+  // but where 1024 threads leave no registers for them
+  constexpr bool AHEAD = T < 1024 || IO != DSA_DTYPE_F32;
+  typename Raw<IO, V>::T xn[UPT], dn[UPT];
+  float mean_n, rstd_n;
+  auto fetch = [&](int64_t r) {
+    const int64_t rr = min(r, a.rows - 1);
+    const E* x = reinterpret_cast<const E*>(a.x) + rr * a.x_stride;
+    const E* d = reinterpret_cast<const E*>(a.d) + rr * a.d_stride;
+#pragma unroll
+    for (int i = 0; i < UPT; ++i) {
+      xn[i] = load_any<IO, V>(x + col.at(i));
+      dn[i] = load_any<IO, V>(d + col.at(i));
+    }
+    mean_n = a.mean[rr], rstd_n = a.rstd[rr];
+  };
+  if constexpr (AHEAD) fetch((int64_t)blockIdx.x * slots + slot);
   for (int64_t base = (int64_t)blockIdx.x * slots; base < a.rows; base += (int64_t)gridDim.x * slots) {
     const int64_t r = base + slot;
     const bool ok = r < a.rows;
-    const int64_t rr = ok ? r : a.rows - 1;
-    const E* x = reinterpret_cast<const E*>(a.x) + rr * a.x_stride;
-    const E* d = reinterpret_cast<const E*>(a.d) + rr * a.d_stride;
     float h[UPT][V], g[UPT][V], s[2] = {0.f, 0.f};
+    if constexpr (!AHEAD) fetch(r);
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
-      if (ok && col(i) < a.width) {
-        load_vec<IO, V>(x + col(i), h[i]);
-        load_vec<IO, V>(d + col(i), g[i]);
-      }
+      widen<IO, V>(xn[i], h[i]);
+      widen<IO, V>(dn[i], g[i]);
     }
-    const float mean = a.mean[rr], rstd = a.rstd[rr];
+    const float mean = mean_n, rstd = rstd_n;
+    if constexpr (AHEAD) fetch(r + (int64_t)gridDim.x * slots);
 #pragma unroll
-    for (int i = 0; i < UPT; ++i)
-      if (ok && col(i) < a.width)
+    for (int i = 0; i < UPT; ++i) {
+      const int skip = ok ? col.skip(i) : V;
+      if (skip == 0) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           h[i][e] = (h[i][e] - mean) * rstd;
@@ -237,135 +253,127 @@ __global__ __launch_bounds__(T) void layer_norm_grad_kernel(NormK a) {
           s[0] += g[i][e];
           s[1] = fmaf(g[i][e], h[i][e], s[1]);
         }
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          h[i][e] = (h[i][e] - mean) * rstd;
+          dw[i][e] += e >= skip ? g[i][e] * h[i][e] : 0.f;
+          db[i][e] += e >= skip ? g[i][e] : 0.f;
+          g[i][e] *= w[i][e];
+          s[0] += e >= skip ? g[i][e] : 0.f;
+          s[1] += e >= skip ? g[i][e] * h[i][e] : 0.f;
+        }
+      }
+    }
     row_sums<2>(s, a.tr, red, turn);
     if (!ok) continue;
     const float c0 = s[0] * a.inv_n, c1 = s[1] * a.inv_n;
     E* dx = reinterpret_cast<E*>(a.y) + r * a.width;
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
-      if (col(i) >= a.width) continue;
+      if (col.of(i) >= a.width) continue;
 #pragma unroll
       for (int e = 0; e < V; ++e) g[i][e] = (g[i][e] - c0 - h[i][e] * c1) * rstd;
-      store_vec<IO, V>(dx + col(i), g[i]);
+      store_any<IO, V>(dx + col.at(i), g[i]);
     }
   }
   if (!a.part) return;
-  // the slots one after another, the last one leaves the work-group's sums
+  // the work-group's sums: a slot's straight from the registers, of several through LDS
   float* out = a.part + (int64_t)blockIdx.x * 2 * a.width;
-  for (int k = 0; k < slots; ++k) {
-    if (slot == k) {
+  float* to = slots > 1 ? join + slot * 2 * a.width : out;
 #pragma unroll
-      for (int i = 0; i < UPT; ++i) {
-        if (col(i) >= a.width) continue;
+  for (int i = 0; i < UPT; ++i) {
+    const int skip = col.skip(i), c = col.at(i);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const int c = col(i) + e;
-          float p = dw[i][e], q = db[i][e];
-          if (k > 0) {
-            p += join[c];
-            q += join[a.width + c];
-          }
-          if (k + 1 < slots) {
-            join[c] = p;
-            join[a.width + c] = q;
-          } else {
-            out[c] = p;
-            out[a.width + c] = q;
-          }
-        }
+    for (int e = 0; e < V; ++e)
+      if (e >= skip) {
+        to[c + e] = dw[i][e];
+        to[a.width + c + e] = db[i][e];
       }
-    }
-    if (slots > 1) __syncthreads();
+  }
+  if (slots == 1) return;
+  __syncthreads();
+  for (int c = threadIdx.x; c < 2 * a.width; c += blockDim.x) {
+    float p = join[c];
+    for (int k = 1; k < slots; ++k) p += join[k * 2 * a.width + c];
+    out[c] = p;
   }
 }
 
-// Column sums of the partial rows: 64 columns a work-group, 16 threads to a column. blockIdx.y: dw or db.
+// Column sums of the partial rows: 32 columns a work-group, 32 threads to a column. blockIdx.y: dw or db.
 template <int WDT>
 __global__ __launch_bounds__(1024) void layer_norm_join_kernel(const float* part, int groups, int width, void* dw, void* db) {
-  __shared__ float red[16][64];
+  __shared__ float red[32][33];
   using E = typename Elem<WDT>::T;
   E* out = reinterpret_cast<E*>(blockIdx.y ? db : dw);
   if (!out) return;
-  const int lane = threadIdx.x & 63, row = threadIdx.x >> 6, c = (int)blockIdx.x * 64 + lane;
+  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, c = (int)blockIdx.x * 32 + lane;
   float s = 0.f;
-  if (c < width)
-    for (int g = row; g < groups; g += 16) s += part[((int64_t)g * 2 + blockIdx.y) * width + c];
+  if (c < width) {
+    const float* p = part + (int64_t)blockIdx.y * width + c;
+#pragma unroll 8
+    for (int g = row; g < groups; g += 32) s += p[(int64_t)g * 2 * width];
+  }
   red[row][lane] = s;
   __syncthreads();
-  if (row == 0 && c < width) {
+  if (row) return;
 #pragma unroll
-    for (int k = 1; k < 16; ++k) s += red[k][lane];
+  for (int k = 1; k < 32; ++k) s += red[k][lane];
+  if (c < width) {
     const float v[1] = {s};
     store_vec<WDT, 1>(out + c, v);
   }
 }
 
-// Threads a row, and units of V elements a thread
-struct Shape {
-  int tr, upt, threads;
-};
 int pow2_above(int n) {
   int p = 1;
   while (p < n) p <<= 1;
   return p;
 }
-Shape shape_of(int units, int v) {
-  if (units <= 64) return {pow2_above(units), 1, 256};
-  if (v == 1) {
-    if (units <= 256) return {64, 4, 256};
-    if (units <= 1024) return {256, 4, 256};
-    return {1024, 16, 1024};
-  }
-  if (units <= 128) return {64, 2, 256};
-  if (units <= 256) return {64, 4, 256};
-  if (units <= 512) return {256, 2, 256};
-  if (units <= 1024) return {256, 4, 256};
-  return {pow2_above((units + 3) / 4), 4, 1024};   // (fp32 to 16384 columns, 16 bits to 16384 in 512 threads)
-}
 
 template <int IO, int V, int UPT, int T>
-hipError_t launch(const NormK& k, bool grad, int threads, hipStream_t s) {
-  const int slots = threads / k.tr;
+hipError_t launch(const NormK& k, bool grad, hipStream_t s) {
+  const int slots = k.tr > 128 ? 1 : 256 / k.tr, threads = slots * k.tr;
+  const int64_t trips = (k.rows + slots - 1) / slots;
   if (!grad) {
-    const int64_t groups = std::min<int64_t>((k.rows + slots - 1) / slots, 4096);
-    hipLaunchKernelGGL((layer_norm_kernel<IO, V, UPT, T>), dim3((unsigned)groups), dim3(threads), 0, s, k);
+    const unsigned groups = (unsigned)std::min<int64_t>(trips, 4096);
+    hipLaunchKernelGGL((layer_norm_kernel<IO, V, UPT, T>), dim3(groups), dim3(threads), 0, s, k);
   } else {
-    const size_t lds = slots > 1 && k.part ? (size_t)k.width * 2 * sizeof(float) : 0;
-    *k.groups = (int)std::min<int64_t>((k.rows + slots - 1) / slots, MAX_GROUPS);
+    // a work-group's row of partial sums costs as much as some rows of the input: at least four trips for it
+    *k.groups = (int)std::min<int64_t>(std::max<int64_t>((trips + 3) / 4, std::min<int64_t>(trips, 64)), MAX_GROUPS);
+    const size_t lds = slots > 1 && k.part ? (size_t)slots * k.width * 2 * sizeof(float) : 0;
     hipLaunchKernelGGL((layer_norm_grad_kernel<IO, V, UPT, T>), dim3(*k.groups), dim3(threads), lds, s, k);
   }
   return hipGetLastError();
 }
 
-template <int IO, int V>
-hipError_t launch_v(NormK k, bool grad, hipStream_t s) {
-  const Shape sh = shape_of((k.width + V - 1) / V, V);
-  k.tr = sh.tr;
-  switch (sh.upt) {
-    case 1: return launch<IO, V, 1, 256>(k, grad, sh.threads, s);
-    case 2: if constexpr (V > 1) return launch<IO, V, 2, 256>(k, grad, sh.threads, s); break;
-    case 4:
-      if (sh.threads == 256) return launch<IO, V, 4, 256>(k, grad, sh.threads, s);
-      // rows of more than 256 threads: one to a work-group
-      if constexpr (V == 8) return launch<IO, V, 4, 512>(k, grad, k.tr, s);
-      if constexpr (V == 4) return launch<IO, V, 4, 1024>(k, grad, k.tr, s);
-      break;
-    case 16: if constexpr (V == 1) return launch<IO, V, 16, 1024>(k, grad, sh.threads, s); break;
-  }
-  return hipErrorInvalidValue;
-}
-
 template <int IO>
 hipError_t launch_io(NormK k, bool grad, hipStream_t s) {
-  using T = typename Elem<IO>::T;
   constexpr int V = Elem<IO>::V;
-  auto on16 = [](const void* p, int64_t stride) { return ((uintptr_t)p & 15) == 0 && stride * (int64_t)sizeof(T) % 16 == 0; };
-  const bool vec = k.width % V == 0 && on16(k.x, k.x_stride) && on16(k.y, k.width) && (!grad || on16(k.d, k.d_stride));
-  return vec ? launch_v<IO, V>(k, grad, s) : launch_v<IO, 1>(k, grad, s);
+  if (k.width < V) {
+    k.tr = pow2_above(k.width);
+    return launch<IO, 1, 1, 256>(k, grad, s);
+  }
+  // One unit a thread up to a wave a row; then 16 columns a thread, from 256 threads on as many waves as that takes.
+  const int units = (k.width + V - 1) / V;
+  k.tr = pow2_above(units);
+  if (k.tr <= 64) return launch<IO, V, 1, 256>(k, grad, s);
+  constexpr int UPT = 16 / V;
+  const int threads = ((units + UPT - 1) / UPT + 63) / 64 * 64;
+  k.tr = threads <= 128 ? pow2_above(threads) : threads;
+  if (k.tr <= 256) return launch<IO, V, UPT, 256>(k, grad, s);
+  if (k.tr <= 512) return launch<IO, V, UPT, 512>(k, grad, s);
+  // (two work-groups of 512 threads on a CU pass the time of each other's barriers, one of 1024 has nobody to: 4096 rows of
+  // 16384 in bf16 take 83 against 88 us, their gradient 112 against 124. In 32 bits 512 threads would have twice the registers.)
+  if constexpr (V == 8) {
+    k.tr = ((units + 3) / 4 + 63) / 64 * 64;
+    return launch<IO, V, 4, 512>(k, grad, s);
+  } else {
+    return launch<IO, V, UPT, 1024>(k, grad, s);
+  }
 }
 
 hipError_t launch_any(NormK k, int io, bool grad, hipStream_t s) {
-  k.w_vec = (((uintptr_t)k.w | (uintptr_t)k.b) & 15) == 0;
   k.inv_n = 1.f / (float)k.width;
   switch (io) {
     case DSA_DTYPE_F16: return launch_io<DSA_DTYPE_F16>(k, grad, s);
@@ -403,7 +411,7 @@ hipError_t launch_layer_norm_grad(const NormArgs& a, hipStream_t s) {
     if (e != hipSuccess) return e;
   }
   if (!sums) return hipSuccess;
-  const dim3 grid((unsigned)((a.width + 63) / 64), 2);
+  const dim3 grid((unsigned)((a.width + 31) / 32), 2);
   if (a.wdt == DSA_DTYPE_F16)
     hipLaunchKernelGGL(layer_norm_join_kernel<DSA_DTYPE_F16>, grid, dim3(1024), 0, s, a.part, groups, a.width, a.dw, a.db);
   else if (a.wdt == DSA_DTYPE_BF16)
