@@ -88,6 +88,21 @@ def upload(lib, device: torch.device, *arrays: list[int], zero: torch.Tensor | N
     stream, and these arrays bound its addresses. A call that builds its plan and runs it at
     once, on one stream, needs no wait. Under stream capture there is none to wait for: the
     write is a node of the graph, and a plan built there runs in that graph."""
+    t, sizes = _upload(lib, device, arrays, zero, wait)
+    return t.split(sizes)
+
+
+def upload_pointers(lib, device: torch.device, *arrays: list[int], zero: torch.Tensor | None = None, wait: bool = True):
+    """:func:`upload`, giving the tensor that holds the arrays and their addresses in it (views cost a call more time)"""
+    t, sizes = _upload(lib, device, arrays, zero, wait)
+    at, out = t.data_ptr(), []
+    for n in sizes:
+        out.append(at)
+        at += 4 * n
+    return t, out
+
+
+def _upload(lib, device, arrays, zero, wait):
     flat, sizes = array("i"), []
     try:
         for a in arrays:
@@ -113,7 +128,7 @@ def upload(lib, device: torch.device, *arrays: list[int], zero: torch.Tensor | N
         t = torch.frombuffer(flat, dtype=torch.int32).to(device) if n else torch.empty(0, dtype=torch.int32, device=device)
     if wait and not torch.cuda.is_current_stream_capturing():
         torch.cuda.current_stream(device).synchronize()
-    return t.split(sizes)
+    return t, sizes
 
 
 def stream_ptr(device: torch.device) -> int:
@@ -127,6 +142,11 @@ def on_device(device: torch.device, call):
         return call()
     with torch.cuda.device(device):
         return call()
+
+
+def empty_as(t: torch.Tensor) -> torch.Tensor:
+    """A new contiguous tensor of t's shape, dtype and device (half of torch.empty's time on the host)"""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def aligned16(t: torch.Tensor) -> torch.Tensor:

@@ -14,6 +14,7 @@ from . import _host as H
 from . import _lib
 
 VALID_D = (64, 128)
+FEW_STATISTICS = 16384   # fp32 values
 D_ROPE = 64
 
 
@@ -112,12 +113,12 @@ class _Arguments:
         self.scale, self.sparse_mode = float(scale_value), sparse_mode
         self.operands = (query, query_rope, key, key_rope, value)
 
-    def place(self, lib, wait):
-        """Operands and lengths on the device, with the device current"""
+    def place(self, lib, wait, zero=None):
+        """Operands and lengths on the device (and zeros in a byte tensor), with the device current"""
         heads = (self.n1, self.n1, self.n2, self.n2, self.n2)
         self.q, self.qr, self.k, self.kr, self.v = (None if t is None else _packed(t, n) for t, n in zip(self.operands, heads))
-        self.d_row_start, self.d_key_start, self.d_act_q, self.d_act_k = H.upload(
-            lib, self.dev, self.row_start, self.key_start, self.act_q, self.act_k, wait=wait)
+        self.d_lengths, self.at = H.upload_pointers(lib, self.dev, self.row_start, self.key_start, self.act_q, self.act_k,
+                                                    zero=zero, wait=wait)
 
     def tensors(self, *more):
         """Pointers and strides as the C entries take them"""
@@ -128,8 +129,7 @@ class _Arguments:
         return out
 
     def lengths(self):
-        return [self.d_row_start.data_ptr(), self.d_key_start.data_ptr(), self.d_act_q.data_ptr(), self.d_act_k.data_ptr(),
-                self.batch]
+        return *self.at, self.batch
 
 
 class DenseAttentionPlan:
@@ -154,15 +154,27 @@ class DenseAttentionPlan:
         def place():
             nothing = not (a.batch and a.total_rows)
             empty = nothing or not a.total_keys
-            self.out = (torch.zeros if empty else torch.empty)(query.shape, dtype=query.dtype, device=self.dev)
-            stats = torch.empty if return_softmax_lse and not empty else torch.zeros
-            self.sm_max, self.sm_sum = stats((2,) + a.stat_shape, dtype=torch.float32, device=self.dev).unbind(0)
+            self.out = H.empty_as(query)
+            if empty:
+                self.out.zero_()
+            # statistics that nobody asked for are zeros: a small tensor's come with the lengths' launch
+            stats = (2,) + a.stat_shape
+            total = 2 * a.n1 * a.total_rows
+            few = not return_softmax_lse and not empty and total <= FEW_STATISTICS
+            zero = None
+            if few:
+                zero = torch.empty((total + 3) // 4 * 16, dtype=torch.uint8, device=self.dev)
+                both = zero.view(torch.float32)[:total].view(stats)
+            else:
+                both = (torch.empty if return_softmax_lse and not empty else torch.zeros)(stats, dtype=torch.float32,
+                                                                                          device=self.dev)
+            self.sm_max, self.sm_sum = both.unbind(0)
             if empty:   # no key: zeros, as for rows that see none
                 return
             size = self.lib.dsa_dense_attn_workspace_bytes(a.batch, a.total_rows, a.rows_behind, a.n1, a.n2, a.d, a.max_rows,
                                                            a.max_kv, int(kv_splits))
             self.ws = torch.empty(size, dtype=torch.uint8, device=self.dev) if size else None
-            a.place(self.lib, _wait)
+            a.place(self.lib, _wait, zero)
             self.q, self.qr, self.k, self.kr, self.v = a.q, a.qr, a.k, a.kr, a.v
             lse = return_softmax_lse
             self.args = (*a.tensors(), a.io, *a.lengths(), a.total_rows, a.total_keys, a.rows_behind, a.n1, a.n2, a.d, a.dr,
@@ -219,10 +231,11 @@ class DenseAttentionGradPlan:
 
         def place():
             empty = not (a.batch and a.total_rows and a.total_keys)
-            new = torch.zeros if empty else torch.empty
-            self.grads = tuple(None if t is None else new(t.shape, dtype=t.dtype, device=self.dev)
-                               for t in (query, key, value, query_rope, key_rope))
+            self.grads = tuple(None if t is None else H.empty_as(t) for t in (query, key, value, query_rope, key_rope))
             if empty:
+                for t in self.grads:
+                    if t is not None:
+                        t.zero_()
                 return
             size = self.lib.dsa_dense_attn_grad_workspace_bytes(a.batch, a.total_rows, a.total_keys, a.rows_behind,
                                                                 a.keys_behind, a.n1, a.n2, a.d, a.dr, a.max_rows, a.max_keys,

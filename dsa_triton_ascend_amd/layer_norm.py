@@ -61,7 +61,7 @@ def layer_norm(x, norm_weight=None, norm_bias=None, norm_eps=1e-6, return_stats=
 
     def call():
         w, b = (None if t is None else t.contiguous() for t in (norm_weight, norm_bias))
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        y = H.empty_as(x)
         mean = rstd = None
         if return_stats:
             mean, rstd = torch.empty((2,) + lead, dtype=torch.float32, device=dev).unbind(0)
@@ -95,12 +95,12 @@ def layer_norm_grad(d_out, x, mean, rstd, norm_weight=None, norm_bias=None):
     def call():
         w = None if norm_weight is None else norm_weight.contiguous()
         m, r = mean.contiguous(), rstd.contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        dx = H.empty_as(x)
         dw = db = ws = None
         size = 0
         if w is not None:
-            dw = torch.empty(width, dtype=w.dtype, device=dev)
-            db = None if norm_bias is None else torch.empty(width, dtype=w.dtype, device=dev)
+            dw = H.empty_as(w)
+            db = None if norm_bias is None else H.empty_as(w)
             size = lib.dsa_layer_norm_grad_workspace_bytes(n, width)
             ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         if not n:   # sums of nothing
