@@ -100,6 +100,9 @@ def written_just_before(ins, k, uses):
                 out = operands[0] + ("," + operands[1] if "swap" in op else "")
                 if _regs(out) & uses:
                     return ins[j]
+            m = _MFMA.match(text)
+            if m:
+                uses = uses - _regs(m.group(1))
             wait += 1
         j -= 1
     return None
