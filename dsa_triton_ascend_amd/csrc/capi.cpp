@@ -790,7 +790,10 @@ size_t dsa_dense_attn_workspace_bytes(int batch, int total_rows, int rows_behind
   DenseArgs a{};
   a.batch = batch, a.total_rows = total_rows, a.rows_behind = rows_behind, a.n1 = n1, a.n2 = n2, a.d = d;
   a.max_rows = max_rows, a.max_kv = max_kv, a.kv_splits = kv_splits;
-  return dense_attn_workspace_bytes(a);
+  a.sparse_mode = 0;   // either mask's
+  const size_t full = dense_attn_workspace_bytes(a);
+  a.sparse_mode = 3;
+  return std::max(full, dense_attn_workspace_bytes(a));
 }
 
 int dsa_dense_attn(const void* query, int64_t q_row, int64_t q_head, const void* query_rope, int64_t qr_row, int64_t qr_head,

@@ -4,11 +4,18 @@
 //   score = (q . k_t + q_rope . k_rope_t) * scale,   out = softmax(score) . v
 // limit(s) = act_k - act_q + s + 1 (causal, the last query is the last token) or act_k.
 //
-// A work-group of four waves has 128 RT head rows of one key head: the heads of a group lie side by side as rows,
-// so keys and values are read once for all of them, and a single token's group still fills the MFMA's columns. Each wave
-// owns 32 RT rows. Tiles of 64 tokens go direct to LDS. S^T = K Q^T has the tokens as M; the online softmax
+// A work-group has 256 or 128 head rows of one key head: the heads of a group lie side by side as rows, so keys and
+// values are read once for all of them, and a single token's group still fills the MFMA's columns. Each wave owns 32 RT
+// rows. Tiles of 64 tokens go direct to LDS, into a ring of three. S^T = K Q^T has the tokens as M; the online softmax
 // runs in each lane's scores of its own head row plus one exchange between lane halves, and its result is already
 // the B operand of O^T += V^T P^T. P is rounded to the io type for that product; scores, sums and O have 32 bits.
+//
+// Bound by the matrix instructions, and by the issue of all others beside them: the softmax of one half tile (32 tokens)
+// is placed, a few operations at a time, among the products O += V P of the half before it and S of the one after (8192
+// tokens, 32 heads on 8 of 128, bf16: 898 -> 621 us). Eight waves of 32 rows, two a SIMD, pass the time of each other's
+// waits where the registers allow it (621 -> 553; heads of 64: 490 -> 372); with 192 wide scores Q alone would take the
+// registers, and four waves of 64 rows read each fragment half as often. Loads whose addresses need no branch: 533 -> 513,
+// 1070 TFLOP/s of those that the mask leaves.
 #include <algorithm>
 
 #include "dense_attn.hpp"
@@ -593,7 +600,7 @@ __global__ __launch_bounds__(256) void dense_merge_kernel(DenseK a) {
 
 // ---------------------------------------------------------------- how a call is cut
 struct Cut {
-  int rt, even, through, splits, chunk, blocks;
+  int rt, even, splits, chunk, blocks;
   int64_t groups;
 };
 int64_t div_up(int64_t x, int64_t y) { return (x + y - 1) / y; }
@@ -601,24 +608,33 @@ int64_t div_up(int64_t x, int64_t y) { return (x + y - 1) / y; }
 Cut make_cut(const DenseArgs& a) {
   const int64_t seqs = a.batch + (a.rows_behind > 0), per = a.n1 / a.n2;
   Cut c{};
-  // 256 rows a work-group where that leaves two rounds of the CUs, else 128
   auto tiles = [&](int rows) { return div_up((int64_t)a.max_rows * per, rows); };
-  c.rt = (int64_t)a.total_rows * per * a.n2 / 256 >= 160 ? 2 : 1;
+  // Work-groups of 256 rows read each tile half as often as those of 128, which balance better. With all items about as
+  // long (no mask, or a chunk after many tokens; bf16, us of 256 and of 128 rows): 188 items 200 and 262, 256 items of
+  // heads of 64 83 and 88. Below a diagonal, where the longest has twice the mean: 256 items 199 and 167, 320 items 75
+  // and 83, 1024 items 504 and 631 (rotary 637 and 753); heads of 64, several of whose work-groups a CU holds, 344 and 335.
+  const bool flat = a.sparse_mode == 0 || a.max_kv >= 2 * (int64_t)a.max_rows;
+  const int64_t items256 = (int64_t)a.total_rows * per * a.n2 / 256;
+  c.rt = flat ? (items256 >= 160 ? 2 : 1) : (a.d == 128 && items256 > 256 ? 2 : 1);
   const int rows = 128 * c.rt;
   const int64_t even = std::max<int64_t>(1, tiles(rows)) * seqs, through = (int64_t)a.total_rows * per / rows + seqs;
+  // All sequences get the longest's tiles, by levels, the last, which see most, first. Numbered through, that order is
+  // lost: 43 sequences, the longest 512, 3.3 times as many even items: 32 and 38 us; 9, the longest 4096, 5.5 times: 161 and 152.
   const bool compact = even > 4 * through;
   const int64_t items = (compact ? through : even) * a.n2;
   const int64_t real = std::min(even, (int64_t)a.total_rows * per / rows + a.batch) * a.n2;   // about so many have rows
+  // Fewer items than CUs: ranges of tokens that make one round of them, of two tiles at least (a work-group's LDS fills its
+  // CU; four single tokens, 4 key heads, 8190 keys: 8, 16, 32 ranges take 29.9, 22.9, 27.8 us with their join), from
+  // 512 tokens on (600 keys: 16.2 us in one range, 11.8 in four; 333: 10.0 in one, 13.0 in two).
   int splits = a.kv_splits;
   if (splits <= 0) {
     splits = 1;
-    if (real < 256) splits = (int)std::max<int64_t>(1, std::min<int64_t>(256 / std::max<int64_t>(real, 1), a.max_kv / 128));
+    if (real < 256 && a.max_kv >= 512) splits = (int)std::max<int64_t>(1, std::min<int64_t>(256 / std::max<int64_t>(real, 1), a.max_kv / 128));
   }
   splits = std::min(splits, MAX_SPLITS);
   c.chunk = (int)div_up(std::max<int64_t>(div_up(a.max_kv, splits), 1), BN) * BN;
   c.splits = (int)std::max<int64_t>(1, div_up(a.max_kv, c.chunk));
   c.even = compact ? 0 : (int)std::max<int64_t>(1, tiles(rows));
-  c.through = (int)through;
   c.groups = items * c.splits;
   c.blocks = (int)(((int64_t)a.total_rows * per / 32 + seqs + 1) * a.n2);
   return c;
@@ -661,7 +677,7 @@ hipError_t launch_dense_attn(const DenseArgs& a, size_t* lacking, hipStream_t s)
   auto rows = [](const DenseTensor& t) { return Rows{(const uint16_t*)t.p, t.row, t.head}; };
   k.q = rows(a.q), k.qr = rows(a.qr), k.k = rows(a.k), k.kr = rows(a.kr), k.v = rows(a.v);
   k.len = {a.row_start, a.key_start, a.act_q, a.act_k, a.batch, a.total_rows, a.total_keys, a.sparse_mode};
-  k.tiles = {a.batch + (a.rows_behind > 0), a.n2, c.even, c.through};
+  k.tiles = {a.batch + (a.rows_behind > 0), a.n2, c.even};
   k.per = a.n1 / a.n2;
   k.heads = a.n1;
   k.stat_padded = a.stat_padded;

@@ -122,20 +122,6 @@ template <int RB, int BN, int NW> struct Stream {
 __device__ __forceinline__ int s_row(int m) { return 16 * (m >> 4) + 8 * ((m >> 2) & 1) + 4 * ((m >> 3) & 1) + (m & 3); }
 __device__ __forceinline__ int s_token(int i, int kg) { return 16 * (i >> 3) + 8 * kg + (i & 7); }
 
-// Operand fragment: row t, values 16 ks + 8 kg .. of a tile
-template <int RB>
-__device__ __forceinline__ uint4 op_frag(uint32_t tile, int t, int ks, int kg) {
-  return lds_read16_at(tile + tile_off<RB>(t, 2 * ks + kg));
-}
-// Transposed operand fragment: column 32 n + lane % 32 of the rows t0 + 8 (lane / 32) .. + 7 (t0 a multiple of 16)
-template <int RB>
-__device__ __forceinline__ uint4 tr_frag(uint32_t tile, int t0, int n, int lane) {
-  const int g16 = lane >> 4, c16 = lane & 15;
-  const int t4 = t0 + (g16 >> 1) * 8 + (c16 >> 2), c = 4 * n + (g16 & 1) * 2 + ((c16 & 3) >> 1), o = (c16 & 1) * 8;
-  const uint2 lo = ds_read_tr_at(tile + tile_off<RB>(t4, c) + o), hi = ds_read_tr_at(tile + tile_off<RB>(t4 + 4, c) + o);
-  return make_uint4(lo.x, lo.y, hi.x, hi.y);
-}
-
 // Values that are not finite become zeros in this wave's share of a tile (its loads have landed); returns the rows
 // (bit) that held one.
 template <int IO, int RB, int BN, int NW>
@@ -289,7 +275,6 @@ __device__ __forceinline__ void pack_tile(const f32x16& v, float f, uint4 (&out)
 struct Tiles {
   int seqs, heads;       // sequences (with what lies behind the last), key heads
   int even;              // tiles of the longest, 0: numbered through
-  int through;           // tiles of all sequences, numbered through
 };
 
 }  // namespace dsa

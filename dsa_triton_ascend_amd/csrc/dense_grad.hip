@@ -7,13 +7,22 @@
 //
 // Three launches, without atomics, so results do not depend on timing:
 //  * rows: delta and the logarithm of the sum for every head row (fp16: also the norms that bound dS);
+//  * queries: 128 head rows, 32 a wave, Q and dO in registers, running over the tokens: S^T = K Q^T, dP^T = V dO^T,
+//    dQ^T += K^T dS^T; on its way it makes delta anew, without the rounding of O;
 //  * keys: a work-group has 128 tokens of one key head, 32 a wave, K and V in registers, and runs over the head rows
 //    that see them (the group's heads are rows side by side): S = Q K^T and dP = dO V^T with the head rows as M, whose
-//    results are already the B operands of dV^T += dO^T P and dK^T += Q^T dS;
-//  * queries: 128 head rows, 32 a wave, Q and dO in registers, running over the tokens: S^T = K Q^T, dP^T = V dO^T,
-//    dQ^T += K^T dS^T.
+//    results are already the B operands of dV^T += dO^T P and dK^T += Q^T dS.
+// Few tokens or rows are cut into ranges over the other axis, whose sums a further launch adds.
+//
 // S and dP are computed in both, 7 products instead of 5; what that saves is the addition of dQ from many work-groups,
 // in 32 bits and an order of its own. P and dS are rounded to the io type for their products.
+//
+// Bound by the issue of instructions beside the matrix ones: a wave holds two operands and up to 10 accumulators, so there is
+// one to a SIMD, and P and dS of one half tile are placed among the products of the half before it and the scores of
+// the one after (8192 tokens, 32 heads on 8 of 128, bf16: 3079 -> 2189 us). Loads whose addresses need no branch: 1954;
+// all work-groups of a key head at the same head rows at the same time, and dP that starts from -delta: 1836 (prep
+// 43, queries 856, keys 940; 1048 TFLOP/s of the 7 products). Two waves to 32 tokens, one for dV and one for dK, each
+// with the scores of both, were no faster (1954).
 #include <algorithm>
 
 #include "dense_attn.hpp"
@@ -1033,15 +1042,20 @@ struct Part {   // one of the two main launches
   int even, splits, chunk, blocks, seqs;
   int64_t groups;
 };
+// Tiles of TOK rows (or tokens) of every sequence: by levels of the longest's number (the heaviest of all first), or
+// numbered through where that is more than half as many again (1.9 times: 980 and 959 us, 3.3: 166 and 155, 22: 1991
+// and 1814). Ranges of the other axis where there are fewer tiles than CUs: each loads its operands anew, and a launch
+// adds their sums; of 512 rows, two rounds' worth, or up to four of 128 (a sample of 2048, 8 heads on 4: one range
+// 153 us, 4 100, 8 133; one of 300: 56, 50, 47).
 Part make_part(int64_t total, int64_t longest, int batch, bool behind, int heads, int64_t other, int forced) {
   Part p{};
   const int64_t seqs = batch + (behind ? 1 : 0);
   const int64_t tiles = std::max<int64_t>(1, div_up(longest, TOK));
   const int64_t even = tiles * seqs, through = total / TOK + seqs;
-  const bool compact = even > 4 * through;
+  const bool compact = 2 * even > 3 * through;
   const int64_t real = (total / TOK + batch) * heads;
   int64_t splits = forced;
-  if (splits <= 0) splits = real >= 256 ? 1 : std::max<int64_t>(1, std::min<int64_t>(512 / real, other / 512));
+  if (splits <= 0) splits = real >= 256 ? 1 : std::max<int64_t>(1, std::min(512 / real, std::max(other / 512, std::min<int64_t>(4, other / 128))));
   splits = std::min<int64_t>(splits, 64);
   p.chunk = (int)(div_up(std::max<int64_t>(div_up(other, splits), 1), BN) * BN);
   p.splits = (int)std::max<int64_t>(1, div_up(other, p.chunk));
