@@ -114,6 +114,11 @@ CASES = [  # n1, n2, d, dr, tokens, kv, mode, packed, behind
     (16, 16, 64, 0, [2300, 2100], [2500, 2100], 3, False, 0),
     (16, 16, 128, 64, [4200], [4200], 3, True, 0),
     (12, 4, 128, 0, [3000], [3001], 0, True, 0),
+    (16, 16, 64, 0, [2300, 2100], [4700, 2100], 3, False, 0),                    # the same after as many earlier tokens
+    (32, 8, 64, 0, [1400], [1401], 0, True, 0),
+    (32, 8, 128, 0, [1400], [2900], 3, True, 3),
+    (12, 2, 128, 64, [2], [511], 3, True, 0),                                    # one range, then several
+    (12, 2, 128, 64, [2], [512], 3, True, 0),
 ]
 
 
@@ -214,6 +219,20 @@ def test_values_that_are_not_finite(what, value, mode):
     if value != value or what == "value":
         assert not torch.isfinite(got[0][1, first:200, 2:]).all(-1).any()
     assert not got[0][0, 50:].any() and not got[0][1, 200:].any()
+
+
+@pytest.mark.parametrize("d,dr,mode", [(64, 0, 0), (128, 0, 0), (128, 0, 3), (128, 64, 0), (128, 64, 3)])
+def test_values_that_are_not_finite_in_wide_work_groups(d, dr, mode):
+    tokens = [1400, 900]
+    t = make(BF, 32, 8, d, dr, tokens, tokens, False, 41)
+    want = call(t, tokens, tokens, False, 0.1, mode)
+    t["value"][1, 333, 1] = math.inf
+    t["key"][1, 900:], t["value"][1, 900:], t["query"][1, 900:] = math.nan, math.nan, math.inf
+    got = call(t, tokens, tokens, False, 0.1, mode)
+    first = 333 if mode == 3 else 0
+    assert torch.equal(got[0][0], want[0][0]) and torch.equal(got[0][1, :first], want[0][1, :first])
+    assert torch.equal(got[0][1, :, :4], want[0][1, :, :4]) and torch.equal(got[0][1, :, 8:], want[0][1, :, 8:])
+    assert not torch.isfinite(got[0][1, first:900, 4:8]).all(-1).any() and not got[0][1, 900:].any()
 
 
 def test_no_rows_no_keys():
