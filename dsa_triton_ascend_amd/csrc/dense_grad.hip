@@ -34,7 +34,7 @@ constexpr int NWV = 4;
 constexpr int BN = 64;     // rows of a tile in LDS
 constexpr int NBUF = 3;
 constexpr int TOK = NWV * 32;     // tokens, or head rows, of a work-group
-constexpr int PREP = 512;         // work-groups of the first launch
+constexpr int PREP = 1024;        // work-groups of the first launch
 
 // fp16 keeps 11 bits down to 2^-14 and none below 2^-25. P <= 1 is multiplied by 2^15 for its product. dS is bounded by
 // 2 max|dO| max|v| (row norms), and multiplied by the power of two that takes this bound to 2^15.

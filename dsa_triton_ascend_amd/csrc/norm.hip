@@ -6,8 +6,12 @@
 //
 // Bound by memory: a row is read once into registers, and all its sums are made there (the variance from
 // the centered values, so a large mean costs no bits). Statistics and sums are 32-bit, each output is
-// rounded once. A row has TR threads, a power of two: up to a wave's 64 they sum by VALU lane exchanges,
-// a work-group then taking several rows at a time; wider rows add through LDS.
+// rounded once. A row has TR threads: up to a wave's 64 (a power of two) they sum by VALU lane exchanges, a work-group
+// then taking several rows at a time; wider rows add through LDS. The next row is loaded before this one's sums, which
+// wait for each other. 16383 rows of 4096 in bf16: forward 52 us (5.2 TB/s), gradient 84 (4.8); in fp32 5.8 and 5.0 TB/s.
+//
+// Rows of an odd width, or strided ones, begin anywhere: the accesses are of 16 bytes all the same, which the hardware
+// takes at any alignment (8192 rows of 2049 in bf16: 126 -> 20 us against single elements, the gradient 139 -> 32).
 //
 // The sums over rows: each work-group adds up its rows' d h and d in registers (a thread's columns are the
 // same in every row), joins its row slots in LDS and leaves one row of partial sums; a second launch adds those, in
