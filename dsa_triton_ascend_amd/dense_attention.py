@@ -114,7 +114,7 @@ class _Arguments:
         self.operands = (query, query_rope, key, key_rope, value)
 
     def place(self, lib, wait, zero=None):
-        """Operands and lengths on the device (and zeros in a byte tensor), with the device current"""
+        """Operands and lengths on the device (and zeros in a tensor), with the device current"""
         heads = (self.n1, self.n1, self.n2, self.n2, self.n2)
         self.q, self.qr, self.k, self.kr, self.v = (None if t is None else _packed(t, n) for t, n in zip(self.operands, heads))
         self.d_lengths, self.at = H.upload_pointers(lib, self.dev, self.row_start, self.key_start, self.act_q, self.act_k,
@@ -157,24 +157,18 @@ class DenseAttentionPlan:
             self.out = H.empty_as(query)
             if empty:
                 self.out.zero_()
-            # statistics that nobody asked for are zeros: a small tensor's come with the lengths' launch
-            stats = (2,) + a.stat_shape
+            # statistics that nobody asked for are zeros: a small tensor is cleared by the lengths' launch
             total = 2 * a.n1 * a.total_rows
-            few = not return_softmax_lse and not empty and total <= FEW_STATISTICS
-            zero = None
-            if few:
-                zero = torch.empty((total + 3) // 4 * 16, dtype=torch.uint8, device=self.dev)
-                both = zero.view(torch.float32)[:total].view(stats)
-            else:
-                both = (torch.empty if return_softmax_lse and not empty else torch.zeros)(stats, dtype=torch.float32,
-                                                                                          device=self.dev)
+            few = not return_softmax_lse and not empty and total <= FEW_STATISTICS and total % 4 == 0
+            both = (torch.empty if (return_softmax_lse and not empty) or few else torch.zeros)(
+                (2,) + a.stat_shape, dtype=torch.float32, device=self.dev)
             self.sm_max, self.sm_sum = both.unbind(0)
             if empty:   # no key: zeros, as for rows that see none
                 return
             size = self.lib.dsa_dense_attn_workspace_bytes(a.batch, a.total_rows, a.rows_behind, a.n1, a.n2, a.d, a.max_rows,
                                                            a.max_kv, int(kv_splits))
             self.ws = torch.empty(size, dtype=torch.uint8, device=self.dev) if size else None
-            a.place(self.lib, _wait, zero)
+            a.place(self.lib, _wait, both if few else None)
             self.q, self.qr, self.k, self.kr, self.v = a.q, a.qr, a.k, a.kr, a.v
             lse = return_softmax_lse
             self.args = (*a.tensors(), a.io, *a.lengths(), a.total_rows, a.total_keys, a.rows_behind, a.n1, a.n2, a.d, a.dr,
