@@ -85,7 +85,7 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
     sp = 0;
     if (a.tiles.even) {
       const int level = i / pairs;
-      i -= level * pairs;
+      i = pair_of(i, level, pairs, a.splits);
       b = i / a.tiles.heads;
       n = i - b * a.tiles.heads;
       sp = level % a.splits;

@@ -183,7 +183,7 @@ __device__ __forceinline__ Place place_of(int i, int seqs, int heads, int splits
   Place p;
   if (even) {
     const int pairs = seqs * heads, level = i / pairs;
-    i -= level * pairs;
+    i = pair_of(i, level, pairs, splits);
     p.b = i / heads;
     p.n = i - p.b * heads;
     p.sp = level % splits;
