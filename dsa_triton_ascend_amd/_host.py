@@ -82,19 +82,20 @@ UPLOAD_MAX = 8192   # values a dsa_upload_i32 call takes
 def upload(lib, device: torch.device, *arrays: list[int], zero: torch.Tensor | None = None, wait: bool = True):
     """The int32 length and offset arrays of a call on the device, views of one tensor (each padded
     to 16 bytes), written on the current stream by dsa_upload_i32 (one launch up to 56 values, then
-    one per 960); `zero` (a tensor of a multiple of 16 bytes) is cleared by the first. For a device that is not the
+    one per 960); `zero` (a byte tensor) is cleared by the first. For a device that is not the
     current one they go by a copy. With `wait` the host waits until the arrays and
     all that the caller put on this stream before are in place: a kept plan may run on any
     stream, and these arrays bound its addresses. A call that builds its plan and runs it at
     once, on one stream, needs no wait. Under stream capture there is none to wait for: the
     write is a node of the graph, and a plan built there runs in that graph."""
-    t, sizes = _upload(lib, device, arrays, zero, wait)
+    t, sizes = _upload(lib, device, arrays, zero, 0 if zero is None else zero.numel(), wait)
     return t.split(sizes)
 
 
 def upload_pointers(lib, device: torch.device, *arrays: list[int], zero: torch.Tensor | None = None, wait: bool = True):
-    """:func:`upload`, giving the tensor that holds the arrays and their addresses in it (views cost a call more time)"""
-    t, sizes = _upload(lib, device, arrays, zero, wait)
+    """:func:`upload`, giving the tensor that holds the arrays and their addresses in it (views cost a call more time); `zero` may
+    be of any type, a multiple of 16 bytes"""
+    t, sizes = _upload(lib, device, arrays, zero, 0 if zero is None else zero.numel() * zero.element_size(), wait)
     at, out = t.data_ptr(), []
     for n in sizes:
         out.append(at)
@@ -102,7 +103,7 @@ def upload_pointers(lib, device: torch.device, *arrays: list[int], zero: torch.T
     return t, out
 
 
-def _upload(lib, device, arrays, zero, wait):
+def _upload(lib, device, arrays, zero, zero_bytes, wait):
     flat, sizes = array("i"), []
     try:
         for a in arrays:
@@ -117,7 +118,7 @@ def _upload(lib, device, arrays, zero, wait):
     if device.index in (None, torch.cuda.current_device()):
         t = torch.empty(n, dtype=torch.int32, device=device)
         src, dst, stream = flat.buffer_info()[0], t.data_ptr(), stream_ptr(device)
-        zero_ptr, zero_bytes = ptr(zero), 0 if zero is None else zero.numel() * zero.element_size()
+        zero_ptr = ptr(zero)
         for i in range(0, max(n, 1), UPLOAD_MAX):
             _lib.check(lib.dsa_upload_i32(src + 4 * i, min(n - i, UPLOAD_MAX), dst + 4 * i, zero_ptr, zero_bytes,
                                           stream), "dsa_upload_i32")
