@@ -20,8 +20,9 @@
 // Bound by the issue of instructions beside the matrix ones: a wave holds two operands and up to 10 accumulators, so there is
 // one to a SIMD, and P and dS of one half tile are placed among the products of the half before it and the scores of
 // the one after (8192 tokens, 32 heads on 8 of 128, bf16: 3079 -> 2189 us). Loads whose addresses need no branch: 1954;
-// all work-groups of a key head at the same head rows at the same time, and dP that starts from -delta: 1836 (prep
-// 43, queries 856, keys 940; 1048 TFLOP/s of the 7 products). Two waves to 32 tokens, one for dV and one for dK, each
+// all work-groups of a key head at the same head rows at the same time, and dP that starts from -delta: 1836;
+// levels turned (pair_of) and twice the work-groups for the rows: 1770 (rows 29, queries 780, keys 960; 1080 TFLOP/s of
+// the 7 products). Two waves to 32 tokens, one for dV and one for dK, each
 // with the scores of both, were no faster (1954).
 #include <algorithm>
 
