@@ -8,7 +8,8 @@
 // the centered values, so a large mean costs no bits). Statistics and sums are 32-bit, each output is
 // rounded once. A row has TR threads: up to a wave's 64 (a power of two) they sum by VALU lane exchanges, a work-group
 // then taking several rows at a time; wider rows add through LDS. The next row is loaded before this one's sums, which
-// wait for each other. 16383 rows of 4096 in bf16: forward 52 us (5.2 TB/s), gradient 84 (4.8); in fp32 5.8 and 5.0 TB/s.
+// wait for each other. 16383 rows of 4096 in bf16: forward 44 us (6.1 TB/s; 48 right before the gradient), gradient 83
+// (4.8); in fp32 100 (5.4) and 154 (5.2).
 //
 // Rows of an odd width, or strided ones, begin anywhere: the accesses are of 16 bytes all the same, which the hardware
 // takes at any alignment (8192 rows of 2049 in bf16: 126 -> 20 us against single elements, the gradient 139 -> 32).
@@ -340,12 +341,18 @@ hipError_t launch(const NormK& k, bool grad, hipStream_t s) {
   const int slots = k.tr > 128 ? 1 : 256 / k.tr, threads = slots * k.tr;
   const int64_t trips = (k.rows + slots - 1) / slots;
   if (!grad) {
-    const unsigned groups = (unsigned)std::min<int64_t>(trips, 4096);
+    // Four work-groups a CU, or two wide ones, that stay, so that a row's loads hide behind the one before it and the
+    // parameters are read once: 16383 rows of 4096 in bf16 take 57, 43, 44, 48 us with 512, 1024, 4096, 8192 work-groups
+    // of 256 threads; 8192 rows of 8192 43, 44, 53, 61 with 512 threads; 100,000 rows of 128 14, 11, 11, 11. In fp32, whose
+    // rows of 4096 are two loads a thread longer, 1024 against 4096 take 100 and 97
+    const unsigned groups = (unsigned)std::min<int64_t>(trips, threads <= 320 ? 1024 : 512);
     hipLaunchKernelGGL((layer_norm_kernel<IO, V, UPT, T>), dim3(groups), dim3(threads), 0, s, k);
   } else {
-    // a work-group's row of partial sums costs as much as some rows of the input: eight trips for it, where that leaves
-    // half the CUs one (2048 rows of 4096 in bf16: 512 work-groups 25.5 us, 256 22.1; 512 rows: 512 23.5, 128 17.8)
-    *k.groups = (int)std::min<int64_t>(std::max<int64_t>((trips + 7) / 8, std::min<int64_t>(trips, 128)), MAX_GROUPS);
+    // a work-group's row of partial sums costs as much as some rows of the input: eight trips for it (2048 rows of 4096 in
+    // bf16: 512 work-groups 25.5 us, 256 22.1; 512 rows: 512 23.5, 128 17.8), four of several narrow rows (16384 of
+    // 128: 128 work-groups 9.9, 256 7.6), but no fewer than half the CUs, or all
+    const int64_t few = slots > 1 ? (trips + 3) / 4 : (trips + 7) / 8;
+    *k.groups = (int)std::min<int64_t>(std::max(few, std::min<int64_t>(trips, slots > 1 ? 256 : 128)), MAX_GROUPS);
     const size_t lds = slots > 1 && k.part ? (size_t)slots * k.width * 2 * sizeof(float) : 0;
     hipLaunchKernelGGL((layer_norm_grad_kernel<IO, V, UPT, T>), dim3(*k.groups), dim3(threads), lds, s, k);
   }
@@ -369,7 +376,8 @@ hipError_t launch_io(NormK k, bool grad, hipStream_t s) {
   if (k.tr <= 256) return launch<IO, V, UPT, 256>(k, grad, s);
   if (k.tr <= 512) return launch<IO, V, UPT, 512>(k, grad, s);
   // (two work-groups of 512 threads on a CU pass the time of each other's barriers, one of 1024 has nobody to: 4096 rows of
-  // 16384 in bf16 take 83 against 88 us, their gradient 112 against 124. In 32 bits 512 threads would have twice the registers.)
+  // 16384 in bf16 take 83 against 88 us at a work-group a row, their gradient 112 against 124. In 32 bits 512 threads
+  // would have twice the registers.)
   if constexpr (V == 8) {
     k.tr = ((units + 3) / 4 + 63) / 64 * 64;
     return launch<IO, V, 4, 512>(k, grad, s);
