@@ -64,9 +64,12 @@ SIGNATURES = {
                               _P, _I, _P, _I, _I, _I, _I, _I, _I64, _P, _P]),
     "dsa_dense_attn_workspace_bytes": (_SZ, [_I] * 9),
     "dsa_dense_attn": (_I, [_P, _I64, _I64] * 5 + [_I, _P, _P, _P, _P] + [_I] * 11 + [_F, _P, _I, _P, _P, _P, _SZ, _I, _P]),
+    "dsa_dense_attn_batched": (_I, [_P, _I64, _I64] * 5 + [_I, _P, _P, _P, _P] + [_I] * 11 + [_F, _P, _I, _P, _P, _P, _SZ, _I, _P, _P]),
     "dsa_dense_attn_grad_workspace_bytes": (_SZ, [_I] * 13),
     "dsa_dense_attn_grad": (_I, [_P, _I64, _I64] * 7 + [_I, _P, _P, _P, _P] + [_I] * 13 + [_F, _I, _P, _P] + [_P] * 6
                             + [_SZ, _I, _P]),
+    "dsa_dense_attn_grad_batched": (_I, [_P, _I64, _I64] * 7 + [_I, _P, _P, _P, _P] + [_I] * 13 + [_F, _I, _P, _P] + [_P] * 6
+                                    + [_SZ, _I, _P, _P]),
     "dsa_layer_norm": (_I, [_P, _I64, _I, _I64, _I, _P, _P, _I, _F, _P, _P, _P, _P]),
     "dsa_layer_norm_grad_workspace_bytes": (_SZ, [_I64, _I]),
     "dsa_layer_norm_grad": (_I, [_P, _I64, _P, _I64, _I, _I64, _I, _P, _P, _P, _I, _P, _P, _P, _P, _SZ, _P]),

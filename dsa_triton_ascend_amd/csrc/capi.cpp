@@ -11,6 +11,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 
 #include "../../include/dsa_mi355x.h"
 #include "dsa_common.hpp"
@@ -753,6 +754,17 @@ int dsa_layer_norm_grad(const void* d_out, int64_t d_row_stride, const void* x, 
 }
 
 namespace {
+void set_batches(std::initializer_list<DenseTensor*> tensors, const int64_t* strides, DenseArgs& a) {
+  for (DenseTensor* t : tensors) t->batch = *strides++;
+  a.apart = 1;
+}
+int check_strides(const char* fn, const DenseTensor& t) {
+  if (((uintptr_t)t.p & 15) != 0 || t.row % 8 != 0 || t.head % 8 != 0 || t.batch % 8 != 0)
+    return fail(DSA_ERR_INVALID, "%s: sequences, rows and heads must begin on 16-byte borders", fn);
+  if (t.row < 0 || t.head < 0 || t.batch < 0 || t.row >= (1 << 24) || t.head >= (1ll << 40) || t.batch >= (1ll << 45))
+    return fail(DSA_ERR_UNSUPPORTED, "%s: row strides of 2^24 elements, or sequences 2^45 apart", fn);
+  return DSA_OK;
+}
 int check_dense(const char* fn, const DenseArgs& a) {
   const bool rope = a.dr > 0;
   if (!a.q.p || !a.k.p || !a.v.p || (rope && (!a.qr.p || !a.kr.p)) || !a.row_start || !a.key_start || !a.act_q || !a.act_k)
@@ -770,14 +782,14 @@ int check_dense(const char* fn, const DenseArgs& a) {
     return fail(DSA_ERR_INVALID, "%s: rows_behind, max_rows or max_kv past the tensors' rows", fn);
   if (a.stat_padded && a.total_rows % a.batch != 0)
     return fail(DSA_ERR_INVALID, "%s: padded statistics of rows that do not split evenly", fn);
+  if (a.apart && (!a.stat_padded || a.rows_behind != 0 || a.total_keys % a.batch != 0))
+    return fail(DSA_ERR_INVALID, "%s: batch strides are for padded batches", fn);
   if ((int64_t)a.total_rows * a.n1 >= (1 << 30) || (int64_t)a.total_keys * a.n2 >= (1 << 30) || a.batch > 65535)
     return fail(DSA_ERR_UNSUPPORTED, "%s: 2^30 head rows, or more than 65535 sequences", fn);
   for (const DenseTensor* t : {&a.q, &a.qr, &a.k, &a.kr, &a.v}) {
     if (!rope && (t == &a.qr || t == &a.kr)) continue;
-    if (((uintptr_t)t->p & 15) != 0 || t->row % 8 != 0 || t->head % 8 != 0)
-      return fail(DSA_ERR_INVALID, "%s: rows and heads must begin on 16-byte borders", fn);
-    if (t->row < 0 || t->head < 0 || t->row >= (1 << 24) || t->head >= (1ll << 40))
-      return fail(DSA_ERR_UNSUPPORTED, "%s: row strides of 2^24 elements", fn);
+    const int st = check_strides(fn, *t);
+    if (st != DSA_OK) return st;
   }
   return DSA_OK;
 }
@@ -796,13 +808,13 @@ size_t dsa_dense_attn_workspace_bytes(int batch, int total_rows, int rows_behind
   return std::max(full, dense_attn_workspace_bytes(a));
 }
 
-int dsa_dense_attn(const void* query, int64_t q_row, int64_t q_head, const void* query_rope, int64_t qr_row, int64_t qr_head,
-                   const void* key, int64_t k_row, int64_t k_head, const void* key_rope, int64_t kr_row, int64_t kr_head,
-                   const void* value, int64_t v_row, int64_t v_head, int io_dtype, const int32_t* row_start,
-                   const int32_t* key_start, const int32_t* act_q, const int32_t* act_k, int batch, int total_rows,
-                   int total_keys, int rows_behind, int n1, int n2, int d, int dr, int max_rows, int max_kv, int sparse_mode,
-                   float scale, void* out, int stat_padded, float* sm_max, float* sm_sum, void* workspace,
-                   size_t workspace_bytes, int kv_splits, void* stream) {
+int dsa_dense_attn_batched(const void* query, int64_t q_row, int64_t q_head, const void* query_rope, int64_t qr_row, int64_t qr_head,
+                           const void* key, int64_t k_row, int64_t k_head, const void* key_rope, int64_t kr_row, int64_t kr_head,
+                           const void* value, int64_t v_row, int64_t v_head, int io_dtype, const int32_t* row_start,
+                           const int32_t* key_start, const int32_t* act_q, const int32_t* act_k, int batch, int total_rows,
+                           int total_keys, int rows_behind, int n1, int n2, int d, int dr, int max_rows, int max_kv, int sparse_mode,
+                           float scale, void* out, int stat_padded, float* sm_max, float* sm_sum, void* workspace,
+                           size_t workspace_bytes, int kv_splits, const int64_t* batch_strides, void* stream) {
   DenseArgs a{};
   a.q = {query, q_row, q_head}, a.qr = {query_rope, qr_row, qr_head}, a.k = {key, k_row, k_head};
   a.kr = {key_rope, kr_row, kr_head}, a.v = {value, v_row, v_head}, a.io = io_dtype;
@@ -811,6 +823,7 @@ int dsa_dense_attn(const void* query, int64_t q_row, int64_t q_head, const void*
   a.max_rows = max_rows, a.max_kv = max_kv, a.sparse_mode = sparse_mode, a.scale = scale, a.out = out;
   a.stat_padded = stat_padded, a.sm_max = sm_max, a.sm_sum = sm_sum, a.ws = workspace, a.ws_bytes = workspace_bytes;
   a.kv_splits = kv_splits;
+  if (batch_strides) set_batches({&a.q, &a.qr, &a.k, &a.kr, &a.v}, batch_strides, a);
   const int st = check_dense("dsa_dense_attn", a);
   if (st != DSA_OK) return st;
   if (!out) return fail(DSA_ERR_INVALID, "dsa_dense_attn: null pointer argument");
@@ -830,6 +843,19 @@ int dsa_dense_attn(const void* query, int64_t q_row, int64_t q_head, const void*
   return hip_status(e, "dsa_dense_attn launch");
 }
 
+int dsa_dense_attn(const void* query, int64_t q_row, int64_t q_head, const void* query_rope, int64_t qr_row, int64_t qr_head,
+                   const void* key, int64_t k_row, int64_t k_head, const void* key_rope, int64_t kr_row, int64_t kr_head,
+                   const void* value, int64_t v_row, int64_t v_head, int io_dtype, const int32_t* row_start,
+                   const int32_t* key_start, const int32_t* act_q, const int32_t* act_k, int batch, int total_rows,
+                   int total_keys, int rows_behind, int n1, int n2, int d, int dr, int max_rows, int max_kv, int sparse_mode,
+                   float scale, void* out, int stat_padded, float* sm_max, float* sm_sum, void* workspace,
+                   size_t workspace_bytes, int kv_splits, void* stream) {
+  return dsa_dense_attn_batched(query, q_row, q_head, query_rope, qr_row, qr_head, key, k_row, k_head, key_rope, kr_row,
+                                kr_head, value, v_row, v_head, io_dtype, row_start, key_start, act_q, act_k, batch,
+                                total_rows, total_keys, rows_behind, n1, n2, d, dr, max_rows, max_kv, sparse_mode, scale,
+                                out, stat_padded, sm_max, sm_sum, workspace, workspace_bytes, kv_splits, nullptr, stream);
+}
+
 size_t dsa_dense_attn_grad_workspace_bytes(int batch, int total_rows, int total_keys, int rows_behind, int keys_behind, int n1,
                                            int n2, int d, int dr, int max_rows, int max_keys, int max_kv, int splits) {
   if (batch <= 0 || total_rows < 0 || total_keys < 0 || rows_behind < 0 || keys_behind < 0 || n1 <= 0 || n2 <= 0 || n1 % n2 != 0 ||
@@ -842,15 +868,15 @@ size_t dsa_dense_attn_grad_workspace_bytes(int batch, int total_rows, int total_
   return dense_grad_workspace_bytes(g);
 }
 
-int dsa_dense_attn_grad(const void* query, int64_t q_row, int64_t q_head, const void* query_rope, int64_t qr_row, int64_t qr_head,
-                        const void* key, int64_t k_row, int64_t k_head, const void* key_rope, int64_t kr_row, int64_t kr_head,
-                        const void* value, int64_t v_row, int64_t v_head, const void* d_out, int64_t d_row, int64_t d_head,
-                        const void* out, int64_t o_row, int64_t o_head, int io_dtype, const int32_t* row_start,
-                        const int32_t* key_start, const int32_t* act_q, const int32_t* act_k, int batch, int total_rows,
-                        int total_keys, int rows_behind, int keys_behind, int n1, int n2, int d, int dr, int max_rows,
-                        int max_keys, int max_kv, int sparse_mode, float scale, int stat_padded, const float* sm_max,
-                        const float* sm_sum, void* d_query, void* d_query_rope, void* d_key, void* d_key_rope, void* d_value,
-                        void* workspace, size_t workspace_bytes, int splits, void* stream) {
+int dsa_dense_attn_grad_batched(const void* query, int64_t q_row, int64_t q_head, const void* query_rope, int64_t qr_row, int64_t qr_head,
+                                const void* key, int64_t k_row, int64_t k_head, const void* key_rope, int64_t kr_row, int64_t kr_head,
+                                const void* value, int64_t v_row, int64_t v_head, const void* d_out, int64_t d_row, int64_t d_head,
+                                const void* out, int64_t o_row, int64_t o_head, int io_dtype, const int32_t* row_start,
+                                const int32_t* key_start, const int32_t* act_q, const int32_t* act_k, int batch, int total_rows,
+                                int total_keys, int rows_behind, int keys_behind, int n1, int n2, int d, int dr, int max_rows,
+                                int max_keys, int max_kv, int sparse_mode, float scale, int stat_padded, const float* sm_max,
+                                const float* sm_sum, void* d_query, void* d_query_rope, void* d_key, void* d_key_rope, void* d_value,
+                                void* workspace, size_t workspace_bytes, int splits, const int64_t* batch_strides, void* stream) {
   static const char* fn = "dsa_dense_attn_grad";
   DenseGradArgs g{};
   DenseArgs& a = g.f;
@@ -862,16 +888,16 @@ int dsa_dense_attn_grad(const void* query, int64_t q_row, int64_t q_head, const 
   a.sm_max = const_cast<float*>(sm_max), a.sm_sum = const_cast<float*>(sm_sum), a.ws = workspace, a.ws_bytes = workspace_bytes;
   a.kv_splits = splits, g.d_out = {d_out, d_row, d_head}, g.out = {out, o_row, o_head}, g.keys_behind = keys_behind;
   g.max_keys = max_keys, g.dq = d_query, g.dqr = d_query_rope, g.dk = d_key, g.dkr = d_key_rope, g.dv = d_value;
+  if (batch_strides) set_batches({&a.q, &a.qr, &a.k, &a.kr, &a.v, &g.d_out, &g.out}, batch_strides, a);
   const int st = check_dense(fn, a);
   if (st != DSA_OK) return st;
   if (!d_out || !out || !sm_max || !sm_sum || !d_query || !d_key || !d_value || (dr > 0 && (!d_query_rope || !d_key_rope)))
     return fail(DSA_ERR_INVALID, "%s: null pointer argument", fn);
   for (const DenseTensor* t : {&g.d_out, &g.out}) {
-    if (((uintptr_t)t->p & 15) != 0 || t->row % 8 != 0 || t->head % 8 != 0)
-      return fail(DSA_ERR_INVALID, "%s: rows and heads must begin on 16-byte borders", fn);
-    if (t->row < 0 || t->head < 0 || t->row >= (1 << 24) || t->head >= (1ll << 40))
-      return fail(DSA_ERR_UNSUPPORTED, "%s: row strides of 2^24 elements", fn);
+    const int of = check_strides(fn, *t);
+    if (of != DSA_OK) return of;
   }
+  if (a.apart && keys_behind != 0) return fail(DSA_ERR_INVALID, "%s: batch strides are for padded batches", fn);
   if ((((uintptr_t)d_query | (uintptr_t)d_query_rope | (uintptr_t)d_key | (uintptr_t)d_key_rope | (uintptr_t)d_value) & 15) != 0)
     return fail(DSA_ERR_INVALID, "%s: outputs must be 16-byte aligned", fn);
   if (keys_behind < 0 || keys_behind > total_keys || max_keys < 0 || max_keys > total_keys)
@@ -887,6 +913,23 @@ int dsa_dense_attn_grad(const void* query, int64_t q_row, int64_t q_head, const 
     return fail(DSA_ERR_INVALID, "%s: a 16-byte aligned workspace of %zu bytes required, %zu given", fn, lacking,
                 workspace ? workspace_bytes : (size_t)0);
   return hip_status(e, "dsa_dense_attn_grad launch");
+}
+
+int dsa_dense_attn_grad(const void* query, int64_t q_row, int64_t q_head, const void* query_rope, int64_t qr_row, int64_t qr_head,
+                        const void* key, int64_t k_row, int64_t k_head, const void* key_rope, int64_t kr_row, int64_t kr_head,
+                        const void* value, int64_t v_row, int64_t v_head, const void* d_out, int64_t d_row, int64_t d_head,
+                        const void* out, int64_t o_row, int64_t o_head, int io_dtype, const int32_t* row_start,
+                        const int32_t* key_start, const int32_t* act_q, const int32_t* act_k, int batch, int total_rows,
+                        int total_keys, int rows_behind, int keys_behind, int n1, int n2, int d, int dr, int max_rows,
+                        int max_keys, int max_kv, int sparse_mode, float scale, int stat_padded, const float* sm_max,
+                        const float* sm_sum, void* d_query, void* d_query_rope, void* d_key, void* d_key_rope, void* d_value,
+                        void* workspace, size_t workspace_bytes, int splits, void* stream) {
+  return dsa_dense_attn_grad_batched(query, q_row, q_head, query_rope, qr_row, qr_head, key, k_row, k_head, key_rope,
+                                     kr_row, kr_head, value, v_row, v_head, d_out, d_row, d_head, out, o_row, o_head,
+                                     io_dtype, row_start, key_start, act_q, act_k, batch, total_rows, total_keys,
+                                     rows_behind, keys_behind, n1, n2, d, dr, max_rows, max_keys, max_kv, sparse_mode,
+                                     scale, stat_padded, sm_max, sm_sum, d_query, d_query_rope, d_key, d_key_rope, d_value,
+                                     workspace, workspace_bytes, splits, nullptr, stream);
 }
 
 }  // extern "C"

@@ -135,8 +135,8 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
     const int r = valid[m] ? row[m] : r_end - 1, s = r / a.per, g = r - s * a.per;
     lim[m] = valid[m] ? min(limit_of(a.len, seq, s), t_hi) : 0;
     dead[m] = lim[m] <= t_lo;
-    qp[m] = a.q.p + (seq.r0 + s) * a.q.row + (n * a.per + g) * a.q.head;
-    if constexpr (DR > 0) qrp[m] = a.qr.p + (seq.r0 + s) * a.qr.row + (n * a.per + g) * a.qr.head;
+    qp[m] = first_of(a.len, a.q, b, seq.r0) + s * a.q.row + (n * a.per + g) * a.q.head;
+    if constexpr (DR > 0) qrp[m] = first_of(a.len, a.qr, b, seq.r0) + s * a.qr.row + (n * a.per + g) * a.qr.head;
   }
 
   f32x16 o[RT][ON];
@@ -161,9 +161,9 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
 
     // ---- tiles: each wave loads a share, in GPW loads, one tile after another (past the last one it again, into
     // buffers that nobody reads: no load then depends on a branch)
-    Stream<RB, BN, NWV> ks(a.k.p + (int64_t)(seq.k0 + t_lo) * a.k.row + n * a.k.head, (uint32_t)a.k.row * 2, L.k[0], wave, lane);
-    Stream<RB, BN, NWV> vs(a.v.p + (int64_t)(seq.k0 + t_lo) * a.v.row + n * a.v.head, (uint32_t)a.v.row * 2, L.v[0], wave, lane);
-    Stream<128, BN, NWV> rs(DR ? a.kr.p + (int64_t)(seq.k0 + t_lo) * a.kr.row + n * a.kr.head : nullptr, (uint32_t)a.kr.row * 2, L.kr[0], wave, lane);
+    Stream<RB, BN, NWV> ks(first_of(a.len, a.k, b, seq.k0) + t_lo * a.k.row + n * a.k.head, (uint32_t)a.k.row * 2, L.k[0], wave, lane);
+    Stream<RB, BN, NWV> vs(first_of(a.len, a.v, b, seq.k0) + t_lo * a.v.row + n * a.v.head, (uint32_t)a.v.row * 2, L.v[0], wave, lane);
+    Stream<128, BN, NWV> rs(DR ? first_of(a.len, a.kr, b, seq.k0) + t_lo * a.kr.row + n * a.kr.head : nullptr, (uint32_t)a.kr.row * 2, L.kr[0], wave, lane);
     constexpr int CK = ks.sh.CNT, CR = DR ? rs.sh.CNT : 0, GPW = 2 * CK + CR;
     auto load_part = [&](auto jc, int buf) __attribute__((always_inline)) {
       constexpr int j = decltype(jc)::value;
@@ -674,9 +674,9 @@ hipError_t launch_dense_attn(const DenseArgs& a, size_t* lacking, hipStream_t s)
   if (*lacking) return hipSuccess;
   if (c.groups >= (1 << 24) || (c.splits > 1 && (int64_t)c.blocks * (a.d / 32) >= (1 << 24))) return hipErrorInvalidConfiguration;   // 2^32 threads
   DenseK k{};
-  auto rows = [](const DenseTensor& t) { return Rows{(const uint16_t*)t.p, t.row, t.head}; };
+  auto rows = [](const DenseTensor& t) { return Rows{(const uint16_t*)t.p, t.row, t.head, t.batch}; };
   k.q = rows(a.q), k.qr = rows(a.qr), k.k = rows(a.k), k.kr = rows(a.kr), k.v = rows(a.v);
-  k.len = {a.row_start, a.key_start, a.act_q, a.act_k, a.batch, a.total_rows, a.total_keys, a.sparse_mode};
+  k.len = {a.row_start, a.key_start, a.act_q, a.act_k, a.batch, a.total_rows, a.total_keys, a.sparse_mode, a.apart};
   k.tiles = {a.batch + (a.rows_behind > 0), a.n2, c.even};
   k.per = a.n1 / a.n2;
   k.heads = a.n1;

@@ -11,10 +11,10 @@ namespace dsa {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-// A tensor [rows, heads, width] by strides in elements
+// A tensor [rows, heads, width], or [sequences, rows, heads, width], by strides in elements
 struct Rows {
   const uint16_t* p;
-  int64_t row, head;
+  int64_t row, head, batch;
 };
 
 // Lengths of a call. Sequence b's query rows begin at row_start[b], its keys at key_start[b]; sequence `batch` is
@@ -25,7 +25,12 @@ struct Lens {
   const int32_t* act_q;
   const int32_t* act_k;
   int batch, rows, keys, mode;   // rows, keys: of the tensors
+  int apart;                     // operands' sequences lie batch strides apart, else their rows follow each other
 };
+// where the rows of sequence b, whose first one is row r0 of all, begin in an operand
+__device__ __forceinline__ const uint16_t* first_of(const Lens& l, const Rows& x, int b, int r0) {
+  return x.p + (l.apart ? (int64_t)b * x.batch : (int64_t)r0 * x.row);
+}
 struct Seq {
   int r0, rows;   // first query row, rows that belong to it (act_q of them are queries)
   int k0, keys;

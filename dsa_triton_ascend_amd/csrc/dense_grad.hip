@@ -96,14 +96,16 @@ __global__ __launch_bounds__(256) void dense_prep_kernel(GradK a) {
     const int h = (int)(i - row * a.heads);
     const int n = row_div(a, h), g = h - n * a.per;
     float d[8], o[8], s = 0.f, q = 0.f;
-    values(a.d.p + row * a.d.row + h * a.d.head, d);
-    values(a.o.p + row * a.o.row + h * a.o.head, o);
+    int64_t b = 0, r = row;   // where it lies: row r of sequence b, or of all
+    if (a.len.apart) b = row / a.s1, r = row - b * a.s1;
+    values(a.d.p + b * a.d.batch + r * a.d.row + h * a.d.head, d);
+    values(a.o.p + b * a.o.batch + r * a.o.row + h * a.o.head, o);
 #pragma unroll
     for (int e = 0; e < 8; ++e) s = fmaf(d[e], o[e], s), q = fmaf(d[e], d[e], q);
     const int64_t at = n * (int64_t)a.len.rows * a.per + row * a.per + g;
     int64_t st = at;
     if (a.stat_padded) {
-      const int64_t b = row / a.s1;
+      b = row / a.s1;
       st = ((b * a.key_heads + n) * a.s1 + (row - b * a.s1)) * a.per + g;
     }
     const float m = a.sm_max[st], l = a.sm_sum[st];
@@ -125,7 +127,8 @@ __global__ __launch_bounds__(256) void dense_prep_kernel(GradK a) {
       const int b = batch_of_row(a.len.key_start, a.len.batch, (int)row);
       if (row - a.len.key_start[b] >= a.len.act_k[b]) continue;   // padding
       float v[8], q = 0.f;
-      values(a.v.p + row * a.v.row + (i - row * a.key_heads) * a.v.head, v);
+      const int k0 = a.len.key_start[b];
+      values(first_of(a.len, a.v, b, k0) + (row - k0) * a.v.row + (i - row * a.key_heads) * a.v.head, v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) q = fmaf(v[e], v[e], q);
       q = row_sum(q);
@@ -278,7 +281,7 @@ __global__ __launch_bounds__(NWV * 64) void dense_keys_kernel(GradK a) {
       return ((int64_t)s * x.row + (int64_t)(r - s * a.per) * x.head) * 2;
     };
     auto base_of = [&](const Rows& x) {
-      return reinterpret_cast<const char*>(x.p + (int64_t)seq.r0 * x.row + (int64_t)n * a.per * x.head);
+      return reinterpret_cast<const char*>(first_of(a.len, x, b, seq.r0) + (int64_t)n * a.per * x.head);
     };
     const char* const qb = base_of(a.q);
     const char* const db = base_of(a.d);
@@ -353,13 +356,13 @@ __global__ __launch_bounds__(NWV * 64) void dense_keys_kernel(GradK a) {
     load_tile(0);
     uint4 kf[KS], vf[KSN];
     {
-      const int64_t tt = seq.k0 + min(t, t_seen - 1);
-      const uint16_t* kp = a.k.p + tt * a.k.row + n * a.k.head + kg * 8;
-      const uint16_t* vp = a.v.p + tt * a.v.row + n * a.v.head + kg * 8;
+      const int64_t tt = min(t, t_seen - 1);
+      const uint16_t* kp = first_of(a.len, a.k, b, seq.k0) + tt * a.k.row + n * a.k.head + kg * 8;
+      const uint16_t* vp = first_of(a.len, a.v, b, seq.k0) + tt * a.v.row + n * a.v.head + kg * 8;
 #pragma unroll
       for (int j = 0; j < KSN; ++j) kf[j] = ldg16(kp + j * 16), vf[j] = ldg16(vp + j * 16);
       if constexpr (DR > 0) {
-        const uint16_t* rp = a.kr.p + tt * a.kr.row + n * a.kr.head + kg * 8;
+        const uint16_t* rp = first_of(a.len, a.kr, b, seq.k0) + tt * a.kr.row + n * a.kr.head + kg * 8;
 #pragma unroll
         for (int j = KSN; j < KS; ++j) kf[j] = ldg16(rp + (j - KSN) * 16);
       }
@@ -679,9 +682,9 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
     const float sl2 = (a.scale == 0.f ? 1e-30f : a.scale) * LOG2E;
     const float masked = sl2 > 0.f ? -INFINITY : INFINITY;
     // (as in the forward: past the last tile it again)
-    Stream<RB, BN, NWV> ks(a.k.p + (int64_t)(seq.k0 + t_lo) * a.k.row + n * a.k.head, (uint32_t)a.k.row * 2, L.t[0].k, wave, lane);
-    Stream<RB, BN, NWV> vs(a.v.p + (int64_t)(seq.k0 + t_lo) * a.v.row + n * a.v.head, (uint32_t)a.v.row * 2, L.t[0].v, wave, lane);
-    Stream<128, BN, NWV> rs(DR ? a.kr.p + (int64_t)(seq.k0 + t_lo) * a.kr.row + n * a.kr.head : nullptr, (uint32_t)a.kr.row * 2, L.kr[0], wave, lane);
+    Stream<RB, BN, NWV> ks(first_of(a.len, a.k, b, seq.k0) + t_lo * a.k.row + n * a.k.head, (uint32_t)a.k.row * 2, L.t[0].k, wave, lane);
+    Stream<RB, BN, NWV> vs(first_of(a.len, a.v, b, seq.k0) + t_lo * a.v.row + n * a.v.head, (uint32_t)a.v.row * 2, L.t[0].v, wave, lane);
+    Stream<128, BN, NWV> rs(DR ? first_of(a.len, a.kr, b, seq.k0) + t_lo * a.kr.row + n * a.kr.head : nullptr, (uint32_t)a.kr.row * 2, L.kr[0], wave, lane);
     constexpr int CK = ks.sh.CNT, CR = DR ? rs.sh.CNT : 0, GPW = 2 * CK + CR;
     auto load_part = [&](auto jc, int buf) __attribute__((always_inline)) {
       constexpr int j = decltype(jc)::value;
@@ -724,13 +727,13 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
     const float lse = a.lse[stat];
     float delta = -a.delta[stat];
     {
-      const int64_t q_row = seq.r0 + s, head = n * a.per + g;
-      const uint16_t* qp = a.q.p + q_row * a.q.row + head * a.q.head + kg * 8;
-      const uint16_t* dp = a.d.p + q_row * a.d.row + head * a.d.head + kg * 8;
+      const int64_t head = n * a.per + g;
+      const uint16_t* qp = first_of(a.len, a.q, b, seq.r0) + s * a.q.row + head * a.q.head + kg * 8;
+      const uint16_t* dp = first_of(a.len, a.d, b, seq.r0) + s * a.d.row + head * a.d.head + kg * 8;
 #pragma unroll
       for (int j = 0; j < KSN; ++j) qf[j] = ldg16(qp + j * 16), df[j] = ldg16(dp + j * 16);
       if constexpr (DR > 0) {
-        const uint16_t* rp = a.qr.p + q_row * a.qr.row + head * a.qr.head + kg * 8;
+        const uint16_t* rp = first_of(a.len, a.qr, b, seq.r0) + s * a.qr.row + head * a.qr.head + kg * 8;
 #pragma unroll
         for (int j = KSN; j < KS; ++j) qf[j] = ldg16(rp + (j - KSN) * 16);
       }
@@ -1117,9 +1120,9 @@ hipError_t launch_dense_grad(const DenseGradArgs& g, size_t* lacking, hipStream_
   if (*lacking) return hipSuccess;
   if (c.keys.groups >= (1 << 24) || c.queries.groups >= (1 << 24)) return hipErrorInvalidConfiguration;   // 2^32 threads
   GradK k{};
-  auto rows = [](const DenseTensor& t) { return Rows{(const uint16_t*)t.p, t.row, t.head}; };
+  auto rows = [](const DenseTensor& t) { return Rows{(const uint16_t*)t.p, t.row, t.head, t.batch}; };
   k.q = rows(a.q), k.qr = rows(a.qr), k.k = rows(a.k), k.kr = rows(a.kr), k.v = rows(a.v), k.d = rows(g.d_out), k.o = rows(g.out);
-  k.len = {a.row_start, a.key_start, a.act_q, a.act_k, a.batch, a.total_rows, a.total_keys, a.sparse_mode};
+  k.len = {a.row_start, a.key_start, a.act_q, a.act_k, a.batch, a.total_rows, a.total_keys, a.sparse_mode, a.apart};
   k.heads = a.n1;
   k.key_heads = a.n2;
   k.per = a.n1 / a.n2;

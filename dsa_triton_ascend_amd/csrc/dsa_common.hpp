@@ -536,13 +536,14 @@ size_t layer_norm_grad_workspace_bytes(int64_t rows, int width);
 hipError_t launch_layer_norm_grad(const NormArgs& a, hipStream_t s);
 // Dense attention over keys and values of their own: tensors [rows, heads, width] by strides (elements)
 struct DenseTensor {
-  const void* p; int64_t row, head;
+  const void* p; int64_t row, head, batch;   // batch: from a sequence's first row to the next one's, where they lie apart
 };
 struct DenseArgs {
   DenseTensor q, qr, k, kr, v; int io;
   const int32_t* row_start; const int32_t* key_start;   // [batch + 1]
   const int32_t* act_q; const int32_t* act_k;
   int batch, total_rows, total_keys, n1, n2, d, dr, rows_behind, max_rows, max_kv, sparse_mode; float scale;
+  int apart;                    // sequences by their tensors' batch strides, else by row_start and key_start
   int stat_padded;              // statistics [batch, n2, rows a sequence, n1 / n2], else [n2, total_rows, n1 / n2]
   void* out; float* sm_max; float* sm_sum;
   void* ws; size_t ws_bytes; int kv_splits;

@@ -8,6 +8,8 @@ cache there is ``shared_prefix_attention``.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _host as H
@@ -16,32 +18,38 @@ from . import _lib
 VALID_D = (64, 128)
 FEW_STATISTICS = 16384   # fp32 values
 D_ROPE = 64
+MAX_ROW = 1 << 24   # elements from one row to the next
 
 
 def _packed(t: torch.Tensor, heads: int) -> torch.Tensor:
-    """t as [rows, heads, width], in place where the kernels can read its strides, else a copy"""
+    """t as [rows, heads, width], or where a padded batch's sequences do not join as [sequences, rows, heads, width]; in place
+    where the kernels can read its strides, else a copy"""
     if t.numel() == 0:
         return t.reshape(-1, heads, t.shape[-1]) if t.shape[-1] and heads else t
     if t.dim() == 4:
         B, S = t.shape[:2]
-        if B > 1 and t.stride(0) != S * t.stride(1):
-            t = t.contiguous()
-        if S == 1 and B > 1:
-            t = t[:, 0]
-        elif B == 1:
+        batch, row = t.stride()[:2]
+        if B == 1:
             t = t[0]
-        else:
+        elif S == 1 and batch < MAX_ROW:
+            t = t[:, 0]
+        elif S > 1 and batch == S * row:
             t = t.flatten(0, 1)
-    row, head, last = t.stride()
-    if last != 1 or row % 8 or head % 8 or t.data_ptr() % 16 or row >= 1 << 24:
+    if t.dim() == 3:
+        row, head, last = t.stride()
+        if last == 1 and not (row % 8 or head % 8 or t.data_ptr() % 16) and row < MAX_ROW:
+            return t
+    *lead, row, head = (x if n > 1 else 0 for x, n in zip(t.stride()[:-1], t.shape))   # (of one, it does not matter)
+    if t.stride(-1) != 1 or row % 8 or head % 8 or t.data_ptr() % 16 or row >= MAX_ROW or (lead and lead[0] % 8):
         t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
+        t = _packed(t.clone() if t.data_ptr() % 16 else t, heads)
     return t
 
 
 class _Arguments:
     """What the forward and the gradient share: checked operands as packed rows, and lengths"""
+
+    batches = None
 
     def __init__(self, query, key, value, query_rope, key_rope, actual_seq_lengths_query, actual_seq_lengths_kv, scale_value,
                  layout, sparse_mode):
@@ -121,11 +129,14 @@ class _Arguments:
                                                     zero=zero, wait=wait)
 
     def tensors(self, *more):
-        """Pointers and strides as the C entries take them"""
-        out = []
-        for t in (self.q, self.qr, self.k, self.kr, self.v) + more:
-            out += [None, 0, 0] if t is None else [t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0,
-                                                   t.stride(1) if t.shape[1] > 1 else 0]
+        """Pointers and strides as the C entries take them; `batches`: those of the sequences if some do not join, else None"""
+        out, operands = [], (self.q, self.qr, self.k, self.kr, self.v) + more
+        for t in operands:
+            out += [None, 0, 0] if t is None else [t.data_ptr(), t.stride(-3) if t.shape[-3] > 1 else 0,
+                                                   t.stride(-2) if t.shape[-2] > 1 else 0]
+        if self.padded and any(t is not None and t.dim() == 4 for t in operands):
+            self.batches = (ctypes.c_int64 * len(operands))(*(
+                0 if t is None else t.stride(0) if t.dim() == 4 else t.stride(0) * (t.shape[0] // self.batch) for t in operands))
         return out
 
     def lengths(self):
@@ -135,9 +146,10 @@ class _Arguments:
 class DenseAttentionPlan:
     """Validated arguments of one dense_attention call (outputs, workspace, int32 index arrays), all in place when
     the constructor returns; ``run()`` launches on the current stream, which may be another one. The operands are
-    read on the device in each run: a loop that keeps the plan may write them anew between runs (in the plan's copy
-    ``q``, ``qr``, ``k``, ``kr``, ``v``, where one had to be made: strides within the last dimension or off 16-byte
-    borders). Runs write the same outputs and workspace: the caller orders them."""
+    read on the device in each run: a loop that keeps the plan may write them anew between runs, also where they are slices of
+    longer tensors or transposed ones. Only an operand with strides within the last dimension, with heads, rows or sequences off
+    16-byte borders or with 2^24 elements or more from row to row is copied here, once: then the plan's copy (``q``, ``qr``,
+    ``k``, ``kr``, ``v``) is what to write. Runs write the same outputs and workspace: the caller orders them."""
 
     def __init__(self, query, key, value, scale_value=1.0, actual_seq_lengths_query=None, actual_seq_lengths_kv=None,
                  query_rope=None, key_rope=None, layout="BSND", sparse_mode=3, return_softmax_lse=False, kv_splits=0, *,
@@ -175,13 +187,15 @@ class DenseAttentionPlan:
                          a.max_rows, a.max_kv, a.sparse_mode, a.scale, self.out.data_ptr(), a.padded,
                          self.sm_max.data_ptr() if lse else None, self.sm_sum.data_ptr() if lse else None, H.ptr(self.ws),
                          size, int(kv_splits))
+            self.entry = self.lib.dsa_dense_attn
+            if a.batches is not None:
+                self.entry, self.args = self.lib.dsa_dense_attn_batched, self.args + (a.batches,)
 
         H.on_device(self.dev, place)
 
     def run(self):
         if self.args is not None:
-            H.on_device(self.dev, lambda: _lib.check(self.lib.dsa_dense_attn(*self.args, H.stream_ptr(self.dev)),
-                                                     "dsa_dense_attn"))
+            H.on_device(self.dev, lambda: _lib.check(self.entry(*self.args, H.stream_ptr(self.dev)), "dsa_dense_attn"))
         return self.out, self.sm_max, self.sm_sum
 
 
@@ -191,8 +205,9 @@ def dense_attention(query, key, value, scale_value=1.0, actual_seq_lengths_query
 
     query [B,S1,N1,D] (BSND) or [T1,N1,D] (TND), key and value [B,S2,N2,D] or [T2,N2,D], D 64 or 128, fp16 / bf16; query
     head h reads key head h // (N1 // N2). query_rope and key_rope [..,64] (D = 128) add their product to the scores;
-    one rotary key for all heads is passed expanded. Operands are read in place by their strides where rows
-    and heads begin on 16-byte borders (slices of one projection, expanded heads), else copied.
+    one rotary key for all heads is passed expanded. Operands are read in place by their strides where sequences, rows
+    and heads begin on 16-byte borders, rows less than 2^24 elements from each other (slices of one projection or of a longer
+    cache, heads before rows, expanded heads or sequences), else copied.
     actual_seq_lengths_query / _kv: per batch (BSND; default: all) or cumulative (TND; default: one sequence). A query sees
     the tokens up to its own (sparse_mode 3: its sequence's last query is its last token) or all of its sequence (0).
     Returns (attention_out, softmax_max, softmax_sum), the statistics fp32 [B,N2,S1,N1//N2], as ``dense_loss_backward``
@@ -204,8 +219,8 @@ def dense_attention(query, key, value, scale_value=1.0, actual_seq_lengths_query
 
 class DenseAttentionGradPlan:
     """Validated arguments of one dense_attention_grad call (outputs, workspace, int32 index arrays), all in place when
-    the constructor returns; ``run()`` launches on the current stream, which may be another one. Operands are read in
-    each run, as by :class:`DenseAttentionPlan`."""
+    the constructor returns; ``run()`` launches on the current stream, which may be another one. Operands, d_out (``d``) and out
+    (``o``) are read in each run, as by :class:`DenseAttentionPlan`; the statistics too where they are contiguous."""
 
     def __init__(self, query, key, value, d_out, out, softmax_max, softmax_sum, scale_value=1.0, query_rope=None, key_rope=None,
                  actual_seq_lengths_query=None, actual_seq_lengths_kv=None, layout="BSND", sparse_mode=3, splits=0, *, _wait=True):
@@ -243,13 +258,15 @@ class DenseAttentionGradPlan:
                          a.keys_behind, a.n1, a.n2, a.d, a.dr, a.max_rows, a.max_keys, a.max_kv, a.sparse_mode, a.scale, a.padded,
                          self.sm_max.data_ptr(), self.sm_sum.data_ptr(), dq.data_ptr(), H.ptr(dqr), dk.data_ptr(), H.ptr(dkr),
                          dv.data_ptr(), self.ws.data_ptr(), size, int(splits))
+            self.entry = self.lib.dsa_dense_attn_grad
+            if a.batches is not None:
+                self.entry, self.args = self.lib.dsa_dense_attn_grad_batched, self.args + (a.batches,)
 
         H.on_device(self.dev, place)
 
     def run(self):
         if self.args is not None:
-            H.on_device(self.dev, lambda: _lib.check(self.lib.dsa_dense_attn_grad(*self.args, H.stream_ptr(self.dev)),
-                                                     "dsa_dense_attn_grad"))
+            H.on_device(self.dev, lambda: _lib.check(self.entry(*self.args, H.stream_ptr(self.dev)), "dsa_dense_attn_grad"))
         return self.grads
 
 

@@ -510,6 +510,22 @@ int dsa_dense_attn(const void* query, int64_t q_row, int64_t q_head, const void*
                    size_t workspace_bytes, int kv_splits, void* stream);
 
 /*
+ * dsa_dense_attn of padded batches whose sequences lie apart, each operand's in its own way (slices of longer caches, heads before
+ * rows): batch_strides holds, for query, query_rope, key, key_rope and value, the elements from a sequence's first row to the next
+ * one's (on the host, read before the call returns; multiples of 8, 0 for sequences that share one; below 2^45; what stands for
+ * an operand that is NULL is not read). Sequence b's operand rows are then row_start[b] = b * total_rows / batch and
+ * key_start[b] = b * total_keys / batch by number only; outputs and statistics stay contiguous, stat_padded is 1 and
+ * rows_behind 0. batch_strides NULL: as dsa_dense_attn.
+ */
+int dsa_dense_attn_batched(const void* query, int64_t q_row, int64_t q_head, const void* query_rope, int64_t qr_row, int64_t qr_head,
+                           const void* key, int64_t k_row, int64_t k_head, const void* key_rope, int64_t kr_row, int64_t kr_head,
+                           const void* value, int64_t v_row, int64_t v_head, int io_dtype, const int32_t* row_start,
+                           const int32_t* key_start, const int32_t* act_q, const int32_t* act_k, int batch, int total_rows,
+                           int total_keys, int rows_behind, int n1, int n2, int d, int dr, int max_rows, int max_kv, int sparse_mode,
+                           float scale, void* out, int stat_padded, float* sm_max, float* sm_sum, void* workspace,
+                           size_t workspace_bytes, int kv_splits, const int64_t* batch_strides, void* stream);
+
+/*
  * Gradients of dsa_dense_attn: with P = exp(score - sm_max) / sm_sum, dP = d_out . v, dS = P (dP - d_out . out),
  *   d_query = scale dS (key | key_rope), d_key = scale dS^T (query | query_rope), d_value = P^T d_out,
  * those of a key head summed over its query heads. query .. value, lengths, bounds and statistics as in the forward, whose
@@ -535,6 +551,16 @@ int dsa_dense_attn_grad(const void* query, int64_t q_row, int64_t q_head, const 
                         int max_keys, int max_kv, int sparse_mode, float scale, int stat_padded, const float* sm_max,
                         const float* sm_sum, void* d_query, void* d_query_rope, void* d_key, void* d_key_rope, void* d_value,
                         void* workspace, size_t workspace_bytes, int splits, void* stream);
+/* The same for the gradients: batch_strides of query, query_rope, key, key_rope, value, d_out and out; keys_behind is 0. */
+int dsa_dense_attn_grad_batched(const void* query, int64_t q_row, int64_t q_head, const void* query_rope, int64_t qr_row, int64_t qr_head,
+                                const void* key, int64_t k_row, int64_t k_head, const void* key_rope, int64_t kr_row, int64_t kr_head,
+                                const void* value, int64_t v_row, int64_t v_head, const void* d_out, int64_t d_row, int64_t d_head,
+                                const void* out, int64_t o_row, int64_t o_head, int io_dtype, const int32_t* row_start,
+                                const int32_t* key_start, const int32_t* act_q, const int32_t* act_k, int batch, int total_rows,
+                                int total_keys, int rows_behind, int keys_behind, int n1, int n2, int d, int dr, int max_rows,
+                                int max_keys, int max_kv, int sparse_mode, float scale, int stat_padded, const float* sm_max,
+                                const float* sm_sum, void* d_query, void* d_query_rope, void* d_key, void* d_key_rope, void* d_value,
+                                void* workspace, size_t workspace_bytes, int splits, const int64_t* batch_strides, void* stream);
 
 #define DSA_NORM_MAX_WIDTH 16384
 
