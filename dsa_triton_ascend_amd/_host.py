@@ -127,9 +127,14 @@ def _upload(lib, device, arrays, zero, zero_bytes, wait):
         if zero is not None:
             zero.zero_()
         t = torch.frombuffer(flat, dtype=torch.int32).to(device) if n else torch.empty(0, dtype=torch.int32, device=device)
+    settle(device, wait)
+    return t, sizes
+
+
+def settle(device: torch.device, wait: bool = True):
+    """With `wait`, and but for a stream that is being captured: what the caller put on the current stream is done"""
     if wait and not torch.cuda.is_current_stream_capturing():
         torch.cuda.current_stream(device).synchronize()
-    return t, sizes
 
 
 def stream_ptr(device: torch.device) -> int:

@@ -161,21 +161,20 @@ class DenseAttentionPlan:
         self.dev = a.dev = H.require_device(*a.operands)
         self.return_lse = return_softmax_lse
         self.lib = _lib.load()
-        self.args = None   # of the launch, but for the stream; None: nothing to do
+        self.args = None   # of the launch, but for the stream; None: no row or no key, each run clears the outputs
 
         def place():
-            nothing = not (a.batch and a.total_rows)
-            empty = nothing or not a.total_keys
+            empty = not (a.batch and a.total_rows and a.total_keys)
             self.out = H.empty_as(query)
-            if empty:
-                self.out.zero_()
             # statistics that nobody asked for are zeros: a small tensor is cleared by the lengths' launch
             total = 2 * a.n1 * a.total_rows
             few = not return_softmax_lse and not empty and total <= FEW_STATISTICS and total % 4 == 0
-            both = (torch.empty if (return_softmax_lse and not empty) or few else torch.zeros)(
+            both = (torch.empty if return_softmax_lse or empty or few else torch.zeros)(
                 (2,) + a.stat_shape, dtype=torch.float32, device=self.dev)
             self.sm_max, self.sm_sum = both.unbind(0)
-            if empty:   # no key: zeros, as for rows that see none
+            if empty:
+                self.cleared = (self.out, both)
+                H.settle(self.dev, _wait)
                 return
             size = self.lib.dsa_dense_attn_workspace_bytes(a.batch, a.total_rows, a.rows_behind, a.n1, a.n2, a.d, a.max_rows,
                                                            a.max_kv, int(kv_splits))
@@ -196,6 +195,9 @@ class DenseAttentionPlan:
     def run(self):
         if self.args is not None:
             H.on_device(self.dev, lambda: _lib.check(self.entry(*self.args, H.stream_ptr(self.dev)), "dsa_dense_attn"))
+        else:
+            for t in self.cleared:
+                t.zero_()
         return self.out, self.sm_max, self.sm_sum
 
 
@@ -236,15 +238,13 @@ class DenseAttentionGradPlan:
             raise ValueError("splits must lie between 0 and 64")
         self.dev = a.dev = H.require_device(*a.operands, d_out, out, softmax_max, softmax_sum)
         self.lib = _lib.load()
-        self.args = None   # of the launch, but for the stream; None: nothing to do
+        self.args = None   # of the launch, but for the stream; None: no row or no key, each run clears the gradients
 
         def place():
             empty = not (a.batch and a.total_rows and a.total_keys)
             self.grads = tuple(None if t is None else H.empty_as(t) for t in (query, key, value, query_rope, key_rope))
             if empty:
-                for t in self.grads:
-                    if t is not None:
-                        t.zero_()
+                H.settle(self.dev, _wait)
                 return
             size = self.lib.dsa_dense_attn_grad_workspace_bytes(a.batch, a.total_rows, a.total_keys, a.rows_behind,
                                                                 a.keys_behind, a.n1, a.n2, a.d, a.dr, a.max_rows, a.max_keys,
@@ -267,6 +267,10 @@ class DenseAttentionGradPlan:
     def run(self):
         if self.args is not None:
             H.on_device(self.dev, lambda: _lib.check(self.entry(*self.args, H.stream_ptr(self.dev)), "dsa_dense_attn_grad"))
+        else:
+            for t in self.grads:
+                if t is not None:
+                    t.zero_()
         return self.grads
 
 
