@@ -48,7 +48,7 @@ struct DenseK {
   // ranges of tokens
   int splits, chunk;
   float4* part;            // [splits][blocks][D / 8][64]: 32 head rows as the MFMAs leave them
-  float4* part_s;          // [splits][blocks][32]: reference maximum, true maximum, sum
+  float4* part_s;          // [splits][blocks][32]: reference maximum, true maximum, sum, NaN where a value is not finite
   int blocks;              // of 32 head rows, all key heads
 };
 
@@ -141,10 +141,11 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
 
   f32x16 o[RT][ON];
   float m_used[RT], m_true[RT], l_part[RT], alpha[RT];
+  float taint[RT];   // NaN: a value that this row sees was not finite
 #pragma unroll
   for (int m = 0; m < RT; ++m) {
     m_used[m] = m_true[m] = -INFINITY;
-    l_part[m] = 0.f;
+    l_part[m] = taint[m] = 0.f;
     alpha[m] = 1.f;
 #pragma unroll
     for (int c = 0; c < ON; ++c)
@@ -189,8 +190,8 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
       static_for<0, GPW>([&](auto j) __attribute__((always_inline)) { load_part(j, buf); });
     };
     // A tile that some rows see only in part: a masked token has P = 0, but 0 times a value that is not finite would
-    // still reach the rows that do not see it. Such values become 0 in LDS, and the token's score NaN for the
-    // rows that do see it.
+    // still reach the rows that do not see it. Such values become 0 in LDS, and the output of the rows that do see them
+    // NaN; the statistics are of the scores alone.
     auto is_mixed = [&](int u) { return t_lo + u * BN + BN > min_lim; };
     auto sanitize = [&](int u, int buf) __attribute__((always_inline)) {
       if (!is_mixed(u)) return;
@@ -300,11 +301,8 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
       const uint32_t bad = (uint32_t)(all >> (h * 32));
 #pragma unroll
       for (int m = 0; m < RT; ++m) {
-        if (__builtin_amdgcn_readfirstlane(bad))
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if ((bad >> s_token(i, kg)) & 1u) sv[m][i] = __builtin_nanf("");
         const int l = dead[m] ? INT_MAX : lim[m] - t0;
+        if (l > 0 && (bad & (0xFFFFFFFFu >> (l < 32 ? 32 - l : 0)))) taint[m] = __builtin_nanf("");
 #pragma unroll
         for (int i = 0; i < 16; ++i) sv[m][i] = s_token(i, kg) < l ? sv[m][i] : -INFINITY;
       }
@@ -462,7 +460,7 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
       const int blk = first_block(a, b, seq, n) + r_base / 32 + wave * RT + m;
       const int64_t at = (int64_t)sp * a.blocks + blk;
       if (lane < 32 && valid[m])
-        a.part_s[at * 32 + rr] = make_float4(m_used[m], top, dead[m] ? 0.f : l_tot, 0.f);
+        a.part_s[at * 32 + rr] = make_float4(m_used[m], top, dead[m] ? 0.f : l_tot, dead[m] ? 0.f : taint[m]);
       if (valid[m] && !dead[m]) {
         float4* dst = a.part + at * (D / 8) * 64 + lane;
 #pragma unroll
@@ -479,7 +477,7 @@ __global__ __launch_bounds__(NWV * 64) void dense_attn_kernel(DenseK a) {
       a.sm_max[at] = dead[m] ? 0.f : top;
       a.sm_sum[at] = dead[m] ? 0.f : l_tot * exp2f((m_used[m] - top) * LOG2E);
     }
-    const float inv = 1.f / l_tot;
+    const float inv = 1.f / l_tot + taint[m];
     uint16_t* dst = a.out + ((int64_t)(seq.r0 + s) * a.heads + n * a.per + g) * D + 8 * kg;
 #pragma unroll
     for (int c = 0; c < ON; ++c) {
@@ -541,7 +539,7 @@ __global__ __launch_bounds__(256) void dense_merge_kernel(DenseK a) {
     // (a range whose scores are all NaN has no maximum: its weight is its sum, or the NaN would be left out)
     const float w = st[j].z != st[j].z ? st[j].z : st[j].z != 0.f ? exp2f((st[j].x - M) * LOG2E) : 0.f;
     if (w != 0.f) sum += w * st[j].z;
-    s_w[k8 + 8 * j][rr] = w;
+    s_w[k8 + 8 * j][rr] = w + st[j].w;
   }
   s_sum[k8][rr] = sum;
   __syncthreads();

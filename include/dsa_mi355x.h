@@ -488,8 +488,8 @@ size_t dsa_dense_attn_workspace_bytes(int batch, int total_rows, int rows_behind
  *   score = (q . k + q_rope . k_rope) * scale, out = softmax(score) v, sm_max = max score,
  *   sm_sum = sum exp(score - sm_max)   (both or neither may be NULL)
  * Rows with s >= act_q[b], that see no token, or behind the last batch get out = 0, sm = 0. A row that sees a value that
- * is not finite gets NaN in that column at least, and may get NaN in all; a row that does not see it is not affected. Where
- * a score is NaN, sm_sum is NaN; sm_max need not be.
+ * is not finite gets one in that column at least, and may get NaN in all; a row that does not see it is not affected, nor
+ * are sm_max and sm_sum, which are of the scores alone. Where a score is NaN, sm_sum is NaN; sm_max need not be.
  *   query [total_rows, N1, D], query_rope [.., 64], key [total_keys, N2, D], key_rope [.., 64], value [total_keys, N2, D]:
  *   rows and heads by strides in elements (0 for heads that share one), multiples of 8, on 16-byte borders, row
  *   strides below 2^24; fp16 / bf16; D in {64, 128}, dr 0 or (D = 128) 64. total_rows * N1 and total_keys * N2 < 2^30.
