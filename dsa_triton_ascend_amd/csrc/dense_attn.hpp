@@ -199,6 +199,24 @@ __device__ __forceinline__ void mfma32_va_end2(f32x16& c0, uint4 a0, uint4 b0, f
     asm volatile("v_mfma_f32_32x32x16_f16 %0, %2, %4, %0\n\tv_mfma_f32_32x32x16_f16 %1, %3, %5, %1\n\ts_nop 15"
                  : "+v"(c0), "+v"(c1) : "v"(p0), "v"(p1), "a"(v0), "a"(v1));
 }
+// the same with operands that lie in VGPRs, where the AGPRs are full
+template <int IO>
+__device__ __forceinline__ void mfma32_vv(f32x16& c, uint4 a, uint4 b) {
+  const i32x4v av = __builtin_bit_cast(i32x4v, a), bv = __builtin_bit_cast(i32x4v, b);
+  if constexpr (IO == IO_BF16) asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(av), "v"(bv));
+  else asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(c) : "v"(av), "v"(bv));
+}
+template <int IO>
+__device__ __forceinline__ void mfma32_vv_va_end2(f32x16& c0, uint4 a0, uint4 b0, f32x16& c1, uint4 a1, uint4 b1) {
+  const i32x4v p0 = __builtin_bit_cast(i32x4v, a0), p1 = __builtin_bit_cast(i32x4v, a1);
+  const i32x4v v0 = __builtin_bit_cast(i32x4v, b0), v1 = __builtin_bit_cast(i32x4v, b1);
+  if constexpr (IO == IO_BF16)
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %2, %4, %0\n\tv_mfma_f32_32x32x16_bf16 %1, %3, %5, %1\n\ts_nop 15"
+                 : "+v"(c0), "+v"(c1) : "v"(p0), "v"(p1), "v"(v0), "a"(v1));
+  else
+    asm volatile("v_mfma_f32_32x32x16_f16 %0, %2, %4, %0\n\tv_mfma_f32_32x32x16_f16 %1, %3, %5, %1\n\ts_nop 15"
+                 : "+v"(c0), "+v"(c1) : "v"(p0), "v"(p1), "v"(v0), "a"(v1));
+}
 // v in AGPRs from here on
 __device__ __forceinline__ uint4 in_agprs(uint4 u) {
   i32x4v v = __builtin_bit_cast(i32x4v, u);

@@ -8,22 +8,22 @@
 // Three launches, without atomics, so results do not depend on timing:
 //  * rows: delta and the logarithm of the sum for every head row (fp16: also the norms that bound dS);
 //  * queries: 128 head rows, 32 a wave, Q and dO in registers, running over the tokens: S^T = K Q^T, dP^T = V dO^T,
-//    dQ^T += K^T dS^T; on its way it makes delta anew, without the rounding of O;
+//    dQ^T += K^T dS^T; on its way it makes delta anew, without the rounding of O, and sum P K, which corrects dQ for it;
 //  * keys: a work-group has 128 tokens of one key head, 32 a wave, K and V in registers, and runs over the head rows
 //    that see them (the group's heads are rows side by side): S = Q K^T and dP = dO V^T with the head rows as M, whose
 //    results are already the B operands of dV^T += dO^T P and dK^T += Q^T dS.
 // Few tokens or rows are cut into ranges over the other axis, whose sums a further launch adds.
 //
-// S and dP are computed in both, 7 products instead of 5; what that saves is the addition of dQ from many work-groups,
-// in 32 bits and an order of its own. P and dS are rounded to the io type for their products.
+// S and dP are computed in both, with sum P K 8 products instead of 5; what that saves is the addition of dQ from many
+// work-groups, in 32 bits and an order of its own. P and dS are rounded to the io type for their products.
 //
 // Bound by the issue of instructions beside the matrix ones: a wave holds two operands and up to 10 accumulators, so there is
 // one to a SIMD, and P and dS of one half tile are placed among the products of the half before it and the scores of
 // the one after (8192 tokens, 32 heads on 8 of 128, bf16: 3079 -> 2189 us). Loads whose addresses need no branch: 1954;
 // all work-groups of a key head at the same head rows at the same time, and dP that starts from -delta: 1836;
-// levels turned (pair_of) and twice the work-groups for the rows: 1770 (rows 29, queries 780, keys 960; 1080 TFLOP/s of
-// the 7 products). Two waves to 32 tokens, one for dV and one for dK, each
-// with the scores of both, were no faster (1954).
+// levels turned (pair_of) and twice the work-groups for the rows: 1770; with sum P K: 1900 (rows 29, queries 920, keys 950;
+// 1150 TFLOP/s of the 8 products). Two waves to 32 tokens, one for dV and one for dK, each with the scores of both, were no
+// faster than one for both (1954).
 #include <algorithm>
 
 #include "dense_attn.hpp"
@@ -67,6 +67,7 @@ struct GradK {
   int q_splits, q_chunk, q_blocks;   // ranges of tokens; blocks of 32 head rows
   float4* k_part;
   float4* q_part;
+  float* q_sum;            // [splits][blocks][32]: a range's sum of P dP
 };
 
 __device__ __forceinline__ int row_div(const GradK& a, int r) { return (int)(((uint64_t)(uint32_t)r * a.per_mul) >> (31 + a.per_shift)); }
@@ -633,13 +634,11 @@ template <int D, int DR> struct QueryLds {
   float red[2][NWV];
 };
 
-// delta = dO . O takes the rounded output, off by half a step of it: next to nothing beside dP where a row's weight
-// lies on many tokens, as much as the rounding of dS where it lies on few. The sum of P dP over the row's tokens is the
-// same number without that error, and comes along here for one operation an element: it goes to the keys' kernel, which
-// runs after this one. This kernel itself needs it beforehand: rows of up to SHORT tokens run over them once more first
-// (random queries and keys, bf16, 200 tokens: dQ's error against 64 bits 1.57 times that of rounding the exact one, 1.43 so).
-constexpr int SHORT = 256;
-
+// delta = dO . O takes the rounded output, off by half a step of it on every token of the row alike: that adds up along what
+// the keys have in common, and where dP and delta cancel it is all there is (keys and values with a common part as large as
+// the rest, bf16, 4100 tokens: dQ's error 38 times that of rounding the exact dS). The sum of P dP over the row's tokens is
+// the same number without that error, known at the end: sum P K comes along, and dQ gets its share of the difference. It
+// needs no fragment of its own, but a third product, D / 32 accumulators and a rounding of P.
 template <int IO, int D, int DR>
 __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
   constexpr int KSN = D / 16, KS = (D + DR) / 16, ON = D / 32, RN = DR / 32, RB = D * 2;
@@ -671,11 +670,12 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
   const int lim = valid ? min(limit_of(a.len, seq, s), t_hi) : 0;
   const bool dead = lim <= t_lo;
 
-  f32x16 dq[ON + RN];
+  f32x16 dq[ON + RN], pk[ON + RN];
 #pragma unroll
   for (int c = 0; c < ON + RN; ++c)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) dq[c][i] = 0.f;
+    for (int i = 0; i < 16; ++i) dq[c][i] = pk[c][i] = 0.f;
+  float sum = 0.f;   // of P dP
 
   if (ntiles > 0) {
     // (a zero scale becomes 1e-30: scores round to 0, and a masked one, of the sign that makes it so, to P = 0)
@@ -698,15 +698,12 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
       vs.aim(last);
       if constexpr (DR > 0) rs.aim(last);
     };
-    auto move = [&](int64_t tiles) __attribute__((always_inline)) {
-      ks.base = uniform(ks.base + tiles * (int64_t)BN * ks.row_bytes);
-      vs.base = uniform(vs.base + tiles * (int64_t)BN * vs.row_bytes);
-      if constexpr (DR > 0) rs.base = uniform(rs.base + tiles * (int64_t)BN * rs.row_bytes);
-    };
     // the streams to tile u, from the tile before it
     auto advance = [&](int u) __attribute__((always_inline)) {
       if (u >= ntiles) return;
-      move(1);
+      ks.base = uniform(ks.base + (int64_t)BN * ks.row_bytes);
+      vs.base = uniform(vs.base + (int64_t)BN * vs.row_bytes);
+      if constexpr (DR > 0) rs.base = uniform(rs.base + (int64_t)BN * rs.row_bytes);
       if (t_lo + (u + 1) * BN > seq.ak) aim(u);
     };
     auto load_tile = [&](int buf) __attribute__((always_inline)) {
@@ -722,10 +719,11 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
     };
     aim(0);
     load_tile(0);
+    constexpr int QA = KSN;   // of Q's fragments in AGPRs: the accumulators leave room for no more
     uint4 qf[KS], df[KSN];
     const int64_t stat = n * (int64_t)a.len.rows * a.per + (int64_t)seq.r0 * a.per + r;
     const float lse = a.lse[stat];
-    float delta = -a.delta[stat];
+    const float delta = -a.delta[stat];
     {
       const int64_t head = n * a.per + g;
       const uint16_t* qp = first_of(a.len, a.q, b, seq.r0) + s * a.q.row + head * a.q.head + kg * 8;
@@ -738,7 +736,7 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
         for (int j = KSN; j < KS; ++j) qf[j] = ldg16(rp + (j - KSN) * 16);
       }
 #pragma unroll
-      for (int j = 0; j < KS; ++j) qf[j] = in_agprs(qf[j]);
+      for (int j = 0; j < QA; ++j) qf[j] = in_agprs(qf[j]);
 #pragma unroll
       for (int j = 0; j < KSN; ++j) df[j] = in_agprs(df[j]);
     }
@@ -779,7 +777,8 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
       for (int j = 0; j < KS - 1; ++j) {
         const uint4 f = k_frag(j, h);
         if (j == 0) mfma32_va<IO, true>(sv, f, qf[j]);
-        else mfma32_va<IO, false>(sv, f, qf[j]);
+        else if (j < QA) mfma32_va<IO, false>(sv, f, qf[j]);
+        else mfma32_vv<IO>(sv, f, qf[j]);
       }
 #pragma unroll
       for (int j = 0; j < KSN - 1; ++j) {
@@ -787,7 +786,8 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
         if (j == 0) mfma32_va<IO, true>(dp, f, df[j]);
         else mfma32_va<IO, false>(dp, f, df[j]);
       }
-      mfma32_va_end2<IO>(sv, k_frag(KS - 1, h), qf[KS - 1], dp, v_frag(KSN - 1, h), df[KSN - 1]);
+      if constexpr (QA < KS) mfma32_vv_va_end2<IO>(sv, k_frag(KS - 1, h), qf[KS - 1], dp, v_frag(KSN - 1, h), df[KSN - 1]);
+      else mfma32_va_end2<IO>(sv, k_frag(KS - 1, h), qf[KS - 1], dp, v_frag(KSN - 1, h), df[KSN - 1]);
     };
     auto mask = [&](int u, int buf, int h, f32x16& sv, f32x16& dp) __attribute__((always_inline)) {
       if (!is_mixed(u)) return;
@@ -800,42 +800,10 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
         if (s_token(i, kg) >= l) sv[i] = masked, dp[i] = 0.f;
       }
     };
-    float sum = 0.f;   // of P dP
-    // (only where this range is all that every row of the work-group sees)
-    if (t_lo == 0 && limit_of(a.len, seq, min((r_end - 1) / a.per, seq.aq - 1)) <= min(SHORT, t_hi)) {
-      for (int u = 0; u < ntiles; ++u) {
-        if (u > 0) {
-          lds_barrier();   // every wave is done with the buffer
-          advance(u);
-          load_tile(0);
-        }
-        wait_vmcnt<0>();
-        asm volatile("" ::: "memory");
-        sanitize(u, 0);
-        lds_barrier();
-        point_op(0);
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          f32x16 sv, dp;
-          if (h == 0) scores(0, sv, dp);
-          else scores(1, sv, dp);
-          mask(u, 0, h, sv, dp);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sum = fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], sl2, -lse)), dp[i], sum);
-        }
-      }
-      delta = add_half_swap(sum) * (IO == IO_F16 ? 0x1p-15f : 1.f);
-      sum = 0.f;
-      lds_barrier();
-      move(1 - ntiles);
-      aim(0);
-      load_tile(0);   // (anew also where it is the only one: cleaned values are gone from it)
-    }
-
-    // ---- dS of 32 tokens in NST stages of two each, placed among the products before and after them
+    // ---- P and dS of 32 tokens in NST stages of two each, placed among the products before and after them
     constexpr int NST = 8;
     const float fs = factor.x * 0x1p-15f;   // (fp16's P has the factor 2^15)
-    auto stage = [&](int st, f32x16& sv, f32x16& dp, uint32_t (&wn)[8]) __attribute__((always_inline)) {
+    auto stage = [&](int st, f32x16& sv, f32x16& dp, uint32_t (&pn)[8], uint32_t (&wn)[8]) __attribute__((always_inline)) {
       const int i = 2 * st;
       const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], sl2, -lse));
       const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i + 1], sl2, -lse));
@@ -843,39 +811,44 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
       sum = fmaf(p1, dp[i + 1], sum);
       float x0 = p0 * (dp[i] - delta), x1 = p1 * (dp[i + 1] - delta);
       if constexpr (IO == IO_F16) x0 *= fs, x1 *= fs;
+      pn[st] = pack2<IO>(p0, p1);
       wn[st] = pack2<IO>(x0, x1);
-      asm volatile("" : "+v"(wn[st]), "+v"(sum));   // here, not where the next step needs it
+      asm volatile("" : "+v"(pn[st]), "+v"(wn[st]), "+v"(sum));   // here, not where the next step needs them
     };
 
     // ---- One step handles 32 tokens: the products of those before them, S and dP of those after them, each MFMA
-    // followed by a part of this one's dS. Fragments are read a few MFMAs ahead.
+    // followed by a part of this one's P and dS. Fragments are read a few MFMAs ahead.
     constexpr int LAG = KS - KSN, NS = KS + KSN;   // S and dP end together
-    constexpr int TR = 4, KR = 4, VR = 4;
+    constexpr int TR = 4, KR = D == 64 ? 2 : 4, VR = KR;   // (heads of 64: 254 registers, two work-groups on a CU)
     uint4 tf[TR], kf[KR], vf[VR];
-    auto step = [&](auto pvc, auto sc, auto hc, f32x16& cs, f32x16& cd, f32x16& ns, f32x16& nd, uint32_t (&wb)[8], uint32_t (&wn)[8],
-                    auto&& between, auto&& ride) __attribute__((always_inline)) {
+    auto step = [&](auto pvc, auto sc, auto hc, f32x16& cs, f32x16& cd, f32x16& ns, f32x16& nd, uint32_t (&pb)[8], uint32_t (&wb)[8],
+                    uint32_t (&pn)[8], uint32_t (&wn)[8], auto&& between, auto&& ride) __attribute__((always_inline)) {
       constexpr bool PV = decltype(pvc)::value, S = decltype(sc)::value;
       constexpr int H = decltype(hc)::value;
-      constexpr int M0 = PV ? NP : 0, NMM = M0 + (S ? NS : 0), LEAD = NMM > 8 ? 2 : 0;
+      constexpr int M0 = PV ? 2 * NP : 0, NMM = M0 + (S ? NS : 0), LEAD = NMM > 8 ? 2 : 0;
       auto values_at = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
         for (int st = 0; st < NST; ++st)
-          if (LEAD + st * (NMM - LEAD) / NST == slot) stage(st, cs, cd, wn);
+          if (LEAD + st * (NMM - LEAD) / NST == slot) stage(st, cs, cd, pn, wn);
       };
       if constexpr (PV)
-        static_for<0, NP>([&](auto ic) __attribute__((always_inline)) {
-          constexpr int i = decltype(ic)::value, st = i / NC, c = i % NC;
-          dq[c] = Mfma<IO>::m32(tf[i % TR], make_uint4(wb[4 * st], wb[4 * st + 1], wb[4 * st + 2], wb[4 * st + 3]), dq[c]);
-          if constexpr (i + TR < NP) tf[i % TR] = t_frag(i + TR, H);
+        static_for<0, 2 * NP>([&](auto ic) __attribute__((always_inline)) {
+          constexpr int i = decltype(ic)::value / 2, st = i / NC, c = i % NC;
+          if constexpr (decltype(ic)::value % 2 == 0) {
+            dq[c] = Mfma<IO>::m32(tf[i % TR], make_uint4(wb[4 * st], wb[4 * st + 1], wb[4 * st + 2], wb[4 * st + 3]), dq[c]);
+          } else {
+            pk[c] = Mfma<IO>::m32(tf[i % TR], make_uint4(pb[4 * st], pb[4 * st + 1], pb[4 * st + 2], pb[4 * st + 3]), pk[c]);
+            if constexpr (i + TR < NP) tf[i % TR] = t_frag(i + TR, H);
+          }
           if constexpr (S)
             static_for<0, KR + VR>([&](auto gc) __attribute__((always_inline)) {
               constexpr int g = decltype(gc)::value;
-              if constexpr (g * NP / (KR + VR) == i) {
+              if constexpr (g * 2 * NP / (KR + VR) == decltype(ic)::value) {
                 if constexpr (g < KR) kf[g] = k_frag(g, H);
                 else vf[g - KR] = v_frag(g - KR, H);
               }
             });
-          values_at(i);
+          values_at(decltype(ic)::value);
           __builtin_amdgcn_sched_barrier(0);
         });
       between();
@@ -884,9 +857,11 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
           constexpr int j = decltype(jc)::value;
           constexpr bool is_s = j < LAG || (j - LAG) % 2 == 0;
           constexpr int i = j < LAG ? j : is_s ? LAG + (j - LAG) / 2 : (j - LAG) / 2;   // step of its chain
-          if constexpr (j == NS - 1) mfma32_va_end2<IO>(ns, kf[(KS - 1) % KR], qf[KS - 1], nd, vf[(KSN - 1) % VR], df[KSN - 1]);
+          if constexpr (j == NS - 1 && QA < KS) mfma32_vv_va_end2<IO>(ns, kf[(KS - 1) % KR], qf[KS - 1], nd, vf[(KSN - 1) % VR], df[KSN - 1]);
+          else if constexpr (j == NS - 1) mfma32_va_end2<IO>(ns, kf[(KS - 1) % KR], qf[KS - 1], nd, vf[(KSN - 1) % VR], df[KSN - 1]);
           else if constexpr (is_s && i < KS - 1) {
-            mfma32_va<IO, i == 0>(ns, kf[i % KR], qf[i]);
+            if constexpr (i < QA) mfma32_va<IO, i == 0>(ns, kf[i % KR], qf[i]);
+            else mfma32_vv<IO>(ns, kf[i % KR], qf[i]);
             if constexpr (i + KR < KS) kf[i % KR] = k_frag(i + KR, H);
           } else if constexpr (!is_s) {
             mfma32_va<IO, i == 0>(nd, vf[i % VR], df[i]);
@@ -911,7 +886,7 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
     advance(1);
     load_tile(1);
     f32x16 s0, s1, d0, d1;
-    uint32_t w0[8], w1[8];
+    uint32_t p0[8], p1[8], w0[8], w1[8];
     point_op(0);
     scores(0, s0, d0);
 #pragma unroll
@@ -924,7 +899,7 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
       const int nb = buf == NBUF - 1 ? 0 : buf + 1, lb = buf == 0 ? NBUF - 1 : buf - 1;   // of tiles u + 1 and u - 1 (u + 2)
       mask(u, buf, 0, s0, d0);
       advance(u + 2);
-      step(pvc, yes, h1, s0, d0, s1, d1, w1, w0,
+      step(pvc, yes, h1, s0, d0, s1, d1, p1, w1, p0, w0,
            [&]() __attribute__((always_inline)) {
              wait_vmcnt<0>();
              asm volatile("" ::: "memory");
@@ -945,36 +920,49 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
       const int nb = buf == NBUF - 1 ? 0 : buf + 1;
       point_op(nb);
       mask(u, buf, 1, s1, d1);
-      step(yes, yes, h0, s1, d1, s0, d0, w0, w1, nothing, nothing);
+      step(yes, yes, h0, s1, d1, s0, d0, p0, w0, p1, w1, nothing, nothing);
       buf = nb;
       half0(yes, u + 1);
     }
     mask(ntiles - 1, buf, 1, s1, d1);
-    step(yes, no, h0, s1, d1, s0, d0, w0, w1, nothing, nothing);
+    step(yes, no, h0, s1, d1, s0, d0, p0, w0, p1, w1, nothing, nothing);
 #pragma unroll
     for (int i = 0; i < TR; ++i) tf[i] = t_frag(i, 1);
     static_for<0, NP>([&](auto ic) __attribute__((always_inline)) {
       constexpr int i = decltype(ic)::value, st = i / NC, c = i % NC;
       dq[c] = Mfma<IO>::m32(tf[i % TR], make_uint4(w1[4 * st], w1[4 * st + 1], w1[4 * st + 2], w1[4 * st + 3]), dq[c]);
+      pk[c] = Mfma<IO>::m32(tf[i % TR], make_uint4(p1[4 * st], p1[4 * st + 1], p1[4 * st + 2], p1[4 * st + 3]), pk[c]);
       if constexpr (i + TR < NP) tf[i % TR] = t_frag(i + TR, 1);
     });
     wait_vmcnt<0>();   // the last (unused) loads land before the LDS is released
     sum = add_half_swap(sum) * (IO == IO_F16 ? 0x1p-15f : 1.f);
-    // (all that the row sees lies in this range: others keep dO . O)
-    if (lane < 32 && valid && !dead && t_lo == 0 && (at.sp == a.q_splits - 1 || limit_of(a.len, seq, s) <= t_hi)) a.delta[stat] = -sum;
+    if (a.q_splits == 1) {
+      if (lane < 32 && valid && !dead) a.delta[stat] = -sum;
+      const float more = (delta - sum) * (IO == IO_F16 ? fs : 1.f);
+#pragma unroll
+      for (int c = 0; c < ON + RN; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dq[c][i] = fmaf(more, pk[c][i], dq[c][i]);
+    }
   }
 
   const float f = a.scale * factor.y;
   if (a.q_splits > 1) {
     if (w_base >= r_end) return;
     const int blk = n * (a.q_blocks / a.key_heads) + (int)((int64_t)seq.r0 * a.per / 32) + b + w_base / 32;
-    float4* dst = a.q_part + ((int64_t)at.sp * a.q_blocks + blk) * ((D + DR) / 8) * 64 + lane;
+    // both sums and that of P dP: the join knows all of it
+    if (lane < 32) a.q_sum[((int64_t)at.sp * a.q_blocks + blk) * 32 + rr] = dead ? 0.f : sum;
+    float4* dst = a.q_part + ((int64_t)at.sp * a.q_blocks + blk) * (2 * (D + DR) / 8) * 64 + lane;
+    const float fp = a.scale * (IO == IO_F16 ? 0x1p-15f : 1.f);
 #pragma unroll
-    for (int c = 0; c < ON + RN; ++c)
+    for (int c = 0; c < 2 * (ON + RN); ++c) {
+      const f32x16& v = c < ON + RN ? dq[c < ON + RN ? c : 0] : pk[c >= ON + RN ? c - ON - RN : 0];
+      const float x = c < ON + RN ? f : fp;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         dst[(c * 4 + e) * 64] = dead ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                     : make_float4(dq[c][4 * e] * f, dq[c][4 * e + 1] * f, dq[c][4 * e + 2] * f, dq[c][4 * e + 3] * f);
+                                     : make_float4(v[4 * e] * x, v[4 * e + 1] * x, v[4 * e + 2] * x, v[4 * e + 3] * x);
+    }
     return;
   }
   const int64_t head_row = (int64_t)(seq.r0 + s) * a.heads + n * a.per + g;
@@ -994,7 +982,8 @@ __global__ __launch_bounds__(NWV * 64) void dense_queries_kernel(GradK a) {
 
 // ---------------------------------------------------------------- joins
 // Adds the ranges' blocks of 32 rows (tokens or head rows), in order. The columns are those of one, two or three
-// outputs side by side: D + DR (+ D).
+// outputs side by side: D + DR (+ D); the queries' blocks have those of sum P K behind them, whose share goes by the sum of
+// P dP over all ranges, which is left for the keys' kernel.
 template <int IO, int D, int DR, bool KEYS>
 __global__ __launch_bounds__(256) void dense_join_kernel(GradK a) {
   constexpr int W8 = ((KEYS ? 2 * D : D) + DR) / 8;
@@ -1019,16 +1008,36 @@ __global__ __launch_bounds__(256) void dense_join_kernel(GradK a) {
     const int s = row / a.per;
     out_row = (int64_t)(seq.r0 + s) * a.heads + n * a.per + (row - s * a.per);
   }
-  for (int grp = wave; grp < W8; grp += 4) {
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float4* p = (KEYS ? a.k_part : a.q_part) + ((int64_t)blockIdx.x * W8 + grp) * 64 + lane;
+  constexpr int ALL8 = KEYS ? W8 : 2 * W8;
+  float more = 0.f;
+  if constexpr (!KEYS) {
+    const int64_t stat = n * (int64_t)a.len.rows * a.per + (int64_t)seq.r0 * a.per + min(row, count - 1);
+    const float delta = -a.delta[stat];
+    float sum = 0.f;
 #pragma unroll 4
-    for (int k = 0; k < splits; ++k) {
-      const uint4 v = ldg16(p + (int64_t)k * blocks * W8 * 64);
-      acc.x += __uint_as_float(v.x);
-      acc.y += __uint_as_float(v.y);
-      acc.z += __uint_as_float(v.z);
-      acc.w += __uint_as_float(v.w);
+    for (int k = 0; k < splits; ++k) sum += a.q_sum[((int64_t)k * blocks + blockIdx.x) * 32 + rr];
+    more = delta - sum;
+    __syncthreads();   // every wave has read it
+    if (threadIdx.x < 32 && row < count) a.delta[stat] = -sum;
+  }
+  for (int grp = wave; grp < W8; grp += 4) {
+    auto total = [&](int g) {
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4* p = (KEYS ? a.k_part : a.q_part) + ((int64_t)blockIdx.x * ALL8 + g) * 64 + lane;
+#pragma unroll 4
+      for (int k = 0; k < splits; ++k) {
+        const uint4 v = ldg16(p + (int64_t)k * blocks * ALL8 * 64);
+        acc.x += __uint_as_float(v.x);
+        acc.y += __uint_as_float(v.y);
+        acc.z += __uint_as_float(v.z);
+        acc.w += __uint_as_float(v.w);
+      }
+      return acc;
+    };
+    float4 acc = total(grp);
+    if constexpr (!KEYS) {
+      const float4 pk = total(W8 + grp);
+      acc.x = fmaf(more, pk.x, acc.x), acc.y = fmaf(more, pk.y, acc.y), acc.z = fmaf(more, pk.z, acc.z), acc.w = fmaf(more, pk.w, acc.w);
     }
     if (row >= count) continue;
     const int c = grp * 8;
@@ -1071,7 +1080,7 @@ Part make_part(int64_t total, int64_t longest, int batch, bool behind, int heads
 }
 struct Cut {
   Part keys, queries;
-  size_t stats, norms, k_part, q_part, bytes;
+  size_t stats, norms, k_part, q_part, q_sum, bytes;
 };
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 Cut make_cut(const DenseGradArgs& g) {
@@ -1083,8 +1092,11 @@ Cut make_cut(const DenseGradArgs& g) {
   c.stats = align256((size_t)a.total_rows * a.n1 * sizeof(float));
   c.norms = 2 * PREP * sizeof(float);
   if (c.keys.splits > 1) c.k_part = (size_t)c.keys.splits * c.keys.blocks * (size_t)((2 * a.d + a.dr) / w) * 64 * sizeof(float4);
-  if (c.queries.splits > 1) c.q_part = (size_t)c.queries.splits * c.queries.blocks * (size_t)((a.d + a.dr) / w) * 64 * sizeof(float4);
-  c.bytes = 2 * c.stats + c.norms + c.k_part + c.q_part;
+  if (c.queries.splits > 1) {
+    c.q_part = (size_t)c.queries.splits * c.queries.blocks * (size_t)(2 * (a.d + a.dr) / w) * 64 * sizeof(float4);
+    c.q_sum = align256((size_t)c.queries.splits * c.queries.blocks * 32 * sizeof(float));
+  }
+  c.bytes = 2 * c.stats + c.norms + c.k_part + c.q_part + c.q_sum;
   return c;
 }
 
@@ -1143,6 +1155,7 @@ hipError_t launch_dense_grad(const DenseGradArgs& g, size_t* lacking, hipStream_
   k.norms = (float*)(ws + 2 * c.stats);
   k.k_part = (float4*)(ws + 2 * c.stats + c.norms);
   k.q_part = (float4*)(ws + 2 * c.stats + c.norms + c.k_part);
+  k.q_sum = (float*)(ws + 2 * c.stats + c.norms + c.k_part + c.q_part);
   k.dq = (uint16_t*)g.dq, k.dqr = (uint16_t*)g.dqr, k.dk = (uint16_t*)g.dk, k.dkr = (uint16_t*)g.dkr, k.dv = (uint16_t*)g.dv;
   k.k_splits = c.keys.splits, k.k_chunk = c.keys.chunk, k.k_blocks = c.keys.blocks;
   k.q_splits = c.queries.splits, k.q_chunk = c.queries.chunk, k.q_blocks = c.queries.blocks;

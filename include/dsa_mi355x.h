@@ -526,7 +526,7 @@ int dsa_dense_attn_batched(const void* query, int64_t q_row, int64_t q_head, con
                            size_t workspace_bytes, int kv_splits, const int64_t* batch_strides, void* stream);
 
 /*
- * Gradients of dsa_dense_attn: with P = exp(score - sm_max) / sm_sum, dP = d_out . v, dS = P (dP - d_out . out),
+ * Gradients of dsa_dense_attn: with P = exp(score - sm_max) / sm_sum, dP = d_out . v, dS = P (dP - sum P dP),
  *   d_query = scale dS (key | key_rope), d_key = scale dS^T (query | query_rope), d_value = P^T d_out,
  * those of a key head summed over its query heads. query .. value, lengths, bounds and statistics as in the forward, whose
  * out, sm_max and sm_sum are given (out and d_out [total_rows, N1, D] by strides as the operands); outputs
