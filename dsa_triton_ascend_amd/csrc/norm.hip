@@ -4,8 +4,9 @@
 // and with g = d w (d the gradient of y):
 //   dx = (g - sum g / n - h sum(g h) / n) rstd,   dw = sum over rows of d h,   db = sum over rows of d
 //
-// Bound by memory: a row is read once into registers, and all its sums are made there (the variance from
-// the centered values, so a large mean costs no bits). Statistics and sums are 32-bit, each output is
+// Bound by memory: a row is read once into registers, and all its sums are made there: the mean, then sum and squares of
+// what is left without it. That sum is the rounding of the mean, which a row far from zero would keep in each of its values
+// (a constant row of 10^4 in fp32 gave outputs up to 0.6 where they are 0), and corrects mean and variance. Statistics and sums are 32-bit, each output is
 // rounded once. A row has TR threads: up to a wave's 64 (a power of two) they sum by VALU lane exchanges, a work-group
 // then taking several rows at a time; wider rows add through LDS. The next row is loaded before this one's sums, which
 // wait for each other. 16383 rows of 4096 in bf16: forward 44 us (6.1 TB/s; 48 right before the gradient), gradient 83
@@ -124,14 +125,21 @@ struct Columns {
   __device__ __forceinline__ int skip(int i) const { return max(0, of(i) - at(i)); }   // not added; V or more: no unit
 };
 
+// x as it is rounded: the compiler would otherwise take a product into the sums that use it in some of a row's units and
+// not in others, which then differ by the product's rounding, columns that two units hold too
+__device__ __forceinline__ float rounded(float x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // UPT units of V elements a thread; T threads a work-group at most
 template <int IO, int V, int UPT, int T>
 __global__ __launch_bounds__(T) void layer_norm_kernel(NormK a) {
   using E = typename Elem<IO>::T;
-  __shared__ float red[2][16][1];
+  __shared__ float red[2][16][1], red2[2][16][2];
   const int slots = (int)blockDim.x / a.tr, slot = (int)threadIdx.x / a.tr;
   const Columns<V> col{(int)threadIdx.x - slot * a.tr, a.tr, a.width};
-  int turn = 0;
+  int turn = 0, turn2 = 0;
   float w[UPT][V], b[UPT][V];
 #pragma unroll
   for (int i = 0; i < UPT; ++i) {
@@ -165,23 +173,29 @@ __global__ __launch_bounds__(T) void layer_norm_kernel(NormK a) {
       }
     }
     row_sums<1>(s, a.tr, red, turn);
-    const float mean = s[0] * a.inv_n;
-    s[0] = 0.f;
+    const float first = rounded(s[0] * a.inv_n);
+    float q[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
       const int skip = col.skip(i);
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[i][e] -= mean;
+      for (int e = 0; e < V; ++e) v[i][e] -= first;
       if (skip == 0) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) s[0] = fmaf(v[i][e], v[i][e], s[0]);
+        for (int e = 0; e < V; ++e) q[0] += v[i][e], q[1] = fmaf(v[i][e], v[i][e], q[1]);
       } else {
 #pragma unroll
-        for (int e = 0; e < V; ++e) s[0] += e >= skip ? v[i][e] * v[i][e] : 0.f;
+        for (int e = 0; e < V; ++e) {
+          q[0] += e >= skip ? v[i][e] : 0.f;
+          q[1] += e >= skip ? v[i][e] * v[i][e] : 0.f;
+        }
       }
     }
-    row_sums<1>(s, a.tr, red, turn);
-    const float rstd = 1.f / sqrtf(s[0] * a.inv_n + a.eps);
+    row_sums<2>(q, a.tr, red2, turn2);
+    const float off = rounded(q[0] * a.inv_n), mean = first + off;
+    float var = fmaf(-off, off, q[1] * a.inv_n);
+    var = var < 0.f ? 0.f : var;   // (NaN stays)
+    const float rstd = 1.f / sqrtf(var + a.eps);
     if (r >= a.rows) continue;   // (the slots' trips through the barriers are the same: base is the work-group's)
     if (col.t == 0 && a.mean) {
       a.mean[r] = mean;
@@ -192,7 +206,7 @@ __global__ __launch_bounds__(T) void layer_norm_kernel(NormK a) {
     for (int i = 0; i < UPT; ++i) {
       if (col.of(i) >= a.width) continue;
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[i][e] = fmaf(v[i][e] * rstd, w[i][e], b[i][e]);
+      for (int e = 0; e < V; ++e) v[i][e] = fmaf((v[i][e] - off) * rstd, w[i][e], b[i][e]);
       store_any<IO, V>(y + col.at(i), v[i]);
     }
   }
@@ -272,7 +286,7 @@ __global__ __launch_bounds__(T) void layer_norm_grad_kernel(NormK a) {
     }
     row_sums<2>(s, a.tr, red, turn);
     if (!ok) continue;
-    const float c0 = s[0] * a.inv_n, c1 = s[1] * a.inv_n;
+    const float c0 = rounded(s[0] * a.inv_n), c1 = rounded(s[1] * a.inv_n);
     E* dx = reinterpret_cast<E*>(a.y) + r * a.width;
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
