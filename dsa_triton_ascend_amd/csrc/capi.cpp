@@ -840,6 +840,8 @@ int dsa_dense_attn_batched(const void* query, int64_t q_row, int64_t q_head, con
   if (lacking > 0)
     return fail(DSA_ERR_INVALID, "dsa_dense_attn: a 16-byte aligned workspace of %zu bytes required, %zu given", lacking,
                 workspace ? workspace_bytes : (size_t)0);
+  if (e == hipErrorInvalidConfiguration)
+    return fail(DSA_ERR_UNSUPPORTED, "dsa_dense_attn: 2^32 threads in a launch (sequences times key heads, times kv_splits)");
   return hip_status(e, "dsa_dense_attn launch");
 }
 
@@ -912,6 +914,8 @@ int dsa_dense_attn_grad_batched(const void* query, int64_t q_row, int64_t q_head
   if (lacking > 0)
     return fail(DSA_ERR_INVALID, "%s: a 16-byte aligned workspace of %zu bytes required, %zu given", fn, lacking,
                 workspace ? workspace_bytes : (size_t)0);
+  if (e == hipErrorInvalidConfiguration)
+    return fail(DSA_ERR_UNSUPPORTED, "dsa_dense_attn_grad: 2^32 threads in a launch (sequences times key heads, times splits)");
   return hip_status(e, "dsa_dense_attn_grad launch");
 }
 

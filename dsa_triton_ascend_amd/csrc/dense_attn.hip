@@ -616,10 +616,6 @@ Cut make_cut(const DenseArgs& a) {
   c.rt = flat ? (items256 >= 160 ? 2 : 1) : (a.d == 128 && items256 > 256 ? 2 : 1);
   const int rows = 128 * c.rt;
   const int64_t even = std::max<int64_t>(1, tiles(rows)) * seqs, through = (int64_t)a.total_rows * per / rows + seqs;
-  // All sequences get the longest's tiles, by levels, the last, which see most, first. Numbered through, that order is
-  // lost: 43 sequences, the longest 512, 3.3 times as many even items: 32 and 38 us; 9, the longest 4096, 5.5 times: 161 and 152.
-  const bool compact = even > 4 * through;
-  const int64_t items = (compact ? through : even) * a.n2;
   const int64_t real = std::min(even, (int64_t)a.total_rows * per / rows + a.batch) * a.n2;   // about so many have rows
   // Fewer items than CUs: ranges of tokens that make one round of them, of two tiles at least (a work-group's LDS fills its
   // CU; four single tokens, 4 key heads, 8190 keys: 8, 16, 32 ranges take 29.9, 22.9, 27.8 us with their join), from
@@ -632,8 +628,11 @@ Cut make_cut(const DenseArgs& a) {
   splits = std::min(splits, MAX_SPLITS);
   c.chunk = (int)div_up(std::max<int64_t>(div_up(a.max_kv, splits), 1), BN) * BN;
   c.splits = (int)std::max<int64_t>(1, div_up(a.max_kv, c.chunk));
+  // All sequences get the longest's tiles, by levels, the last, which see most, first. Numbered through, that order is
+  // lost: 43 sequences, the longest 512, 3.3 times as many even items: 32 and 38 us; 9, the longest 4096, 5.5 times: 161 and 152.
+  const bool compact = even > 4 * through || even * a.n2 * c.splits * 2 * rows >= MAX_THREADS;
   c.even = compact ? 0 : (int)std::max<int64_t>(1, tiles(rows));
-  c.groups = items * c.splits;
+  c.groups = (compact ? through : even) * a.n2 * c.splits;
   c.blocks = (int)(((int64_t)a.total_rows * per / 32 + seqs + 1) * a.n2);
   return c;
 }
@@ -670,7 +669,8 @@ hipError_t launch_dense_attn(const DenseArgs& a, size_t* lacking, hipStream_t s)
   const size_t need = workspace_bytes(c, a.d);
   *lacking = need > 0 && (!a.ws || a.ws_bytes < need || ((uintptr_t)a.ws & 15) != 0) ? need : 0;
   if (*lacking) return hipSuccess;
-  if (c.groups >= (1 << 24) || (c.splits > 1 && (int64_t)c.blocks * (a.d / 32) >= (1 << 24))) return hipErrorInvalidConfiguration;   // 2^32 threads
+  if (c.groups * (c.rt == 2 && a.dr == 0 ? 512 : 256) >= MAX_THREADS || (c.splits > 1 && (int64_t)c.blocks * (a.d / 32) * 256 >= MAX_THREADS))
+    return hipErrorInvalidConfiguration;
   DenseK k{};
   auto rows = [](const DenseTensor& t) { return Rows{(const uint16_t*)t.p, t.row, t.head, t.batch}; };
   k.q = rows(a.q), k.qr = rows(a.qr), k.k = rows(a.k), k.kr = rows(a.kr), k.v = rows(a.v);

@@ -292,6 +292,9 @@ __device__ __forceinline__ void pack_tile(const f32x16& v, float f, uint4 (&out)
   out[1] = make_uint4(d[2][0], d[2][1], d[3][0], d[3][1]);
 }
 
+// A launch has fewer than 2^32 threads
+constexpr int64_t MAX_THREADS = 1ll << 32;
+
 // Work-groups of a launch: tiles of rows of every sequence and key head. Even numbering, levels of one tile of
 // each (the last, which see most, first); or numbered through, where sequences are much shorter than the longest:
 // those of sequence b begin at start(b) * per / tile + b, which leaves each enough.

@@ -1065,13 +1065,13 @@ Part make_part(int64_t total, int64_t longest, int batch, bool behind, int heads
   const int64_t seqs = batch + (behind ? 1 : 0);
   const int64_t tiles = std::max<int64_t>(1, div_up(longest, TOK));
   const int64_t even = tiles * seqs, through = total / TOK + seqs;
-  const bool compact = 2 * even > 3 * through;
   const int64_t real = (total / TOK + batch) * heads;
   int64_t splits = forced;
   if (splits <= 0) splits = real >= 256 ? 1 : std::max<int64_t>(1, std::min(512 / real, std::max(other / 512, std::min<int64_t>(4, other / 128))));
   splits = std::min<int64_t>(splits, 64);
   p.chunk = (int)(div_up(std::max<int64_t>(div_up(other, splits), 1), BN) * BN);
   p.splits = (int)std::max<int64_t>(1, div_up(other, p.chunk));
+  const bool compact = 2 * even > 3 * through || even * heads * p.splits * NWV * 64 >= MAX_THREADS;
   p.even = compact ? 0 : (int)tiles;
   p.seqs = (int)seqs;
   p.groups = (compact ? through : even) * heads * p.splits;
@@ -1130,7 +1130,8 @@ hipError_t launch_dense_grad(const DenseGradArgs& g, size_t* lacking, hipStream_
   const Cut c = make_cut(g);
   *lacking = !a.ws || a.ws_bytes < c.bytes || ((uintptr_t)a.ws & 15) != 0 ? c.bytes : 0;
   if (*lacking) return hipSuccess;
-  if (c.keys.groups >= (1 << 24) || c.queries.groups >= (1 << 24)) return hipErrorInvalidConfiguration;   // 2^32 threads
+  for (const Part* p : {&c.keys, &c.queries})
+    if (p->groups * NWV * 64 >= MAX_THREADS || (p->splits > 1 && (int64_t)p->blocks * 256 >= MAX_THREADS)) return hipErrorInvalidConfiguration;
   GradK k{};
   auto rows = [](const DenseTensor& t) { return Rows{(const uint16_t*)t.p, t.row, t.head, t.batch}; };
   k.q = rows(a.q), k.qr = rows(a.qr), k.k = rows(a.k), k.kr = rows(a.kr), k.v = rows(a.v), k.d = rows(g.d_out), k.o = rows(g.out);

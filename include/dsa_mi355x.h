@@ -492,7 +492,9 @@ size_t dsa_dense_attn_workspace_bytes(int batch, int total_rows, int rows_behind
  * are sm_max and sm_sum, which are of the scores alone. Where a score is NaN, sm_sum is NaN; sm_max need not be.
  *   query [total_rows, N1, D], query_rope [.., 64], key [total_keys, N2, D], key_rope [.., 64], value [total_keys, N2, D]:
  *   rows and heads by strides in elements (0 for heads that share one), multiples of 8, on 16-byte borders, row
- *   strides below 2^24; fp16 / bf16; D in {64, 128}, dr 0 or (D = 128) 64. total_rows * N1 and total_keys * N2 < 2^30.
+ *   strides below 2^24; fp16 / bf16; D in {64, 128}, dr 0 or (D = 128) 64. total_rows * N1 and total_keys * N2 < 2^30,.
+ *   A launch has fewer than 2^32 threads, else DSA_ERR_UNSUPPORTED: total_rows * N1 / 128 + (batch + 1) * N2, times the ranges of
+ *   tokens, < 2^23 is enough, with several ranges also total_rows * N1 < 2^26.
  *   out [total_rows, N1, D] contiguous; sm_max, sm_sum fp32 [batch, N2, total_rows / batch, N1 / N2] (stat_padded:
  *   row_start[b] = b * total_rows / batch) or [N2, total_rows, N1 / N2].
  *   row_start, key_start [batch + 1] ascending from 0, act_q, act_k [batch], on the device. rows_behind: total_rows -
@@ -534,7 +536,8 @@ int dsa_dense_attn_batched(const void* query, int64_t q_row, int64_t q_head, con
  * [total_keys, N2, 64] (heads that share a rotary key get one gradient each). Rows and keys that take no part get zeros.
  * Values that are not finite reach the gradients of what sees them only.
  *   keys_behind: total_keys - key_start[batch]; max_keys: the most of key_start[b + 1] - key_start[b] and keys_behind.
- *   splits (<= 64): 0, or the ranges that each key's rows and each row's keys are cut into. Sums have a fixed order.
+ *   splits (<= 64): 0, or the ranges that each key's rows and each row's keys are cut into. Sums have a fixed order. Work-groups
+ *   as in the forward, those of keys (total_keys * N2 / 128 + (batch + 1) * N2) too.
  *   fp16: dS gets a factor, a power of two from the largest norms of d_out's and value's rows, so that neither its small
  *   values nor its large ones leave the type's range.
  *   workspace: dsa_dense_attn_grad_workspace_bytes, 16-byte aligned, needs no initialisation. Calls that share one must be
