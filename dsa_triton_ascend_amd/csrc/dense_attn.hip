@@ -608,12 +608,16 @@ Cut make_cut(const DenseArgs& a) {
   Cut c{};
   auto tiles = [&](int rows) { return div_up((int64_t)a.max_rows * per, rows); };
   // Work-groups of 256 rows read each tile half as often as those of 128, which balance better. With all items about as
-  // long (no mask, or a chunk after many tokens; bf16, us of 256 and of 128 rows): 188 items 200 and 262, 256 items of
-  // heads of 64 83 and 88. Below a diagonal, where the longest has twice the mean: 256 items 199 and 167, 320 items 75
-  // and 83, 1024 items 504 and 631 (rotary 637 and 753); heads of 64, several of whose work-groups a CU holds, 344 and 335.
+  // long (no mask, or a chunk after many tokens; 16 heads, bf16, us of 256 and of 128 rows): those of 128 as long as they are one
+  // round of the CUs (128 items: one sequence 54 and 43, 16 sequences 10.2 and 9.3; rotary, 100 items, 56 and 37), those of 256
+  // from there on (129 items: 57 and 82, 12.6 and 18.7; 155: 66 and 96, rotary 85 and 109; 260: 220 and 225, 33 and 39; 1030:
+  // 2339 and 2641, 197 and 236). Heads of 64, several of whose work-groups a CU holds: 128 items 42 and 36, 129 43 and 45,
+  // 200 62 and 64, 240 76 and 81, 260 157 and 136, 1030 1552 and 1443; a chunk after twice as many tokens, 200 items 175 and
+  // 153, 1030 items 10,987 and 10,191 (after six times as many). Below a diagonal, where the longest has twice the mean: 256
+  // items 199 and 167, 320 items 75 and 83, 1024 items 504 and 631 (rotary 637 and 753); heads of 64 344 and 335.
   const bool flat = a.sparse_mode == 0 || a.max_kv >= 2 * (int64_t)a.max_rows;
   const int64_t items256 = (int64_t)a.total_rows * per * a.n2 / 256;
-  c.rt = flat ? (items256 >= 160 ? 2 : 1) : (a.d == 128 && items256 > 256 ? 2 : 1);
+  c.rt = a.d == 128 ? (items256 > (flat ? 128 : 256) ? 2 : 1) : (a.sparse_mode == 0 && items256 > 128 && items256 <= 256 ? 2 : 1);
   const int rows = 128 * c.rt;
   const int64_t even = std::max<int64_t>(1, tiles(rows)) * seqs, through = (int64_t)a.total_rows * per / rows + seqs;
   const int64_t real = std::min(even, (int64_t)a.total_rows * per / rows + a.batch) * a.n2;   // about so many have rows
