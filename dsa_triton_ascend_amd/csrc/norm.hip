@@ -4,9 +4,10 @@
 // and with g = d w (d the gradient of y):
 //   dx = (g - sum g / n - h sum(g h) / n) rstd,   dw = sum over rows of d h,   db = sum over rows of d
 //
-// Bound by memory: a row is read once into registers, and all its sums are made there: the mean, then sum and squares of
-// what is left without it. That sum is the rounding of the mean, which a row far from zero would keep in each of its values
-// (a constant row of 10^4 in fp32 gave outputs up to 0.6 where they are 0), and corrects mean and variance. Statistics and sums are 32-bit, each output is
+// Bound by memory: a row is read once into registers, and all its sums are made there: the mean, then the squares of what is
+// left without it. Where the row lies far from zero, what is left has a sum as well: the rounding of the mean, which would
+// stay in each value (a constant row of 10^4 in fp32 gave outputs up to 0.6 where they are 0); it corrects mean, variance and
+// output. (For every row: 8192 rows of 8192 in bf16 45 us for 44, 4096 of 16384 57 for 50.) Statistics and sums are 32-bit, each output is
 // rounded once. A row has TR threads: up to a wave's 64 (a power of two) they sum by VALU lane exchanges, a work-group
 // then taking several rows at a time; wider rows add through LDS. The next row is loaded before this one's sums, which
 // wait for each other. 16383 rows of 4096 in bf16: forward 44 us (6.1 TB/s; 48 right before the gradient), gradient 83
@@ -136,10 +137,10 @@ __device__ __forceinline__ float rounded(float x) {
 template <int IO, int V, int UPT, int T>
 __global__ __launch_bounds__(T) void layer_norm_kernel(NormK a) {
   using E = typename Elem<IO>::T;
-  __shared__ float red[2][16][1], red2[2][16][2];
+  __shared__ float red[2][16][1];
   const int slots = (int)blockDim.x / a.tr, slot = (int)threadIdx.x / a.tr;
   const Columns<V> col{(int)threadIdx.x - slot * a.tr, a.tr, a.width};
-  int turn = 0, turn2 = 0;
+  int turn = 0;
   float w[UPT][V], b[UPT][V];
 #pragma unroll
   for (int i = 0; i < UPT; ++i) {
@@ -174,7 +175,7 @@ __global__ __launch_bounds__(T) void layer_norm_kernel(NormK a) {
     }
     row_sums<1>(s, a.tr, red, turn);
     const float first = rounded(s[0] * a.inv_n);
-    float q[2] = {0.f, 0.f};
+    s[0] = 0.f;
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
       const int skip = col.skip(i);
@@ -182,20 +183,33 @@ __global__ __launch_bounds__(T) void layer_norm_kernel(NormK a) {
       for (int e = 0; e < V; ++e) v[i][e] -= first;
       if (skip == 0) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) q[0] += v[i][e], q[1] = fmaf(v[i][e], v[i][e], q[1]);
+        for (int e = 0; e < V; ++e) s[0] = fmaf(v[i][e], v[i][e], s[0]);
       } else {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          q[0] += e >= skip ? v[i][e] : 0.f;
-          q[1] += e >= skip ? v[i][e] * v[i][e] : 0.f;
-        }
+        for (int e = 0; e < V; ++e) s[0] += e >= skip ? v[i][e] * v[i][e] : 0.f;
       }
     }
-    row_sums<2>(q, a.tr, red2, turn2);
-    const float off = rounded(q[0] * a.inv_n), mean = first + off;
-    float var = fmaf(-off, off, q[1] * a.inv_n);
-    var = var < 0.f ? 0.f : var;   // (NaN stays)
-    const float rstd = 1.f / sqrtf(var + a.eps);
+    row_sums<1>(s, a.tr, red, turn);
+    float mean = first, var = s[0] * a.inv_n, off = 0.f;
+    // (within four deviations the mean's rounding is that of the sums; a work-group's rows that share barriers go together)
+    const bool far = first * first > 16.f * (var + a.eps);
+    if (a.tr <= 64 ? __builtin_amdgcn_ballot_w64(far) != 0 : far || slots > 1) {
+      s[0] = 0.f;
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) {
+        const int skip = col.skip(i);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[0] += e >= skip ? v[i][e] : 0.f;
+      }
+      row_sums<1>(s, a.tr, red, turn);
+      if (far) {
+        off = s[0] * a.inv_n;
+        mean = first + off;
+        var = fmaf(-off, off, var);
+        var = var < 0.f ? 0.f : var;   // (NaN stays)
+      }
+    }
+    const float rstd = 1.f / sqrtf(var + a.eps), shift = rounded(-off * rstd);
     if (r >= a.rows) continue;   // (the slots' trips through the barriers are the same: base is the work-group's)
     if (col.t == 0 && a.mean) {
       a.mean[r] = mean;
@@ -206,7 +220,7 @@ __global__ __launch_bounds__(T) void layer_norm_kernel(NormK a) {
     for (int i = 0; i < UPT; ++i) {
       if (col.of(i) >= a.width) continue;
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[i][e] = fmaf((v[i][e] - off) * rstd, w[i][e], b[i][e]);
+      for (int e = 0; e < V; ++e) v[i][e] = fmaf(fmaf(v[i][e], rstd, shift), w[i][e], b[i][e]);
       store_any<IO, V>(y + col.at(i), v[i]);
     }
   }
