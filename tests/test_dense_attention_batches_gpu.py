@@ -107,3 +107,15 @@ def test_sequences_far_apart():
         t[what] = far
     got = call(t, [256, 250], [256, 250], False, 0.1)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_what_a_plan_copies_is_written_in_the_plan():
+    """Strides within the last dimension: the documented copy, and the others in place beside it"""
+    t = make(BF, 4, 2, 128, 0, [50, 20], [70, 64], False, 55)
+    wide = torch.empty(2, 70, 2, 256, dtype=BF, device="cuda")
+    key = wide[..., ::2].copy_(t["key"])
+    plan = dsa.DenseAttentionPlan(t["query"], key, lie(t["value"], "longer"), 0.1, [50, 20], [70, 64], return_softmax_lse=True)
+    assert all(torch.equal(a, b) for a, b in zip(plan.run(), call(t, [50, 20], [70, 64], False, 0.1)))
+    t["key"] = make(BF, 4, 2, 128, 0, [50, 20], [70, 64], False, 56)["key"]
+    plan.k.copy_(t["key"].flatten(0, 1))
+    assert all(torch.equal(a, b) for a, b in zip(plan.run(), call(t, [50, 20], [70, 64], False, 0.1)))
