@@ -305,7 +305,7 @@ struct Tiles {
 // Work-group i's sequence and key head within its level. Work-groups go to the 8 XCDs in turn, and there to groups of CUs
 // in turn, so a number of pairs that 8 or 32 divides gives the same CUs the same pairs in every level, long and short ones
 // alike: levels are turned, by 8 (a key head's tiles stay on one XCD, whose L2 they share) or, as ranges share nothing, by one.
-// Samples of 4093 and 2100, 16 heads of 128 + 64: forward 161 -> 141 us, backward 548 -> 443.
+// Samples of 4093 and 2100, 16 heads of 128 + 64: forward 161 -> 141 us, backward (without sum P K) 548 -> 443.
 __device__ __forceinline__ int pair_of(int i, int level, int pairs, int splits) {
   return (int)(((uint32_t)(i - level * pairs) + (uint32_t)level * (splits > 1 ? 1u : 8u)) % (uint32_t)pairs);
 }

@@ -1056,10 +1056,11 @@ struct Part {   // one of the two main launches
   int64_t groups;
 };
 // Tiles of TOK rows (or tokens) of every sequence: by levels of the longest's number (the heaviest of all first), or
-// numbered through where that is more than half as many again (1.9 times: 980 and 959 us, 3.3: 166 and 155, 22: 1991
-// and 1814). Ranges of the other axis where there are fewer tiles than CUs: each loads its operands anew, and a launch
-// adds their sums; of 512 rows, two rounds' worth, or up to four of 128 (a sample of 2048, 8 heads on 4: one range
-// 153 us, 4 100, 8 133; one of 300: 56, 50, 47).
+// numbered through where that is more than half as many again (1.9 times: 1069 and 1033 us, 4.1: 160 and 140, 24: 6068
+// and 1975; 1.25: 1042 and 1113, 1.2: 445 and 466. Two sequences of 8 key heads, whose pairs turn by half a round, are the
+// exception: 1.3: 882 and 755). Ranges of the other axis where there are fewer tiles than CUs: each loads its operands
+// anew, and a launch adds their sums; of 512 rows, two rounds' worth, or up to four of 128 (a sample of 2048, 8 heads on 4:
+// one range 159 us, 4 109, 8 149, as chosen 106; one of 300: 50, 53, 51, as chosen 50).
 Part make_part(int64_t total, int64_t longest, int batch, bool behind, int heads, int64_t other, int forced) {
   Part p{};
   const int64_t seqs = batch + (behind ? 1 : 0);

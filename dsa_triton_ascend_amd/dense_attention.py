@@ -2,8 +2,8 @@
 grouped key heads, on MI355X.
 
 The reference attends sparsely only. The dense form beside it is what the indexer is trained against first:
-the statistics come in the layout that ``dense_loss_backward`` and its aliases take, and the gradients train the
-attention itself. Keys and values are tensors of their own ([B, S2, N2, D] or [T2, N2, D]); for the paged latent
+the statistics of padded batches with heads of 128 are those that ``dense_loss_backward`` and its aliases take, and the
+gradients train the attention itself. Keys and values are tensors of their own ([B, S2, N2, D] or [T2, N2, D]); for the paged latent
 cache there is ``shared_prefix_attention``.
 """
 from __future__ import annotations
@@ -212,9 +212,10 @@ def dense_attention(query, key, value, scale_value=1.0, actual_seq_lengths_query
     cache, heads before rows, expanded heads or sequences), else copied.
     actual_seq_lengths_query / _kv: per batch (BSND; default: all) or cumulative (TND; default: one sequence). A query sees
     the tokens up to its own (sparse_mode 3: its sequence's last query is its last token) or all of its sequence (0).
-    Returns (attention_out, softmax_max, softmax_sum), the statistics fp32 [B,N2,S1,N1//N2], as ``dense_loss_backward``
-    takes them, or [N2,T1,N1//N2] (zeros unless return_softmax_lse); rows that see no token give zeros. autograd does not
-    follow it: :func:`dense_attention_grad` is the gradient. `kv_splits` > 0 forces the number of token ranges (tuning)."""
+    Returns (attention_out, softmax_max, softmax_sum), the statistics fp32 [B,N2,S1,N1//N2] or (TND) [N2,T1,N1//N2] (zeros
+    unless return_softmax_lse); rows that see no token give zeros. ``dense_loss_backward`` takes those of BSND with D = 128: it
+    has no heads of 64 and no packed layout, and its D = 256 and 512 have no counterpart here. autograd does not follow
+    it: :func:`dense_attention_grad` is the gradient. `kv_splits` > 0 forces the number of token ranges (tuning)."""
     return DenseAttentionPlan(query, key, value, scale_value, actual_seq_lengths_query, actual_seq_lengths_kv, query_rope,
                               key_rope, layout, sparse_mode, return_softmax_lse, kv_splits, _wait=False).run()
 

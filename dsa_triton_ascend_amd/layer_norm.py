@@ -114,7 +114,9 @@ def layer_norm_grad(d_out, x, mean, rstd, norm_weight=None, norm_bias=None):
 
 
 class LayerNorm(torch.nn.Module):
-    """Module form: keeps weight and bias (autograd does not follow it)."""
+    """Module form: keeps weight and bias. autograd does not follow it: a training loop sets their gradients itself,
+    ``module.weight.grad, module.bias.grad = d_weight, d_bias`` of :func:`layer_norm_grad`; without that an optimiser leaves
+    them as they are."""
 
     def __init__(self, width, norm_eps=1e-6, bias=True, dtype=torch.float32, device=None):
         super().__init__()

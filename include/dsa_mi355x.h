@@ -538,8 +538,8 @@ int dsa_dense_attn_batched(const void* query, int64_t q_row, int64_t q_head, con
  *   keys_behind: total_keys - key_start[batch]; max_keys: the most of key_start[b + 1] - key_start[b] and keys_behind.
  *   splits (<= 64): 0, or the ranges that each key's rows and each row's keys are cut into. Sums have a fixed order. Work-groups
  *   as in the forward, those of keys (total_keys * N2 / 128 + (batch + 1) * N2) too.
- *   fp16: dS gets a factor, a power of two from the largest norms of d_out's and value's rows, so that neither its small
- *   values nor its large ones leave the type's range.
+ *   fp16: dS gets one factor for the call, a power of two from the largest norms of d_out's and value's rows: it stays in the
+ *   type's range and is off by at most 2^-38 of those norms' product beside its rounding.
  *   workspace: dsa_dense_attn_grad_workspace_bytes, 16-byte aligned, needs no initialisation. Calls that share one must be
  *   ordered.
  */
