@@ -133,6 +133,9 @@ __device__ __forceinline__ float rounded(float x) {
   return x;
 }
 
+constexpr float FAR = 4.f;
+__device__ __forceinline__ bool far_from_zero(float mean, float rstd) { return fabsf(mean) * rstd > FAR; }
+
 // UPT units of V elements a thread; T threads a work-group at most
 template <int IO, int V, int UPT, int T>
 __global__ __launch_bounds__(T) void layer_norm_kernel(NormK a) {
@@ -191,8 +194,8 @@ __global__ __launch_bounds__(T) void layer_norm_kernel(NormK a) {
     }
     row_sums<1>(s, a.tr, red, turn);
     float mean = first, var = s[0] * a.inv_n, off = 0.f;
-    // (within four deviations the mean's rounding is that of the sums; a work-group's rows that share barriers go together)
-    const bool far = first * first > 16.f * (var + a.eps);
+    // (within FAR deviations the mean's rounding is that of the sums; a work-group's rows that share barriers go together)
+    const bool far = first * first > FAR * FAR * (var + a.eps);
     if (a.tr <= 64 ? __builtin_amdgcn_ballot_w64(far) != 0 : far || slots > 1) {
       s[0] = 0.f;
 #pragma unroll
@@ -229,11 +232,11 @@ __global__ __launch_bounds__(T) void layer_norm_kernel(NormK a) {
 template <int IO, int V, int UPT, int T>
 __global__ __launch_bounds__(T) void layer_norm_grad_kernel(NormK a) {
   using E = typename Elem<IO>::T;
-  __shared__ float red[2][16][2];
+  __shared__ float red[2][16][2], red1[2][16][1];
   extern __shared__ float join[];   // [slots][2][width], where a work-group has several
   const int slots = (int)blockDim.x / a.tr, slot = (int)threadIdx.x / a.tr;
   const Columns<V> col{(int)threadIdx.x - slot * a.tr, a.tr, a.width};
-  int turn = 0;
+  int turn = 0, turn1 = 0;
   float w[UPT][V], dw[UPT][V], db[UPT][V];
 #pragma unroll
   for (int i = 0; i < UPT; ++i) {
@@ -272,14 +275,40 @@ __global__ __launch_bounds__(T) void layer_norm_grad_kernel(NormK a) {
       widen<IO, V>(dn[i], g[i]);
     }
     const float mean = mean_n, rstd = rstd_n;
+#pragma unroll
+    for (int i = 0; i < UPT; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) h[i][e] -= mean;
     if constexpr (AHEAD) fetch(r + (int64_t)gridDim.x * slots);
+    // far from zero, the mean as it was handed over is rounded too much (as in the forward); rows that share barriers go together
+    float shift = 0.f;
+    const bool far = far_from_zero(mean, rstd);
+    bool any = far;
+    if (a.tr <= 64) any = __builtin_amdgcn_ballot_w64(far) != 0;
+    else
+      for (int k = 0; k < slots - 1; ++k) {
+        const int64_t rr = min(base + (slot + 1 + k) % slots, a.rows - 1);
+        any = any || far_from_zero(a.mean[rr], a.rstd[rr]);
+      }
+    if (any) {
+      float t[1] = {0.f};
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) {
+        const int skip = col.skip(i);
+#pragma unroll
+        for (int e = 0; e < V; ++e) t[0] += e >= skip ? h[i][e] : 0.f;
+      }
+      row_sums<1>(t, a.tr, red1, turn1);
+      if (far) shift = -t[0] * a.inv_n * rstd;
+    }
+    shift = rounded(shift);
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
       const int skip = ok ? col.skip(i) : V;
       if (skip == 0) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          h[i][e] = (h[i][e] - mean) * rstd;
+          h[i][e] = fmaf(h[i][e], rstd, shift);
           dw[i][e] = fmaf(g[i][e], h[i][e], dw[i][e]);
           db[i][e] += g[i][e];
           g[i][e] *= w[i][e];
@@ -289,7 +318,7 @@ __global__ __launch_bounds__(T) void layer_norm_grad_kernel(NormK a) {
       } else {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          h[i][e] = (h[i][e] - mean) * rstd;
+          h[i][e] = fmaf(h[i][e], rstd, shift);
           dw[i][e] += e >= skip ? g[i][e] * h[i][e] : 0.f;
           db[i][e] += e >= skip ? g[i][e] : 0.f;
           g[i][e] *= w[i][e];
