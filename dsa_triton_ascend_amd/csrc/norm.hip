@@ -237,15 +237,20 @@ __global__ __launch_bounds__(T) void layer_norm_grad_kernel(NormK a) {
   const int slots = (int)blockDim.x / a.tr, slot = (int)threadIdx.x / a.tr;
   const Columns<V> col{(int)threadIdx.x - slot * a.tr, a.tr, a.width};
   int turn = 0, turn1 = 0;
-  float w[UPT][V], dw[UPT][V], db[UPT][V];
+  // the parameters in registers; 1024 threads in 32 bits, which have too few, read them for each row (6000 rows of 9000: 189 ->
+  // 158 us, 4096 of 16384: 212 -> 201)
+  constexpr bool HOLD = T < 1024 || IO != DSA_DTYPE_F32;
+  float w[HOLD ? UPT : 1][V], dw[UPT][V], db[UPT][V];
+  auto parameters = [&](int i, float (&p)[V]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) p[e] = 1.f;
+    if (a.w) params<V>(a.w, a.wdt, col.at(i), p);
+  };
 #pragma unroll
   for (int i = 0; i < UPT; ++i) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      w[i][e] = 1.f;
-      dw[i][e] = db[i][e] = 0.f;
-    }
-    if (a.w) params<V>(a.w, a.wdt, col.at(i), w[i]);
+    for (int e = 0; e < V; ++e) dw[i][e] = db[i][e] = 0.f;
+    if constexpr (HOLD) parameters(i, w[i]);
   }
   // the next row's elements are on their way while this one's sums are made (16383 rows of 4096 in bf16: 157 -> 83 us),
   // but where 1024 threads leave no registers for them
@@ -284,12 +289,13 @@ __global__ __launch_bounds__(T) void layer_norm_grad_kernel(NormK a) {
     float shift = 0.f;
     const bool far = far_from_zero(mean, rstd);
     bool any = far;
-    if (a.tr <= 64) any = __builtin_amdgcn_ballot_w64(far) != 0;
-    else
-      for (int k = 0; k < slots - 1; ++k) {
-        const int64_t rr = min(base + (slot + 1 + k) % slots, a.rows - 1);
-        any = any || far_from_zero(a.mean[rr], a.rstd[rr]);
+    if constexpr (T == 256) {   // (wider work-groups have one row)
+      if (a.tr <= 64) any = __builtin_amdgcn_ballot_w64(far) != 0;
+      else if (slots > 1) {     // two rows of 128 threads
+        const int64_t other = min(base + 1 - slot, a.rows - 1);
+        any = any || far_from_zero(a.mean[other], a.rstd[other]);
       }
+    }
     if (any) {
       float t[1] = {0.f};
 #pragma unroll
@@ -305,13 +311,15 @@ __global__ __launch_bounds__(T) void layer_norm_grad_kernel(NormK a) {
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
       const int skip = ok ? col.skip(i) : V;
+      if constexpr (!HOLD) parameters(i, w[0]);
+      float(&wi)[V] = w[HOLD ? i : 0];
       if (skip == 0) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           h[i][e] = fmaf(h[i][e], rstd, shift);
           dw[i][e] = fmaf(g[i][e], h[i][e], dw[i][e]);
           db[i][e] += g[i][e];
-          g[i][e] *= w[i][e];
+          g[i][e] *= wi[e];
           s[0] += g[i][e];
           s[1] = fmaf(g[i][e], h[i][e], s[1]);
         }
@@ -321,7 +329,7 @@ __global__ __launch_bounds__(T) void layer_norm_grad_kernel(NormK a) {
           h[i][e] = fmaf(h[i][e], rstd, shift);
           dw[i][e] += e >= skip ? g[i][e] * h[i][e] : 0.f;
           db[i][e] += e >= skip ? g[i][e] : 0.f;
-          g[i][e] *= w[i][e];
+          g[i][e] *= wi[e];
           s[0] += e >= skip ? g[i][e] : 0.f;
           s[1] += e >= skip ? g[i][e] * h[i][e] : 0.f;
         }
